@@ -6,6 +6,7 @@
  * Part 2 declares new mmoe_* entry points that keep the whole MoE layer on the device (router logits,
  * softmax/top-8, grouping, quantisation, expert products, combine), which maple.c would call in place of its
  * CPU routing (maple.c:734-755) and expert block (maple.c:824-834).
+ * Part 3 declares the operators that serve many sequences at once: block tables, rotary positions, paged attention.
  *
  * Conventions, as in the reference: plain C; int returns are 0 on success and -1 on failure, double
  * returns are seconds (or -1.0 on failure); messages go to stderr (and mmoe_last_error()); host arrays
@@ -226,7 +227,10 @@ void *mmoe_stream(void);
 #define MMOE_K_ATT_SCORES 11
 #define MMOE_K_ATT_SOFTMAX 12
 #define MMOE_K_ATT_PV 13        /* weighted sum of values; with short windows the whole attention (k_att_local) */
-#define MMOE_PROF_NKERNELS 14
+#define MMOE_K_KV_PLAN 14
+#define MMOE_K_ROPE 15
+#define MMOE_K_ATT_PAGED 16     /* every kernel of mmoe_attn_paged */
+#define MMOE_PROF_NKERNELS 17
 int mmoe_event_record(int slot);
 double mmoe_event_elapsed_ms(void);
 int mmoe_prof(int on);
@@ -258,5 +262,110 @@ int mmoe_ckpt_load(int L0, int nl);
  * against g / (1 + exp(-g)) with IEEE division, bit for bit, over the fp32 bit patterns [lo, lo + n).
  * *nbad = number of mismatches, *first = smallest mismatching pattern (0xffffffff if none). */
 int mmoe_selftest_silu(uint32_t lo, uint32_t n, unsigned long long *nbad, uint32_t *first);
+
+/* ============================ Part 3: many sequences at once ============================
+ * No counterpart in the reference's GPU files: maple.c runs its many-sequence step (--multi, maple.c:1166-1206) with attention
+ * on the CPU and a cache of a full context per sequence (maple.c:323). Here the keys and values of all sequences of a layer
+ * live in blocks of block_size positions that sequences take from one list and give back, so memory follows the lengths:
+ *   mmoe_kv_plan      block tables, slots and positions of a step, from the sequences' lengths
+ *   mmoe_rope_kv      rotary positions of its queries and keys; keys and values written into the blocks
+ *   mmoe_attn_paged   attention of its queries over the blocks
+ * A step of a layer is mmoe_rope_kv, mmoe_attn_paged and then mmoe_moe_dev, with one mmoe_kv_plan for all layers (each layer
+ * has its own blocks and the same tables). All pointers are device memory of the library's device; the work is queued on
+ * the library stream (mmoe_stream) without waiting, so data that another stream writes or reads has to be ordered with it
+ * (an event, or a wait). The device that is current in the caller is left as it was. The calls allocate nothing and can be
+ * captured into a graph; what the host passes by value (counts, bounds) is then fixed, what it passes in device memory is read at each replay.
+ * A refused call returns -1 and queues nothing. No call keeps anything between calls. */
+#define MMOE_F32 0
+#define MMOE_F16 1
+#define MMOE_BF16 2
+#define MMOE_KV_MAXSEQ 4096      /* sequences per call */
+
+/* A layer's keys and values: head_dim consecutive values at k (v) + block * block_stride + head * head_stride + (position in
+ * the block) * token_stride, strides in values, multiples of 8; pointers aligned to 16 bytes. block_size: a power of two, 16 to 1024. */
+typedef struct {
+    void *k, *v;
+    int64_t block_stride, head_stride, token_stride;
+    int32_t nblocks, block_size, heads, head_dim, dtype;
+} mmoe_kv_cache;
+
+/* One step's tables. For sequence s (0 <= nseq <= MMOE_KV_MAXSEQ): ctx[s] positions are cached, add[s] tokens come now;
+ * table[s][width]: block ids of its positions, block_size each.
+ * 1. Sequences with done[s] != 0 (done may be NULL) give back the blocks of their positions from `shared` on (a multiple of
+ *    block_size: the positions of a common prefix stay), appended in order to free_list, of which nfree[0] entries are
+ *    free, and then have min(ctx[s], shared) cached positions.
+ * 2. In order of s, while everything fits (blocks, ntok tokens in all, width * block_size positions per sequence): blocks for
+ *    the new tokens are taken from the end of the list into table[s]. From the first sequence that does not fit on, none
+ *    gets its tokens.
+ * 3. len[s] = cached positions with the new ones, qstart[nseq + 1] = prefix sums of the tokens taken, nfree_out[0] = free blocks
+ *    left; for token t of sequence s pos[t] and slot[t] = block * block_size + position in the block. Tokens from
+ *    qstart[nseq] on: slot -1, position 0. A slot whose block id is not in 0 .. nblocks - 1 is -1.
+ * free_list has nblocks entries. len may be ctx and nfree_out may be nfree (a step that is replayed); other outputs must not
+ * overlap inputs. Negative lengths do not fit. */
+typedef struct {
+    const int32_t *ctx, *add, *done;
+    int32_t *table, *free_list;
+    const int32_t *nfree;
+    int32_t *nfree_out, *len, *qstart, *pos, *slot;
+    int32_t nseq, width, nblocks, block_size, shared, ntok;
+} mmoe_kv_plan_args;
+int mmoe_kv_plan(const mmoe_kv_plan_args *a);
+
+/* Rotation frequencies, in radians per position, of rot dims: freq[rot / 2] (host memory, no GPU needed).
+ * f_i = base^(-2 i / rot). factor > 1 stretches them for contexts longer than trained on: with orig 0 all by 1 / factor
+ * (linear interpolation); with orig > 0 by parts (the ramp of YaRN, Peng et al. 2023): a pair that turns t = orig f / 2 pi times over the
+ * orig trained positions keeps g f + (1 - g) f / factor, g = clamp((t - slow) / (fast - slow), 0, 1), usually slow 1, fast 32. */
+int mmoe_rope_freqs(int rot, double base, double factor, int orig, double slow, double fast, double *freq);
+
+/* Rotary positions. q [ntok][heads][head_dim], k and v [ntok][kv_heads][head_dim] with strides in values (dims contiguous),
+ * of in_dtype (MMOE_F32, _F16 or _BF16); a pair (x0, x1) turns by the angle pos[t] * freq[i], computed in 64 bits:
+ * (mag (x0 cos - x1 sin), mag (x1 cos + x0 sin)), each rounded once to out_dtype. Pairs: dims (i, i + rot / 2), or (2 i, 2 i + 1) with interleaved; dims
+ * from rot (even, 0 .. head_dim) on are copied. head_dim: a multiple of 8, at most 256. freq: device, rot / 2 doubles.
+ * q goes to q_out (out_dtype; NULL with heads 0). With a cache (its dtype out_dtype, its heads kv_heads): k and v (as it is)
+ * go to slot[t]; a token whose slot is not in the cache is left out altogether, its q_out row as it was; no two tokens may have the same slot. Without one (kv
+ * NULL): k goes to k_out, v and slot are not read. q_out may be q and k_out may be k where type and strides are the same.
+ * Pointers aligned to 16 bytes, strides multiples of 8 values. */
+typedef struct {
+    const void *q, *k, *v;
+    void *q_out, *k_out;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head, qo_token, qo_head, ko_token, ko_head;
+    const int32_t *pos, *slot;
+    const double *freq;
+    int32_t ntok, heads, kv_heads, head_dim, rot, interleaved, in_dtype, out_dtype;
+    float mag;
+} mmoe_rope_args;
+int mmoe_rope_kv(const mmoe_rope_args *a, const mmoe_kv_cache *kv);
+
+/* Attention of nseq sequences over their blocks. Sequence s has the tokens qstart[s] .. qstart[s + 1] - 1 of q [ntok][heads][head_dim]
+ * (none, one or many), its last ones of len[s] positions; query head h reads key/value head h / (heads / kv heads).
+ * head_dim 64 or 128; q, out and the cache of one type, MMOE_F16 or MMOE_BF16; scores, softmax and sums in 32 bits.
+ *   score of position p for the token at position i:  x = scale q.k;  cap > 0: x = cap tanh(x / cap);
+ *   slopes != NULL: x -= slopes[h] |i - p|
+ *   visible: max(lo[t], i - window) <= p < min(hi[t], len[s]); lo NULL: 0; hi NULL: i + 1 (causal); window 0: unlimited
+ * lo and hi are per token: a document mask gives each token its document's first position, a prefix mask lets hi reach past
+ * the token. out = softmax of the visible scores times v, lse (may be NULL) [ntok][heads] = log of the sum of their exp. A token that sees
+ * nothing, or whose scores are all -inf, gets 0 and -inf. A key or value that a token does not see never reaches it, whatever it
+ * holds (cache never written, infinities, NaN). Positions whose block id is not in 0 .. nblocks - 1 are seen by none.
+ * out rows and lse from qstart[nseq] on stay as they are.
+ * shared > 0 (a multiple of block_size): the first shared positions are the same blocks in every table row (row 0's are read) and in every
+ * sequence (len[s] >= shared): they are read once for all sequences instead of once for each. The result is the same.
+ * max_q and max_len bound the tokens and positions of one sequence (they choose the kernels and their grids); more tokens or positions than
+ * that are not served: tokens past max_q keep their out rows, positions past max_len are not seen.
+ * ws: mmoe_attn_paged_ws bytes (it depends on the values in a and kv, not on what pointers point to), aligned to 256; its content
+ * need not survive. Calls that can run at the same time (graphs replayed on several streams) need their own. */
+typedef struct {
+    const void *q;
+    void *out;
+    float *lse;
+    int64_t q_token, q_head, out_token, out_head;
+    const int32_t *qstart, *len, *table, *lo, *hi;
+    const float *slopes;
+    void *ws;
+    size_t ws_bytes;
+    int32_t nseq, ntok, heads, width, max_q, max_len, shared, window;
+    float scale, cap;
+} mmoe_attn_args;
+size_t mmoe_attn_paged_ws(const mmoe_attn_args *a, const mmoe_kv_cache *kv);
+int mmoe_attn_paged(const mmoe_attn_args *a, const mmoe_kv_cache *kv);
 
 #endif

@@ -22,6 +22,7 @@
 #include "decode.h"
 #include "split.h"
 #include "attn.h"
+#include "ctx.h"
 #ifndef GU16_W
 #define GU16_W 4    // small-tile gate/up: waves per workgroup, 16-row fragments per wave
 #define GU16_RF 1
@@ -143,6 +144,7 @@ static struct {
     hipGraphExec_t graph = nullptr;
     struct { int L0, nl, nb, order; float *x; } gkey = {};   // the arguments the graph was captured with
     int ncu = 256;             // compute units of the device (persistent grids)
+    int dev = 0;               // the device the context lives on
 } S;
 
 // Kernel launch on the library stream. The arguments are converted to the kernel's parameter types and passed
@@ -216,8 +218,8 @@ static int ctx_ready() {
     HC(hipStreamCreateWithFlags(&S.cst, hipStreamNonBlocking));
     for (HostRing &r : S.hs) { HC(hipHostMalloc((void **)&r.p, HS_TABLES)); HC(hipEventCreateWithFlags(&r.ev, hipEventDisableTiming)); }
     HC(hipHostMalloc((void **)&S.hs_out, HS_OUT));
-    int dev = 0; HC(hipGetDevice(&dev));
-    HC(hipDeviceGetAttribute(&S.ncu, hipDeviceAttributeMultiprocessorCount, dev));
+    HC(hipGetDevice(&S.dev));
+    HC(hipDeviceGetAttribute(&S.ncu, hipDeviceAttributeMultiprocessorCount, S.dev));
     // the no-alloc work set: carved from the static scratch of this device (one device per process here)
     void *sp = nullptr;
     HC(hipGetSymbolAddress(&sp, HIP_SYMBOL(scratch)));
@@ -244,6 +246,22 @@ static int launch(int kid, F &&f) {
         S.prof_ms[kid] += ms; S.prof_n[kid]++;
     }
     return 0;
+}
+
+// What paged.hip needs of the context (ctx.h)
+int mm_ready() { return ctx_ready(); }
+int mm_device() { return S.dev; }
+int mm_cus() { return S.ncu; }
+void mm_error(const char *fmt, ...) {
+    char b[480];
+    va_list ap; va_start(ap, fmt); vsnprintf(b, sizeof b, fmt, ap); va_end(ap);
+    seterr("%s", b);
+}
+int mm_launch(int kid, const void *f, dim3 g, dim3 b, void **args) {
+    return launch(kid, [&] {
+        hipError_t e = g_ke[0] ? hipExtLaunchKernel(f, g, b, args, 0, S.st, g_ke[0], g_ke[1], 0) : hipLaunchKernel(f, g, b, args, 0, S.st);
+        if (e != hipSuccess) g_klerr = e;
+    });
 }
 
 // ------------------------------------------------------------------------------------------------------

@@ -1,0 +1,189 @@
+// paged.hip -- the operators that serve many sequences at once (include/maplemoe.h, Part 3): argument checks and launches.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <tuple>
+#include <type_traits>
+#include "ctx.h"
+extern "C" {
+#include "../../include/maplemoe.h"
+}
+#include "paged.h"
+
+// One kernel on the library stream: the arguments converted to the kernel's parameter types and passed by address
+template <typename... P, typename... A>
+static int run(int kid, void (*f)(P...), dim3 g, dim3 b, A &&...a) {
+    static_assert(sizeof...(P) == sizeof...(A), "kernel argument count");
+    std::tuple<P...> v(static_cast<P>(a)...);
+    void *ptr[sizeof...(P)];
+    std::apply([&](auto &...x) { int i = 0; ((ptr[i++] = (void *)&x), ...); }, v);
+    return mm_launch(kid, (const void *)f, g, b, ptr);
+}
+
+// The library's device current for the duration of a call
+struct OnDevice {
+    int prev = -1;
+    bool ok = true;
+    OnDevice() {
+        int d = 0;
+        if (hipGetDevice(&d) != hipSuccess) { ok = false; return; }
+        if (d != mm_device()) { prev = d; ok = hipSetDevice(mm_device()) == hipSuccess; }
+        if (!ok) mm_error("device %d of the library cannot be made current", mm_device());
+    }
+    ~OnDevice() { if (prev >= 0) (void)hipSetDevice(prev); }
+};
+
+#define REFUSE(...) do { mm_error(__VA_ARGS__); return -1; } while (0)
+static bool apart(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
+static int log2_block(int bs) {   // -1: not a block size
+    for (int s = 4; s <= 10; s++) if (bs == 1 << s) return s;
+    return -1;
+}
+
+static int check_cache(const char *who, const mmoe_kv_cache *c) {
+    if (!c->k || !c->v || apart(c->k, 16) || apart(c->v, 16)) REFUSE("%s: cache pointers must be set and aligned to 16 bytes", who);
+    if (c->dtype != MMOE_F32 && c->dtype != MMOE_F16 && c->dtype != MMOE_BF16) REFUSE("%s: cache type %d", who, c->dtype);
+    if (log2_block(c->block_size) < 0) REFUSE("%s: block size %d is not a power of two from 16 to 1024", who, c->block_size);
+    if (c->nblocks < 1 || (int64_t)c->nblocks * c->block_size > INT32_MAX) REFUSE("%s: %d blocks of %d positions", who, c->nblocks, c->block_size);
+    if (c->heads < 1 || c->heads > 1024) REFUSE("%s: %d key/value heads", who, c->heads);
+    if (c->block_stride < 0 || c->head_stride < 0 || c->token_stride < 0 || ((c->block_stride | c->head_stride | c->token_stride) & 7))
+        REFUSE("%s: cache strides must be multiples of 8", who);
+    return 0;
+}
+
+extern "C" {
+
+int mmoe_kv_plan(const mmoe_kv_plan_args *p) {
+    if (!p) REFUSE("mmoe_kv_plan: no arguments");
+    const mmoe_kv_plan_args &a = *p;
+    int sh = log2_block(a.block_size);
+    if (sh < 0) REFUSE("mmoe_kv_plan: block size %d is not a power of two from 16 to 1024", a.block_size);
+    if (a.nseq < 0 || a.nseq > MMOE_KV_MAXSEQ) REFUSE("mmoe_kv_plan: %d sequences outside 0..%d", a.nseq, MMOE_KV_MAXSEQ);
+    if (a.ntok < 0) REFUSE("mmoe_kv_plan: %d tokens", a.ntok);
+    if (a.nblocks < 0 || (int64_t)a.nblocks * a.block_size > INT32_MAX) REFUSE("mmoe_kv_plan: %d blocks of %d positions", a.nblocks, a.block_size);
+    if (a.width < 1 || (int64_t)a.width * a.block_size > INT32_MAX) REFUSE("mmoe_kv_plan: tables of %d blocks of %d positions", a.width, a.block_size);
+    if (a.shared < 0 || a.shared % a.block_size || a.shared / a.block_size > a.width)
+        REFUSE("mmoe_kv_plan: %d shared positions (block size %d, %d blocks per table)", a.shared, a.block_size, a.width);
+    if (!a.nfree || !a.nfree_out || !a.qstart || (a.nseq && (!a.ctx || !a.add || !a.table || !a.len)) || (a.nblocks && !a.free_list) ||
+        (a.ntok && (!a.pos || !a.slot)))
+        REFUSE("mmoe_kv_plan: a pointer is missing");
+    if (mm_ready()) return -1;
+    OnDevice dev;
+    if (!dev.ok) return -1;
+    bool one = a.ntok <= 4096;
+    if (run(MMOE_K_KV_PLAN, k_kv_plan, 1, KP_T, a, sh, one)) return -1;
+    return one ? 0 : run(MMOE_K_KV_PLAN, k_kv_tokens, (a.ntok + 1023) / 1024, 256, a, sh);
+}
+
+int mmoe_rope_freqs(int rot, double base, double factor, int orig, double slow, double fast, double *freq) {
+    if (rot < 0 || rot > 256 || (rot & 1)) REFUSE("mmoe_rope_freqs: %d rotated dims", rot);
+    if (!freq) REFUSE("mmoe_rope_freqs: no output");
+    if (!(base > 1.0) || !(base < 1e300)) REFUSE("mmoe_rope_freqs: base %g", base);
+    if (!(factor >= 1.0) || !(factor < 1e300)) REFUSE("mmoe_rope_freqs: factor %g", factor);
+    if (orig < 0 || (orig > 0 && !(fast > slow && slow >= 0.0 && fast < 1e300))) REFUSE("mmoe_rope_freqs: orig %d, slow %g, fast %g", orig, slow, fast);
+    for (int i = 0; i < rot / 2; i++) {
+        double f = pow(base, -2.0 * i / rot), g = 0.0;
+        if (orig > 0) {
+            g = (orig * f / (2.0 * M_PI) - slow) / (fast - slow);
+            g = g < 0.0 ? 0.0 : g > 1.0 ? 1.0 : g;
+        }
+        freq[i] = f * g + f / factor * (1.0 - g);
+    }
+    return 0;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------------------
+// Rotary positions
+// ------------------------------------------------------------------------------------------------------
+template <int IN, int OUT>
+static int rope_launch(const mmoe_rope_args &a, const mmoe_kv_cache &kv, int cached, int sh) {
+    int tb = a.ntok >= 8192 ? 8 : a.ntok >= 2048 ? 2 : 1;
+    dim3 g((a.ntok + tb - 1) / tb);
+    if (a.interleaved) return run(MMOE_K_ROPE, k_rope<IN, OUT, RP_INTER>, g, RP_T, a, kv, cached, sh, tb);
+    if (a.rot % 16 == 0) return run(MMOE_K_ROPE, k_rope<IN, OUT, RP_SPLIT>, g, RP_T, a, kv, cached, sh, tb);
+    return run(MMOE_K_ROPE, k_rope<IN, OUT, RP_ODD>, g, RP_T, a, kv, cached, sh, tb);
+}
+template <int IN>
+static int rope_out(const mmoe_rope_args &a, const mmoe_kv_cache &kv, int cached, int sh) {
+    return a.out_dtype == MMOE_F32 ? rope_launch<IN, MMOE_F32>(a, kv, cached, sh) : a.out_dtype == MMOE_F16 ? rope_launch<IN, MMOE_F16>(a, kv, cached, sh)
+                                   : rope_launch<IN, MMOE_BF16>(a, kv, cached, sh);
+}
+
+// ------------------------------------------------------------------------------------------------------
+// Attention
+// ------------------------------------------------------------------------------------------------------
+static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
+    if (!p || !kv) REFUSE("mmoe_attn_paged: no arguments");
+    const mmoe_attn_args &a = *p;
+    if (check_cache("mmoe_attn_paged", kv)) return -1;
+    if (kv->dtype == MMOE_F32) REFUSE("mmoe_attn_paged: cache type %d (fp16 or bf16)", kv->dtype);
+    if (kv->head_dim != 64 && kv->head_dim != 128) REFUSE("mmoe_attn_paged: head_dim %d is not 64 or 128", kv->head_dim);
+    if (a.heads < 1 || a.heads > 65535 || a.heads % kv->heads) REFUSE("mmoe_attn_paged: %d query heads over %d key/value heads", a.heads, kv->heads);
+    if (a.nseq < 0 || a.nseq > MMOE_KV_MAXSEQ) REFUSE("mmoe_attn_paged: %d sequences outside 0..%d", a.nseq, MMOE_KV_MAXSEQ);
+    if (a.ntok < 0 || (int64_t)a.ntok * a.heads > INT32_MAX) REFUSE("mmoe_attn_paged: %d tokens", a.ntok);
+    if (a.width < 1 || (int64_t)a.width * kv->block_size > INT32_MAX) REFUSE("mmoe_attn_paged: tables of %d blocks", a.width);
+    if (a.max_q < 0 || a.max_len < 0 || a.max_len > (int64_t)a.width * kv->block_size) REFUSE("mmoe_attn_paged: max_q %d, max_len %d (tables of %d blocks)", a.max_q, a.max_len, a.width);
+    if (a.shared < 0 || a.shared % kv->block_size || a.shared > a.max_len) REFUSE("mmoe_attn_paged: %d shared positions (block size %d, max_len %d)", a.shared, kv->block_size, a.max_len);
+    if (a.window < 0) REFUSE("mmoe_attn_paged: window %d", a.window);
+    if (!isfinite(a.scale) || !isfinite(a.cap) || a.cap < 0) REFUSE("mmoe_attn_paged: scale %g, cap %g", a.scale, a.cap);
+    if (a.q_token < 0 || a.q_head < 0 || a.out_token < 0 || a.out_head < 0 || ((a.q_token | a.q_head | a.out_token | a.out_head) & 7))
+        REFUSE("mmoe_attn_paged: strides must be multiples of 8");
+    return 0;
+}
+
+extern "C" {
+
+int mmoe_rope_kv(const mmoe_rope_args *p, const mmoe_kv_cache *kv) {
+    if (!p) REFUSE("mmoe_rope_kv: no arguments");
+    const mmoe_rope_args &a = *p;
+    if (a.in_dtype < MMOE_F32 || a.in_dtype > MMOE_BF16 || a.out_dtype < MMOE_F32 || a.out_dtype > MMOE_BF16) REFUSE("mmoe_rope_kv: types %d, %d", a.in_dtype, a.out_dtype);
+    if (a.head_dim < 8 || a.head_dim > 256 || a.head_dim % 8) REFUSE("mmoe_rope_kv: head_dim %d is not a multiple of 8 up to 256", a.head_dim);
+    if (a.rot < 0 || a.rot > a.head_dim || (a.rot & 1)) REFUSE("mmoe_rope_kv: %d rotated dims of %d", a.rot, a.head_dim);
+    if (a.ntok < 0 || a.heads < 0 || a.heads > 65535 || a.kv_heads < 0 || a.kv_heads > 1024) REFUSE("mmoe_rope_kv: %d tokens, %d heads, %d key/value heads", a.ntok, a.heads, a.kv_heads);
+    if (!isfinite(a.mag)) REFUSE("mmoe_rope_kv: mag %g", a.mag);
+    int sh = 0;
+    if (kv) {
+        if (check_cache("mmoe_rope_kv", kv)) return -1;
+        if (kv->dtype != a.out_dtype || kv->heads != a.kv_heads || kv->head_dim != a.head_dim)
+            REFUSE("mmoe_rope_kv: cache of %d heads of %d, type %d, for %d heads of %d, type %d", kv->heads, kv->head_dim, kv->dtype, a.kv_heads, a.head_dim, a.out_dtype);
+        sh = log2_block(kv->block_size);
+    }
+    if (!a.ntok || (!a.heads && !a.kv_heads)) return 0;
+    if (!a.pos || (a.rot && !a.freq) || (a.heads && (!a.q || !a.q_out)) || (a.kv_heads && !a.k) || (kv && (!a.v || !a.slot)) || (!kv && a.kv_heads && !a.k_out))
+        REFUSE("mmoe_rope_kv: a pointer is missing");
+    if (apart(a.q, 16) || apart(a.k, 16) || apart(a.v, 16) || apart(a.q_out, 16) || apart(a.k_out, 16)) REFUSE("mmoe_rope_kv: pointers must be aligned to 16 bytes");
+    if ((a.q_token | a.q_head | a.k_token | a.k_head | a.v_token | a.v_head | a.qo_token | a.qo_head | a.ko_token | a.ko_head) & 7)
+        REFUSE("mmoe_rope_kv: strides must be multiples of 8");
+    if (mm_ready()) return -1;
+    OnDevice dev;
+    if (!dev.ok) return -1;
+    mmoe_kv_cache none = {};
+    const mmoe_kv_cache &c = kv ? *kv : none;
+    return a.in_dtype == MMOE_F32 ? rope_out<MMOE_F32>(a, c, kv != nullptr, sh) : a.in_dtype == MMOE_F16 ? rope_out<MMOE_F16>(a, c, kv != nullptr, sh)
+                                  : rope_out<MMOE_BF16>(a, c, kv != nullptr, sh);
+}
+
+size_t mmoe_attn_paged_ws(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
+    if (check_attn(p, kv)) return 0;
+    return 256;
+}
+
+int mmoe_attn_paged(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
+    if (check_attn(p, kv)) return -1;
+    const mmoe_attn_args &a = *p;
+    if (!a.nseq || !a.ntok) return 0;
+    if (!a.q || !a.out || !a.qstart || !a.len || !a.table) REFUSE("mmoe_attn_paged: a pointer is missing");
+    if (apart(a.q, 16) || apart(a.out, 16)) REFUSE("mmoe_attn_paged: q and out must be aligned to 16 bytes");
+    size_t need = mmoe_attn_paged_ws(p, kv);
+    if (!a.ws || a.ws_bytes < need || apart(a.ws, 256)) REFUSE("mmoe_attn_paged: workspace of %zu bytes (%zu needed, aligned to 256)", a.ws ? a.ws_bytes : 0, need);
+    if (mm_ready()) return -1;
+    OnDevice dev;
+    if (!dev.ok) return -1;
+    AttArgs A{a, *kv, log2_block(kv->block_size), a.heads / kv->heads};
+    dim3 g(a.ntok, a.heads);
+    if (kv->dtype == MMOE_F16) return kv->head_dim == 64 ? run(MMOE_K_ATT_PAGED, k_attn_simple<MMOE_F16, 64>, g, 64, A) : run(MMOE_K_ATT_PAGED, k_attn_simple<MMOE_F16, 128>, g, 64, A);
+    return kv->head_dim == 64 ? run(MMOE_K_ATT_PAGED, k_attn_simple<MMOE_BF16, 64>, g, 64, A) : run(MMOE_K_ATT_PAGED, k_attn_simple<MMOE_BF16, 128>, g, 64, A);
+}
+
+}  // extern "C"

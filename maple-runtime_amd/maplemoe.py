@@ -26,7 +26,27 @@ COMBINE_OVERWRITE, COMBINE_BATCH, COMBINE_ADD, COMBINE_STEP = 0, 1, 4, 6
 R = dict(LOGITS=0, TOP=1, TW=2, PLAN=3, UTOK=4, UW=5, TP=6, SP=7, QX=8, QSX=9, QSUMX=10, ACT=11, QA=12, QSA=13,
          QSUMA=14, DOWN=15, GU_I32=16, DN_I32=17, X=18, HN=19)
 KERNELS = ["rmsnorm", "router", "topk", "group", "quant", "gateup", "quant_act", "down", "combine", "dense", "qkn",
-           "att_scores", "att_softmax", "att_pv"]
+           "att_scores", "att_softmax", "att_pv", "kv_plan", "rope", "att_paged"]
+F32, F16, BF16 = 0, 1, 2
+DTYPE = dict(f32=F32, f16=F16, bf16=BF16)
+KV_MAXSEQ = 4096
+
+
+def _struct(name, doc, *fields):
+    return type(name, (C.Structure,), dict(__doc__=doc, __module__=__name__, _fields_=[(n, t) for t, names in fields for n in names.split()]))
+
+
+# the argument blocks of the many-sequence operators (include/maplemoe.h, Part 3); pointers are device addresses
+KvCache = _struct("KvCache", "mmoe_kv_cache", (C.c_void_p, "k v"), (C.c_int64, "block_stride head_stride token_stride"),
+                  (C.c_int32, "nblocks block_size heads head_dim dtype"))
+KvPlan = _struct("KvPlan", "mmoe_kv_plan_args", (C.c_void_p, "ctx add done table free_list nfree nfree_out len qstart pos slot"),
+                 (C.c_int32, "nseq width nblocks block_size shared ntok"))
+Rope = _struct("Rope", "mmoe_rope_args", (C.c_void_p, "q k v q_out k_out"),
+               (C.c_int64, "q_token q_head k_token k_head v_token v_head qo_token qo_head ko_token ko_head"), (C.c_void_p, "pos slot freq"),
+               (C.c_int32, "ntok heads kv_heads head_dim rot interleaved in_dtype out_dtype"), (C.c_float, "mag"))
+PagedAttn = _struct("PagedAttn", "mmoe_attn_args", (C.c_void_p, "q out lse"), (C.c_int64, "q_token q_head out_token out_head"),
+                    (C.c_void_p, "qstart len table lo hi slopes ws"), (C.c_size_t, "ws_bytes"),
+                    (C.c_int32, "nseq ntok heads width max_q max_len shared window"), (C.c_float, "scale cap"))
 
 _lib = None
 _slib = None
@@ -89,6 +109,9 @@ def _declare(L):
         "mmoe_selftest_silu": (i, [C.c_uint32, C.c_uint32, C.POINTER(C.c_ulonglong), u32p]),
         "mmoe_ckpt_open": (i, [C.c_char_p]), "mmoe_ckpt_close": (None, []), "mmoe_ckpt_error": (C.c_char_p, []),
         "mmoe_ckpt_layer_plan": (i, [i, ip, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64), vp]),
+        "mmoe_kv_plan": (i, [C.POINTER(KvPlan)]), "mmoe_rope_freqs": (i, [i, d, d, i, d, d, vp]),
+        "mmoe_rope_kv": (i, [C.POINTER(Rope), C.POINTER(KvCache)]),
+        "mmoe_attn_paged_ws": (sz, [C.POINTER(PagedAttn), C.POINTER(KvCache)]), "mmoe_attn_paged": (i, [C.POINTER(PagedAttn), C.POINTER(KvCache)]),
         "mmoe_ckpt_bf16": (vp, [i, i]), "mmoe_ckpt_load": (i, [i, i]),
     }
     for name, (res, args) in sig.items():

@@ -1,0 +1,277 @@
+"""The operators that serve many sequences at once (include/maplemoe.h, Part 3) on the card, against plain numpy in 64 bits."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import maplemoe as M
+from paged_ref import HALF, Batch, Dev, decode, encode, plan, rotate
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------------- block tables
+def make_plan(rng, n, ctx, add, bs, width, nblocks, shared=0, done=None, nfree=None, ntok=None):
+    ctx, add = np.array(ctx, np.int32), np.array(add, np.int32)
+    keep = shared // bs
+    ids = rng.permutation(nblocks).astype(np.int32)
+    table = np.full((n, width), -1, np.int32)
+    table[:, :keep] = ids[:keep]
+    at = keep
+    for s in range(n):
+        held = min(-(-max(int(ctx[s]), 0) // bs), width)
+        k = max(held - keep, 0)
+        table[s, keep:keep + k] = ids[at:at + k]
+        at += k
+    assert at <= nblocks
+    free = np.full(nblocks, -5, np.int32)
+    free[:nblocks - at] = ids[at:]
+    return dict(ctx=ctx, add=add, done=None if done is None else np.array(done, np.int32), table=table, free=free,
+                nfree=nblocks - at if nfree is None else nfree, bs=bs, shared=shared, ntok=int(add.clip(0).sum()) if ntok is None else ntok, nblocks=nblocks)
+
+
+def run_plan(c, in_place=False):
+    n, width = c["table"].shape
+    with Dev() as d:
+        z = lambda k: np.full(k, -99, np.int32)  # noqa: E731
+        ctx, nf = d.put(c["ctx"]), d.put(np.array([c["nfree"]], np.int32))
+        held = dict(table=(d.put(c["table"]), c["table"]), free_list=(d.put(c["free"]), c["free"]), nfree_out=(nf if in_place else d.put(z(1)), z(1)),
+                    len=(ctx if in_place else d.put(z(n)), z(n)), qstart=(d.put(z(n + 1)), z(n + 1)), pos=(d.put(z(c["ntok"])), z(c["ntok"])),
+                    slot=(d.put(z(c["ntok"])), z(c["ntok"])))
+        a = M.KvPlan(ctx=ctx, add=d.put(c["add"]), done=d.put(c["done"]), nfree=nf, nseq=n, width=width, nblocks=c["nblocks"], block_size=c["bs"],
+                     shared=c["shared"], ntok=c["ntok"], **{k: v[0] for k, v in held.items()})
+        M.check(d.lib.mmoe_kv_plan(a), "mmoe_kv_plan")
+        return {k: d.get(p, like) for k, (p, like) in held.items()}
+
+
+def check_plan(c, **kw):
+    want = plan(c["ctx"], c["add"], c["done"], c["table"], c["free"], c["nfree"], c["bs"], c["shared"], c["ntok"], c["nblocks"])
+    got = run_plan(c, **kw)
+    for k in want:
+        assert np.array_equal(got[k], want[k]), (k, got[k], want[k])
+    return want
+
+
+@pytest.mark.parametrize("n,bs,add,in_place", [(1, 16, 1, False), (1, 1024, 3000, False), (7, 16, 40, True), (64, 16, 1, False), (301, 64, 90, False),
+                                               (1023, 16, 1, True), (1500, 32, 3, False), (4096, 16, 2, True)])
+def test_plan_ragged(n, bs, add, in_place):
+    print(f"\n  n={n} bs={bs} add={add} in_place={in_place}", flush=True)
+    rng = np.random.default_rng(n * 7 + bs)
+    ctx, new = rng.integers(0, 5 * bs, n), rng.integers(0, add + 1, n)
+    width = int((-(-(ctx + new) // bs)).max()) + 2
+    total = int((-(-(ctx + new) // bs)).sum())
+    done = (rng.random(n) < 0.2).astype(int) if n > 1 else [1]
+    check_plan(make_plan(rng, n, ctx, new, bs, width, total + 9, done=done), in_place=in_place)
+
+
+def test_plan_shared_prefix_and_padding():
+    rng = np.random.default_rng(5)
+    n, bs, shared = 40, 32, 128
+    ctx = shared + rng.integers(0, 200, n)
+    ctx[3] = 40          # a row that has not got the whole prefix yet
+    new = rng.integers(0, 9, n)
+    c = make_plan(rng, n, ctx, new, bs, 20, 700, shared=shared, done=rng.random(n) < 0.3, ntok=int(new.sum()) + 33)
+    w = check_plan(c)
+    assert (w["slot"][-33:] == -1).all()
+    check_plan(dict(c, ntok=9000))     # padded past one workgroup's tokens
+
+
+@pytest.mark.parametrize("what", ["blocks", "tokens", "width", "negative ctx", "negative add", "no free", "huge add", "list count"])
+def test_plan_what_does_not_fit(what):
+    print(f"\n  {what}", flush=True)
+    rng = np.random.default_rng(11)
+    n, bs = 30, 16
+    ctx, new = rng.integers(0, 90, n), rng.integers(1, 60, n)
+    kw = {}
+    if what == "width":
+        new[17] = 16 * 40
+    if what == "negative add":
+        new[12] = -3
+    if what == "huge add":
+        new[9:12] = 2 ** 31 - 1
+    if what == "tokens":
+        kw["ntok"] = int(new[:20].sum()) + 3
+    c = make_plan(rng, n, ctx, new, bs, 14, 700, done=rng.random(n) < 0.2, **dict(dict(ntok=2000), **kw))
+    if what == "negative ctx":
+        c["ctx"][8] = -1
+    if what == "blocks":
+        c["nfree"] = 25
+    if what == "no free":
+        c["nfree"] = -4
+    if what == "list count":
+        c["nfree"] = 2 ** 31 - 1     # more than the list holds: as many as it holds
+        c["done"] = None
+    w = check_plan(c)
+    if what not in ("list count",):
+        assert w["qstart"][-1] < max(int(new.clip(0, 10 ** 6).sum()), 1)
+
+
+def test_plan_bad_block_of_a_begun_page_and_empty_batch():
+    rng = np.random.default_rng(3)
+    c = make_plan(rng, 3, [5, 17, 3], [4, 4, 14], 16, 4, 40)
+    c["table"][1, 1] = 40       # not a block of the cache: its tokens have no slot
+    c["table"][2, 0] = -1       # the first 13 tokens of the third have none either, its last is in a new block
+    w = check_plan(c)
+    assert (w["slot"][4:8] == -1).all() and (w["slot"][8:21] == -1).all() and w["slot"][21] >= 0
+    with Dev() as d:
+        nf, q, out = d.put(np.array([7], np.int32)), d.put(np.array([-1], np.int32)), np.zeros(1, np.int32)
+        slot, free = d.put(np.full(5, 3, np.int32)), d.put(np.zeros(9, np.int32))
+        a = M.KvPlan(nfree=nf, nfree_out=nf, qstart=q, pos=d.put(np.full(5, 3, np.int32)), slot=slot, free_list=free, nseq=0, width=1, nblocks=9, block_size=16, ntok=5)
+        M.check(d.lib.mmoe_kv_plan(a), "empty batch")
+        assert d.get(nf, out)[0] == 7 and d.get(q, out)[0] == 0 and (d.get(slot, np.zeros(5, np.int32)) == -1).all()
+
+
+# ---------------------------------------------------------------------------------------------------- rotary positions
+ROPES = [  # tokens, heads, kv heads, head_dim, rot, interleaved, in, out, block size (0: no cache), token-major cache, far
+    (1, 16, 4, 128, 64, 0, "f32", "f16", 16, False, 4096),
+    (64, 16, 4, 128, 128, 1, "f16", "f16", 32, True, 4096),
+    (37, 3, 1, 64, 20, 0, "bf16", "bf16", 16, False, 1000000),
+    (37, 3, 1, 64, 20, 1, "bf16", "bf16", 16, True, 1000000),
+    (130, 12, 12, 64, 64, 0, "f32", "bf16", 64, False, 100000),
+    (2100, 5, 1, 24, 2, 0, "f16", "f32", 0, False, 9),
+    (300, 6, 2, 256, 256, 0, "f32", "f32", 1024, False, 200000),
+    (8200, 2, 1, 72, 70, 0, "f16", "f16", 16, False, 50000),
+    (9001, 2, 2, 128, 0, 0, "bf16", "bf16", 64, False, 50000),
+    (50, 0, 2, 128, 32, 1, "f32", "f16", 16, False, 500),
+    (50, 4, 0, 128, 32, 0, "f32", "f16", 0, False, 500),
+]
+
+
+@pytest.mark.parametrize("n,heads,kv,dim,rot,inter,tin,tout,bs,token_major,far", ROPES)
+def test_rope(n, heads, kv, dim, rot, inter, tin, tout, bs, token_major, far):
+    print(f"\n  n={n} heads={heads}/{kv} dim={dim} rot={rot} inter={inter} {tin}->{tout} bs={bs}", flush=True)
+    rng = np.random.default_rng(n + dim + rot)
+    freq = np.zeros(max(rot // 2, 1))
+    M.check(M.lib().mmoe_rope_freqs(rot, 10000.0, 4.0, 2048, 1.0, 32.0, M.ptr(freq)), "freqs")
+    row = (heads + 2 * kv) * dim + 16
+    x = rng.standard_normal((n, row)).astype(np.float32)
+    xe = encode(x, tin)
+    part = lambda a, b: decode(np.ascontiguousarray(xe[:, a * dim:b * dim]), tin).reshape(n, b - a, dim)  # noqa: E731
+    pos = rng.integers(0, far, n).astype(np.int32)
+    pos[0] = far
+    mag = np.float32(1.1)
+    q, k, v = rotate(part(0, heads), pos, freq, rot, inter, float(mag)), rotate(part(heads, heads + kv), pos, freq, rot, inter, float(mag)), part(heads + kv, heads + 2 * kv)
+    # half a step of the result; 32-bit cos, sin and products: 2^-21 of the pair's size (mag * 1.42 * |x|), for the angle's 32-bit half turns included
+    def off(y, big):
+        return HALF[tout] * np.abs(y) + 2.0 ** -20 * np.abs(big).max() * 1.6 + 2.0 ** -25
+    with Dev() as d:
+        size = 4 if tin == "f32" else 2
+        px = d.put(xe)
+        q0 = encode(np.full((n, heads, dim + 8), 9.0), tout)
+        pq = d.put(q0)
+        a = M.Rope(q=px, k=px + heads * dim * size, v=px + (heads + kv) * dim * size, q_out=pq, q_token=row, q_head=dim, k_token=row, k_head=dim, v_token=row,
+                   v_head=dim, qo_token=heads * (dim + 8), qo_head=dim + 8, pos=d.put(pos), freq=d.put(freq), ntok=n, heads=heads, kv_heads=kv, head_dim=dim,
+                   rot=rot, interleaved=inter, in_dtype=M.DTYPE[tin], out_dtype=M.DTYPE[tout], mag=mag)
+        skip = np.zeros(n, bool)
+        if bs:
+            nblocks = -(-n // bs) + 2
+            slot = rng.permutation(nblocks * bs)[:n].astype(np.int32)
+            skip = rng.random(n) < 0.1
+            slot[skip] = rng.choice([-1, -50, nblocks * bs, 2 ** 31 - 1], skip.sum())
+            c0 = encode(np.full((nblocks, bs, kv, dim) if token_major else (nblocks, kv, bs, dim), 5.0), tout)
+            pk, pv = d.put(c0), d.put(c0)
+            a.slot = d.put(slot)
+            cache = M.KvCache(k=pk, v=pv, block_stride=bs * kv * dim, head_stride=dim if token_major else bs * dim, token_stride=kv * dim if token_major else dim,
+                              nblocks=nblocks, block_size=bs, heads=kv, head_dim=dim, dtype=M.DTYPE[tout])
+            M.check(d.lib.mmoe_rope_kv(a, cache), "rope")
+            for p, y, big in ((pk, k, k), (pv, v, v * 0)):
+                c = decode(d.get(p, c0), tout)
+                c = (c if token_major else c.transpose(0, 2, 1, 3)).reshape(nblocks * bs, kv, dim)
+                want = np.full(c.shape, 5.0)
+                want[slot[~skip]] = y[~skip]
+                tol = np.zeros(c.shape)
+                tol[slot[~skip]] = off(y, big)[~skip]
+                assert (np.abs(c - want) <= tol).all(), np.abs(c - want).max()
+        else:
+            k0 = encode(np.full((n, kv, dim), 5.0), tout)
+            a.k_out, a.ko_token, a.ko_head = d.put(k0), kv * dim, dim
+            M.check(d.lib.mmoe_rope_kv(a, None), "rope")
+            if kv:
+                assert (np.abs(decode(d.get(a.k_out, k0), tout) - k) <= off(k, k)).all()
+        got = decode(d.get(pq, q0), tout).reshape(n, heads, dim + 8)
+        assert (got[..., dim:] == 9).all() and (got[skip] == 9).all()
+        if heads:
+            err = np.abs(got[..., :dim] - q)[~skip]
+            assert (err <= off(q, q)[~skip]).all(), err.max()
+
+
+@pytest.mark.parametrize("rot,inter", [(64, 0), (64, 1), (20, 0), (128, 0)])
+def test_rope_in_place_equals_out_of_place(rot, inter):
+    print(f"\n  rot={rot} inter={inter}", flush=True)
+    rng = np.random.default_rng(rot)
+    n, heads, kv, dim = 700, 6, 2, 128
+    freq = np.zeros(rot // 2)
+    M.check(M.lib().mmoe_rope_freqs(rot, 10000.0, 1.0, 0, 0.0, 0.0, M.ptr(freq)), "freqs")
+    x = encode(rng.standard_normal((n, heads + kv, dim)), "bf16")
+    row = (heads + kv) * dim
+    with Dev() as d:
+        got = []
+        for same in (False, True):
+            px = d.put(x)
+            po = px if same else d.put(x * 0)
+            a = M.Rope(q=px, k=px + heads * dim * 2, q_out=po, k_out=po + heads * dim * 2, q_token=row, q_head=dim, k_token=row, k_head=dim, qo_token=row, qo_head=dim,
+                       ko_token=row, ko_head=dim, pos=d.put(np.arange(n, dtype=np.int32)), freq=d.put(freq), ntok=n, heads=heads, kv_heads=kv, head_dim=dim, rot=rot,
+                       interleaved=inter, in_dtype=M.BF16, out_dtype=M.BF16, mag=1.0)
+            M.check(d.lib.mmoe_rope_kv(a, None), "rope")
+            got.append(d.get(po, x))
+        assert np.array_equal(*got) and not np.array_equal(got[0], x)
+
+
+# ---------------------------------------------------------------------------------------------------- attention
+ATTN = {
+    "one token, one position": dict(qlens=[1], lens=[1]),
+    "one token at block and tile borders": dict(qlens=[1] * 9, lens=[2, 15, 16, 17, 31, 32, 33, 63, 65], heads=16, kv=4),
+    "one token, long": dict(qlens=[1], lens=[5000], heads=16, kv=4, kind="bf16", width_more=40),
+    "one token each, many sequences": dict(qlens=[1] * 40, lens=[1 + (s * 37) % 400 for s in range(40)], heads=8, kv=2, kind="bf16", bs=32),
+    "multi-query heads": dict(qlens=[1, 3, 2], lens=[300, 70, 2], heads=20, kv=1, dim=64),
+    "every head its own keys": dict(qlens=[1, 40, 2], lens=[130, 77, 700], heads=3, kv=3, dim=64, kind="bf16"),
+    "groups of three, of five, of seven": [dict(qlens=[1, 30], lens=[100, 200], heads=3 * 2, kv=2), dict(qlens=[1, 30], lens=[100, 31], heads=5, kv=1),
+                                           dict(qlens=[2, 61], lens=[100, 61], heads=14, kv=2)],
+    "a few drafted tokens": dict(qlens=[4, 1, 5, 2], lens=[900, 44, 5, 1030], heads=16, kv=4, kind="bf16", bs=64),
+    "sequences without tokens, without positions": dict(qlens=[0, 2, 0, 0, 1, 0], lens=[50, 20, 0, 0, 1, 3000], heads=4, kv=2),
+    "prompts": dict(qlens=[33, 129, 1, 64, 65], lens=[33, 129, 1, 64, 65], heads=8, kv=2),
+    "a prompt, heads of 64": dict(qlens=[300], lens=[300], heads=4, kv=4, dim=64, kind="bf16", bs=64),
+    "chunks after cached positions": dict(qlens=[100, 17, 40], lens=[612, 17, 1025], heads=4, kv=1, kind="bf16", bs=128),
+    "blocks of 1024": dict(qlens=[1, 50], lens=[1500, 1100], heads=4, kv=2, bs=1024, width_more=0),
+    "prompts and single tokens together": dict(qlens=[1, 200, 1, 1, 3], lens=[900, 200, 2, 64, 333], heads=8, kv=2, pad=21),
+    "cap": dict(qlens=[1, 70, 3], lens=[500, 90, 3], heads=8, kv=2, cap=3.0, spread=2.0),
+    "cap, bf16": dict(qlens=[1, 70, 3], lens=[500, 90, 3], heads=8, kv=2, cap=30.0, spread=4.0, kind="bf16"),
+    "distance bias": dict(qlens=[1, 70, 3], lens=[3000, 90, 700], heads=8, kv=2, alibi=True, kind="bf16"),
+    "distance bias, cap, window": dict(qlens=[1, 130, 3], lens=[3000, 190, 700], heads=8, kv=2, alibi=True, cap=20.0, window=100),
+    "window of one": dict(qlens=[1, 70, 2], lens=[500, 70, 90], heads=4, kv=1, window=1),
+    "window of 512": dict(qlens=[1, 600, 2], lens=[2000, 700, 513], heads=4, kv=1, window=512, kind="bf16"),
+    "documents": dict(qlens=[250, 1, 40], lens=[250, 300, 500], heads=4, kv=1, lo=lambda p: p // 37 * 37),
+    "documents, distance bias, heads of 64": dict(qlens=[250, 1], lens=[250, 300], heads=4, kv=2, dim=64, lo=lambda p: p // 100 * 100, alibi=True, kind="bf16"),
+    "prefix mask": dict(qlens=[250, 1, 40], lens=[250, 300, 90], heads=4, kv=2, hi=lambda p: np.maximum(p + 1, 120)),
+    "prefix mask, distance bias, window": dict(qlens=[250, 40], lens=[250, 90], heads=4, kv=2, hi=lambda p: np.maximum(p + 1, 70), alibi=True, window=30, dim=64),
+    "limits beyond the sequence": dict(qlens=[50, 1], lens=[60, 10], heads=4, kv=1, lo=lambda p: p * 0 - 9, hi=lambda p: p * 0 + 2 ** 31 - 1),
+    "rows that see nothing": dict(qlens=[90, 1, 1, 5], lens=[150, 30, 31, 900], heads=4, kv=1, lo=lambda p: np.where(p % 3 == 0, p + 1, 0), kind="bf16"),
+    "nothing seen at all": dict(qlens=[40, 1], lens=[50, 500], heads=4, kv=1, hi=lambda p: p * 0),
+    "bounds shorter than the sequences": dict(qlens=[40, 1, 3], lens=[200, 500, 90], heads=4, kv=1, max_q=7, max_len=160),
+    "loose bounds": dict(qlens=[1, 2], lens=[200, 90], heads=16, kv=4, max_q=900, width_more=300, max_len=4000),
+    "no lse": dict(qlens=[1, 30, 2], lens=[700, 90, 3], heads=4, kv=1, with_lse=False),
+    "token-major cache": dict(qlens=[1, 100, 3], lens=[700, 100, 90], heads=8, kv=4, token_major=True, kind="bf16"),
+    "lost blocks": dict(qlens=[1, 100, 3, 1], lens=[700, 300, 90, 10], heads=8, kv=2, lost=[(0, 3), (0, 43), (1, 0), (1, 18), (2, 5), (3, 0)]),
+    "shared prefix, one token each": dict(qlens=[1] * 7, lens=[512 + 1 + 13 * s for s in range(7)], shared=512, heads=16, kv=4),
+    "shared prefix, bf16, many": dict(qlens=[1] * 40, lens=[1024 + 1 + (29 * s) % 200 for s in range(40)], shared=1024, heads=8, kv=2, kind="bf16", bs=64),
+    "shared prefix, heads of 64, drafts": dict(qlens=[1, 4, 3, 0, 2], lens=[300, 330, 291, 288, 500], shared=288, heads=6, kv=2, dim=64, bs=32),
+    "shared prefix is everything but the token": dict(qlens=[1, 1, 1], lens=[65, 65, 65], shared=64, heads=4, kv=1),
+    "shared prefix, window inside and outside": [dict(qlens=[1, 2, 1], lens=[600, 530, 900], shared=512, heads=4, kv=1, window=w) for w in (50, 300, 700)],
+    "shared prefix, cap, distance bias": dict(qlens=[1, 2, 1], lens=[600, 530, 900], shared=512, heads=8, kv=2, cap=9.0, alibi=True, kind="bf16"),
+    "shared prefix, prompts": dict(qlens=[100, 1, 300], lens=[356, 300, 556], shared=256, heads=8, kv=2, pad=9),
+    "shared prefix, limits": dict(qlens=[20, 1, 3], lens=[300, 280, 290], shared=256, heads=4, kv=1, lo=lambda p: p // 100 * 100, hi=lambda p: np.maximum(p + 1, 262)),
+    "shared prefix longer than a sequence": dict(qlens=[1, 2, 5], lens=[100, 300, 129], shared=256, heads=4, kv=1, max_len=300),
+    "shared prefix, lost blocks": dict(qlens=[1, 2], lens=[300, 290], shared=256, heads=4, kv=2, lost=[(0, 5), (1, 5), (1, 17)]),
+}
+
+
+@pytest.mark.parametrize("name", list(ATTN))
+def test_attention(name):
+    cases = ATTN[name] if isinstance(ATTN[name], list) else [ATTN[name]]
+    for i, c in enumerate(cases):
+        b = Batch(np.random.default_rng(sum(map(ord, name)) + i), **c)
+        print(f"\n  {name} {i}: q {b.qlens[:8]} len {b.lens[:8]}", flush=True)
+        with Dev() as d:
+            a = b.upload(d)
+            M.check(d.lib.mmoe_attn_paged(a, b.cache), "attention")
+            b.check(d, name)
