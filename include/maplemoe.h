@@ -282,7 +282,8 @@ int mmoe_selftest_silu(uint32_t lo, uint32_t n, unsigned long long *nbad, uint32
 #define MMOE_KV_MAXSEQ 4096      /* sequences per call */
 
 /* A layer's keys and values: head_dim consecutive values at k (v) + block * block_stride + head * head_stride + (position in
- * the block) * token_stride, strides in values, multiples of 8; pointers aligned to 16 bytes. block_size: a power of two, 16 to 1024. */
+ * the block) * token_stride, strides in values, multiples of 8 (token_stride up to 2^26);
+ * pointers aligned to 16 bytes. block_size: a power of two, 16 to 1024. */
 typedef struct {
     void *k, *v;
     int64_t block_stride, head_stride, token_stride;
@@ -339,7 +340,7 @@ int mmoe_rope_kv(const mmoe_rope_args *a, const mmoe_kv_cache *kv);
 /* Attention of nseq sequences over their blocks. Sequence s has the tokens qstart[s] .. qstart[s + 1] - 1 of q [ntok][heads][head_dim]
  * (none, one or many), its last ones of len[s] positions; query head h reads key/value head h / (heads / kv heads).
  * head_dim 64 or 128; q, out and the cache of one type, MMOE_F16 or MMOE_BF16; scores, softmax and sums in 32 bits.
- *   score of position p for the token at position i:  x = scale q.k;  cap > 0: x = cap tanh(x / cap);
+ *   score of position p for the token at position i:  x = scale q.k (scale > 0);  cap > 0: x = cap tanh(x / cap);
  *   slopes != NULL: x -= slopes[h] |i - p|
  *   visible: max(lo[t], i - window) <= p < min(hi[t], len[s]); lo NULL: 0; hi NULL: i + 1 (causal); window 0: unlimited
  * lo and hi are per token: a document mask gives each token its document's first position, a prefix mask lets hi reach past
@@ -349,9 +350,9 @@ int mmoe_rope_kv(const mmoe_rope_args *a, const mmoe_kv_cache *kv);
  * out rows and lse from qstart[nseq] on stay as they are.
  * shared > 0 (a multiple of block_size): the first shared positions are the same blocks in every table row (row 0's are read) and in every
  * sequence (len[s] >= shared): they are read once for all sequences instead of once for each. The result is the same.
- * max_q and max_len bound the tokens and positions of one sequence (they choose the kernels and their grids); more tokens or positions than
+ * max_q and max_len bound the tokens and positions (at most 2^30) of one sequence (they choose the kernels and their grids); more tokens or positions than
  * that are not served: tokens past max_q keep their out rows, positions past max_len are not seen.
- * ws: mmoe_attn_paged_ws bytes (it depends on the values in a and kv, not on what pointers point to), aligned to 256; its content
+ * ws: mmoe_attn_paged_ws bytes (0: refused; it depends on the values in a and kv, not on what pointers point to), aligned to 256; its content
  * need not survive. Calls that can run at the same time (graphs replayed on several streams) need their own. */
 typedef struct {
     const void *q;

@@ -340,62 +340,374 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
 // ------------------------------------------------------------------------------------------------------
 // Attention over the blocks (mmoe_attn_paged)
 // ------------------------------------------------------------------------------------------------------
+// Every kernel here keeps a softmax's running maximum and sum and one pass over the positions. A query row is a (token, query
+// head) pair; the rows that read one key/value head, token by token and its group of query heads within, share its keys. The
+// rows' visible runs [lo, hi) are all there is to masks: a tile that every live row sees whole needs none.
+#define ATT_BN 64          // positions per tile
+#define ATT_LOG2E 1.44269504088896340736f
+#define ATT_LN2 0.69314718055994530942f
+
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef short s8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) s4v ls4;
+typedef __attribute__((address_space(3))) u4 lu4;
+typedef __attribute__((address_space(3))) uint8_t lb;
+typedef __attribute__((address_space(1))) const uint8_t gb;
+
 struct AttArgs {
     mmoe_attn_args a;
     mmoe_kv_cache kv;
-    int sh, group;   // log2 of the block size, query heads per key/value head
+    int sh, group;       // log2 of the block size, query heads per key/value head
+    int nsplit, part0, parts;   // runs of positions this launch divides a tile's into, its first partial result, partial results in all
+    int over_shared;     // this launch: all tokens over the shared positions; else each sequence over the rest
+    float s1, s2;        // cap 0: score = s1 q.k in units of log 2; else s2 tanh, with exp(2 z) = exp2(s1 q.k)
+    float *po;           // partial results [parts][ntok * heads][head_dim], each over its own sum
+    float2 *pm;          // their maxima (in units of log 2) and sums
 };
 
-// A wave per (token, query head): 64 positions at a time, one per lane for the scores, dims over lanes for the values.
-template <int T, int D>
-__global__ void __launch_bounds__(64) k_attn_simple(AttArgs A) {
+template <int T> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
+    if (T == MMOE_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// 16 bytes per lane from base + off to LDS at to + 16 * lane. Asm, so that the compiler does not wait for it before every later LDS
+// read; nothing is written to a register. The waits are the caller's.
+__device__ __forceinline__ void load_lds(const uint8_t *base, uint32_t off, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory", "m0");
+}
+// what two half-waves hold of one column
+__device__ __forceinline__ float max_halves(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_halves(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ int wave_min(int v) { for (int d = 1; d < 64; d <<= 1) v = min(v, __shfl_xor(v, d, 64)); return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int wave_max(int v) { for (int d = 1; d < 64; d <<= 1) v = max(v, __shfl_xor(v, d, 64)); return __builtin_amdgcn_readfirstlane(v); }
+
+// The sequence and row tile of virtual tile v, with tiles of bm rows: sequence s has the tiles from floor(rows before it / bm) + s
+// on; no two sequences' tiles meet, and some virtual tiles are nobody's. No sums over the sequences are needed.
+__device__ __forceinline__ int att_start(const mmoe_attn_args &a, int s) { return min(max(a.qstart[s], 0), a.ntok); }   // never past the arrays
+struct AttTileAt { int s, row0, rows, t0; };   // first row of the tile in its sequence, the sequence's rows, its first token
+__device__ __forceinline__ bool att_find(const AttArgs &A, int bm, int v, AttTileAt &o) {
     const mmoe_attn_args &a = A.a;
-    __shared__ float qs[D], ps[64];
-    __shared__ int64_t ofs[64];
-    int t = blockIdx.x, h = blockIdx.y, l = threadIdx.x;
-    if (t >= a.qstart[a.nseq]) return;
-    int s = max(count_le(a.qstart, a.nseq, t) - 1, 0), len = a.len[s], pos = len - (a.qstart[s + 1] - t);
-    if (t - a.qstart[s] >= a.max_q) return;
-    int lo = a.lo ? a.lo[t] : 0, hi = a.hi ? a.hi[t] : pos + 1;
-    if (a.window > 0) lo = max(lo, pos - a.window);
-    lo = max(lo, 0); hi = min(min(hi, len), a.max_len);
-    for (int d = l; d < D; d += 64) qs[d] = half_to_f<T>(((const uint16_t *)a.q)[t * a.q_token + h * a.q_head + d]);
-    __syncthreads();
-    float m = -__builtin_inff(), sum = 0, o[D / 64] = {};
-    for (int p0 = lo; p0 < hi; p0 += 64) {
-        int p = p0 + l, blk = -1;
-        if (p < hi) blk = a.table[(int64_t)s * a.width + (p >> A.sh)];
-        bool see = (unsigned)blk < (unsigned)A.kv.nblocks;
-        int64_t at = see ? blk * A.kv.block_stride + (h / A.group) * A.kv.head_stride + (p & (A.kv.block_size - 1)) * A.kv.token_stride : 0;
-        float x = -__builtin_inff();
-        if (see) {
-            float v = 0;
-            for (int d = 0; d < D; d += 8) {
-                float k[8];
-                load8<T>(k, A.kv.k, at + d);
-                for (int i = 0; i < 8; i++) v = fmaf(k[i], qs[d + i], v);
-            }
-            x = v * a.scale;
-            if (a.cap > 0) x = a.cap * tanhf(x / a.cap);
-            if (a.slopes) x -= a.slopes[h] * (float)abs(pos - p);
-        }
-        float mx = x;
-        for (int d = 1; d < 64; d <<= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-        float mn = fmaxf(m, mx), base = mn == -__builtin_inff() ? 0 : mn, alpha = expf(m - base), e = see ? expf(x - base) : 0;
-        m = mn;
-        ps[l] = e; ofs[l] = see ? at : -1;
-        float es = e;
-        for (int d = 1; d < 64; d <<= 1) es += __shfl_xor(es, d, 64);
-        sum = sum * alpha + es;
-        __syncthreads();
-        for (int i = 0; i < D / 64; i++) o[i] *= alpha;
-        for (int j = 0; j < 64; j++) {
-            if (ofs[j] < 0) continue;
-            for (int i = 0; i < D / 64; i++) o[i] = fmaf(ps[j], half_to_f<T>(((const uint16_t *)A.kv.v)[ofs[j] + l + 64 * i]), o[i]);
-        }
-        __syncthreads();
+    if (A.over_shared) {
+        o.s = 0; o.t0 = 0; o.row0 = v * bm; o.rows = att_start(a, a.nseq) * A.group;
+        return o.row0 < o.rows;
     }
-    for (int i = 0; i < D / 64; i++)
-        ((uint16_t *)a.out)[t * a.out_token + h * a.out_head + l + 64 * i] = (uint16_t)pack2<T>(sum == 0 ? 0.0f : o[i] / sum, 0);
-    if (a.lse && l == 0) a.lse[(int64_t)t * a.heads + h] = sum == 0 ? -__builtin_inff() : m + logf(sum);
+    int lo = 0, hi = a.nseq;   // the last s whose first tile is <= v
+    while (hi - lo > 1) {
+        int m = (lo + hi) >> 1;
+        if ((int)((int64_t)att_start(a, m) * A.group / bm) + m <= v) lo = m; else hi = m;
+    }
+    o.s = lo; o.t0 = att_start(a, lo);
+    o.row0 = (v - (int)((int64_t)o.t0 * A.group / bm) - lo) * bm;
+    o.rows = min(att_start(a, lo + 1) - o.t0, a.max_q) * A.group;
+    return o.row0 < o.rows;
+}
+
+// One query row as a lane sees it
+struct AttRow { int tok, head, pos, lo, hi; bool live; };
+__device__ __forceinline__ AttRow att_row(const AttArgs &A, const AttTileAt &at, int r, int kvh) {
+    const mmoe_attn_args &a = A.a;
+    AttRow o;
+    o.live = r < at.rows;
+    if (!o.live) r = at.rows - 1;
+    int j = r / A.group, s = at.s;
+    o.tok = at.t0 + j;
+    o.head = kvh * A.group + r - j * A.group;
+    if (A.over_shared) s = max(count_le(a.qstart, a.nseq, o.tok) - 1, 0);
+    int len = a.len[s], t0 = a.qstart[s];
+    o.pos = len - (a.qstart[s + 1] - o.tok);
+    if (o.tok - t0 >= a.max_q) o.live = false;
+    o.lo = a.lo ? max(a.lo[o.tok], 0) : 0;
+    o.hi = a.hi ? a.hi[o.tok] : o.pos + 1;
+    if (a.window > 0) o.lo = max(o.lo, o.pos - a.window);
+    o.hi = max(min(min(o.hi, len), a.max_len), 0);
+    if (A.over_shared) o.hi = min(o.hi, a.shared); else o.lo = max(o.lo, a.shared);
+    return o;
+}
+
+// Values of a tile that is not seen whole: are all of them finite? (bits: the type's exponent)
+template <int T> __device__ __forceinline__ bool odd16(uint32_t v) { constexpr uint32_t e = T == MMOE_BF16 ? 0x7f80 : 0x7c00; return (v & e) == e; }
+template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
+    if (odd16<T>(v)) v &= 0xffff0000u;
+    if (odd16<T>(v >> 16)) v &= 0xffffu;
+    return v;
+}
+
+// Row tiles of 128 in a workgroup of 4 waves, 32 rows each, over tiles of 64 positions that all waves share through LDS.
+// S^T = K Q^T, so a lane holds one row's scores (half of the positions, the other half in the lane 32 away): the softmax needs
+// one exchange per tile, and P^T, packed to 16 bits, is the second product's operand as it lies. O^T = V^T P^T takes its V^T from
+// rows of V through the transposing LDS reads. A tile's keys and values go from the cache straight to LDS, one tile ahead, in 16-byte
+// pieces whose place in a row is exchanged by the row's number, so that neither the reads of 8 rows at one column nor the transposing
+// reads of 4 rows meet in a bank. P is rounded to the cache's type (half a step relative, as the result itself is), its
+// sum is of the unrounded 32-bit values.
+template <int T, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
+    constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // bytes and chunks of a row, rows and instructions of a wave's load
+    __shared__ __attribute__((aligned(1024))) uint8_t tiles[2][2 * ATT_BN * RB];   // keys, values
+    __shared__ int range[2][4];
+    const mmoe_attn_args &a = A.a;
+    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 31, hh = l >> 5;
+    const int kvh = blockIdx.x % A.kv.heads, rest = blockIdx.x / A.kv.heads, split = rest % A.nsplit;
+    AttTileAt at;
+    if (!att_find(A, 128, gridDim.x / A.kv.heads / A.nsplit - 1 - rest / A.nsplit, at)) return;   // the last tiles see most: first
+    AttRow R = att_row(A, at, at.row0 + w * 32 + n, kvh);
+    // the wave's and the workgroup's positions
+    const bool some = R.live && R.lo < R.hi;
+    const int wlo = wave_min(some ? R.lo : INT32_MAX), whi = wave_max(some ? R.hi : 0);
+    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
+    if (l == 0) { range[0][w] = wlo; range[1][w] = whi; }
+    __syncthreads();
+    int p0 = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3])) & ~(ATT_BN - 1);
+    int p1 = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
+    if (A.nsplit > 1 && p0 < p1) {
+        int run = ((p1 - p0 + ATT_BN - 1) / ATT_BN + A.nsplit - 1) / A.nsplit * ATT_BN;
+        p0 += split * run;
+        p1 = min(p1, p0 + run);
+    }
+    p0 = __builtin_amdgcn_readfirstlane(p0); p1 = __builtin_amdgcn_readfirstlane(p1);
+
+    // queries: operand B, lane (hh, n) holds dims 16 s + 8 hh .. + 8 of row n
+    u4 q[KS];
+    {
+        const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * hh;
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 16 * s);
+    }
+    const float slope = BIAS ? a.slopes[R.head] * ATT_LOG2E : 0.0f;
+
+    // what the lane loads of a tile: row 16 w + RPI i + l / CH, piece l % CH of LDS
+    uint32_t ko[NI], vo[NI];
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+        int r = RPI * i + l / CH, c = l % CH;
+        ko[i] = (uint32_t)(r * A.kv.token_stride + (c ^ (r & (CH - 1))) * 8) * 2;
+        vo[i] = (uint32_t)(r * A.kv.token_stride + (c ^ ((r & (CH / 2 - 1)) << 1)) * 8) * 2;
+    }
+    // where it reads them back: K row n (and n + 32), pieces 2 k + hh; V rows vr (and on by eights), dims 32 i + 16 (l / 16 % 2) + 4 (l % 4) ..
+    // (the number that exchanges a row's pieces is the same for rows 32 (K) and 8 (V) apart: what is added are constants)
+    uint32_t ka[KS], va[DS];
+    const int vr = 4 * hh + ((l & 15) >> 2);
+#pragma unroll
+    for (int k = 0; k < KS; k++) ka[k] = n * RB + (((2 * k + hh) ^ (n & (CH - 1))) << 4);
+#pragma unroll
+    for (int i = 0; i < DS; i++) va[i] = ATT_BN * RB + vr * RB + ((64 * i + 32 * ((l >> 4) & 1) + 8 * (l & 3)) ^ ((vr & (CH / 2 - 1)) << 5));
+    const int32_t *table = a.table + (int64_t)at.s * a.width;
+    auto ids = [&](int p) { return table[min((p + 16 * (l & 3)) >> A.sh, a.width - 1)]; };   // lane i % 4: positions p + 16 i ..
+    auto fetch = [&](uint32_t buf, int p, int id) {
+        int blk = __builtin_amdgcn_readlane(id, w);
+        if ((unsigned)blk >= (unsigned)A.kv.nblocks) blk = 0;
+        const int64_t at0 = (blk * A.kv.block_stride + kvh * A.kv.head_stride + ((p + 16 * w) & (A.kv.block_size - 1)) * A.kv.token_stride) * 2;
+        const uint8_t *kp = (const uint8_t *)A.kv.k + at0, *vp = (const uint8_t *)A.kv.v + at0;
+#pragma unroll
+        for (int i = 0; i < NI; i++) load_lds(kp, ko[i], buf + w * 16 * RB + i * 1024);
+#pragma unroll
+        for (int i = 0; i < NI; i++) load_lds(vp, vo[i], buf + ATT_BN * RB + w * 16 * RB + i * 1024);
+    };
+
+    f16v acc[DS];
+#pragma unroll
+    for (int i = 0; i < DS; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
+    float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f;   // mb: m, 0 while that is -inf
+
+    auto tile = [&](uint32_t buf, int p, unsigned bad) {
+        const lb *kl = (const lb *)(uintptr_t)buf;
+        f16v s[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[u][j] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                u4 kf = *(const lu4 *)(kl + ka[k] + 32 * u * RB);
+                s[u] = mfma32<T>(kf, q[k], s[u]);
+            }
+        }
+        // scores in units of log 2
+        const float dist = BIAS ? (float)(R.pos - p - 4 * hh) : 0.0f;
+        if (CAP || BIAS)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    float x = s[u][j] * A.s1;
+                    if (CAP) x = fmaf(-2.0f * A.s2, __builtin_amdgcn_rcpf(1.0f + exp2_(x)), A.s2);   // tanh z = 1 - 2 / (1 + exp 2 z)
+                    if (BIAS) x = fmaf(-slope, fabsf(dist - (float)(32 * u + 8 * (j >> 2) + (j & 3))), x);
+                    s[u][j] = x;
+                }
+        const float sc = CAP || BIAS ? 1.0f : A.s1;
+        const bool part = p < inlo || p + ATT_BN > inhi || bad;
+        if (part) {
+            const unsigned from = (unsigned)(R.lo - p - 4 * hh), span = (unsigned)max(R.hi - R.lo, 0);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    bool see = (unsigned)(32 * u + 8 * (j >> 2) + (j & 3)) - from < span && !((bad >> (2 * u + (j >> 3))) & 1);
+                    s[u][j] = see ? s[u][j] : -__builtin_inff();
+                }
+        }
+        float mt = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) mt = fmaxf(mt, fmaxf(s[u][j], s[u][j + 1]));
+        mt = max_halves(mt) * sc;
+        // a new maximum only once it is 2^8 past the old: until then weights stay below 2^8, in every type's range
+        if (__any(mt > m + 8.0f)) {
+            float mn = fmaxf(m, mt), bn = mn == -__builtin_inff() ? 0.0f : mn, al = exp2_(m - bn);
+            m = mn; mb = bn; sum *= al;
+#pragma unroll
+            for (int i = 0; i < DS; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) acc[i][j] *= al;
+        }
+        u4 pf[4];
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+                float e0 = exp2_(fmaf(s[u][j], sc, -mb)), e1 = exp2_(fmaf(s[u][j + 1], sc, -mb));
+                sum += e0 + e1;
+                pf[2 * u + (j >> 3)][(j & 7) >> 1] = pack2<T>(e0, e1);
+            }
+        // V^T: lane (hh, n) of operand A holds dim 32 i + n, positions 16 k + 4 hh + {0 .. 3, 8 .. 11}
+        auto value = [&](int i, int k) {
+            uint2 t0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(kl + va[i] + 16 * k * RB)));
+            uint2 t1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(kl + va[i] + (16 * k + 8) * RB)));
+            return u4{t0.x, t0.y, t1.x, t1.y};
+        };
+        bool odd = false;
+        if (part) {   // a value that is not finite times a weight of 0 is NaN: such tiles take the long way
+            bool o = false;
+#pragma unroll 1
+            for (int i = 0; i < ATT_BN * RB / 1024; i++) {
+                u4 v = *(const lu4 *)(kl + ATT_BN * RB + i * 1024 + l * 16);
+#pragma unroll
+                for (int x = 0; x < 4; x++) o |= odd16<T>(v[x]) | odd16<T>(v[x] >> 16);
+            }
+            odd = __any(o);
+        }
+        if (!odd) {
+#pragma unroll
+            for (int i = 0; i < DS; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) acc[i] = mfma32<T>(value(i, k), pf[k], acc[i]);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < DS; i++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                u4 f = value(i, k);
+#pragma unroll
+                for (int x = 0; x < 4; x++) f[x] = only_finite<T>(f[x]);
+                acc[i] = mfma32<T>(f, pf[k], acc[i]);
+                __builtin_amdgcn_sched_barrier(0);   // registers, not speed
+            }
+        // infinities and NaN of the positions a row does see, added as they are
+#pragma unroll 1
+        for (int r = 0; r < ATT_BN; r++) {
+            const bool see = p + r >= R.lo && p + r < R.hi && !((bad >> (r >> 4)) & 1);
+            uint32_t row = ATT_BN * RB + r * RB + 8 * hh, x = (r & (CH / 2 - 1)) << 5;
+            asm("" : "+v"(row));   // its 64 addresses are not worth a register outside
+#pragma unroll
+            for (int i = 0; i < DS; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j += 4) {
+                    typedef __attribute__((address_space(3))) uint64_t l8;
+                    uint64_t v = *(const l8 *)(kl + row + ((64 * i + 4 * j) ^ x));
+#pragma unroll
+                    for (int y = 0; y < 4; y++, v >>= 16) {
+                        acc[i][j + y] += see & odd16<T>((uint32_t)v) ? half_to_f<T>((uint32_t)v & 0xffff) : 0.0f;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+        }
+    };
+
+    if (p0 < p1) {
+        uint32_t buf = (uint32_t)(uintptr_t)(lb *)tiles;
+        int id = ids(p0), next = ids(p0 + ATT_BN);
+        fetch(buf, p0, id);
+        for (int p = p0; p < p1; p += ATT_BN) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the loads below are the compiler's no more than they are its waits'
+            __syncthreads();   // the tile has arrived, and every wave is done with the other buffer
+            const unsigned bad = (unsigned)__ballot((unsigned)id >= (unsigned)A.kv.nblocks) & 15u;
+            const uint32_t other = buf ^ (2 * ATT_BN * RB);
+            if (p + ATT_BN < p1) {
+                id = next;
+                next = ids(p + 2 * ATT_BN);
+                fetch(other, p + ATT_BN, id);
+            }
+            if (p < whi && p + ATT_BN > wlo) tile(buf, p, bad);
+            buf = other;
+        }
+    }
+    sum = add_halves(sum);
+    if (!R.live) return;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    if (A.parts == 1) {
+        uint16_t *o = (uint16_t *)a.out + (int64_t)R.tok * a.out_token + R.head * a.out_head + 4 * hh;
+#pragma unroll
+        for (int i = 0; i < DS; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+                uint2 v = make_uint2(pack2<T>(acc[i][j] * inv, acc[i][j + 1] * inv), pack2<T>(acc[i][j + 2] * inv, acc[i][j + 3] * inv));
+                if (sum == 0.0f) v = make_uint2(0, 0);
+                *(uint2 *)(o + 32 * i + 2 * j) = v;
+            }
+        if (a.lse && hh == 0) a.lse[(int64_t)R.tok * a.heads + R.head] = sum == 0.0f ? -__builtin_inff() : (mb + __builtin_amdgcn_logf(sum)) * ATT_LN2;
+        return;
+    }
+    const int64_t row = ((int64_t)(A.part0 + split) * a.ntok + R.tok) * a.heads + R.head;
+    if (hh == 0) A.pm[row] = make_float2(mb, sum);
+    if (sum == 0.0f) return;
+    float *o = A.po + row * D + 4 * hh;
+#pragma unroll
+    for (int i = 0; i < DS; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) *(f4 *)(o + 32 * i + 2 * j) = f4{acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]};
+}
+
+// The partial results of a row: their maxima and sums give each a weight. A workgroup per row, a part per wave in turn.
+template <int T, int D>
+__global__ void __launch_bounds__(256) k_attn_join(AttArgs A) {
+    const mmoe_attn_args &a = A.a;
+    __shared__ float acc[4][D];
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6, tok = blockIdx.x / a.heads, head = blockIdx.x - tok * a.heads;
+    if (tok >= a.qstart[a.nseq]) return;
+    int s = max(count_le(a.qstart, a.nseq, tok) - 1, 0);
+    if (tok - a.qstart[s] >= a.max_q) return;
+    const int64_t rows = (int64_t)a.ntok * a.heads;
+    float m = -__builtin_inff(), sum = 0.0f, o[D / 64] = {};
+    for (int p = l; p < A.parts; p += 64) { float2 v = A.pm[p * rows + blockIdx.x]; if (v.y != 0.0f) m = fmaxf(m, v.x); }
+    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+    for (int p = 0; p < A.parts; p++) {
+        float2 v = A.pm[p * rows + blockIdx.x];
+        if (v.y == 0.0f) continue;
+        float e = exp2_(v.x - m);
+        sum = fmaf(v.y, e, sum);
+        if ((p & 3) == w)
+#pragma unroll
+            for (int i = 0; i < D / 64; i++) o[i] = fmaf(e, A.po[(p * rows + blockIdx.x) * D + l * (D / 64) + i], o[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) acc[w][l * (D / 64) + i] = o[i];
+    __syncthreads();
+    if (threadIdx.x < D / 2) {
+        int d = threadIdx.x * 2;
+        float inv = 1.0f / sum, x = acc[0][d] + acc[1][d] + (acc[2][d] + acc[3][d]), y = acc[0][d + 1] + acc[1][d + 1] + (acc[2][d + 1] + acc[3][d + 1]);
+        *(uint32_t *)((uint16_t *)a.out + (int64_t)tok * a.out_token + head * a.out_head + d) = sum == 0.0f ? 0u : pack2<T>(x * inv, y * inv);
+    }
+    if (a.lse && threadIdx.x == 0) a.lse[blockIdx.x] = sum == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * ATT_LN2;
 }

@@ -1,6 +1,7 @@
 // paged.hip -- the operators that serve many sequences at once (include/maplemoe.h, Part 3): argument checks and launches.
 #include <hip/hip_runtime.h>
 #include <math.h>
+#include <algorithm>
 #include <tuple>
 #include <type_traits>
 #include "ctx.h"
@@ -47,6 +48,7 @@ static int check_cache(const char *who, const mmoe_kv_cache *c) {
     if (c->heads < 1 || c->heads > 1024) REFUSE("%s: %d key/value heads", who, c->heads);
     if (c->block_stride < 0 || c->head_stride < 0 || c->token_stride < 0 || ((c->block_stride | c->head_stride | c->token_stride) & 7))
         REFUSE("%s: cache strides must be multiples of 8", who);
+    if (c->token_stride > 1 << 26) REFUSE("%s: token stride %lld above %d", who, (long long)c->token_stride, 1 << 26);
     return 0;
 }
 
@@ -123,13 +125,56 @@ static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
     if (a.nseq < 0 || a.nseq > MMOE_KV_MAXSEQ) REFUSE("mmoe_attn_paged: %d sequences outside 0..%d", a.nseq, MMOE_KV_MAXSEQ);
     if (a.ntok < 0 || (int64_t)a.ntok * a.heads > INT32_MAX) REFUSE("mmoe_attn_paged: %d tokens", a.ntok);
     if (a.width < 1 || (int64_t)a.width * kv->block_size > INT32_MAX) REFUSE("mmoe_attn_paged: tables of %d blocks", a.width);
-    if (a.max_q < 0 || a.max_len < 0 || a.max_len > (int64_t)a.width * kv->block_size) REFUSE("mmoe_attn_paged: max_q %d, max_len %d (tables of %d blocks)", a.max_q, a.max_len, a.width);
+    if (a.max_q < 0 || a.max_len < 0 || a.max_len > (int64_t)a.width * kv->block_size || a.max_len > 1 << 30)
+        REFUSE("mmoe_attn_paged: max_q %d, max_len %d (tables of %d blocks)", a.max_q, a.max_len, a.width);
     if (a.shared < 0 || a.shared % kv->block_size || a.shared > a.max_len) REFUSE("mmoe_attn_paged: %d shared positions (block size %d, max_len %d)", a.shared, kv->block_size, a.max_len);
     if (a.window < 0) REFUSE("mmoe_attn_paged: window %d", a.window);
-    if (!isfinite(a.scale) || !isfinite(a.cap) || a.cap < 0) REFUSE("mmoe_attn_paged: scale %g, cap %g", a.scale, a.cap);
+    if (!(a.scale > 0) || !isfinite(a.scale) || !isfinite(a.cap) || a.cap < 0) REFUSE("mmoe_attn_paged: scale %g, cap %g", a.scale, a.cap);
     if (a.q_token < 0 || a.q_head < 0 || a.out_token < 0 || a.out_head < 0 || ((a.q_token | a.q_head | a.out_token | a.out_head) & 7))
         REFUSE("mmoe_attn_paged: strides must be multiples of 8");
     return 0;
+}
+
+// How a call is divided: row tiles, and runs of positions where the tiles alone are too few workgroups.
+struct AttPlan { int tiles, split, tiles_sh, split_sh, parts; size_t bytes; };
+static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
+    AttPlan p = {};
+    const int64_t rows = (int64_t)a.ntok * (a.heads / kv.heads), want = 512;
+    p.tiles = (int)((rows + 127) / 128) + a.nseq;
+    auto runs = [&](int64_t tiles, int64_t positions) {
+        int64_t n = (want + tiles * kv.heads - 1) / (tiles * kv.heads), most = (positions + 255) / 256;
+        return (int)(n < 1 || most < 1 ? 1 : n > most ? most : n);
+    };
+    p.split = runs(p.tiles - a.nseq, a.window ? std::min(a.max_len - a.shared, a.window + a.max_q) : a.max_len - a.shared);
+    if (a.shared) {
+        p.tiles_sh = (int)((rows + 127) / 128);
+        p.split_sh = runs(p.tiles_sh, a.shared);
+    }
+    p.parts = p.split + p.split_sh;
+    p.bytes = 256;
+    if (p.parts > 1) p.bytes += (size_t)p.parts * a.ntok * a.heads * (kv.head_dim * 4 + 8);
+    return p;
+}
+
+template <int T, int D>
+static int att_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPlan &p) {
+    AttArgs A{};
+    A.a = a; A.kv = kv;
+    A.sh = log2_block(kv.block_size); A.group = a.heads / kv.heads;
+    A.parts = p.parts;
+    A.s1 = a.cap > 0 ? 2.0f * a.scale / a.cap * ATT_LOG2E : a.scale * ATT_LOG2E;
+    A.s2 = a.cap * ATT_LOG2E;
+    A.pm = (float2 *)a.ws;
+    A.po = (float *)((uint8_t *)a.ws + (size_t)p.parts * a.ntok * a.heads * 8);
+    auto tile = [&](int tiles, int split, int part0, int over) {
+        A.nsplit = split; A.part0 = part0; A.over_shared = over;
+        dim3 g((unsigned)tiles * split * kv.heads);
+        if (a.cap > 0) return a.slopes ? run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, true, true>, g, 256, A) : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, true, false>, g, 256, A);
+        return a.slopes ? run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, false, true>, g, 256, A) : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, false, false>, g, 256, A);
+    };
+    if (p.split_sh && tile(p.tiles_sh, p.split_sh, 0, 1)) return -1;
+    if (tile(p.tiles, p.split, p.split_sh, 0)) return -1;
+    return p.parts > 1 ? run(MMOE_K_ATT_PAGED, k_attn_join<T, D>, dim3((unsigned)a.ntok * a.heads), 256, A) : 0;
 }
 
 extern "C" {
@@ -166,7 +211,7 @@ int mmoe_rope_kv(const mmoe_rope_args *p, const mmoe_kv_cache *kv) {
 
 size_t mmoe_attn_paged_ws(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
     if (check_attn(p, kv)) return 0;
-    return 256;
+    return att_plan(*p, *kv).bytes;
 }
 
 int mmoe_attn_paged(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
@@ -175,15 +220,13 @@ int mmoe_attn_paged(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
     if (!a.nseq || !a.ntok) return 0;
     if (!a.q || !a.out || !a.qstart || !a.len || !a.table) REFUSE("mmoe_attn_paged: a pointer is missing");
     if (apart(a.q, 16) || apart(a.out, 16)) REFUSE("mmoe_attn_paged: q and out must be aligned to 16 bytes");
-    size_t need = mmoe_attn_paged_ws(p, kv);
-    if (!a.ws || a.ws_bytes < need || apart(a.ws, 256)) REFUSE("mmoe_attn_paged: workspace of %zu bytes (%zu needed, aligned to 256)", a.ws ? a.ws_bytes : 0, need);
+    AttPlan pl = att_plan(a, *kv);
+    if (!a.ws || a.ws_bytes < pl.bytes || apart(a.ws, 256)) REFUSE("mmoe_attn_paged: workspace of %zu bytes (%zu needed, aligned to 256)", a.ws ? a.ws_bytes : 0, pl.bytes);
     if (mm_ready()) return -1;
     OnDevice dev;
     if (!dev.ok) return -1;
-    AttArgs A{a, *kv, log2_block(kv->block_size), a.heads / kv->heads};
-    dim3 g(a.ntok, a.heads);
-    if (kv->dtype == MMOE_F16) return kv->head_dim == 64 ? run(MMOE_K_ATT_PAGED, k_attn_simple<MMOE_F16, 64>, g, 64, A) : run(MMOE_K_ATT_PAGED, k_attn_simple<MMOE_F16, 128>, g, 64, A);
-    return kv->head_dim == 64 ? run(MMOE_K_ATT_PAGED, k_attn_simple<MMOE_BF16, 64>, g, 64, A) : run(MMOE_K_ATT_PAGED, k_attn_simple<MMOE_BF16, 128>, g, 64, A);
+    if (kv->dtype == MMOE_F16) return kv->head_dim == 64 ? att_run<MMOE_F16, 64>(a, *kv, pl) : att_run<MMOE_F16, 128>(a, *kv, pl);
+    return kv->head_dim == 64 ? att_run<MMOE_BF16, 64>(a, *kv, pl) : att_run<MMOE_BF16, 128>(a, *kv, pl);
 }
 
 }  // extern "C"
