@@ -361,8 +361,10 @@ struct AttArgs {
     mmoe_attn_args a;
     mmoe_kv_cache kv;
     int sh, group;       // log2 of the block size, query heads per key/value head
-    int nsplit, part0, parts;   // runs of positions this launch divides a tile's into, its first partial result, partial results in all
+    int nsplit, part0, parts;   // runs of positions that this launch divides a tile's into, its first partial result, partial results in all
     int over_shared;     // this launch: all tokens over the shared positions; else each sequence over the rest
+    int chunk, chunks, few;   // k_attn_few: positions per workgroup, most chunks of a sequence; sequences of up to few rows per key/value head are its own (0: none are)
+    int split, split_sh; // the call's runs per row tile over a sequence's own positions and over the shared ones
     float s1, s2;        // cap 0: score = s1 q.k in units of log 2; else s2 tanh, with exp(2 z) = exp2(s1 q.k)
     float *po;           // partial results [parts][ntok * heads][head_dim], each over its own sum
     float2 *pm;          // their maxima (in units of log 2) and sums
@@ -408,7 +410,17 @@ __device__ __forceinline__ bool att_find(const AttArgs &A, int bm, int v, AttTil
     o.s = lo; o.t0 = att_start(a, lo);
     o.row0 = (v - (int)((int64_t)o.t0 * A.group / bm) - lo) * bm;
     o.rows = min(att_start(a, lo + 1) - o.t0, a.max_q) * A.group;
-    return o.row0 < o.rows;
+    return o.row0 < o.rows && o.rows > A.few;
+}
+// A sequence's own positions in chunks: from `from` on, n of them (k_attn_few and k_attn_join agree through this)
+struct AttChunks { int from, n; };
+__device__ __forceinline__ AttChunks att_chunks(const AttArgs &A, int s, int tokens) {
+    const mmoe_attn_args &a = A.a;
+    int len = a.len[s], from = a.shared, to = a.hi ? len : len - max(tokens - a.max_q, 0);   // the last served token's end
+    if (a.window > 0) from = max(from, len - tokens - a.window);
+    from &= ~31;
+    to = min(to, a.max_len);
+    return {from, to > from ? min((to - from + A.chunk - 1) / A.chunk, A.chunks) : 0};
 }
 
 // One query row as a lane sees it
@@ -679,35 +691,282 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
         for (int j = 0; j < 16; j += 4) *(f4 *)(o + 32 * i + 2 * j) = f4{acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]};
 }
 
-// The partial results of a row: their maxima and sums give each a weight. A workgroup per row, a part per wave in turn.
-template <int T, int D>
-__global__ void __launch_bounds__(256) k_attn_join(AttArgs A) {
+// Few rows (up to 16 per key/value head: single tokens, a few drafted ones): the cache's bytes are the bound, so a workgroup takes a chunk
+// of positions, its 4 waves every fourth run of 32 each, keys and values straight into registers; a run's keys give their
+// registers to the next run's as soon as its scores are there, its values after the second product. S^T = K Q^T and O^T = V^T P^T as in k_attn_tile, on 16 x 16 x 32
+// products; V^T is put together from rows by byte permutes (32 per run of 32 positions, hidden behind the loads). The waves join
+// through LDS, the chunks in k_attn_join.
+template <int T> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
+    if (T == MMOE_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ float max_quarters(float x) { x = fmaxf(x, __shfl_xor(x, 16, 64)); return fmaxf(x, __shfl_xor(x, 32, 64)); }
+__device__ __forceinline__ float add_quarters(float x) { x += __shfl_xor(x, 16, 64); return x + __shfl_xor(x, 32, 64); }
+
+template <int T, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256, 3) k_attn_few(AttArgs A) {
+    constexpr int KS = D / 32, E = D / 16;   // products over the dims, values of a row per lane
+    __shared__ __attribute__((aligned(16))) float joint[4][16][D + 4];
+    __shared__ float2 stat[4][16];
     const mmoe_attn_args &a = A.a;
-    __shared__ float acc[4][D];
-    const int l = threadIdx.x & 63, w = threadIdx.x >> 6, tok = blockIdx.x / a.heads, head = blockIdx.x - tok * a.heads;
-    if (tok >= a.qstart[a.nseq]) return;
-    int s = max(count_le(a.qstart, a.nseq, tok) - 1, 0);
-    if (tok - a.qstart[s] >= a.max_q) return;
-    const int64_t rows = (int64_t)a.ntok * a.heads;
-    float m = -__builtin_inff(), sum = 0.0f, o[D / 64] = {};
-    for (int p = l; p < A.parts; p += 64) { float2 v = A.pm[p * rows + blockIdx.x]; if (v.y != 0.0f) m = fmaxf(m, v.x); }
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    for (int p = 0; p < A.parts; p++) {
-        float2 v = A.pm[p * rows + blockIdx.x];
-        if (v.y == 0.0f) continue;
-        float e = exp2_(v.x - m);
-        sum = fmaf(v.y, e, sum);
-        if ((p & 3) == w)
-#pragma unroll
-            for (int i = 0; i < D / 64; i++) o[i] = fmaf(e, A.po[(p * rows + blockIdx.x) * D + l * (D / 64) + i], o[i]);
+    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 15, g = l >> 4;
+    const int kvh = blockIdx.x % A.kv.heads, c = blockIdx.x / A.kv.heads;
+    AttTileAt at;
+    int from, end;
+    if (A.over_shared) {
+        at.s = 0; at.t0 = 0; at.row0 = blockIdx.y * 16; at.rows = att_start(a, a.nseq) * A.group;
+        from = c * A.chunk; end = min(from + A.chunk, a.shared);
+    } else {
+        at.s = blockIdx.y; at.t0 = att_start(a, at.s); at.row0 = 0;
+        int tokens = att_start(a, at.s + 1) - at.t0;
+        at.rows = min(tokens, a.max_q) * A.group;
+        if (at.rows > A.few || tokens < 1) return;
+        AttChunks ch = att_chunks(A, at.s, tokens);
+        if (c >= ch.n) return;
+        from = ch.from + c * A.chunk; end = from + A.chunk;
     }
+    if (at.row0 >= at.rows) return;
+    const AttRow R = att_row(A, at, at.row0 + n, kvh);
+    const bool some = R.live && R.lo < R.hi;
+    int p0 = max(from, wave_min(some ? R.lo : INT32_MAX) & ~31), p1 = min(end, wave_max(some ? R.hi : 0));
+    if (p0 >= p1) p0 = p1 = 0;   // nothing seen (p0 may be close to the largest int: no wave's first run is counted from it)
+    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
+    u4 q[KS];
+    {
+        const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * g;
 #pragma unroll
-    for (int i = 0; i < D / 64; i++) acc[w][l * (D / 64) + i] = o[i];
+        for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 32 * s);
+    }
+    const float slope = BIAS ? a.slopes[R.head] * ATT_LOG2E : 0.0f;
+    const int32_t *table = a.table + (int64_t)at.s * a.width;
+    auto ids = [&](int p) { return table[min((p + 16 * (l & 1)) >> A.sh, a.width - 1)]; };   // lane i % 2: positions p + 16 i ..
+    // keys: lane (g, n) row n, dims 32 s + 8 g ..; values: rows 4 g + i, dims E n ..
+    const uint32_t ko = (uint32_t)(n * A.kv.token_stride + 8 * g) * 2;
+    uint32_t vo[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) vo[i] = (uint32_t)((4 * g + i) * A.kv.token_stride + E * n) * 2;
+    struct Run { u4 k[2][KS]; uint32_t v[2][4][E / 2]; unsigned bad; } r;
+    auto place = [&](const void *base, int p, int id, int u) {
+        int blk = __builtin_amdgcn_readlane(id, u);
+        if ((unsigned)blk >= (unsigned)A.kv.nblocks) blk = 0;
+        return (gb *)base + (blk * A.kv.block_stride + kvh * A.kv.head_stride + ((p + 16 * u) & (A.kv.block_size - 1)) * A.kv.token_stride) * 2;
+    };
+    auto load_k = [&](int p, int id) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            gb *kp = place(A.kv.k, p, id, u);
+#pragma unroll
+            for (int s = 0; s < KS; s++) r.k[u][s] = *(const gu4 *)(kp + ko + 64 * s);
+        }
+    };
+    auto load_v = [&](int p, int id) {
+        r.bad = (unsigned)__ballot((unsigned)id >= (unsigned)A.kv.nblocks) & 3u;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            gb *vp = place(A.kv.v, p, id, u);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (E == 8) {
+                    u4 v = *(const gu4 *)(vp + vo[i]);
+#pragma unroll
+                    for (int x = 0; x < E / 2; x++) r.v[u][i][x] = v[x & 3];
+                } else {
+                    typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+                    u2v v = *(const __attribute__((address_space(1))) u2v *)(vp + vo[i]);
+                    r.v[u][i][0] = v[0]; r.v[u][i][1] = v[1];
+                }
+            }
+        }
+    };
+    f4 acc[E];
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[e] = f4{0, 0, 0, 0};
+    float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f;
+
+    auto step = [&](int p, auto &&after_scores) {
+        f4 s[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            s[u] = f4{0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KS; k++) s[u] = mfma16<T>(r.k[u][k], q[k], s[u]);
+        }
+        after_scores();
+        const float dist = BIAS ? (float)(R.pos - p - 4 * g) : 0.0f;
+        const bool part = p < inlo || p + 32 > inhi || r.bad;
+        float mt = -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float x = s[u][j] * A.s1;
+                if (CAP) x = fmaf(-2.0f * A.s2, __builtin_amdgcn_rcpf(1.0f + exp2_(x)), A.s2);
+                if (BIAS) x = fmaf(-slope, fabsf(dist - (float)(16 * u + j)), x);
+                int at = p + 16 * u + 4 * g + j;
+                if (part) x = at >= R.lo && at < R.hi && !((r.bad >> u) & 1) ? x : -__builtin_inff();
+                s[u][j] = x;
+                mt = fmaxf(mt, x);
+            }
+        mt = max_quarters(mt);
+        if (__any(mt > m + 8.0f)) {
+            float mn = fmaxf(m, mt), bn = mn == -__builtin_inff() ? 0.0f : mn, al = exp2_(m - bn);
+            m = mn; mb = bn; sum *= al;
+#pragma unroll
+            for (int e = 0; e < E; e++) acc[e] *= al;
+        }
+        u4 pf;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                float e0 = exp2_(s[u][j] - mb), e1 = exp2_(s[u][j + 1] - mb);
+                sum += e0 + e1;
+                pf[2 * u + (j >> 1)] = pack2<T>(e0, e1);
+            }
+        bool odd = false;
+        if (part) {
+            bool o = false;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int x = 0; x < E / 2; x++) o |= odd16<T>(r.v[u][i][x]) | odd16<T>(r.v[u][i][x] >> 16);
+            odd = __any(o);
+        }
+        if (odd) {   // infinities and NaN go round the product, to the rows that see their position (the wave's values through its part of LDS)
+            uint32_t *t = (uint32_t *)joint[w];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int x = 0; x < E / 2; x++) {
+                        t[(16 * u + 4 * g + i) * (D / 2) + n * (E / 2) + x] = r.v[u][i][x];
+                        r.v[u][i][x] = only_finite<T>(r.v[u][i][x]);
+                    }
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+            for (int k = 0; k < 32; k++) {
+                const bool see = p + k >= R.lo && p + k < R.hi && !((r.bad >> (k >> 4)) & 1);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        uint32_t v = t[k * (D / 2) + ((4 * g + j) * E + e) / 2] >> (16 * (e & 1));
+                        acc[e][j] += see & odd16<T>(v) ? half_to_f<T>(v & 0xffff) : 0.0f;
+                    }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            u4 f;
+#pragma unroll
+            for (int x = 0; x < 4; x++)   // positions 2 x and 2 x + 1 of the lane's eight
+                f[x] = __builtin_amdgcn_perm(r.v[x >> 1][2 * (x & 1) + 1][e >> 1], r.v[x >> 1][2 * (x & 1)][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
+            acc[e] = mfma16<T>(f, pf, acc[e]);
+        }
+    };
+    int p = p0 + 32 * w;
+    if (p < p1) {
+        int id = ids(p), next = ids(p + 128);
+        load_k(p, id);
+        load_v(p, id);
+        for (; p + 128 < p1; p += 128) {
+            step(p, [&] { load_k(p + 128, next); });
+            load_v(p + 128, next);
+            next = ids(p + 256);
+        }
+        step(p, [] {});
+    }
+    sum = add_quarters(sum);
+    if (g == 0) stat[w][n] = make_float2(mb, sum);
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int e = 0; e < E; e += 4) *(f4 *)&joint[w][n][(4 * g + j) * E + e] = f4{acc[e][j], acc[e + 1][j], acc[e + 2][j], acc[e + 3][j]};
     __syncthreads();
-    if (threadIdx.x < D / 2) {
-        int d = threadIdx.x * 2;
-        float inv = 1.0f / sum, x = acc[0][d] + acc[1][d] + (acc[2][d] + acc[3][d]), y = acc[0][d + 1] + acc[1][d + 1] + (acc[2][d + 1] + acc[3][d + 1]);
-        *(uint32_t *)((uint16_t *)a.out + (int64_t)tok * a.out_token + head * a.out_head + d) = sum == 0.0f ? 0u : pack2<T>(x * inv, y * inv);
+    // rows of 16 threads, D / 16 dims each
+    const int jr = threadIdx.x >> 4, d = (threadIdx.x & 15) * E, row = at.row0 + jr;
+    if (row >= at.rows) return;
+    float2 st[4];
+    float mx = -__builtin_inff(), total = 0.0f, o[E] = {};
+#pragma unroll
+    for (int i = 0; i < 4; i++) { st[i] = stat[i][jr]; if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x); }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (st[i].y == 0.0f) continue;
+        float e = exp2_(st[i].x - mx);
+        total = fmaf(st[i].y, e, total);
+#pragma unroll
+        for (int x = 0; x < E; x++) o[x] = fmaf(e, joint[i][jr][d + x], o[x]);
     }
-    if (a.lse && threadIdx.x == 0) a.lse[blockIdx.x] = sum == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * ATT_LN2;
+    const int j = row / A.group, tok = at.t0 + j, head = kvh * A.group + row - j * A.group;
+    if (A.over_shared) {   // tokens past max_q have no partial results
+        int s = max(count_le(a.qstart, a.nseq, tok) - 1, 0);
+        if (tok - a.qstart[s] >= a.max_q) return;
+    }
+    if (A.parts == 1) {
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        uint32_t *op = (uint32_t *)((uint16_t *)a.out + (int64_t)tok * a.out_token + head * a.out_head + d);
+#pragma unroll
+        for (int x = 0; x < E; x += 2) op[x / 2] = total == 0.0f ? 0u : pack2<T>(o[x] * inv, o[x + 1] * inv);
+        if (a.lse && d == 0) a.lse[(int64_t)tok * a.heads + head] = total == 0.0f ? -__builtin_inff() : (mx + __builtin_amdgcn_logf(total)) * ATT_LN2;
+        return;
+    }
+    const int64_t at_row = ((int64_t)(A.part0 + c) * a.ntok + tok) * a.heads + head;
+    if (d == 0) A.pm[at_row] = make_float2(mx, total);
+    if (total == 0.0f) return;
+#pragma unroll
+    for (int x = 0; x < E; x += 4) *(f4 *)(A.po + at_row * D + d + x) = f4{o[x], o[x + 1], o[x + 2], o[x + 3]};
+}
+
+// The partial results of a row: their maxima and sums give each a weight. D / 4 lanes per row and part; ALL: every lane group
+// of the workgroup on one row (many parts), else each on its own.
+template <int T, int D, bool ALL>
+__global__ void __launch_bounds__(256) k_attn_join(AttArgs A) {
+    constexpr int LPR = D / 4, GR = 256 / LPR;
+    const mmoe_attn_args &a = A.a;
+    __shared__ float red[GR], acc[GR][D];
+    const int gi = threadIdx.x / LPR, x = (threadIdx.x % LPR) * 4, row = ALL ? blockIdx.x : blockIdx.x * GR + gi;
+    const int tok = row / a.heads, head = row - tok * a.heads;
+    if (tok >= att_start(a, a.nseq)) return;
+    const int s = max(count_le(a.qstart, a.nseq, tok) - 1, 0), t0 = att_start(a, s), tokens = att_start(a, s + 1) - t0;
+    if (tok - t0 >= a.max_q) return;
+    const int parts = A.split_sh + (min(tokens, a.max_q) * A.group <= A.few ? att_chunks(A, s, tokens).n : A.split);
+    const int64_t rows = (int64_t)a.ntok * a.heads;
+    const int first = ALL ? gi : 0, by = ALL ? GR : 1;
+    float m = -__builtin_inff(), sum = 0.0f;
+    f4 o = {0, 0, 0, 0};
+    for (int p = first; p < parts; p += by) { float2 v = A.pm[p * rows + row]; if (v.y != 0.0f) m = fmaxf(m, v.x); }
+    if (ALL) {
+        if (x == 0) red[gi] = m;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < GR; i++) m = fmaxf(m, red[i]);
+        __syncthreads();
+    }
+#pragma unroll 4
+    for (int p = first; p < parts; p += by) {
+        float2 v = A.pm[p * rows + row];
+        f4 y = v.y != 0.0f ? *(const f4 *)(A.po + (p * rows + row) * D + x) : f4{0, 0, 0, 0};
+        float e = v.y != 0.0f ? exp2_(v.x - m) : 0.0f;
+        sum = fmaf(v.y, e, sum);
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[i] = fmaf(e, y[i], o[i]);
+    }
+    if (ALL) {
+        *(f4 *)&acc[gi][x] = o;
+        if (x == 0) red[gi] = sum;
+        __syncthreads();
+        if (gi) return;
+#pragma unroll
+        for (int i = 1; i < GR; i++) { o += *(const f4 *)&acc[i][x]; sum += red[i]; }
+    }
+    const float inv = 1.0f / sum;
+    uint2 v = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+    if (sum == 0.0f) v = make_uint2(0, 0);
+    *(uint2 *)((uint16_t *)a.out + (int64_t)tok * a.out_token + head * a.out_head + x) = v;
+    if (a.lse && x == 0) a.lse[row] = sum == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * ATT_LN2;
 }

@@ -135,46 +135,76 @@ static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
     return 0;
 }
 
-// How a call is divided: row tiles, and runs of positions where the tiles alone are too few workgroups.
-struct AttPlan { int tiles, split, tiles_sh, split_sh, parts; size_t bytes; };
+// How a call is divided: row tiles, and runs or chunks of positions where the tiles alone are too few workgroups.
+struct AttPlan { int few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts; size_t bytes; };
 static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     AttPlan p = {};
-    const int64_t rows = (int64_t)a.ntok * (a.heads / kv.heads), want = 512;
-    p.tiles = (int)((rows + 127) / 128) + a.nseq;
-    auto runs = [&](int64_t tiles, int64_t positions) {
-        int64_t n = (want + tiles * kv.heads - 1) / (tiles * kv.heads), most = (positions + 255) / 256;
-        return (int)(n < 1 || most < 1 ? 1 : n > most ? most : n);
+    const int group = a.heads / kv.heads;
+    const int64_t rows = (int64_t)a.ntok * group, tiles = (rows + 127) / 128;
+    const int own = a.window && !a.hi ? (int)std::min<int64_t>(a.max_len - a.shared, (int64_t)a.window + a.max_q) : a.max_len - a.shared;
+    // runs of at least `least` positions until there are about `want` workgroups
+    auto runs = [&](int64_t groups, int positions, int want, int least) {
+        int64_t n = (want + groups * kv.heads - 1) / (groups * kv.heads), most = (positions + least - 1) / least;
+        return (int)std::max<int64_t>(1, std::min(n, most));
     };
-    p.split = runs(p.tiles - a.nseq, a.window ? std::min(a.max_len - a.shared, a.window + a.max_q) : a.max_len - a.shared);
+    p.chunk = 512;
     if (a.shared) {
-        p.tiles_sh = (int)((rows + 127) / 128);
-        p.split_sh = runs(p.tiles_sh, a.shared);
+        p.few_sh = rows <= 32;
+        if (p.few_sh) {
+            while (p.chunk > 128 && (rows + 15) / 16 * kv.heads * (a.shared / p.chunk) < 512) p.chunk >>= 1;
+            p.split_sh = (a.shared + p.chunk - 1) / p.chunk;
+        } else {
+            p.tiles_sh = (int)tiles;
+            p.split_sh = runs(tiles, a.shared, 512, 256);
+        }
     }
-    p.parts = p.split + p.split_sh;
+    if (std::min<int64_t>(a.max_q, a.ntok) * group <= 16 || a.nseq > 1) {
+        p.few = 16;
+        if (!p.few_sh) while (p.chunk > 128 && (int64_t)a.nseq * kv.heads * (own / p.chunk) < 512) p.chunk >>= 1;
+        p.chunks = (own + 31 + p.chunk - 1) / p.chunk;
+        p.split = p.chunks;
+    }
+    if (std::min<int64_t>(a.max_q, a.ntok) * group > p.few) {
+        p.tiles = (int)tiles + a.nseq;
+        p.split = runs(tiles, own, 256, 256);
+    }
+    p.parts = p.split_sh + std::max(p.split, p.chunks);
     p.bytes = 256;
     if (p.parts > 1) p.bytes += (size_t)p.parts * a.ntok * a.heads * (kv.head_dim * 4 + 8);
     return p;
 }
 
-template <int T, int D>
+template <int T, int D, bool CAP, bool BIAS>
 static int att_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPlan &p) {
     AttArgs A{};
     A.a = a; A.kv = kv;
     A.sh = log2_block(kv.block_size); A.group = a.heads / kv.heads;
-    A.parts = p.parts;
-    A.s1 = a.cap > 0 ? 2.0f * a.scale / a.cap * ATT_LOG2E : a.scale * ATT_LOG2E;
+    A.parts = p.parts; A.chunk = p.chunk; A.chunks = p.chunks; A.few = p.few; A.split = p.split; A.split_sh = p.split_sh;
+    A.s1 = CAP ? 2.0f * a.scale / a.cap * ATT_LOG2E : a.scale * ATT_LOG2E;
     A.s2 = a.cap * ATT_LOG2E;
     A.pm = (float2 *)a.ws;
     A.po = (float *)((uint8_t *)a.ws + (size_t)p.parts * a.ntok * a.heads * 8);
-    auto tile = [&](int tiles, int split, int part0, int over) {
-        A.nsplit = split; A.part0 = part0; A.over_shared = over;
-        dim3 g((unsigned)tiles * split * kv.heads);
-        if (a.cap > 0) return a.slopes ? run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, true, true>, g, 256, A) : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, true, false>, g, 256, A);
-        return a.slopes ? run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, false, true>, g, 256, A) : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, false, false>, g, 256, A);
-    };
-    if (p.split_sh && tile(p.tiles_sh, p.split_sh, 0, 1)) return -1;
-    if (tile(p.tiles, p.split, p.split_sh, 0)) return -1;
-    return p.parts > 1 ? run(MMOE_K_ATT_PAGED, k_attn_join<T, D>, dim3((unsigned)a.ntok * a.heads), 256, A) : 0;
+    const unsigned kvh = kv.heads, rows = (unsigned)a.ntok * A.group;
+    if (a.shared) {
+        A.over_shared = 1;
+        A.nsplit = p.split_sh;
+        if (p.few_sh ? run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, dim3(kvh * p.split_sh, (rows + 15) / 16), 256, A)
+                     : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS>, dim3(kvh * p.split_sh * p.tiles_sh), 256, A)) return -1;
+        A.over_shared = 0;
+        A.part0 = p.split_sh;
+    }
+    if (p.chunks && run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, dim3(kvh * p.chunks, a.nseq), 256, A)) return -1;
+    A.nsplit = p.split;
+    if (p.tiles && run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS>, dim3(kvh * p.split * p.tiles), 256, A)) return -1;
+    if (p.parts == 1) return 0;
+    constexpr int per = 256 / (D / 4);   // rows of a workgroup where each is a lane group's
+    return p.parts > 8 ? run(MMOE_K_ATT_PAGED, k_attn_join<T, D, true>, dim3((unsigned)a.ntok * a.heads), 256, A)
+                       : run(MMOE_K_ATT_PAGED, k_attn_join<T, D, false>, dim3(((unsigned)a.ntok * a.heads + per - 1) / per), 256, A);
+}
+template <int T, int D>
+static int att_pick(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPlan &p) {
+    if (a.cap > 0) return a.slopes ? att_run<T, D, true, true>(a, kv, p) : att_run<T, D, true, false>(a, kv, p);
+    return a.slopes ? att_run<T, D, false, true>(a, kv, p) : att_run<T, D, false, false>(a, kv, p);
 }
 
 extern "C" {
@@ -225,8 +255,8 @@ int mmoe_attn_paged(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
     if (mm_ready()) return -1;
     OnDevice dev;
     if (!dev.ok) return -1;
-    if (kv->dtype == MMOE_F16) return kv->head_dim == 64 ? att_run<MMOE_F16, 64>(a, *kv, pl) : att_run<MMOE_F16, 128>(a, *kv, pl);
-    return kv->head_dim == 64 ? att_run<MMOE_BF16, 64>(a, *kv, pl) : att_run<MMOE_BF16, 128>(a, *kv, pl);
+    if (kv->dtype == MMOE_F16) return kv->head_dim == 64 ? att_pick<MMOE_F16, 64>(a, *kv, pl) : att_pick<MMOE_F16, 128>(a, *kv, pl);
+    return kv->head_dim == 64 ? att_pick<MMOE_BF16, 64>(a, *kv, pl) : att_pick<MMOE_BF16, 128>(a, *kv, pl);
 }
 
 }  // extern "C"
