@@ -375,6 +375,8 @@ template <int T> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+// the larger of two numbers, without fmaxf's quieting of each (a NaN shows in the weights, whatever the maximum then is)
+__device__ __forceinline__ float max_(float x, float y) { return __builtin_amdgcn_fmed3f(x, y, __builtin_inff()); }
 // 16 bytes per lane from base + off to LDS at to + 16 * lane. Asm, so that the compiler does not wait for it before every later LDS
 // read; nothing is written to a register. The waits are the caller's.
 __device__ __forceinline__ void load_lds(const uint8_t *base, uint32_t off, uint32_t to) {
@@ -464,7 +466,7 @@ template <int T, int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
     constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // bytes and chunks of a row, rows and instructions of a wave's load
     __shared__ __attribute__((aligned(1024))) uint8_t tiles[2][2 * ATT_BN * RB];   // keys, values
-    __shared__ int range[2][4];
+    __shared__ int range[4][4], flag[2][4];
     const mmoe_attn_args &a = A.a;
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 31, hh = l >> 5;
     const int kvh = blockIdx.x % A.kv.heads, rest = blockIdx.x / A.kv.heads, split = rest % A.nsplit;
@@ -475,10 +477,12 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
     const bool some = R.live && R.lo < R.hi;
     const int wlo = wave_min(some ? R.lo : INT32_MAX), whi = wave_max(some ? R.hi : 0);
     const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
-    if (l == 0) { range[0][w] = wlo; range[1][w] = whi; }
+    if (l == 0) { range[0][w] = wlo; range[1][w] = whi; range[2][w] = inlo; range[3][w] = inhi; }
     __syncthreads();
     int p0 = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3])) & ~(ATT_BN - 1);
     int p1 = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
+    const int glo = __builtin_amdgcn_readfirstlane(max(max(range[2][0], range[2][1]), max(range[2][2], range[2][3])));
+    const int ghi = __builtin_amdgcn_readfirstlane(min(min(range[3][0], range[3][1]), min(range[3][2], range[3][3])));
     if (A.nsplit > 1 && p0 < p1) {
         int run = ((p1 - p0 + ATT_BN - 1) / ATT_BN + A.nsplit - 1) / A.nsplit * ATT_BN;
         p0 += split * run;
@@ -511,10 +515,18 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
     for (int k = 0; k < KS; k++) ka[k] = n * RB + (((2 * k + hh) ^ (n & (CH - 1))) << 4);
 #pragma unroll
     for (int i = 0; i < DS; i++) va[i] = ATT_BN * RB + vr * RB + ((64 * i + 32 * ((l >> 4) & 1) + 8 * (l & 3)) ^ ((vr & (CH / 2 - 1)) << 5));
+    // block ids of 64 groups of 16 positions at a time, group l in lane l; a load of their own each tile would have to be waited for
+    // with the tile's
     const int32_t *table = a.table + (int64_t)at.s * a.width;
-    auto ids = [&](int p) { return table[min((p + 16 * (l & 3)) >> A.sh, a.width - 1)]; };   // lane i % 4: positions p + 16 i ..
-    auto fetch = [&](uint32_t buf, int p, int id) {
-        int blk = __builtin_amdgcn_readlane(id, w);
+    int id = 0, idp = 0;      // ids of the positions from idp on
+    uint64_t lost = 0;        // those that are none of the cache's
+    auto ids = [&](int p) {
+        idp = p;
+        id = table[min((p + 16 * l) >> A.sh, a.width - 1)];
+        lost = __ballot((unsigned)id >= (unsigned)A.kv.nblocks);
+    };
+    auto fetch = [&](uint32_t buf, int p) {
+        int blk = __builtin_amdgcn_readlane(id, ((p - idp) >> 4) + w);
         if ((unsigned)blk >= (unsigned)A.kv.nblocks) blk = 0;
         const int64_t at0 = (blk * A.kv.block_stride + kvh * A.kv.head_stride + ((p + 16 * w) & (A.kv.block_size - 1)) * A.kv.token_stride) * 2;
         const uint8_t *kp = (const uint8_t *)A.kv.k + at0, *vp = (const uint8_t *)A.kv.v + at0;
@@ -535,15 +547,18 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
         const lb *kl = (const lb *)(uintptr_t)buf;
         f16v s[2];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
+        for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int j = 0; j < 16; j++) s[u][j] = 0.0f;
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                u4 kf = *(const lu4 *)(kl + ka[k] + 32 * u * RB);
-                s[u] = mfma32<T>(kf, q[k], s[u]);
-            }
-        }
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) s[u] = mfma32<T>(*(const lu4 *)(kl + ka[k] + 32 * u * RB), q[k], s[u]);
+        // six reads ahead of the products
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int k = 0; k < 2 * KS - 6; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
+        __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
         // scores in units of log 2
         const float dist = BIAS ? (float)(R.pos - p - 4 * hh) : 0.0f;
         if (CAP || BIAS)
@@ -572,7 +587,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int j = 0; j < 16; j += 2) mt = fmaxf(mt, fmaxf(s[u][j], s[u][j + 1]));
+            for (int j = 0; j < 16; j++) mt = max_(mt, s[u][j]);
         mt = max_halves(mt) * sc;
         // a new maximum only once it is 2^8 past the old: until then weights stay below 2^8, in every type's range
         if (__any(mt > m + 8.0f)) {
@@ -583,6 +598,16 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
 #pragma unroll
                 for (int j = 0; j < 16; j++) acc[i][j] *= al;
         }
+        // V^T: lane (hh, n) of operand A holds dim 32 i + n, positions 16 k + 4 hh + {0 .. 3, 8 .. 11}
+        auto value = [&](int i, int k) {
+            uint2 t0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(kl + va[i] + 16 * k * RB)));
+            uint2 t1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(kl + va[i] + (16 * k + 8) * RB)));
+            return u4{t0.x, t0.y, t1.x, t1.y};
+        };
+        u4 f0[DS];   // the first positions' are on their way during the exponentials
+#pragma unroll
+        for (int i = 0; i < DS; i++) f0[i] = value(i, 0);
+        __builtin_amdgcn_sched_barrier(0);
         u4 pf[4];
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -592,52 +617,39 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
                 sum += e0 + e1;
                 pf[2 * u + (j >> 3)][(j & 7) >> 1] = pack2<T>(e0, e1);
             }
-        // V^T: lane (hh, n) of operand A holds dim 32 i + n, positions 16 k + 4 hh + {0 .. 3, 8 .. 11}
-        auto value = [&](int i, int k) {
-            uint2 t0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(kl + va[i] + 16 * k * RB)));
-            uint2 t1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(kl + va[i] + (16 * k + 8) * RB)));
-            return u4{t0.x, t0.y, t1.x, t1.y};
-        };
-        bool odd = false;
-        if (part) {   // a value that is not finite times a weight of 0 is NaN: such tiles take the long way
-            bool o = false;
-#pragma unroll 1
-            for (int i = 0; i < ATT_BN * RB / 1024; i++) {
-                u4 v = *(const lu4 *)(kl + ATT_BN * RB + i * 1024 + l * 16);
 #pragma unroll
-                for (int x = 0; x < 4; x++) o |= odd16<T>(v[x]) | odd16<T>(v[x] >> 16);
-            }
-            odd = __any(o);
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int i = 0; i < DS; i++) acc[i] = mfma32<T>(k ? value(i, k) : f0[i], pf[k], acc[i]);
+#pragma unroll
+        for (int k = 0; k < 3 * DS; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
+        __builtin_amdgcn_sched_group_barrier(0x8, DS, 0);
+    };
+    // A value that is not finite times a weight of 0 is NaN, so in a tile that is not seen whole such values go round the product:
+    // the tile's are set aside in the other buffer and zeroed, and afterwards added, as they are, to the rows that see their position.
+    auto set_aside = [&](uint32_t buf, uint32_t other) {
+#pragma unroll
+        for (int x = 0; x < NI; x++) {
+            const uint32_t o = ATT_BN * RB + w * 16 * RB + x * 1024 + l * 16;
+            u4 v = *(const lu4 *)((lb *)(uintptr_t)buf + o);
+            *(lu4 *)((lb *)(uintptr_t)other + o) = v;
+#pragma unroll
+            for (int y = 0; y < 4; y++) v[y] = only_finite<T>(v[y]);
+            *(lu4 *)((lb *)(uintptr_t)buf + o) = v;
         }
-        if (!odd) {
-#pragma unroll
-            for (int i = 0; i < DS; i++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) acc[i] = mfma32<T>(value(i, k), pf[k], acc[i]);
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < DS; i++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                u4 f = value(i, k);
-#pragma unroll
-                for (int x = 0; x < 4; x++) f[x] = only_finite<T>(f[x]);
-                acc[i] = mfma32<T>(f, pf[k], acc[i]);
-                __builtin_amdgcn_sched_barrier(0);   // registers, not speed
-            }
-        // infinities and NaN of the positions a row does see, added as they are
+    };
+    auto add_aside = [&](uint32_t other, int p, unsigned bad) {
 #pragma unroll 1
         for (int r = 0; r < ATT_BN; r++) {
             const bool see = p + r >= R.lo && p + r < R.hi && !((bad >> (r >> 4)) & 1);
             uint32_t row = ATT_BN * RB + r * RB + 8 * hh, x = (r & (CH / 2 - 1)) << 5;
-            asm("" : "+v"(row));   // its 64 addresses are not worth a register outside
+            asm("" : "+v"(row));   // its addresses are not worth a register outside
 #pragma unroll
             for (int i = 0; i < DS; i++)
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
                     typedef __attribute__((address_space(3))) uint64_t l8;
-                    uint64_t v = *(const l8 *)(kl + row + ((64 * i + 4 * j) ^ x));
+                    uint64_t v = *(const l8 *)((const lb *)(uintptr_t)other + row + ((64 * i + 4 * j) ^ x));
 #pragma unroll
                     for (int y = 0; y < 4; y++, v >>= 16) {
                         acc[i][j + y] += see & odd16<T>((uint32_t)v) ? half_to_f<T>((uint32_t)v & 0xffff) : 0.0f;
@@ -649,19 +661,45 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
 
     if (p0 < p1) {
         uint32_t buf = (uint32_t)(uintptr_t)(lb *)tiles;
-        int id = ids(p0), next = ids(p0 + ATT_BN);
-        fetch(buf, p0, id);
-        for (int p = p0; p < p1; p += ATT_BN) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the loads below are the compiler's no more than they are its waits'
-            __syncthreads();   // the tile has arrived, and every wave is done with the other buffer
-            const unsigned bad = (unsigned)__ballot((unsigned)id >= (unsigned)A.kv.nblocks) & 15u;
-            const uint32_t other = buf ^ (2 * ATT_BN * RB);
-            if (p + ATT_BN < p1) {
-                id = next;
-                next = ids(p + 2 * ATT_BN);
-                fetch(other, p + ATT_BN, id);
+        ids(p0);
+        fetch(buf, p0);
+        unsigned bad = (unsigned)lost & 15u;
+#pragma unroll
+        for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));   // the queries are there: nothing in the loop waits for them
+        for (int p = p0, i = 0; p < p1; p += ATT_BN, i ^= 1) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the compiler does not know of these loads
+            const bool part = p < glo || p + ATT_BN > ghi || bad;
+            if (part) {   // the wave's own 16 rows of values: are they finite?
+                bool o = false;
+#pragma unroll
+                for (int x = 0; x < NI; x++) {
+                    u4 v = *(const lu4 *)((const lb *)(uintptr_t)buf + ATT_BN * RB + w * 16 * RB + x * 1024 + l * 16);
+#pragma unroll
+                    for (int y = 0; y < 4; y++) o |= odd16<T>(v[y]) | odd16<T>(v[y] >> 16);
+                }
+                o = __any(o);
+                if (l == 0) flag[i][w] = o;
             }
-            if (p < whi && p + ATT_BN > wlo) tile(buf, p, bad);
+            __syncthreads();   // the tile has arrived, and every wave is done with the other buffer
+            bool odd = false;
+            if (part) odd = __builtin_amdgcn_readfirstlane(flag[i][0] | flag[i][1] | flag[i][2] | flag[i][3]) != 0;
+            const uint32_t other = buf ^ (2 * ATT_BN * RB);
+            const unsigned now = bad;
+            const bool more = p + ATT_BN < p1, mine = p < whi && p + ATT_BN > wlo;
+            if (more) {
+                if (p + ATT_BN - idp == 1024) ids(p + ATT_BN);
+                bad = (unsigned)(lost >> ((p + ATT_BN - idp) >> 4)) & 15u;
+            }
+            if (odd) {
+                set_aside(buf, other);
+                __syncthreads();
+            } else if (more) fetch(other, p + ATT_BN);
+            if (mine) tile(buf, p, now);
+            if (odd) {
+                if (mine) add_aside(other, p, now);
+                __syncthreads();
+                if (more) fetch(other, p + ATT_BN);
+            }
             buf = other;
         }
     }

@@ -146,6 +146,9 @@ def attend(q, keys, values, pos, see, scale, cap, slopes, half):
                 top = x.max()
                 if top == -np.inf:
                     continue
+                if not top < np.inf:     # a score that is NaN or infinite
+                    out[i, h], lse[i, h] = np.nan, np.nan
+                    continue
                 w = np.exp(x - top)
                 e = (e + 2.0 ** -22 * np.abs(x - top) + 2.0 ** -21)
                 l = w.sum()
@@ -287,6 +290,7 @@ class Batch:
             assert (gl[~served] == 77.0).all()
             gl, l, lo = gl[:live][sv].astype(np.float64), lse[:live][sv], loff[:live][sv]
             f = np.isfinite(l)
-            assert np.array_equal(gl[~f], l[~f]) or np.isnan(gl[~f]).all()
-            assert (np.abs(gl - l)[f] <= lo[f]).all(), (note, "lse", np.abs(gl - l)[f].max())
+            assert np.array_equal(gl[l == -np.inf], l[l == -np.inf]) and not np.isfinite(gl[np.isnan(l)]).any()
+            gl, l, lo = gl[f], l[f], lo[f]
+            assert (np.abs(gl - l) <= lo).all(), (note, "lse", np.abs(gl - l).max())
         return worst

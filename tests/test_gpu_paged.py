@@ -218,6 +218,19 @@ def test_rope_in_place_equals_out_of_place(rot, inter):
 
 
 # ---------------------------------------------------------------------------------------------------- attention
+def poison(*where):
+    """(sequence, position, k or v, value, dims) written into the cache"""
+    def put(b):
+        for s, p, which, x, dims in where:
+            c = b.k if which == "k" else b.v
+            c[b.table[s, p // b.bs], p % b.bs, :, dims] = encode(np.array([x]), b.kind)[0]
+    return put
+
+
+INF, NAN = float("inf"), float("nan")
+SOME = slice(3, 9)
+ODD = [(0, 250, "v", INF, SOME), (0, 251, "v", NAN, slice(60, 62)), (0, 20, "v", -INF, slice(10, 11)), (0, 290, "v", INF, slice(0, 1)), (0, 291, "v", -INF, slice(0, 1)),
+       (1, 128, "v", NAN, slice(0, 64)), (2, 5, "v", INF, slice(63, 64))]
 ATTN = {
     "one token, one position": dict(qlens=[1], lens=[1]),
     "one token at block and tile borders": dict(qlens=[1] * 9, lens=[2, 15, 16, 17, 31, 32, 33, 63, 65], heads=16, kv=4),
@@ -254,6 +267,14 @@ ATTN = {
     "no lse": dict(qlens=[1, 30, 2], lens=[700, 90, 3], heads=4, kv=1, with_lse=False),
     "token-major cache": dict(qlens=[1, 100, 3], lens=[700, 100, 90], heads=8, kv=4, token_major=True, kind="bf16"),
     "lost blocks": dict(qlens=[1, 100, 3, 1], lens=[700, 300, 90, 10], heads=8, kv=2, lost=[(0, 3), (0, 43), (1, 0), (1, 18), (2, 5), (3, 0)]),
+    "values that are not finite": [dict(qlens=[100, 1, 1], lens=[300, 129, 90], heads=4, kv=2, poison=poison(*ODD), kind=k, dim=d) for k, d in (("f16", 128), ("bf16", 64))],
+    "values that are not finite, window, mask": [dict(qlens=[100, 1, 4], lens=[300, 129, 90], heads=4, kv=1, poison=poison(*ODD), window=60),
+                                                 dict(qlens=[100, 1, 4], lens=[300, 129, 90], heads=4, kv=1, poison=poison(*ODD), lo=lambda p: p // 50 * 50, kind="bf16"),
+                                                 dict(qlens=[100, 1, 4], lens=[300, 129, 90], heads=4, kv=1, poison=poison(*ODD), hi=lambda p: np.minimum(p + 1, 128), kind="bf16")],
+    "values that are not finite, shared prefix": [dict(qlens=[1, 2, 1], lens=[300, 290, 270], shared=256, heads=h, kv=1, lo=lambda p: p % 3 * 50 + 180, poison=poison(
+        (0, 250, "v", INF, SOME), (0, 251, "v", NAN, slice(60, 62)), (0, 20, "v", -INF, SOME), (0, 200, "v", INF, slice(0, 1)), (1, 289, "v", NAN, slice(9, 10)))) for h in (4, 16)],
+    "keys that are not finite": [dict(qlens=[100, 1, 3], lens=[300, 129, 90], heads=4, kv=1, kind="bf16", poison=poison((0, 270, "k", NAN, SOME), (1, 128, "k", INF, slice(0, 1)),
+                                                                                                            (2, 88, "k", INF, SOME)))],
     "shared prefix, one token each": dict(qlens=[1] * 7, lens=[512 + 1 + 13 * s for s in range(7)], shared=512, heads=16, kv=4),
     "shared prefix, bf16, many": dict(qlens=[1] * 40, lens=[1024 + 1 + (29 * s) % 200 for s in range(40)], shared=1024, heads=8, kv=2, kind="bf16", bs=64),
     "shared prefix, heads of 64, drafts": dict(qlens=[1, 4, 3, 0, 2], lens=[300, 330, 291, 288, 500], shared=288, heads=6, kv=2, dim=64, bs=32),
