@@ -361,12 +361,14 @@ struct AttArgs {
     mmoe_attn_args a;
     mmoe_kv_cache kv;
     int sh, group;       // log2 of the block size, query heads per key/value head
-    int nsplit, part0, parts;   // runs of positions that this launch divides a tile's into, its first partial result, partial results in all
-    int over_shared;     // this launch: all tokens over the shared positions; else each sequence over the rest
-    int chunk, chunks, few;   // k_attn_few: positions per workgroup, most chunks of a sequence; sequences of up to few rows per key/value head are its own (0: none are)
-    int split, split_sh; // the call's runs per row tile over a sequence's own positions and over the shared ones
+    // one launch: n_sh workgroups over the shared positions (row tiles of 128, or of 16 with sh_few), n_tile over each sequence's own
+    // positions in row tiles of 128, n_few over those of sequences with up to `few` rows per key/value head (0: none) in chunks
+    unsigned n_sh, n_tile, n_few;
+    int sh_few, few;
+    int split_sh, split, chunk, chunks;   // runs of the shared positions, runs per row tile of the own ones; positions per chunk, most chunks
+    int parts_sh;        // partial results of the shared positions: split_sh, or 0
     float s1, s2;        // cap 0: score = s1 q.k in units of log 2; else s2 tanh, with exp(2 z) = exp2(s1 q.k)
-    float *po;           // partial results [parts][ntok * heads][head_dim], each over its own sum
+    float *po;           // partial results [parts][ntok * heads][head_dim], each over its own sum: the shared positions', then the own
     float2 *pm;          // their maxima (in units of log 2) and sums
 };
 
@@ -398,9 +400,9 @@ __device__ __forceinline__ int wave_max(int v) { for (int d = 1; d < 64; d <<= 1
 // on; no two sequences' tiles meet, and some virtual tiles are nobody's. No sums over the sequences are needed.
 __device__ __forceinline__ int att_start(const mmoe_attn_args &a, int s) { return min(max(a.qstart[s], 0), a.ntok); }   // never past the arrays
 struct AttTileAt { int s, row0, rows, t0; };   // first row of the tile in its sequence, the sequence's rows, its first token
-__device__ __forceinline__ bool att_find(const AttArgs &A, int bm, int v, AttTileAt &o) {
+__device__ __forceinline__ bool att_find(const AttArgs &A, bool shared, int bm, int v, AttTileAt &o) {
     const mmoe_attn_args &a = A.a;
-    if (A.over_shared) {
+    if (shared) {
         o.s = 0; o.t0 = 0; o.row0 = v * bm; o.rows = att_start(a, a.nseq) * A.group;
         return o.row0 < o.rows;
     }
@@ -414,7 +416,7 @@ __device__ __forceinline__ bool att_find(const AttArgs &A, int bm, int v, AttTil
     o.rows = min(att_start(a, lo + 1) - o.t0, a.max_q) * A.group;
     return o.row0 < o.rows && o.rows > A.few;
 }
-// A sequence's own positions in chunks: from `from` on, n of them (k_attn_few and k_attn_join agree through this)
+// A sequence's own positions in chunks: from `from` on, n of them, at least one (att_few and k_attn_join agree through this)
 struct AttChunks { int from, n; };
 __device__ __forceinline__ AttChunks att_chunks(const AttArgs &A, int s, int tokens) {
     const mmoe_attn_args &a = A.a;
@@ -422,12 +424,12 @@ __device__ __forceinline__ AttChunks att_chunks(const AttArgs &A, int s, int tok
     if (a.window > 0) from = max(from, len - tokens - a.window);
     from &= ~31;
     to = min(to, a.max_len);
-    return {from, to > from ? min((to - from + A.chunk - 1) / A.chunk, A.chunks) : 0};
+    return {from, to > from ? min((to - from + A.chunk - 1) / A.chunk, A.chunks) : 1};
 }
 
 // One query row as a lane sees it
 struct AttRow { int tok, head, pos, lo, hi; bool live; };
-__device__ __forceinline__ AttRow att_row(const AttArgs &A, const AttTileAt &at, int r, int kvh) {
+__device__ __forceinline__ AttRow att_row(const AttArgs &A, bool shared, const AttTileAt &at, int r, int kvh) {
     const mmoe_attn_args &a = A.a;
     AttRow o;
     o.live = r < at.rows;
@@ -435,7 +437,7 @@ __device__ __forceinline__ AttRow att_row(const AttArgs &A, const AttTileAt &at,
     int j = r / A.group, s = at.s;
     o.tok = at.t0 + j;
     o.head = kvh * A.group + r - j * A.group;
-    if (A.over_shared) s = max(count_le(a.qstart, a.nseq, o.tok) - 1, 0);
+    if (shared) s = max(count_le(a.qstart, a.nseq, o.tok) - 1, 0);
     int len = a.len[s], t0 = a.qstart[s];
     o.pos = len - (a.qstart[s + 1] - o.tok);
     if (o.tok - t0 >= a.max_q) o.live = false;
@@ -443,7 +445,7 @@ __device__ __forceinline__ AttRow att_row(const AttArgs &A, const AttTileAt &at,
     o.hi = a.hi ? a.hi[o.tok] : o.pos + 1;
     if (a.window > 0) o.lo = max(o.lo, o.pos - a.window);
     o.hi = max(min(min(o.hi, len), a.max_len), 0);
-    if (A.over_shared) o.hi = min(o.hi, a.shared); else o.lo = max(o.lo, a.shared);
+    if (shared) o.hi = min(o.hi, a.shared); else o.lo = max(o.lo, a.shared);
     return o;
 }
 
@@ -462,29 +464,32 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
 // pieces whose place in a row is exchanged by the row's number, so that neither the reads of 8 rows at one column nor the transposing
 // reads of 4 rows meet in a bank. P is rounded to the cache's type (half a step relative, as the result itself is), its
 // sum is of the unrounded 32-bit values.
+template <int D> struct AttTileMem {
+    __attribute__((aligned(1024))) uint8_t tiles[2][2 * ATT_BN * D * 2];   // keys, values
+    int range[4][4], flag[2][4];
+};
 template <int T, int D, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
+__device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, const unsigned block, AttTileMem<D> &M) {
     constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // bytes and chunks of a row, rows and instructions of a wave's load
-    __shared__ __attribute__((aligned(1024))) uint8_t tiles[2][2 * ATT_BN * RB];   // keys, values
-    __shared__ int range[4][4], flag[2][4];
     const mmoe_attn_args &a = A.a;
+    const int nsplit = shared ? A.split_sh : A.split;
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 31, hh = l >> 5;
-    const int kvh = blockIdx.x % A.kv.heads, rest = blockIdx.x / A.kv.heads, split = rest % A.nsplit;
+    const int kvh = block % A.kv.heads, rest = block / A.kv.heads, split = rest % nsplit;
     AttTileAt at;
-    if (!att_find(A, 128, gridDim.x / A.kv.heads / A.nsplit - 1 - rest / A.nsplit, at)) return;   // the last tiles see most: first
-    AttRow R = att_row(A, at, at.row0 + w * 32 + n, kvh);
+    if (!att_find(A, shared, 128, (shared ? A.n_sh : A.n_tile) / A.kv.heads / nsplit - 1 - rest / nsplit, at)) return;   // the last tiles see most: first
+    AttRow R = att_row(A, shared, at, at.row0 + w * 32 + n, kvh);
     // the wave's and the workgroup's positions
     const bool some = R.live && R.lo < R.hi;
     const int wlo = wave_min(some ? R.lo : INT32_MAX), whi = wave_max(some ? R.hi : 0);
     const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
-    if (l == 0) { range[0][w] = wlo; range[1][w] = whi; range[2][w] = inlo; range[3][w] = inhi; }
+    if (l == 0) { M.range[0][w] = wlo; M.range[1][w] = whi; M.range[2][w] = inlo; M.range[3][w] = inhi; }
     __syncthreads();
-    int p0 = min(min(range[0][0], range[0][1]), min(range[0][2], range[0][3])) & ~(ATT_BN - 1);
-    int p1 = max(max(range[1][0], range[1][1]), max(range[1][2], range[1][3]));
-    const int glo = __builtin_amdgcn_readfirstlane(max(max(range[2][0], range[2][1]), max(range[2][2], range[2][3])));
-    const int ghi = __builtin_amdgcn_readfirstlane(min(min(range[3][0], range[3][1]), min(range[3][2], range[3][3])));
-    if (A.nsplit > 1 && p0 < p1) {
-        int run = ((p1 - p0 + ATT_BN - 1) / ATT_BN + A.nsplit - 1) / A.nsplit * ATT_BN;
+    int p0 = min(min(M.range[0][0], M.range[0][1]), min(M.range[0][2], M.range[0][3])) & ~(ATT_BN - 1);
+    int p1 = max(max(M.range[1][0], M.range[1][1]), max(M.range[1][2], M.range[1][3]));
+    const int glo = __builtin_amdgcn_readfirstlane(max(max(M.range[2][0], M.range[2][1]), max(M.range[2][2], M.range[2][3])));
+    const int ghi = __builtin_amdgcn_readfirstlane(min(min(M.range[3][0], M.range[3][1]), min(M.range[3][2], M.range[3][3])));
+    if (nsplit > 1 && p0 < p1) {
+        int run = ((p1 - p0 + ATT_BN - 1) / ATT_BN + nsplit - 1) / nsplit * ATT_BN;
         p0 += split * run;
         p1 = min(p1, p0 + run);
     }
@@ -660,7 +665,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
     };
 
     if (p0 < p1) {
-        uint32_t buf = (uint32_t)(uintptr_t)(lb *)tiles;
+        uint32_t buf = (uint32_t)(uintptr_t)(lb *)M.tiles;
         ids(p0);
         fetch(buf, p0);
         unsigned bad = (unsigned)lost & 15u;
@@ -678,11 +683,11 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
                     for (int y = 0; y < 4; y++) o |= odd16<T>(v[y]) | odd16<T>(v[y] >> 16);
                 }
                 o = __any(o);
-                if (l == 0) flag[i][w] = o;
+                if (l == 0) M.flag[i][w] = o;
             }
             __syncthreads();   // the tile has arrived, and every wave is done with the other buffer
             bool odd = false;
-            if (part) odd = __builtin_amdgcn_readfirstlane(flag[i][0] | flag[i][1] | flag[i][2] | flag[i][3]) != 0;
+            if (part) odd = __builtin_amdgcn_readfirstlane(M.flag[i][0] | M.flag[i][1] | M.flag[i][2] | M.flag[i][3]) != 0;
             const uint32_t other = buf ^ (2 * ATT_BN * RB);
             const unsigned now = bad;
             const bool more = p + ATT_BN < p1, mine = p < whi && p + ATT_BN > wlo;
@@ -706,7 +711,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
     sum = add_halves(sum);
     if (!R.live) return;
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (A.parts == 1) {
+    if (nsplit == 1 && !A.parts_sh) {
         uint16_t *o = (uint16_t *)a.out + (int64_t)R.tok * a.out_token + R.head * a.out_head + 4 * hh;
 #pragma unroll
         for (int i = 0; i < DS; i++)
@@ -719,7 +724,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
         if (a.lse && hh == 0) a.lse[(int64_t)R.tok * a.heads + R.head] = sum == 0.0f ? -__builtin_inff() : (mb + __builtin_amdgcn_logf(sum)) * ATT_LN2;
         return;
     }
-    const int64_t row = ((int64_t)(A.part0 + split) * a.ntok + R.tok) * a.heads + R.head;
+    const int64_t row = ((int64_t)((shared ? 0 : A.parts_sh) + split) * a.ntok + R.tok) * a.heads + R.head;
     if (hh == 0) A.pm[row] = make_float2(mb, sum);
     if (sum == 0.0f) return;
     float *o = A.po + row * D + 4 * hh;
@@ -741,30 +746,34 @@ template <int T> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
 __device__ __forceinline__ float max_quarters(float x) { x = fmaxf(x, __shfl_xor(x, 16, 64)); return fmaxf(x, __shfl_xor(x, 32, 64)); }
 __device__ __forceinline__ float add_quarters(float x) { x += __shfl_xor(x, 16, 64); return x + __shfl_xor(x, 32, 64); }
 
+template <int D> struct AttFewMem {
+    __attribute__((aligned(16))) float joint[4][16][D + 4];
+    float2 stat[4][16];
+};
 template <int T, int D, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(256, 3) k_attn_few(AttArgs A) {
+__device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, const unsigned block, AttFewMem<D> &M) {
     constexpr int KS = D / 32, E = D / 16;   // products over the dims, values of a row per lane
-    __shared__ __attribute__((aligned(16))) float joint[4][16][D + 4];
-    __shared__ float2 stat[4][16];
     const mmoe_attn_args &a = A.a;
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 15, g = l >> 4;
-    const int kvh = blockIdx.x % A.kv.heads, c = blockIdx.x / A.kv.heads;
+    const int kvh = block % A.kv.heads, rest = block / A.kv.heads, runs = shared ? A.split_sh : A.chunks, c = rest % runs;
     AttTileAt at;
     int from, end;
-    if (A.over_shared) {
-        at.s = 0; at.t0 = 0; at.row0 = blockIdx.y * 16; at.rows = att_start(a, a.nseq) * A.group;
+    bool whole = false;   // the rows' only result
+    if (shared) {
+        at.s = 0; at.t0 = 0; at.row0 = rest / runs * 16; at.rows = att_start(a, a.nseq) * A.group;
         from = c * A.chunk; end = min(from + A.chunk, a.shared);
     } else {
-        at.s = blockIdx.y; at.t0 = att_start(a, at.s); at.row0 = 0;
+        at.s = rest / runs; at.t0 = att_start(a, at.s); at.row0 = 0;
         int tokens = att_start(a, at.s + 1) - at.t0;
         at.rows = min(tokens, a.max_q) * A.group;
         if (at.rows > A.few || tokens < 1) return;
         AttChunks ch = att_chunks(A, at.s, tokens);
         if (c >= ch.n) return;
+        whole = ch.n == 1 && !A.parts_sh;
         from = ch.from + c * A.chunk; end = from + A.chunk;
     }
     if (at.row0 >= at.rows) return;
-    const AttRow R = att_row(A, at, at.row0 + n, kvh);
+    const AttRow R = att_row(A, shared, at, at.row0 + n, kvh);
     const bool some = R.live && R.lo < R.hi;
     int p0 = max(from, wave_min(some ? R.lo : INT32_MAX) & ~31), p1 = min(end, wave_max(some ? R.hi : 0));
     if (p0 >= p1) p0 = p1 = 0;   // nothing seen (p0 may be close to the largest int: no wave's first run is counted from it)
@@ -873,7 +882,7 @@ __global__ void __launch_bounds__(256, 3) k_attn_few(AttArgs A) {
             odd = __any(o);
         }
         if (odd) {   // infinities and NaN go round the product, to the rows that see their position (the wave's values through its part of LDS)
-            uint32_t *t = (uint32_t *)joint[w];
+            uint32_t *t = (uint32_t *)M.joint[w];
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -919,11 +928,11 @@ __global__ void __launch_bounds__(256, 3) k_attn_few(AttArgs A) {
         step(p, [] {});
     }
     sum = add_quarters(sum);
-    if (g == 0) stat[w][n] = make_float2(mb, sum);
+    if (g == 0) M.stat[w][n] = make_float2(mb, sum);
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
-        for (int e = 0; e < E; e += 4) *(f4 *)&joint[w][n][(4 * g + j) * E + e] = f4{acc[e][j], acc[e + 1][j], acc[e + 2][j], acc[e + 3][j]};
+        for (int e = 0; e < E; e += 4) *(f4 *)&M.joint[w][n][(4 * g + j) * E + e] = f4{acc[e][j], acc[e + 1][j], acc[e + 2][j], acc[e + 3][j]};
     __syncthreads();
     // rows of 16 threads, D / 16 dims each
     const int jr = threadIdx.x >> 4, d = (threadIdx.x & 15) * E, row = at.row0 + jr;
@@ -931,21 +940,21 @@ __global__ void __launch_bounds__(256, 3) k_attn_few(AttArgs A) {
     float2 st[4];
     float mx = -__builtin_inff(), total = 0.0f, o[E] = {};
 #pragma unroll
-    for (int i = 0; i < 4; i++) { st[i] = stat[i][jr]; if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x); }
+    for (int i = 0; i < 4; i++) { st[i] = M.stat[i][jr]; if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x); }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if (st[i].y == 0.0f) continue;
         float e = exp2_(st[i].x - mx);
         total = fmaf(st[i].y, e, total);
 #pragma unroll
-        for (int x = 0; x < E; x++) o[x] = fmaf(e, joint[i][jr][d + x], o[x]);
+        for (int x = 0; x < E; x++) o[x] = fmaf(e, M.joint[i][jr][d + x], o[x]);
     }
     const int j = row / A.group, tok = at.t0 + j, head = kvh * A.group + row - j * A.group;
-    if (A.over_shared) {   // tokens past max_q have no partial results
+    if (shared) {   // tokens past max_q have no partial results
         int s = max(count_le(a.qstart, a.nseq, tok) - 1, 0);
         if (tok - a.qstart[s] >= a.max_q) return;
     }
-    if (A.parts == 1) {
+    if (whole) {
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
         uint32_t *op = (uint32_t *)((uint16_t *)a.out + (int64_t)tok * a.out_token + head * a.out_head + d);
 #pragma unroll
@@ -953,54 +962,108 @@ __global__ void __launch_bounds__(256, 3) k_attn_few(AttArgs A) {
         if (a.lse && d == 0) a.lse[(int64_t)tok * a.heads + head] = total == 0.0f ? -__builtin_inff() : (mx + __builtin_amdgcn_logf(total)) * ATT_LN2;
         return;
     }
-    const int64_t at_row = ((int64_t)(A.part0 + c) * a.ntok + tok) * a.heads + head;
+    const int64_t at_row = ((int64_t)((shared ? 0 : A.parts_sh) + c) * a.ntok + tok) * a.heads + head;
     if (d == 0) A.pm[at_row] = make_float2(mx, total);
     if (total == 0.0f) return;
 #pragma unroll
     for (int x = 0; x < E; x += 4) *(f4 *)(A.po + at_row * D + d + x) = f4{o[x], o[x + 1], o[x + 2], o[x + 3]};
 }
 
-// The partial results of a row: their maxima and sums give each a weight. D / 4 lanes per row and part; ALL: every lane group
-// of the workgroup on one row (many parts), else each on its own.
-template <int T, int D, bool ALL>
-__global__ void __launch_bounds__(256) k_attn_join(AttArgs A) {
-    constexpr int LPR = D / 4, GR = 256 / LPR;
+// One launch for everything, the long work first. With no row tiles of 128 in it a kernel of its own: fewer registers, more waves.
+template <int T, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256, 3) k_attn_few(AttArgs A) {
+    __shared__ AttFewMem<D> M;
+    const unsigned b = blockIdx.x;
+    const bool shared = b < A.n_sh;
+    att_few<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh, M);
+}
+template <int T, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
+    __shared__ union { AttTileMem<D> tile; AttFewMem<D> few; } M;
+    const unsigned b = blockIdx.x;
+    const bool shared = b < A.n_sh;
+    if (shared ? !A.sh_few : b < A.n_sh + A.n_tile) att_tile<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh, M.tile);
+    else att_few<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh - A.n_tile, M.few);
+}
+
+// The partial results of a row: their maxima and sums give each a weight. D / 4 lanes read a part; with all, every such group of the
+// workgroup works on one row (the loads of a row's parts are what there is to wait for), else each has its own.
+// few_only: the rows are those of the sequences of few rows, 16 per key/value head.
+#define ATT_PARTS 1024     // most partial results of a row
+template <int T, int D>
+__global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_only) {
+    constexpr int LPR = D / 4;
     const mmoe_attn_args &a = A.a;
-    __shared__ float red[GR], acc[GR][D];
-    const int gi = threadIdx.x / LPR, x = (threadIdx.x % LPR) * 4, row = ALL ? blockIdx.x : blockIdx.x * GR + gi;
-    const int tok = row / a.heads, head = row - tok * a.heads;
-    if (tok >= att_start(a, a.nseq)) return;
-    const int s = max(count_le(a.qstart, a.nseq, tok) - 1, 0), t0 = att_start(a, s), tokens = att_start(a, s + 1) - t0;
+    __shared__ float red[2][16], wt[ATT_PARTS];
+    __shared__ __attribute__((aligned(16))) float acc[1024 / LPR][D];
+    const int gr = blockDim.x / LPR, gi = threadIdx.x / LPR, x = (threadIdx.x % LPR) * 4, row0 = all ? blockIdx.x : blockIdx.x * gr + gi;
+    int tok, head, s, t0, tokens;
+    if (few_only) {
+        const int per = 16 * A.kv.heads;
+        s = row0 / per;
+        if (s >= a.nseq) return;
+        t0 = att_start(a, s); tokens = att_start(a, s + 1) - t0;
+        const int r = row0 - s * per, j = r / a.heads;
+        if (min(tokens, a.max_q) * A.group > A.few || j >= tokens) return;
+        tok = t0 + j; head = r - j * a.heads;
+    } else {
+        tok = row0 / a.heads; head = row0 - tok * a.heads;
+        if (tok >= att_start(a, a.nseq)) return;
+        s = max(count_le(a.qstart, a.nseq, tok) - 1, 0); t0 = att_start(a, s); tokens = att_start(a, s + 1) - t0;
+    }
     if (tok - t0 >= a.max_q) return;
-    const int parts = A.split_sh + (min(tokens, a.max_q) * A.group <= A.few ? att_chunks(A, s, tokens).n : A.split);
-    const int64_t rows = (int64_t)a.ntok * a.heads;
-    const int first = ALL ? gi : 0, by = ALL ? GR : 1;
+    const int own = min(tokens, a.max_q) * A.group <= A.few ? att_chunks(A, s, tokens).n : A.split, parts = A.parts_sh + own;
+    if (parts == 1) return;   // written by the one that had it
+    const int64_t rows = (int64_t)a.ntok * a.heads, row = (int64_t)tok * a.heads + head;
     float m = -__builtin_inff(), sum = 0.0f;
     f4 o = {0, 0, 0, 0};
-    for (int p = first; p < parts; p += by) { float2 v = A.pm[p * rows + row]; if (v.y != 0.0f) m = fmaxf(m, v.x); }
-    if (ALL) {
-        if (x == 0) red[gi] = m;
-        __syncthreads();
+    if (all) {
+        const int l = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+        float2 v[ATT_PARTS / 256];
 #pragma unroll
-        for (int i = 0; i < GR; i++) m = fmaxf(m, red[i]);
+        for (int i = 0; i < ATT_PARTS / 256; i++) {
+            int p = threadIdx.x + i * blockDim.x;
+            v[i] = p < parts ? A.pm[p * rows + row] : make_float2(0, 0);
+            if (v[i].y != 0.0f) m = fmaxf(m, v[i].x);
+        }
+        for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+        if (l == 0) red[0][w] = m;
         __syncthreads();
-    }
-#pragma unroll 4
-    for (int p = first; p < parts; p += by) {
-        float2 v = A.pm[p * rows + row];
-        f4 y = v.y != 0.0f ? *(const f4 *)(A.po + (p * rows + row) * D + x) : f4{0, 0, 0, 0};
-        float e = v.y != 0.0f ? exp2_(v.x - m) : 0.0f;
-        sum = fmaf(v.y, e, sum);
+        for (int i = 0; i < nw; i++) m = fmaxf(m, red[0][i]);
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] = fmaf(e, y[i], o[i]);
-    }
-    if (ALL) {
+        for (int i = 0; i < ATT_PARTS / 256; i++) {
+            int p = threadIdx.x + i * blockDim.x;
+            float e = v[i].y != 0.0f ? exp2_(v[i].x - m) : 0.0f;
+            if (p < parts) wt[p] = e;
+            sum = fmaf(v[i].y, e, sum);
+        }
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
+        if (l == 0) red[1][w] = sum;
+        __syncthreads();
+        sum = 0.0f;
+        for (int i = 0; i < nw; i++) sum += red[1][i];
+#pragma unroll 8
+        for (int p = gi; p < parts; p += gr) {
+            float e = wt[p];
+            f4 y = e != 0.0f ? *(const f4 *)(A.po + (p * rows + row) * D + x) : f4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = fmaf(e, y[i], o[i]);
+        }
         *(f4 *)&acc[gi][x] = o;
-        if (x == 0) red[gi] = sum;
         __syncthreads();
         if (gi) return;
+        for (int i = 1; i < gr; i++) o += *(const f4 *)&acc[i][x];
+    } else {
+        for (int p = 0; p < parts; p++) { float2 v = A.pm[p * rows + row]; if (v.y != 0.0f) m = fmaxf(m, v.x); }
+#pragma unroll 4
+        for (int p = 0; p < parts; p++) {
+            float2 v = A.pm[p * rows + row];
+            f4 y = v.y != 0.0f ? *(const f4 *)(A.po + (p * rows + row) * D + x) : f4{0, 0, 0, 0};
+            float e = v.y != 0.0f ? exp2_(v.x - m) : 0.0f;
+            sum = fmaf(v.y, e, sum);
 #pragma unroll
-        for (int i = 1; i < GR; i++) { o += *(const f4 *)&acc[i][x]; sum += red[i]; }
+            for (int i = 0; i < 4; i++) o[i] = fmaf(e, y[i], o[i]);
+        }
     }
     const float inv = 1.0f / sum;
     uint2 v = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));

@@ -145,25 +145,21 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     // runs of at least `least` positions until there are about `want` workgroups
     auto runs = [&](int64_t groups, int positions, int want, int least) {
         int64_t n = (want + groups * kv.heads - 1) / (groups * kv.heads), most = (positions + least - 1) / least;
-        return (int)std::max<int64_t>(1, std::min(n, most));
+        return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(n, most), ATT_PARTS / 2));
     };
+    p.few_sh = rows <= 32;
+    if (std::min<int64_t>(a.max_q, a.ntok) * group <= 16 || a.nseq > 1) p.few = 16;
+    // chunks of 512 positions, down to 128 while there are fewer than 512 workgroups, and never more than ATT_PARTS / 2
+    const int64_t few_groups = (a.shared && p.few_sh ? (rows + 15) / 16 * (a.shared / 128) : 0) + (p.few ? a.nseq * (int64_t)(own / 128 + 1) : 0);
     p.chunk = 512;
+    while (p.chunk > 128 && few_groups * kv.heads * 128 / p.chunk < 512) p.chunk >>= 1;
+    p.chunk = std::max(p.chunk, (std::max(own, a.shared) / (ATT_PARTS / 2 - 1) + 128) & ~127);
     if (a.shared) {
-        p.few_sh = rows <= 32;
-        if (p.few_sh) {
-            while (p.chunk > 128 && (rows + 15) / 16 * kv.heads * (a.shared / p.chunk) < 512) p.chunk >>= 1;
-            p.split_sh = (a.shared + p.chunk - 1) / p.chunk;
-        } else {
-            p.tiles_sh = (int)tiles;
-            p.split_sh = runs(tiles, a.shared, 512, 256);
-        }
+        p.tiles_sh = p.few_sh ? (int)((rows + 15) / 16) : (int)tiles;
+        p.split_sh = p.few_sh ? (a.shared + p.chunk - 1) / p.chunk : runs(tiles, a.shared, 512, 256);
     }
-    if (std::min<int64_t>(a.max_q, a.ntok) * group <= 16 || a.nseq > 1) {
-        p.few = 16;
-        if (!p.few_sh) while (p.chunk > 128 && (int64_t)a.nseq * kv.heads * (own / p.chunk) < 512) p.chunk >>= 1;
-        p.chunks = (own + 31 + p.chunk - 1) / p.chunk;
-        p.split = p.chunks;
-    }
+    if (p.few) p.chunks = std::max(1, (own + 31 + p.chunk - 1) / p.chunk);
+    p.split = 1;
     if (std::min<int64_t>(a.max_q, a.ntok) * group > p.few) {
         p.tiles = (int)tiles + a.nseq;
         p.split = runs(tiles, own, 256, 256);
@@ -179,27 +175,24 @@ static int att_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPl
     AttArgs A{};
     A.a = a; A.kv = kv;
     A.sh = log2_block(kv.block_size); A.group = a.heads / kv.heads;
-    A.parts = p.parts; A.chunk = p.chunk; A.chunks = p.chunks; A.few = p.few; A.split = p.split; A.split_sh = p.split_sh;
+    A.n_sh = (unsigned)p.tiles_sh * p.split_sh * kv.heads;
+    A.n_tile = (unsigned)p.tiles * p.split * kv.heads;
+    A.n_few = (unsigned)p.chunks * a.nseq * kv.heads;
+    A.sh_few = p.few_sh; A.few = p.few;
+    A.split_sh = p.split_sh; A.split = p.split; A.chunk = p.chunk; A.chunks = p.chunks;
+    A.parts_sh = p.split_sh;
     A.s1 = CAP ? 2.0f * a.scale / a.cap * ATT_LOG2E : a.scale * ATT_LOG2E;
     A.s2 = a.cap * ATT_LOG2E;
     A.pm = (float2 *)a.ws;
     A.po = (float *)((uint8_t *)a.ws + (size_t)p.parts * a.ntok * a.heads * 8);
-    const unsigned kvh = kv.heads, rows = (unsigned)a.ntok * A.group;
-    if (a.shared) {
-        A.over_shared = 1;
-        A.nsplit = p.split_sh;
-        if (p.few_sh ? run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, dim3(kvh * p.split_sh, (rows + 15) / 16), 256, A)
-                     : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS>, dim3(kvh * p.split_sh * p.tiles_sh), 256, A)) return -1;
-        A.over_shared = 0;
-        A.part0 = p.split_sh;
-    }
-    if (p.chunks && run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, dim3(kvh * p.chunks, a.nseq), 256, A)) return -1;
-    A.nsplit = p.split;
-    if (p.tiles && run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS>, dim3(kvh * p.split * p.tiles), 256, A)) return -1;
+    const dim3 g(A.n_sh + A.n_tile + A.n_few);
+    if (A.n_tile || (A.n_sh && !A.sh_few) ? run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS>, g, 256, A)
+                                          : run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, g, 256, A)) return -1;
     if (p.parts == 1) return 0;
-    constexpr int per = 256 / (D / 4);   // rows of a workgroup where each is a lane group's
-    return p.parts > 8 ? run(MMOE_K_ATT_PAGED, k_attn_join<T, D, true>, dim3((unsigned)a.ntok * a.heads), 256, A)
-                       : run(MMOE_K_ATT_PAGED, k_attn_join<T, D, false>, dim3(((unsigned)a.ntok * a.heads + per - 1) / per), 256, A);
+    const bool few_only = !p.split_sh && p.tiles && p.split == 1, all = p.parts > 8;   // only sequences of few rows have partial results
+    const unsigned rows = few_only ? 16u * kv.heads * a.nseq : (unsigned)a.ntok * a.heads, lpr = D / 4;
+    const unsigned threads = all && p.parts > 64 ? 1024 : 256;
+    return run(MMOE_K_ATT_PAGED, k_attn_join<T, D>, all ? rows : (rows + threads / lpr - 1) / (threads / lpr), threads, A, all, few_only);
 }
 template <int T, int D>
 static int att_pick(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPlan &p) {
