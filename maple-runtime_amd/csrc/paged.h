@@ -70,6 +70,16 @@ __device__ __forceinline__ int count_le(const int *a, int n, int v) {
     return lo;
 }
 
+// the number of i in 0 .. n - 1 for which f holds, by a wave for one f: every load under way at once instead of a search's one by one
+template <typename F> __device__ __forceinline__ int count_wave(int n, F &&f) {
+    int c = 0;
+    for (int i = 0; i < n; i += 64) {
+        int j = i + (threadIdx.x & 63);
+        c += __popcll(__ballot(j < n && f(j)));
+    }
+    return c;
+}
+
 // ------------------------------------------------------------------------------------------------------
 // Block tables and slot maps (mmoe_kv_plan)
 // ------------------------------------------------------------------------------------------------------
@@ -406,11 +416,8 @@ __device__ __forceinline__ bool att_find(const AttArgs &A, bool shared, int bm, 
         o.s = 0; o.t0 = 0; o.row0 = v * bm; o.rows = att_start(a, a.nseq) * A.group;
         return o.row0 < o.rows;
     }
-    int lo = 0, hi = a.nseq;   // the last s whose first tile is <= v
-    while (hi - lo > 1) {
-        int m = (lo + hi) >> 1;
-        if ((int)((int64_t)att_start(a, m) * A.group / bm) + m <= v) lo = m; else hi = m;
-    }
+    // the last s whose first tile is <= v
+    const int lo = max(count_wave(a.nseq, [&](int m) { return (int)((int64_t)att_start(a, m) * A.group / bm) + m <= v; }) - 1, 0);
     o.s = lo; o.t0 = att_start(a, lo);
     o.row0 = (v - (int)((int64_t)o.t0 * A.group / bm) - lo) * bm;
     o.rows = min(att_start(a, lo + 1) - o.t0, a.max_q) * A.group;
@@ -427,26 +434,36 @@ __device__ __forceinline__ AttChunks att_chunks(const AttArgs &A, int s, int tok
     return {from, to > from ? min((to - from + A.chunk - 1) / A.chunk, A.chunks) : 1};
 }
 
-// One query row as a lane sees it
+// One query row as a lane sees it: its token and head, then (with a search for its sequence, if that is not the tile's) its limits
 struct AttRow { int tok, head, pos, lo, hi; bool live; };
-__device__ __forceinline__ AttRow att_row(const AttArgs &A, bool shared, const AttTileAt &at, int r, int kvh) {
-    const mmoe_attn_args &a = A.a;
+__device__ __forceinline__ AttRow att_row(const AttArgs &A, const AttTileAt &at, int r, int kvh) {
     AttRow o;
     o.live = r < at.rows;
     if (!o.live) r = at.rows - 1;
-    int j = r / A.group, s = at.s;
+    int j = r / A.group;
     o.tok = at.t0 + j;
     o.head = kvh * A.group + r - j * A.group;
-    if (shared) s = max(count_le(a.qstart, a.nseq, o.tok) - 1, 0);
-    int len = a.len[s], t0 = a.qstart[s];
-    o.pos = len - (a.qstart[s + 1] - o.tok);
+    return o;
+}
+// starts: room for all of qstart in LDS, every thread of the workgroup here
+__device__ __forceinline__ void att_limits(const AttArgs &A, bool shared, const AttTileAt &at, int *starts, AttRow &o) {
+    const mmoe_attn_args &a = A.a;
+    int s = at.s, t0, t1;
+    if (shared) {
+        for (int i = threadIdx.x; i <= a.nseq; i += blockDim.x) starts[i] = a.qstart[i];
+        __syncthreads();
+        s = max(count_le(starts, a.nseq, o.tok) - 1, 0);
+        t0 = starts[s]; t1 = starts[s + 1];
+        __syncthreads();
+    } else { t0 = a.qstart[s]; t1 = a.qstart[s + 1]; }
+    int len = a.len[s];
+    o.pos = len - (t1 - o.tok);
     if (o.tok - t0 >= a.max_q) o.live = false;
     o.lo = a.lo ? max(a.lo[o.tok], 0) : 0;
     o.hi = a.hi ? a.hi[o.tok] : o.pos + 1;
     if (a.window > 0) o.lo = max(o.lo, o.pos - a.window);
     o.hi = max(min(min(o.hi, len), a.max_len), 0);
     if (shared) o.hi = min(o.hi, a.shared); else o.lo = max(o.lo, a.shared);
-    return o;
 }
 
 // Values of a tile that is not seen whole: are all of them finite? (bits: the type's exponent)
@@ -464,20 +481,35 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
 // pieces whose place in a row is exchanged by the row's number, so that neither the reads of 8 rows at one column nor the transposing
 // reads of 4 rows meet in a bank. P is rounded to the cache's type (half a step relative, as the result itself is), its
 // sum is of the unrounded 32-bit values.
-template <int D> struct AttTileMem {
-    __attribute__((aligned(1024))) uint8_t tiles[2][2 * ATT_BN * D * 2];   // keys, values
-    int range[4][4], flag[2][4];
+template <int D, int NG> struct AttTileMem {
+    union {
+        __attribute__((aligned(1024))) uint8_t tiles[NG][2][2 * ATT_BN * D * 2];   // keys, values
+        int starts[MMOE_KV_MAXSEQ + 1];
+        float other[NG > 1 ? D / 2 + 2 : 1][256];    // another group's results
+    };
+    int range[4][4], flag[NG][2][4];
 };
-template <int T, int D, bool CAP, bool BIAS>
-__device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, const unsigned block, AttTileMem<D> &M) {
+// NG groups of 4 waves share the rows and take the tiles in turn, joined at the end: the second wave per SIMD where there are not
+// two workgroups per CU.
+template <int T, int D, bool CAP, bool BIAS, int NG>
+__device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, const unsigned block, AttTileMem<D, NG> &M) {
     constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // bytes and chunks of a row, rows and instructions of a wave's load
     const mmoe_attn_args &a = A.a;
     const int nsplit = shared ? A.split_sh : A.split;
-    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 31, hh = l >> 5;
+    const int l = threadIdx.x & 63, wg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wg & 3, grp = wg >> 2, n = l & 31, hh = l >> 5;
     const int kvh = block % A.kv.heads, rest = block / A.kv.heads, split = rest % nsplit;
     AttTileAt at;
     if (!att_find(A, shared, 128, (shared ? A.n_sh : A.n_tile) / A.kv.heads / nsplit - 1 - rest / nsplit, at)) return;   // the last tiles see most: first
-    AttRow R = att_row(A, shared, at, at.row0 + w * 32 + n, kvh);
+    AttRow R = att_row(A, at, at.row0 + w * 32 + n, kvh);
+    // queries: operand B, lane (hh, n) holds dims 16 s + 8 hh .. + 8 of row n
+    u4 q[KS];
+    {
+        const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * hh;
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 16 * s);
+    }
+    const float slope = BIAS ? a.slopes[R.head] * ATT_LOG2E : 0.0f;
+    att_limits(A, shared, at, M.starts, R);
     // the wave's and the workgroup's positions
     const bool some = R.live && R.lo < R.hi;
     const int wlo = wave_min(some ? R.lo : INT32_MAX), whi = wave_max(some ? R.hi : 0);
@@ -494,15 +526,6 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         p1 = min(p1, p0 + run);
     }
     p0 = __builtin_amdgcn_readfirstlane(p0); p1 = __builtin_amdgcn_readfirstlane(p1);
-
-    // queries: operand B, lane (hh, n) holds dims 16 s + 8 hh .. + 8 of row n
-    u4 q[KS];
-    {
-        const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * hh;
-#pragma unroll
-        for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 16 * s);
-    }
-    const float slope = BIAS ? a.slopes[R.head] * ATT_LOG2E : 0.0f;
 
     // what the lane loads of a tile: row 16 w + RPI i + l / CH, piece l % CH of LDS
     uint32_t ko[NI], vo[NI];
@@ -665,15 +688,20 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     };
 
     if (p0 < p1) {
-        uint32_t buf = (uint32_t)(uintptr_t)(lb *)M.tiles;
-        ids(p0);
-        fetch(buf, p0);
-        unsigned bad = (unsigned)lost & 15u;
+        uint32_t buf = (uint32_t)(uintptr_t)(lb *)M.tiles[grp];
+        const int step = NG * ATT_BN;
+        int p = p0 + grp * ATT_BN;   // the group's tile; past p1 it only keeps the others company
+        unsigned bad = 0;
+        if (p < p1) {
+            ids(p);
+            fetch(buf, p);
+            bad = (unsigned)lost & 15u;
+        }
 #pragma unroll
         for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));   // the queries are there: nothing in the loop waits for them
-        for (int p = p0, i = 0; p < p1; p += ATT_BN, i ^= 1) {
+        for (int i = 0, left = (p1 - p0 + step - 1) / step; left > 0; left--, p += step, i ^= 1) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the compiler does not know of these loads
-            const bool part = p < glo || p + ATT_BN > ghi || bad;
+            const bool part = p < p1 && (p < glo || p + ATT_BN > ghi || bad);
             if (part) {   // the wave's own 16 rows of values: are they finite?
                 bool o = false;
 #pragma unroll
@@ -683,30 +711,58 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                     for (int y = 0; y < 4; y++) o |= odd16<T>(v[y]) | odd16<T>(v[y] >> 16);
                 }
                 o = __any(o);
-                if (l == 0) M.flag[i][w] = o;
-            }
+                if (l == 0) M.flag[grp][i][w] = o;
+            } else if (NG > 1 && l == 0) M.flag[grp][i][w] = 0;
             __syncthreads();   // the tile has arrived, and every wave is done with the other buffer
-            bool odd = false;
-            if (part) odd = __builtin_amdgcn_readfirstlane(M.flag[i][0] | M.flag[i][1] | M.flag[i][2] | M.flag[i][3]) != 0;
+            bool odd = false, any = false;   // the group's tile, some group's tile
+            if (part || NG > 1) {
+                int f[NG];
+#pragma unroll
+                for (int x = 0; x < NG; x++) f[x] = __builtin_amdgcn_readfirstlane(M.flag[x][i][0] | M.flag[x][i][1] | M.flag[x][i][2] | M.flag[x][i][3]);
+                odd = (NG > 1 && grp ? f[NG - 1] : f[0]) != 0;
+                any = (f[0] | f[NG - 1]) != 0;
+            }
             const uint32_t other = buf ^ (2 * ATT_BN * RB);
             const unsigned now = bad;
-            const bool more = p + ATT_BN < p1, mine = p < whi && p + ATT_BN > wlo;
+            const bool more = p + step < p1, mine = p < p1 && p < whi && p + ATT_BN > wlo;
             if (more) {
-                if (p + ATT_BN - idp == 1024) ids(p + ATT_BN);
-                bad = (unsigned)(lost >> ((p + ATT_BN - idp) >> 4)) & 15u;
+                if (p + step - idp >= 1024) ids(p + step);
+                bad = (unsigned)(lost >> ((p + step - idp) >> 4)) & 15u;
             }
-            if (odd) {
-                set_aside(buf, other);
-                __syncthreads();
-            } else if (more) fetch(other, p + ATT_BN);
+            if (odd) set_aside(buf, other);
+            else if (more) fetch(other, p + step);
+            if (any) __syncthreads();
             if (mine) tile(buf, p, now);
-            if (odd) {
-                if (mine) add_aside(other, p, now);
+            if (any) {
+                if (odd && mine) add_aside(other, p, now);
                 __syncthreads();
-                if (more) fetch(other, p + ATT_BN);
+                if (odd && more) fetch(other, p + step);
             }
             buf = other;
         }
+    }
+    if (NG > 1) {
+        __syncthreads();   // the tiles' room is free
+        const int t = threadIdx.x & 255;
+        if (grp) {
+#pragma unroll
+            for (int i = 0; i < DS; i++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) M.other[16 * i + j][t] = acc[i][j];
+            M.other[D / 2][t] = mb; M.other[D / 2 + 1][t] = sum;
+        }
+        __syncthreads();
+        if (grp) return;
+        // each half-wave's sum is its own positions', the maximum both halves'
+        const float mo = M.other[D / 2][t], so = M.other[D / 2 + 1][t];
+        const bool none = add_halves(so) == 0.0f, mine = add_halves(sum) != 0.0f;
+        const float mm = none ? mb : mine ? fmaxf(mb, mo) : mo, e0 = exp2_(mb - mm), e1 = none ? 0.0f : exp2_(mo - mm);
+        mb = mm;
+        sum = (mine ? sum * e0 : 0.0f) + (none ? 0.0f : so * e1);
+#pragma unroll
+        for (int i = 0; i < DS; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) acc[i][j] = (mine ? acc[i][j] * e0 : 0.0f) + (none ? 0.0f : M.other[16 * i + j][t] * e1);
     }
     sum = add_halves(sum);
     if (!R.live) return;
@@ -735,7 +791,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 }
 
 // Few rows (up to 16 per key/value head: single tokens, a few drafted ones): the cache's bytes are the bound, so a workgroup takes a chunk
-// of positions, its 4 waves every fourth run of 32 each, keys and values straight into registers; a run's keys give their
+// of positions, its waves runs of 32 in turn, keys and values straight into registers; a run's keys give their
 // registers to the next run's as soon as its scores are there, its values after the second product. S^T = K Q^T and O^T = V^T P^T as in k_attn_tile, on 16 x 16 x 32
 // products; V^T is put together from rows by byte permutes (32 per run of 32 positions, hidden behind the loads). The waves join
 // through LDS, the chunks in k_attn_join.
@@ -746,12 +802,15 @@ template <int T> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
 __device__ __forceinline__ float max_quarters(float x) { x = fmaxf(x, __shfl_xor(x, 16, 64)); return fmaxf(x, __shfl_xor(x, 32, 64)); }
 __device__ __forceinline__ float add_quarters(float x) { x += __shfl_xor(x, 16, 64); return x + __shfl_xor(x, 32, 64); }
 
-template <int D> struct AttFewMem {
-    __attribute__((aligned(16))) float joint[4][16][D + 4];
-    float2 stat[4][16];
+template <int D, int NW> struct AttFewMem {
+    union {
+        __attribute__((aligned(16))) float joint[NW][16][D + 4];
+        int starts[MMOE_KV_MAXSEQ + 1];
+    };
+    float2 stat[NW][16];
 };
-template <int T, int D, bool CAP, bool BIAS>
-__device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, const unsigned block, AttFewMem<D> &M) {
+template <int T, int D, bool CAP, bool BIAS, int NW>
+__device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, const unsigned block, AttFewMem<D, NW> &M) {
     constexpr int KS = D / 32, E = D / 16;   // products over the dims, values of a row per lane
     const mmoe_attn_args &a = A.a;
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 15, g = l >> 4;
@@ -773,11 +832,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         from = ch.from + c * A.chunk; end = from + A.chunk;
     }
     if (at.row0 >= at.rows) return;
-    const AttRow R = att_row(A, shared, at, at.row0 + n, kvh);
-    const bool some = R.live && R.lo < R.hi;
-    int p0 = max(from, wave_min(some ? R.lo : INT32_MAX) & ~31), p1 = min(end, wave_max(some ? R.hi : 0));
-    if (p0 >= p1) p0 = p1 = 0;   // nothing seen (p0 may be close to the largest int: no wave's first run is counted from it)
-    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
+    AttRow R = att_row(A, at, at.row0 + n, kvh);
     u4 q[KS];
     {
         const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * g;
@@ -785,6 +840,11 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 32 * s);
     }
     const float slope = BIAS ? a.slopes[R.head] * ATT_LOG2E : 0.0f;
+    att_limits(A, shared, at, M.starts, R);
+    const bool some = R.live && R.lo < R.hi;
+    int p0 = max(from, wave_min(some ? R.lo : INT32_MAX) & ~31), p1 = min(end, wave_max(some ? R.hi : 0));
+    if (p0 >= p1) p0 = p1 = 0;   // nothing seen (p0 may be close to the largest int: no wave's first run is counted from it)
+    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
     const int32_t *table = a.table + (int64_t)at.s * a.width;
     auto ids = [&](int p) { return table[min((p + 16 * (l & 1)) >> A.sh, a.width - 1)]; };   // lane i % 2: positions p + 16 i ..
     // keys: lane (g, n) row n, dims 32 s + 8 g ..; values: rows 4 g + i, dims E n ..
@@ -917,13 +977,13 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     };
     int p = p0 + 32 * w;
     if (p < p1) {
-        int id = ids(p), next = ids(p + 128);
+        int id = ids(p), next = ids(p + 32 * NW);
         load_k(p, id);
         load_v(p, id);
-        for (; p + 128 < p1; p += 128) {
-            step(p, [&] { load_k(p + 128, next); });
-            load_v(p + 128, next);
-            next = ids(p + 256);
+        for (; p + 32 * NW < p1; p += 32 * NW) {
+            step(p, [&] { load_k(p + 32 * NW, next); });
+            load_v(p + 32 * NW, next);
+            next = ids(p + 64 * NW);
         }
         step(p, [] {});
     }
@@ -935,14 +995,15 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         for (int e = 0; e < E; e += 4) *(f4 *)&M.joint[w][n][(4 * g + j) * E + e] = f4{acc[e][j], acc[e + 1][j], acc[e + 2][j], acc[e + 3][j]};
     __syncthreads();
     // rows of 16 threads, D / 16 dims each
+    if (threadIdx.x >= 256) return;
     const int jr = threadIdx.x >> 4, d = (threadIdx.x & 15) * E, row = at.row0 + jr;
     if (row >= at.rows) return;
-    float2 st[4];
+    float2 st[NW];
     float mx = -__builtin_inff(), total = 0.0f, o[E] = {};
 #pragma unroll
-    for (int i = 0; i < 4; i++) { st[i] = M.stat[i][jr]; if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x); }
+    for (int i = 0; i < NW; i++) { st[i] = M.stat[i][jr]; if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x); }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < NW; i++) {
         if (st[i].y == 0.0f) continue;
         float e = exp2_(st[i].x - mx);
         total = fmaf(st[i].y, e, total);
@@ -971,19 +1032,19 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
 
 // One launch for everything, the long work first. With no row tiles of 128 in it a kernel of its own: fewer registers, more waves.
 template <int T, int D, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(256, 3) k_attn_few(AttArgs A) {
-    __shared__ AttFewMem<D> M;
+__global__ void __launch_bounds__(256, 2) k_attn_few(AttArgs A) {
+    __shared__ AttFewMem<D, 4> M;
     const unsigned b = blockIdx.x;
     const bool shared = b < A.n_sh;
-    att_few<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh, M);
+    att_few<T, D, CAP, BIAS, 4>(A, shared, shared ? b : b - A.n_sh, M);
 }
-template <int T, int D, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
-    __shared__ union { AttTileMem<D> tile; AttFewMem<D> few; } M;
+template <int T, int D, bool CAP, bool BIAS, int NG>
+__global__ void __launch_bounds__(256 * NG, 2) k_attn_tile(AttArgs A) {
+    __shared__ union { AttTileMem<D, NG> tile; AttFewMem<D, 4 * NG> few; } M;
     const unsigned b = blockIdx.x;
     const bool shared = b < A.n_sh;
-    if (shared ? !A.sh_few : b < A.n_sh + A.n_tile) att_tile<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh, M.tile);
-    else att_few<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh - A.n_tile, M.few);
+    if (shared ? !A.sh_few : b < A.n_sh + A.n_tile) att_tile<T, D, CAP, BIAS, NG>(A, shared, shared ? b : b - A.n_sh, M.tile);
+    else att_few<T, D, CAP, BIAS, 4 * NG>(A, shared, shared ? b : b - A.n_sh - A.n_tile, M.few);
 }
 
 // The partial results of a row: their maxima and sums give each a weight. D / 4 lanes read a part; with all, every such group of the
@@ -1009,7 +1070,8 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
     } else {
         tok = row0 / a.heads; head = row0 - tok * a.heads;
         if (tok >= att_start(a, a.nseq)) return;
-        s = max(count_le(a.qstart, a.nseq, tok) - 1, 0); t0 = att_start(a, s); tokens = att_start(a, s + 1) - t0;
+        s = max((all ? count_wave(a.nseq, [&](int i) { return a.qstart[i] <= tok; }) : count_le(a.qstart, a.nseq, tok)) - 1, 0);
+        t0 = att_start(a, s); tokens = att_start(a, s + 1) - t0;
     }
     if (tok - t0 >= a.max_q) return;
     const int own = min(tokens, a.max_q) * A.group <= A.few ? att_chunks(A, s, tokens).n : A.split, parts = A.parts_sh + own;

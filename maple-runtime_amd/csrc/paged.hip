@@ -136,7 +136,7 @@ static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
 }
 
 // How a call is divided: row tiles, and runs or chunks of positions where the tiles alone are too few workgroups.
-struct AttPlan { int few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts; size_t bytes; };
+struct AttPlan { int groups, few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts; size_t bytes; };
 static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     AttPlan p = {};
     const int group = a.heads / kv.heads;
@@ -156,7 +156,7 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     p.chunk = std::max(p.chunk, (std::max(own, a.shared) / (ATT_PARTS / 2 - 1) + 128) & ~127);
     if (a.shared) {
         p.tiles_sh = p.few_sh ? (int)((rows + 15) / 16) : (int)tiles;
-        p.split_sh = p.few_sh ? (a.shared + p.chunk - 1) / p.chunk : runs(tiles, a.shared, 512, 256);
+        p.split_sh = p.few_sh ? (a.shared + p.chunk - 1) / p.chunk : runs(tiles, a.shared, 256, 256);
     }
     if (p.few) p.chunks = std::max(1, (own + 31 + p.chunk - 1) / p.chunk);
     p.split = 1;
@@ -164,6 +164,8 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
         p.tiles = (int)tiles + a.nseq;
         p.split = runs(tiles, own, 256, 256);
     }
+    // two groups of waves per row tile while the tiles fill no more than one workgroup per CU
+    p.groups = ((p.few_sh ? 0 : (int64_t)p.tiles_sh * p.split_sh) + (p.tiles ? tiles * p.split : 0)) * kv.heads <= 384 ? 2 : 1;
     p.parts = p.split_sh + std::max(p.split, p.chunks);
     p.bytes = 256;
     if (p.parts > 1) p.bytes += (size_t)p.parts * a.ntok * a.heads * (kv.head_dim * 4 + 8);
@@ -186,8 +188,10 @@ static int att_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPl
     A.pm = (float2 *)a.ws;
     A.po = (float *)((uint8_t *)a.ws + (size_t)p.parts * a.ntok * a.heads * 8);
     const dim3 g(A.n_sh + A.n_tile + A.n_few);
-    if (A.n_tile || (A.n_sh && !A.sh_few) ? run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS>, g, 256, A)
-                                          : run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, g, 256, A)) return -1;
+    const bool has_tiles = A.n_tile || (A.n_sh && !A.sh_few);
+    if (!has_tiles ? run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, g, 256, A)
+        : p.groups == 2 ? run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS, 2>, g, 512, A)
+                        : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS, 1>, g, 256, A)) return -1;
     if (p.parts == 1) return 0;
     const bool few_only = !p.split_sh && p.tiles && p.split == 1, all = p.parts > 8;   // only sequences of few rows have partial results
     const unsigned rows = few_only ? 16u * kv.heads * a.nseq : (unsigned)a.ntok * a.heads, lpr = D / 4;
