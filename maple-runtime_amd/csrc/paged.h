@@ -483,7 +483,7 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
 // sum is of the unrounded 32-bit values.
 template <int D, int NG> struct AttTileMem {
     union {
-        __attribute__((aligned(1024))) uint8_t tiles[NG][2][2 * ATT_BN * D * 2];   // keys, values
+        __attribute__((aligned(1024))) uint8_t tiles[NG][4][ATT_BN * D * 2];   // keys of two tiles, values of two
         int starts[MMOE_KV_MAXSEQ + 1];
         float other[NG > 1 ? D / 2 + 2 : 1][256];    // another group's results
     };
@@ -542,38 +542,38 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 #pragma unroll
     for (int k = 0; k < KS; k++) ka[k] = n * RB + (((2 * k + hh) ^ (n & (CH - 1))) << 4);
 #pragma unroll
-    for (int i = 0; i < DS; i++) va[i] = ATT_BN * RB + vr * RB + ((64 * i + 32 * ((l >> 4) & 1) + 8 * (l & 3)) ^ ((vr & (CH / 2 - 1)) << 5));
+    for (int i = 0; i < DS; i++) va[i] = vr * RB + ((64 * i + 32 * ((l >> 4) & 1) + 8 * (l & 3)) ^ ((vr & (CH / 2 - 1)) << 5));
     // block ids of 64 groups of 16 positions at a time, group l in lane l; a load of their own each tile would have to be waited for
     // with the tile's
     const int32_t *table = a.table + (int64_t)at.s * a.width;
-    int id = 0, idp = 0;      // ids of the positions from idp on
-    uint64_t lost = 0;        // those that are none of the cache's
-    auto ids = [&](int p) {
-        idp = p;
-        id = table[min((p + 16 * l) >> A.sh, a.width - 1)];
-        lost = __ballot((unsigned)id >= (unsigned)A.kv.nblocks);
-    };
-    auto fetch = [&](uint32_t buf, int p) {
+    int id = 0, idp = INT32_MIN / 2;      // ids of the positions from idp on
+    uint64_t lost = 0;                    // those that are none of the cache's
+    auto block_of = [&](int p, unsigned &bad) {   // the wave's block of a tile
+        if (p - idp >= 1024) {
+            idp = p;
+            id = table[min((p + 16 * l) >> A.sh, a.width - 1)];
+            lost = __ballot((unsigned)id >= (unsigned)A.kv.nblocks);
+        }
+        bad = (unsigned)(lost >> ((p - idp) >> 4)) & 15u;
         int blk = __builtin_amdgcn_readlane(id, ((p - idp) >> 4) + w);
-        if ((unsigned)blk >= (unsigned)A.kv.nblocks) blk = 0;
-        const int64_t at0 = (blk * A.kv.block_stride + kvh * A.kv.head_stride + ((p + 16 * w) & (A.kv.block_size - 1)) * A.kv.token_stride) * 2;
-        const uint8_t *kp = (const uint8_t *)A.kv.k + at0, *vp = (const uint8_t *)A.kv.v + at0;
+        return (unsigned)blk < (unsigned)A.kv.nblocks ? blk : 0;
+    };
+    auto fetch = [&](uint32_t buf, const void *base, const uint32_t *off, int p, int blk) {
+        const uint8_t *from = (const uint8_t *)base + (blk * A.kv.block_stride + kvh * A.kv.head_stride + ((p + 16 * w) & (A.kv.block_size - 1)) * A.kv.token_stride) * 2;
 #pragma unroll
-        for (int i = 0; i < NI; i++) load_lds(kp, ko[i], buf + w * 16 * RB + i * 1024);
-#pragma unroll
-        for (int i = 0; i < NI; i++) load_lds(vp, vo[i], buf + ATT_BN * RB + w * 16 * RB + i * 1024);
+        for (int i = 0; i < NI; i++) load_lds(from, off[i], buf + w * 16 * RB + i * 1024);
     };
 
-    f16v acc[DS];
+    f16v acc[DS], sc[2];
 #pragma unroll
     for (int i = 0; i < DS; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
-    float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f;   // mb: m, 0 while that is -inf
+    float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f, mt;   // mb: m, 0 while that is -inf; mt: the last tile's
+    constexpr bool MATH = CAP || BIAS;
+    const float s1 = MATH ? 1.0f : A.s1;
 
-    auto tile = [&](uint32_t buf, int p, unsigned bad) {
-        const lb *kl = (const lb *)(uintptr_t)buf;
-        f16v s[2];
+    auto scores = [&](f16v *s, uint32_t buf) {
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -581,84 +581,82 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) s[u] = mfma32<T>(*(const lu4 *)(kl + ka[k] + 32 * u * RB), q[k], s[u]);
-        // six reads ahead of the products
-        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-#pragma unroll
-        for (int k = 0; k < 2 * KS - 6; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
-        __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
-        // scores in units of log 2
+            for (int u = 0; u < 2; u++) s[u] = mfma32<T>(*(const lu4 *)((const lb *)(uintptr_t)buf + ka[k] + 32 * u * RB), q[k], s[u]);
+    };
+    // scores in units of log 2 (without cap and bias: but for s1) and their maximum
+    auto math = [&](f16v *s, int p) {
         const float dist = BIAS ? (float)(R.pos - p - 4 * hh) : 0.0f;
-        if (CAP || BIAS)
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    float x = s[u][j] * A.s1;
-                    if (CAP) x = fmaf(-2.0f * A.s2, __builtin_amdgcn_rcpf(1.0f + exp2_(x)), A.s2);   // tanh z = 1 - 2 / (1 + exp 2 z)
-                    if (BIAS) x = fmaf(-slope, fabsf(dist - (float)(32 * u + 8 * (j >> 2) + (j & 3))), x);
-                    s[u][j] = x;
-                }
-        const float sc = CAP || BIAS ? 1.0f : A.s1;
-        const bool part = p < inlo || p + ATT_BN > inhi || bad;
-        if (part) {
-            const unsigned from = (unsigned)(R.lo - p - 4 * hh), span = (unsigned)max(R.hi - R.lo, 0);
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    bool see = (unsigned)(32 * u + 8 * (j >> 2) + (j & 3)) - from < span && !((bad >> (2 * u + (j >> 3))) & 1);
-                    s[u][j] = see ? s[u][j] : -__builtin_inff();
-                }
-        }
-        float mt = -__builtin_inff();
+        mt = -__builtin_inff();
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) mt = max_(mt, s[u][j]);
-        mt = max_halves(mt) * sc;
-        // a new maximum only once it is 2^8 past the old: until then weights stay below 2^8, in every type's range
-        if (__any(mt > m + 8.0f)) {
-            float mn = fmaxf(m, mt), bn = mn == -__builtin_inff() ? 0.0f : mn, al = exp2_(m - bn);
-            m = mn; mb = bn; sum *= al;
+            for (int j = 0; j < 16; j++) {
+                const int at = 32 * u + 8 * (j >> 2) + (j & 3);
+                float x = s[u][j];
+                if (MATH) x *= A.s1;
+                if (CAP) x = fmaf(-2.0f * A.s2, __builtin_amdgcn_rcpf(1.0f + exp2_(x)), A.s2);   // tanh z = 1 - 2 / (1 + exp 2 z)
+                if (BIAS) x = fmaf(-slope, fabsf(dist - (float)at), x);
+                s[u][j] = x;
+                mt = max_(mt, x);
+            }
+    };
+    // a tile that is not seen whole
+    auto mask = [&](f16v *s, int p, unsigned bad) {
+        const unsigned from = (unsigned)(R.lo - p - 4 * hh), span = (unsigned)max(R.hi - R.lo, 0);
+        mt = -__builtin_inff();
 #pragma unroll
-            for (int i = 0; i < DS; i++)
+        for (int u = 0; u < 2; u++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) acc[i][j] *= al;
-        }
-        // V^T: lane (hh, n) of operand A holds dim 32 i + n, positions 16 k + 4 hh + {0 .. 3, 8 .. 11}
-        auto value = [&](int i, int k) {
-            uint2 t0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(kl + va[i] + 16 * k * RB)));
-            uint2 t1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(kl + va[i] + (16 * k + 8) * RB)));
-            return u4{t0.x, t0.y, t1.x, t1.y};
-        };
-        u4 f0[DS];   // the first positions' are on their way during the exponentials
+            for (int j = 0; j < 16; j++) {
+                s[u][j] = ((unsigned)(32 * u + 8 * (j >> 2) + (j & 3)) - from < span) & !((bad >> (2 * u + (j >> 3))) & 1) ? s[u][j] : -__builtin_inff();
+                mt = max_(mt, s[u][j]);
+            }
+    };
+    // a new maximum only once it is 2^8 past the old: until then weights stay below 2^8, in every type's range
+    auto rescale = [&] {
+        mt = max_halves(mt) * s1;
+        if (!__any(mt > m + 8.0f)) return;
+        float mn = fmaxf(m, mt), bn = mn == -__builtin_inff() ? 0.0f : mn, al = exp2_(m - bn);
+        m = mn; mb = bn; sum *= al;
 #pragma unroll
-        for (int i = 0; i < DS; i++) f0[i] = value(i, 0);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int i = 0; i < DS; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) acc[i][j] *= al;
+    };
+    // One block of instructions: the weights of the tile in sc and their product with its values, the next tile's scores beside them
+    auto body = [&](uint32_t kbuf, uint32_t vbuf, int p, auto last) {
+        f16v next[2];
+        if (!last.value) scores(next, kbuf);
         u4 pf[4];
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-                float e0 = exp2_(fmaf(s[u][j], sc, -mb)), e1 = exp2_(fmaf(s[u][j + 1], sc, -mb));
+                float e0 = exp2_(fmaf(sc[u][j], s1, -mb)), e1 = exp2_(fmaf(sc[u][j + 1], s1, -mb));
                 sum += e0 + e1;
                 pf[2 * u + (j >> 3)][(j & 7) >> 1] = pack2<T>(e0, e1);
             }
+        // V^T: lane (hh, n) of operand A holds dim 32 i + n, positions 16 k + 4 hh + {0 .. 3, 8 .. 11}
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
-            for (int i = 0; i < DS; i++) acc[i] = mfma32<T>(k ? value(i, k) : f0[i], pf[k], acc[i]);
-#pragma unroll
-        for (int k = 0; k < 3 * DS; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
-        __builtin_amdgcn_sched_group_barrier(0x8, DS, 0);
+            for (int i = 0; i < DS; i++) {
+                const lb *v = (const lb *)(uintptr_t)vbuf + va[i] + 16 * k * RB;
+                uint2 t0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)v));
+                uint2 t1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(v + 8 * RB)));
+                acc[i] = mfma32<T>(u4{t0.x, t0.y, t1.x, t1.y}, pf[k], acc[i]);
+            }
+        if (!last.value) {
+            math(next, p);
+            sc[0] = next[0]; sc[1] = next[1];
+        }
     };
     // A value that is not finite times a weight of 0 is NaN, so in a tile that is not seen whole such values go round the product:
     // the tile's are set aside in the other buffer and zeroed, and afterwards added, as they are, to the rows that see their position.
     auto set_aside = [&](uint32_t buf, uint32_t other) {
 #pragma unroll
         for (int x = 0; x < NI; x++) {
-            const uint32_t o = ATT_BN * RB + w * 16 * RB + x * 1024 + l * 16;
+            const uint32_t o = w * 16 * RB + x * 1024 + l * 16;
             u4 v = *(const lu4 *)((lb *)(uintptr_t)buf + o);
             *(lu4 *)((lb *)(uintptr_t)other + o) = v;
 #pragma unroll
@@ -670,7 +668,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 #pragma unroll 1
         for (int r = 0; r < ATT_BN; r++) {
             const bool see = p + r >= R.lo && p + r < R.hi && !((bad >> (r >> 4)) & 1);
-            uint32_t row = ATT_BN * RB + r * RB + 8 * hh, x = (r & (CH / 2 - 1)) << 5;
+            uint32_t row = r * RB + 8 * hh, x = (r & (CH / 2 - 1)) << 5;
             asm("" : "+v"(row));   // its addresses are not worth a register outside
 #pragma unroll
             for (int i = 0; i < DS; i++)
@@ -688,32 +686,49 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     };
 
     if (p0 < p1) {
-        uint32_t buf = (uint32_t)(uintptr_t)(lb *)M.tiles[grp];
+        typedef std::integral_constant<bool, true> yes;
+        typedef std::integral_constant<bool, false> no;
+        constexpr uint32_t TB = ATT_BN * RB;
+        const uint32_t kb = (uint32_t)(uintptr_t)(lb *)M.tiles[grp], vb = kb + 2 * TB;
         const int step = NG * ATT_BN;
-        int p = p0 + grp * ATT_BN;   // the group's tile; past p1 it only keeps the others company
-        unsigned bad = 0;
+        int p = p0 + grp * ATT_BN, blk = 0;   // the group's tile (past p1 it only keeps the others company), the next one's block
+        unsigned bad = 0, bad1 = 0;           // the tile's lost blocks, the next one's
         if (p < p1) {
-            ids(p);
-            fetch(buf, p);
-            bad = (unsigned)lost & 15u;
+            blk = block_of(p, bad);
+            fetch(kb, A.kv.k, ko, p, blk);
+            fetch(vb, A.kv.v, vo, p, blk);
+            if (p + step < p1) {
+                blk = block_of(p + step, bad1);
+                fetch(kb + TB, A.kv.k, ko, p + step, blk);
+            }
         }
 #pragma unroll
         for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));   // the queries are there: nothing in the loop waits for them
-        for (int i = 0, left = (p1 - p0 + step - 1) / step; left > 0; left--, p += step, i ^= 1) {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the compiler does not know of these loads
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the compiler does not know of the tiles' loads
+        __syncthreads();
+        if (p < p1) {
+            scores(sc, kb);
+            math(sc, p);
+            mask(sc, p, bad);
+            rescale();
+        }
+        auto round = [&](int i, auto last) {
+            // here the next tile's keys and this one's values have arrived
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const uint32_t kbuf = kb + (i ^ 1) * TB, vbuf = vb + i * TB, vother = vb + (i ^ 1) * TB;
             const bool part = p < p1 && (p < glo || p + ATT_BN > ghi || bad);
             if (part) {   // the wave's own 16 rows of values: are they finite?
                 bool o = false;
 #pragma unroll
                 for (int x = 0; x < NI; x++) {
-                    u4 v = *(const lu4 *)((const lb *)(uintptr_t)buf + ATT_BN * RB + w * 16 * RB + x * 1024 + l * 16);
+                    u4 v = *(const lu4 *)((const lb *)(uintptr_t)vbuf + w * 16 * RB + x * 1024 + l * 16);
 #pragma unroll
                     for (int y = 0; y < 4; y++) o |= odd16<T>(v[y]) | odd16<T>(v[y] >> 16);
                 }
                 o = __any(o);
                 if (l == 0) M.flag[grp][i][w] = o;
             } else if (NG > 1 && l == 0) M.flag[grp][i][w] = 0;
-            __syncthreads();   // the tile has arrived, and every wave is done with the other buffer
+            __syncthreads();   // for every wave, and every wave is done with the buffers of the tile before
             bool odd = false, any = false;   // the group's tile, some group's tile
             if (part || NG > 1) {
                 int f[NG];
@@ -722,24 +737,32 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                 odd = (NG > 1 && grp ? f[NG - 1] : f[0]) != 0;
                 any = (f[0] | f[NG - 1]) != 0;
             }
-            const uint32_t other = buf ^ (2 * ATT_BN * RB);
-            const unsigned now = bad;
-            const bool more = p + step < p1, mine = p < p1 && p < whi && p + ATT_BN > wlo;
-            if (more) {
-                if (p + step - idp >= 1024) ids(p + step);
-                bad = (unsigned)(lost >> ((p + step - idp) >> 4)) & 15u;
+            const bool more = p + step < p1;
+            const int blk1 = blk;
+            unsigned bad2 = 0;
+            if (odd) set_aside(vbuf, vother);
+            else if (!last.value && more) fetch(vother, A.kv.v, vo, p + step, blk1);
+            if (!last.value && p + 2 * step < p1) {
+                blk = block_of(p + 2 * step, bad2);
+                fetch(kb + i * TB, A.kv.k, ko, p + 2 * step, blk);
             }
-            if (odd) set_aside(buf, other);
-            else if (more) fetch(other, p + step);
             if (any) __syncthreads();
-            if (mine) tile(buf, p, now);
+            if (!last.value) {   // without a next tile the scores are of what the buffer holds, and masked
+                body(kbuf, vbuf, p + step, last);
+                if (p + step < inlo || p + step + ATT_BN > inhi || bad1 || !more) mask(sc, p + step, more ? bad1 : 15u);
+                rescale();
+            } else if (p < p1) body(0, vbuf, 0, last);
             if (any) {
-                if (odd && mine) add_aside(other, p, now);
+                if (odd) add_aside(vother, p, bad);
                 __syncthreads();
-                if (odd && more) fetch(other, p + step);
+                if (!last.value && odd && more) fetch(vother, A.kv.v, vo, p + step, blk1);
             }
-            buf = other;
-        }
+            bad = bad1; bad1 = bad2;
+            p += step;
+        };
+        int i = 0;
+        for (int left = (p1 - p0 + step - 1) / step; left > 1; left--, i ^= 1) round(i, no());
+        round(i, yes());
     }
     if (NG > 1) {
         __syncthreads();   // the tiles' room is free
