@@ -84,131 +84,144 @@ template <typename F> __device__ __forceinline__ int count_wave(int n, F &&f) {
 // Block tables and slot maps (mmoe_kv_plan)
 // ------------------------------------------------------------------------------------------------------
 // Everything is a prefix sum over the sequences followed by flat loops (blocks given back, blocks taken, tokens) in which an
-// item finds its sequence by a binary search of the sums in LDS, so one long sequence costs no more than many short ones.
-// One workgroup holds it all: sums of up to 4096 sequences are 4 per thread, and the steps depend on each other through
-// the free list. Bound: the latency of its dependent loads and barriers, not bytes (a step of 64 sequences moves 5 KB).
-#define KP_T 1024
+// item finds its sequence by a binary search of the sums in LDS, so one long sequence costs no more than many short ones. One
+// workgroup holds it all, since the steps depend on each other through the free list. Bound: the latency of dependent loads
+// (lengths; a table's begun block and the list's end; the stores), not bytes (a step of 64 sequences moves 5 KB), so what a later step
+// needs is loaded as soon as its address is known and kept in LDS.
+#define KP_LIM (1 << 30)     // sums stop here: above every count there is room for, and two of them still fit
+#define KP_TOP 1024          // list entries and the like kept in LDS
 
-// exclusive prefix sums of a and b over the workgroup; totals in *ta, *tb. 64 bits: lengths come unchecked from the device.
-__device__ __forceinline__ void scan2(long long &a, long long &b, long long *ta, long long *tb, long long (*red)[2]) {
-    int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-    long long x = a, y = b;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        long long u = __shfl_up(x, d, 64), v = __shfl_up(y, d, 64);
-        if (l >= d) { x += u; y += v; }
-    }
+// inclusive sums over a wave, stopping at KP_LIM (a sum that has stopped stays, so the order of the additions does not matter)
+__device__ __forceinline__ unsigned scan_wave(unsigned v) {
+#define KP_STEP(ctrl, rows) v = min(v + (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 15, false), (unsigned)KP_LIM)
+    KP_STEP(0x111, 15); KP_STEP(0x112, 15); KP_STEP(0x114, 15); KP_STEP(0x118, 15);   // from 1, 2, 4, 8 lanes below in the row of 16
+    KP_STEP(0x142, 10); KP_STEP(0x143, 12);                                          // the row before's last, the first half's last
+#undef KP_STEP
+    return v;
+}
+// exclusive sums of a and b over the workgroup, and their totals
+__device__ __forceinline__ void scan2(unsigned &a, unsigned &b, unsigned *ta, unsigned *tb, uint2 *red) {
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+    const unsigned x = scan_wave(a), y = scan_wave(b);
     __syncthreads();   // red may still be read from the scan before
-    if (l == 63) { red[w][0] = x; red[w][1] = y; }
+    if (l == 63) red[w] = make_uint2(x, y);
     __syncthreads();
-    long long p = 0, q = 0, tp = 0, tq = 0;
-#pragma unroll
-    for (int i = 0; i < KP_T / 64; i++) {
-        if (i < w) { p += red[i][0]; q += red[i][1]; }
-        tp += red[i][0]; tq += red[i][1];
+    unsigned p = 0, q = 0, tp = 0, tq = 0;
+    for (int i = 0; i < nw; i++) {
+        uint2 r = red[i];
+        if (i < w) { p = min(p + r.x, (unsigned)KP_LIM); q = min(q + r.y, (unsigned)KP_LIM); }
+        tp = min(tp + r.x, (unsigned)KP_LIM); tq = min(tq + r.y, (unsigned)KP_LIM);
     }
-    a = p + x - a; b = q + y - b;
+    // the lanes below this one (a difference would not undo a sum that has stopped)
+    unsigned ex = (unsigned)__shfl_up((int)x, 1, 64), ey = (unsigned)__shfl_up((int)y, 1, 64);
+    if (l == 0) ex = ey = 0;
+    a = min(p + ex, (unsigned)KP_LIM); b = min(q + ey, (unsigned)KP_LIM);
     *ta = tp; *tb = tq;
 }
 
-// position and slot of token t, whose sequence s the caller found; the tokens behind the last sequence get 0 and -1
-__device__ __forceinline__ void kv_token(const mmoe_kv_plan_args &a, int sh, int t, int total, int s, int begin, int end) {
-    int pos = 0, slot = -1;
-    if (t < total) {
-        pos = a.len[s] - (end - t);
-        int blk = a.table[(int64_t)s * a.width + (pos >> sh)];
-        if ((unsigned)blk < (unsigned)a.nblocks) slot = (blk << sh) + (pos & (a.block_size - 1));
-    }
-    a.pos[t] = pos; a.slot[t] = slot;
-}
-
-__global__ void __launch_bounds__(KP_T) k_kv_plan(mmoe_kv_plan_args a, int sh, int tokens) {
-    __shared__ int start[MMOE_KV_MAXSEQ + 1], first[MMOE_KV_MAXSEQ + 1];
-    __shared__ long long red[KP_T / 64][2];
-    __shared__ int took[2];   // tokens and blocks of the sequences that fit
-    const int tid = threadIdx.x, n = a.nseq, bs1 = a.block_size - 1, keep = a.shared >> sh;
-    const int per = (n + KP_T - 1) / KP_T, s0 = tid * per;
-    const long long room = (long long)a.width << sh;
-    int ctx[MMOE_KV_MAXSEQ / KP_T], add[MMOE_KV_MAXSEQ / KP_T];
-    bool fin[MMOE_KV_MAXSEQ / KP_T];
+// PER: consecutive sequences of a thread
+template <int PER>
+__global__ void __launch_bounds__(1024) k_kv_plan(mmoe_kv_plan_args a, int sh, int tokens) {
+    constexpr int NS = PER * 1024;
+    __shared__ int start[NS + 1], first[NS + 1], lens[NS], tail[NS], top[KP_TOP];
+    __shared__ uint2 red[16];
+    __shared__ unsigned took[2];   // tokens and blocks of the sequences that fit
+    const int tid = threadIdx.x, nt = blockDim.x, n = a.nseq, bs1 = a.block_size - 1, keep = a.shared >> sh, s0 = tid * PER;
+    const int room = a.width << sh;   // < 2^31
+    int ctx[PER], add[PER], old[PER];
+    bool fin[PER];
     if (tid < 2) took[tid] = 0;
     const int nfree0 = min(max(a.nfree[0], 0), a.nblocks);
 #pragma unroll
-    for (int i = 0; i < MMOE_KV_MAXSEQ / KP_T; i++) {
-        bool in = i < per && s0 + i < n;
+    for (int i = 0; i < PER; i++) {
+        const bool in = s0 + i < n;
         ctx[i] = in ? a.ctx[s0 + i] : 0;
         add[i] = in ? a.add[s0 + i] : 0;
         fin[i] = in && a.done && a.done[s0 + i] != 0;
     }
+    // the block that a sequence has begun
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        if (fin[i]) old[i] = max((min(max(ctx[i], 0), room) + bs1 >> sh) - keep, 0);   // to be given back
+        else old[i] = 0;
+        if (fin[i]) ctx[i] = min(ctx[i], a.shared);
+        const int at = ctx[i] >> sh;
+        if (s0 + i < n) tail[s0 + i] = ctx[i] > 0 && (ctx[i] & bs1) && at < a.width ? a.table[(int64_t)(s0 + i) * a.width + at] : -1;
+    }
     // 1. blocks given back, appended to the list
     int nfree = nfree0;
     if (a.done) {
-        long long g = 0, z = 0, tg, tz;
+        unsigned g = 0, z = 0, tg, tz;
 #pragma unroll
-        for (int i = 0; i < MMOE_KV_MAXSEQ / KP_T; i++)
-            if (fin[i]) g += max((int)((min((long long)max(ctx[i], 0), room) + bs1) >> sh) - keep, 0);
+        for (int i = 0; i < PER; i++) g = min(g + old[i], (unsigned)KP_LIM);
         scan2(g, z, &tg, &tz, red);
 #pragma unroll
-        for (int i = 0; i < MMOE_KV_MAXSEQ / KP_T; i++) {
-            if (i < per && s0 + i < n) first[s0 + i] = (int)min(g, (long long)a.nblocks);
-            if (fin[i]) g += max((int)((min((long long)max(ctx[i], 0), room) + bs1) >> sh) - keep, 0);
+        for (int i = 0; i < PER; i++) {
+            if (s0 + i < n) first[s0 + i] = (int)min(g, (unsigned)a.nblocks);
+            g = min(g + old[i], (unsigned)KP_LIM);
         }
         __syncthreads();
-        int back = (int)min(tg, (long long)(a.nblocks - nfree0));
-        for (int j = tid; j < back; j += KP_T) {
+        const int back = (int)min(tg, (unsigned)(a.nblocks - nfree0));
+        for (int j = tid; j < back; j += nt) {
             int s = count_le(first, n, j) - 1;
             a.free_list[nfree0 + j] = a.table[(int64_t)s * a.width + keep + j - first[s]];
         }
         nfree += back;
+        if (back) __syncthreads();
     }
+    for (int j = tid; j < min(nfree, KP_TOP); j += nt) top[j] = a.free_list[nfree - 1 - j];
     // 2. the sequences that fit: a prefix, since both sums only grow (one that cannot fit counts more tokens than there is room for)
-    long long need[MMOE_KV_MAXSEQ / KP_T], tok[MMOE_KV_MAXSEQ / KP_T], cn = 0, ct = 0, tn, tt;
+    unsigned need[PER], tok[PER], cn = 0, ct = 0, tn, tt;
 #pragma unroll
-    for (int i = 0; i < MMOE_KV_MAXSEQ / KP_T; i++) {
-        if (fin[i]) ctx[i] = min(ctx[i], a.shared);
-        long long c = ctx[i], e = c + add[i];
-        bool ok = c >= 0 && add[i] >= 0 && e <= room;
-        need[i] = ok && add[i] > 0 ? ((e + bs1) >> sh) - ((c + bs1) >> sh) : 0;
-        tok[i] = ok ? add[i] : (long long)a.ntok + 1;
-        if (i >= per || s0 + i >= n) tok[i] = 0;
-        cn += need[i]; ct += tok[i];
+    for (int i = 0; i < PER; i++) {
+        const long long e = (long long)ctx[i] + add[i];
+        const bool ok = ctx[i] >= 0 && add[i] >= 0 && e <= room;
+        need[i] = ok && add[i] > 0 ? (unsigned)(((e + bs1) >> sh) - (((long long)ctx[i] + bs1) >> sh)) : 0;
+        tok[i] = ok ? min((unsigned)add[i], (unsigned)KP_LIM) : (unsigned)KP_LIM;
+        if (s0 + i >= n) tok[i] = 0;
+        cn = min(cn + need[i], (unsigned)KP_LIM); ct = min(ct + tok[i], (unsigned)KP_LIM);
     }
     scan2(cn, ct, &tn, &tt, red);
     unsigned fits = 0;
 #pragma unroll
-    for (int i = 0; i < MMOE_KV_MAXSEQ / KP_T; i++) {
-        if (i >= per || s0 + i >= n) continue;
-        first[s0 + i] = (int)min(cn, (long long)a.nblocks + 1);
-        start[s0 + i] = (int)min(ct, (long long)a.ntok);
-        cn += need[i]; ct += tok[i];
-        if (cn <= nfree && ct <= a.ntok) {
+    for (int i = 0; i < PER; i++) {
+        if (s0 + i >= n) continue;
+        first[s0 + i] = (int)cn; start[s0 + i] = (int)ct;
+        cn = min(cn + need[i], (unsigned)KP_LIM); ct = min(ct + tok[i], (unsigned)KP_LIM);
+        if (cn <= (unsigned)nfree && ct <= (unsigned)a.ntok && ct < KP_LIM) {
             fits |= 1u << i;
-            atomicMax(&took[0], (int)ct); atomicMax(&took[1], (int)cn);
+            // sums grow: the last of them is the total (nothing to record where all fit)
+            if (cn != tn || ct != tt || s0 + i == n - 1) { atomicMax(&took[0], ct); atomicMax(&took[1], cn); }
         }
     }
     __syncthreads();
-    const int total = took[0], blocks = took[1];
+    const int total = (int)took[0], blocks = (int)took[1];
 #pragma unroll
-    for (int i = 0; i < MMOE_KV_MAXSEQ / KP_T; i++) {
-        if (i >= per || s0 + i >= n) continue;
-        bool f = (fits >> i) & 1;
-        if (!f) { start[s0 + i] = total; first[s0 + i] = blocks; add[i] = 0; }
+    for (int i = 0; i < PER; i++) {
+        if (s0 + i >= n) continue;
+        if (!((fits >> i) & 1)) { start[s0 + i] = total; first[s0 + i] = blocks; add[i] = 0; }
         a.qstart[s0 + i] = start[s0 + i];
-        a.len[s0 + i] = ctx[i] + add[i];
+        a.len[s0 + i] = lens[s0 + i] = ctx[i] + add[i];
     }
-    if (tid == 0) { start[n] = total; a.qstart[n] = total; a.nfree_out[0] = nfree - blocks; }
-    __syncthreads();   // also: the list's appended entries and len are written
+    if (tid == 0) { start[n] = total; first[n] = blocks; a.qstart[n] = total; a.nfree_out[0] = nfree - blocks; }
+    __syncthreads();
     // 3. new blocks, from the end of the list; then the tokens
-    for (int j = tid; j < blocks; j += KP_T) {
+    for (int j = tid; j < blocks; j += nt) {
         int s = count_le(first, n, j) - 1;
-        int held = (a.len[s] - (start[s + 1] - start[s]) + bs1) >> sh;
-        a.table[(int64_t)s * a.width + held + j - first[s]] = a.free_list[nfree - 1 - j];
+        int held = (lens[s] - (start[s + 1] - start[s]) + bs1) >> sh;
+        a.table[(int64_t)s * a.width + held + j - first[s]] = j < KP_TOP ? top[j] : a.free_list[nfree - 1 - j];
     }
     if (!tokens) return;
-    __syncthreads();
-    for (int t = tid; t < a.ntok; t += KP_T) {
-        int s = max(count_le(start, n, t) - 1, 0);
-        kv_token(a, sh, t, total, s, start[s], start[s + 1]);
+    for (int t = tid; t < a.ntok; t += nt) {
+        int pos = 0, slot = -1;
+        if (t < total) {
+            const int s = count_le(start, n, t) - 1, c = lens[s] - (start[s + 1] - start[s]);
+            pos = c + t - start[s];
+            const int j = (pos >> sh) - ((c + bs1) >> sh) + first[s];   // of the blocks taken; before the sequence's first: the begun one
+            const int blk = j < first[s] ? tail[s] : j < KP_TOP ? top[j] : a.free_list[nfree - 1 - j];
+            if ((unsigned)blk < (unsigned)a.nblocks) slot = (blk << sh) + (pos & bs1);
+        }
+        a.pos[t] = pos; a.slot[t] = slot;
     }
 }
 
@@ -217,10 +230,16 @@ __global__ void __launch_bounds__(256) k_kv_tokens(mmoe_kv_plan_args a, int sh) 
     __shared__ int start[MMOE_KV_MAXSEQ + 1];
     for (int i = threadIdx.x; i <= a.nseq; i += 256) start[i] = a.qstart[i];
     __syncthreads();
-    for (int t = blockIdx.x * 256 + threadIdx.x; t < a.ntok; t += gridDim.x * 256) {
-        int s = max(count_le(start, a.nseq, t) - 1, 0);
-        kv_token(a, sh, t, start[a.nseq], s, start[s], start[s + 1]);
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= a.ntok) return;
+    int pos = 0, slot = -1;
+    if (t < start[a.nseq]) {
+        const int s = count_le(start, a.nseq, t) - 1;
+        pos = a.len[s] - (start[s + 1] - t);
+        const int blk = a.table[(int64_t)s * a.width + (pos >> sh)];
+        if ((unsigned)blk < (unsigned)a.nblocks) slot = (blk << sh) + (pos & (a.block_size - 1));
     }
+    a.pos[t] = pos; a.slot[t] = slot;
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -231,7 +250,7 @@ __global__ void __launch_bounds__(256) k_kv_tokens(mmoe_kv_plan_args a, int sh) 
 #define RP_T 256
 #define RP_HALF 128   // largest rot / 2
 #define RP_TB 8       // most tokens per workgroup
-enum { RP_INTER, RP_SPLIT, RP_ODD };   // pairs (2 i, 2 i + 1); (i, i + rot / 2) with rot / 2 in whole units of 8, or not
+enum { RP_INTER, RP_SPLIT, RP_ODD };   // pairs (2 i, 2 i + 1); (i, i + rot / 2) with rot / 2 in whole units of 8; any rot, any head_dim
 
 __device__ __forceinline__ void rope_angles(const mmoe_rope_args &a, int t0, int nt, float2 *cs) {
     const int half = a.rot >> 1;
@@ -303,8 +322,10 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
                     int d = d0 + i;
                     y[i] = x[i];
                     if (!r.turn || d >= a.rot) continue;
-                    float2 c = cs[t * RP_HALF + (d < half ? d : d - half)];
-                    y[i] = d < half ? fmaf(x[i], c.x, -(head[d + half] * c.y)) : fmaf(x[i], c.x, head[d - half] * c.y);
+                    const bool low = a.interleaved ? !(d & 1) : d < half;   // of its pair
+                    const float2 c = cs[t * RP_HALF + (a.interleaved ? d >> 1 : low ? d : d - half)];
+                    const float z = head[a.interleaved ? d ^ 1 : low ? d + half : d - half];
+                    y[i] = low ? fmaf(x[i], c.x, -(z * c.y)) : fmaf(x[i], c.x, z * c.y);
                 }
                 store8<OUT>(r.out, r.dst + d0, y);
             }
@@ -312,37 +333,49 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
         }
         return;
     }
-    for (int j = threadIdx.x; j < all * dc; j += RP_T) {
-        int hd = j / dc, d0 = (j - hd * dc) * 8, t = hd / nh;
-        RopeHead r = rope_head(a, kv, cached, sh, t0 + t, hd - t * nh);
-        if (!r.live) continue;
-        const float2 *w = cs + t * RP_HALF;
-        float x[8], y[8];
-        if (!r.turn || d0 >= a.rot) {
-            load8<IN>(x, r.in, r.src + d0);
-            store8<OUT>(r.out, r.dst + d0, x);
-        } else if (LAY == RP_INTER) {
-            load8<IN>(x, r.in, r.src + d0);
+    // A head is dc lanes of one wave (dc a power of two), a unit of 8 values each; four heads' loads under way per lane. With split pairs a
+    // lane loads its partner's unit too (the same lines again): in place, too, a head is read whole before any of it is written.
+    const int sd = 31 - __builtin_clz(dc), d0 = (threadIdx.x & (dc - 1)) * 8, hpr = RP_T >> sd;
+    int hd = threadIdx.x >> sd, t = 0;
+    for (int left = (all - hd + hpr - 1) / hpr; left > 0; left -= 4) {
+        RopeHead r[4];
+        float x[4][8], z[4][8];
+        const float2 *w[4];
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) {
-                bool in = d0 + i < a.rot;
-                float2 c = in ? w[(d0 + i) >> 1] : make_float2(1.0f, 0.0f);
-                y[i] = in ? fmaf(x[i], c.x, -(x[i + 1] * c.y)) : x[i];
-                y[i + 1] = in ? fmaf(x[i + 1], c.x, x[i] * c.y) : x[i + 1];
-            }
-            store8<OUT>(r.out, r.dst + d0, y);
-        } else if (d0 < half) {   // the first half's unit takes its partner along: in place, none may read what another has written
-            float z[8];
-            load8<IN>(x, r.in, r.src + d0);
-            load8<IN>(z, r.in, r.src + d0 + half);
+        for (int k = 0; k < 4; k++) {
+            r[k].live = false;
+            if (k >= left) continue;
+            while (hd >= nh) { hd -= nh; t++; }
+            r[k] = rope_head(a, kv, cached, sh, t0 + t, hd);
+            w[k] = cs + t * RP_HALF;
+            hd += hpr;
+            if (!r[k].live) continue;
+            load8<IN>(x[k], r[k].in, r[k].src + d0);
+            if (LAY == RP_SPLIT && r[k].turn && d0 < a.rot) load8<IN>(z[k], r[k].in, r[k].src + (d0 < half ? d0 + half : d0 - half));
+        }
 #pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float2 c = w[d0 + i];
-                y[i] = fmaf(x[i], c.x, -(z[i] * c.y));
-                z[i] = fmaf(z[i], c.x, x[i] * c.y);
-            }
-            store8<OUT>(r.out, r.dst + d0, y);
-            store8<OUT>(r.out, r.dst + d0 + half, z);
+        for (int k = 0; k < 4; k++) {
+            if (!r[k].live) continue;
+            if (r[k].turn && d0 < a.rot) {
+                float y[8];
+                if (LAY == RP_INTER) {
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const bool in = d0 + i < a.rot;
+                        const float2 c = in ? w[k][(d0 + i) >> 1] : make_float2(1.0f, 0.0f);
+                        y[i] = in ? fmaf(x[k][i], c.x, -(x[k][i + 1] * c.y)) : x[k][i];
+                        y[i + 1] = in ? fmaf(x[k][i + 1], c.x, x[k][i] * c.y) : x[k][i + 1];
+                    }
+                } else {
+                    const float sign = d0 < half ? -1.0f : 1.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float2 c = w[k][(d0 < half ? d0 : d0 - half) + i];
+                        y[i] = fmaf(x[k][i], c.x, sign * (z[k][i] * c.y));
+                    }
+                }
+                store8<OUT>(r[k].out, r[k].dst + d0, y);
+            } else store8<OUT>(r[k].out, r[k].dst + d0, x[k]);
         }
     }
 }
@@ -353,7 +386,8 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
 // Every kernel here keeps a softmax's running maximum and sum and one pass over the positions. A query row is a (token, query
 // head) pair; the rows that read one key/value head, token by token and its group of query heads within, share its keys. The
 // rows' visible runs [lo, hi) are all there is to masks: a tile that every live row sees whole needs none.
-#define ATT_BN 64          // positions per tile
+#define ATT_BM 128         // rows and positions of a tile
+#define ATT_BN 64
 #define ATT_LOG2E 1.44269504088896340736f
 #define ATT_LN2 0.69314718055994530942f
 
@@ -389,10 +423,20 @@ template <int T> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // the larger of two numbers, without fmaxf's quieting of each (a NaN shows in the weights, whatever the maximum then is)
 __device__ __forceinline__ float max_(float x, float y) { return __builtin_amdgcn_fmed3f(x, y, __builtin_inff()); }
-// 16 bytes per lane from base + off to LDS at to + 16 * lane. Asm, so that the compiler does not wait for it before every later LDS
-// read; nothing is written to a register. The waits are the caller's.
-__device__ __forceinline__ void load_lds(const uint8_t *base, uint32_t off, uint32_t to) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(to)) : "memory", "m0");
+// N pieces of 16 bytes per lane from base + off[i] + 1024 i to LDS at to + 1024 i + 16 * lane (the offset of the instruction counts on both
+// sides). Asm, so that the compiler does not wait for them before every later LDS read; nothing is written to a register. The
+// waits are the caller's.
+template <int N> __device__ __forceinline__ void load_lds(const uint8_t *base, const uint32_t *off, uint32_t to) {
+    static_assert(N == 1 || N == 2 || N == 4, "loads");
+    to = __builtin_amdgcn_readfirstlane(to);
+    if (N == 1) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[0]), "s"(base), "s"(to) : "memory", "m0");
+    if (N == 2)
+        asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024" ::"v"(off[0]), "v"(off[1]), "s"(base), "s"(to)
+                     : "memory", "m0");
+    if (N == 4)
+        asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:1024\n\t"
+                     "global_load_lds_dwordx4 %2, %4 offset:2048\n\tglobal_load_lds_dwordx4 %3, %4 offset:3072" ::"v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(to)
+                     : "memory", "m0");
 }
 // what two half-waves hold of one column
 __device__ __forceinline__ float max_halves(float x) {
@@ -403,8 +447,18 @@ __device__ __forceinline__ float add_halves(float x) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-__device__ __forceinline__ int wave_min(int v) { for (int d = 1; d < 64; d <<= 1) v = min(v, __shfl_xor(v, d, 64)); return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ int wave_max(int v) { for (int d = 1; d < 64; d <<= 1) v = max(v, __shfl_xor(v, d, 64)); return __builtin_amdgcn_readfirstlane(v); }
+template <typename F> __device__ __forceinline__ int wave_reduce(int v, F &&f) {   // in registers: an exchange through LDS costs 100 cycles a step
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0xb1, 15, 15, false));    // lane ^ 1
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x4e, 15, 15, false));    // lane ^ 2
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 15, 15, false));   // mirrored in 8
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 15, 15, false));   // mirrored in 16
+    auto a = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+    v = f((int)a[0], (int)a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+    return __builtin_amdgcn_readfirstlane(f((int)b[0], (int)b[1]));
+}
+__device__ __forceinline__ int wave_min(int v) { return wave_reduce(v, [](int x, int y) { return min(x, y); }); }
+__device__ __forceinline__ int wave_max(int v) { return wave_reduce(v, [](int x, int y) { return max(x, y); }); }
 
 // The sequence and row tile of virtual tile v, with tiles of bm rows: sequence s has the tiles from floor(rows before it / bm) + s
 // on; no two sequences' tiles meet, and some virtual tiles are nobody's. No sums over the sequences are needed.
@@ -417,7 +471,7 @@ __device__ __forceinline__ bool att_find(const AttArgs &A, bool shared, int bm, 
         return o.row0 < o.rows;
     }
     // the last s whose first tile is <= v
-    const int lo = max(count_wave(a.nseq, [&](int m) { return (int)((int64_t)att_start(a, m) * A.group / bm) + m <= v; }) - 1, 0);
+    const int lo = a.nseq == 1 ? 0 : max(count_wave(a.nseq, [&](int m) { return (int)((int64_t)att_start(a, m) * A.group / bm) + m <= v; }) - 1, 0);
     o.s = lo; o.t0 = att_start(a, lo);
     o.row0 = (v - (int)((int64_t)o.t0 * A.group / bm) - lo) * bm;
     o.rows = min(att_start(a, lo + 1) - o.t0, a.max_q) * A.group;
@@ -474,32 +528,29 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
     return v;
 }
 
-// Row tiles of 128 in a workgroup of 4 waves, 32 rows each, over tiles of 64 positions that all waves share through LDS.
+// Row tiles of 4 waves, 32 rows each, over tiles of 64 positions that all waves share through LDS.
 // S^T = K Q^T, so a lane holds one row's scores (half of the positions, the other half in the lane 32 away): the softmax needs
 // one exchange per tile, and P^T, packed to 16 bits, is the second product's operand as it lies. O^T = V^T P^T takes its V^T from
 // rows of V through the transposing LDS reads. A tile's keys and values go from the cache straight to LDS, one tile ahead, in 16-byte
 // pieces whose place in a row is exchanged by the row's number, so that neither the reads of 8 rows at one column nor the transposing
 // reads of 4 rows meet in a bank. P is rounded to the cache's type (half a step relative, as the result itself is), its
 // sum is of the unrounded 32-bit values.
-template <int D, int NG> struct AttTileMem {
+template <int D> struct AttTileMem {
     union {
-        __attribute__((aligned(1024))) uint8_t tiles[NG][4][ATT_BN * D * 2];   // keys of two tiles, values of two
+        __attribute__((aligned(1024))) uint8_t tiles[4][ATT_BN * D * 2];   // keys of two tiles, values of two
         int starts[MMOE_KV_MAXSEQ + 1];
-        float other[NG > 1 ? D / 2 + 2 : 1][256];    // another group's results
     };
-    int range[4][4], flag[NG][2][4];
+    int range[4][4], flag[2][4];
 };
-// NG groups of 4 waves share the rows and take the tiles in turn, joined at the end: the second wave per SIMD where there are not
-// two workgroups per CU.
-template <int T, int D, bool CAP, bool BIAS, int NG>
-__device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, const unsigned block, AttTileMem<D, NG> &M) {
-    constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // bytes and chunks of a row, rows and instructions of a wave's load
+template <int T, int D, bool CAP, bool BIAS>
+__device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, const unsigned block, AttTileMem<D> &M) {
+    constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // a row's bytes and chunks; rows of a load, a wave's loads
     const mmoe_attn_args &a = A.a;
     const int nsplit = shared ? A.split_sh : A.split;
-    const int l = threadIdx.x & 63, wg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wg & 3, grp = wg >> 2, n = l & 31, hh = l >> 5;
+    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 31, hh = l >> 5;
     const int kvh = block % A.kv.heads, rest = block / A.kv.heads, split = rest % nsplit;
     AttTileAt at;
-    if (!att_find(A, shared, 128, (shared ? A.n_sh : A.n_tile) / A.kv.heads / nsplit - 1 - rest / nsplit, at)) return;   // the last tiles see most: first
+    if (!att_find(A, shared, ATT_BM, (shared ? A.n_sh : A.n_tile) / A.kv.heads / nsplit - 1 - rest / nsplit, at)) return;   // the last tiles see most: first
     AttRow R = att_row(A, at, at.row0 + w * 32 + n, kvh);
     // queries: operand B, lane (hh, n) holds dims 16 s + 8 hh .. + 8 of row n
     u4 q[KS];
@@ -516,10 +567,14 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
     if (l == 0) { M.range[0][w] = wlo; M.range[1][w] = whi; M.range[2][w] = inlo; M.range[3][w] = inhi; }
     __syncthreads();
-    int p0 = min(min(M.range[0][0], M.range[0][1]), min(M.range[0][2], M.range[0][3])) & ~(ATT_BN - 1);
-    int p1 = max(max(M.range[1][0], M.range[1][1]), max(M.range[1][2], M.range[1][3]));
-    const int glo = __builtin_amdgcn_readfirstlane(max(max(M.range[2][0], M.range[2][1]), max(M.range[2][2], M.range[2][3])));
-    const int ghi = __builtin_amdgcn_readfirstlane(min(min(M.range[3][0], M.range[3][1]), min(M.range[3][2], M.range[3][3])));
+    int p0 = INT32_MAX, p1 = 0, glo = 0, ghi = INT32_MAX;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        p0 = min(p0, M.range[0][i]); p1 = max(p1, M.range[1][i]);
+        glo = max(glo, M.range[2][i]); ghi = min(ghi, M.range[3][i]);
+    }
+    p0 &= ~(ATT_BN - 1);
+    glo = __builtin_amdgcn_readfirstlane(glo); ghi = __builtin_amdgcn_readfirstlane(ghi);
     if (nsplit > 1 && p0 < p1) {
         int run = ((p1 - p0 + ATT_BN - 1) / ATT_BN + nsplit - 1) / nsplit * ATT_BN;
         p0 += split * run;
@@ -527,13 +582,14 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     }
     p0 = __builtin_amdgcn_readfirstlane(p0); p1 = __builtin_amdgcn_readfirstlane(p1);
 
-    // what the lane loads of a tile: row 16 w + RPI i + l / CH, piece l % CH of LDS
+    // What the lane loads of a tile: row RPI i + l / CH of the wave's 16, piece l % CH of LDS, less the instruction's own offset (rows are at
+    // least head_dim values apart, so it stays positive).
     uint32_t ko[NI], vo[NI];
 #pragma unroll
     for (int i = 0; i < NI; i++) {
         int r = RPI * i + l / CH, c = l % CH;
-        ko[i] = (uint32_t)(r * A.kv.token_stride + (c ^ (r & (CH - 1))) * 8) * 2;
-        vo[i] = (uint32_t)(r * A.kv.token_stride + (c ^ ((r & (CH / 2 - 1)) << 1)) * 8) * 2;
+        ko[i] = (uint32_t)(r * A.kv.token_stride + (c ^ (r & (CH - 1))) * 8) * 2 - 1024 * i;
+        vo[i] = (uint32_t)(r * A.kv.token_stride + (c ^ ((r & (CH / 2 - 1)) << 1)) * 8) * 2 - 1024 * i;
     }
     // where it reads them back: K row n (and n + 32), pieces 2 k + hh; V rows vr (and on by eights), dims 32 i + 16 (l / 16 % 2) + 4 (l % 4) ..
     // (the number that exchanges a row's pieces is the same for rows 32 (K) and 8 (V) apart: what is added are constants)
@@ -560,8 +616,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     };
     auto fetch = [&](uint32_t buf, const void *base, const uint32_t *off, int p, int blk) {
         const uint8_t *from = (const uint8_t *)base + (blk * A.kv.block_stride + kvh * A.kv.head_stride + ((p + 16 * w) & (A.kv.block_size - 1)) * A.kv.token_stride) * 2;
-#pragma unroll
-        for (int i = 0; i < NI; i++) load_lds(from, off[i], buf + w * 16 * RB + i * 1024);
+        load_lds<NI>(from, off, buf + w * 16 * RB);
     };
 
     f16v acc[DS], sc[2];
@@ -582,11 +637,16 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         for (int k = 0; k < KS; k++)
 #pragma unroll
             for (int u = 0; u < 2; u++) s[u] = mfma32<T>(*(const lu4 *)((const lb *)(uintptr_t)buf + ka[k] + 32 * u * RB), q[k], s[u]);
+        // six reads ahead of the products
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int k = 0; k < 2 * KS - 6; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
+        __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
     };
     // scores in units of log 2 (without cap and bias: but for s1) and their maximum
     auto math = [&](f16v *s, int p) {
         const float dist = BIAS ? (float)(R.pos - p - 4 * hh) : 0.0f;
-        mt = -__builtin_inff();
+        float top[4];   // no chain of 32
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -597,20 +657,22 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                 if (CAP) x = fmaf(-2.0f * A.s2, __builtin_amdgcn_rcpf(1.0f + exp2_(x)), A.s2);   // tanh z = 1 - 2 / (1 + exp 2 z)
                 if (BIAS) x = fmaf(-slope, fabsf(dist - (float)at), x);
                 s[u][j] = x;
-                mt = max_(mt, x);
+                top[j & 3] = u || j > 3 ? max_(top[j & 3], x) : x;
             }
+        mt = max_(max_(top[0], top[1]), max_(top[2], top[3]));
     };
     // a tile that is not seen whole
     auto mask = [&](f16v *s, int p, unsigned bad) {
         const unsigned from = (unsigned)(R.lo - p - 4 * hh), span = (unsigned)max(R.hi - R.lo, 0);
-        mt = -__builtin_inff();
+        float top[4];
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 s[u][j] = ((unsigned)(32 * u + 8 * (j >> 2) + (j & 3)) - from < span) & !((bad >> (2 * u + (j >> 3))) & 1) ? s[u][j] : -__builtin_inff();
-                mt = max_(mt, s[u][j]);
+                top[j & 3] = u || j > 3 ? max_(top[j & 3], s[u][j]) : s[u][j];
             }
+        mt = max_(max_(top[0], top[1]), max_(top[2], top[3]));
     };
     // a new maximum only once it is 2^8 past the old: until then weights stay below 2^8, in every type's range
     auto rescale = [&] {
@@ -623,10 +685,18 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 #pragma unroll
             for (int j = 0; j < 16; j++) acc[i][j] *= al;
     };
-    // One block of instructions: the weights of the tile in sc and their product with its values, the next tile's scores beside them
-    auto body = [&](uint32_t kbuf, uint32_t vbuf, int p, auto last) {
-        f16v next[2];
-        if (!last.value) scores(next, kbuf);
+    auto product = [&](uint32_t vbuf) {
+        // V^T: lane (hh, n) of operand A holds dim 32 i + n, positions 16 k + 4 hh + {0 .. 3, 8 .. 11}
+        auto value = [&](int i, int k) {
+            const lb *v = (const lb *)(uintptr_t)vbuf + va[i] + 16 * k * RB;
+            uint2 t0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)v));
+            uint2 t1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(v + 8 * RB)));
+            return u4{t0.x, t0.y, t1.x, t1.y};
+        };
+        u4 f0[DS];   // the first positions' are on their way during the exponentials
+#pragma unroll
+        for (int i = 0; i < DS; i++) f0[i] = value(i, 0);
+        __builtin_amdgcn_sched_barrier(0);
         u4 pf[4];
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -636,20 +706,13 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                 sum += e0 + e1;
                 pf[2 * u + (j >> 3)][(j & 7) >> 1] = pack2<T>(e0, e1);
             }
-        // V^T: lane (hh, n) of operand A holds dim 32 i + n, positions 16 k + 4 hh + {0 .. 3, 8 .. 11}
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
-            for (int i = 0; i < DS; i++) {
-                const lb *v = (const lb *)(uintptr_t)vbuf + va[i] + 16 * k * RB;
-                uint2 t0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)v));
-                uint2 t1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(v + 8 * RB)));
-                acc[i] = mfma32<T>(u4{t0.x, t0.y, t1.x, t1.y}, pf[k], acc[i]);
-            }
-        if (!last.value) {
-            math(next, p);
-            sc[0] = next[0]; sc[1] = next[1];
-        }
+            for (int i = 0; i < DS; i++) acc[i] = mfma32<T>(k ? value(i, k) : f0[i], pf[k], acc[i]);
+#pragma unroll
+        for (int k = 0; k < 3 * DS; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
+        __builtin_amdgcn_sched_group_barrier(0x8, DS, 0);
     };
     // A value that is not finite times a weight of 0 is NaN, so in a tile that is not seen whole such values go round the product:
     // the tile's are set aside in the other buffer and zeroed, and afterwards added, as they are, to the rows that see their position.
@@ -686,37 +749,18 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     };
 
     if (p0 < p1) {
-        typedef std::integral_constant<bool, true> yes;
-        typedef std::integral_constant<bool, false> no;
         constexpr uint32_t TB = ATT_BN * RB;
-        const uint32_t kb = (uint32_t)(uintptr_t)(lb *)M.tiles[grp], vb = kb + 2 * TB;
-        const int step = NG * ATT_BN;
-        int p = p0 + grp * ATT_BN, blk = 0;   // the group's tile (past p1 it only keeps the others company), the next one's block
-        unsigned bad = 0, bad1 = 0;           // the tile's lost blocks, the next one's
-        if (p < p1) {
-            blk = block_of(p, bad);
-            fetch(kb, A.kv.k, ko, p, blk);
-            fetch(vb, A.kv.v, vo, p, blk);
-            if (p + step < p1) {
-                blk = block_of(p + step, bad1);
-                fetch(kb + TB, A.kv.k, ko, p + step, blk);
-            }
-        }
+        const uint32_t kb = (uint32_t)(uintptr_t)(lb *)M.tiles, vb = kb + 2 * TB;
+        unsigned bad, next = 0;   // the tile's lost blocks, the next one's
+        int blk = block_of(p0, bad);
+        fetch(kb, A.kv.k, ko, p0, blk);
+        fetch(vb, A.kv.v, vo, p0, blk);
 #pragma unroll
         for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));   // the queries are there: nothing in the loop waits for them
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the compiler does not know of the tiles' loads
-        __syncthreads();
-        if (p < p1) {
-            scores(sc, kb);
-            math(sc, p);
-            mask(sc, p, bad);
-            rescale();
-        }
-        auto round = [&](int i, auto last) {
-            // here the next tile's keys and this one's values have arrived
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            const uint32_t kbuf = kb + (i ^ 1) * TB, vbuf = vb + i * TB, vother = vb + (i ^ 1) * TB;
-            const bool part = p < p1 && (p < glo || p + ATT_BN > ghi || bad);
+        for (int p = p0, i = 0; p < p1; p += ATT_BN, i ^= 1, bad = next) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the compiler does not know of these loads
+            const uint32_t kbuf = kb + i * TB, kother = kb + (i ^ 1) * TB, vbuf = vb + i * TB, vother = vb + (i ^ 1) * TB;
+            const bool part = p < glo || p + ATT_BN > ghi || bad, more = p + ATT_BN < p1;
             if (part) {   // the wave's own 16 rows of values: are they finite?
                 bool o = false;
 #pragma unroll
@@ -726,66 +770,34 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                     for (int y = 0; y < 4; y++) o |= odd16<T>(v[y]) | odd16<T>(v[y] >> 16);
                 }
                 o = __any(o);
-                if (l == 0) M.flag[grp][i][w] = o;
-            } else if (NG > 1 && l == 0) M.flag[grp][i][w] = 0;
-            __syncthreads();   // for every wave, and every wave is done with the buffers of the tile before
-            bool odd = false, any = false;   // the group's tile, some group's tile
-            if (part || NG > 1) {
-                int f[NG];
-#pragma unroll
-                for (int x = 0; x < NG; x++) f[x] = __builtin_amdgcn_readfirstlane(M.flag[x][i][0] | M.flag[x][i][1] | M.flag[x][i][2] | M.flag[x][i][3]);
-                odd = (NG > 1 && grp ? f[NG - 1] : f[0]) != 0;
-                any = (f[0] | f[NG - 1]) != 0;
+                if (l == 0) M.flag[i][w] = o;
             }
-            const bool more = p + step < p1;
-            const int blk1 = blk;
-            unsigned bad2 = 0;
-            if (odd) set_aside(vbuf, vother);
-            else if (!last.value && more) fetch(vother, A.kv.v, vo, p + step, blk1);
-            if (!last.value && p + 2 * step < p1) {
-                blk = block_of(p + 2 * step, bad2);
-                fetch(kb + i * TB, A.kv.k, ko, p + 2 * step, blk);
+            __syncthreads();   // the tile has arrived, and every wave is done with the other buffers
+            bool odd = false;
+            if (part) odd = __builtin_amdgcn_readfirstlane(M.flag[i][0] | M.flag[i][1] | M.flag[i][2] | M.flag[i][3]) != 0;
+            if (more) {
+                blk = block_of(p + ATT_BN, next);
+                fetch(kother, A.kv.k, ko, p + ATT_BN, blk);
+                if (!odd) fetch(vother, A.kv.v, vo, p + ATT_BN, blk);
             }
-            if (any) __syncthreads();
-            if (!last.value) {   // without a next tile the scores are of what the buffer holds, and masked
-                body(kbuf, vbuf, p + step, last);
-                if (p + step < inlo || p + step + ATT_BN > inhi || bad1 || !more) mask(sc, p + step, more ? bad1 : 15u);
-                rescale();
-            } else if (p < p1) body(0, vbuf, 0, last);
-            if (any) {
-                if (odd) add_aside(vother, p, bad);
+            if (odd) {
+                set_aside(vbuf, vother);
                 __syncthreads();
-                if (!last.value && odd && more) fetch(vother, A.kv.v, vo, p + step, blk1);
             }
-            bad = bad1; bad1 = bad2;
-            p += step;
-        };
-        int i = 0;
-        for (int left = (p1 - p0 + step - 1) / step; left > 1; left--, i ^= 1) round(i, no());
-        round(i, yes());
-    }
-    if (NG > 1) {
-        __syncthreads();   // the tiles' room is free
-        const int t = threadIdx.x & 255;
-        if (grp) {
-#pragma unroll
-            for (int i = 0; i < DS; i++)
-#pragma unroll
-                for (int j = 0; j < 16; j++) M.other[16 * i + j][t] = acc[i][j];
-            M.other[D / 2][t] = mb; M.other[D / 2 + 1][t] = sum;
+            const bool mine = p < whi && p + ATT_BN > wlo;
+            if (mine) {
+                scores(sc, kbuf);
+                math(sc, p);
+                if (p < inlo || p + ATT_BN > inhi || bad) mask(sc, p, bad);
+                rescale();
+                product(vbuf);
+            }
+            if (odd) {
+                if (mine) add_aside(vother, p, bad);
+                __syncthreads();
+                if (more) fetch(vother, A.kv.v, vo, p + ATT_BN, blk);
+            }
         }
-        __syncthreads();
-        if (grp) return;
-        // each half-wave's sum is its own positions', the maximum both halves'
-        const float mo = M.other[D / 2][t], so = M.other[D / 2 + 1][t];
-        const bool none = add_halves(so) == 0.0f, mine = add_halves(sum) != 0.0f;
-        const float mm = none ? mb : mine ? fmaxf(mb, mo) : mo, e0 = exp2_(mb - mm), e1 = none ? 0.0f : exp2_(mo - mm);
-        mb = mm;
-        sum = (mine ? sum * e0 : 0.0f) + (none ? 0.0f : so * e1);
-#pragma unroll
-        for (int i = 0; i < DS; i++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) acc[i][j] = (mine ? acc[i][j] * e0 : 0.0f) + (none ? 0.0f : M.other[16 * i + j][t] * e1);
     }
     sum = add_halves(sum);
     if (!R.live) return;
@@ -825,15 +837,15 @@ template <int T> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
 __device__ __forceinline__ float max_quarters(float x) { x = fmaxf(x, __shfl_xor(x, 16, 64)); return fmaxf(x, __shfl_xor(x, 32, 64)); }
 __device__ __forceinline__ float add_quarters(float x) { x += __shfl_xor(x, 16, 64); return x + __shfl_xor(x, 32, 64); }
 
-template <int D, int NW> struct AttFewMem {
+template <int D> struct AttFewMem {
     union {
-        __attribute__((aligned(16))) float joint[NW][16][D + 4];
+        __attribute__((aligned(16))) float joint[4][16][D + 4];
         int starts[MMOE_KV_MAXSEQ + 1];
     };
-    float2 stat[NW][16];
+    float2 stat[4][16];
 };
-template <int T, int D, bool CAP, bool BIAS, int NW>
-__device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, const unsigned block, AttFewMem<D, NW> &M) {
+template <int T, int D, bool CAP, bool BIAS>
+__device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, const unsigned block, AttFewMem<D> &M) {
     constexpr int KS = D / 32, E = D / 16;   // products over the dims, values of a row per lane
     const mmoe_attn_args &a = A.a;
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 15, g = l >> 4;
@@ -1000,13 +1012,13 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     };
     int p = p0 + 32 * w;
     if (p < p1) {
-        int id = ids(p), next = ids(p + 32 * NW);
+        int id = ids(p), next = ids(p + 128);
         load_k(p, id);
         load_v(p, id);
-        for (; p + 32 * NW < p1; p += 32 * NW) {
-            step(p, [&] { load_k(p + 32 * NW, next); });
-            load_v(p + 32 * NW, next);
-            next = ids(p + 64 * NW);
+        for (; p + 128 < p1; p += 128) {
+            step(p, [&] { load_k(p + 128, next); });
+            load_v(p + 128, next);
+            next = ids(p + 256);
         }
         step(p, [] {});
     }
@@ -1018,15 +1030,14 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         for (int e = 0; e < E; e += 4) *(f4 *)&M.joint[w][n][(4 * g + j) * E + e] = f4{acc[e][j], acc[e + 1][j], acc[e + 2][j], acc[e + 3][j]};
     __syncthreads();
     // rows of 16 threads, D / 16 dims each
-    if (threadIdx.x >= 256) return;
     const int jr = threadIdx.x >> 4, d = (threadIdx.x & 15) * E, row = at.row0 + jr;
     if (row >= at.rows) return;
-    float2 st[NW];
+    float2 st[4];
     float mx = -__builtin_inff(), total = 0.0f, o[E] = {};
 #pragma unroll
-    for (int i = 0; i < NW; i++) { st[i] = M.stat[i][jr]; if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x); }
+    for (int i = 0; i < 4; i++) { st[i] = M.stat[i][jr]; if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x); }
 #pragma unroll
-    for (int i = 0; i < NW; i++) {
+    for (int i = 0; i < 4; i++) {
         if (st[i].y == 0.0f) continue;
         float e = exp2_(st[i].x - mx);
         total = fmaf(st[i].y, e, total);
@@ -1056,18 +1067,18 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
 // One launch for everything, the long work first. With no row tiles of 128 in it a kernel of its own: fewer registers, more waves.
 template <int T, int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(256, 2) k_attn_few(AttArgs A) {
-    __shared__ AttFewMem<D, 4> M;
+    __shared__ AttFewMem<D> M;
     const unsigned b = blockIdx.x;
     const bool shared = b < A.n_sh;
-    att_few<T, D, CAP, BIAS, 4>(A, shared, shared ? b : b - A.n_sh, M);
+    att_few<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh, M);
 }
-template <int T, int D, bool CAP, bool BIAS, int NG>
-__global__ void __launch_bounds__(256 * NG, 2) k_attn_tile(AttArgs A) {
-    __shared__ union { AttTileMem<D, NG> tile; AttFewMem<D, 4 * NG> few; } M;
+template <int T, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
+    __shared__ union { AttTileMem<D> tile; AttFewMem<D> few; } M;
     const unsigned b = blockIdx.x;
     const bool shared = b < A.n_sh;
-    if (shared ? !A.sh_few : b < A.n_sh + A.n_tile) att_tile<T, D, CAP, BIAS, NG>(A, shared, shared ? b : b - A.n_sh, M.tile);
-    else att_few<T, D, CAP, BIAS, 4 * NG>(A, shared, shared ? b : b - A.n_sh - A.n_tile, M.few);
+    if (shared ? !A.sh_few : b < A.n_sh + A.n_tile) att_tile<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh, M.tile);
+    else att_few<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh - A.n_tile, M.few);
 }
 
 // The partial results of a row: their maxima and sums give each a weight. D / 4 lanes read a part; with all, every such group of the

@@ -48,7 +48,7 @@ static int check_cache(const char *who, const mmoe_kv_cache *c) {
     if (c->heads < 1 || c->heads > 1024) REFUSE("%s: %d key/value heads", who, c->heads);
     if (c->block_stride < 0 || c->head_stride < 0 || c->token_stride < 0 || ((c->block_stride | c->head_stride | c->token_stride) & 7))
         REFUSE("%s: cache strides must be multiples of 8", who);
-    if (c->token_stride > 1 << 26) REFUSE("%s: token stride %lld above %d", who, (long long)c->token_stride, 1 << 26);
+    if (c->token_stride < c->head_dim || c->token_stride > 1 << 26) REFUSE("%s: token stride %lld outside %d..%d", who, (long long)c->token_stride, c->head_dim, 1 << 26);
     return 0;
 }
 
@@ -71,9 +71,10 @@ int mmoe_kv_plan(const mmoe_kv_plan_args *p) {
     if (mm_ready()) return -1;
     OnDevice dev;
     if (!dev.ok) return -1;
-    bool one = a.ntok <= 4096;
-    if (run(MMOE_K_KV_PLAN, k_kv_plan, 1, KP_T, a, sh, one)) return -1;
-    return one ? 0 : run(MMOE_K_KV_PLAN, k_kv_tokens, (a.ntok + 1023) / 1024, 256, a, sh);
+    const bool one = a.ntok <= 4096;
+    const unsigned threads = std::max(a.nseq, a.ntok) <= 256 ? 256 : 1024;
+    if (a.nseq <= 1024 ? run(MMOE_K_KV_PLAN, k_kv_plan<1>, 1, threads, a, sh, one) : run(MMOE_K_KV_PLAN, k_kv_plan<4>, 1, threads, a, sh, one)) return -1;
+    return one ? 0 : run(MMOE_K_KV_PLAN, k_kv_tokens, (a.ntok + 255) / 256, 256, a, sh);
 }
 
 int mmoe_rope_freqs(int rot, double base, double factor, int orig, double slow, double fast, double *freq) {
@@ -102,8 +103,9 @@ template <int IN, int OUT>
 static int rope_launch(const mmoe_rope_args &a, const mmoe_kv_cache &kv, int cached, int sh) {
     int tb = a.ntok >= 8192 ? 8 : a.ntok >= 2048 ? 2 : 1;
     dim3 g((a.ntok + tb - 1) / tb);
-    if (a.interleaved) return run(MMOE_K_ROPE, k_rope<IN, OUT, RP_INTER>, g, RP_T, a, kv, cached, sh, tb);
-    if (a.rot % 16 == 0) return run(MMOE_K_ROPE, k_rope<IN, OUT, RP_SPLIT>, g, RP_T, a, kv, cached, sh, tb);
+    const bool pow2 = (a.head_dim & (a.head_dim - 1)) == 0;
+    if (pow2 && a.interleaved) return run(MMOE_K_ROPE, k_rope<IN, OUT, RP_INTER>, g, RP_T, a, kv, cached, sh, tb);
+    if (pow2 && a.rot % 16 == 0) return run(MMOE_K_ROPE, k_rope<IN, OUT, RP_SPLIT>, g, RP_T, a, kv, cached, sh, tb);
     return run(MMOE_K_ROPE, k_rope<IN, OUT, RP_ODD>, g, RP_T, a, kv, cached, sh, tb);
 }
 template <int IN>
@@ -136,11 +138,12 @@ static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
 }
 
 // How a call is divided: row tiles, and runs or chunks of positions where the tiles alone are too few workgroups.
-struct AttPlan { int groups, few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts; size_t bytes; };
+struct AttPlan { int few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts; size_t bytes; };
 static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     AttPlan p = {};
     const int group = a.heads / kv.heads;
-    const int64_t rows = (int64_t)a.ntok * group, tiles = (rows + 127) / 128;
+    const int64_t rows = (int64_t)a.ntok * group;
+    const int64_t tiles = (rows + ATT_BM - 1) / ATT_BM;
     const int own = a.window && !a.hi ? (int)std::min<int64_t>(a.max_len - a.shared, (int64_t)a.window + a.max_q) : a.max_len - a.shared;
     // runs of at least `least` positions until there are about `want` workgroups
     auto runs = [&](int64_t groups, int positions, int want, int least) {
@@ -164,8 +167,6 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
         p.tiles = (int)tiles + a.nseq;
         p.split = runs(tiles, own, 256, 256);
     }
-    // two groups of waves per row tile while the tiles fill no more than one workgroup per CU
-    p.groups = ((p.few_sh ? 0 : (int64_t)p.tiles_sh * p.split_sh) + (p.tiles ? tiles * p.split : 0)) * kv.heads <= 384 ? 2 : 1;
     p.parts = p.split_sh + std::max(p.split, p.chunks);
     p.bytes = 256;
     if (p.parts > 1) p.bytes += (size_t)p.parts * a.ntok * a.heads * (kv.head_dim * 4 + 8);
@@ -190,8 +191,7 @@ static int att_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPl
     const dim3 g(A.n_sh + A.n_tile + A.n_few);
     const bool has_tiles = A.n_tile || (A.n_sh && !A.sh_few);
     if (!has_tiles ? run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, g, 256, A)
-        : p.groups == 2 ? run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS, 2>, g, 512, A)
-                        : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS, 1>, g, 256, A)) return -1;
+                   : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS>, g, 256, A)) return -1;
     if (p.parts == 1) return 0;
     const bool few_only = !p.split_sh && p.tiles && p.split == 1, all = p.parts > 8;   // only sequences of few rows have partial results
     const unsigned rows = few_only ? 16u * kv.heads * a.nseq : (unsigned)a.ntok * a.heads, lpr = D / 4;
