@@ -33,21 +33,25 @@ template <int T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
     h2 r = {(_Float16)a, (_Float16)b};
     return __builtin_bit_cast(uint32_t, r);
 }
-template <int T> __device__ __forceinline__ void load8(float *x, const void *p, int64_t at) {
-    if (T == MMOE_F32) {
-        const gu4 *q = (const gu4 *)((const float *)p + at);
-        u4 a = q[0], b = q[1];
+// eight values as they lie in memory
+template <int T> struct Raw8 { u4 w[T == MMOE_F32 ? 2 : 1]; };
+template <int T> __device__ __forceinline__ Raw8<T> load8(const void *p, int64_t at) {
+    const gu4 *q = (const gu4 *)((const uint8_t *)p + at * Elem<T>::size);
+    Raw8<T> r;
 #pragma unroll
-        for (int i = 0; i < 4; i++) { x[i] = __uint_as_float(a[i]); x[4 + i] = __uint_as_float(b[i]); }
-    } else {
-        u4 a = *(const gu4 *)((const uint16_t *)p + at);
+    for (int i = 0; i < Elem<T>::size / 2; i++) r.w[i] = q[i];
+    return r;
+}
+template <int T> __device__ __forceinline__ void unpack8(float *x, const Raw8<T> &r) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) { x[2 * i] = half_to_f<T>(a[i] & 0xffff); x[2 * i + 1] = half_to_f<T>(a[i] >> 16); }
+    for (int i = 0; i < 4; i++) {
+        if (T == MMOE_F32) { x[i] = __uint_as_float(r.w[0][i]); x[4 + i] = __uint_as_float(r.w[Elem<T>::size / 4][i]); }
+        else { x[2 * i] = half_to_f<T>(r.w[0][i] & 0xffff); x[2 * i + 1] = half_to_f<T>(r.w[0][i] >> 16); }
     }
 }
-template <int T> __device__ __forceinline__ void store8(void *p, int64_t at, const float *x) {
+template <int T> __device__ __forceinline__ void store8(void *p, const float *x) {
     if (T == MMOE_F32) {
-        gu4 *q = (gu4 *)((float *)p + at);
+        gu4 *q = (gu4 *)p;
         u4 a, b;
 #pragma unroll
         for (int i = 0; i < 4; i++) { a[i] = __float_as_uint(x[i]); b[i] = __float_as_uint(x[4 + i]); }
@@ -56,7 +60,7 @@ template <int T> __device__ __forceinline__ void store8(void *p, int64_t at, con
         u4 a;
 #pragma unroll
         for (int i = 0; i < 4; i++) a[i] = pack2<T>(x[2 * i], x[2 * i + 1]);
-        *(gu4 *)((uint16_t *)p + at) = a;
+        *(gu4 *)p = a;
     }
 }
 
@@ -264,29 +268,32 @@ __device__ __forceinline__ void rope_angles(const mmoe_rope_args &a, int t0, int
     }
 }
 
-// Head hd of a token's query heads | key heads | value heads (the last with a cache only): where it comes from and goes to.
+// Head hd of a token's query heads | key heads | value heads (the last with a cache only): where it comes from and goes to (NULL: nowhere).
 struct RopeHead {
-    const void *in; void *out;
-    int64_t src, dst;
-    bool turn, live;
+    const void *in;
+    int64_t src;
+    uint8_t *out;
+    bool turn;
 };
-__device__ __forceinline__ RopeHead rope_head(const mmoe_rope_args &a, const mmoe_kv_cache &kv, int cached, int sh, int64_t tok, int hd) {
+template <int OUT> __device__ __forceinline__ RopeHead rope_head(const mmoe_rope_args &a, const mmoe_kv_cache &kv, int cached, int sh, int64_t tok, int hd) {
     RopeHead r;
-    r.live = true;
-    int64_t slot = 0;
+    bool live = true;
+    int64_t slot = 0, dst;
+    void *out;
     if (cached) {
         int s = a.slot[tok];
-        r.live = s >= 0 && (s >> sh) < kv.nblocks;
+        live = s >= 0 && (s >> sh) < kv.nblocks;
         slot = (int64_t)(s >> sh) * kv.block_stride + (int64_t)(s & (kv.block_size - 1)) * kv.token_stride;
     }
     int hk = hd - a.heads, hv = hk - a.kv_heads;
     r.turn = hv < 0;
-    if (hk < 0) { r.in = a.q; r.src = tok * a.q_token + hd * a.q_head; r.out = a.q_out; r.dst = tok * a.qo_token + hd * a.qo_head; }
+    if (hk < 0) { r.in = a.q; r.src = tok * a.q_token + hd * a.q_head; out = a.q_out; dst = tok * a.qo_token + hd * a.qo_head; }
     else if (hv < 0) {
         r.in = a.k; r.src = tok * a.k_token + hk * a.k_head;
-        r.out = cached ? kv.k : a.k_out;
-        r.dst = cached ? slot + hk * kv.head_stride : tok * a.ko_token + hk * a.ko_head;
-    } else { r.in = a.v; r.src = tok * a.v_token + hv * a.v_head; r.out = kv.v; r.dst = slot + hv * kv.head_stride; }
+        out = cached ? kv.k : a.k_out;
+        dst = cached ? slot + hk * kv.head_stride : tok * a.ko_token + hk * a.ko_head;
+    } else { r.in = a.v; r.src = tok * a.v_token + hv * a.v_head; out = kv.v; dst = slot + hv * kv.head_stride; }
+    r.out = live ? (uint8_t *)out + dst * Elem<OUT>::size : nullptr;
     return r;
 }
 
@@ -296,9 +303,9 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
     __shared__ float row[LAY == RP_ODD ? RP_T * 8 : 1];
     const int t0 = blockIdx.x * tb, nt = min(tb, a.ntok - t0), half = a.rot >> 1, dc = a.head_dim >> 3;
     const int nh = a.heads + a.kv_heads + (cached ? a.kv_heads : 0), all = nt * nh;   // heads of the workgroup's tokens
-    rope_angles(a, t0, nt, cs);
-    __syncthreads();
     if (LAY == RP_ODD) {
+        rope_angles(a, t0, nt, cs);
+        __syncthreads();
         // the round's heads through LDS: a unit's partners start anywhere in another unit
         const int hpr = RP_T / dc, hl = threadIdx.x / dc, d0 = (threadIdx.x - hl * dc) * 8;
         for (int j0 = 0; j0 < all; j0 += hpr) {
@@ -307,11 +314,11 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
             RopeHead r;
             float x[8], y[8], *mine = row + threadIdx.x * 8, *head = row + hl * a.head_dim;
             if (on) {
-                r = rope_head(a, kv, cached, sh, t0 + t, j - t * nh);
-                on = r.live;
+                r = rope_head<OUT>(a, kv, cached, sh, t0 + t, j - t * nh);
+                on = r.out != nullptr;
             }
             if (on) {
-                load8<IN>(x, r.in, r.src + d0);
+                unpack8<IN>(x, load8<IN>(r.in, r.src + d0));
 #pragma unroll
                 for (int i = 0; i < 8; i++) mine[i] = x[i];
             }
@@ -327,56 +334,75 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
                     const float z = head[a.interleaved ? d ^ 1 : low ? d + half : d - half];
                     y[i] = low ? fmaf(x[i], c.x, -(z * c.y)) : fmaf(x[i], c.x, z * c.y);
                 }
-                store8<OUT>(r.out, r.dst + d0, y);
+                store8<OUT>(r.out + d0 * Elem<OUT>::size, y);
             }
             __syncthreads();
         }
         return;
     }
-    // A head is dc lanes of one wave (dc a power of two), a unit of 8 values each; four heads' loads under way per lane. With split pairs a
-    // lane loads its partner's unit too (the same lines again): in place, too, a head is read whole before any of it is written.
+    // A head is dc lanes of one wave (dc a power of two), a unit of 8 values each; four heads' loads under way per lane, the first four
+    // beside the angles. With split pairs a lane loads its partner's unit too (the same lines again): in place, too, a head is read
+    // whole before any of it is written.
     const int sd = 31 - __builtin_clz(dc), d0 = (threadIdx.x & (dc - 1)) * 8, hpr = RP_T >> sd;
     int hd = threadIdx.x >> sd, t = 0;
-    for (int left = (all - hd + hpr - 1) / hpr; left > 0; left -= 4) {
-        RopeHead r[4];
-        float x[4][8], z[4][8];
-        const float2 *w[4];
+    Raw8<IN> x[4], z[4];
+    uint8_t *out[4];
+    int tk[4];
+    bool turn[4];
+    auto load = [&](int left) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            r[k].live = false;
+            out[k] = nullptr;
             if (k >= left) continue;
             while (hd >= nh) { hd -= nh; t++; }
-            r[k] = rope_head(a, kv, cached, sh, t0 + t, hd);
-            w[k] = cs + t * RP_HALF;
+            const RopeHead r = rope_head<OUT>(a, kv, cached, sh, t0 + t, hd);
+            out[k] = r.out ? r.out + d0 * Elem<OUT>::size : nullptr;
+            turn[k] = r.turn && d0 < a.rot;
+            tk[k] = t;
             hd += hpr;
-            if (!r[k].live) continue;
-            load8<IN>(x[k], r[k].in, r[k].src + d0);
-            if (LAY == RP_SPLIT && r[k].turn && d0 < a.rot) load8<IN>(z[k], r[k].in, r[k].src + (d0 < half ? d0 + half : d0 - half));
+            x[k] = load8<IN>(r.in, r.src + d0);
+            if (LAY == RP_SPLIT && turn[k]) z[k] = load8<IN>(r.in, r.src + (d0 < half ? d0 + half : d0 - half));
         }
+    };
+    auto store = [&] {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if (!r[k].live) continue;
-            if (r[k].turn && d0 < a.rot) {
-                float y[8];
+            if (!out[k]) continue;
+            float y[8];
+            unpack8<IN>(y, x[k]);
+            if (turn[k]) {
+                const float2 *w = cs + tk[k] * RP_HALF;
                 if (LAY == RP_INTER) {
 #pragma unroll
                     for (int i = 0; i < 8; i += 2) {
-                        const bool in = d0 + i < a.rot;
-                        const float2 c = in ? w[k][(d0 + i) >> 1] : make_float2(1.0f, 0.0f);
-                        y[i] = in ? fmaf(x[k][i], c.x, -(x[k][i + 1] * c.y)) : x[k][i];
-                        y[i + 1] = in ? fmaf(x[k][i + 1], c.x, x[k][i] * c.y) : x[k][i + 1];
+                        if (d0 + i >= a.rot) continue;
+                        const float2 c = w[(d0 + i) >> 1];
+                        const float lo = y[i], hi = y[i + 1];
+                        y[i] = fmaf(lo, c.x, -(hi * c.y));
+                        y[i + 1] = fmaf(hi, c.x, lo * c.y);
                     }
                 } else {
+                    float other[8];
+                    unpack8<IN>(other, z[k]);
                     const float sign = d0 < half ? -1.0f : 1.0f;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
-                        const float2 c = w[k][(d0 < half ? d0 : d0 - half) + i];
-                        y[i] = fmaf(x[k][i], c.x, sign * (z[k][i] * c.y));
+                        const float2 c = w[(d0 < half ? d0 : d0 - half) + i];
+                        y[i] = fmaf(y[i], c.x, sign * (other[i] * c.y));
                     }
                 }
-                store8<OUT>(r[k].out, r[k].dst + d0, y);
-            } else store8<OUT>(r[k].out, r[k].dst + d0, x[k]);
+            }
+            store8<OUT>(out[k], y);
         }
+    };
+    int left = (all - hd + hpr - 1) / hpr;
+    load(left);
+    rope_angles(a, t0, nt, cs);
+    __syncthreads();
+    for (;;) {
+        store();
+        if ((left -= 4) <= 0) return;
+        load(left);
     }
 }
 
