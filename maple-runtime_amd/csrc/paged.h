@@ -84,6 +84,19 @@ template <typename F> __device__ __forceinline__ int count_wave(int n, F &&f) {
     return c;
 }
 
+template <typename F> __device__ __forceinline__ int wave_reduce(int v, F &&f) {   // in registers: an exchange through LDS costs 100 cycles a step
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0xb1, 15, 15, false));    // lane ^ 1
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x4e, 15, 15, false));    // lane ^ 2
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 15, 15, false));   // mirrored in 8
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 15, 15, false));   // mirrored in 16
+    auto a = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+    v = f((int)a[0], (int)a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+    return __builtin_amdgcn_readfirstlane(f((int)b[0], (int)b[1]));
+}
+__device__ __forceinline__ int wave_min(int v) { return wave_reduce(v, [](int x, int y) { return min(x, y); }); }
+__device__ __forceinline__ int wave_max(int v) { return wave_reduce(v, [](int x, int y) { return max(x, y); }); }
+
 // ------------------------------------------------------------------------------------------------------
 // Block tables and slot maps (mmoe_kv_plan)
 // ------------------------------------------------------------------------------------------------------
@@ -127,15 +140,14 @@ __device__ __forceinline__ void scan2(unsigned &a, unsigned &b, unsigned *ta, un
 template <int PER>
 __global__ void __launch_bounds__(1024) k_kv_plan(mmoe_kv_plan_args a, int sh, int tokens) {
     constexpr int NS = PER * 1024;
-    __shared__ int start[NS + 1], first[NS + 1], lens[NS], tail[NS], top[KP_TOP];
+    __shared__ int start[NS + 1], first[NS + 1], lens[NS], tail[NS], given[KP_TOP], top[KP_TOP];
     __shared__ uint2 red[16];
-    __shared__ unsigned took[2];   // tokens and blocks of the sequences that fit
     const int tid = threadIdx.x, nt = blockDim.x, n = a.nseq, bs1 = a.block_size - 1, keep = a.shared >> sh, s0 = tid * PER;
     const int room = a.width << sh;   // < 2^31
     int ctx[PER], add[PER], old[PER];
     bool fin[PER];
-    if (tid < 2) took[tid] = 0;
     const int nfree0 = min(max(a.nfree[0], 0), a.nblocks);
+    for (int j = tid; j < min(nfree0, KP_TOP); j += nt) top[j] = a.free_list[nfree0 - 1 - j];
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         const bool in = s0 + i < n;
@@ -168,12 +180,16 @@ __global__ void __launch_bounds__(1024) k_kv_plan(mmoe_kv_plan_args a, int sh, i
         const int back = (int)min(tg, (unsigned)(a.nblocks - nfree0));
         for (int j = tid; j < back; j += nt) {
             int s = count_le(first, n, j) - 1;
-            a.free_list[nfree0 + j] = a.table[(int64_t)s * a.width + keep + j - first[s]];
+            const int b = a.table[(int64_t)s * a.width + keep + j - first[s]];
+            a.free_list[nfree0 + j] = b;
+            if (j < KP_TOP) given[j] = b;
         }
-        nfree += back;
-        if (back) __syncthreads();
+        nfree += back;   // (scan2 waits for given, and for what is only in memory)
     }
-    for (int j = tid; j < min(nfree, KP_TOP); j += nt) top[j] = a.free_list[nfree - 1 - j];
+    auto taken = [&](int j) {   // the j-th block from the end of the list
+        const int at = nfree - 1 - j, g = at - nfree0;
+        return g >= 0 ? g < KP_TOP ? given[g] : a.free_list[at] : -g - 1 < KP_TOP ? top[-g - 1] : a.free_list[at];
+    };
     // 2. the sequences that fit: a prefix, since both sums only grow (one that cannot fit counts more tokens than there is room for)
     unsigned need[PER], tok[PER], cn = 0, ct = 0, tn, tt;
 #pragma unroll
@@ -187,19 +203,20 @@ __global__ void __launch_bounds__(1024) k_kv_plan(mmoe_kv_plan_args a, int sh, i
     }
     scan2(cn, ct, &tn, &tt, red);
     unsigned fits = 0;
+    int total = 0, blocks = 0;   // tokens and blocks of the sequences that fit
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         if (s0 + i >= n) continue;
         first[s0 + i] = (int)cn; start[s0 + i] = (int)ct;
         cn = min(cn + need[i], (unsigned)KP_LIM); ct = min(ct + tok[i], (unsigned)KP_LIM);
-        if (cn <= (unsigned)nfree && ct <= (unsigned)a.ntok && ct < KP_LIM) {
-            fits |= 1u << i;
-            // sums grow: the last of them is the total (nothing to record where all fit)
-            if (cn != tn || ct != tt || s0 + i == n - 1) { atomicMax(&took[0], ct); atomicMax(&took[1], cn); }
-        }
+        if (cn <= (unsigned)nfree && ct <= (unsigned)a.ntok && ct < KP_LIM) { fits |= 1u << i; total = (int)ct; blocks = (int)cn; }
     }
+    // sums only grow: the largest of those that fit are the totals
+    total = wave_max(total); blocks = wave_max(blocks);
+    __syncthreads();   // red has been read
+    if ((tid & 63) == 0) red[tid >> 6] = make_uint2(total, blocks);
     __syncthreads();
-    const int total = (int)took[0], blocks = (int)took[1];
+    for (int i = 0; i < nt >> 6; i++) { total = max(total, (int)red[i].x); blocks = max(blocks, (int)red[i].y); }
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         if (s0 + i >= n) continue;
@@ -213,7 +230,7 @@ __global__ void __launch_bounds__(1024) k_kv_plan(mmoe_kv_plan_args a, int sh, i
     for (int j = tid; j < blocks; j += nt) {
         int s = count_le(first, n, j) - 1;
         int held = (lens[s] - (start[s + 1] - start[s]) + bs1) >> sh;
-        a.table[(int64_t)s * a.width + held + j - first[s]] = j < KP_TOP ? top[j] : a.free_list[nfree - 1 - j];
+        a.table[(int64_t)s * a.width + held + j - first[s]] = taken(j);
     }
     if (!tokens) return;
     for (int t = tid; t < a.ntok; t += nt) {
@@ -222,7 +239,7 @@ __global__ void __launch_bounds__(1024) k_kv_plan(mmoe_kv_plan_args a, int sh, i
             const int s = count_le(start, n, t) - 1, c = lens[s] - (start[s + 1] - start[s]);
             pos = c + t - start[s];
             const int j = (pos >> sh) - ((c + bs1) >> sh) + first[s];   // of the blocks taken; before the sequence's first: the begun one
-            const int blk = j < first[s] ? tail[s] : j < KP_TOP ? top[j] : a.free_list[nfree - 1 - j];
+            const int blk = j < first[s] ? tail[s] : taken(j);
             if ((unsigned)blk < (unsigned)a.nblocks) slot = (blk << sh) + (pos & bs1);
         }
         a.pos[t] = pos; a.slot[t] = slot;
@@ -254,6 +271,8 @@ __global__ void __launch_bounds__(256) k_kv_tokens(mmoe_kv_plan_args a, int sh) 
 #define RP_T 256
 #define RP_HALF 128   // largest rot / 2
 #define RP_TB 8       // most tokens per workgroup
+#define RP_U 3        // heads of a lane whose loads are under way together (8191 tokens: 1 or 2 26.5 us, 3 24.1, 4 26.5, 6 26.0: with 3 two tokens of
+                      // Maple's 24 heads are one turn)
 enum { RP_INTER, RP_SPLIT, RP_ODD };   // pairs (2 i, 2 i + 1); (i, i + rot / 2) with rot / 2 in whole units of 8; any rot, any head_dim
 
 __device__ __forceinline__ void rope_angles(const mmoe_rope_args &a, int t0, int nt, float2 *cs) {
@@ -345,13 +364,13 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
     // whole before any of it is written.
     const int sd = 31 - __builtin_clz(dc), d0 = (threadIdx.x & (dc - 1)) * 8, hpr = RP_T >> sd;
     int hd = threadIdx.x >> sd, t = 0;
-    Raw8<IN> x[4], z[4];
-    uint8_t *out[4];
-    int tk[4];
-    bool turn[4];
+    Raw8<IN> x[RP_U], z[RP_U];
+    uint8_t *out[RP_U];
+    int tk[RP_U];
+    bool turn[RP_U];
     auto load = [&](int left) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < RP_U; k++) {
             out[k] = nullptr;
             if (k >= left) continue;
             while (hd >= nh) { hd -= nh; t++; }
@@ -366,7 +385,7 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
     };
     auto store = [&] {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < RP_U; k++) {
             if (!out[k]) continue;
             float y[8];
             unpack8<IN>(y, x[k]);
@@ -401,7 +420,7 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
     __syncthreads();
     for (;;) {
         store();
-        if ((left -= 4) <= 0) return;
+        if ((left -= RP_U) <= 0) return;
         load(left);
     }
 }
@@ -473,19 +492,6 @@ __device__ __forceinline__ float add_halves(float x) {
     auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-template <typename F> __device__ __forceinline__ int wave_reduce(int v, F &&f) {   // in registers: an exchange through LDS costs 100 cycles a step
-    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0xb1, 15, 15, false));    // lane ^ 1
-    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x4e, 15, 15, false));    // lane ^ 2
-    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 15, 15, false));   // mirrored in 8
-    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 15, 15, false));   // mirrored in 16
-    auto a = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
-    v = f((int)a[0], (int)a[1]);
-    auto b = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
-    return __builtin_amdgcn_readfirstlane(f((int)b[0], (int)b[1]));
-}
-__device__ __forceinline__ int wave_min(int v) { return wave_reduce(v, [](int x, int y) { return min(x, y); }); }
-__device__ __forceinline__ int wave_max(int v) { return wave_reduce(v, [](int x, int y) { return max(x, y); }); }
-
 // The sequence and row tile of virtual tile v, with tiles of bm rows: sequence s has the tiles from floor(rows before it / bm) + s
 // on; no two sequences' tiles meet, and some virtual tiles are nobody's. No sums over the sequences are needed.
 __device__ __forceinline__ int att_start(const mmoe_attn_args &a, int s) { return min(max(a.qstart[s], 0), a.ntok); }   // never past the arrays

@@ -101,8 +101,8 @@ int mmoe_rope_freqs(int rot, double base, double factor, int orig, double slow, 
 // ------------------------------------------------------------------------------------------------------
 template <int IN, int OUT>
 static int rope_launch(const mmoe_rope_args &a, const mmoe_kv_cache &kv, int cached, int sh) {
-    // as many tokens per workgroup as four heads per lane cover, once there are workgroups enough
-    const int nh = a.heads + a.kv_heads * (1 + cached), at_once = 4 * RP_T / (a.head_dim / 8);
+    // as many tokens per workgroup as RP_U heads per lane cover, once there are workgroups enough
+    const int nh = a.heads + a.kv_heads * (1 + cached), at_once = RP_U * RP_T / (a.head_dim / 8);
     const int tb = std::max(1, std::min(std::min(at_once / nh, RP_TB), a.ntok / 1024));
     dim3 g((a.ntok + tb - 1) / tb);
     const bool pow2 = (a.head_dim & (a.head_dim - 1)) == 0;
