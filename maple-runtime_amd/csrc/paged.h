@@ -818,11 +818,15 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
             }
             const bool mine = p < whi && p + ATT_BN > wlo;
             if (mine) {
+                __builtin_amdgcn_s_setprio(1);
                 scores(sc, kbuf);
+                __builtin_amdgcn_s_setprio(0);
                 math(sc, p);
                 if (p < inlo || p + ATT_BN > inhi || bad) mask(sc, p, bad);
                 rescale();
+                __builtin_amdgcn_s_setprio(1);
                 product(vbuf);
+                __builtin_amdgcn_s_setprio(0);
             }
             if (odd) {
                 if (mine) add_aside(vother, p, bad);
