@@ -446,13 +446,21 @@ typedef __attribute__((address_space(3))) u4 lu4;
 typedef __attribute__((address_space(3))) uint8_t lb;
 typedef __attribute__((address_space(1))) const uint8_t gb;
 
+// n / d for every 32-bit n by a multiplication (Granlund and Montgomery 1994); a division costs some 40 instructions
+struct Div {
+    uint32_t d, m, s1, s2;
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const { uint32_t t = __umulhi(m, n); return (t + ((n - t) >> s1)) >> s2; }
+};
+
 struct AttArgs {
     mmoe_attn_args a;
     mmoe_kv_cache kv;
     int sh, group;       // log2 of the block size, query heads per key/value head
+    Div by_heads, by_kv, by_group, by_split, by_split_sh, by_chunks;
     // one launch: n_sh workgroups over the shared positions (row tiles of 128, or of 16 with sh_few), n_tile over each sequence's own
     // positions in row tiles of 128, n_few over those of sequences with up to `few` rows per key/value head (0: none) in chunks
     unsigned n_sh, n_tile, n_few;
+    int tiles_sh, tiles;   // their row tiles
     int sh_few, few;
     int split_sh, split, chunk, chunks;   // runs of the shared positions, runs per row tile of the own ones; positions per chunk, most chunks
     int parts_sh;        // partial results of the shared positions: split_sh, or 0
@@ -526,7 +534,7 @@ __device__ __forceinline__ AttRow att_row(const AttArgs &A, const AttTileAt &at,
     AttRow o;
     o.live = r < at.rows;
     if (!o.live) r = at.rows - 1;
-    int j = r / A.group;
+    const int j = (int)A.by_group(r);
     o.tok = at.t0 + j;
     o.head = kvh * A.group + r - j * A.group;
     return o;
@@ -568,8 +576,9 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
 // reads of 4 rows meet in a bank. P is rounded to the cache's type (half a step relative, as the result itself is), its
 // sum is of the unrounded 32-bit values.
 template <int D> struct AttTileMem {
+    __attribute__((aligned(1024))) uint8_t first[2 * ATT_BN * D * 2];   // keys and values of a tile
     union {
-        __attribute__((aligned(1024))) uint8_t tiles[4][ATT_BN * D * 2];   // keys of two tiles, values of two
+        __attribute__((aligned(1024))) uint8_t second[2 * ATT_BN * D * 2];
         int starts[MMOE_KV_MAXSEQ + 1];
     };
     int range[4][4], flag[2][4];
@@ -577,42 +586,14 @@ template <int D> struct AttTileMem {
 template <int T, int D, bool CAP, bool BIAS>
 __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, const unsigned block, AttTileMem<D> &M) {
     constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // a row's bytes and chunks; rows of a load, a wave's loads
+    constexpr uint32_t TB = ATT_BN * RB;
     const mmoe_attn_args &a = A.a;
     const int nsplit = shared ? A.split_sh : A.split;
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 31, hh = l >> 5;
-    const int kvh = block % A.kv.heads, rest = block / A.kv.heads, split = rest % nsplit;
+    const unsigned rest = A.by_kv(block), v = (shared ? A.by_split_sh : A.by_split)(rest);
+    const int kvh = block - rest * A.kv.heads, split = rest - v * nsplit;
     AttTileAt at;
-    if (!att_find(A, shared, ATT_BM, (shared ? A.n_sh : A.n_tile) / A.kv.heads / nsplit - 1 - rest / nsplit, at)) return;   // the last tiles see most: first
-    AttRow R = att_row(A, at, at.row0 + w * 32 + n, kvh);
-    // queries: operand B, lane (hh, n) holds dims 16 s + 8 hh .. + 8 of row n
-    u4 q[KS];
-    {
-        const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * hh;
-#pragma unroll
-        for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 16 * s);
-    }
-    const float slope = BIAS ? a.slopes[R.head] * ATT_LOG2E : 0.0f;
-    att_limits(A, shared, at, M.starts, R);
-    // the wave's and the workgroup's positions
-    const bool some = R.live && R.lo < R.hi;
-    const int wlo = wave_min(some ? R.lo : INT32_MAX), whi = wave_max(some ? R.hi : 0);
-    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
-    if (l == 0) { M.range[0][w] = wlo; M.range[1][w] = whi; M.range[2][w] = inlo; M.range[3][w] = inhi; }
-    __syncthreads();
-    int p0 = INT32_MAX, p1 = 0, glo = 0, ghi = INT32_MAX;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        p0 = min(p0, M.range[0][i]); p1 = max(p1, M.range[1][i]);
-        glo = max(glo, M.range[2][i]); ghi = min(ghi, M.range[3][i]);
-    }
-    p0 &= ~(ATT_BN - 1);
-    glo = __builtin_amdgcn_readfirstlane(glo); ghi = __builtin_amdgcn_readfirstlane(ghi);
-    if (nsplit > 1 && p0 < p1) {
-        int run = ((p1 - p0 + ATT_BN - 1) / ATT_BN + nsplit - 1) / nsplit * ATT_BN;
-        p0 += split * run;
-        p1 = min(p1, p0 + run);
-    }
-    p0 = __builtin_amdgcn_readfirstlane(p0); p1 = __builtin_amdgcn_readfirstlane(p1);
+    if (!att_find(A, shared, ATT_BM, (shared ? A.tiles_sh : A.tiles) - 1 - (int)v, at)) return;   // the last tiles see most: first
 
     // What the lane loads of a tile: row RPI i + l / CH of the wave's 16, piece l % CH of LDS, less the instruction's own offset (rows are at
     // least head_dim values apart, so it stays positive).
@@ -623,14 +604,6 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         ko[i] = (uint32_t)(r * A.kv.token_stride + (c ^ (r & (CH - 1))) * 8) * 2 - 1024 * i;
         vo[i] = (uint32_t)(r * A.kv.token_stride + (c ^ ((r & (CH / 2 - 1)) << 1)) * 8) * 2 - 1024 * i;
     }
-    // where it reads them back: K row n (and n + 32), pieces 2 k + hh; V rows vr (and on by eights), dims 32 i + 16 (l / 16 % 2) + 4 (l % 4) ..
-    // (the number that exchanges a row's pieces is the same for rows 32 (K) and 8 (V) apart: what is added are constants)
-    uint32_t ka[KS], va[DS];
-    const int vr = 4 * hh + ((l & 15) >> 2);
-#pragma unroll
-    for (int k = 0; k < KS; k++) ka[k] = n * RB + (((2 * k + hh) ^ (n & (CH - 1))) << 4);
-#pragma unroll
-    for (int i = 0; i < DS; i++) va[i] = vr * RB + ((64 * i + 32 * ((l >> 4) & 1) + 8 * (l & 3)) ^ ((vr & (CH / 2 - 1)) << 5));
     // block ids of 64 groups of 16 positions at a time, group l in lane l; a load of their own each tile would have to be waited for
     // with the tile's
     const int32_t *table = a.table + (int64_t)at.s * a.width;
@@ -650,7 +623,66 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         const uint8_t *from = (const uint8_t *)base + (blk * A.kv.block_stride + kvh * A.kv.head_stride + ((p + 16 * w) & (A.kv.block_size - 1)) * A.kv.token_stride) * 2;
         load_lds<NI>(from, off, buf + w * 16 * RB);
     };
-
+    const uint32_t lds = (uint32_t)(uintptr_t)(lb *)M.first;   // tile i: keys at lds + 2 TB (i % 2), values TB behind them
+    unsigned bad = 0, next = 0;   // the tile's lost blocks, the next one's
+    int p0, p1, blk;
+    if (shared) {   // which positions is known already: the first tile comes while the rows look for their sequences
+        const int run = ((a.shared + ATT_BN - 1) / ATT_BN + nsplit - 1) / nsplit * ATT_BN;
+        p0 = split * run; p1 = min(p0 + run, a.shared);
+        if (p0 < p1) {
+            blk = block_of(p0, bad);
+            fetch(lds, A.kv.k, ko, p0, blk);
+            fetch(lds + TB, A.kv.v, vo, p0, blk);
+        }
+    }
+    AttRow R = att_row(A, at, at.row0 + w * 32 + n, kvh);
+    att_limits(A, shared, at, M.starts, R);
+    // queries: operand B, lane (hh, n) holds dims 16 s + 8 hh .. + 8 of row n
+    u4 q[KS];
+    {
+        const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * hh;
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 16 * s);
+    }
+    const float slope = BIAS ? a.slopes[R.head] * ATT_LOG2E : 0.0f;
+    // the wave's and the workgroup's positions
+    const bool some = R.live && R.lo < R.hi;
+    const int wlo = wave_min(some ? R.lo : INT32_MAX), whi = wave_max(some ? R.hi : 0);
+    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
+    if (l == 0) { M.range[0][w] = wlo; M.range[1][w] = whi; M.range[2][w] = inlo; M.range[3][w] = inhi; }
+    __syncthreads();
+    int lo = INT32_MAX, hi = 0, glo = 0, ghi = INT32_MAX;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        lo = min(lo, M.range[0][i]); hi = max(hi, M.range[1][i]);
+        glo = max(glo, M.range[2][i]); ghi = min(ghi, M.range[3][i]);
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo) & ~(ATT_BN - 1); hi = __builtin_amdgcn_readfirstlane(hi);
+    glo = __builtin_amdgcn_readfirstlane(glo); ghi = __builtin_amdgcn_readfirstlane(ghi);
+    if (shared) {
+        p1 = lo < hi ? min(p1, hi) : p0;   // (the first tile is there, also where it lies before lo: nobody looks)
+        if (p0 >= p1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // and is not left on its way into LDS that is another's
+    } else {
+        p0 = lo; p1 = hi;
+        if (nsplit > 1 && p0 < p1) {
+            int run = ((p1 - p0 + ATT_BN - 1) / ATT_BN + nsplit - 1) / nsplit * ATT_BN;
+            p0 += split * run;
+            p1 = min(p1, p0 + run);
+        }
+        if (p0 < p1) {
+            blk = block_of(p0, bad);
+            fetch(lds, A.kv.k, ko, p0, blk);
+            fetch(lds + TB, A.kv.v, vo, p0, blk);
+        }
+    }
+    // where it reads them back: K row n (and n + 32), pieces 2 k + hh; V rows vr (and on by eights), dims 32 i + 16 (l / 16 % 2) + 4 (l % 4) ..
+    // (the number that exchanges a row's pieces is the same for rows 32 (K) and 8 (V) apart: what is added are constants)
+    uint32_t ka[KS], va[DS];
+    const int vr = 4 * hh + ((l & 15) >> 2);
+#pragma unroll
+    for (int k = 0; k < KS; k++) ka[k] = n * RB + (((2 * k + hh) ^ (n & (CH - 1))) << 4);
+#pragma unroll
+    for (int i = 0; i < DS; i++) va[i] = vr * RB + ((64 * i + 32 * ((l >> 4) & 1) + 8 * (l & 3)) ^ ((vr & (CH / 2 - 1)) << 5));
     f16v acc[DS], sc[2];
 #pragma unroll
     for (int i = 0; i < DS; i++)
@@ -781,17 +813,11 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     };
 
     if (p0 < p1) {
-        constexpr uint32_t TB = ATT_BN * RB;
-        const uint32_t kb = (uint32_t)(uintptr_t)(lb *)M.tiles, vb = kb + 2 * TB;
-        unsigned bad, next = 0;   // the tile's lost blocks, the next one's
-        int blk = block_of(p0, bad);
-        fetch(kb, A.kv.k, ko, p0, blk);
-        fetch(vb, A.kv.v, vo, p0, blk);
 #pragma unroll
         for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));   // the queries are there: nothing in the loop waits for them
         for (int p = p0, i = 0; p < p1; p += ATT_BN, i ^= 1, bad = next) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the compiler does not know of these loads
-            const uint32_t kbuf = kb + i * TB, kother = kb + (i ^ 1) * TB, vbuf = vb + i * TB, vother = vb + (i ^ 1) * TB;
+            const uint32_t kbuf = lds + i * 2 * TB, vbuf = kbuf + TB, kother = lds + (i ^ 1) * 2 * TB, vother = kother + TB;
             const bool part = p < glo || p + ATT_BN > ghi || bad, more = p + ATT_BN < p1;
             if (part) {   // the wave's own 16 rows of values: are they finite?
                 bool o = false;
@@ -885,15 +911,16 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     constexpr int KS = D / 32, E = D / 16;   // products over the dims, values of a row per lane
     const mmoe_attn_args &a = A.a;
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 15, g = l >> 4;
-    const int kvh = block % A.kv.heads, rest = block / A.kv.heads, runs = shared ? A.split_sh : A.chunks, c = rest % runs;
+    const unsigned rest = A.by_kv(block), v = (shared ? A.by_split_sh : A.by_chunks)(rest);
+    const int kvh = block - rest * A.kv.heads, c = rest - v * (shared ? A.split_sh : A.chunks);
     AttTileAt at;
     int from, end;
     bool whole = false;   // the rows' only result
     if (shared) {
-        at.s = 0; at.t0 = 0; at.row0 = rest / runs * 16; at.rows = att_start(a, a.nseq) * A.group;
+        at.s = 0; at.t0 = 0; at.row0 = (int)v * 16; at.rows = att_start(a, a.nseq) * A.group;
         from = c * A.chunk; end = min(from + A.chunk, a.shared);
     } else {
-        at.s = rest / runs; at.t0 = att_start(a, at.s); at.row0 = 0;
+        at.s = (int)v; at.t0 = att_start(a, at.s); at.row0 = 0;
         int tokens = att_start(a, at.s + 1) - at.t0;
         at.rows = min(tokens, a.max_q) * A.group;
         if (at.rows > A.few || tokens < 1) return;
@@ -904,6 +931,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     }
     if (at.row0 >= at.rows) return;
     AttRow R = att_row(A, at, at.row0 + n, kvh);
+    att_limits(A, shared, at, M.starts, R);
     u4 q[KS];
     {
         const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * g;
@@ -911,7 +939,6 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 32 * s);
     }
     const float slope = BIAS ? a.slopes[R.head] * ATT_LOG2E : 0.0f;
-    att_limits(A, shared, at, M.starts, R);
     const bool some = R.live && R.lo < R.hi;
     int p0 = max(from, wave_min(some ? R.lo : INT32_MAX) & ~31), p1 = min(end, wave_max(some ? R.hi : 0));
     if (p0 >= p1) p0 = p1 = 0;   // nothing seen (p0 may be close to the largest int: no wave's first run is counted from it)
@@ -1080,7 +1107,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
 #pragma unroll
         for (int x = 0; x < E; x++) o[x] = fmaf(e, M.joint[i][jr][d + x], o[x]);
     }
-    const int j = row / A.group, tok = at.t0 + j, head = kvh * A.group + row - j * A.group;
+    const int j = (int)A.by_group(row), tok = at.t0 + j, head = kvh * A.group + row - j * A.group;
     if (shared) {   // tokens past max_q have no partial results
         int s = max(count_le(a.qstart, a.nseq, tok) - 1, 0);
         if (tok - a.qstart[s] >= a.max_q) return;
@@ -1138,7 +1165,7 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
         if (min(tokens, a.max_q) * A.group > A.few || j >= tokens) return;
         tok = t0 + j; head = r - j * a.heads;
     } else {
-        tok = row0 / a.heads; head = row0 - tok * a.heads;
+        tok = (int)A.by_heads(row0); head = row0 - tok * a.heads;
         if (tok >= att_start(a, a.nseq)) return;
         s = max((all ? count_wave(a.nseq, [&](int i) { return a.qstart[i] <= tok; }) : count_le(a.qstart, a.nseq, tok)) - 1, 0);
         t0 = att_start(a, s); tokens = att_start(a, s + 1) - t0;

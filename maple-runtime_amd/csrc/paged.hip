@@ -175,6 +175,12 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     return p;
 }
 
+static Div divisor(uint32_t d) {
+    uint32_t l = 0;
+    while (l < 32 && (1ull << l) < d) l++;
+    return Div{d, (uint32_t)(((1ull << 32) * ((1ull << l) - d)) / d + 1), std::min(l, 1u), l ? l - 1 : 0};
+}
+
 template <int T, int D, bool CAP, bool BIAS>
 static int att_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPlan &p) {
     AttArgs A{};
@@ -183,6 +189,9 @@ static int att_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPl
     A.n_sh = (unsigned)p.tiles_sh * p.split_sh * kv.heads;
     A.n_tile = (unsigned)p.tiles * p.split * kv.heads;
     A.n_few = (unsigned)p.chunks * a.nseq * kv.heads;
+    A.tiles_sh = p.tiles_sh; A.tiles = p.tiles;
+    A.by_heads = divisor(a.heads); A.by_kv = divisor(kv.heads); A.by_group = divisor(A.group);
+    A.by_split = divisor(std::max(p.split, 1)); A.by_split_sh = divisor(std::max(p.split_sh, 1)); A.by_chunks = divisor(std::max(p.chunks, 1));
     A.sh_few = p.few_sh; A.few = p.few;
     A.split_sh = p.split_sh; A.split = p.split; A.chunk = p.chunk; A.chunks = p.chunks;
     A.parts_sh = p.split_sh;
