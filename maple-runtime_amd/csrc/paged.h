@@ -688,7 +688,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     for (int i = 0; i < DS; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
-    float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f, mt;   // mb: m, 0 while that is -inf; mt: the last tile's
+    float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f;   // mb: m, 0 while that is -inf
     constexpr bool MATH = CAP || BIAS;
     const float s1 = MATH ? 1.0f : A.s1;
 
@@ -707,40 +707,42 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         for (int k = 0; k < 2 * KS - 6; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
         __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
     };
-    // scores in units of log 2 (without cap and bias: but for s1) and their maximum
+    // scores in units of log 2 (without cap and bias: but for s1)
     auto math = [&](f16v *s, int p) {
         const float dist = BIAS ? (float)(R.pos - p - 4 * hh) : 0.0f;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                float x = s[u][j] * A.s1;
+                if (CAP) x = fmaf(-2.0f * A.s2, __builtin_amdgcn_rcpf(1.0f + exp2_(x)), A.s2);   // tanh z = 1 - 2 / (1 + exp 2 z)
+                if (BIAS) x = fmaf(-slope, fabsf(dist - (float)(32 * u + 8 * (j >> 2) + (j & 3))), x);
+                s[u][j] = x;
+            }
+    };
+    // a tile that is not seen whole: -inf where a row does not look
+    auto mask = [&](f16v *s, int p, unsigned bad) {
+        const unsigned at = (unsigned)(p + 4 * hh - R.lo), span = (unsigned)max(R.hi - R.lo, 0);
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) s[u][j] = at + (32 * u + 8 * (j >> 2) + (j & 3)) < span ? s[u][j] : -__builtin_inff();
+        if (bad)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int j = 0; j < 16; j++) s[u][j] = (bad >> (2 * u + (j >> 3))) & 1 ? -__builtin_inff() : s[u][j];
+    };
+    auto largest = [&](const f16v *s) {
         float top[4];   // no chain of 32
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) {
-                const int at = 32 * u + 8 * (j >> 2) + (j & 3);
-                float x = s[u][j];
-                if (MATH) x *= A.s1;
-                if (CAP) x = fmaf(-2.0f * A.s2, __builtin_amdgcn_rcpf(1.0f + exp2_(x)), A.s2);   // tanh z = 1 - 2 / (1 + exp 2 z)
-                if (BIAS) x = fmaf(-slope, fabsf(dist - (float)at), x);
-                s[u][j] = x;
-                top[j & 3] = u || j > 3 ? max_(top[j & 3], x) : x;
-            }
-        mt = max_(max_(top[0], top[1]), max_(top[2], top[3]));
-    };
-    // a tile that is not seen whole
-    auto mask = [&](f16v *s, int p, unsigned bad) {
-        const unsigned from = (unsigned)(R.lo - p - 4 * hh), span = (unsigned)max(R.hi - R.lo, 0);
-        float top[4];
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                s[u][j] = ((unsigned)(32 * u + 8 * (j >> 2) + (j & 3)) - from < span) & !((bad >> (2 * u + (j >> 3))) & 1) ? s[u][j] : -__builtin_inff();
-                top[j & 3] = u || j > 3 ? max_(top[j & 3], s[u][j]) : s[u][j];
-            }
-        mt = max_(max_(top[0], top[1]), max_(top[2], top[3]));
+            for (int j = 0; j < 16; j++) top[j & 3] = u || j > 3 ? max_(top[j & 3], s[u][j]) : s[u][j];
+        return max_halves(max_(max_(top[0], top[1]), max_(top[2], top[3]))) * s1;
     };
     // a new maximum only once it is 2^8 past the old: until then weights stay below 2^8, in every type's range
-    auto rescale = [&] {
-        mt = max_halves(mt) * s1;
+    auto rescale = [&](float mt) {
         if (!__any(mt > m + 8.0f)) return;
         float mn = fmaxf(m, mt), bn = mn == -__builtin_inff() ? 0.0f : mn, al = exp2_(m - bn);
         m = mn; mb = bn; sum *= al;
@@ -847,9 +849,9 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                 __builtin_amdgcn_s_setprio(1);
                 scores(sc, kbuf);
                 __builtin_amdgcn_s_setprio(0);
-                math(sc, p);
+                if (MATH) math(sc, p);
                 if (p < inlo || p + ATT_BN > inhi || bad) mask(sc, p, bad);
-                rescale();
+                rescale(largest(sc));
                 __builtin_amdgcn_s_setprio(1);
                 product(vbuf);
                 __builtin_amdgcn_s_setprio(0);
@@ -1145,32 +1147,40 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
 }
 
 // The partial results of a row: their maxima and sums give each a weight. D / 4 lanes read a part; with all, every such group of the
-// workgroup works on one row (the loads of a row's parts are what there is to wait for), else each has its own.
+// workgroup works on one row (the loads of a row's parts are what there is to wait for), else each has its own (up to ATT_PER parts).
 // few_only: the rows are those of the sequences of few rows, 16 per key/value head.
 #define ATT_PARTS 1024     // most partial results of a row
+#define ATT_PER 16
 template <int T, int D>
 __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_only) {
     constexpr int LPR = D / 4;
     const mmoe_attn_args &a = A.a;
     __shared__ float red[2][16], wt[ATT_PARTS];
-    __shared__ __attribute__((aligned(16))) float acc[1024 / LPR][D];
+    __shared__ union { __attribute__((aligned(16))) float acc[1024 / LPR][D]; int starts[MMOE_KV_MAXSEQ + 1]; } M;
     const int gr = blockDim.x / LPR, gi = threadIdx.x / LPR, x = (threadIdx.x % LPR) * 4, row0 = all ? blockIdx.x : blockIdx.x * gr + gi;
     int tok, head, s, t0, tokens;
+    bool on = true;
     if (few_only) {
         const int per = 16 * A.kv.heads;
         s = row0 / per;
-        if (s >= a.nseq) return;
+        on = s < a.nseq;
+        if (!on) s = 0;
         t0 = att_start(a, s); tokens = att_start(a, s + 1) - t0;
-        const int r = row0 - s * per, j = r / a.heads;
-        if (min(tokens, a.max_q) * A.group > A.few || j >= tokens) return;
+        const int r = row0 - s * per, j = (int)A.by_heads(r);
+        on = on && min(tokens, a.max_q) * A.group <= A.few && j < tokens;
         tok = t0 + j; head = r - j * a.heads;
     } else {
         tok = (int)A.by_heads(row0); head = row0 - tok * a.heads;
-        if (tok >= att_start(a, a.nseq)) return;
-        s = max((all ? count_wave(a.nseq, [&](int i) { return a.qstart[i] <= tok; }) : count_le(a.qstart, a.nseq, tok)) - 1, 0);
+        if (all) s = max(count_wave(a.nseq, [&](int i) { return a.qstart[i] <= tok; }) - 1, 0);
+        else {
+            for (int i = threadIdx.x; i <= a.nseq; i += blockDim.x) M.starts[i] = a.qstart[i];
+            __syncthreads();
+            s = max(count_le(M.starts, a.nseq, tok) - 1, 0);
+        }
+        on = tok < att_start(a, a.nseq);
         t0 = att_start(a, s); tokens = att_start(a, s + 1) - t0;
     }
-    if (tok - t0 >= a.max_q) return;
+    if (!on || tok - t0 >= a.max_q) return;   // (with all: the whole workgroup)
     const int own = min(tokens, a.max_q) * A.group <= A.few ? att_chunks(A, s, tokens).n : A.split, parts = A.parts_sh + own;
     if (parts == 1) return;   // written by the one that had it
     const int64_t rows = (int64_t)a.ntok * a.heads, row = (int64_t)tok * a.heads + head;
@@ -1208,18 +1218,21 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
 #pragma unroll
             for (int i = 0; i < 4; i++) o[i] = fmaf(e, y[i], o[i]);
         }
-        *(f4 *)&acc[gi][x] = o;
+        *(f4 *)&M.acc[gi][x] = o;
         __syncthreads();
         if (gi) return;
-        for (int i = 1; i < gr; i++) o += *(const f4 *)&acc[i][x];
+        for (int i = 1; i < gr; i++) o += *(const f4 *)&M.acc[i][x];
     } else {
-        for (int p = 0; p < parts; p++) { float2 v = A.pm[p * rows + row]; if (v.y != 0.0f) m = fmaxf(m, v.x); }
-#pragma unroll 4
-        for (int p = 0; p < parts; p++) {
-            float2 v = A.pm[p * rows + row];
-            f4 y = v.y != 0.0f ? *(const f4 *)(A.po + (p * rows + row) * D + x) : f4{0, 0, 0, 0};
-            float e = v.y != 0.0f ? exp2_(v.x - m) : 0.0f;
-            sum = fmaf(v.y, e, sum);
+        float2 v[ATT_PER];   // every part's, all loads under way at once
+#pragma unroll
+        for (int p = 0; p < ATT_PER; p++) v[p] = p < parts ? A.pm[p * rows + row] : make_float2(0, 0);
+#pragma unroll
+        for (int p = 0; p < ATT_PER; p++) if (v[p].y != 0.0f) m = fmaxf(m, v[p].x);
+#pragma unroll
+        for (int p = 0; p < ATT_PER; p++) {
+            f4 y = v[p].y != 0.0f ? *(const f4 *)(A.po + (p * rows + row) * D + x) : f4{0, 0, 0, 0};
+            float e = v[p].y != 0.0f ? exp2_(v[p].x - m) : 0.0f;
+            sum = fmaf(v[p].y, e, sum);
 #pragma unroll
             for (int i = 0; i < 4; i++) o[i] = fmaf(e, y[i], o[i]);
         }

@@ -139,35 +139,39 @@ static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
     return 0;
 }
 
-// How a call is divided: row tiles, and runs or chunks of positions where the tiles alone are too few workgroups.
+// How a call is divided: row tiles, and runs or chunks of positions where the tiles alone are too few workgroups. Only the values in the
+// arguments count (a captured call keeps its grid), and few of them: tokens, heads, the bounds.
 struct AttPlan { int few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts; size_t bytes; };
 static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     AttPlan p = {};
     const int group = a.heads / kv.heads;
-    const int64_t rows = (int64_t)a.ntok * group;
-    const int64_t tiles = (rows + ATT_BM - 1) / ATT_BM;
+    const int64_t rows = (int64_t)a.ntok * group, tiles = (rows + ATT_BM - 1) / ATT_BM, most_rows = (int64_t)std::min(a.max_q, a.ntok) * group;
     const int own = a.window && !a.hi ? (int)std::min<int64_t>(a.max_len - a.shared, (int64_t)a.window + a.max_q) : a.max_len - a.shared;
-    // runs of at least `least` positions until there are about `want` workgroups
-    auto runs = [&](int64_t groups, int positions, int want, int least) {
-        int64_t n = (want + groups * kv.heads - 1) / (groups * kv.heads), most = (positions + least - 1) / least;
-        return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(n, most), ATT_PARTS / 2));
+    // Runs of a row tile's positions: about 256 workgroups, half as many again where their runs stay above 2048 positions (a second
+    // workgroup on a CU adds a quarter to its rate, its partial results cost their bytes twice). 960 rows over 40000 positions, 256 / 384 / 512
+    // workgroups: 121 / 114 / 128 us; 256 rows over 16384: 31 / 38 / 56.
+    auto runs = [&](int64_t groups, int positions) {
+        const int64_t wgs = groups * kv.heads, n = (256 + wgs - 1) / wgs, n2 = (384 + wgs - 1) / wgs, most = (positions + 255) / 256;
+        return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(positions / n2 >= 2048 ? n2 : n, most), ATT_PARTS / 2));
     };
+    // Rows of a key/value head that k_attn_few takes: 16 are one product's, 32 over shared positions read them twice (from cache)
     p.few_sh = rows <= 32;
-    if (std::min<int64_t>(a.max_q, a.ntok) * group <= 16 || a.nseq > 1) p.few = 16;
-    // chunks of 512 positions, down to 128 while there are fewer than 512 workgroups, and never more than ATT_PARTS / 2
-    const int64_t few_groups = (a.shared && p.few_sh ? (rows + 15) / 16 * (a.shared / 128) : 0) + (p.few ? a.nseq * (int64_t)(own / 128 + 1) : 0);
-    p.chunk = 512;
-    while (p.chunk > 128 && few_groups * kv.heads * 128 / p.chunk < 512) p.chunk >>= 1;
+    if (most_rows <= 16 || a.nseq > 1) p.few = 16;
+    // Chunks: 1024 positions, down to 256 while there are fewer than 384 workgroups (one sequence of 100000: 256 50.5 us, 512 50.3, 1024 47.6,
+    // 2048 47.9; 64 of up to 3000: 52.2, 49.6, 47.9, 62.5; 7 over 2048 shared: 128 12.9, 256 12.0, 512 13.9), and never more than ATT_PARTS / 2
+    const int64_t units = (a.shared && p.few_sh ? (rows + 15) / 16 * (a.shared / 128) : 0) + (p.few ? a.nseq * (int64_t)(own / 128 + 1) : 0);
+    p.chunk = 1024;
+    while (p.chunk > 256 && units * kv.heads * 128 / p.chunk < 384) p.chunk >>= 1;
     p.chunk = std::max(p.chunk, (std::max(own, a.shared) / (ATT_PARTS / 2 - 1) + 128) & ~127);
     if (a.shared) {
         p.tiles_sh = p.few_sh ? (int)((rows + 15) / 16) : (int)tiles;
-        p.split_sh = p.few_sh ? (a.shared + p.chunk - 1) / p.chunk : runs(tiles, a.shared, 256, 256);
+        p.split_sh = p.few_sh ? (a.shared + p.chunk - 1) / p.chunk : runs(tiles, a.shared);
     }
     if (p.few) p.chunks = std::max(1, (own + 31 + p.chunk - 1) / p.chunk);
     p.split = 1;
-    if (std::min<int64_t>(a.max_q, a.ntok) * group > p.few) {
+    if (most_rows > p.few) {
         p.tiles = (int)tiles + a.nseq;
-        p.split = runs(tiles, own, 256, 256);
+        p.split = runs(tiles, own);
     }
     p.parts = p.split_sh + std::max(p.split, p.chunks);
     p.bytes = 256;
@@ -175,6 +179,7 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     return p;
 }
 
+// d > 0
 static Div divisor(uint32_t d) {
     uint32_t l = 0;
     while (l < 32 && (1ull << l) < d) l++;
@@ -204,7 +209,7 @@ static int att_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPl
     if (!has_tiles ? run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, g, 256, A)
                    : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS>, g, 256, A)) return -1;
     if (p.parts == 1) return 0;
-    const bool few_only = !p.split_sh && p.tiles && p.split == 1, all = p.parts > 8;   // only sequences of few rows have partial results
+    const bool few_only = !p.split_sh && p.tiles && p.split == 1, all = p.parts > ATT_PER;   // only sequences of few rows have partial results
     const unsigned rows = few_only ? 16u * kv.heads * a.nseq : (unsigned)a.ntok * a.heads, lpr = D / 4;
     const unsigned threads = all && p.parts > 64 ? 1024 : 256;
     return run(MMOE_K_ATT_PAGED, k_attn_join<T, D>, all ? rows : (rows + threads / lpr - 1) / (threads / lpr), threads, A, all, few_only);
