@@ -465,8 +465,11 @@ struct AttArgs {
     int split_sh, split, chunk, chunks;   // runs of the shared positions, runs per row tile of the own ones; positions per chunk, most chunks
     int parts_sh;        // partial results of the shared positions: split_sh, or 0
     float s1, s2;        // cap 0: score = s1 q.k in units of log 2; else s2 tanh, with exp(2 z) = exp2(s1 q.k)
-    float *po;           // partial results [parts][ntok * heads][head_dim], each over its own sum: the shared positions', then the own
-    float2 *pm;          // their maxima (in units of log 2) and sums
+    // partial results, [head_dim] values over their own sum each, and their maxima (in units of log 2) and sums: of the shared positions
+    // [split_sh][ntok][heads], from at_tile on of row tiles over the own ones [split][ntok][heads], from at_few on of chunks [chunks][nseq][16 kv heads]
+    float *po;
+    float2 *pm;
+    int64_t at_tile, at_few;
 };
 
 template <int T> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
@@ -879,7 +882,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         if (a.lse && hh == 0) a.lse[(int64_t)R.tok * a.heads + R.head] = sum == 0.0f ? -__builtin_inff() : (mb + __builtin_amdgcn_logf(sum)) * ATT_LN2;
         return;
     }
-    const int64_t row = ((int64_t)((shared ? 0 : A.parts_sh) + split) * a.ntok + R.tok) * a.heads + R.head;
+    const int64_t row = (shared ? 0 : A.at_tile) + ((int64_t)split * a.ntok + R.tok) * a.heads + R.head;
     if (hh == 0) A.pm[row] = make_float2(mb, sum);
     if (sum == 0.0f) return;
     float *o = A.po + row * D + 4 * hh;
@@ -1122,7 +1125,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         if (a.lse && d == 0) a.lse[(int64_t)tok * a.heads + head] = total == 0.0f ? -__builtin_inff() : (mx + __builtin_amdgcn_logf(total)) * ATT_LN2;
         return;
     }
-    const int64_t at_row = ((int64_t)((shared ? 0 : A.parts_sh) + c) * a.ntok + tok) * a.heads + head;
+    const int64_t at_row = shared ? ((int64_t)c * a.ntok + tok) * a.heads + head : A.at_few + ((int64_t)c * a.nseq + at.s) * 16 * A.kv.heads + j * a.heads + head;
     if (d == 0) A.pm[at_row] = make_float2(mx, total);
     if (total == 0.0f) return;
 #pragma unroll
@@ -1181,9 +1184,13 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
         t0 = att_start(a, s); tokens = att_start(a, s + 1) - t0;
     }
     if (!on || tok - t0 >= a.max_q) return;   // (with all: the whole workgroup)
-    const int own = min(tokens, a.max_q) * A.group <= A.few ? att_chunks(A, s, tokens).n : A.split, parts = A.parts_sh + own;
+    const bool few = min(tokens, a.max_q) * A.group <= A.few;
+    const int parts = A.parts_sh + (few ? att_chunks(A, s, tokens).n : A.split);
     if (parts == 1) return;   // written by the one that had it
     const int64_t rows = (int64_t)a.ntok * a.heads, row = (int64_t)tok * a.heads + head;
+    const int64_t own = few ? A.at_few + (int64_t)s * 16 * A.kv.heads + (tok - t0) * a.heads + head : A.at_tile + row;
+    const int64_t by = few ? (int64_t)a.nseq * 16 * A.kv.heads : rows;
+    auto part = [&](int p) { return p < A.parts_sh ? p * rows + row : own + (p - A.parts_sh) * by; };
     float m = -__builtin_inff(), sum = 0.0f;
     f4 o = {0, 0, 0, 0};
     if (all) {
@@ -1192,7 +1199,7 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
 #pragma unroll
         for (int i = 0; i < ATT_PARTS / 256; i++) {
             int p = threadIdx.x + i * blockDim.x;
-            v[i] = p < parts ? A.pm[p * rows + row] : make_float2(0, 0);
+            v[i] = p < parts ? A.pm[part(p)] : make_float2(0, 0);
             if (v[i].y != 0.0f) m = fmaxf(m, v[i].x);
         }
         for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
@@ -1214,7 +1221,7 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
 #pragma unroll 8
         for (int p = gi; p < parts; p += gr) {
             float e = wt[p];
-            f4 y = e != 0.0f ? *(const f4 *)(A.po + (p * rows + row) * D + x) : f4{0, 0, 0, 0};
+            f4 y = e != 0.0f ? *(const f4 *)(A.po + part(p) * D + x) : f4{0, 0, 0, 0};
 #pragma unroll
             for (int i = 0; i < 4; i++) o[i] = fmaf(e, y[i], o[i]);
         }
@@ -1225,12 +1232,12 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
     } else {
         float2 v[ATT_PER];   // every part's, all loads under way at once
 #pragma unroll
-        for (int p = 0; p < ATT_PER; p++) v[p] = p < parts ? A.pm[p * rows + row] : make_float2(0, 0);
+        for (int p = 0; p < ATT_PER; p++) v[p] = p < parts ? A.pm[part(p)] : make_float2(0, 0);
 #pragma unroll
         for (int p = 0; p < ATT_PER; p++) if (v[p].y != 0.0f) m = fmaxf(m, v[p].x);
 #pragma unroll
         for (int p = 0; p < ATT_PER; p++) {
-            f4 y = v[p].y != 0.0f ? *(const f4 *)(A.po + (p * rows + row) * D + x) : f4{0, 0, 0, 0};
+            f4 y = v[p].y != 0.0f ? *(const f4 *)(A.po + part(p) * D + x) : f4{0, 0, 0, 0};
             float e = v[p].y != 0.0f ? exp2_(v[p].x - m) : 0.0f;
             sum = fmaf(v[p].y, e, sum);
 #pragma unroll

@@ -141,7 +141,7 @@ static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
 
 // How a call is divided: row tiles, and runs or chunks of positions where the tiles alone are too few workgroups. Only the values in the
 // arguments count (a captured call keeps its grid), and few of them: tokens, heads, the bounds.
-struct AttPlan { int few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts; size_t bytes; };
+struct AttPlan { int few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts; int64_t at_tile, at_few, entries; size_t bytes; };
 static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     AttPlan p = {};
     const int group = a.heads / kv.heads;
@@ -174,8 +174,11 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
         p.split = runs(tiles, own);
     }
     p.parts = p.split_sh + std::max(p.split, p.chunks);
-    p.bytes = 256;
-    if (p.parts > 1) p.bytes += (size_t)p.parts * a.ntok * a.heads * (kv.head_dim * 4 + 8);
+    const int64_t all = (int64_t)a.ntok * a.heads;
+    p.at_tile = p.split_sh * all;
+    p.at_few = p.at_tile + (p.tiles && (p.split > 1 || p.split_sh) ? p.split * all : 0);
+    p.entries = p.at_few + (p.few && (p.chunks > 1 || p.split_sh) ? (int64_t)p.chunks * a.nseq * 16 * kv.heads : 0);
+    p.bytes = 256 + (size_t)p.entries * (kv.head_dim * 4 + 8);
     return p;
 }
 
@@ -203,7 +206,8 @@ static int att_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPl
     A.s1 = CAP ? 2.0f * a.scale / a.cap * ATT_LOG2E : a.scale * ATT_LOG2E;
     A.s2 = a.cap * ATT_LOG2E;
     A.pm = (float2 *)a.ws;
-    A.po = (float *)((uint8_t *)a.ws + (size_t)p.parts * a.ntok * a.heads * 8);
+    A.po = (float *)((uint8_t *)a.ws + (size_t)(p.entries + 1) / 2 * 16);
+    A.at_tile = p.at_tile; A.at_few = p.at_few;
     const dim3 g(A.n_sh + A.n_tile + A.n_few);
     const bool has_tiles = A.n_tile || (A.n_sh && !A.sh_few);
     if (!has_tiles ? run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, g, 256, A)

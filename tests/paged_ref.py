@@ -166,7 +166,7 @@ class Batch:
     """A batch of sequences over a block cache whose unused places hold NaN, with its device arrays, and the reference result."""
 
     def __init__(self, rng, kind="f16", dim=128, heads=4, kv=1, bs=16, qlens=(1,), lens=(1,), shared=0, window=0, cap=0.0, alibi=False, lo=None,
-                 hi=None, pad=0, token_major=False, width_more=2, max_q=None, max_len=None, spread=1.0, poison=None, lost=(), with_lse=True):
+                 hi=None, pad=0, token_major=False, width_more=2, max_q=None, max_len=None, spread=1.0, poison=None, lost=(), with_lse=True, cut=None):
         self.kind, self.dim, self.heads, self.kv, self.bs, self.qlens, self.lens = kind, dim, heads, kv, bs, list(qlens), list(lens)
         self.shared, self.window, self.cap, self.pad, self.with_lse = shared, window, cap, pad, with_lse
         n, keep = len(lens), shared // bs
@@ -182,7 +182,6 @@ class Batch:
             at += held[s] - keep
         shape = (self.nblocks, bs, kv, dim)
         self.k, self.v = (encode(np.full(shape, np.nan), kind) for _ in range(2))
-        kf, vf = {}, {}
         for s in range(n):
             for p in range(max(lens[s], keep * bs if s == 0 else 0)):
                 b = self.table[s, p // bs]
@@ -194,6 +193,7 @@ class Batch:
             poison(self)
         self.qstart = np.concatenate([[0], np.cumsum(self.qlens)]).astype(np.int32)
         self.ntok = int(self.qstart[-1]) + pad
+        self.cut = self.ntok if cut is None else cut     # tokens the call is told of
         self.q = encode(rng.standard_normal((self.ntok, heads, dim)) * 1.5, kind)
         self.slopes = (2.0 ** (-8.0 * np.arange(1, heads + 1) / heads)).astype(np.float32) if alibi else None
         self.pos = np.concatenate([np.arange(L - ql, L) for ql, L in zip(self.qlens, lens)] + [np.zeros(pad)]).astype(np.int64)
@@ -250,7 +250,7 @@ class Batch:
         self.p_out, self.p_lse = d.put(self.out0), d.put(self.lse0)
         a = M.PagedAttn(q=d.put(qw) + 8 * e, out=self.p_out + 16, lse=self.p_lse if self.with_lse else None, q_token=self.qrow, q_head=dim, out_token=self.orow,
                         out_head=dim + 8, qstart=d.put(self.qstart), len=d.put(np.array(self.lens, np.int32)), table=d.put(self.table), lo=d.put(self.lo),
-                        hi=d.put(self.hi), slopes=d.put(self.slopes), nseq=len(self.lens), ntok=n, heads=h, width=self.width, max_q=self.max_q,
+                        hi=d.put(self.hi), slopes=d.put(self.slopes), nseq=len(self.lens), ntok=self.cut, heads=h, width=self.width, max_q=self.max_q,
                         max_len=self.max_len, shared=self.shared, window=self.window, scale=self.scale, cap=self.cap)
         size = d.lib.mmoe_attn_paged_ws(a, self.cache)
         assert size, d.lib.mmoe_last_error()
@@ -271,6 +271,7 @@ class Batch:
         served = np.zeros(n, bool)
         for s in range(len(self.lens)):
             served[self.qstart[s]:min(self.qstart[s + 1], self.qstart[s] + self.max_q)] = True
+        served[self.cut:] = False
         assert (raw[:, :8] == 0x1234).all() and (raw[:, 8 + h * (dim + 8):] == 0x1234).all() and (body[:, :, dim:] == 0x1234).all(), "written beside the rows"
         assert (raw[~served] == 0x1234).all(), "rows of no token written"
         assert np.array_equal(d.get(self.args.ws + self.args.ws_bytes, self.ws_guard), self.ws_guard), "written behind the workspace"
@@ -278,13 +279,14 @@ class Batch:
         fin = np.isfinite(out[:live])
         assert np.array_equal(np.isnan(got)[sv], np.isnan(out[:live])[sv]), f"NaN at other places {note}"
         same = ~fin & ~np.isnan(out[:live])
+        got, out = np.where(sv[:, None, None], got, 0), np.where(served[:, None, None], out, 0)
         assert np.array_equal(got[same & sv[:, None, None]], out[:live][same & sv[:, None, None]])
         fin &= sv[:, None, None]
-        bad = np.abs(got - out[:live]) > off[:live]
-        bad &= fin
-        worst = (np.abs(got - out[:live])[fin] / np.maximum(off[:live][fin], 1e-30)).max() if fin.any() else 0.0
+        got, out = np.where(fin, got, 0), np.where(fin, out[:live], 0)
+        bad = np.abs(got - out) > off[:live]
+        worst = (np.abs(got - out)[fin] / np.maximum(off[:live][fin], 1e-30)).max() if fin.any() else 0.0
         print(f"  {note}: {live} tokens, error at most {worst:.2f} of the bound", flush=True)
-        assert not bad.any(), (note, np.argwhere(bad)[:5], got[bad][:5], out[:live][bad][:5])
+        assert not bad.any(), (note, np.argwhere(bad)[:5], got[bad][:5], out[bad][:5])
         if self.with_lse:
             gl = d.get(self.p_lse, self.lse0)
             assert (gl[~served] == 77.0).all()

@@ -242,6 +242,10 @@ ATTN = {
                                            dict(qlens=[2, 61], lens=[100, 61], heads=14, kv=2)],
     "a few drafted tokens": dict(qlens=[4, 1, 5, 2], lens=[900, 44, 5, 1030], heads=16, kv=4, kind="bf16", bs=64),
     "sequences without tokens, without positions": dict(qlens=[0, 2, 0, 0, 1, 0], lens=[50, 20, 0, 0, 1, 3000], heads=4, kv=2),
+    "no tokens at all": [dict(qlens=[0, 0], lens=[70, 0], heads=4, kv=2, pad=5), dict(qlens=[0, 0], lens=[70, 64], heads=4, kv=2, pad=5, shared=64),
+                         dict(qlens=[0] * 9, lens=[70] * 9, heads=4, kv=2, pad=50, shared=64, max_q=50)],
+    "starts past the tokens": [dict(qlens=[3, 6], lens=[30, 60], heads=4, kv=1, cut=5), dict(qlens=[30, 60], lens=[30, 60], heads=4, kv=1, cut=50),
+                               dict(qlens=[30, 60], lens=[300, 330], heads=4, kv=1, cut=50, shared=256)],
     "prompts": dict(qlens=[33, 129, 1, 64, 65], lens=[33, 129, 1, 64, 65], heads=8, kv=2),
     "a prompt, heads of 64": dict(qlens=[300], lens=[300], heads=4, kv=4, dim=64, kind="bf16", bs=64),
     "chunks after cached positions": dict(qlens=[100, 17, 40], lens=[612, 17, 1025], heads=4, kv=1, kind="bf16", bs=128),
@@ -298,3 +302,223 @@ def test_attention(name):
             a = b.upload(d)
             M.check(d.lib.mmoe_attn_paged(a, b.cache), "attention")
             b.check(d, name)
+
+
+def test_attention_of_most_sequences():
+    rng = np.random.default_rng(4)
+    for shared in (0, 32):
+        b = Batch(rng, qlens=[1] * M.KV_MAXSEQ, lens=[shared + 1 + s % 3 for s in range(M.KV_MAXSEQ)], shared=shared, heads=2, kv=1, dim=64)
+        with Dev() as d:
+            a = b.upload(d)
+            M.check(d.lib.mmoe_attn_paged(a, b.cache), "attention")
+            b.check(d, f"4096 sequences, {shared} shared")
+
+
+def test_offsets_past_32_bits():
+    """a cache whose blocks lie 2^25 values apart: the last one begins at byte 8.6e9"""
+    rng = np.random.default_rng(8)
+    n, bs, dim, kv, heads, apart = 129, 16, 64, 1, 4, 1 << 25
+    lens, qlens = [2000, 40], [1, 30]
+    b = Batch(rng, qlens=qlens, lens=lens, heads=heads, kv=kv, dim=dim, bs=bs, kind="bf16")
+    assert b.nblocks > 128
+    with Dev() as d:
+        a = b.upload(d)
+        c = b.cache
+        c.block_stride = apart
+        c.k = d.room((b.nblocks - 1) * apart * 2 + bs * dim * 2 + 4096)
+        c.v = c.k + bs * dim * 2
+        for i in range(b.nblocks):
+            d.write(c.k + i * apart * 2, b.k[i].transpose(1, 0, 2))
+            d.write(c.v + i * apart * 2, b.v[i].transpose(1, 0, 2))
+        M.check(d.lib.mmoe_attn_paged(a, c), "attention")
+        b.check(d, "far blocks")
+        # and the write of keys and values
+        x = encode(rng.standard_normal((3, 3 * dim)), "bf16")
+        slot = np.array([(b.nblocks - 1) * bs + 3, 5, (b.nblocks - 2) * bs], np.int32)
+        px = d.put(x)
+        r = M.Rope(q=px, k=px + dim * 2, v=px + 2 * dim * 2, q_out=d.room(4096), q_token=3 * dim, q_head=dim, k_token=3 * dim, k_head=dim, v_token=3 * dim, v_head=dim,
+                   qo_token=dim, qo_head=dim, pos=d.put(np.zeros(3, np.int32)), slot=d.put(slot), freq=d.put(np.ones(dim // 2)), ntok=3, heads=1, kv_heads=1,
+                   head_dim=dim, rot=dim, in_dtype=M.BF16, out_dtype=M.BF16, mag=1.0)
+        M.check(d.lib.mmoe_rope_kv(r, c), "rope")
+        for t, s in enumerate(slot.tolist()):   # position 0: the rotation changes nothing
+            row = d.get(c.v + (s // bs * apart + s % bs * dim) * 2, np.zeros(dim, np.uint16))
+            assert np.array_equal(row, x[t, 2 * dim:])
+            row = d.get(c.k + (s // bs * apart + s % bs * dim) * 2, np.zeros(dim, np.uint16))
+            assert np.array_equal(row, x[t, dim:2 * dim])
+
+
+class Server:
+    """Sequences that come and go over one layer's blocks: the three operators together, step by step, and what they should hold"""
+    H, KV, D, BS, ROT, N, WIDTH, NB = 8, 2, 128, 16, 64, 6, 24, 80
+
+    def __init__(self, d, rng, ntok):
+        self.d, self.rng, self.ntok, h, kv, dim = d, rng, ntok, self.H, self.KV, self.D
+        freq = np.zeros(self.ROT // 2)
+        M.check(d.lib.mmoe_rope_freqs(self.ROT, 10000.0, 1.0, 0, 0.0, 0.0, M.ptr(freq)), "freqs")
+        self.freq, n, w = freq, self.N, self.WIDTH
+        self.seen = [[] for _ in range(n)]       # (key, value) of each cached position, as the cache holds them
+        z = lambda *s: np.zeros(s, np.int32)  # noqa: E731
+        self.len, self.add, self.done, self.table = d.put(z(n)), d.put(z(n)), d.put(z(n)), d.put(z(n, w) - 1)
+        self.free, self.nfree = d.put(np.arange(self.NB, dtype=np.int32)), d.put(np.array([self.NB], np.int32))
+        self.qstart, self.pos, self.slot = d.put(z(n + 1)), d.put(z(ntok)), d.put(z(ntok))
+        self.row = (h + 2 * kv) * dim
+        self.x, self.q, self.out = d.room(ntok * self.row * 4), d.room(ntok * h * dim * 2), d.room(ntok * h * dim * 2)
+        shape = (self.NB, kv, self.BS, dim)
+        self.kc, self.vc, self.shape = d.put(encode(np.full(shape, np.nan), "f16")), d.put(encode(np.full(shape, np.nan), "f16")), shape
+        self.cache = M.KvCache(k=self.kc, v=self.vc, block_stride=kv * self.BS * dim, head_stride=self.BS * dim, token_stride=dim, nblocks=self.NB, block_size=self.BS,
+                               heads=kv, head_dim=dim, dtype=M.F16)
+        self.plan = M.KvPlan(ctx=self.len, add=self.add, done=self.done, table=self.table, free_list=self.free, nfree=self.nfree, nfree_out=self.nfree, len=self.len,
+                             qstart=self.qstart, pos=self.pos, slot=self.slot, nseq=n, width=w, nblocks=self.NB, block_size=self.BS, ntok=ntok)
+        self.rope = M.Rope(q=self.x, k=self.x + h * dim * 4, v=self.x + (h + kv) * dim * 4, q_out=self.q, q_token=self.row, q_head=dim, k_token=self.row, k_head=dim,
+                           v_token=self.row, v_head=dim, qo_token=h * dim, qo_head=dim, pos=self.pos, slot=self.slot, freq=d.put(freq), ntok=ntok, heads=h, kv_heads=kv,
+                           head_dim=dim, rot=self.ROT, in_dtype=M.F32, out_dtype=M.F16, mag=1.0)
+        self.attn = M.PagedAttn(q=self.q, out=self.out, q_token=h * dim, q_head=dim, out_token=h * dim, out_head=dim, qstart=self.qstart, len=self.len, table=self.table,
+                                nseq=n, ntok=ntok, heads=h, width=w, max_q=ntok, max_len=w * self.BS, scale=dim ** -0.5)
+        size = d.lib.mmoe_attn_paged_ws(self.attn, self.cache)
+        self.attn.ws, self.attn.ws_bytes = d.room(size), size
+
+    def queue(self):
+        lib = self.d.lib
+        M.check(lib.mmoe_kv_plan(self.plan), "plan")
+        M.check(lib.mmoe_rope_kv(self.rope, self.cache), "rope")
+        M.check(lib.mmoe_attn_paged(self.attn, self.cache), "attention")
+
+    def feed(self, add, done):
+        self.add_now, self.done_now = add, done
+        self.x_now = self.rng.standard_normal((self.ntok, self.row)).astype(np.float32)
+        self.d.write(self.add, np.array(add, np.int32)); self.d.write(self.done, np.array(done, np.int32)); self.d.write(self.x, self.x_now)
+
+    def check(self, note):
+        from paged_ref import attend
+        d, h, kv, dim, n = self.d, self.H, self.KV, self.D, self.N
+        table, start, length = d.get(self.table, np.zeros((n, self.WIDTH), np.int32)), d.get(self.qstart, np.zeros(n + 1, np.int32)), d.get(self.len, np.zeros(n, np.int32))
+        kc, vc = (decode(d.get(p, np.zeros(self.shape, np.uint16)), "f16") for p in (self.kc, self.vc))
+        out = decode(d.get(self.out, np.zeros((self.ntok, h, dim), np.uint16)), "f16")
+        q = decode(d.get(self.q, np.zeros((self.ntok, h, dim), np.uint16)), "f16")
+        x = self.x_now.reshape(self.ntok, h + 2 * kv, dim).astype(np.float64)
+        used = []
+        for s in range(n):
+            if self.done_now[s]:
+                self.seen[s] = []
+            t = np.arange(start[s], start[s + 1])
+            assert len(t) == self.add_now[s]
+            p = len(self.seen[s]) + np.arange(len(t))
+            want_k, want_q = rotate(x[t, h:h + kv], p, self.freq, self.ROT, 0, 1.0), rotate(x[t, :h], p, self.freq, self.ROT, 0, 1.0)
+            assert (np.abs(q[t] - want_q) <= HALF["f16"] * np.abs(want_q) + 2.0 ** -19).all(), note
+            self.seen[s] += [(a, b) for a, b in zip(want_k, x[t, h + kv:])]
+            assert length[s] == len(self.seen[s]), (note, s)
+            if not len(self.seen[s]):
+                continue
+            at = np.arange(length[s])
+            blocks = table[s, at // self.BS]
+            used += sorted(set(blocks.tolist()))
+            k, v = kc[blocks, :, at % self.BS], vc[blocks, :, at % self.BS]
+            wk, wv = np.array([a for a, _ in self.seen[s]]), np.array([b for _, b in self.seen[s]])
+            assert (np.abs(k - wk) <= HALF["f16"] * np.abs(wk) + 2.0 ** -19).all() and (np.abs(v - wv) <= HALF["f16"] * np.abs(wv) + 2.0 ** -25).all(), (note, s)
+            if len(t):
+                o, _, off, _ = attend(q[t], k, v, p, at <= p[:, None], dim ** -0.5, 0.0, None, HALF["f16"])
+                assert (np.abs(out[t] - o) <= off).all(), (note, s, np.abs(out[t] - o).max())
+        assert len(used) == len(set(used)), "a block in two tables"
+        assert d.get(self.nfree, np.zeros(1, np.int32))[0] == self.NB - len(used), note
+        print(f"  {note}: lengths {length.tolist()}", flush=True)
+
+
+def test_steps_of_a_server():
+    """prompts, then single tokens, sequences that end and others that begin in their rows"""
+    with Dev() as d:
+        s = Server(d, np.random.default_rng(21), 260)
+        for i, (add, done) in enumerate([([100, 7, 0, 33, 1, 0], [0] * 6), ([1, 1, 60, 1, 1, 0], [0] * 6), ([1, 1, 1, 1, 1, 140], [0] * 6), ([1, 0, 1, 40, 1, 1], [0, 1, 0, 1, 0, 0]),
+                                         ([1, 90, 1, 1, 0, 1], [0] * 6), ([0] * 6, [1, 0, 0, 0, 1, 0]), ([150, 1, 1, 1, 1, 1], [0] * 6)]):
+            s.feed(add, done)
+            s.queue()
+            s.check(f"step {i}")
+
+
+def test_captured_step_replayed_with_others_between():
+    """one step captured into a graph, replayed for growing, ending and new sequences, with eager steps of another server between"""
+    with Dev() as d:
+        s, other = Server(d, np.random.default_rng(5), 6), Server(d, np.random.default_rng(6), 200)
+        s.feed([1, 1, 0, 1, 1, 1], [0] * 6)
+        s.queue()
+        s.check("eager")
+        hip = C.CDLL("libamdhip64.so")
+        stream, graph, ex = C.c_void_p(d.lib.mmoe_stream()), C.c_void_p(), C.c_void_p()
+        assert hip.hipStreamBeginCapture(stream, 1) == 0
+        s.queue()
+        assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(C.byref(ex), graph, None, None, C.c_size_t(0)) == 0
+        try:
+            for i in range(20):
+                done = [1 if (i * 5 + j) % 11 == 0 else 0 for j in range(6)]
+                s.feed([0 if (i + j) % 7 == 0 else 1 for j in range(6)], done)
+                assert hip.hipGraphLaunch(ex, stream) == 0
+                s.check(f"replay {i}")
+                if i % 4 == 0:
+                    other.feed([20, 0, 5, 1, 30, 1], [1, 1, 0, 1, 1, 0] if i else [0] * 6)
+                    other.queue()
+                    other.check(f"eager between, {i}")
+        finally:
+            hip.hipGraphExecDestroy(ex); hip.hipGraphDestroy(graph)
+
+
+def test_two_calls_at_once_with_workspaces_of_their_own():
+    """two captured attention calls replayed on two other streams at the same time"""
+    rng = np.random.default_rng(31)
+    bs = [Batch(rng, qlens=[1] * 5, lens=[900 + 100 * i for i in range(5)], heads=8, kv=2), Batch(rng, qlens=[1, 3, 60], lens=[700, 800, 900], shared=512, heads=8, kv=2, kind="bf16")]
+    hip = C.CDLL("libamdhip64.so")
+    with Dev() as d:
+        made = []
+        for b in bs:
+            a = b.upload(d)
+            lib_stream, graph, ex, st = C.c_void_p(d.lib.mmoe_stream()), C.c_void_p(), C.c_void_p(), C.c_void_p()
+            assert hip.hipStreamBeginCapture(lib_stream, 1) == 0
+            M.check(d.lib.mmoe_attn_paged(a, b.cache), "attention")
+            assert hip.hipStreamEndCapture(lib_stream, C.byref(graph)) == 0
+            assert hip.hipGraphInstantiate(C.byref(ex), graph, None, None, C.c_size_t(0)) == 0
+            assert hip.hipStreamCreate(C.byref(st)) == 0
+            made.append((graph, ex, st))
+        try:
+            assert hip.hipDeviceSynchronize() == 0
+            for i in range(30):
+                for _, ex, st in made:
+                    assert hip.hipGraphLaunch(ex, st) == 0
+            assert hip.hipDeviceSynchronize() == 0
+            for b in bs:
+                b.check(d, "two at once")
+        finally:
+            for graph, ex, st in made:
+                hip.hipGraphExecDestroy(ex); hip.hipGraphDestroy(graph); hip.hipStreamDestroy(st)
+
+
+def test_results_repeat_and_do_not_depend_on_the_workspace():
+    rng = np.random.default_rng(77)
+    for kw in (dict(qlens=[1, 2, 70], lens=[5000, 600, 700], heads=8, kv=2), dict(qlens=[1] * 9, lens=[1500 + s for s in range(9)], shared=1024, heads=16, kv=4, kind="bf16")):
+        b = Batch(rng, **kw)
+        with Dev() as d:
+            a = b.upload(d)
+            got = []
+            for fill in (0, 0xff, 0x7f):
+                d.write(a.ws, np.full(a.ws_bytes, fill, np.uint8))
+                M.check(d.lib.mmoe_attn_paged(a, b.cache), "attention")
+                got.append(d.get(b.p_out, b.out0))
+            assert all(np.array_equal(g, got[0]) for g in got[1:])
+            b.check(d, "workspace of any content")
+            a.ws_bytes -= 1
+            assert d.lib.mmoe_attn_paged(a, b.cache) == -1 and b"workspace" in d.lib.mmoe_last_error()
+            a.ws_bytes += 1
+
+
+def test_profile_counts_the_operators():
+    rng = np.random.default_rng(1)
+    b = Batch(rng, qlens=[1], lens=[100], heads=4, kv=1)
+    with Dev() as d:
+        a = b.upload(d)
+        ms, cnt = C.c_double(), C.c_long()
+        M.check(d.lib.mmoe_prof_reset(), "reset"); M.check(d.lib.mmoe_prof(1), "prof")
+        try:
+            M.check(d.lib.mmoe_attn_paged(a, b.cache), "attention")
+        finally:
+            M.check(d.lib.mmoe_prof(0), "prof off")
+        M.check(d.lib.mmoe_prof_get(M.KERNELS.index("att_paged"), C.byref(ms), C.byref(cnt)), "get")
+        assert cnt.value == 1 and 0 < ms.value < 50
+        b.check(d, "profiled")
