@@ -64,7 +64,7 @@ ATTN = [
     (dict(ntok=1 << 28), {}, b"tokens"), (dict(width=0), {}, b"tables"), (dict(width=1 << 27), {}, b"tables"), (dict(max_q=-1), {}, b"max_q"), (dict(max_len=-1), {}, b"max_len"),
     (dict(max_len=129), {}, b"max_len"), (dict(shared=8), {}, b"shared"), (dict(shared=-16), {}, b"shared"), (dict(shared=112), {}, b"shared"), (dict(window=-1), {}, b"window"),
     (dict(scale=float("inf")), {}, b"scale"), (dict(scale=0.0), {}, b"scale"), (dict(scale=-0.1), {}, b"scale"), (dict(cap=-1.0), {}, b"cap"), (dict(cap=float("nan")), {}, b"cap"), (dict(q_head=4), {}, b"strides"), (dict(out_token=-8), {}, b"strides"),
-    ({}, dict(dtype=M.F32), b"cache type"), ({}, dict(token_stride=(1 << 26) + 8), b"stride"), ({}, dict(head_dim=96), b"head_dim"), ({}, dict(head_dim=256), b"head_dim"), ({}, dict(block_size=17), b"block size"),
+    ({}, dict(dtype=M.F32), b"cache type"), ({}, dict(token_stride=(1 << 26) + 8), b"stride"), ({}, dict(head_dim=96), b"head_dim"), ({}, dict(head_dim=256, token_stride=256), b"head_dim"), ({}, dict(token_stride=120), b"stride"), ({}, dict(block_size=17), b"block size"),
     ({}, dict(k=None), b"set"), ({}, dict(nblocks=0), b"blocks")]
 
 
