@@ -275,14 +275,15 @@ int mmoe_selftest_silu(uint32_t lo, uint32_t n, unsigned long long *nbad, uint32
  * the library stream (mmoe_stream) without waiting, so data that another stream writes or reads has to be ordered with it
  * (an event, or a wait). The device that is current in the caller is left as it was. The calls allocate nothing and can be
  * captured into a graph; what the host passes by value (counts, bounds) is then fixed, what it passes in device memory is read at each replay.
- * A refused call returns -1 and queues nothing. No call keeps anything between calls. */
+ * A refused call returns -1 and queues nothing. No call keeps anything between calls. Limits: 2^30 positions per sequence, 2^23
+ * tokens per call. */
 #define MMOE_F32 0
 #define MMOE_F16 1
 #define MMOE_BF16 2
 #define MMOE_KV_MAXSEQ 4096      /* sequences per call */
 
 /* A layer's keys and values: head_dim consecutive values at k (v) + block * block_stride + head * head_stride + (position in
- * the block) * token_stride, strides in values, multiples of 8 (token_stride up to 2^26);
+ * the block) * token_stride, strides in values, multiples of 8 (token_stride from head_dim to 2^26);
  * pointers aligned to 16 bytes. block_size: a power of two, 16 to 1024. */
 typedef struct {
     void *k, *v;
@@ -339,8 +340,8 @@ int mmoe_rope_kv(const mmoe_rope_args *a, const mmoe_kv_cache *kv);
 
 /* Attention of nseq sequences over their blocks. Sequence s has the tokens qstart[s] .. qstart[s + 1] - 1 of q [ntok][heads][head_dim]
  * (none, one or many), its last ones of len[s] positions; query head h reads key/value head h / (heads / kv heads).
- * head_dim 64 or 128; q, out and the cache of one type, MMOE_F16 or MMOE_BF16; scores, softmax and sums in 32 bits.
- *   score of position p for the token at position i:  x = scale q.k (scale > 0);  cap > 0: x = cap tanh(x / cap);
+ * head_dim 64 or 128; q, out and the cache of one type, MMOE_F16 or MMOE_BF16; scores, softmax and sums in 32 bits. ntok heads at most 2^30.
+ *   score of position p for the token at position i:  x = scale q.k (scale > 0);  cap > 0 (at most 1024): x = cap tanh(x / cap);
  *   slopes != NULL: x -= slopes[h] |i - p|
  *   visible: max(lo[t], i - window) <= p < min(hi[t], len[s]); lo NULL: 0; hi NULL: i + 1 (causal); window 0: unlimited
  * lo and hi are per token: a document mask gives each token its document's first position, a prefix mask lets hi reach past
@@ -348,9 +349,9 @@ int mmoe_rope_kv(const mmoe_rope_args *a, const mmoe_kv_cache *kv);
  * nothing, or whose scores are all -inf, gets 0 and -inf. A key or value that a token does not see never reaches it, whatever it
  * holds (cache never written, infinities, NaN). Positions whose block id is not in 0 .. nblocks - 1 are seen by none.
  * out rows and lse from qstart[nseq] on stay as they are.
- * shared > 0 (a multiple of block_size): the first shared positions are the same blocks in every table row (row 0's are read) and in every
- * sequence (len[s] >= shared): they are read once for all sequences instead of once for each. The result is the same.
- * max_q and max_len bound the tokens and positions (at most 2^30) of one sequence (they choose the kernels and their grids); more tokens or positions than
+ * shared > 0 (a multiple of block_size): the first shared positions are the same blocks in every table row (row 0's are read):
+ * they are read once for all sequences instead of once for each. The result is the same.
+ * max_q and max_len bound the tokens and positions of one sequence (they choose the kernels and their grids); more tokens or positions than
  * that are not served: tokens past max_q keep their out rows, positions past max_len are not seen.
  * ws: mmoe_attn_paged_ws bytes (0: refused; it depends on the values in a and kv, not on what pointers point to), aligned to 256; its content
  * need not survive. Calls that can run at the same time (graphs replayed on several streams) need their own. */

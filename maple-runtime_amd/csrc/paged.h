@@ -476,6 +476,9 @@ template <int T> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
     if (T == MMOE_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
 }
+// Weights are 2^(x - m + lift): in fp16 their smallest step is 2^-24, which a tail of many small weights would be rounded to; lifted by 2^7
+// (they reach 2^15 before the maximum m follows) it is 2^-31 of the largest weight. Sums and results carry the same factor.
+template <int T> constexpr float lift = T == MMOE_F16 ? 7.0f : 0.0f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // the larger of two numbers, without fmaxf's quieting of each (a NaN shows in the weights, whatever the maximum then is)
 __device__ __forceinline__ float max_(float x, float y) { return __builtin_amdgcn_fmed3f(x, y, __builtin_inff()); }
@@ -691,7 +694,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     for (int i = 0; i < DS; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
-    float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f;   // mb: m, 0 while that is -inf
+    float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f;   // mb: m - lift, - lift while m is -inf
     constexpr bool MATH = CAP || BIAS;
     const float s1 = MATH ? 1.0f : A.s1;
 
@@ -744,11 +747,11 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
             for (int j = 0; j < 16; j++) top[j & 3] = u || j > 3 ? max_(top[j & 3], s[u][j]) : s[u][j];
         return max_halves(max_(max_(top[0], top[1]), max_(top[2], top[3]))) * s1;
     };
-    // a new maximum only once it is 2^8 past the old: until then weights stay below 2^8, in every type's range
+    // a new maximum only once it is 2^8 past the old: until then weights stay below 2^8 (lifted: 2^15), in every type's range
     auto rescale = [&](float mt) {
         if (!__any(mt > m + 8.0f)) return;
         float mn = fmaxf(m, mt), bn = mn == -__builtin_inff() ? 0.0f : mn, al = exp2_(m - bn);
-        m = mn; mb = bn; sum *= al;
+        m = mn; mb = bn - lift<T>; sum *= al;
 #pragma unroll
         for (int i = 0; i < DS; i++)
 #pragma unroll
@@ -767,14 +770,16 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         for (int i = 0; i < DS; i++) f0[i] = value(i, 0);
         __builtin_amdgcn_sched_barrier(0);
         u4 pf[4];
+        float part = 0;
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
                 float e0 = exp2_(fmaf(sc[u][j], s1, -mb)), e1 = exp2_(fmaf(sc[u][j + 1], s1, -mb));
-                sum += e0 + e1;
+                part += e0 + e1;
                 pf[2 * u + (j >> 3)][(j & 7) >> 1] = pack2<T>(e0, e1);
             }
+        sum += part;   // tile by tile: a long sum of small ones
 #pragma unroll
         for (int k = 0; k < 4; k++)
 #pragma unroll
@@ -1020,7 +1025,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         mt = max_quarters(mt);
         if (__any(mt > m + 8.0f)) {
             float mn = fmaxf(m, mt), bn = mn == -__builtin_inff() ? 0.0f : mn, al = exp2_(m - bn);
-            m = mn; mb = bn; sum *= al;
+            m = mn; mb = bn - lift<T>; sum *= al;
 #pragma unroll
             for (int e = 0; e < E; e++) acc[e] *= al;
         }
@@ -1183,7 +1188,7 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
         on = tok < att_start(a, a.nseq);
         t0 = att_start(a, s); tokens = att_start(a, s + 1) - t0;
     }
-    if (!on || tok - t0 >= a.max_q) return;   // (with all: the whole workgroup)
+    if (!on || tok < t0 || tok - t0 >= min(tokens, a.max_q)) return;   // (with all: the whole workgroup)
     const bool few = min(tokens, a.max_q) * A.group <= A.few;
     const int parts = A.parts_sh + (few ? att_chunks(A, s, tokens).n : A.split);
     if (parts == 1) return;   // written by the one that had it

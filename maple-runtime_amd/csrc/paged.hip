@@ -26,14 +26,18 @@ struct OnDevice {
     bool ok = true;
     OnDevice() {
         int d = 0;
-        if (hipGetDevice(&d) != hipSuccess) { ok = false; return; }
-        if (d != mm_device()) { prev = d; ok = hipSetDevice(mm_device()) == hipSuccess; }
+        ok = hipGetDevice(&d) == hipSuccess;
+        if (ok && d != mm_device()) { prev = d; ok = hipSetDevice(mm_device()) == hipSuccess; }
         if (!ok) mm_error("device %d of the library cannot be made current", mm_device());
     }
     ~OnDevice() { if (prev >= 0) (void)hipSetDevice(prev); }
 };
 
 #define REFUSE(...) do { mm_error(__VA_ARGS__); return -1; } while (0)
+#define MAX_LEN (1 << 30)      // positions of a sequence: positions and a tile's end are 32-bit integers everywhere
+#define MAX_TOKENS (1 << 23)   // tokens of a call, of 256 threads each in a launch; with heads, 2^30 rows: a tile's end is a 32-bit integer too
+#define MAX_CAP 1024           // its error is 2^-22 of it: below half a step of fp16 in the weights
+#define MAX_THREADS 0xffffffffull   // of a launch
 static bool apart(const void *p, uintptr_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
 static int log2_block(int bs) {   // -1: not a block size
     for (int s = 4; s <= 10; s++) if (bs == 1 << s) return s;
@@ -60,9 +64,9 @@ int mmoe_kv_plan(const mmoe_kv_plan_args *p) {
     int sh = log2_block(a.block_size);
     if (sh < 0) REFUSE("mmoe_kv_plan: block size %d is not a power of two from 16 to 1024", a.block_size);
     if (a.nseq < 0 || a.nseq > MMOE_KV_MAXSEQ) REFUSE("mmoe_kv_plan: %d sequences outside 0..%d", a.nseq, MMOE_KV_MAXSEQ);
-    if (a.ntok < 0) REFUSE("mmoe_kv_plan: %d tokens", a.ntok);
+    if (a.ntok < 0 || a.ntok > MAX_TOKENS) REFUSE("mmoe_kv_plan: %d tokens", a.ntok);
     if (a.nblocks < 0 || (int64_t)a.nblocks * a.block_size > INT32_MAX) REFUSE("mmoe_kv_plan: %d blocks of %d positions", a.nblocks, a.block_size);
-    if (a.width < 1 || (int64_t)a.width * a.block_size > INT32_MAX) REFUSE("mmoe_kv_plan: tables of %d blocks of %d positions", a.width, a.block_size);
+    if (a.width < 1 || (int64_t)a.width * a.block_size > MAX_LEN) REFUSE("mmoe_kv_plan: tables of %d blocks of %d positions", a.width, a.block_size);
     if (a.shared < 0 || a.shared % a.block_size || a.shared / a.block_size > a.width)
         REFUSE("mmoe_kv_plan: %d shared positions (block size %d, %d blocks per table)", a.shared, a.block_size, a.width);
     if (!a.nfree || !a.nfree_out || !a.qstart || (a.nseq && (!a.ctx || !a.add || !a.table || !a.len)) || (a.nblocks && !a.free_list) ||
@@ -127,13 +131,13 @@ static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
     if (kv->head_dim != 64 && kv->head_dim != 128) REFUSE("mmoe_attn_paged: head_dim %d is not 64 or 128", kv->head_dim);
     if (a.heads < 1 || a.heads > 65535 || a.heads % kv->heads) REFUSE("mmoe_attn_paged: %d query heads over %d key/value heads", a.heads, kv->heads);
     if (a.nseq < 0 || a.nseq > MMOE_KV_MAXSEQ) REFUSE("mmoe_attn_paged: %d sequences outside 0..%d", a.nseq, MMOE_KV_MAXSEQ);
-    if (a.ntok < 0 || (int64_t)a.ntok * a.heads > INT32_MAX) REFUSE("mmoe_attn_paged: %d tokens", a.ntok);
-    if (a.width < 1 || (int64_t)a.width * kv->block_size > INT32_MAX) REFUSE("mmoe_attn_paged: tables of %d blocks", a.width);
-    if (a.max_q < 0 || a.max_len < 0 || a.max_len > (int64_t)a.width * kv->block_size || a.max_len > 1 << 30)
+    if (a.ntok < 0 || a.ntok > MAX_TOKENS || (int64_t)a.ntok * a.heads > 1 << 30) REFUSE("mmoe_attn_paged: %d tokens", a.ntok);
+    if (a.width < 1 || (int64_t)a.width * kv->block_size > MAX_LEN) REFUSE("mmoe_attn_paged: tables of %d blocks", a.width);
+    if (a.max_q < 0 || a.max_len < 0 || a.max_len > (int64_t)a.width * kv->block_size)
         REFUSE("mmoe_attn_paged: max_q %d, max_len %d (tables of %d blocks)", a.max_q, a.max_len, a.width);
     if (a.shared < 0 || a.shared % kv->block_size || a.shared > a.max_len) REFUSE("mmoe_attn_paged: %d shared positions (block size %d, max_len %d)", a.shared, kv->block_size, a.max_len);
     if (a.window < 0) REFUSE("mmoe_attn_paged: window %d", a.window);
-    if (!(a.scale > 0) || !isfinite(a.scale) || !isfinite(a.cap) || a.cap < 0) REFUSE("mmoe_attn_paged: scale %g, cap %g", a.scale, a.cap);
+    if (!(a.scale > 0) || !isfinite(a.scale) || !(a.cap >= 0) || a.cap > MAX_CAP || (a.cap > 0 && !isfinite(4.0f * a.scale / a.cap))) REFUSE("mmoe_attn_paged: scale %g, cap %g", a.scale, a.cap);
     if (a.q_token < 0 || a.q_head < 0 || a.out_token < 0 || a.out_head < 0 || ((a.q_token | a.q_head | a.out_token | a.out_head) & 7))
         REFUSE("mmoe_attn_paged: strides must be multiples of 8");
     return 0;
@@ -141,7 +145,12 @@ static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
 
 // How a call is divided: row tiles, and runs or chunks of positions where the tiles alone are too few workgroups. Only the values in the
 // arguments count (a captured call keeps its grid), and few of them: tokens, heads, the bounds.
-struct AttPlan { int few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts; int64_t at_tile, at_few, entries; size_t bytes; };
+struct AttPlan {
+    int few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts;
+    int64_t at_tile, at_few, entries, wgs, join_wgs;
+    int join_all, join_few, join_threads;
+    size_t bytes;
+};
 static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     AttPlan p = {};
     const int group = a.heads / kv.heads;
@@ -179,6 +188,12 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     p.at_few = p.at_tile + (p.tiles && (p.split > 1 || p.split_sh) ? p.split * all : 0);
     p.entries = p.at_few + (p.few && (p.chunks > 1 || p.split_sh) ? (int64_t)p.chunks * a.nseq * 16 * kv.heads : 0);
     p.bytes = 256 + (size_t)p.entries * (kv.head_dim * 4 + 8);
+    p.wgs = (int64_t)kv.heads * ((int64_t)p.tiles_sh * p.split_sh + (int64_t)p.tiles * p.split + (int64_t)p.chunks * a.nseq);
+    p.join_few = !p.split_sh && p.tiles && p.split == 1;   // only sequences of few rows have partial results
+    p.join_all = p.parts > ATT_PER;
+    p.join_threads = p.join_all && p.parts > 64 ? 1024 : 256;
+    const int64_t jr = p.join_few ? 16ll * kv.heads * a.nseq : all, per = p.join_threads / (kv.head_dim / 4);
+    p.join_wgs = p.join_all ? jr : (jr + per - 1) / per;
     return p;
 }
 
@@ -213,10 +228,7 @@ static int att_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPl
     if (!has_tiles ? run(MMOE_K_ATT_PAGED, k_attn_few<T, D, CAP, BIAS>, g, 256, A)
                    : run(MMOE_K_ATT_PAGED, k_attn_tile<T, D, CAP, BIAS>, g, 256, A)) return -1;
     if (p.parts == 1) return 0;
-    const bool few_only = !p.split_sh && p.tiles && p.split == 1, all = p.parts > ATT_PER;   // only sequences of few rows have partial results
-    const unsigned rows = few_only ? 16u * kv.heads * a.nseq : (unsigned)a.ntok * a.heads, lpr = D / 4;
-    const unsigned threads = all && p.parts > 64 ? 1024 : 256;
-    return run(MMOE_K_ATT_PAGED, k_attn_join<T, D>, all ? rows : (rows + threads / lpr - 1) / (threads / lpr), threads, A, all, few_only);
+    return run(MMOE_K_ATT_PAGED, k_attn_join<T, D>, (unsigned)p.join_wgs, p.join_threads, A, p.join_all, p.join_few);
 }
 template <int T, int D>
 static int att_pick(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const AttPlan &p) {
@@ -232,7 +244,7 @@ int mmoe_rope_kv(const mmoe_rope_args *p, const mmoe_kv_cache *kv) {
     if (a.in_dtype < MMOE_F32 || a.in_dtype > MMOE_BF16 || a.out_dtype < MMOE_F32 || a.out_dtype > MMOE_BF16) REFUSE("mmoe_rope_kv: types %d, %d", a.in_dtype, a.out_dtype);
     if (a.head_dim < 8 || a.head_dim > 256 || a.head_dim % 8) REFUSE("mmoe_rope_kv: head_dim %d is not a multiple of 8 up to 256", a.head_dim);
     if (a.rot < 0 || a.rot > a.head_dim || (a.rot & 1)) REFUSE("mmoe_rope_kv: %d rotated dims of %d", a.rot, a.head_dim);
-    if (a.ntok < 0 || a.heads < 0 || a.heads > 65535 || a.kv_heads < 0 || a.kv_heads > 1024) REFUSE("mmoe_rope_kv: %d tokens, %d heads, %d key/value heads", a.ntok, a.heads, a.kv_heads);
+    if (a.ntok < 0 || a.ntok > MAX_TOKENS || a.heads < 0 || a.heads > 65535 || a.kv_heads < 0 || a.kv_heads > 1024) REFUSE("mmoe_rope_kv: %d tokens, %d heads, %d key/value heads", a.ntok, a.heads, a.kv_heads);
     if (!isfinite(a.mag)) REFUSE("mmoe_rope_kv: mag %g", a.mag);
     int sh = 0;
     if (kv) {
@@ -268,6 +280,8 @@ int mmoe_attn_paged(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
     if (!a.q || !a.out || !a.qstart || !a.len || !a.table) REFUSE("mmoe_attn_paged: a pointer is missing");
     if (apart(a.q, 16) || apart(a.out, 16)) REFUSE("mmoe_attn_paged: q and out must be aligned to 16 bytes");
     AttPlan pl = att_plan(a, *kv);
+    if (pl.wgs * 256 > (int64_t)MAX_THREADS || pl.join_wgs * pl.join_threads > (int64_t)MAX_THREADS)
+        REFUSE("mmoe_attn_paged: %d sequences of up to %d positions, %d tokens, %d heads: too many for a launch", a.nseq, a.max_len, a.ntok, a.heads);
     if (!a.ws || a.ws_bytes < pl.bytes || apart(a.ws, 256)) REFUSE("mmoe_attn_paged: workspace of %zu bytes (%zu needed, aligned to 256)", a.ws ? a.ws_bytes : 0, pl.bytes);
     if (mm_ready()) return -1;
     OnDevice dev;

@@ -156,8 +156,8 @@ def attend(q, keys, values, pos, see, scale, cap, slopes, half):
                 lse[i, h] = top + np.log(l)
                 e = e[w > 1e-30].max()
                 size = w @ np.abs(vm) / l
-                # weights down to 2^-14 keep half a step; below it they are off by at most 2^-25
-                off[i, h] = half * np.abs(out[i, h]) + (half + 2 * e) * size * 1.01 + (2.0 ** -25 * np.abs(vm).sum(0) / l if half == HALF["f16"] else 0) + 2.0 ** -25
+                # fp16 weights, the largest at least 2^7: down to 2^-21 of it they keep half a step, below that they are off by at most 2^-32
+                off[i, h] = half * np.abs(out[i, h]) + (half + 2 * e) * size * 1.01 + (2.0 ** -32 * np.abs(vm).sum(0) / l if half == HALF["f16"] else 0) + 2.0 ** -25
                 loff[i, h] = e + 2.0 ** -22 * abs(lse[i, h]) + 2.0 ** -20
     return out, lse, off, loff
 

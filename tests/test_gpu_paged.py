@@ -304,6 +304,25 @@ def test_attention(name):
             b.check(d, name)
 
 
+@pytest.mark.parametrize("qlen,shared,kind", [(1, 0, "f16"), (40, 0, "f16"), (3, 16384, "f16"), (40, 16384, "f16"), (40, 0, "bf16")])
+def test_a_tail_of_small_weights(qlen, shared, kind):
+    """one position with all the weight and no value, 20000 with some 2^-24.2 of it each and values: the result is the tail's"""
+    rng = np.random.default_rng(21)
+    b = Batch(rng, qlens=[qlen, 1], lens=[20000, 16500], shared=shared, heads=2, kv=1, dim=64, bs=128, kind=kind)
+    k, v, q = (np.zeros(x.shape) for x in (b.k, b.v, b.q))
+    q[..., 0] = 8.0
+    k[..., 0] = 0.25 + 2.0 ** -6 * rng.integers(-4, 5, k.shape[:-1])
+    v[:] = rng.uniform(90, 110, v.shape)
+    for s, p in ((0, 777), (1, 9)):
+        k[b.table[s, p // 128], p % 128, :, 0] = 17.0
+        v[b.table[s, p // 128], p % 128] = 0
+    b.k, b.v, b.q = (encode(x, kind) for x in (k, v, q))
+    with Dev() as d:
+        a = b.upload(d)
+        M.check(d.lib.mmoe_attn_paged(a, b.cache), "attention")
+        b.check(d, f"tail, {qlen} tokens, {shared} shared")
+
+
 def test_attention_of_most_sequences():
     rng = np.random.default_rng(4)
     for shared in (0, 32):

@@ -34,7 +34,7 @@ def refused(rc, word):
 @pytest.mark.parametrize("kw,word", [
     (dict(block_size=0), b"block size"), (dict(block_size=24), b"block size"), (dict(block_size=8), b"block size"), (dict(block_size=2048), b"block size"),
     (dict(nseq=-1), b"sequences"), (dict(nseq=4097), b"sequences"), (dict(ntok=-1), b"tokens"), (dict(nblocks=-1), b"blocks"), (dict(nblocks=1 << 28), b"blocks"),
-    (dict(width=0), b"tables"), (dict(width=1 << 28), b"tables"), (dict(shared=8), b"shared"), (dict(shared=-16), b"shared"), (dict(shared=80), b"shared"),
+    (dict(width=0), b"tables"), (dict(width=1 << 28), b"tables"), (dict(width=(1 << 26) + 1), b"tables"), (dict(ntok=(1 << 23) + 1), b"tokens"), (dict(shared=8), b"shared"), (dict(shared=-16), b"shared"), (dict(shared=80), b"shared"),
     (dict(ctx=None), b"pointer"), (dict(add=None), b"pointer"), (dict(table=None), b"pointer"), (dict(free_list=None), b"pointer"), (dict(nfree=None), b"pointer"),
     (dict(nfree_out=None), b"pointer"), (dict(len=None), b"pointer"), (dict(qstart=None), b"pointer"), (dict(pos=None), b"pointer"), (dict(slot=None), b"pointer")])
 def test_plan_refusals(kw, word):
@@ -43,7 +43,7 @@ def test_plan_refusals(kw, word):
 
 @pytest.mark.parametrize("kw,ckw,word", [
     (dict(in_dtype=3), {}, b"types"), (dict(out_dtype=-1), {}, b"types"), (dict(head_dim=12), {}, b"head_dim"), (dict(head_dim=264), {}, b"head_dim"),
-    (dict(rot=63), {}, b"rotated"), (dict(rot=130), {}, b"rotated"), (dict(rot=-2), {}, b"rotated"), (dict(ntok=-1), {}, b"tokens"), (dict(heads=-1), {}, b"heads"),
+    (dict(rot=63), {}, b"rotated"), (dict(rot=130), {}, b"rotated"), (dict(rot=-2), {}, b"rotated"), (dict(ntok=-1), {}, b"tokens"), (dict(ntok=(1 << 23) + 1), {}, b"tokens"), (dict(heads=-1), {}, b"heads"),
     (dict(mag=float("nan")), {}, b"mag"), (dict(out_dtype=M.BF16), {}, b"cache of"), (dict(kv_heads=2), {}, b"cache of"), (dict(head_dim=64), {}, b"cache of"),
     ({}, dict(block_size=20), b"block size"), ({}, dict(k=P + 8), b"aligned"), ({}, dict(v=None), b"set"), ({}, dict(nblocks=0), b"blocks"), ({}, dict(nblocks=1 << 27), b"blocks"),
     ({}, dict(dtype=7), b"type"), ({}, dict(heads=0), b"heads"), ({}, dict(token_stride=132), b"strides"), ({}, dict(head_stride=-8), b"strides"),
@@ -63,7 +63,8 @@ ATTN = [
     (dict(heads=6), {}, b"query heads"), (dict(heads=0), {}, b"query heads"), (dict(nseq=-1), {}, b"sequences"), (dict(nseq=5000), {}, b"sequences"), (dict(ntok=-1), {}, b"tokens"),
     (dict(ntok=1 << 28), {}, b"tokens"), (dict(width=0), {}, b"tables"), (dict(width=1 << 27), {}, b"tables"), (dict(max_q=-1), {}, b"max_q"), (dict(max_len=-1), {}, b"max_len"),
     (dict(max_len=129), {}, b"max_len"), (dict(shared=8), {}, b"shared"), (dict(shared=-16), {}, b"shared"), (dict(shared=112), {}, b"shared"), (dict(window=-1), {}, b"window"),
-    (dict(scale=float("inf")), {}, b"scale"), (dict(scale=0.0), {}, b"scale"), (dict(scale=-0.1), {}, b"scale"), (dict(cap=-1.0), {}, b"cap"), (dict(cap=float("nan")), {}, b"cap"), (dict(q_head=4), {}, b"strides"), (dict(out_token=-8), {}, b"strides"),
+    (dict(scale=float("inf")), {}, b"scale"), (dict(scale=0.0), {}, b"scale"), (dict(scale=-0.1), {}, b"scale"), (dict(cap=-1.0), {}, b"cap"), (dict(cap=float("nan")), {}, b"cap"), (dict(cap=1025.0), {}, b"cap"),
+    (dict(cap=1e-39), {}, b"cap"), (dict(ntok=(1 << 22) + 1, heads=256), {}, b"tokens"), (dict(q_head=4), {}, b"strides"), (dict(out_token=-8), {}, b"strides"),
     ({}, dict(dtype=M.F32), b"cache type"), ({}, dict(token_stride=(1 << 26) + 8), b"stride"), ({}, dict(head_dim=96), b"head_dim"), ({}, dict(head_dim=256, token_stride=256), b"head_dim"), ({}, dict(token_stride=120), b"stride"), ({}, dict(block_size=17), b"block size"),
     ({}, dict(k=None), b"set"), ({}, dict(nblocks=0), b"blocks")]
 
@@ -77,9 +78,10 @@ def test_attention_refusals(kw, ckw, word):
 
 @pytest.mark.parametrize("kw,word", [(dict(q=None), b"pointer"), (dict(out=None), b"pointer"), (dict(qstart=None), b"pointer"), (dict(len=None), b"pointer"),
                                      (dict(table=None), b"pointer"), (dict(q=P + 8), b"aligned"), (dict(out=P + 2), b"aligned"), (dict(ws=None), b"workspace"),
-                                     (dict(ws=P + 16), b"workspace"), (dict(ws_bytes=0), b"workspace")])
+                                     (dict(ws=P + 16), b"workspace"), (dict(ws_bytes=0), b"workspace"),
+                                     (dict(nseq=4096, width=1 << 26, max_len=1 << 30, heads=2048), b"key/value heads"), (dict(nseq=4096, width=1 << 26, max_len=1 << 30), b"too many")])
 def test_attention_refusals_of_pointers(kw, word):
-    refused(M.lib().mmoe_attn_paged(attn(**kw), cache()), word)
+    refused(M.lib().mmoe_attn_paged(attn(**kw), cache(heads=2048) if word == b"key/value heads" else cache(heads=16) if word == b"too many" else cache()), word)
 
 
 def test_nothing_to_do_is_no_error():
