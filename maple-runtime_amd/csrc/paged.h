@@ -431,8 +431,8 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
 // Every kernel here keeps a softmax's running maximum and sum and one pass over the positions. A query row is a (token, query
 // head) pair; the rows that read one key/value head, token by token and its group of query heads within, share its keys. The
 // rows' visible runs [lo, hi) are all there is to masks: a tile that every live row sees whole needs none.
-#define ATT_BM 128         // rows and positions of a tile
-#define ATT_BN 64
+#define ATT_BM 128         // rows of a tile
+#define ATT_BN(D) (8192 / (D))   // and its positions: 32 KB of keys and values for either head size
 #define ATT_LOG2E 1.44269504088896340736f
 #define ATT_LN2 0.69314718055994530942f
 
@@ -574,7 +574,7 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
     return v;
 }
 
-// Row tiles of 4 waves, 32 rows each, over tiles of 64 positions that all waves share through LDS.
+// Row tiles of 4 waves, 32 rows each, over tiles of 64 positions (128 with heads of 64) that all waves share through LDS.
 // S^T = K Q^T, so a lane holds one row's scores (half of the positions, the other half in the lane 32 away): the softmax needs
 // one exchange per tile, and P^T, packed to 16 bits, is the second product's operand as it lies. O^T = V^T P^T takes its V^T from
 // rows of V through the transposing LDS reads. A tile's keys and values go from the cache straight to LDS, one tile ahead, in 16-byte
@@ -582,17 +582,18 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
 // reads of 4 rows meet in a bank. P is rounded to the cache's type (half a step relative, as the result itself is), its
 // sum is of the unrounded 32-bit values.
 template <int D> struct AttTileMem {
-    __attribute__((aligned(1024))) uint8_t first[2 * ATT_BN * D * 2];   // keys and values of a tile
+    __attribute__((aligned(1024))) uint8_t first[2 * ATT_BN(D) * D * 2];   // keys and values of a tile
     union {
-        __attribute__((aligned(1024))) uint8_t second[2 * ATT_BN * D * 2];
+        __attribute__((aligned(1024))) uint8_t second[2 * ATT_BN(D) * D * 2];
         int starts[MMOE_KV_MAXSEQ + 1];
     };
     int range[4][4], flag[2][4];
 };
 template <int T, int D, bool CAP, bool BIAS>
 __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, const unsigned block, AttTileMem<D> &M) {
-    constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // a row's bytes and chunks; rows of a load, a wave's loads
-    constexpr uint32_t TB = ATT_BN * RB;
+    constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // a row's bytes and chunks; rows of a load, loads of 16 rows
+    constexpr int BN = ATT_BN(D), GW = BN / 64, NU = BN / 32, NK = BN / 16;   // groups of 16 positions that a wave loads; score blocks, steps of the second product
+    constexpr uint32_t TB = BN * RB;
     const mmoe_attn_args &a = A.a;
     const int nsplit = shared ? A.split_sh : A.split;
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 31, hh = l >> 5;
@@ -615,25 +616,35 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     const int32_t *table = a.table + (int64_t)at.s * a.width;
     int id = 0, idp = INT32_MIN / 2;      // ids of the positions from idp on
     uint64_t lost = 0;                    // those that are none of the cache's
-    auto block_of = [&](int p, unsigned &bad) {   // the wave's block of a tile
+    auto block_of = [&](int p, unsigned &bad) {   // the wave's blocks of a tile
         if (p - idp >= 1024) {
             idp = p;
             id = table[min((p + 16 * l) >> A.sh, a.width - 1)];
             lost = __ballot((unsigned)id >= (unsigned)A.kv.nblocks);
         }
-        bad = (unsigned)(lost >> ((p - idp) >> 4)) & 15u;
-        int blk = __builtin_amdgcn_readlane(id, ((p - idp) >> 4) + w);
-        return (unsigned)blk < (unsigned)A.kv.nblocks ? blk : 0;
+        bad = (unsigned)(lost >> ((p - idp) >> 4)) & ((1u << NK) - 1);
+        struct { int at[GW]; } blk;
+#pragma unroll
+        for (int g = 0; g < GW; g++) {
+            const int b = __builtin_amdgcn_readlane(id, ((p - idp) >> 4) + GW * w + g);
+            blk.at[g] = (unsigned)b < (unsigned)A.kv.nblocks ? b : 0;
+        }
+        return blk;
     };
-    auto fetch = [&](uint32_t buf, const void *base, const uint32_t *off, int p, int blk) {
-        const uint8_t *from = (const uint8_t *)base + (blk * A.kv.block_stride + kvh * A.kv.head_stride + ((p + 16 * w) & (A.kv.block_size - 1)) * A.kv.token_stride) * 2;
-        load_lds<NI>(from, off, buf + w * 16 * RB);
+    auto fetch = [&](uint32_t buf, const void *base, const uint32_t *off, int p, const auto &blk) {
+#pragma unroll
+        for (int g = 0; g < GW; g++) {
+            const int r = 16 * (GW * w + g);
+            const uint8_t *from = (const uint8_t *)base + (blk.at[g] * A.kv.block_stride + kvh * A.kv.head_stride + ((p + r) & (A.kv.block_size - 1)) * A.kv.token_stride) * 2;
+            load_lds<NI>(from, off, buf + r * RB);
+        }
     };
     const uint32_t lds = (uint32_t)(uintptr_t)(lb *)M.first;   // tile i: keys at lds + 2 TB (i % 2), values TB behind them
     unsigned bad = 0, next = 0;   // the tile's lost blocks, the next one's
-    int p0, p1, blk;
+    int p0, p1;
+    decltype(block_of(0, bad)) blk;
     if (shared) {   // which positions is known already: the first tile comes while the rows look for their sequences
-        const int run = ((a.shared + ATT_BN - 1) / ATT_BN + nsplit - 1) / nsplit * ATT_BN;
+        const int run = ((a.shared + BN - 1) / BN + nsplit - 1) / nsplit * BN;
         p0 = split * run; p1 = min(p0 + run, a.shared);
         if (p0 < p1) {
             blk = block_of(p0, bad);
@@ -663,7 +674,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         lo = min(lo, M.range[0][i]); hi = max(hi, M.range[1][i]);
         glo = max(glo, M.range[2][i]); ghi = min(ghi, M.range[3][i]);
     }
-    lo = __builtin_amdgcn_readfirstlane(lo) & ~(ATT_BN - 1); hi = __builtin_amdgcn_readfirstlane(hi);
+    lo = __builtin_amdgcn_readfirstlane(lo) & ~(BN - 1); hi = __builtin_amdgcn_readfirstlane(hi);
     glo = __builtin_amdgcn_readfirstlane(glo); ghi = __builtin_amdgcn_readfirstlane(ghi);
     if (shared) {
         p1 = lo < hi ? min(p1, hi) : p0;   // (the first tile is there, also where it lies before lo: nobody looks)
@@ -671,7 +682,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     } else {
         p0 = lo; p1 = hi;
         if (nsplit > 1 && p0 < p1) {
-            int run = ((p1 - p0 + ATT_BN - 1) / ATT_BN + nsplit - 1) / nsplit * ATT_BN;
+            int run = ((p1 - p0 + BN - 1) / BN + nsplit - 1) / nsplit * BN;
             p0 += split * run;
             p1 = min(p1, p0 + run);
         }
@@ -689,7 +700,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     for (int k = 0; k < KS; k++) ka[k] = n * RB + (((2 * k + hh) ^ (n & (CH - 1))) << 4);
 #pragma unroll
     for (int i = 0; i < DS; i++) va[i] = vr * RB + ((64 * i + 32 * ((l >> 4) & 1) + 8 * (l & 3)) ^ ((vr & (CH / 2 - 1)) << 5));
-    f16v acc[DS], sc[2];
+    f16v acc[DS], sc[NU];
 #pragma unroll
     for (int i = 0; i < DS; i++)
 #pragma unroll
@@ -700,24 +711,24 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 
     auto scores = [&](f16v *s, uint32_t buf) {
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int u = 0; u < NU; u++)
 #pragma unroll
             for (int j = 0; j < 16; j++) s[u][j] = 0.0f;
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll
-            for (int u = 0; u < 2; u++) s[u] = mfma32<T>(*(const lu4 *)((const lb *)(uintptr_t)buf + ka[k] + 32 * u * RB), q[k], s[u]);
+            for (int u = 0; u < NU; u++) s[u] = mfma32<T>(*(const lu4 *)((const lb *)(uintptr_t)buf + ka[k] + 32 * u * RB), q[k], s[u]);
         // six reads ahead of the products
         __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
-        for (int k = 0; k < 2 * KS - 6; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
+        for (int k = 0; k < NU * KS - 6; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
         __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
     };
     // scores in units of log 2 (without cap and bias: but for s1)
     auto math = [&](f16v *s, int p) {
         const float dist = BIAS ? (float)(R.pos - p - 4 * hh) : 0.0f;
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int u = 0; u < NU; u++)
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 float x = s[u][j] * A.s1;
@@ -730,19 +741,19 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     auto mask = [&](f16v *s, int p, unsigned bad) {
         const unsigned at = (unsigned)(p + 4 * hh - R.lo), span = (unsigned)max(R.hi - R.lo, 0);
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int u = 0; u < NU; u++)
 #pragma unroll
             for (int j = 0; j < 16; j++) s[u][j] = at + (32 * u + 8 * (j >> 2) + (j & 3)) < span ? s[u][j] : -__builtin_inff();
         if (bad)
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+            for (int u = 0; u < NU; u++)
 #pragma unroll
                 for (int j = 0; j < 16; j++) s[u][j] = (bad >> (2 * u + (j >> 3))) & 1 ? -__builtin_inff() : s[u][j];
     };
     auto largest = [&](const f16v *s) {
         float top[4];   // no chain of 32
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int u = 0; u < NU; u++)
 #pragma unroll
             for (int j = 0; j < 16; j++) top[j & 3] = u || j > 3 ? max_(top[j & 3], s[u][j]) : s[u][j];
         return max_halves(max_(max_(top[0], top[1]), max_(top[2], top[3]))) * s1;
@@ -765,14 +776,15 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
             uint2 t1 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((ls4 *)(v + 8 * RB)));
             return u4{t0.x, t0.y, t1.x, t1.y};
         };
-        u4 f0[DS];   // the first positions' are on their way during the exponentials
+        constexpr int AHEAD = 4 / DS;
+        u4 f0[4];   // the first positions' are on their way during the exponentials
 #pragma unroll
-        for (int i = 0; i < DS; i++) f0[i] = value(i, 0);
+        for (int i = 0; i < 4; i++) f0[i] = value(i % DS, i / DS);
         __builtin_amdgcn_sched_barrier(0);
-        u4 pf[4];
+        u4 pf[NK];
         float part = 0;
 #pragma unroll
-        for (int u = 0; u < 2; u++)
+        for (int u = 0; u < NU; u++)
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
                 float e0 = exp2_(fmaf(sc[u][j], s1, -mb)), e1 = exp2_(fmaf(sc[u][j + 1], s1, -mb));
@@ -781,19 +793,19 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
             }
         sum += part;   // tile by tile: a long sum of small ones
 #pragma unroll
-        for (int k = 0; k < 4; k++)
+        for (int k = 0; k < NK; k++)
 #pragma unroll
-            for (int i = 0; i < DS; i++) acc[i] = mfma32<T>(k ? value(i, k) : f0[i], pf[k], acc[i]);
+            for (int i = 0; i < DS; i++) acc[i] = mfma32<T>(k < AHEAD ? f0[k * DS + i] : value(i, k), pf[k], acc[i]);
 #pragma unroll
-        for (int k = 0; k < 3 * DS; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
-        __builtin_amdgcn_sched_group_barrier(0x8, DS, 0);
+        for (int k = 0; k < NK * DS - 4; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
+        __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
     };
     // A value that is not finite times a weight of 0 is NaN, so in a tile that is not seen whole such values go round the product:
     // the tile's are set aside in the other buffer and zeroed, and afterwards added, as they are, to the rows that see their position.
     auto set_aside = [&](uint32_t buf, uint32_t other) {
 #pragma unroll
-        for (int x = 0; x < NI; x++) {
-            const uint32_t o = w * 16 * RB + x * 1024 + l * 16;
+        for (int x = 0; x < GW * NI; x++) {
+            const uint32_t o = w * 16 * GW * RB + x * 1024 + l * 16;
             u4 v = *(const lu4 *)((lb *)(uintptr_t)buf + o);
             *(lu4 *)((lb *)(uintptr_t)other + o) = v;
 #pragma unroll
@@ -803,7 +815,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     };
     auto add_aside = [&](uint32_t other, int p, unsigned bad) {
 #pragma unroll 1
-        for (int r = 0; r < ATT_BN; r++) {
+        for (int r = 0; r < BN; r++) {
             const bool see = p + r >= R.lo && p + r < R.hi && !((bad >> (r >> 4)) & 1);
             uint32_t row = r * RB + 8 * hh, x = (r & (CH / 2 - 1)) << 5;
             asm("" : "+v"(row));   // its addresses are not worth a register outside
@@ -825,15 +837,15 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     if (p0 < p1) {
 #pragma unroll
         for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));   // the queries are there: nothing in the loop waits for them
-        for (int p = p0, i = 0; p < p1; p += ATT_BN, i ^= 1, bad = next) {
+        for (int p = p0, i = 0; p < p1; p += BN, i ^= 1, bad = next) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the compiler does not know of these loads
             const uint32_t kbuf = lds + i * 2 * TB, vbuf = kbuf + TB, kother = lds + (i ^ 1) * 2 * TB, vother = kother + TB;
-            const bool part = p < glo || p + ATT_BN > ghi || bad, more = p + ATT_BN < p1;
-            if (part) {   // the wave's own 16 rows of values: are they finite?
+            const bool part = p < glo || p + BN > ghi || bad, more = p + BN < p1;
+            if (part) {   // the wave's own rows of values: are they finite?
                 bool o = false;
 #pragma unroll
-                for (int x = 0; x < NI; x++) {
-                    u4 v = *(const lu4 *)((const lb *)(uintptr_t)vbuf + w * 16 * RB + x * 1024 + l * 16);
+                for (int x = 0; x < GW * NI; x++) {
+                    u4 v = *(const lu4 *)((const lb *)(uintptr_t)vbuf + w * 16 * GW * RB + x * 1024 + l * 16);
 #pragma unroll
                     for (int y = 0; y < 4; y++) o |= odd16<T>(v[y]) | odd16<T>(v[y] >> 16);
                 }
@@ -844,21 +856,21 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
             bool odd = false;
             if (part) odd = __builtin_amdgcn_readfirstlane(M.flag[i][0] | M.flag[i][1] | M.flag[i][2] | M.flag[i][3]) != 0;
             if (more) {
-                blk = block_of(p + ATT_BN, next);
-                fetch(kother, A.kv.k, ko, p + ATT_BN, blk);
-                if (!odd) fetch(vother, A.kv.v, vo, p + ATT_BN, blk);
+                blk = block_of(p + BN, next);
+                fetch(kother, A.kv.k, ko, p + BN, blk);
+                if (!odd) fetch(vother, A.kv.v, vo, p + BN, blk);
             }
             if (odd) {
                 set_aside(vbuf, vother);
                 __syncthreads();
             }
-            const bool mine = p < whi && p + ATT_BN > wlo;
+            const bool mine = p < whi && p + BN > wlo;
             if (mine) {
                 __builtin_amdgcn_s_setprio(1);
                 scores(sc, kbuf);
                 __builtin_amdgcn_s_setprio(0);
                 if (MATH) math(sc, p);
-                if (p < inlo || p + ATT_BN > inhi || bad) mask(sc, p, bad);
+                if (p < inlo || p + BN > inhi || bad) mask(sc, p, bad);
                 rescale(largest(sc));
                 __builtin_amdgcn_s_setprio(1);
                 product(vbuf);
@@ -867,7 +879,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
             if (odd) {
                 if (mine) add_aside(vother, p, bad);
                 __syncthreads();
-                if (more) fetch(vother, A.kv.v, vo, p + ATT_BN, blk);
+                if (more) fetch(vother, A.kv.v, vo, p + BN, blk);
             }
         }
     }
