@@ -341,7 +341,7 @@ int mmoe_rope_kv(const mmoe_rope_args *a, const mmoe_kv_cache *kv);
 /* Attention of nseq sequences over their blocks. Sequence s has the tokens qstart[s] .. qstart[s + 1] - 1 of q [ntok][heads][head_dim]
  * (none, one or many), its last ones of len[s] positions; query head h reads key/value head h / (heads / kv heads).
  * head_dim 64 or 128; q, out and the cache of one type, MMOE_F16 or MMOE_BF16; scores, softmax and sums in 32 bits. ntok heads at most 2^30.
- *   score of position p for the token at position i:  x = scale q.k (scale > 0);  cap > 0 (at most 1024): x = cap tanh(x / cap);
+ *   score of position p for the token at position i:  x = scale q.k (scale 1e-20 to 1e20);  cap > 0 (at most 1024): x = cap tanh(x / cap);
  *   slopes != NULL: x -= slopes[h] |i - p|
  *   visible: max(lo[t], i - window) <= p < min(hi[t], len[s]); lo NULL: 0; hi NULL: i + 1 (causal); window 0: unlimited
  * lo and hi are per token: a document mask gives each token its document's first position, a prefix mask lets hi reach past

@@ -464,7 +464,7 @@ struct AttArgs {
     int sh_few, few;
     int split_sh, split, chunk, chunks;   // runs of the shared positions, runs per row tile of the own ones; positions per chunk, most chunks
     int parts_sh;        // partial results of the shared positions: split_sh, or 0
-    float s1, s2;        // cap 0: score = s1 q.k in units of log 2; else s2 tanh, with exp(2 z) = exp2(s1 q.k)
+    float s1, s2;        // cap 0: score = s1 q.k in units of log 2; else s2 tanh z, with exp(2 z) = exp2(s1 q.k)
     // partial results, [head_dim] values over their own sum each, and their maxima (in units of log 2) and sums: of the shared positions
     // [split_sh][ntok][heads], from at_tile on of row tiles over the own ones [split][ntok][heads], from at_few on of chunks [chunks][nseq][16 kv heads]
     float *po;
@@ -482,6 +482,7 @@ template <int T> constexpr float lift = T == MMOE_F16 ? 7.0f : 0.0f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // the larger of two numbers, without fmaxf's quieting of each (a NaN shows in the weights, whatever the maximum then is)
 __device__ __forceinline__ float max_(float x, float y) { return __builtin_amdgcn_fmed3f(x, y, __builtin_inff()); }
+__device__ __forceinline__ float min_(float x, float y) { return __builtin_amdgcn_fmed3f(x, y, -__builtin_inff()); }
 // N pieces of 16 bytes per lane from base + off[i] + 1024 i to LDS at to + 1024 i + 16 * lane (the offset of the instruction counts on both
 // sides). Asm, so that the compiler does not wait for them before every later LDS read; nothing is written to a register. The
 // waits are the caller's.
@@ -661,7 +662,10 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 #pragma unroll
         for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 16 * s);
     }
-    const float slope = BIAS ? a.slopes[R.head] * ATT_LOG2E : 0.0f;
+    // A score is sc s1 + s0 in units of log 2, in which sc is the product's with the bias in its units, or with a cap 1 / (1 + exp 2 z):
+    // what is left of them is in the exponentials' own multiplication.
+    const float s0 = CAP && !BIAS ? A.s2 : 0.0f, s1 = CAP ? BIAS ? 1.0f : -2.0f * A.s2 : A.s1;
+    const float slope = BIAS ? a.slopes[R.head] * (CAP ? ATT_LOG2E : ATT_LOG2E / A.s1) : 0.0f;
     // the wave's and the workgroup's positions
     const bool some = R.live && R.lo < R.hi;
     const int wlo = wave_min(some ? R.lo : INT32_MAX), whi = wave_max(some ? R.hi : 0);
@@ -706,8 +710,8 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 #pragma unroll
         for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
     float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f;   // mb: m - lift, - lift while m is -inf
-    constexpr bool MATH = CAP || BIAS;
-    const float s1 = MATH ? 1.0f : A.s1;
+    constexpr bool FALLS = CAP && !BIAS;   // sc falls as the score grows
+    constexpr float NONE = FALLS ? __builtin_inff() : -__builtin_inff();   // sc of a position that is not seen
 
     auto scores = [&](f16v *s, uint32_t buf) {
 #pragma unroll
@@ -724,39 +728,40 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         for (int k = 0; k < NU * KS - 6; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); }
         __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
     };
-    // scores in units of log 2 (without cap and bias: but for s1)
     auto math = [&](f16v *s, int p) {
         const float dist = BIAS ? (float)(R.pos - p - 4 * hh) : 0.0f;
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll
             for (int j = 0; j < 16; j++) {
-                float x = s[u][j] * A.s1;
-                if (CAP) x = fmaf(-2.0f * A.s2, __builtin_amdgcn_rcpf(1.0f + exp2_(x)), A.s2);   // tanh z = 1 - 2 / (1 + exp 2 z)
+                float x = s[u][j];
+                if (CAP) x = __builtin_amdgcn_rcpf(1.0f + exp2_(x * A.s1));   // tanh z = 1 - 2 / (1 + exp 2 z)
+                if (CAP && BIAS) x = fmaf(-2.0f * A.s2, x, A.s2);
                 if (BIAS) x = fmaf(-slope, fabsf(dist - (float)(32 * u + 8 * (j >> 2) + (j & 3))), x);
                 s[u][j] = x;
             }
     };
-    // a tile that is not seen whole: -inf where a row does not look
+    // a tile that is not seen whole: a score of -inf where a row does not look
     auto mask = [&](f16v *s, int p, unsigned bad) {
         const unsigned at = (unsigned)(p + 4 * hh - R.lo), span = (unsigned)max(R.hi - R.lo, 0);
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) s[u][j] = at + (32 * u + 8 * (j >> 2) + (j & 3)) < span ? s[u][j] : -__builtin_inff();
+            for (int j = 0; j < 16; j++) s[u][j] = at + (32 * u + 8 * (j >> 2) + (j & 3)) < span ? s[u][j] : NONE;
         if (bad)
 #pragma unroll
             for (int u = 0; u < NU; u++)
 #pragma unroll
-                for (int j = 0; j < 16; j++) s[u][j] = (bad >> (2 * u + (j >> 3))) & 1 ? -__builtin_inff() : s[u][j];
+                for (int j = 0; j < 16; j++) s[u][j] = (bad >> (2 * u + (j >> 3))) & 1 ? NONE : s[u][j];
     };
     auto largest = [&](const f16v *s) {
         float top[4];   // no chain of 32
+        auto higher = [](float x, float y) { return FALLS ? min_(x, y) : max_(x, y); };
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) top[j & 3] = u || j > 3 ? max_(top[j & 3], s[u][j]) : s[u][j];
-        return max_halves(max_(max_(top[0], top[1]), max_(top[2], top[3]))) * s1;
+            for (int j = 0; j < 16; j++) top[j & 3] = u || j > 3 ? higher(top[j & 3], s[u][j]) : s[u][j];
+        return max_halves(fmaf(higher(higher(top[0], top[1]), higher(top[2], top[3])), s1, s0));
     };
     // a new maximum only once it is 2^8 past the old: until then weights stay below 2^8 (lifted: 2^15), in every type's range
     auto rescale = [&](float mt) {
@@ -783,11 +788,12 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         __builtin_amdgcn_sched_barrier(0);
         u4 pf[NK];
         float part = 0;
+        const float off = s0 - mb;
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-                float e0 = exp2_(fmaf(sc[u][j], s1, -mb)), e1 = exp2_(fmaf(sc[u][j + 1], s1, -mb));
+                float e0 = exp2_(fmaf(sc[u][j], s1, off)), e1 = exp2_(fmaf(sc[u][j + 1], s1, off));
                 part += e0 + e1;
                 pf[2 * u + (j >> 3)][(j & 7) >> 1] = pack2<T>(e0, e1);
             }
@@ -869,7 +875,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                 __builtin_amdgcn_s_setprio(1);
                 scores(sc, kbuf);
                 __builtin_amdgcn_s_setprio(0);
-                if (MATH) math(sc, p);
+                if (CAP || BIAS) math(sc, p);
                 if (p < inlo || p + BN > inhi || bad) mask(sc, p, bad);
                 rescale(largest(sc));
                 __builtin_amdgcn_s_setprio(1);

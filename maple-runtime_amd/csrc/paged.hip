@@ -137,7 +137,7 @@ static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
         REFUSE("mmoe_attn_paged: max_q %d, max_len %d (tables of %d blocks)", a.max_q, a.max_len, a.width);
     if (a.shared < 0 || a.shared % kv->block_size || a.shared > a.max_len) REFUSE("mmoe_attn_paged: %d shared positions (block size %d, max_len %d)", a.shared, kv->block_size, a.max_len);
     if (a.window < 0) REFUSE("mmoe_attn_paged: window %d", a.window);
-    if (!(a.scale > 0) || !isfinite(a.scale) || !(a.cap >= 0) || a.cap > MAX_CAP || (a.cap > 0 && !isfinite(4.0f * a.scale / a.cap))) REFUSE("mmoe_attn_paged: scale %g, cap %g", a.scale, a.cap);
+    if (!(a.scale >= 1e-20f) || !(a.scale <= 1e20f) || !(a.cap >= 0) || a.cap > MAX_CAP || (a.cap > 0 && !isfinite(4.0f * a.scale / a.cap))) REFUSE("mmoe_attn_paged: scale %g, cap %g", a.scale, a.cap);
     if (a.q_token < 0 || a.q_head < 0 || a.out_token < 0 || a.out_head < 0 || ((a.q_token | a.q_head | a.out_token | a.out_head) & 7))
         REFUSE("mmoe_attn_paged: strides must be multiples of 8");
     return 0;
