@@ -156,15 +156,18 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     const int group = a.heads / kv.heads;
     const int64_t rows = (int64_t)a.ntok * group, tiles = (rows + ATT_BM - 1) / ATT_BM, most_rows = (int64_t)std::min(a.max_q, a.ntok) * group;
     const int own = a.window && !a.hi ? (int)std::min<int64_t>(a.max_len - a.shared, (int64_t)a.window + a.max_q) : a.max_len - a.shared;
-    // Runs of a row tile's positions: about 256 workgroups, half as many again where their runs stay above 2048 positions (a second
-    // workgroup on a CU adds a quarter to its rate, its partial results cost their bytes twice). 960 rows over 40000 positions, 256 / 384 / 512
-    // workgroups: 121 / 114 / 128 us; 256 rows over 16384: 31 / 38 / 56.
+    // Runs of a row tile's positions: about 256 workgroups, half as many again where their runs stay above 512 positions (a second
+    // workgroup on a CU adds a quarter to its rate, its partial results cost their bytes twice), none below 192. 960 rows over 40000
+    // positions, 256 / 384 / 512 workgroups: 121 / 114 / 128 us; 256 rows over 16384: 31 / 38 / 56; 1200 over 20000: 85 / 74 / 89.
+    // Runs of 256 / 512 / 1024 of 1000 positions: 20.1 / 22.9 / 25.7 us; one of 382 or two: 20.7 / 24.5.
     auto runs = [&](int64_t groups, int positions) {
-        const int64_t wgs = groups * kv.heads, n = (256 + wgs - 1) / wgs, n2 = (384 + wgs - 1) / wgs, most = (positions + 255) / 256;
-        return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(positions / n2 >= 2048 ? n2 : n, most), ATT_PARTS / 2));
+        const int64_t wgs = groups * kv.heads, n = (256 + wgs - 1) / wgs, n2 = (384 + wgs - 1) / wgs, most = positions / 192;
+        return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(positions / n2 >= 512 ? n2 : n, most), ATT_PARTS / 2));
     };
-    // Rows of a key/value head that k_attn_few takes: 16 are one product's, 32 over shared positions read them twice (from cache)
-    p.few_sh = rows <= 32;
+    // Rows of a key/value head that k_attn_few takes: 16 are one product's, 32 over shared positions read them twice (from cache). So few
+    // that all its workgroups are on the card at once start sooner than row tiles do: 46 rows, 2 heads, 5088 positions (120 workgroups)
+    // 14.4 us, as row tiles 18.4; 36, 8, 3136 (312) 16.9, 18.4; but 228, 4, 1312 (360) 20.3, 18.6.
+    p.few_sh = rows <= 32 || (rows + 15) / 16 * kv.heads * (a.shared / 256 + 1) <= 320;
     if (most_rows <= 16 || a.nseq > 1) p.few = 16;
     // Chunks: 1024 positions, down to 256 while there are fewer than 384 workgroups (one sequence of 100000: 256 50.5 us, 512 50.3, 1024 47.6,
     // 2048 47.9; 64 of up to 3000: 52.2, 49.6, 47.9, 62.5; 7 over 2048 shared: 128 12.9, 256 12.0, 512 13.9), and never more than ATT_PARTS / 2
@@ -176,11 +179,12 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
         p.tiles_sh = p.few_sh ? (int)((rows + 15) / 16) : (int)tiles;
         p.split_sh = p.few_sh ? (a.shared + p.chunk - 1) / p.chunk : runs(tiles, a.shared);
     }
-    if (p.few) p.chunks = std::max(1, (own + 31 + p.chunk - 1) / p.chunk);
+    if (p.few) p.chunks = std::max(1, (own + (a.window ? 31 : a.shared & 31) + p.chunk - 1) / p.chunk);   // (they begin at a multiple of 32)
     p.split = 1;
     if (most_rows > p.few) {
         p.tiles = (int)tiles + a.nseq;
-        p.split = runs(tiles, own);
+        // (with a window a tile sees that and its own tokens)
+        p.split = runs(tiles, a.window && !a.hi ? (int)std::min<int64_t>(own, (int64_t)a.window + ATT_BM / group) : own);
     }
     p.parts = p.split_sh + std::max(p.split, p.chunks);
     const int64_t all = (int64_t)a.ntok * a.heads;
