@@ -75,7 +75,9 @@ int mmoe_kv_plan(const mmoe_kv_plan_args *p) {
     if (mm_ready()) return -1;
     OnDevice dev;
     if (!dev.ok) return -1;
+    // The tokens in the same launch, or in one of their own over the whole card: 1000 tokens 6.0 / 8.8 us, 4000 7.4 / 8.9, 8000 8.3 / 8.2
     const bool one = a.ntok <= 4096;
+    // 256 threads have fewer waves to wait for: 64 sequences 5.6 us, with 1024 threads 6.8
     const unsigned threads = std::max(a.nseq, a.ntok) <= 256 ? 256 : 1024;
     if (a.nseq <= 1024 ? run(MMOE_K_KV_PLAN, k_kv_plan<1>, 1, threads, a, sh, one) : run(MMOE_K_KV_PLAN, k_kv_plan<4>, 1, threads, a, sh, one)) return -1;
     return one ? 0 : run(MMOE_K_KV_PLAN, k_kv_tokens, (a.ntok + 255) / 256, 256, a, sh);
@@ -105,9 +107,10 @@ int mmoe_rope_freqs(int rot, double base, double factor, int orig, double slow, 
 // ------------------------------------------------------------------------------------------------------
 template <int IN, int OUT>
 static int rope_launch(const mmoe_rope_args &a, const mmoe_kv_cache &kv, int cached, int sh) {
-    // as many tokens per workgroup as RP_U heads per lane cover, once there are workgroups enough
+    // As many tokens per workgroup as RP_U heads per lane cover, once there are 512 workgroups: two tokens of 24 heads instead of one
+    // 24.5 instead of 28.4 us at 8191 tokens, 7.7 instead of 8.9 at 2000; 6.8 instead of 6.5 at 1000
     const int nh = a.heads + a.kv_heads * (1 + cached), at_once = RP_U * RP_T / (a.head_dim / 8);
-    const int tb = std::max(1, std::min(std::min(at_once / nh, RP_TB), a.ntok / 1024));
+    const int tb = std::max(1, std::min(std::min(at_once / nh, RP_TB), a.ntok / 512));
     dim3 g((a.ntok + tb - 1) / tb);
     const bool pow2 = (a.head_dim & (a.head_dim - 1)) == 0;
     if (pow2 && a.interleaved) return run(MMOE_K_ROPE, k_rope<IN, OUT, RP_INTER>, g, RP_T, a, kv, cached, sh, tb);
@@ -159,10 +162,11 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     // Runs of a row tile's positions: about 256 workgroups, half as many again where their runs stay above 512 positions (a second
     // workgroup on a CU adds a quarter to its rate, its partial results cost their bytes twice), none below 192. 960 rows over 40000
     // positions, 256 / 384 / 512 workgroups: 121 / 114 / 128 us; 256 rows over 16384: 31 / 38 / 56; 1200 over 20000: 85 / 74 / 89.
-    // Runs of 256 / 512 / 1024 of 1000 positions: 20.1 / 22.9 / 25.7 us; one of 382 or two: 20.7 / 24.5.
+    // Runs of 256 / 512 / 1024 of 1000 positions: 20.1 / 22.9 / 25.7 us; one of 382 or two: 20.7 / 24.5. Tiles enough for one run each stay
+    // whole: 3500 rows of 12 heads over up to 1100 positions 22.6 us, in two runs 33.
     auto runs = [&](int64_t groups, int positions) {
         const int64_t wgs = groups * kv.heads, n = (256 + wgs - 1) / wgs, n2 = (384 + wgs - 1) / wgs, most = positions / 192;
-        return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(positions / n2 >= 512 ? n2 : n, most), ATT_PARTS / 2));
+        return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(n > 1 && positions / n2 >= 512 ? n2 : n, most), ATT_PARTS / 2));
     };
     // Rows of a key/value head that k_attn_few takes: 16 are one product's, 32 over shared positions read them twice (from cache). So few
     // that all its workgroups are on the card at once start sooner than row tiles do: 46 rows, 2 heads, 5088 positions (120 workgroups)
@@ -179,12 +183,18 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
         p.tiles_sh = p.few_sh ? (int)((rows + 15) / 16) : (int)tiles;
         p.split_sh = p.few_sh ? (a.shared + p.chunk - 1) / p.chunk : runs(tiles, a.shared);
     }
-    if (p.few) p.chunks = std::max(1, (own + (a.window ? 31 : a.shared & 31) + p.chunk - 1) / p.chunk);   // (they begin at a multiple of 32)
     p.split = 1;
     if (most_rows > p.few) {
         p.tiles = (int)tiles + a.nseq;
         // (with a window a tile sees that and its own tokens)
         p.split = runs(tiles, a.window && !a.hi ? (int)std::min<int64_t>(own, (int64_t)a.window + ATT_BM / group) : own);
+    }
+    if (p.few) {
+        const int span = own + (a.window ? 31 : a.shared & 31);   // chunks begin at a multiple of 32
+        // One chunk, and no join, beside row tiles that go over as many positions in one run: five prompts of up to 1100 tokens 21.8 us, with
+        // a join of nothing 23.6; 8 sequences of 1 to 300 tokens over 1500 positions 40.7 and 40.6
+        if (p.tiles && p.split == 1 && !p.split_sh && span <= 2048) p.chunk = std::max(128, (span + 127) & ~127);
+        p.chunks = std::max(1, (span + p.chunk - 1) / p.chunk);
     }
     p.parts = p.split_sh + std::max(p.split, p.chunks);
     const int64_t all = (int64_t)a.ntok * a.heads;
@@ -194,8 +204,10 @@ static AttPlan att_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     p.bytes = 256 + (size_t)p.entries * (kv.head_dim * 4 + 8);
     p.wgs = (int64_t)kv.heads * ((int64_t)p.tiles_sh * p.split_sh + (int64_t)p.tiles * p.split + (int64_t)p.chunks * a.nseq);
     p.join_few = !p.split_sh && p.tiles && p.split == 1;   // only sequences of few rows have partial results
+    // A workgroup per row from 17 parts on (10 parts that way 81 us instead of 74 for the call; 32 parts in one lane group's registers 19
+    // instead of 12), of 1024 threads from 129 on (390 parts: 162.3 us for the call, with 256 threads 164.6; 21 parts: 46, 34)
     p.join_all = p.parts > ATT_PER;
-    p.join_threads = p.join_all && p.parts > 64 ? 1024 : 256;
+    p.join_threads = p.join_all && p.parts > 128 ? 1024 : 256;
     const int64_t jr = p.join_few ? 16ll * kv.heads * a.nseq : all, per = p.join_threads / (kv.head_dim / 4);
     p.join_wgs = p.join_all ? jr : (jr + per - 1) / per;
     return p;
