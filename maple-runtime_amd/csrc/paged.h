@@ -104,7 +104,8 @@ __device__ __forceinline__ int wave_max(int v) { return wave_reduce(v, [](int x,
 // item finds its sequence by a binary search of the sums in LDS, so one long sequence costs no more than many short ones. One
 // workgroup holds it all, since the steps depend on each other through the free list. Bound: the latency of dependent loads
 // (lengths; a table's begun block and the list's end; the stores), not bytes (a step of 64 sequences moves 5 KB), so what a later step
-// needs is loaded as soon as its address is known and kept in LDS.
+// needs is loaded as soon as its address is known and kept in LDS. Measured: 64 sequences of one token, 3 finished, 6.2 us (12.3 with
+// what is taken and given back read from memory again, 9.4 with the totals by atomics in LDS); 301 prompts of up to 400 tokens 7.0 us.
 #define KP_LIM (1 << 30)     // sums stop here: above every count there is room for, and two of them still fit
 #define KP_TOP 1024          // list entries and the like kept in LDS
 
@@ -246,7 +247,8 @@ __global__ void __launch_bounds__(1024) k_kv_plan(mmoe_kv_plan_args a, int sh, i
     }
 }
 
-// The tokens of a large step, in a launch of their own over the whole card
+// The tokens of a large step, in a launch of their own over the whole card: 60000 in 2.7 us (their starts into LDS, then a search and two
+// dependent loads; 0.5 MB written)
 __global__ void __launch_bounds__(256) k_kv_tokens(mmoe_kv_plan_args a, int sh) {
     __shared__ int start[MMOE_KV_MAXSEQ + 1];
     for (int i = threadIdx.x; i <= a.nseq; i += 256) start[i] = a.qstart[i];
@@ -267,7 +269,9 @@ __global__ void __launch_bounds__(256) k_kv_tokens(mmoe_kv_plan_args a, int sh) 
 // Rotary positions and the cache write (mmoe_rope_kv)
 // ------------------------------------------------------------------------------------------------------
 // A workgroup takes tb tokens: their cos / sin into LDS once for all heads, then the heads in units of 8 values. The angle is
-// reduced to half turns in 64 bits (pos * freq reaches 1e6 radians, where 32 bits are 0.06 off) before the 32-bit sine.
+// reduced to half turns in 64 bits (pos * freq reaches 1e6 radians, where 32 bits are 0.06 off) before the 32-bit sine. Bound by the
+// bytes at long prompts (8191 tokens of 24 heads of 128 in bf16: 100.7 MB in 22.9 us, 4.4 TB/s; a copy of as many reaches 4.9), by latency
+// at short ones (64 tokens 3.8 us, 777 tokens 4.8 us: the angles' 64-bit product and sine beside the first heads' loads).
 #define RP_T 256
 #define RP_HALF 128   // largest rot / 2
 #define RP_TB 8       // most tokens per workgroup
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
         }
         return;
     }
-    // A head is dc lanes of one wave (dc a power of two), a unit of 8 values each; four heads' loads under way per lane, the first four
+    // A head is dc lanes of one wave (dc a power of two), a unit of 8 values each; RP_U heads' loads under way per lane, the first ones
     // beside the angles. With split pairs a lane loads its partner's unit too (the same lines again): in place, too, a head is read
     // whole before any of it is written.
     const int sd = 31 - __builtin_clz(dc), d0 = (threadIdx.x & (dc - 1)) * 8, hpr = RP_T >> sd;
@@ -581,7 +585,12 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
 // rows of V through the transposing LDS reads. A tile's keys and values go from the cache straight to LDS, one tile ahead, in 16-byte
 // pieces whose place in a row is exchanged by the row's number, so that neither the reads of 8 rows at one column nor the transposing
 // reads of 4 rows meet in a bank. P is rounded to the cache's type (half a step relative, as the result itself is), its
-// sum is of the unrounded 32-bit values.
+// sum is of the unrounded 32-bit values. With two workgroups on a CU a SIMD's two waves take turns: one's matrix products (which go
+// first, s_setprio: 6% of a long run) run beside the other's exponentials.
+// Bound at long runs: 4096 tokens over 16096 positions, 16 heads of 128, 471 GFLOP: 468 us, 1.01 PFLOP/s (a product of 8192 cubed reaches 1.28;
+// the clock falls to 1.5 GHz); with a cap 539 us (three more instructions and two of the transcendental unit per score), with a distance bias
+// 525. Short runs: 2.5 us to the first tile (sequence, limits, block ids, tile: loads that depend on each other), 1.7 us per tile of a wave
+// alone on its SIMD.
 template <int D> struct AttTileMem {
     __attribute__((aligned(1024))) uint8_t first[2 * ATT_BN(D) * D * 2];   // keys and values of a tile
     union {
@@ -919,7 +928,9 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 // of positions, its waves runs of 32 in turn, keys and values straight into registers; a run's keys give their
 // registers to the next run's as soon as its scores are there, its values after the second product. S^T = K Q^T and O^T = V^T P^T as in k_attn_tile, on 16 x 16 x 32
 // products; V^T is put together from rows by byte permutes (32 per run of 32 positions, hidden behind the loads). The waves join
-// through LDS, the chunks in k_attn_join.
+// through LDS, the chunks in k_attn_join. Measured: one token over 100000 positions of 4 key/value heads of 128, 204.8 MB in 41.1 us, 5.0 TB/s
+// (a copy of 1 GB reaches 5.06); 7 tokens over 2048 shared positions 7.9 us, latency. Two waves per SIMD: a third leaves too few registers
+// for the loads under way (52 us instead of 43).
 template <int T> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
     if (T == MMOE_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
@@ -1175,6 +1186,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
 // The partial results of a row: their maxima and sums give each a weight. D / 4 lanes read a part; with all, every such group of the
 // workgroup works on one row (the loads of a row's parts are what there is to wait for), else each has its own (up to ATT_PER parts).
 // few_only: the rows are those of the sequences of few rows, 16 per key/value head.
+// 1024 rows of 18 parts 7.8 us, 16 rows of 98 parts 5.9, 28 of 9 3.8: latency of two dependent loads (a part's maximum and sum, its values).
 #define ATT_PARTS 1024     // most partial results of a row
 #define ATT_PER 16
 template <int T, int D>

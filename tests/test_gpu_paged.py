@@ -288,6 +288,14 @@ ATTN = {
     "shared prefix, prompts": dict(qlens=[100, 1, 300], lens=[356, 300, 556], shared=256, heads=8, kv=2, pad=9),
     "shared prefix, limits": dict(qlens=[20, 1, 3], lens=[300, 280, 290], shared=256, heads=4, kv=1, lo=lambda p: p // 100 * 100, hi=lambda p: np.maximum(p + 1, 262)),
     "shared prefix longer than a sequence": dict(qlens=[1, 2, 5], lens=[100, 300, 129], shared=256, heads=4, kv=1, max_len=300),
+    "heads of 64, tiles that end inside": [dict(qlens=[60, 1, 90], lens=[300, 260, 90 + 144], heads=6, kv=2, dim=64, shared=144, kind=k, pad=3) for k in ("f16", "bf16")],
+    "heads of 64, lost blocks and values that are not finite": [
+        dict(qlens=[100, 1, 40], lens=[300, 129, 700], heads=4, kv=1, dim=64, lost=[(0, 2), (0, 17), (2, 8), (2, 43)], poison=poison(*ODD), window=w) for w in (0, 90)],
+    "heads of 64, far positions": dict(qlens=[70, 2], lens=[2300, 1111], heads=4, kv=1, dim=64, cap=20.0, alibi=True, bs=128),
+    "a prompt beside positions of one chunk and of more": [dict(qlens=[40, 1, 2], lens=[100, n, n - 5], heads=8, kv=2, window=w) for n, w in ((2047, 0), (2049, 0), (2100, 2017), (2100, 2018))],
+    "a batch over shared positions, in chunks and in tiles": [dict(qlens=[1] * n, lens=[1200 + 16 * (s % 3) for s in range(n)], heads=4, kv=1, shared=1184, kind=k) for n, k in
+                                                                     ((32, "f16"), (255, "bf16"), (257, "f16"))],
+    "runs, windows": [dict(qlens=[150, 3], lens=[n, n], heads=4, kv=1, window=w) for n, w in ((383, 0), (385, 0), (1300, 351), (1300, 353), (1300, 900))],
     "shared prefix, lost blocks": dict(qlens=[1, 2], lens=[300, 290], shared=256, heads=4, kv=2, lost=[(0, 5), (1, 5), (1, 17)]),
 }
 
