@@ -267,6 +267,8 @@ ATTN = {
     "bounds shorter than the sequences": dict(qlens=[40, 1, 3], lens=[200, 500, 90], heads=4, kv=1, max_q=7, max_len=160),
     "bounds shorter than the sequences, window": [dict(qlens=[9, 3], lens=[300, 200], heads=4, kv=1, max_q=2, window=40),
                                                   dict(qlens=[9, 3], lens=[300, 200], heads=4, kv=1, max_q=2, window=40, hi=lambda p: p + 100)],
+    "bounds of zero": [dict(qlens=[3, 1], lens=[30, 19], heads=4, kv=1, **kw) for kw in (dict(max_q=0), dict(max_q=0, shared=16), dict(max_len=0))] +
+                      [dict(qlens=[90, 1], lens=[300, 219], heads=4, kv=1, **kw) for kw in (dict(max_q=0, shared=208), dict(max_len=0))],
     "loose bounds": dict(qlens=[1, 2], lens=[200, 90], heads=16, kv=4, max_q=900, width_more=300, max_len=4000),
     "no lse": dict(qlens=[1, 30, 2], lens=[700, 90, 3], heads=4, kv=1, with_lse=False),
     "token-major cache": dict(qlens=[1, 100, 3], lens=[700, 100, 90], heads=8, kv=4, token_major=True, kind="bf16"),
