@@ -933,7 +933,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 // of positions, its waves runs of 32 in turn, keys and values straight into registers; a run's keys give their
 // registers to the next run's as soon as its scores are there, its values after the second product. S^T = K Q^T and O^T = V^T P^T as in k_attn_tile, on 16 x 16 x 32
 // products; V^T is put together from rows by byte permutes (32 per run of 32 positions, hidden behind the loads). The waves join
-// through LDS, the chunks in k_attn_join. Measured: one token over 100000 positions of 4 key/value heads of 128, 204.8 MB in 41.1 us, 5.0 TB/s
+// through LDS, the chunks in k_attn_join. Measured: one token over 100000 positions of 4 key/value heads of 128, 204.8 MB in 40.9 us, 5.0 TB/s
 // (a copy of 1 GB reaches 5.06); 7 tokens over 2048 shared positions 7.9 us, latency. Two waves per SIMD: a third leaves too few registers
 // for the loads under way (52 us instead of 43).
 template <int T> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
