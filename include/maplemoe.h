@@ -347,7 +347,8 @@ int mmoe_rope_kv(const mmoe_rope_args *a, const mmoe_kv_cache *kv);
  * lo and hi are per token: a document mask gives each token its document's first position, a prefix mask lets hi reach past
  * the token. out = softmax of the visible scores times v, lse (may be NULL) [ntok][heads] = log of the sum of their exp. A token that sees
  * nothing, or whose scores are all -inf, gets 0 and -inf. A key or value that a token does not see never reaches it, whatever it
- * holds (cache never written, infinities, NaN). Positions whose block id is not in 0 .. nblocks - 1 are seen by none.
+ * holds (cache never written, infinities, NaN); an infinite value that it does see reaches it as infinity, however small its weight (NaN, or
+ * infinities of both signs in one dim, as NaN). Positions whose block id is not in 0 .. nblocks - 1 are seen by none.
  * out rows and lse from qstart[nseq] on stay as they are.
  * shared > 0 (a multiple of block_size): the first shared positions are the same blocks in every table row (row 0's are read):
  * they are read once for all sequences instead of once for each. The result is the same.

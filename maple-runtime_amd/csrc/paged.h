@@ -469,7 +469,8 @@ struct AttArgs {
     int split_sh, split, chunk, chunks;   // runs of the shared positions, runs per row tile of the own ones; positions per chunk, most chunks
     int parts_sh;        // partial results of the shared positions: split_sh, or 0
     float s1, s2;        // cap 0: score = s1 q.k in units of log 2; else s2 tanh z, with exp(2 z) = exp2(s1 q.k)
-    // partial results, [head_dim] values over their own sum each, and their maxima (in units of log 2) and sums: of the shared positions
+    // partial results, [head_dim] values over their own sum each, and their maxima (in units of log 2) and sums (negative where results may not
+    // be finite): of the shared positions
     // [split_sh][ntok][heads], from at_tile on of row tiles over the own ones [split][ntok][heads], from at_few on of chunks [chunks][nseq][16 kv heads]
     float *po;
     float2 *pm;
@@ -578,6 +579,12 @@ __device__ __forceinline__ void att_limits(const AttArgs &A, bool shared, const 
 
 // Values of a tile that is not seen whole: are all of them finite? (bits: the type's exponent)
 template <int T> __device__ __forceinline__ bool odd16(uint32_t v) { constexpr uint32_t e = T == MMOE_BF16 ? 0x7f80 : 0x7c00; return (v & e) == e; }
+// the same of both halves of a word: bit 15 or 31 set (a carry out of the exponent; other bits are of no meaning)
+template <int T> __device__ __forceinline__ uint32_t odd_pair(uint32_t v) { return (v & 0x7fff7fffu) + (T == MMOE_BF16 ? 0x00800080u : 0x04000400u); }
+// what is left of a result whose weight has become 0
+__device__ __forceinline__ float only_odd(float y) { return __builtin_isfinite(y) ? 0.0f : y; }
+// the largest size of two numbers, NaN if one of them is
+__device__ __forceinline__ float largest_of(float x, float y) { return __builtin_elementwise_maximum(fabsf(x), fabsf(y)); }
 template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
     if (odd16<T>(v)) v &= 0xffff0000u;
     if (odd16<T>(v >> 16)) v &= 0xffffu;
@@ -719,11 +726,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 #pragma unroll
     for (int i = 0; i < DS; i++) va[i] = vr * RB + ((64 * i + 32 * ((l >> 4) & 1) + 8 * (l & 3)) ^ ((vr & (CH / 2 - 1)) << 5));
     f16v acc[DS], sc[NU];
-#pragma unroll
-    for (int i = 0; i < DS; i++)
-#pragma unroll
-        for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
-    float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f;   // mb: m - lift, - lift while m is -inf
+    float m, mb, sum;   // mb: m - lift, - lift while m is -inf
     constexpr bool FALLS = CAP && !BIAS;   // sc falls as the score grows
     constexpr float NONE = FALLS ? __builtin_inff() : -__builtin_inff();   // sc of a position that is not seen
 
@@ -820,20 +823,33 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         for (int k = 0; k < NK * DS - 4; k++) { __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); __builtin_amdgcn_sched_group_barrier(0x100, 2, 0); }
         __builtin_amdgcn_sched_group_barrier(0x8, 4, 0);
     };
-    // A value that is not finite times a weight of 0 is NaN, so in a tile that is not seen whole such values go round the product:
-    // the tile's are set aside in the other buffer and zeroed, and afterwards added, as they are, to the rows that see their position.
-    auto set_aside = [&](uint32_t buf, uint32_t other) {
+    // A value that is not finite times a weight of 0 is NaN, so in a tile that is not seen whole such values are zeroed before the product
+    // and, once all tiles are through, added as they are to the rows that see their position. In a tile seen whole the product is right unless
+    // a small weight was rounded to 0, or later scaled to 0: then the result is NaN, and the row tile begins again with every tile's
+    // values looked at (at once, that would be an eighth more reads of LDS for every call).
+    auto look = [&](uint32_t buf, int f) {   // at the wave's own rows of values
+        uint32_t o = 0;
 #pragma unroll
         for (int x = 0; x < GW * NI; x++) {
-            const uint32_t o = w * 16 * GW * RB + x * 1024 + l * 16;
-            u4 v = *(const lu4 *)((lb *)(uintptr_t)buf + o);
-            *(lu4 *)((lb *)(uintptr_t)other + o) = v;
+            u4 v = *(const lu4 *)((const lb *)(uintptr_t)buf + w * 16 * GW * RB + x * 1024 + l * 16);
+#pragma unroll
+            for (int y = 0; y < 4; y++) o |= odd_pair<T>(v[y]);
+        }
+        const bool some = __any((o & 0x80008000u) != 0);
+        if (l == 0) M.flag[f][w] = some;
+    };
+    auto found = [&](int f) { return __builtin_amdgcn_readfirstlane(M.flag[f][0] | M.flag[f][1] | M.flag[f][2] | M.flag[f][3]) != 0; };
+    auto zero_odd = [&](uint32_t buf) {
+#pragma unroll
+        for (int x = 0; x < GW * NI; x++) {
+            lu4 *at = (lu4 *)((lb *)(uintptr_t)buf + w * 16 * GW * RB + x * 1024 + l * 16);
+            u4 v = *at;
 #pragma unroll
             for (int y = 0; y < 4; y++) v[y] = only_finite<T>(v[y]);
-            *(lu4 *)((lb *)(uintptr_t)buf + o) = v;
+            *at = v;
         }
     };
-    auto add_aside = [&](uint32_t other, int p, unsigned bad) {
+    auto add_odd = [&](uint32_t buf, int p, unsigned bad) {
 #pragma unroll 1
         for (int r = 0; r < BN; r++) {
             const bool see = p + r >= R.lo && p + r < R.hi && !((bad >> (r >> 4)) & 1);
@@ -844,7 +860,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
                     typedef __attribute__((address_space(3))) uint64_t l8;
-                    uint64_t v = *(const l8 *)((const lb *)(uintptr_t)other + row + ((64 * i + 4 * j) ^ x));
+                    uint64_t v = *(const l8 *)((const lb *)(uintptr_t)buf + row + ((64 * i + 4 * j) ^ x));
 #pragma unroll
                     for (int y = 0; y < 4; y++, v >>= 16) {
                         acc[i][j + y] += see & odd16<T>((uint32_t)v) ? half_to_f<T>((uint32_t)v & 0xffff) : 0.0f;
@@ -854,38 +870,32 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         }
     };
 
-    if (p0 < p1) {
 #pragma unroll
-        for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));   // the queries are there: nothing in the loop waits for them
+    for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));   // the queries are there, on every way into the loop: nothing in it waits for them
+    bool odd = false, wild = false;   // some values were zeroed; results of the wave may not be finite
+    for (bool careful = false;; careful = true) {
+        m = -__builtin_inff(); mb = sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DS; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) acc[i][j] = 0.0f;
         for (int p = p0, i = 0; p < p1; p += BN, i ^= 1, bad = next) {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the compiler does not know of these loads
-            const uint32_t kbuf = lds + i * 2 * TB, vbuf = kbuf + TB, kother = lds + (i ^ 1) * 2 * TB, vother = kother + TB;
-            const bool part = p < glo || p + BN > ghi || bad, more = p + BN < p1;
-            if (part) {   // the wave's own rows of values: are they finite?
-                bool o = false;
-#pragma unroll
-                for (int x = 0; x < GW * NI; x++) {
-                    u4 v = *(const lu4 *)((const lb *)(uintptr_t)vbuf + w * 16 * GW * RB + x * 1024 + l * 16);
-#pragma unroll
-                    for (int y = 0; y < 4; y++) o |= odd16<T>(v[y]) | odd16<T>(v[y] >> 16);
-                }
-                o = __any(o);
-                if (l == 0) M.flag[i][w] = o;
-            }
+            const uint32_t kbuf = lds + i * 2 * TB, vbuf = kbuf + TB, kother = lds + (i ^ 1) * 2 * TB;
+            const bool part = careful || p < glo || p + BN > ghi || bad;
+            if (part) look(vbuf, i);
             __syncthreads();   // the tile has arrived, and every wave is done with the other buffers
-            bool odd = false;
-            if (part) odd = __builtin_amdgcn_readfirstlane(M.flag[i][0] | M.flag[i][1] | M.flag[i][2] | M.flag[i][3]) != 0;
-            if (more) {
+            if (p + BN < p1) {
                 blk = block_of(p + BN, next);
                 fetch(kother, A.kv.k, ko, p + BN, blk);
-                if (!odd) fetch(vother, A.kv.v, vo, p + BN, blk);
+                fetch(kother + TB, A.kv.v, vo, p + BN, blk);
             }
-            if (odd) {
-                set_aside(vbuf, vother);
+            if (part && found(i)) {
+                odd = true;
+                zero_odd(vbuf);
                 __syncthreads();
             }
-            const bool mine = p < whi && p + BN > wlo;
-            if (mine) {
+            if (p < whi && p + BN > wlo) {
                 __builtin_amdgcn_s_setprio(1);
                 scores(sc, kbuf);
                 __builtin_amdgcn_s_setprio(0);
@@ -896,11 +906,34 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                 product(vbuf);
                 __builtin_amdgcn_s_setprio(0);
             }
-            if (odd) {
-                if (mine) add_aside(vother, p, bad);
-                __syncthreads();
-                if (more) fetch(vother, A.kv.v, vo, p + BN, blk);
-            }
+        }
+        if (careful || p0 >= p1) break;
+        float top = 0.0f;
+#pragma unroll
+        for (int i = 0; i < DS; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j++) top = largest_of(top, acc[i][j]);
+        const bool lost = __any(R.live && top != top);
+        wild = __any(!(top < __builtin_inff()));
+        if (l == 0) M.range[0][w] = lost;
+        __syncthreads();
+        if (!__builtin_amdgcn_readfirstlane(M.range[0][0] | M.range[0][1] | M.range[0][2] | M.range[0][3])) break;
+        idp = INT32_MIN / 2;
+        blk = block_of(p0, bad);
+        fetch(lds, A.kv.k, ko, p0, blk);
+        fetch(lds + TB, A.kv.v, vo, p0, blk);
+    }
+    if (odd) {
+        wild = true;
+        idp = INT32_MIN / 2;
+        for (int p = p0; p < p1; p += BN) {
+            blk = block_of(p, bad);
+            __syncthreads();   // every wave is done with the buffer and the flags
+            fetch(lds, A.kv.v, vo, p, blk);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            look(lds, 0);
+            __syncthreads();
+            if (found(0) && p < whi && p + BN > wlo) add_odd(lds, p, bad);
         }
     }
     sum = add_halves(sum);
@@ -920,7 +953,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         return;
     }
     const int64_t row = (shared ? 0 : A.at_tile) + ((int64_t)split * a.ntok + R.tok) * a.heads + R.head;
-    if (hh == 0) A.pm[row] = make_float2(mb, sum);
+    if (hh == 0) A.pm[row] = make_float2(mb, wild ? -sum : sum);
     if (sum == 0.0f) return;
     float *o = A.po + row * D + 4 * hh;
 #pragma unroll
@@ -1038,7 +1071,18 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
 #pragma unroll
     for (int e = 0; e < E; e++) acc[e] = f4{0, 0, 0, 0};
     float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f;
+    bool odd = false, careful = false, wild = false;   // some values were zeroed (as in att_tile); every run's are looked at; results may not be finite
 
+    auto some_odd = [&] {   // of the run's values
+        uint32_t o = 0;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int x = 0; x < E / 2; x++) o |= odd_pair<T>(r.v[u][i][x]);
+        return __any((o & 0x80008000u) != 0) != 0;
+    };
     auto step = [&](int p, auto &&after_scores) {
         f4 s[2];
 #pragma unroll
@@ -1079,41 +1123,14 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
                 sum += e0 + e1;
                 pf[2 * u + (j >> 1)] = pack2<T>(e0, e1);
             }
-        bool odd = false;
-        if (part) {
-            bool o = false;
+        if ((careful || part) && some_odd()) {
+            odd = true;
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int x = 0; x < E / 2; x++) o |= odd16<T>(r.v[u][i][x]) | odd16<T>(r.v[u][i][x] >> 16);
-            odd = __any(o);
-        }
-        if (odd) {   // infinities and NaN go round the product, to the rows that see their position (the wave's values through its part of LDS)
-            uint32_t *t = (uint32_t *)M.joint[w];
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int x = 0; x < E / 2; x++) {
-                        t[(16 * u + 4 * g + i) * (D / 2) + n * (E / 2) + x] = r.v[u][i][x];
-                        r.v[u][i][x] = only_finite<T>(r.v[u][i][x]);
-                    }
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-            for (int k = 0; k < 32; k++) {
-                const bool see = p + k >= R.lo && p + k < R.hi && !((r.bad >> (k >> 4)) & 1);
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        uint32_t v = t[k * (D / 2) + ((4 * g + j) * E + e) / 2] >> (16 * (e & 1));
-                        acc[e][j] += see & odd16<T>(v) ? half_to_f<T>(v & 0xffff) : 0.0f;
-                    }
-            }
-            __builtin_amdgcn_wave_barrier();
+                    for (int x = 0; x < E / 2; x++) r.v[u][i][x] = only_finite<T>(r.v[u][i][x]);
         }
 #pragma unroll
         for (int e = 0; e < E; e++) {
@@ -1129,16 +1146,60 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         id = ids(p); next = ids(p + 128);
         if (p < p1) { load_k(p, id); load_v(p, id); }
     }
-    if (p < p1) {
+    const int start = p;
+    while (p < p1) {
         for (; p + 128 < p1; p += 128) {
             step(p, [&] { load_k(p + 128, next); });
             load_v(p + 128, next);
             next = ids(p + 256);
         }
         step(p, [] {});
+        if (careful) break;
+        float top = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) top = largest_of(top, acc[e][j]);
+        wild = __any(!(top < __builtin_inff()));
+        if (!__any(R.live && top != top)) break;
+        careful = true;   // once more
+        m = -__builtin_inff(); mb = sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] = f4{0, 0, 0, 0};
+        p = start;
+        id = ids(p); next = ids(p + 128);
+        load_k(p, id); load_v(p, id);
+    }
+    if (odd) {   // through the wave's part of LDS
+        wild = true;
+        uint32_t *t = (uint32_t *)M.joint[w];
+        for (p = start; p < p1; p += 128) {
+            load_v(p, ids(p));
+            if (!some_odd()) continue;
+            asm volatile("" ::: "memory");   // (words and floats in the same place)
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int x = 0; x < E / 2; x++) t[(16 * u + 4 * g + i) * (D / 2) + n * (E / 2) + x] = r.v[u][i][x];
+            __builtin_amdgcn_wave_barrier();   // a wave's LDS operations stay in order
+#pragma unroll 1
+            for (int k = 0; k < 32; k++) {
+                const bool see = p + k >= R.lo && p + k < R.hi && !((r.bad >> (k >> 4)) & 1);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int e = 0; e < E; e++) {
+                        uint32_t v = t[k * (D / 2) + ((4 * g + j) * E + e) / 2] >> (16 * (e & 1));
+                        acc[e][j] += see && odd16<T>(v) ? half_to_f<T>(v & 0xffff) : 0.0f;
+                    }
+            }
+        }
+        asm volatile("" ::: "memory");
     }
     sum = add_quarters(sum);
-    if (g == 0) M.stat[w][n] = make_float2(mb, sum);
+    if (g == 0) M.stat[w][n] = make_float2(mb, wild ? -sum : sum);   // a negative sum: look at the results also where their weight is 0
 #pragma unroll
     for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -1149,16 +1210,33 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     if (row >= at.rows) return;
     float2 st[4];
     float mx = -__builtin_inff(), total = 0.0f, o[E] = {};
+    bool any = false;   // of them not finite, perhaps
 #pragma unroll
-    for (int i = 0; i < 4; i++) { st[i] = M.stat[i][jr]; if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x); }
+    for (int i = 0; i < 4; i++) {
+        st[i] = M.stat[i][jr];
+        if (st[i].y != 0.0f) mx = fmaxf(mx, st[i].x);
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if (st[i].y == 0.0f) continue;
         float e = exp2_(st[i].x - mx);
-        total = fmaf(st[i].y, e, total);
+        total = fmaf(fabsf(st[i].y), e, total);
+        any |= st[i].y < 0.0f;
 #pragma unroll
         for (int x = 0; x < E; x++) o[x] = fmaf(e, M.joint[i][jr][d + x], o[x]);
     }
+    if (any)   // results that are not finite count whatever their weight
+#pragma unroll 1
+        for (int x = 0; x < E; x++) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float e = st[i].y != 0.0f ? exp2_(st[i].x - mx) : 0.0f, y = M.joint[i][jr][d + x];
+                if (e != 0.0f) sum = fmaf(e, y, sum); else if (st[i].y != 0.0f) sum += only_odd(y);
+            }
+#pragma unroll
+            for (int y = 0; y < E; y++) if (y == x) o[y] = sum;
+        }
     const int j = (int)A.by_group(row), tok = at.t0 + j, head = kvh * A.group + row - j * A.group;
     if (shared) {   // tokens past max_q have no partial results
         int s = max(count_le(a.qstart, a.nseq, tok) - 1, 0);
@@ -1173,7 +1251,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         return;
     }
     const int64_t at_row = shared ? ((int64_t)c * a.ntok + tok) * a.heads + head : A.at_few + ((int64_t)c * a.nseq + at.s) * 16 * A.kv.heads + j * a.heads + head;
-    if (d == 0) A.pm[at_row] = make_float2(mx, total);
+    if (d == 0) A.pm[at_row] = make_float2(mx, any ? -total : total);
     if (total == 0.0f) return;
 #pragma unroll
     for (int x = 0; x < E; x += 4) *(f4 *)(A.po + at_row * D + d + x) = f4{o[x], o[x + 1], o[x + 2], o[x + 3]};
@@ -1207,6 +1285,7 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
     constexpr int LPR = D / 4;
     const mmoe_attn_args &a = A.a;
     __shared__ float red[2][16], wt[ATT_PARTS];
+    __shared__ int odd[16];
     __shared__ union { __attribute__((aligned(16))) float acc[1024 / LPR][D]; int starts[MMOE_KV_MAXSEQ + 1]; } M;
     const int gr = blockDim.x / LPR, gi = threadIdx.x / LPR, x = (threadIdx.x % LPR) * 4, row0 = all ? blockIdx.x : blockIdx.x * gr + gi;
     int tok, head, s, t0, tokens;
@@ -1241,6 +1320,7 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
     auto part = [&](int p) { return p < A.parts_sh ? p * rows + row : own + (p - A.parts_sh) * by; };
     float m = -__builtin_inff(), sum = 0.0f;
     f4 o = {0, 0, 0, 0};
+    bool some = false;
     if (all) {
         const int l = threadIdx.x & 63, w = threadIdx.x >> 6, nw = blockDim.x >> 6;
         float2 v[ATT_PARTS / 256];
@@ -1258,21 +1338,31 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
         for (int i = 0; i < ATT_PARTS / 256; i++) {
             int p = threadIdx.x + i * blockDim.x;
             float e = v[i].y != 0.0f ? exp2_(v[i].x - m) : 0.0f;
-            if (p < parts) wt[p] = e;
-            sum = fmaf(v[i].y, e, sum);
+            const bool look = v[i].y < 0.0f && e == 0.0f;   // results that are not finite count whatever their weight
+            if (p < parts) wt[p] = look ? -1.0f : e;
+            some |= look;
+            sum = fmaf(fabsf(v[i].y), e, sum);
         }
         for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
-        if (l == 0) red[1][w] = sum;
+        some = __any(some);
+        if (l == 0) { red[1][w] = sum; odd[w] = some; }
         __syncthreads();
         sum = 0.0f;
-        for (int i = 0; i < nw; i++) sum += red[1][i];
+        for (int i = 0; i < nw; i++) { sum += red[1][i]; some |= odd[i] != 0; }
 #pragma unroll 8
         for (int p = gi; p < parts; p += gr) {
             float e = wt[p];
-            f4 y = e != 0.0f ? *(const f4 *)(A.po + part(p) * D + x) : f4{0, 0, 0, 0};
+            f4 y = e <= 0.0f ? f4{0, 0, 0, 0} : *(const f4 *)(A.po + part(p) * D + x);
 #pragma unroll
             for (int i = 0; i < 4; i++) o[i] = fmaf(e, y[i], o[i]);
         }
+        if (some)
+            for (int p = gi; p < parts; p += gr) {
+                if (wt[p] != -1.0f) continue;
+                f4 y = *(const f4 *)(A.po + part(p) * D + x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[i] += only_odd(y[i]);
+            }
         *(f4 *)&M.acc[gi][x] = o;
         __syncthreads();
         if (gi) return;
@@ -1287,9 +1377,22 @@ __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_
         for (int p = 0; p < ATT_PER; p++) {
             f4 y = v[p].y != 0.0f ? *(const f4 *)(A.po + part(p) * D + x) : f4{0, 0, 0, 0};
             float e = v[p].y != 0.0f ? exp2_(v[p].x - m) : 0.0f;
-            sum = fmaf(v[p].y, e, sum);
+            sum = fmaf(fabsf(v[p].y), e, sum);
+            some |= v[p].y < 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; i++) o[i] = fmaf(e, y[i], o[i]);
+        }
+        if (some) {   // results that are not finite count whatever their weight
+            o = f4{0, 0, 0, 0};
+#pragma unroll 1
+            for (int p = 0; p < parts; p++) {
+                const float2 v = A.pm[part(p)];
+                if (v.y == 0.0f) continue;
+                const float e = exp2_(v.x - m);
+                const f4 y = *(const f4 *)(A.po + part(p) * D + x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (e != 0.0f) o[i] = fmaf(e, y[i], o[i]); else o[i] += only_odd(y[i]);
+            }
         }
     }
     const float inv = 1.0f / sum;
