@@ -863,7 +863,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                     uint64_t v = *(const l8 *)((const lb *)(uintptr_t)buf + row + ((64 * i + 4 * j) ^ x));
 #pragma unroll
                     for (int y = 0; y < 4; y++, v >>= 16) {
-                        acc[i][j + y] += see & odd16<T>((uint32_t)v) ? half_to_f<T>((uint32_t)v & 0xffff) : 0.0f;
+                        acc[i][j + y] += see && odd16<T>((uint32_t)v) ? half_to_f<T>((uint32_t)v & 0xffff) : 0.0f;
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
