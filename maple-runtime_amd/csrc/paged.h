@@ -492,15 +492,14 @@ __device__ __forceinline__ float min_(float x, float y) { return __builtin_amdgc
 // sides). Asm, so that the compiler does not wait for them before every later LDS read; nothing is written to a register. The
 // waits are the caller's.
 template <int N> __device__ __forceinline__ void load_lds(const uint8_t *base, const uint32_t *off, uint32_t to) {
-    static_assert(N == 1 || N == 2 || N == 4, "loads");
+    static_assert(N == 2 || N == 4, "loads");
     to = __builtin_amdgcn_readfirstlane(to);
-    if (N == 1) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[0]), "s"(base), "s"(to) : "memory", "m0");
     if (N == 2)
-        asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:1024" ::"v"(off[0]), "v"(off[1]), "s"(base), "s"(to)
+        asm volatile("s_mov_b32 m0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %2\n\tglobal_load_lds_dwordx4 %1, %2 offset:0x400" ::"v"(off[0]), "v"(off[1]), "s"(base), "s"(to)
                      : "memory", "m0");
     if (N == 4)
-        asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:1024\n\t"
-                     "global_load_lds_dwordx4 %2, %4 offset:2048\n\tglobal_load_lds_dwordx4 %3, %4 offset:0xc00" ::"v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(to)
+        asm volatile("s_mov_b32 m0, %5\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %4\n\tglobal_load_lds_dwordx4 %1, %4 offset:0x400\n\t"
+                     "global_load_lds_dwordx4 %2, %4 offset:0x800\n\tglobal_load_lds_dwordx4 %3, %4 offset:0xc00" ::"v"(off[0]), "v"(off[1]), "v"(off[2]), "v"(off[3]), "s"(base), "s"(to)
                      : "memory", "m0");
 }
 // what two half-waves hold of one column
