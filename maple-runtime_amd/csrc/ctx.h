@@ -5,7 +5,6 @@
 #pragma GCC visibility push(hidden)
 int mm_ready();                            // sets the context up once; -1 without a device
 int mm_device();                           // the device it lives on (after mm_ready)
-int mm_cus();                              // its compute units
 void mm_error(const char *fmt, ...);       // mmoe_last_error's text, also to stderr
 int mm_launch(int kid, const void *f, dim3 g, dim3 b, void **args);   // one kernel on the library stream; profiled as kid
 #pragma GCC visibility pop

@@ -251,7 +251,6 @@ static int launch(int kid, F &&f) {
 // What paged.hip needs of the context (ctx.h)
 int mm_ready() { return ctx_ready(); }
 int mm_device() { return S.dev; }
-int mm_cus() { return S.ncu; }
 void mm_error(const char *fmt, ...) {
     char b[480];
     va_list ap; va_start(ap, fmt); vsnprintf(b, sizeof b, fmt, ap); va_end(ap);

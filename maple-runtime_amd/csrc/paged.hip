@@ -147,7 +147,8 @@ static int check_attn(const mmoe_attn_args *p, const mmoe_kv_cache *kv) {
 }
 
 // How a call is divided: row tiles, and runs or chunks of positions where the tiles alone are too few workgroups. Only the values in the
-// arguments count (a captured call keeps its grid), and few of them: tokens, heads, the bounds.
+// arguments count (a captured call keeps its grid), and few of them: tokens, heads, the bounds. The numbers of workgroups are for the 256 compute
+// units of the one device that the kernels are built and were measured for; a partition with fewer runs the same division in more turns.
 struct AttPlan {
     int few, chunk, chunks, tiles, split, few_sh, tiles_sh, split_sh, parts;
     int64_t at_tile, at_few, entries, wgs, join_wgs;
