@@ -270,8 +270,10 @@ int mmoe_selftest_silu(uint32_t lo, uint32_t n, unsigned long long *nbad, uint32
  *   mmoe_kv_plan      block tables, slots and positions of a step, from the sequences' lengths
  *   mmoe_rope_kv      rotary positions of its queries and keys; keys and values written into the blocks
  *   mmoe_attn_paged   attention of its queries over the blocks
- * A step of a layer is mmoe_rope_kv, mmoe_attn_paged and then mmoe_moe_dev, with one mmoe_kv_plan for all layers (each layer
- * has its own blocks and the same tables). All pointers are device memory of the library's device; the work is queued on
+ * One mmoe_kv_plan serves all layers of a step (each layer has its own blocks and the same tables); in a layer mmoe_rope_kv and
+ * mmoe_attn_paged stand between the caller's own projections: its q/k/v projections and head norms come before them, its o projection
+ * (of out, in the cache's type) and then mmoe_moe_dev after. On device memory this library has none of those projections (gpre_dense takes
+ * host arrays). All pointers are device memory of the library's device; the work is queued on
  * the library stream (mmoe_stream) without waiting, so data that another stream writes or reads has to be ordered with it
  * (an event, or a wait). The device that is current in the caller is left as it was. The calls allocate nothing and can be
  * captured into a graph; what the host passes by value (counts, bounds) is then fixed, what it passes in device memory is read at each replay.
@@ -340,9 +342,12 @@ int mmoe_rope_kv(const mmoe_rope_args *a, const mmoe_kv_cache *kv);
 
 /* Attention of nseq sequences over their blocks. Sequence s has the tokens qstart[s] .. qstart[s + 1] - 1 of q [ntok][heads][head_dim]
  * (none, one or many), its last ones of len[s] positions; query head h reads key/value head h / (heads / kv heads).
- * head_dim 64 or 128; q, out and the cache of one type, MMOE_F16 or MMOE_BF16; scores, softmax and sums in 32 bits. ntok heads at most 2^30.
+ * head_dim 64 or 128; q, out and the cache of one type, MMOE_F16 or MMOE_BF16. ntok heads at most 2^30. Scores, maxima, sums and results are
+ * held in 32 bits and rounded to out's type once; the softmax weights are rounded to that type too before they multiply the values (the matrix
+ * units take both of one type), so that out is off by up to two halves of its step instead of one: bf16 0.0023 and fp16 0.00027 (relative, root
+ * mean square) where one rounding alone is off by 0.0017 and 0.00021. gfull_attn, which keeps them in fp32, is closer to maple.c.
  *   score of position p for the token at position i:  x = scale q.k (scale 1e-20 to 1e20);  cap > 0 (at most 1024): x = cap tanh(x / cap);
- *   slopes != NULL: x -= slopes[h] |i - p|
+ *   (within 2^-21 of cap, and lse with it);  slopes != NULL: x -= slopes[h] |i - p| (sizes up to 1e8)
  *   visible: max(lo[t], i - window) <= p < min(hi[t], len[s]); lo NULL: 0; hi NULL: i + 1 (causal); window 0: unlimited
  * lo and hi are per token: a document mask gives each token its document's first position, a prefix mask lets hi reach past
  * the token. out = softmax of the visible scores times v, lse (may be NULL) [ntok][heads] = log of the sum of their exp. A token that sees
