@@ -483,7 +483,11 @@ template <int T> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
 }
 // Weights are 2^(x - m + lift): in fp16 their smallest step is 2^-24, which a tail of many small weights would be rounded to; lifted by 2^7
 // (they reach 2^15 before the maximum m follows) it is 2^-31 of the largest weight. Sums and results carry the same factor.
+// Past 2^20 a maximum takes no lift (m - lift would be rounded), and scores are rounded before it is subtracted: a fused multiply-add's own,
+// more exact one may lie half a step of m above it, and at 2^24 that is a factor of 2 in the weight.
 template <int T> constexpr float lift = T == MMOE_F16 ? 7.0f : 0.0f;
+#define ATT_FAR 1048576.0f
+template <int T> __device__ __forceinline__ float lowered(float m) { return fabsf(m) > ATT_FAR ? m : m - lift<T>; }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // the larger of two numbers, without fmaxf's quieting of each (a NaN shows in the weights, whatever the maximum then is)
 __device__ __forceinline__ float max_(float x, float y) { return __builtin_amdgcn_fmed3f(x, y, __builtin_inff()); }
@@ -726,6 +730,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     for (int i = 0; i < DS; i++) va[i] = vr * RB + ((64 * i + 32 * ((l >> 4) & 1) + 8 * (l & 3)) ^ ((vr & (CH / 2 - 1)) << 5));
     f16v acc[DS], sc[NU];
     float m, mb, sum;   // mb: m - lift, - lift while m is -inf
+    bool far;           // a maximum of the wave is past ATT_FAR
     constexpr bool FALLS = CAP && !BIAS;   // sc falls as the score grows
     constexpr float NONE = FALLS ? __builtin_inff() : -__builtin_inff();   // sc of a position that is not seen
 
@@ -781,9 +786,10 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     };
     // a new maximum only once it is 2^8 past the old: until then weights stay below 2^8 (lifted: 2^15), in every type's range
     auto rescale = [&](float mt) {
-        if (!__any(mt > m + 8.0f)) return;
-        float mn = fmaxf(m, mt), bn = mn == -__builtin_inff() ? 0.0f : mn, al = exp2_(m - bn);
-        m = mn; mb = bn - lift<T>; sum *= al;
+        if (!__any(mt - m > 8.0f)) return;
+        const float mn = fmaxf(m, mt), bn = lowered<T>(mn == -__builtin_inff() ? 0.0f : mn), al = m == -__builtin_inff() ? 0.0f : exp2_(mb - bn);
+        m = mn; mb = bn; sum *= al;
+        far = __any(fabsf(bn) > ATT_FAR);
 #pragma unroll
         for (int i = 0; i < DS; i++)
 #pragma unroll
@@ -804,12 +810,12 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         __builtin_amdgcn_sched_barrier(0);
         u4 pf[NK];
         float part = 0;
-        const float off = s0 - mb;
+        const float mul = far ? 1.0f : s1, off = far ? -mb : s0 - mb;
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll
             for (int j = 0; j < 16; j += 2) {
-                float e0 = exp2_(fmaf(sc[u][j], s1, off)), e1 = exp2_(fmaf(sc[u][j + 1], s1, off));
+                float e0 = exp2_(fmaf(sc[u][j], mul, off)), e1 = exp2_(fmaf(sc[u][j + 1], mul, off));
                 part += e0 + e1;
                 pf[2 * u + (j >> 3)][(j & 7) >> 1] = pack2<T>(e0, e1);
             }
@@ -873,7 +879,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));   // the queries are there, on every way into the loop: nothing in it waits for them
     bool odd = false, wild = false;   // some values were zeroed; results of the wave may not be finite
     for (bool careful = false;; careful = true) {
-        m = -__builtin_inff(); mb = sum = 0.0f;
+        m = -__builtin_inff(); mb = sum = 0.0f; far = false;
 #pragma unroll
         for (int i = 0; i < DS; i++)
 #pragma unroll
@@ -901,6 +907,12 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                 if (CAP || BIAS) math(sc, p);
                 if (p < inlo || p + BN > inhi || bad) mask(sc, p, bad);
                 rescale(largest(sc));
+                if (far) {
+#pragma unroll
+                    for (int u = 0; u < NU; u++)
+#pragma unroll
+                        for (int j = 0; j < 16; j++) sc[u][j] = fmaf(sc[u][j], s1, s0);
+                }
                 __builtin_amdgcn_s_setprio(1);
                 product(vbuf);
                 __builtin_amdgcn_s_setprio(0);
@@ -1107,9 +1119,9 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
                 mt = fmaxf(mt, x);
             }
         mt = max_quarters(mt);
-        if (__any(mt > m + 8.0f)) {
-            float mn = fmaxf(m, mt), bn = mn == -__builtin_inff() ? 0.0f : mn, al = exp2_(m - bn);
-            m = mn; mb = bn - lift<T>; sum *= al;
+        if (__any(mt - m > 8.0f)) {
+            const float mn = fmaxf(m, mt), bn = lowered<T>(mn == -__builtin_inff() ? 0.0f : mn), al = m == -__builtin_inff() ? 0.0f : exp2_(mb - bn);
+            m = mn; mb = bn; sum *= al;
 #pragma unroll
             for (int e = 0; e < E; e++) acc[e] *= al;
         }

@@ -142,7 +142,7 @@ def attend(q, keys, values, pos, see, scale, cap, slopes, half):
                     e = e + 2.0 ** -21 * cap
                 if slopes is not None:
                     x = x - float(slopes[h]) * far[i][m]
-                    e = e + 2.0 ** -22 * float(slopes[h]) * far[i][m]
+                    e = e + 2.0 ** -22 * abs(float(slopes[h])) * far[i][m]   # the product's size counts, whatever its sign
                 top = x.max()
                 if top == -np.inf:
                     continue
