@@ -329,7 +329,8 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
     if (LAY == RP_ODD) {
         rope_angles(a, t0, nt, cs);
         __syncthreads();
-        // the round's heads through LDS: a unit's partners start anywhere in another unit
+        // the round's heads through LDS: a unit's partners start anywhere in another unit. Two barriers a round and no loads ahead: 8191 tokens of
+        // Maple's heads with rot 20 in 29 us, with rot 64 (split) 23; 64 tokens cost the same
         const int hpr = RP_T / dc, hl = threadIdx.x / dc, d0 = (threadIdx.x - hl * dc) * 8;
         for (int j0 = 0; j0 < all; j0 += hpr) {
             int j = j0 + hl, t = j / nh;
@@ -602,9 +603,9 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
 // reads of 4 rows meet in a bank. P is rounded to the cache's type (half a step relative, as the result itself is), its
 // sum is of the unrounded 32-bit values. With two workgroups on a CU a SIMD's two waves take turns: one's matrix products (which go
 // first, s_setprio: 6% of a long run) run beside the other's exponentials.
-// Bound at long runs: 4096 tokens over 16096 positions, 16 heads of 128, 471 GFLOP: 468 us, 1.01 PFLOP/s (a product of 8192 cubed reaches 1.28;
-// the clock falls to 1.5 GHz); with a cap 539 us (three more instructions and two of the transcendental unit per score), with a distance bias
-// 525. Short runs: 2.5 us to the first tile (sequence, limits, block ids, tile: loads that depend on each other), 1.7 us per tile of a wave
+// Bound at long runs: 4096 tokens over 16096 positions, 16 heads of 128, 471 GFLOP: 451 to 472 us on several cards, 1.0 PFLOP/s (a product of
+// 8192 cubed reaches 1.28; the clock falls to 1.5 GHz); with a cap 530 to 553 (three more instructions and two of the transcendental unit per
+// score), with a distance bias 510 to 533. Short runs: 2.5 us to the first tile (sequence, limits, block ids, tile: loads that depend on each other), 1.7 us per tile of a wave
 // alone on its SIMD.
 template <int D> struct AttTileMem {
     __attribute__((aligned(1024))) uint8_t first[2 * ATT_BN(D) * D * 2];   // keys and values of a tile
@@ -625,7 +626,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     const unsigned rest = A.by_kv(block), v = (shared ? A.by_split_sh : A.by_split)(rest);
     const int kvh = block - rest * A.kv.heads, split = rest - v * nsplit;
     AttTileAt at;
-    if (!att_find(A, shared, ATT_BM, (shared ? A.tiles_sh : A.tiles) - 1 - (int)v, at)) return;   // the last tiles see most: first
+    if (!att_find(A, shared, ATT_BM, (shared ? A.tiles_sh : A.tiles) - 1 - (int)v, at)) return;   // a sequence's last tiles see most: first (the sequences in reverse order, whatever their lengths)
 
     // What the lane loads of a tile: row RPI i + l / CH of the wave's 16, piece l % CH of LDS, less the instruction's own offset (rows are at
     // least head_dim values apart, so it stays positive).
@@ -976,8 +977,8 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 // Few rows (up to 16 per key/value head: single tokens, a few drafted ones): the cache's bytes are the bound, so a workgroup takes a chunk
 // of positions, its waves runs of 32 in turn, keys and values straight into registers; a run's keys give their
 // registers to the next run's as soon as its scores are there, its values after the second product. S^T = K Q^T and O^T = V^T P^T as in k_attn_tile, on 16 x 16 x 32
-// products; V^T is put together from rows by byte permutes (32 per run of 32 positions, hidden behind the loads). The waves join
-// through LDS, the chunks in k_attn_join. Measured: one token over 100000 positions of 4 key/value heads of 128, 204.8 MB in 40.9 us, 5.0 TB/s
+// products, the weights rounded to the cache's type there too; V^T is put together from rows by byte permutes (32 per run of 32 positions, hidden
+// behind the loads). The waves join through LDS, the chunks in k_attn_join. Measured: one token over 100000 positions of 4 key/value heads of 128, 204.8 MB in 41 us, 5.0 TB/s
 // (a copy of 1 GB reaches 5.06); 7 tokens over 2048 shared positions 7.9 us, latency. Two waves per SIMD: a third leaves too few registers
 // for the loads under way (52 us instead of 43).
 template <int T> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
