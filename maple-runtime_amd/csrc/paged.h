@@ -703,7 +703,8 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         lo = min(lo, M.range[0][i]); hi = max(hi, M.range[1][i]);
         glo = max(glo, M.range[2][i]); ghi = min(ghi, M.range[3][i]);
     }
-    lo = __builtin_amdgcn_readfirstlane(lo) & ~(BN - 1); hi = __builtin_amdgcn_readfirstlane(hi);
+    const int seen = __builtin_amdgcn_readfirstlane(lo);   // the first position that any row sees
+    lo = seen & ~(BN - 1); hi = __builtin_amdgcn_readfirstlane(hi);
     glo = __builtin_amdgcn_readfirstlane(glo); ghi = __builtin_amdgcn_readfirstlane(ghi);
     if (shared) {
         p1 = lo < hi ? min(p1, hi) : p0;   // (the first tile is there, also where it lies before lo: nobody looks)
@@ -833,18 +834,22 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     // and, once all tiles are through, added as they are to the rows that see their position. In a tile seen whole the product is right unless
     // a small weight was rounded to 0, or later scaled to 0: then the result is NaN, and the row tile begins again with every tile's
     // values looked at (at once, that would be an eighth more reads of LDS for every call).
-    auto look = [&](uint32_t buf, int f) {   // at the wave's own rows of values
-        uint32_t o = 0;
+    auto look = [&](uint32_t buf, int p, int f) {   // at the wave's own rows of values: 1 for those that are not finite, 2 if some row of the tile may see one
+        uint32_t o = 0, see = 0;
 #pragma unroll
         for (int x = 0; x < GW * NI; x++) {
             u4 v = *(const lu4 *)((const lb *)(uintptr_t)buf + w * 16 * GW * RB + x * 1024 + l * 16);
+            uint32_t mine = 0;
 #pragma unroll
-            for (int y = 0; y < 4; y++) o |= odd_pair<T>(v[y]);
+            for (int y = 0; y < 4; y++) mine |= odd_pair<T>(v[y]);
+            const int at = p + w * 16 * GW + x * RPI + l / CH;
+            o |= mine;
+            see |= at >= seen && at < hi ? mine : 0;
         }
-        const bool some = __any((o & 0x80008000u) != 0);
-        if (l == 0) M.flag[f][w] = some;
+        const int bits = (__any((o & 0x80008000u) != 0) ? 1 : 0) | (__any((see & 0x80008000u) != 0) ? 2 : 0);
+        if (l == 0) M.flag[f][w] = bits;
     };
-    auto found = [&](int f) { return __builtin_amdgcn_readfirstlane(M.flag[f][0] | M.flag[f][1] | M.flag[f][2] | M.flag[f][3]) != 0; };
+    auto found = [&](int f) { return __builtin_amdgcn_readfirstlane(M.flag[f][0] | M.flag[f][1] | M.flag[f][2] | M.flag[f][3]); };
     auto zero_odd = [&](uint32_t buf) {
 #pragma unroll
         for (int x = 0; x < GW * NI; x++) {
@@ -878,7 +883,8 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 
 #pragma unroll
     for (int s = 0; s < KS; s++) asm volatile("" : "+v"(q[s]));   // the queries are there, on every way into the loop: nothing in it waits for them
-    bool odd = false, wild = false;   // some values were zeroed; results of the wave may not be finite
+    int odd0 = INT32_MAX, odd1 = 0;   // the tiles in which some row may see a value that was zeroed
+    bool wild = false;                // results of the wave may not be finite
     for (bool careful = false;; careful = true) {
         m = -__builtin_inff(); mb = sum = 0.0f; far = false;
 #pragma unroll
@@ -889,15 +895,16 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the compiler does not know of these loads
             const uint32_t kbuf = lds + i * 2 * TB, vbuf = kbuf + TB, kother = lds + (i ^ 1) * 2 * TB;
             const bool part = careful || p < glo || p + BN > ghi || bad;
-            if (part) look(vbuf, i);
+            if (part) look(vbuf, p, i);
             __syncthreads();   // the tile has arrived, and every wave is done with the other buffers
             if (p + BN < p1) {
                 blk = block_of(p + BN, next);
                 fetch(kother, A.kv.k, ko, p + BN, blk);
                 fetch(kother + TB, A.kv.v, vo, p + BN, blk);
             }
-            if (part && found(i)) {
-                odd = true;
+            const int odd = part ? found(i) : 0;
+            if (odd) {
+                if (odd & 2) { odd0 = min(odd0, p); odd1 = p + 1; }
                 zero_odd(vbuf);
                 __syncthreads();
             }
@@ -935,17 +942,17 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         fetch(lds, A.kv.k, ko, p0, blk);
         fetch(lds + TB, A.kv.v, vo, p0, blk);
     }
-    if (odd) {
+    if (odd0 < odd1) {
         wild = true;
         idp = INT32_MIN / 2;
-        for (int p = p0; p < p1; p += BN) {
+        for (int p = odd0; p < odd1; p += BN) {
             blk = block_of(p, bad);
             __syncthreads();   // every wave is done with the buffer and the flags
             fetch(lds, A.kv.v, vo, p, blk);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            look(lds, 0);
+            look(lds, p, 0);
             __syncthreads();
-            if (found(0) && p < whi && p + BN > wlo) add_odd(lds, p, bad);
+            if ((found(0) & 2) && p < whi && p + BN > wlo) add_odd(lds, p, bad);
         }
     }
     sum = add_halves(sum);
@@ -1076,24 +1083,31 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     }
     const float slope = BIAS ? a.slopes[R.head] * ATT_LOG2E : 0.0f;
     const bool some = R.live && R.lo < R.hi;
-    int p0 = max(from, wave_min(some ? R.lo : INT32_MAX) & ~31), p1 = min(end, wave_max(some ? R.hi : 0));
+    const int seen = wave_min(some ? R.lo : INT32_MAX);   // the first position that any row sees
+    int p0 = max(from, seen & ~31), p1 = min(end, wave_max(some ? R.hi : 0));
     if (p0 >= p1) p0 = p1 = 0;   // nothing seen (p0 may be close to the largest int: no wave's first run is counted from it)
     const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
     f4 acc[E];
 #pragma unroll
     for (int e = 0; e < E; e++) acc[e] = f4{0, 0, 0, 0};
     float m = -__builtin_inff(), mb = 0.0f, sum = 0.0f;
-    bool odd = false, careful = false, wild = false;   // some values were zeroed (as in att_tile); every run's are looked at; results may not be finite
+    int odd0 = INT32_MAX, odd1 = 0;         // the runs in which some row may see a value that was zeroed (as in att_tile)
+    bool careful = false, wild = false;     // every run's values are looked at; results may not be finite
 
-    auto some_odd = [&] {   // of the run's values
-        uint32_t o = 0;
+    auto look = [&](int p) {   // at the run's values: 1 for those that are not finite, 2 if some row may see one
+        uint32_t o = 0, see = 0;
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
+            for (int i = 0; i < 4; i++) {
+                uint32_t mine = 0;
 #pragma unroll
-                for (int x = 0; x < E / 2; x++) o |= odd_pair<T>(r.v[u][i][x]);
-        return __any((o & 0x80008000u) != 0) != 0;
+                for (int x = 0; x < E / 2; x++) mine |= odd_pair<T>(r.v[u][i][x]);
+                const int at = p + 16 * u + 4 * g + i;
+                o |= mine;
+                see |= at >= seen && at < p1 ? mine : 0;
+            }
+        return (__any((o & 0x80008000u) != 0) ? 1 : 0) | (__any((see & 0x80008000u) != 0) ? 2 : 0);
     };
     auto step = [&](int p, auto &&after_scores) {
         f4 s[2];
@@ -1135,8 +1149,9 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
                 sum += e0 + e1;
                 pf[2 * u + (j >> 1)] = pack2<T>(e0, e1);
             }
-        if ((careful || part) && some_odd()) {
-            odd = true;
+        const int odd = careful || part ? look(p) : 0;
+        if (odd) {
+            if (odd & 2) { odd0 = min(odd0, p); odd1 = p + 1; }
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -1182,12 +1197,12 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         id = ids(p); next = ids(p + 128);
         load_k(p, id); load_v(p, id);
     }
-    if (odd) {   // through the wave's part of LDS
+    if (odd0 < odd1) {   // through the wave's part of LDS
         wild = true;
         uint32_t *t = (uint32_t *)M.joint[w];
-        for (p = start; p < p1; p += 128) {
+        for (p = odd0; p < odd1; p += 128) {
             load_v(p, ids(p));
-            if (!some_odd()) continue;
+            if (!(look(p) & 2)) continue;
             asm volatile("" ::: "memory");   // (words and floats in the same place)
 #pragma unroll
             for (int u = 0; u < 2; u++)
