@@ -605,8 +605,8 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
 // first, s_setprio: 6% of a long run) run beside the other's exponentials.
 // Bound at long runs: 4096 tokens over 16096 positions, 16 heads of 128, 471 GFLOP: 451 to 472 us on several cards, 1.0 PFLOP/s (a product of
 // 8192 cubed reaches 1.28; the clock falls to 1.5 GHz); with a cap 530 to 553 (three more instructions and two of the transcendental unit per
-// score), with a distance bias 510 to 533. Short runs: 2.5 us to the first tile (sequence, limits, block ids, tile: loads that depend on each other), 1.7 us per tile of a wave
-// alone on its SIMD.
+// score), with a distance bias 510 to 533. Short runs: 2.5 us to the first tile (sequence, limits, block ids, tile: loads that depend on each
+// other), 1.7 us per tile of a wave alone on its SIMD.
 template <int D> struct AttTileMem {
     __attribute__((aligned(1024))) uint8_t first[2 * ATT_BN(D) * D * 2];   // keys and values of a tile
     union {
@@ -626,7 +626,8 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     const unsigned rest = A.by_kv(block), v = (shared ? A.by_split_sh : A.by_split)(rest);
     const int kvh = block - rest * A.kv.heads, split = rest - v * nsplit;
     AttTileAt at;
-    if (!att_find(A, shared, ATT_BM, (shared ? A.tiles_sh : A.tiles) - 1 - (int)v, at)) return;   // a sequence's last tiles see most: first (the sequences in reverse order, whatever their lengths)
+    // a sequence's last tiles see most: first (the sequences in reverse order, whatever their lengths)
+    if (!att_find(A, shared, ATT_BM, (shared ? A.tiles_sh : A.tiles) - 1 - (int)v, at)) return;
 
     // What the lane loads of a tile: row RPI i + l / CH of the wave's 16, piece l % CH of LDS, less the instruction's own offset (rows are at
     // least head_dim values apart, so it stays positive).
@@ -834,7 +835,8 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     // and, once all tiles are through, added as they are to the rows that see their position. In a tile seen whole the product is right unless
     // a small weight was rounded to 0, or later scaled to 0: then the result is NaN, and the row tile begins again with every tile's
     // values looked at (at once, that would be an eighth more reads of LDS for every call).
-    auto look = [&](uint32_t buf, int p, int f) {   // at the wave's own rows of values: 1 for those that are not finite, 2 if some row of the tile may see one
+    // the wave's own rows of values: 1 if some are not finite, 2 if a row of the tile may see one
+    auto look = [&](uint32_t buf, int p, int f) {
         uint32_t o = 0, see = 0;
 #pragma unroll
         for (int x = 0; x < GW * NI; x++) {
@@ -985,9 +987,9 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
 // of positions, its waves runs of 32 in turn, keys and values straight into registers; a run's keys give their
 // registers to the next run's as soon as its scores are there, its values after the second product. S^T = K Q^T and O^T = V^T P^T as in k_attn_tile, on 16 x 16 x 32
 // products, the weights rounded to the cache's type there too; V^T is put together from rows by byte permutes (32 per run of 32 positions, hidden
-// behind the loads). The waves join through LDS, the chunks in k_attn_join. Measured: one token over 100000 positions of 4 key/value heads of 128, 204.8 MB in 41 us, 5.0 TB/s
-// (a copy of 1 GB reaches 5.06); 7 tokens over 2048 shared positions 7.9 us, latency. Two waves per SIMD: a third leaves too few registers
-// for the loads under way (52 us instead of 43).
+// behind the loads). The waves join through LDS, the chunks in k_attn_join. Measured: one token over 100000 positions of 4 key/value heads
+// of 128, 204.8 MB in 41 us, 5.0 TB/s (a copy of 1 GB reaches 5.06); 7 tokens over 2048 shared positions 7.9 us, latency. Two waves per SIMD:
+// a third leaves too few registers for the loads under way (52 us instead of 43).
 template <int T> __device__ __forceinline__ f4 mfma16(u4 a, u4 b, f4 c) {
     if (T == MMOE_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
@@ -1094,7 +1096,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     int odd0 = INT32_MAX, odd1 = 0;         // the runs in which some row may see a value that was zeroed (as in att_tile)
     bool careful = false, wild = false;     // every run's values are looked at; results may not be finite
 
-    auto look = [&](int p) {   // at the run's values: 1 for those that are not finite, 2 if some row may see one
+    auto look = [&](int p) {   // the run's values: 1 if some are not finite, 2 if a row may see one
         uint32_t o = 0, see = 0;
 #pragma unroll
         for (int u = 0; u < 2; u++)
