@@ -1,0 +1,717 @@
+"""Performance cases of the operators around drafted tokens and shared blocks, for a server of many sequences.
+
+Kinds of case (a case is a dict of plain values; `kind` says what it calls):
+
+  tree    a step's drafts, trees of tokens that may come next: which of a sequence's new tokens each of them follows, as bits, and
+          their positions (mmoe_tree_plan).
+  attn    attention of the drafted tokens over the blocks: each sees its sequence's cached positions and the drafted tokens on its own
+          path (mmoe_attn_tree); with a window, a cap, a bias that falls with the distance, a prefix that all sequences share.
+  verify  the end of such a step: the path that agrees with the model's own choices (mmoe_tree_accept), its keys and values moved
+          together in every layer (mmoe_kv_compact), the blocks behind them given back (mmoe_kv_free).
+  evict   a long sequence of which only some positions stay: their keys and values moved together in every layer (mmoe_kv_compact).
+  fork    copies of sequences that share their full blocks (mmoe_kv_fork) and get the begun one's contents in every layer
+          (mmoe_kv_copy); with `beams` the step of a beam search, which then gives the old rows back (mmoe_kv_free).
+
+The lengths of a case's sequences are a fixed ragged pattern between two bounds; a seed shuffles them and changes every value and
+tree. Caches are [layer][keys, values][block][key/value head][position in the block][dim]. The heads are Maple's (16 query and 4
+key/value heads of 128, 24 layers, window 512) or generic.
+"""
+import math
+import os
+import sys
+
+import numpy as np
+import torch
+
+own = False
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+VOCAB = 151936
+
+
+# ---------------------------------------------------------------------------------------------------- cases
+def _tree(nseq, nodes, back=12, ctx=4000, pad=0):
+    return dict(kind="tree", nseq=nseq, n_lo=nodes[0], n_hi=nodes[1], back=back, ctx=ctx, pad=pad)
+
+
+def _attn(nseq, nodes, ctx, shared=0, type="bf16", heads=16, kv=4, dim=128, bs=16, cap=0.0, alibi=False, window=0, back=12):
+    return dict(kind="attn", nseq=nseq, n_lo=nodes[0], n_hi=nodes[1], ctx_lo=ctx[0], ctx_hi=ctx[1], shared=shared, type=type, heads=heads, kv=kv, dim=dim,
+                bs=bs, cap=cap, alibi=alibi, window=window, back=back)
+
+
+def _verify(nseq, nodes, ctx, layers=24, type="f16", kv=4, dim=128, bs=16, back=12, agree=0.8):
+    return dict(kind="verify", nseq=nseq, n_lo=nodes[0], n_hi=nodes[1], ctx=ctx, layers=layers, type=type, kv=kv, dim=dim, bs=bs, back=back, agree=agree)
+
+
+def _evict(nseq, length, part, layers=24, type="f16", kv=4, dim=128, bs=16):
+    return dict(kind="evict", nseq=nseq, len_lo=length[0], len_hi=length[1], part=part, layers=layers, type=type, kv=kv, dim=dim, bs=bs)
+
+
+def _fork(nseq, copies, ctx, beams=False, layers=24, type="f16", kv=4, dim=128, bs=16, shared=0):
+    return dict(kind="fork", nseq=nseq, copies=copies, ctx_lo=ctx[0], ctx_hi=ctx[1], beams=beams, layers=layers, type=type, kv=kv, dim=dim, bs=bs, shared=shared)
+
+
+def listed():
+    return [
+        # the drafts of a decode step of 64 sequences
+        dict(_tree(64, (10, 40)), name="tree_64"),
+        # large drafts of many sequences (a small draft model on a card of its own), deep trees, into a padded batch
+        dict(_tree(200, (300, 512), back=6, pad=61), name="tree_200_large"),
+        # one sequence with one draft: the latency end
+        dict(_attn(1, (26, 26), (700, 700), type="f16"), name="attn_1"),
+        # a decode step of 64 sequences: Maple's heads
+        dict(_attn(64, (10, 40), (50, 3000), type="f16"), name="attn_64"),
+        # the layers of the same model with a window, longer sequences, full trees of 64
+        dict(_attn(32, (64, 64), (200, 5000), window=512, bs=64), name="attn_window_32"),
+        # a common prompt, each query head with its own keys, heads of 64, a distance bias
+        dict(_attn(17, (5, 61), (1, 900), shared=2048, heads=12, kv=12, dim=64, alibi=True), name="attn_alibi_shared_17"),
+        # large trees over long sequences, capped scores
+        dict(_attn(4, (100, 200), (20000, 30000), cap=30.0, bs=32), name="attn_long_4"),
+        # the end of a step of a few sequences, and of many
+        dict(_verify(5, (4, 26), 100), name="verify_5"),
+        dict(_verify(64, (10, 40), 100), name="verify_64"),
+        # a sequence of 20000 positions cut down to about 8000 that matter
+        dict(_evict(1, (20000, 20000), 0.4), name="evict_20000"),
+        # eight answers to each of four prompts
+        dict(_fork(4, 8, (300, 2000)), name="fork_samples_4x8"),
+        # a step of a beam search: sixteen requests with four beams each
+        dict(_fork(16, 4, (50, 800), beams=True, bs=32), name="fork_beams_16x4"),
+    ]
+
+
+def _log(rng, lo, hi):
+    return min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi + 1))))))
+
+
+def draw(rng):
+    kind = rng.choice(["tree", "attn", "attn", "attn", "attn", "verify", "evict", "fork"])
+    bs, back = rng.choice([16, 16, 32, 64]), rng.choice([1, 4, 12, 60])
+    if kind == "tree":
+        hi = _log(rng, 1, 512)
+        return _tree(_log(rng, 1, 200), (rng.randint(1, hi), hi), back=back, ctx=_log(rng, 1, 100000), pad=rng.choice([0, _log(rng, 1, 100)]))
+    type = rng.choice(["f16", "bf16"])
+    if kind == "attn":
+        kv, dim = rng.choice([1, 2, 4, 4, 8]), rng.choice([64, 128, 128])
+        heads = kv * rng.choice([1, 2, 3, 4, 4, 4])
+        nseq = _log(rng, 1, 96)
+        hi = _log(rng, 2, max(2, min(512, 2560 // nseq)))
+        ctx = _log(rng, 1, min(30000, 192000 // nseq, int(3.5e8) // (nseq * hi * heads)))
+        shared = bs * (_log(rng, 64, 12000) // bs) if rng.random() < 0.25 and nseq > 1 and nseq * hi * heads < 20000 else 0
+        return _attn(nseq, (rng.randint(1, hi), hi), (rng.randint(0, ctx), ctx), shared=shared, type=type, heads=heads, kv=kv, dim=dim, bs=bs, back=back,
+                     cap=rng.choice([0.0, 0.0, 30.0]), alibi=rng.random() < 0.25, window=rng.choice([0, 0, _log(rng, 600, 4000)]))
+    more = dict(layers=rng.choice([1, 6, 24, 24]), type=type, kv=rng.choice([1, 2, 4, 8]), dim=rng.choice([64, 128, 128]), bs=bs)
+    if kind == "verify":
+        hi = _log(rng, 1, 64)
+        return _verify(_log(rng, 1, 64), (rng.randint(1, hi), hi), _log(rng, 1, 100), back=back, agree=round(rng.uniform(0.3, 0.95), 2), **more)
+    if kind == "evict":
+        more["kv"] = rng.choice([1, 2, 4])
+        nseq = _log(rng, 1, 16)
+        hi = _log(rng, 64, 20000 // nseq)
+        return _evict(nseq, (rng.randint(1, hi), hi), round(rng.uniform(0.02, 0.9), 2), **more)
+    more["kv"] = rng.choice([1, 2, 4])
+    nseq, copies = _log(rng, 1, 16), _log(rng, 2, 8)
+    hi = _log(rng, 1, 8000 // nseq)
+    shared = bs * rng.randint(1, 8) if rng.random() < 0.25 else 0
+    return _fork(nseq, copies, (rng.randint(1, hi), hi), beams=rng.random() < 0.5, shared=shared, **more)
+
+
+def _ragged(n, lo, hi):
+    """n lengths between lo and hi, spread evenly and out of order"""
+    return [lo + int((hi - lo + 1) * ((i + 0.5) * 0.6180339887498949 % 1.0)) for i in range(n)]
+
+
+def _up(a, b):
+    return -(-a // b)
+
+
+# ---------------------------------------------------------------------------------------------------- inputs
+def _gen(seed, *key):
+    g = torch.Generator(device="cuda")
+    s = int(seed)
+    for k in key:
+        s = (s * 1000003 + int(k) + 12345) % (1 << 62)
+    g.manual_seed(s)
+    return g
+
+
+def _normal(g, shape, type):
+    return torch.randn(shape, device="cuda", generator=g, dtype=torch.float32).to(TYPES[type])
+
+
+def _ints(a):
+    return torch.from_numpy(np.ascontiguousarray(a, np.int32)).cuda()
+
+
+def _room(*shape):
+    return torch.full(shape, -1, dtype=torch.int32, device="cuda")
+
+
+def _parents(r, nodes, back):
+    """one tree after the other: node i of a tree follows one of the `back` nodes before it"""
+    i = np.concatenate([np.arange(n) for n in nodes])
+    lo = np.maximum(i - back, 0)
+    return np.where(i > 0, lo + (r.rand(len(i)) * (i - lo)).astype(np.int64), -1)
+
+
+def _nodes(case, r=None):
+    """(nodes, cached positions) of a case's sequences, in an order of the seed's"""
+    n = np.array(_ragged(case["nseq"], case["n_lo"], case["n_hi"]))
+    lo, hi = (case["ctx_lo"], case["ctx_hi"]) if "ctx_lo" in case else (case["ctx"] // 3, case["ctx"])
+    ctx = case.get("shared", 0) + np.array(_ragged(case["nseq"], lo, hi))[::-1]
+    if r is not None:
+        order = r.permutation(case["nseq"])
+        n, ctx = n[order], ctx[order]
+    return n, ctx
+
+
+def _table(r, held, keep, spare):
+    """a table of the sequences' blocks in random places, the first `keep` of every row the same ones; what is left of the blocks"""
+    nblocks = keep + int((held - keep).sum()) + spare
+    ids = r.permutation(nblocks)
+    table = np.full((len(held), int(held.max())), -1, np.int32)
+    table[:, :keep] = ids[:keep]
+    at = keep
+    for s, h in enumerate(held):
+        table[s, keep:h] = ids[at:at + h - keep]
+        at += h - keep
+    return table, ids[at:], nblocks
+
+
+def _caches(case, seed, nblocks):
+    """every layer's keys and values; one block behind the cache's own, which the plain forms write where nothing is to be written"""
+    c = torch.empty((case["layers"], 2, nblocks + 1, case["kv"], case["bs"], case["dim"]), dtype=TYPES[case["type"]], device="cuda")
+    return c.normal_(generator=_gen(seed, 3))
+
+
+def _prepare_tree(case, seed):
+    r = np.random.RandomState(seed % (1 << 32))
+    nodes, ctx = _nodes(case, r)
+    ntok = int(nodes.sum()) + case["pad"]
+    parent = np.full(ntok, -1)
+    parent[:ntok - case["pad"]] = _parents(r, nodes, case["back"])
+    words = _up(int(nodes.max()), 64)
+    return dict(kind="tree", n=case["nseq"], ntok=ntok, words=words, most=int(nodes.max()), qstart=_ints(np.concatenate([[0], np.cumsum(nodes)])),
+                len=_ints(ctx + nodes), parent=_ints(parent), pos=_room(ntok), bits=torch.zeros((ntok, words), dtype=torch.int64, device="cuda"))
+
+
+def _prepare_attn(case, seed):
+    r = np.random.RandomState(seed % (1 << 32))
+    nodes, ctx = _nodes(case, r)
+    bs, heads, whole, ntok = case["bs"], case["heads"], ctx + nodes, int(nodes.sum())
+    table, _, nblocks = _table(r, _up(whole, bs), case["shared"] // bs, 1)
+    parent = _parents(r, nodes, case["back"])
+    most = int(nodes.max())
+    qstart, parent_ = _ints(np.concatenate([[0], np.cumsum(nodes)])), _ints(parent)
+    bits = _bits(_paths(qstart, parent_, most), _up(most, 64))
+    cache = lambda k: _normal(_gen(seed, k), (nblocks, case["kv"], bs, case["dim"]), case["type"])  # noqa: E731
+    return dict(kind="attn", n=case["nseq"], bs=bs, dim=case["dim"], kv=case["kv"], heads=heads, shared=case["shared"], ntok=ntok, width=table.shape[1],
+                type=case["type"], cap=case["cap"], window=case["window"], max_q=most, max_len=int(whole.max()), scale=case["dim"] ** -0.5,
+                q=(_normal(_gen(seed, 5), (ntok, heads, case["dim"]), "f32") * 1.5).to(TYPES[case["type"]]), k_cache=cache(6), v_cache=cache(7),
+                qstart=qstart, len=_ints(whole), table=_ints(table), parent=parent_, bits=bits, words=bits.shape[1],
+                slopes=2.0 ** (-8.0 * torch.arange(1, heads + 1, dtype=torch.float32, device="cuda") / heads) if case["alibi"] else None,
+                out=torch.zeros((ntok, heads, case["dim"]), dtype=TYPES[case["type"]], device="cuda"),
+                lse=torch.zeros((ntok, heads), dtype=torch.float32, device="cuda"))
+
+
+def _prepare_verify(case, seed):
+    r = np.random.RandomState(seed % (1 << 32))
+    nodes, ctx = _nodes(case, r)
+    n, bs, ntok = case["nseq"], case["bs"], int(nodes.sum())
+    table, rest, nblocks = _table(r, _up(ctx + nodes, bs), 0, 40)
+    parent = _parents(r, nodes, case["back"])
+    token = r.randint(0, VOCAB, ntok)
+    # the model's choice behind a node: with probability `agree` one of the drafted tokens that follow it, if any do
+    start = np.concatenate([[0], np.cumsum(nodes)])
+    follows = parent + np.repeat(start[:-1], nodes)
+    choice = r.randint(0, VOCAB, ntok)
+    some = r.permutation(np.nonzero((parent >= 0) & (r.rand(ntok) < case["agree"]))[0])
+    choice[follows[some]] = token[some]
+    free = np.full(nblocks, -1)
+    free[:len(rest)] = rest
+    return dict(kind="verify", n=n, ntok=ntok, most=int(nodes.max()), layers=case["layers"], kv=case["kv"], dim=case["dim"], bs=bs, type=case["type"],
+                width=table.shape[1], nblocks=nblocks, qstart=_ints(start), len=_ints(ctx + nodes), parent=_ints(parent), token=_ints(token),
+                next=_ints(choice), table=_ints(table), free=_ints(free), nfree=_ints([len(rest)]), nfree_out=_room(1), kept=_room(ntok), count=_room(n),
+                ctx=_room(n), left=_room(n), last=_room(n), cache=_caches(case, seed, nblocks))
+
+
+def _stay(case):
+    """(length, positions that stay) of an evict case's sequences"""
+    whole = np.array(_ragged(case["nseq"], case["len_lo"], case["len_hi"]))
+    return whole, np.maximum(1, (whole * case["part"]).astype(np.int64))
+
+
+def _prepare_evict(case, seed):
+    r = np.random.RandomState(seed % (1 << 32))
+    whole, stay = _stay(case)
+    table, _, nblocks = _table(r, _up(whole, case["bs"]), 0, 1)
+    # the first positions stay, as they do in earnest, and the last ones; what lies between by chance
+    kept = []
+    for n, k in zip(whole, stay):
+        ends = min(k, 8) // 2
+        some = ends + r.permutation(n - 2 * ends)[:k - 2 * ends]
+        kept.append(np.sort(np.concatenate([np.arange(ends), some, np.arange(n - ends, n)])))
+    return dict(kind="evict", n=case["nseq"], layers=case["layers"], kv=case["kv"], dim=case["dim"], bs=case["bs"], type=case["type"],
+                width=table.shape[1], nblocks=nblocks, ntok=int(stay.sum()), qstart=_ints(np.concatenate([[0], np.cumsum(stay)])), count=_ints(stay),
+                kept=_ints(np.concatenate(kept)), table=_ints(table), cache=_caches(case, seed, nblocks))
+
+
+def _prepare_fork(case, seed):
+    r = np.random.RandomState(seed % (1 << 32))
+    bs, shared, copies, reqs = case["bs"], case["shared"], case["copies"], case["nseq"]
+    keep = shared // bs
+    ctx = shared + np.array(_ragged(reqs, case["ctx_lo"], case["ctx_hi"]))[r.permutation(reqs)]
+    held = _up(ctx, bs)
+    rows = reqs * copies if case["beams"] else reqs * (copies + 1)
+    forks = reqs * copies
+    table, rest, nblocks = _table(r, held, keep, forks * 2 + 7)
+    holders = np.zeros(nblocks, np.int64)
+    whole = np.zeros(rows, np.int64)
+    wide = np.full((rows, table.shape[1] + 2), -1, np.int32)
+    used = 0
+    if case["beams"]:   # a request's beams share their full blocks and have a begun one each; next they follow beams by chance
+        for q in range(reqs):
+            for b in range(copies):
+                wide[q * copies + b, :held[q]] = table[q, :held[q]]
+                if b and ctx[q] % bs:
+                    wide[q * copies + b, held[q] - 1] = rest[used]
+                    used += 1
+            holders[table[q, keep:ctx[q] // bs]] = copies - 1
+        whole[:] = np.repeat(ctx, copies)
+        src, dst = np.repeat(np.arange(reqs) * copies, copies) + r.randint(0, copies, forks), np.arange(forks)
+    else:               # the rows behind the prompts' become their copies
+        wide[:reqs, :table.shape[1]] = table
+        whole[:reqs] = ctx
+        src, dst = np.repeat(np.arange(reqs), copies), reqs + np.arange(forks)
+    free = np.full(nblocks, -1)
+    free[:len(rest) - used] = rest[used:]
+    t = _ints(wide)
+    return dict(kind="fork", n=rows, forks=forks, beams=case["beams"], layers=case["layers"], kv=case["kv"], dim=case["dim"], bs=bs, shared=shared,
+                type=case["type"], width=wide.shape[1], nblocks=nblocks, src=_ints(src), dst=_ints(dst), ctx=_ints(whole), table=t,
+                ctx_out=_room(rows) if case["beams"] else None, table_out=_room(*wide.shape) if case["beams"] else None, holders=_ints(holders),
+                free=_ints(free), nfree=_ints([len(rest) - used]), nfree_out=_room(1), nfree_end=_room(1), old=_room(rows),
+                none=torch.zeros(rows, dtype=torch.int32, device="cuda"), from_=_room(forks), to=_room(forks), copied=_room(forks),
+                cache=_caches(case, seed, nblocks))
+
+
+def prepare(case, seed):
+    return dict(tree=_prepare_tree, attn=_prepare_attn, verify=_prepare_verify, evict=_prepare_evict, fork=_prepare_fork)[case["kind"]](case, seed)
+
+
+# ---------------------------------------------------------------------------------------------------- plain forms
+def _padded(qstart, most):
+    """[seq][node] places of the nodes, each sequence's as many as the longest has, and which of them are nodes"""
+    start, j = qstart.long(), torch.arange(most, device=qstart.device)
+    return start[:-1, None] + j, j < (start[1:] - start[:-1])[:, None]
+
+
+def _paths(qstart, parent, most):
+    """[token][node]: is it the token itself or one that it follows? By steps that double: what a node's 2^i-th ancestor sees, it sees"""
+    at, live = _padded(qstart, most)
+    n, j = at.shape[0], torch.arange(most, device=qstart.device)
+    up = torch.where(live, parent.long()[at.clamp_max(parent.shape[0] - 1)], -1)
+    sees = torch.eye(most, dtype=torch.bool, device=qstart.device).expand(n, -1, -1)
+    for _ in range(max(1, (most - 1).bit_length())):
+        to = up.clamp_min(0)
+        further = up >= 0
+        sees = sees | (sees.gather(1, to[..., None].expand(-1, -1, most)) & further[..., None])
+        up = torch.where(further, up.gather(1, to), -1)
+    t = torch.arange(parent.shape[0], device=qstart.device)
+    start = qstart.long()
+    seq = torch.searchsorted(start[1:], t, right=True)
+    live = seq < n
+    seq = seq.clamp_max(n - 1)
+    return sees[seq, (t - start[seq]).clamp(0, most - 1)] & live[:, None] & (j >= 0)
+
+
+def _bits(sees, words):
+    """[token][node] truth values as words of 64 bits"""
+    b = torch.zeros((sees.shape[0], words * 64), dtype=torch.int64, device=sees.device)
+    b[:, :sees.shape[1]] = sees
+    return (b.reshape(-1, words, 64) << torch.arange(64, device=sees.device)).sum(-1)
+
+
+def _plain_tree(s):
+    sees = _paths(s["qstart"], s["parent"], s["most"])
+    t, start, whole = torch.arange(s["ntok"], device=sees.device), s["qstart"].long(), s["len"].long()
+    seq = torch.searchsorted(start[1:], t, right=True)
+    live = seq < s["n"]
+    seq = seq.clamp_max(s["n"] - 1)
+    pos = whole[seq] - (start[seq + 1] - start[seq]) + sees.sum(-1) - 1
+    return dict(pos=torch.where(live, pos, 0).to(torch.int32), bits=_bits(sees, s["words"]))
+
+
+def _plain_attn(s):
+    n, g, dim, maxq, dev = s["n"], s["heads"] // s["kv"], s["dim"], s["max_q"], s["q"].device
+    start, whole, table = s["qstart"].long(), s["len"].long(), s["table"].long().clamp_min(0)
+    keys = lambda c: c[table].float().permute(0, 2, 1, 3, 4).reshape(n, s["kv"], -1, dim)  # noqa: E731  [seq][head][position][dim]
+    k, v = keys(s["k_cache"]), keys(s["v_cache"])
+    # queries by sequence, padded to the longest
+    at, live = _padded(s["qstart"], maxq)
+    tok = at.clamp_max(s["ntok"] - 1)
+    q = s["q"][tok].float().reshape(n, maxq, s["kv"], g, dim).permute(0, 2, 3, 1, 4).reshape(n, s["kv"], g * maxq, dim)
+    ctx = whole - (start[1:] - start[:-1])
+    p = torch.arange(k.shape[2], device=dev)
+    one = ((s["bits"][..., None] >> torch.arange(64, device=dev)) & 1).flatten(1)[tok]   # [seq][query][node]
+    pos = ctx[:, None] + one.sum(-1) - 1
+    node = (p - ctx[:, None])[:, None].expand(-1, maxq, -1)                              # [seq][query][position]
+    drafted = one.gather(2, node.clamp(0, one.shape[2] - 1)) > 0
+    cached = node < 0
+    if s["window"]:
+        cached = cached & (p >= (pos - s["window"])[..., None])
+    sees = (cached | (drafted & (node >= 0) & (node < one.shape[2]))) & live[..., None]
+    x = torch.matmul(q, k.transpose(2, 3).contiguous()).reshape(n, s["kv"], g, maxq, -1) * s["scale"]
+    if s["cap"]:
+        x = torch.tanh(x / s["cap"]) * s["cap"]
+    if s["slopes"] is not None:   # to a drafted token: as many steps as lie behind it on the path
+        behind = one.sum(-1, keepdim=True) - torch.cumsum(one, -1)
+        far = torch.where(node < 0, pos[..., None] - p, behind.gather(2, node.clamp(0, one.shape[2] - 1)))
+        x = x - s["slopes"].reshape(1, s["kv"], g, 1, 1) * far[:, None, None]
+    x = x.masked_fill_(~sees[:, None, None], -math.inf)
+    top = x.amax(-1, keepdim=True).clamp_min(torch.finfo(torch.float32).min)
+    x = (x - top).exp_()
+    total = x.sum(-1, keepdim=True)
+    o = torch.matmul(x.reshape(n, s["kv"], g * maxq, -1), v).reshape(n, s["kv"], g, maxq, dim) / total.clamp_min(1e-38)
+    lse = (top + total.log()).squeeze(-1)
+    # back to the batch's order of tokens
+    t = torch.arange(s["ntok"], device=dev)
+    seq = torch.searchsorted(start[1:], t, right=True)
+    i = t - start[seq]
+    o = o.permute(0, 3, 1, 2, 4).reshape(n, maxq, s["heads"], dim)[seq, i]
+    return dict(out=o.to(s["out"].dtype), lse=lse.permute(0, 3, 1, 2).reshape(n, maxq, s["heads"])[seq, i])
+
+
+def _plain_accept(s):
+    """a node is accepted if it is the first node or the first of its siblings that the model chose, and so are all that it follows"""
+    at, live = _padded(s["qstart"], s["most"])
+    at, n, most = at.clamp_max(s["ntok"] - 1), s["n"], s["most"]
+    up, token, choice = (torch.where(live, s[k].long()[at], -1) for k in ("parent", "token", "next"))
+    j = torch.arange(most, device=at.device).expand(n, -1)
+    chosen = (up >= 0) & (token == choice.gather(1, up.clamp_min(0)))
+    first = torch.full((n, most + 1), most, device=at.device)
+    first = first.scatter_reduce(1, torch.where(chosen, up, most), torch.where(chosen, j, most), "amin")
+    ok = (chosen & (first.gather(1, up.clamp_min(0)) == j)) | (j == 0)
+    sees = _paths(s["qstart"], s["parent"], most)[at]
+    taken = ~(sees & ~ok[:, None]).any(-1) & live
+    count = taken.sum(1)
+    nodes = s["qstart"].long()
+    nodes = nodes[1:] - nodes[:-1]
+    ctx = s["len"].long() - nodes
+    kept = torch.cat([s["kept"], _room(1)])   # the last place takes what is not accepted
+    to = torch.where(taken, s["qstart"].long()[:-1, None] + torch.cumsum(taken, 1) - 1, s["ntok"])
+    kept[to.flatten()] = torch.where(taken, ctx[:, None] + j, -1).flatten().to(torch.int32)
+    last = choice.gather(1, torch.where(taken, j, 0).amax(1, keepdim=True)).squeeze(1)
+    i = lambda v: v.to(torch.int32)  # noqa: E731
+    return i(kept[:-1]), i(count), i(ctx + count), i(torch.where(nodes > 0, last, -1))
+
+
+def _plain_compact(s, kept, count):
+    t, start = torch.arange(kept.shape[0], device=kept.device), s["qstart"].long()
+    seq = torch.searchsorted(start[1:], t, right=True)
+    j = t - start[seq]
+    live = j < count[seq]
+    bs, table, kept = s["bs"], s["table"].long(), kept.long()
+    to = kept[start[seq]] + j
+    place = lambda p: (torch.where(live, table[seq, (p // bs).clamp(0, s["width"] - 1)], s["nblocks"]), torch.where(live, p % bs, 0))  # noqa: E731
+    (b0, p0), (b1, p1) = place(kept), place(to)
+    s["cache"][:, :, b1, :, p1] = s["cache"][:, :, b0, :, p0]
+    return s["cache"][:, :, :-1]
+
+
+def _plain_free(s, ctx, keep, table, nfree, holders, shared=0):
+    bs, nb, width = s["bs"], s["nblocks"], s["width"]
+    table, ctx, cols = table.long(), ctx.long(), torch.arange(s["width"], device=table.device)
+    keep = torch.minimum(ctx, keep.long().clamp_min(shared))
+    ids = torch.where((table >= 0) & (table < nb), table, nb)
+    if holders is not None:   # a sequence cannot end inside a block that others hold
+        more = torch.cat([holders.long(), torch.zeros(1, dtype=torch.long, device=table.device)])
+        begun = ids.gather(1, (keep // bs).clamp_max(width - 1)[:, None]).squeeze(1)
+        keep = torch.where((keep < ctx) & (keep % bs > 0) & (keep > shared) & (more[begun] > 0), ctx, keep)
+    gives = (cols >= ((keep + bs - 1) // bs)[:, None]) & (cols >= shared // bs) & (cols < ((ctx + bs - 1) // bs)[:, None]) & (ids < nb)
+    ids, gives = torch.where(gives, ids, nb).flatten(), gives.flatten()
+    if holders is not None:
+        at = torch.arange(ids.shape[0], device=ids.device)
+        drops = torch.zeros_like(more).index_add_(0, ids, gives.long())
+        back = drops > more
+        last = torch.zeros_like(more).scatter_reduce(0, ids, at, "amax")
+        holders.copy_(torch.where(back, 0, more - drops)[:-1])
+        gives = gives & back[ids] & (last[ids] == at)
+    n = nfree.long() + torch.cumsum(gives, 0)
+    free = torch.cat([s["free"], _room(1)])
+    free[torch.where(gives, n - 1, nb)] = torch.where(gives, ids, -1).to(torch.int32)
+    s["free"].copy_(free[:-1])
+    return keep.to(torch.int32), n[-1:].to(torch.int32)
+
+
+def _plain_verify(s):
+    kept, count, ctx, last = _plain_accept(s)
+    cache = _plain_compact(s, kept, count)
+    left, nfree = _plain_free(s, s["len"], ctx, s["table"], s["nfree"], None)
+    return dict(kept=kept, count=count, ctx=ctx, last=last, cache=cache, left=left, free=s["free"], nfree=nfree)
+
+
+def _plain_evict(s):
+    return dict(cache=_plain_compact(s, s["kept"], s["count"]))
+
+
+def _plain_fork(s):
+    bs, nb, keep = s["bs"], s["nblocks"], s["shared"] // s["bs"]
+    src, dst, table = s["src"].long(), s["dst"].long(), s["table"].long()
+    cols, n, nfree = torch.arange(s["width"], device=src.device), s["ctx"].long()[src], s["nfree"].long()
+    full = n // bs
+    need = (n % bs > 0) & (n > s["shared"])
+    taken = torch.cumsum(need, 0)
+    fits = taken <= nfree
+    need = need & fits
+    new = s["free"].long()[(nfree - taken).clamp(0, nb - 1)]
+    row = table[src]
+    ids = torch.where((cols >= keep) & (cols < full[:, None]) & fits[:, None], row, nb)
+    ones = torch.zeros(nb + 1, dtype=torch.int32, device=src.device).index_add_(0, ids.flatten(), torch.ones_like(ids.flatten(), dtype=torch.int32))
+    s["holders"] += ones[:-1]
+    table_out = s["table_out"] if s["beams"] else s["table"]
+    ctx_out = s["ctx_out"] if s["beams"] else s["ctx"]
+    begun = row.gather(1, full.clamp_max(s["width"] - 1)[:, None]).squeeze(1)
+    into = torch.where((cols < torch.maximum(full, (n + bs - 1) // bs * (n <= s["shared"]))[:, None]) & fits[:, None], row, table_out.long()[dst])
+    table_out[dst] = torch.where((cols == full[:, None]) & need[:, None], new[:, None], into).to(torch.int32)
+    ctx_out[dst] = torch.where(fits, n, 0).to(torch.int32)
+    b0, b1, k = torch.where(need, begun, -1), torch.where(need, new, -1), torch.where(need, n % bs, 0)
+    # the begun blocks' contents
+    x0, x1 = torch.where(need, begun, nb), torch.where(need, new, nb)
+    some = (torch.arange(bs, device=src.device) < k[:, None])[:, None, :, None]
+    s["cache"][:, :, x1] = torch.where(some, s["cache"][:, :, x0], s["cache"][:, :, x1])
+    i = lambda v: v.to(torch.int32)  # noqa: E731
+    left, nfree = None, i(nfree - need.sum())
+    if s["beams"]:
+        left, nfree = _plain_free(s, s["ctx"], s["none"], s["table"], nfree, s["holders"], s["shared"])
+    return dict(table=table_out, ctx=ctx_out, holders=s["holders"], from_=i(b0), to=i(b1), copied=i(k), free=s["free"], nfree=nfree, left=left,
+                cache=s["cache"][:, :, :-1])
+
+
+# ---------------------------------------------------------------------------------------------------- the library
+def _lib():
+    if "maplemoe" not in sys.modules:
+        sys.path.insert(0, os.path.join(ROOT, "maple-runtime_amd"))
+    import maplemoe as M
+    return M, M.lib()
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _layers(M, s):
+    """the layers' caches, as a program lays them out once"""
+    if "caches" not in s:
+        c = s["cache"]
+        s["caches"] = (M.KvCache * s["layers"])(*(
+            M.KvCache(k=c[i, 0].data_ptr(), v=c[i, 1].data_ptr(), block_stride=c.stride(2), head_stride=c.stride(3), token_stride=c.stride(4),
+                      nblocks=s["nblocks"], block_size=s["bs"], heads=s["kv"], head_dim=s["dim"], dtype=M.DTYPE[s["type"]]) for i in range(s["layers"])))
+    return s["caches"]
+
+
+def _args(s, key, make):
+    """a call's argument block, which a program that steps over the same device arrays keeps"""
+    if key not in s:
+        s[key] = make()
+    return s[key]
+
+
+def _own_tree(s):
+    M, lib = _lib()
+    a = _args(s, "a", lambda: M.TreePlan(qstart=_p(s["qstart"]), len=_p(s["len"]), parent=_p(s["parent"]), pos=_p(s["pos"]), bits=_p(s["bits"]), nseq=s["n"],
+                                         ntok=s["ntok"], words=s["words"]))
+    M.check(lib.mmoe_tree_plan(a), "mmoe_tree_plan")
+    return dict(pos=s["pos"], bits=s["bits"])
+
+
+def _own_attn(s):
+    M, lib = _lib()
+    h, dim = s["heads"], s["dim"]
+    c = _args(s, "c", lambda: M.KvCache(k=_p(s["k_cache"]), v=_p(s["v_cache"]), block_stride=s["kv"] * s["bs"] * dim, head_stride=s["bs"] * dim, token_stride=dim,
+                                        nblocks=s["k_cache"].shape[0], block_size=s["bs"], heads=s["kv"], head_dim=dim, dtype=M.DTYPE[s["type"]]))
+    a = _args(s, "a", lambda: M.PagedAttn(q=_p(s["q"]), out=_p(s["out"]), lse=_p(s["lse"]), q_token=h * dim, q_head=dim, out_token=h * dim, out_head=dim,
+                                          qstart=_p(s["qstart"]), len=_p(s["len"]), table=_p(s["table"]), slopes=_p(s["slopes"]), nseq=s["n"], ntok=s["ntok"],
+                                          heads=h, width=s["width"], max_q=s["max_q"], max_len=s["max_len"], shared=s["shared"], window=s["window"],
+                                          scale=s["scale"], cap=s["cap"]))
+    if "ws" not in s:   # a program keeps one for all its calls
+        s["ws"] = torch.empty(lib.mmoe_attn_tree_ws(a, c, _p(s["bits"]), s["words"]), dtype=torch.uint8, device="cuda")
+        a.ws, a.ws_bytes = s["ws"].data_ptr(), s["ws"].numel()
+    M.check(lib.mmoe_attn_tree(a, c, _p(s["bits"]), s["words"]), "mmoe_attn_tree")
+    return dict(out=s["out"], lse=s["lse"])
+
+
+def _own_verify(s):
+    M, lib = _lib()
+    a = _args(s, "a", lambda: M.TreeAccept(qstart=_p(s["qstart"]), len=_p(s["len"]), parent=_p(s["parent"]), token=_p(s["token"]), next=_p(s["next"]),
+                                           kept=_p(s["kept"]), count=_p(s["count"]), ctx=_p(s["ctx"]), last=_p(s["last"]), nseq=s["n"], ntok=s["ntok"]))
+    M.check(lib.mmoe_tree_accept(a), "mmoe_tree_accept")
+    c = _args(s, "c", lambda: M.KvCompact(table=_p(s["table"]), first=_p(s["qstart"]), count=_p(s["count"]), kept=_p(s["kept"]), nseq=s["n"], width=s["width"],
+                                          nkept=s["ntok"]))
+    M.check(lib.mmoe_kv_compact(c, _layers(M, s), s["layers"]), "mmoe_kv_compact")
+    f = _args(s, "f", lambda: M.KvFree(ctx=_p(s["len"]), keep=_p(s["ctx"]), len=_p(s["left"]), table=_p(s["table"]), free_list=_p(s["free"]), nfree=_p(s["nfree"]),
+                                       nfree_out=_p(s["nfree_out"]), nseq=s["n"], width=s["width"], nblocks=s["nblocks"], block_size=s["bs"]))
+    M.check(lib.mmoe_kv_free(f), "mmoe_kv_free")
+    return dict(kept=s["kept"], count=s["count"], ctx=s["ctx"], last=s["last"], cache=s["cache"][:, :, :-1], left=s["left"], free=s["free"],
+                nfree=s["nfree_out"])
+
+
+def _own_evict(s):
+    M, lib = _lib()
+    c = _args(s, "c", lambda: M.KvCompact(table=_p(s["table"]), first=_p(s["qstart"]), count=_p(s["count"]), kept=_p(s["kept"]), nseq=s["n"], width=s["width"],
+                                          nkept=s["ntok"]))
+    M.check(lib.mmoe_kv_compact(c, _layers(M, s), s["layers"]), "mmoe_kv_compact")
+    return dict(cache=s["cache"][:, :, :-1])
+
+
+def _own_fork(s):
+    M, lib = _lib()
+    table, ctx = (s["table_out"], s["ctx_out"]) if s["beams"] else (s["table"], s["ctx"])
+    a = _args(s, "a", lambda: M.KvFork(src=_p(s["src"]), dst=_p(s["dst"]), ctx=_p(s["ctx"]), ctx_out=_p(ctx), table=_p(s["table"]), table_out=_p(table),
+                                       holders=_p(s["holders"]), free_list=_p(s["free"]), nfree=_p(s["nfree"]), nfree_out=_p(s["nfree_out"]), copy_from=_p(s["from_"]),
+                                       copy_to=_p(s["to"]), copy_count=_p(s["copied"]), nfork=s["forks"], nseq=s["n"], width=s["width"], nblocks=s["nblocks"],
+                                       block_size=s["bs"], shared=s["shared"]))
+    M.check(lib.mmoe_kv_fork(a), "mmoe_kv_fork")
+    c = _args(s, "c", lambda: M.KvCopy(copy_from=_p(s["from_"]), copy_to=_p(s["to"]), copy_count=_p(s["copied"]), ncopy=s["forks"]))
+    M.check(lib.mmoe_kv_copy(c, _layers(M, s), s["layers"]), "mmoe_kv_copy")
+    nfree = s["nfree_out"]
+    if s["beams"]:
+        f = _args(s, "f", lambda: M.KvFree(ctx=_p(s["ctx"]), keep=_p(s["none"]), len=_p(s["old"]), table=_p(s["table"]), free_list=_p(s["free"]),
+                                           nfree=_p(s["nfree_out"]), nfree_out=_p(s["nfree_end"]), holders=_p(s["holders"]), nseq=s["n"], width=s["width"],
+                                           nblocks=s["nblocks"], block_size=s["bs"], shared=s["shared"]))
+        M.check(lib.mmoe_kv_free(f), "mmoe_kv_free")
+        nfree = s["nfree_end"]
+    return dict(table=table, ctx=ctx, holders=s["holders"], from_=s["from_"], to=s["to"], copied=s["copied"], free=s["free"], nfree=nfree,
+                left=s["old"] if s["beams"] else None, cache=s["cache"][:, :, :-1])
+
+
+def run(state):
+    if own:
+        return dict(tree=_own_tree, attn=_own_attn, verify=_own_verify, evict=_own_evict, fork=_own_fork)[state["kind"]](state)
+    return dict(tree=_plain_tree, attn=_plain_attn, verify=_plain_verify, evict=_plain_evict, fork=_plain_fork)[state["kind"]](state)
+
+
+# ---------------------------------------------------------------------------------------------------- work
+def work(case):
+    e = 2.0
+    if case["kind"] == "tree":
+        nodes, _ = _nodes(case)
+        ntok = int(nodes.sum()) + case["pad"]
+        return dict(bytes=ntok * (8.0 + 8 * _up(int(nodes.max()), 64)) + 8.0 * case["nseq"], flops=0.0)
+    if case["kind"] == "attn":
+        nodes, ctx = _nodes(case)
+        seen = np.minimum(ctx, case["window"]) if case["window"] else ctx
+        # a window looks back from the last of a path: as many more cached positions as there are nodes at most
+        keys = float(nodes.sum()) + (float((seen - case["shared"]).clip(0).sum()) + case["shared"] if not case["window"] else float(seen.sum()))
+        rows = float(nodes.sum()) * case["heads"]
+        # of the drafted tokens each sees its own path, which is a few; only the cached positions are counted
+        pairs = float((nodes * seen).sum())
+        return dict(bytes=rows * (case["dim"] * 2 * e + 4) + keys * case["kv"] * case["dim"] * 2 * e + float(nodes.sum()) * 8 * _up(int(nodes.max()), 64),
+                    flops=4.0 * case["dim"] * case["heads"] * pairs)
+    row = 2 * case["layers"] * case["kv"] * case["dim"] * e   # one position in every layer, keys and values
+    if case["kind"] == "verify":
+        nodes, ctx = _nodes(case)
+        # of a draft about three tokens are accepted, of which the first stays where it is
+        return dict(bytes=12.0 * float(nodes.sum()) + 2 * row * 2 * float((nodes > 2).sum()) + 40.0 * case["nseq"], flops=0.0)
+    if case["kind"] == "evict":
+        _, stay = _stay(case)
+        return dict(bytes=2 * row * float(stay.sum()) + 4.0 * float(stay.sum()), flops=0.0)
+    ctx = case["shared"] + np.array(_ragged(case["nseq"], case["ctx_lo"], case["ctx_hi"]))
+    forks, ids = case["copies"], float((ctx // case["bs"]).sum())
+    # begun blocks' positions read and written; ids read and written, holders read and written; of a beam search the old rows' too
+    return dict(bytes=2 * row * forks * float((ctx % case["bs"]).sum()) + forks * ids * 4.0 * (4 + (3 if case["beams"] else 0)), flops=0.0)
+
+
+# ---------------------------------------------------------------------------------------------------- in 64 bits
+def _up_the_tree(parent, i):
+    """a node and what it follows"""
+    path = []
+    while i >= 0:
+        path.append(i)
+        i = parent[i]
+    return path
+
+
+def _exact_attn(case, s):
+    """sequence by sequence and head by head, the paths from the parents"""
+    out = torch.zeros(s["out"].shape, dtype=torch.float64, device="cuda")
+    lse = torch.full(s["lse"].shape, -math.inf, dtype=torch.float64, device="cuda")
+    start, whole, parent, g = s["qstart"].tolist(), s["len"].tolist(), s["parent"].tolist(), s["heads"] // s["kv"]
+    for b in range(s["n"]):
+        t0, t1, n = start[b], start[b + 1], whole[b]
+        ctx = n - (t1 - t0)
+        rows = s["table"][b, :_up(n, s["bs"])].long()
+        hidden = np.ones((t1 - t0, n), bool)
+        far = np.zeros((t1 - t0, n))
+        for i in range(t1 - t0):
+            path = _up_the_tree(parent[t0:t1], i)
+            at = ctx + len(path) - 1
+            hidden[i, max(0, at - case["window"]) if case["window"] else 0:ctx] = False
+            far[i, :ctx] = at - np.arange(ctx)
+            for d, j in enumerate(path):
+                hidden[i, ctx + j], far[i, ctx + j] = False, d
+        hidden, far = torch.from_numpy(hidden).cuda(), torch.from_numpy(far).cuda()
+        for c in range(s["kv"]):
+            k = s["k_cache"][rows, c].reshape(-1, s["dim"])[:n].double()
+            v = s["v_cache"][rows, c].reshape(-1, s["dim"])[:n].double()
+            for h in range(c * g, c * g + g):
+                x = (s["q"][t0:t1, h].double() @ k.t().contiguous()) / math.sqrt(s["dim"])
+                if s["cap"]:
+                    x = s["cap"] * torch.tanh(x / s["cap"])
+                if s["slopes"] is not None:
+                    x = x - s["slopes"][h].double() * far
+                x = x.masked_fill(hidden, -math.inf)
+                lse[t0:t1, h] = torch.logsumexp(x, 1)
+                out[t0:t1, h] = torch.softmax(x, 1) @ v
+    return dict(out=out, lse=lse)
+
+
+def _moved(s, pairs):
+    """the caches with position `a` of the flat order (block, position) copied to `b` for every (a, b), all read before any is written"""
+    c = s["cache"][:, :, :-1].transpose(3, 4)
+    shape = c.shape
+    c = c.double().reshape(shape[0], 2, -1, *shape[4:])
+    if pairs:
+        a, b = torch.tensor(pairs, device="cuda").T.contiguous()
+        c = c.index_copy(2, b, c.index_select(2, a))
+    return c.reshape(shape).transpose(3, 4)
+
+
+def _exact_verify(s):
+    start, whole, parent, token, choice = (s[k].tolist() for k in ("qstart", "len", "parent", "token", "next"))
+    table, pairs = s["table"].tolist(), []
+    for b in range(s["n"]):
+        t0, t1 = start[b], start[b + 1]
+        ctx, node, path = whole[b] - (t1 - t0), 0, []
+        while node is not None:
+            path.append(node)
+            node = next((j for j in range(t1 - t0) if parent[t0 + j] == path[-1] and token[t0 + j] == choice[t0 + path[-1]]), None)
+        slot = lambda p: table[b][p // s["bs"]] * s["bs"] + p % s["bs"]  # noqa: E731
+        pairs += [(slot(ctx + j), slot(ctx + i)) for i, j in enumerate(path) if i != j]
+    none = dict.fromkeys(("kept", "count", "ctx", "last", "left", "free", "nfree"))
+    return dict(none, cache=_moved(s, pairs))
+
+
+def _exact_evict(s):
+    start, kept, table, pairs = s["qstart"].tolist(), s["kept"].tolist(), s["table"].tolist(), []
+    for b in range(s["n"]):
+        slot = lambda p: table[b][p // s["bs"]] * s["bs"] + p % s["bs"]  # noqa: E731
+        pairs += [(slot(kept[i]), slot(kept[start[b]] + i - start[b])) for i in range(start[b], start[b + 1])]
+    return dict(cache=_moved(s, pairs))
+
+
+def _exact_fork(s):
+    src, ctx, table, free, bs = s["src"].tolist(), s["ctx"].tolist(), s["table"].tolist(), s["free"].tolist(), s["bs"]
+    n, pairs = s["nfree"].item(), []
+    for q in src:
+        if ctx[q] % bs and ctx[q] > s["shared"]:
+            n -= 1
+            pairs += [(table[q][ctx[q] // bs] * bs + i, free[n] * bs + i) for i in range(ctx[q] % bs)]
+    none = dict.fromkeys(("table", "ctx", "holders", "from_", "to", "copied", "free", "nfree", "left"))
+    return dict(none, cache=_moved(s, pairs))
+
+
+def exact(case, seed):
+    if case["kind"] == "tree":
+        return None   # whole numbers
+    s = prepare(case, seed)
+    return _exact_attn(case, s) if case["kind"] == "attn" else dict(verify=_exact_verify, evict=_exact_evict, fork=_exact_fork)[case["kind"]](s)
