@@ -482,7 +482,8 @@ def _plain_fork(s):
     i = lambda v: v.to(torch.int32)  # noqa: E731
     left, nfree = None, i(nfree - need.sum())
     if s["beams"]:
-        left, nfree = _plain_free(s, s["ctx"], s["none"], s["table"], nfree, s["holders"], s["shared"])
+        # behind the list as it was, so that its end, which the fork took from, stays there for another pass over the same state
+        left, nfree = _plain_free(s, s["ctx"], s["none"], s["table"], s["nfree"], s["holders"], s["shared"])
     return dict(table=table_out, ctx=ctx_out, holders=s["holders"], from_=i(b0), to=i(b1), copied=i(k), free=s["free"], nfree=nfree, left=left,
                 cache=s["cache"][:, :, :-1])
 
@@ -576,7 +577,7 @@ def _own_fork(s):
     nfree = s["nfree_out"]
     if s["beams"]:
         f = _args(s, "f", lambda: M.KvFree(ctx=_p(s["ctx"]), keep=_p(s["none"]), len=_p(s["old"]), table=_p(s["table"]), free_list=_p(s["free"]),
-                                           nfree=_p(s["nfree_out"]), nfree_out=_p(s["nfree_end"]), holders=_p(s["holders"]), nseq=s["n"], width=s["width"],
+                                           nfree=_p(s["nfree"]), nfree_out=_p(s["nfree_end"]), holders=_p(s["holders"]), nseq=s["n"], width=s["width"],
                                            nblocks=s["nblocks"], block_size=s["bs"], shared=s["shared"]))
         M.check(lib.mmoe_kv_free(f), "mmoe_kv_free")
         nfree = s["nfree_end"]
