@@ -230,7 +230,10 @@ void *mmoe_stream(void);
 #define MMOE_K_KV_PLAN 14
 #define MMOE_K_ROPE 15
 #define MMOE_K_ATT_PAGED 16     /* every kernel of mmoe_attn_paged */
-#define MMOE_PROF_NKERNELS 17
+#define MMOE_K_TREE 17          /* mmoe_tree_plan, mmoe_tree_accept */
+#define MMOE_K_ATT_TREE 18      /* every kernel of mmoe_attn_tree */
+#define MMOE_K_KV_PAGES 19      /* mmoe_kv_compact, mmoe_kv_fork, mmoe_kv_copy, mmoe_kv_free */
+#define MMOE_PROF_NKERNELS 20
 int mmoe_event_record(int slot);
 double mmoe_event_elapsed_ms(void);
 int mmoe_prof(int on);
@@ -270,6 +273,14 @@ int mmoe_selftest_silu(uint32_t lo, uint32_t n, unsigned long long *nbad, uint32
  *   mmoe_kv_plan      block tables, slots and positions of a step, from the sequences' lengths
  *   mmoe_rope_kv      rotary positions of its queries and keys; keys and values written into the blocks
  *   mmoe_attn_paged   attention of its queries over the blocks
+ * and for sequences whose next tokens are drafted as a tree and then accepted or not, and for sequences that share blocks:
+ *   mmoe_tree_plan    what each drafted token follows, and its position
+ *   mmoe_attn_tree    attention of the drafted tokens
+ *   mmoe_tree_accept  the path that agrees with the model
+ *   mmoe_kv_compact   kept positions of a sequence moved together, in every layer
+ *   mmoe_kv_fork      copies of sequences, sharing their full blocks
+ *   mmoe_kv_copy      blocks' contents copied, in every layer
+ *   mmoe_kv_free      sequences shortened or ended, their blocks given back with the last holder
  * One mmoe_kv_plan serves all layers of a step (each layer has its own blocks and the same tables); in a layer mmoe_rope_kv and
  * mmoe_attn_paged stand between the caller's own projections: its q/k/v projections and head norms come before them, its o projection
  * (of out, in the cache's type) and then mmoe_moe_dev after. On device memory this library has none of those projections (gpre_dense takes
@@ -378,5 +389,95 @@ typedef struct {
 } mmoe_attn_args;
 size_t mmoe_attn_paged_ws(const mmoe_attn_args *a, const mmoe_kv_cache *kv);
 int mmoe_attn_paged(const mmoe_attn_args *a, const mmoe_kv_cache *kv);
+
+/* ---- Drafted tokens ----
+ * A sequence's new tokens of a step may be a draft: a tree of tokens that may come next. Its node 0 is the model's own last choice, the others
+ * each follow an earlier node. parent[t] is the node that token t follows, counted from the sequence's first new token; -1 (and anything
+ * that is not an earlier node): none. The step is mmoe_kv_plan (add = nodes; slots as ever), mmoe_tree_plan, per layer mmoe_rope_kv (with
+ * mmoe_tree_plan's positions) and mmoe_attn_tree, then mmoe_tree_accept, mmoe_kv_compact over all layers and mmoe_kv_free. */
+#define MMOE_TREE_MAX 512    /* nodes of a tree */
+
+/* qstart, len: mmoe_kv_plan's. bits[ntok][words]: bit j % 64 of word j / 64 of token t is set where node j is t itself or one that it follows;
+ * pos[t] = the sequence's cached positions (len less its new tokens) + the nodes that t follows. words: 1 to MMOE_TREE_MAX / 64. Nodes from 64 words
+ * on, and tokens from qstart[nseq] on, get position 0 and no bits. */
+typedef struct {
+    const int32_t *qstart, *len, *parent;
+    int32_t *pos;
+    uint64_t *bits;
+    int32_t nseq, ntok, words;
+} mmoe_tree_plan_args;
+int mmoe_tree_plan(const mmoe_tree_plan_args *a);
+
+/* Attention of drafted tokens: mmoe_attn_paged but for what is visible. With ctx = len[s] less the sequence's new tokens, token i of them sees
+ *   cached positions p:  max(lo[t], pos - window) <= p < ctx;   new tokens j <= i (at position ctx + j) whose bit is set, whatever the window
+ * where pos = ctx + the number of its bits below i, and slopes count |pos - p| to a cached position and, to token j < i, one and the bits
+ * between j and i (on mmoe_tree_plan's bits: the steps along the path). bits[ntok][words] need not be a tree's: any bits do; those past i count
+ * for nothing. hi must be NULL and max_q at most 64 words. mmoe_attn_tree_ws: as mmoe_attn_paged_ws. */
+size_t mmoe_attn_tree_ws(const mmoe_attn_args *a, const mmoe_kv_cache *kv, const uint64_t *bits, int words);
+int mmoe_attn_tree(const mmoe_attn_args *a, const mmoe_kv_cache *kv, const uint64_t *bits, int words);
+
+/* Which drafted tokens stay. token[t] is the drafted token, next[t] the model's choice behind it. Node 0 is accepted; then, as long as there
+ * is one, the lowest node that follows the last accepted one and is what the model chose behind that. For sequence s: count[s] nodes accepted,
+ * kept[qstart[s] ..]: their positions in the cache, ascending (entries past count[s] stay as they are); ctx[s] = cached positions with them (may be len);
+ * last[s] = the model's choice behind the last (the next step's node 0). A sequence without new tokens: count 0, ctx = len, last -1. Nodes
+ * from MMOE_TREE_MAX on are never accepted. */
+typedef struct {
+    const int32_t *qstart, *len, *parent, *token, *next;
+    int32_t *kept, *count, *ctx, *last;
+    int32_t nseq, ntok;
+} mmoe_tree_accept_args;
+int mmoe_tree_accept(const mmoe_tree_accept_args *a);
+
+/* ---- Blocks ----
+ * Work on every layer's blocks at once: kv is an array of `layers` caches (at most MMOE_KV_MAXLAYERS) that differ in their pointers only;
+ * head_dim a multiple of 8 up to 256. */
+#define MMOE_KV_MAXLAYERS 128
+
+/* Keys and values of a sequence's kept positions moved together: with k = kept + first[s], position k[j] of sequence s goes to position k[0] + j, for
+ * j < count[s] (as if all were read before any is written). k ascends strictly; entries of kept from nkept on are not read. An entry that is no
+ * position of the table (negative, past width blocks, a block that is not the cache's), or lies before where it would go, stays where it is, and so
+ * does what lies behind the moved ones. Blocks that other sequences hold too must not be among those written. Also for a cache of which
+ * only some positions are to stay; rotated keys stay rotated by their old positions. */
+typedef struct {
+    const int32_t *table, *first, *count, *kept;
+    int32_t nseq, width, nkept;
+} mmoe_kv_compact_args;
+int mmoe_kv_compact(const mmoe_kv_compact_args *a, const mmoe_kv_cache *kv, int layers);
+
+/* Copies of sequences. Fork i makes row dst[i] of table_out a copy of the first n = min(at[i], ctx[src[i]]) positions (at NULL: all) of row src[i] of
+ * table: full blocks are shared (holders[block]++, but for those of the `shared` prefix, which nobody gives back), for a begun one a new
+ * block is taken from the end of the list, and copy_from[i], copy_to[i], copy_count[i] say what mmoe_kv_copy has to copy (-1, -1, 0: nothing).
+ * ctx_out[dst[i]] = n. holders[nblocks]: how many sequences hold a block beside the first; 0 at the start, and blocks that mmoe_kv_plan takes have 0.
+ * From the first fork for which no block is left on, none is made: ctx_out[dst[i]] = 0, the row as it was. Rows that are not 0 .. nseq - 1 are
+ * left out. nfree_out[0] = free blocks left. dst: no row twice. table_out may be table and ctx_out ctx, if no dst is a src then (a beam
+ * search, whose rows follow one another, needs a second table). Where sequences share blocks, mmoe_kv_free gives them back, not mmoe_kv_plan's done. */
+typedef struct {
+    const int32_t *src, *dst, *at, *ctx, *table;
+    int32_t *ctx_out, *table_out, *holders;
+    const int32_t *free_list, *nfree;
+    int32_t *nfree_out, *copy_from, *copy_to, *copy_count;
+    int32_t nfork, nseq, width, nblocks, block_size, shared;
+} mmoe_kv_fork_args;
+int mmoe_kv_fork(const mmoe_kv_fork_args *a);
+
+/* The first copy_count[i] positions (NULL: all) of block copy_from[i] to block copy_to[i], i < ncopy (at most MMOE_KV_MAXSEQ). Pairs of which one is no
+ * block of the cache are left out. No block may be written twice, or be read and written. */
+typedef struct {
+    const int32_t *copy_from, *copy_to, *copy_count;
+    int32_t ncopy;
+} mmoe_kv_copy_args;
+int mmoe_kv_copy(const mmoe_kv_copy_args *a, const mmoe_kv_cache *kv, int layers);
+
+/* Sequence s, of ctx[s] positions, keeps len[s] = min(ctx[s], max(keep[s], shared)) of them (a negative ctx counts as 0) and gives up its blocks behind
+ * those. A block that others hold (holders NULL: none is) loses a holder; one that nobody holds any more goes to the end of the list, blocks in the order
+ * in which their last holders lie in the tables. Ids that are no blocks of the cache are left out. A sequence whose kept positions would
+ * end inside a block that others hold as the call begins, so that its next tokens would be written into it, keeps all (len[s] = ctx[s]: fork it at that length instead).
+ * len may be ctx or keep, and nfree_out may be nfree. */
+typedef struct {
+    const int32_t *ctx, *keep, *table, *nfree;
+    int32_t *len, *free_list, *nfree_out, *holders;
+    int32_t nseq, width, nblocks, block_size, shared;
+} mmoe_kv_free_args;
+int mmoe_kv_free(const mmoe_kv_free_args *a);
 
 #endif

@@ -1,0 +1,312 @@
+// drafts.h -- kernels for drafted tokens (what each follows, which are accepted) and for blocks that sequences share, copy and give back
+// (drafts.hip).
+#pragma once
+#include "paged.h"
+
+// Where sequence s's new tokens begin and how many they are, inside the arrays whatever qstart holds
+struct NewTokens { int t0, n; };
+__device__ __forceinline__ NewTokens new_tokens(const int32_t *qstart, int s, int ntok) {
+    const int t0 = min(max(qstart[s], 0), ntok), t1 = min(max(qstart[s + 1], t0), ntok);
+    return {t0, t1 - t0};
+}
+
+// ------------------------------------------------------------------------------------------------------
+// What drafted tokens follow (mmoe_tree_plan)
+// ------------------------------------------------------------------------------------------------------
+// A workgroup per sequence, a thread per node. By steps that double: what a node's 2^i-th ancestor follows, it follows, so nine rounds through
+// LDS settle the deepest tree of 512, and as many as the depth's logarithm any other.
+template <int W>
+__global__ void __launch_bounds__(64 * W) k_tree_plan(mmoe_tree_plan_args a) {
+    __shared__ uint64_t sees[W][64 * W];
+    __shared__ int up[64 * W];
+    const int s = blockIdx.x, i = threadIdx.x;
+    const NewTokens q = a.nseq ? new_tokens(a.qstart, s, a.ntok) : NewTokens{0, 0};
+    const int n = min(q.n, 64 * a.words), ctx = a.nseq ? a.len[s] - q.n : 0;
+    int to = -1;
+    if (i < n) to = a.parent[q.t0 + i];
+    if (to >= i) to = -1;
+    uint64_t b[W];
+#pragma unroll
+    for (int w = 0; w < W; w++) b[w] = w == i >> 6 ? 1ull << (i & 63) : 0;
+    while (__syncthreads_or(to >= 0)) {
+#pragma unroll
+        for (int w = 0; w < W; w++) sees[w][i] = b[w];
+        up[i] = to;
+        __syncthreads();
+        if (to >= 0) {
+#pragma unroll
+            for (int w = 0; w < W; w++) b[w] |= sees[w][to];
+            to = up[to];
+        }
+    }
+    int depth = -1;
+#pragma unroll
+    for (int w = 0; w < W; w++) depth += __popcll(b[w]);
+    if (i < n) {
+        a.pos[q.t0 + i] = ctx + depth;
+#pragma unroll
+        for (int w = 0; w < W; w++) if (w < a.words) a.bits[(int64_t)(q.t0 + i) * a.words + w] = b[w];
+    }
+    // nodes past the words, and tokens of no sequence
+    for (int t = q.t0 + n + i; t < q.t0 + q.n; t += 64 * W) {
+        a.pos[t] = 0;
+        for (int w = 0; w < a.words; w++) a.bits[(int64_t)t * a.words + w] = 0;
+    }
+    for (int64_t t = min(max(a.qstart[a.nseq], 0), a.ntok) + (int64_t)s * 64 * W + i; t < a.ntok; t += (int64_t)gridDim.x * 64 * W) {
+        a.pos[t] = 0;
+        for (int w = 0; w < a.words; w++) a.bits[t * a.words + w] = 0;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------
+// Which drafted tokens stay (mmoe_tree_accept)
+// ------------------------------------------------------------------------------------------------------
+// A workgroup per sequence: every node that is what the model chose behind its parent offers itself to it, the lowest one wins; then the walk from node
+// 0 is a chain of reads from LDS.
+__global__ void __launch_bounds__(128) k_tree_accept(mmoe_tree_accept_args a) {
+    __shared__ int child[MMOE_TREE_MAX];
+    const int s = blockIdx.x;
+    const NewTokens q = new_tokens(a.qstart, s, a.ntok);
+    const int n = min(q.n, MMOE_TREE_MAX), ctx = a.len[s] - q.n;
+    for (int i = threadIdx.x; i < n; i += 128) child[i] = INT32_MAX;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += 128) {
+        const int p = a.parent[q.t0 + i];
+        if (p >= 0 && p < i && a.token[q.t0 + i] == a.next[q.t0 + p]) atomicMin(&child[p], i);
+    }
+    __syncthreads();
+    if (threadIdx.x) return;
+    int count = 0, last = 0;
+    for (int i = 0; i < n; i = child[i]) {   // (a child lies behind its parent: the walk ends)
+        a.kept[q.t0 + count++] = ctx + i;
+        last = i;
+    }
+    a.count[s] = count;
+    a.last[s] = n ? a.next[q.t0 + last] : -1;
+    a.ctx[s] = ctx + count;
+}
+
+// ------------------------------------------------------------------------------------------------------
+// Blocks in every layer (mmoe_kv_compact, mmoe_kv_copy)
+// ------------------------------------------------------------------------------------------------------
+// A position is heads * pieces pieces of 16 bytes, numbered head by head. The layers' arrays differ in their pointers only.
+struct PageArgs {
+    mmoe_kv_cache kv;                  // the layers' strides and sizes (k and v unused)
+    int sh, esize, pieces, all;        // log2 of the block size, bytes of a value, pieces of a head, of a position
+    Div by_pieces;
+    void *base[2 * MMOE_KV_MAXLAYERS]; // keys and values of each layer
+};
+__device__ __forceinline__ int64_t page_at(const PageArgs &P, int block, int at, int piece) {   // in bytes
+    const int head = (int)P.by_pieces(piece);
+    return (block * P.kv.block_stride + head * P.kv.head_stride + at * P.kv.token_stride) * P.esize + (int64_t)(piece - head * P.pieces) * 16;
+}
+
+// Kept positions moved together. Entry j goes from k[j] to k[0] + j <= k[j], so that writing it touches the source of no later one: a
+// workgroup goes through the list in steps of as many entries as its threads hold, all read before any is written.
+#define KC_T 256
+#define KC_U 8
+__global__ void __launch_bounds__(KC_T) k_kv_compact(mmoe_kv_compact_args a, PageArgs P, int lanes, int units, Div by_lanes, Div by_units, Div by_arrays, int arrays) {
+    const unsigned rest = by_units(blockIdx.x), s = by_arrays(rest);
+    const int unit = blockIdx.x - rest * units, array = rest - s * arrays;
+    const int first = a.first[s], n = a.count[s];
+    if (first < 0 || first >= a.nkept || n < 2) return;
+    const int count = min(n, a.nkept - first), per = (int)by_lanes(KC_T), e = (int)by_lanes(threadIdx.x);
+    const int piece = unit * lanes + threadIdx.x - e * lanes;
+    const bool on = e < per && piece < P.all;
+    const int32_t *k = a.kept + first, *table = a.table + (int64_t)s * a.width;
+    const int to0 = k[0];
+    uint8_t *base = (uint8_t *)P.base[array];
+    auto block = [&](int64_t p) { return p < 0 || (p >> P.sh) >= a.width ? -1 : table[p >> P.sh]; };
+    for (int j0 = 1; j0 < count; j0 += per * KC_U) {
+        u4 x[KC_U];
+        int64_t to[KC_U];
+#pragma unroll
+        for (int u = 0; u < KC_U; u++) {
+            const int j = j0 + u * per + e;
+            to[u] = -1;
+            if (!on || j >= count) continue;
+            const int from = k[j];
+            const int64_t t = (int64_t)to0 + j;
+            if (from <= t) continue;
+            const int b0 = block(from), b1 = block(t);
+            if ((unsigned)b0 >= (unsigned)P.kv.nblocks || (unsigned)b1 >= (unsigned)P.kv.nblocks) continue;
+            x[u] = *(const gu4 *)(base + page_at(P, b0, from & (P.kv.block_size - 1), piece));
+            to[u] = page_at(P, b1, (int)t & (P.kv.block_size - 1), piece);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // every wave's values are there before any is written over
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < KC_U; u++) if (to[u] >= 0) *(gu4 *)(base + to[u]) = x[u];
+    }
+}
+
+#define KY_T 256
+#define KY_U 8
+__global__ void __launch_bounds__(KY_T) k_kv_copy(mmoe_kv_copy_args a, PageArgs P, int units, Div by_units, Div by_arrays, int arrays) {
+    const unsigned rest = by_units(blockIdx.x), i = by_arrays(rest);
+    const int unit = blockIdx.x - rest * units, array = rest - i * arrays;
+    const int from = a.copy_from[i], to = a.copy_to[i], bs = P.kv.block_size;
+    const int count = a.copy_count ? min(max(a.copy_count[i], 0), bs) : bs;
+    if ((unsigned)from >= (unsigned)P.kv.nblocks || (unsigned)to >= (unsigned)P.kv.nblocks || from == to) return;
+    uint8_t *base = (uint8_t *)P.base[array];
+    u4 x[KY_U];
+    int64_t at[KY_U];
+#pragma unroll
+    for (int u = 0; u < KY_U; u++) {   // head by head, positions within, pieces within those
+        const int item = (unit * KY_U + u) * KY_T + threadIdx.x, row = (int)P.by_pieces(item), head = row >> P.sh, pos = row & (bs - 1);
+        at[u] = -1;
+        if (head >= P.kv.heads || pos >= count) continue;
+        at[u] = (head * P.kv.head_stride + pos * P.kv.token_stride) * P.esize + (int64_t)(item - row * P.pieces) * 16;
+        x[u] = *(const gu4 *)(base + from * P.kv.block_stride * P.esize + at[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < KY_U; u++) if (at[u] >= 0) *(gu4 *)(base + to * P.kv.block_stride * P.esize + at[u]) = x[u];
+}
+
+// ------------------------------------------------------------------------------------------------------
+// Copies of sequences (mmoe_kv_fork)
+// ------------------------------------------------------------------------------------------------------
+// One workgroup settles which forks are made and which blocks they take (a prefix sum over them); the rows, which are independent, follow in the
+// same launch or in one of their own.
+__device__ __forceinline__ void fork_row(const mmoe_kv_fork_args &a, int sh, int src, int dst, int n, int lane, int lanes) {
+    const int keep = a.shared >> sh, cols = n <= a.shared ? (n + a.block_size - 1) >> sh : n >> sh;
+    for (int c = lane; c < cols; c += lanes) {
+        const int b = a.table[(int64_t)src * a.width + c];
+        a.table_out[(int64_t)dst * a.width + c] = b;
+        if (c >= keep && (unsigned)b < (unsigned)a.nblocks) atomicAdd(&a.holders[b], 1);
+    }
+}
+template <int PER>
+__global__ void __launch_bounds__(1024) k_kv_fork(mmoe_kv_fork_args a, int sh, int rows) {
+    __shared__ int src_[PER * 1024], dst_[PER * 1024], len_[PER * 1024];
+    __shared__ uint2 red[16];
+    const int tid = threadIdx.x, i0 = tid * PER, nt = blockDim.x;
+    const int nfree = min(max(a.nfree[0], 0), a.nblocks);
+    int src[PER], dst[PER], n[PER], begun[PER];
+    unsigned need[PER], sum = 0, zero = 0, total, z;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const bool in = i0 + i < a.nfork;
+        src[i] = in ? a.src[i0 + i] : -1; dst[i] = in ? a.dst[i0 + i] : -1;
+        const bool ok = (unsigned)src[i] < (unsigned)a.nseq && (unsigned)dst[i] < (unsigned)a.nseq;
+        if (!ok) src[i] = -1;
+        n[i] = ok ? a.ctx[src[i]] : 0;
+        if (ok && a.at) n[i] = min(n[i], a.at[i0 + i]);
+        n[i] = min(max(n[i], 0), a.width << sh);
+        need[i] = (n[i] & (a.block_size - 1)) && n[i] > a.shared;
+        begun[i] = need[i] ? a.table[(int64_t)src[i] * a.width + (n[i] >> sh)] : -1;
+        sum += need[i];
+    }
+    scan2(sum, zero, &total, &z, red);   // (and every length has been read before one is written)
+    if (tid == 0) a.nfree_out[0] = nfree - (int)min(total, (unsigned)nfree);
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        if (i0 + i >= a.nfork) continue;
+        const unsigned at = sum;
+        sum += need[i];
+        const bool fits = sum <= (unsigned)nfree, takes = need[i] && fits;
+        const int b = takes ? a.free_list[nfree - 1 - at] : -1;
+        if (!fits) n[i] = 0;
+        if (src[i] >= 0) {
+            a.ctx_out[dst[i]] = n[i];
+            if (takes) a.table_out[(int64_t)dst[i] * a.width + (n[i] >> sh)] = b;
+        } else if ((unsigned)dst[i] < (unsigned)a.nseq) a.ctx_out[dst[i]] = 0;
+        a.copy_from[i0 + i] = takes ? begun[i] : -1;
+        a.copy_to[i0 + i] = b;
+        a.copy_count[i0 + i] = takes ? n[i] & (a.block_size - 1) : 0;
+        src_[i0 + i] = src[i]; dst_[i0 + i] = dst[i]; len_[i0 + i] = n[i];
+    }
+    if (!rows) return;
+    __syncthreads();
+    for (int i = tid >> 6; i < a.nfork; i += nt >> 6)
+        if (src_[i] >= 0) fork_row(a, sh, src_[i], dst_[i], len_[i], tid & 63, 64);
+}
+__global__ void __launch_bounds__(256) k_kv_fork_rows(mmoe_kv_fork_args a, int sh) {
+    const int src = a.src[blockIdx.x], dst = a.dst[blockIdx.x];
+    if ((unsigned)src < (unsigned)a.nseq && (unsigned)dst < (unsigned)a.nseq) fork_row(a, sh, src, dst, a.ctx_out[dst], threadIdx.x, 256);
+}
+
+// ------------------------------------------------------------------------------------------------------
+// Blocks given back (mmoe_kv_free)
+// ------------------------------------------------------------------------------------------------------
+// What sequences give up, one behind the other, is a list of places in the tables; a block goes back with the last of them that drops it to
+// nobody. Three passes over that list with holders: every place drops a holder; of the places of a block that nobody holds now the last one marks
+// it; the marked ones are appended in order. Sums and marks, not the order of the atomics, decide, so the list comes out the same every time.
+#define KF_U 4
+template <int PER>
+__global__ void __launch_bounds__(1024) k_kv_free(mmoe_kv_free_args a, int sh) {
+    constexpr int NS = PER * 1024;
+    __shared__ int first[NS + 1], col[NS];
+    __shared__ uint2 red[16];
+    const int tid = threadIdx.x, nt = blockDim.x, s0 = tid * PER, bs1 = a.block_size - 1, pre = a.shared >> sh, nfree = min(max(a.nfree[0], 0), a.nblocks);
+    const int room = a.width << sh;
+    unsigned old[PER], sum = 0, zero = 0, total, z;
+    int len[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        old[i] = 0;
+        if (s0 + i >= a.nseq) continue;
+        const int ctx = min(max(a.ctx[s0 + i], 0), room);
+        int k = min(ctx, max(a.keep[s0 + i], a.shared));
+        if (a.holders && k < ctx && (k & bs1) && k > a.shared) {
+            const int b = a.table[(int64_t)(s0 + i) * a.width + (k >> sh)];
+            if ((unsigned)b < (unsigned)a.nblocks && a.holders[b] > 0) k = ctx;
+        }
+        len[i] = k;
+        const int c0 = max((k + bs1) >> sh, pre), c1 = (ctx + bs1) >> sh;
+        col[s0 + i] = c0;
+        old[i] = (unsigned)max(c1 - c0, 0);
+        sum = min(sum + old[i], (unsigned)KP_LIM);
+    }
+    scan2(sum, zero, &total, &z, red);
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        if (s0 + i >= a.nseq) continue;
+        a.len[s0 + i] = len[i];
+        first[s0 + i] = (int)sum;
+        sum = min(sum + old[i], (unsigned)KP_LIM);
+    }
+    __syncthreads();
+    const int n = (int)total;
+    auto id = [&](int j) {
+        const int s = count_le(first, a.nseq, j) - 1;
+        return a.table[(int64_t)s * a.width + col[s] + j - first[s]];
+    };
+    if (a.holders) {
+        for (int j = tid; j < n; j += nt) {
+            const int b = id(j);
+            if ((unsigned)b < (unsigned)a.nblocks) atomicSub(&a.holders[b], 1);
+        }
+        __threadfence();
+        __syncthreads();
+        for (int j = tid; j < n; j += nt) {
+            const int b = id(j);
+            if ((unsigned)b < (unsigned)a.nblocks && __hip_atomic_load(&a.holders[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < 0) atomicMin(&a.holders[b], -2 - j);
+        }
+        __threadfence();
+        __syncthreads();
+    }
+    int at = nfree;
+    for (int j0 = 0; j0 < n; j0 += nt * KF_U) {
+        int b[KF_U];
+        unsigned mine = 0, none = 0, all, z2;
+#pragma unroll
+        for (int u = 0; u < KF_U; u++) {
+            const int j = j0 + tid * KF_U + u;
+            b[u] = j < n ? id(j) : -1;
+            if ((unsigned)b[u] >= (unsigned)a.nblocks) b[u] = -1;
+            else if (a.holders && __hip_atomic_load(&a.holders[b[u]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != -2 - j) b[u] = -1;
+            mine += b[u] >= 0;
+        }
+        scan2(mine, none, &all, &z2, red);
+#pragma unroll
+        for (int u = 0; u < KF_U; u++) {
+            if (b[u] < 0) continue;
+            if (at + (int)mine < a.nblocks) a.free_list[at + mine] = b[u];
+            if (a.holders) a.holders[b[u]] = 0;
+            mine++;
+        }
+        at = min(at + (int)all, a.nblocks);
+    }
+    if (tid == 0) a.nfree_out[0] = at;
+}

@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(1024) k_kv_plan(mmoe_kv_plan_args a, int sh, i
 
 // The tokens of a large step, in a launch of their own over the whole card: 60000 in 2.7 us (their starts into LDS, then a search and two
 // dependent loads; 0.5 MB written)
-__global__ void __launch_bounds__(256) k_kv_tokens(mmoe_kv_plan_args a, int sh) {
+static __global__ void __launch_bounds__(256) k_kv_tokens(mmoe_kv_plan_args a, int sh) {
     __shared__ int start[MMOE_KV_MAXSEQ + 1];
     for (int i = threadIdx.x; i <= a.nseq; i += 256) start[i] = a.qstart[i];
     __syncthreads();
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
 }
 
 // ------------------------------------------------------------------------------------------------------
-// Attention over the blocks (mmoe_attn_paged)
+// Attention over the blocks (mmoe_attn_paged; with TREE mmoe_attn_tree)
 // ------------------------------------------------------------------------------------------------------
 // Every kernel here keeps a softmax's running maximum and sum and one pass over the positions. A query row is a (token, query
 // head) pair; the rows that read one key/value head, token by token and its group of query heads within, share its keys. The
@@ -476,6 +476,8 @@ struct AttArgs {
     float *po;
     float2 *pm;
     int64_t at_tile, at_few;
+    const uint64_t *bits;   // drafted tokens (TREE): words per token, bit j: it sees its sequence's j-th new token
+    int words;
 };
 
 template <int T> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
@@ -545,7 +547,9 @@ __device__ __forceinline__ AttChunks att_chunks(const AttArgs &A, int s, int tok
 }
 
 // One query row as a lane sees it: its token and head, then (with a search for its sequence, if that is not the tile's) its limits
-struct AttRow { int tok, head, pos, lo, hi; bool live; };
+// full: where the row stops seeing every position from lo on. TREE: the sequence's cached positions, the token's place among the new
+// ones, and its bits where they are one word.
+struct AttRow { int tok, head, pos, lo, hi, full, ctx, own; uint64_t bits; bool live; };
 __device__ __forceinline__ AttRow att_row(const AttArgs &A, const AttTileAt &at, int r, int kvh) {
     AttRow o;
     o.live = r < at.rows;
@@ -569,16 +573,59 @@ __device__ __forceinline__ AttSeq att_seq(const AttArgs &A, bool shared, const A
     } else { t0 = a.qstart[s]; t1 = a.qstart[s + 1]; }
     return {s, t0, t1};
 }
-__device__ __forceinline__ void att_limits(const AttArgs &A, bool shared, const AttSeq &q, AttRow &o) {
+// Masks of drafted tokens. What a token sees of the new ones is in its bits, so that of a run of 64 positions it sees a word: ones below the
+// cached positions' end, its bits from there on, cut to [lo, hi) (hi is the token's own position's end: bits past it do not count).
+__device__ __forceinline__ uint64_t ones_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
+__device__ __forceinline__ uint64_t tree_word(const AttArgs &A, const AttRow &o, int i) {
+    if (A.words == 1) return i == 0 ? o.bits : 0;
+    return (unsigned)i < (unsigned)A.words ? A.bits[(int64_t)o.tok * A.words + i] : 0;
+}
+// the bits from node `at` on (which may be negative)
+__device__ __forceinline__ uint64_t tree_bits(const AttArgs &A, const AttRow &o, int at) {
+    const int i = at >> 6, sh = at & 63;
+    const uint64_t v = tree_word(A, o, i) >> sh;
+    return sh ? v | tree_word(A, o, i + 1) << (64 - sh) : v;
+}
+// how many are set of nodes from .. the token's own, without it
+__device__ __forceinline__ int tree_count(const AttArgs &A, const AttRow &o, int from) {
+    if (A.words == 1) return __popcll(o.bits & ones_below(o.own) & ~ones_below(from));
+    int n = 0;
+    for (int i = max(from, 0) >> 6; i < min(A.words, (o.own + 63) >> 6); i++)
+        n += __popcll(A.bits[(int64_t)o.tok * A.words + i] & ones_below(o.own - 64 * i) & ~ones_below(from - 64 * i));
+    return n;
+}
+__device__ __forceinline__ uint64_t tree_sees(const AttArgs &A, const AttRow &o, int p) {   // of positions p .. p + 63
+    return (ones_below(o.ctx - p) | tree_bits(A, o, p - o.ctx)) & ones_below(o.hi - p) & ~ones_below(o.lo - p);
+}
+// The distance to position p + x (x below 64): along the path to a drafted token, which is one and the bits between. Bits of the run's nodes before the
+// token's own, and what lies behind the run.
+struct TreeFar { uint64_t bits; int at, rest; };
+__device__ __forceinline__ TreeFar tree_far(const AttArgs &A, const AttRow &o, int p) {
+    const int at = p - o.ctx;
+    return {tree_bits(A, o, at) & ones_below(o.own - at), at, tree_count(A, o, at + 64) + 1};
+}
+__device__ __forceinline__ float tree_distance(const AttRow &o, const TreeFar &f, int x) {
+    const int j = f.at + x;
+    return (float)(j < 0 ? o.pos - o.ctx - j : j >= o.own ? 0 : __popcll(f.bits >> x >> 1) + f.rest);
+}
+
+template <bool TREE> __device__ __forceinline__ void att_limits(const AttArgs &A, bool shared, const AttSeq &q, AttRow &o) {
     const mmoe_attn_args &a = A.a;
     int len = a.len[q.s];
     o.pos = len - (q.t1 - o.tok);
     if (o.tok - q.t0 >= a.max_q) o.live = false;
     o.lo = a.lo ? max(a.lo[o.tok], 0) : 0;
-    o.hi = a.hi ? a.hi[o.tok] : o.pos + 1;
+    o.hi = !TREE && a.hi ? a.hi[o.tok] : o.pos + 1;
+    if (TREE) {
+        o.ctx = len - (q.t1 - q.t0); o.own = o.tok - q.t0;
+        if (A.words == 1) o.bits = A.bits[o.tok];
+        o.pos = o.ctx + tree_count(A, o, 0);
+    }
     if (a.window > 0) o.lo = max(o.lo, o.pos - a.window);
+    if (TREE) o.lo = max(min(o.lo, o.ctx), 0);   // new tokens are seen by their bits alone
     o.hi = max(min(min(o.hi, len), a.max_len), 0);
     if (shared) o.hi = min(o.hi, a.shared); else o.lo = max(o.lo, a.shared);
+    o.full = TREE ? min(o.hi, o.ctx) : o.hi;
 }
 
 // Values of a tile that is not seen whole: are all of them finite? (bits: the type's exponent)
@@ -615,7 +662,7 @@ template <int D> struct AttTileMem {
     };
     int range[4][4], flag[2][4];
 };
-template <int T, int D, bool CAP, bool BIAS>
+template <int T, int D, bool CAP, bool BIAS, bool TREE>
 __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, const unsigned block, AttTileMem<D> &M) {
     constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // a row's bytes and chunks; rows of a load, loads of 16 rows
     constexpr int BN = ATT_BN(D), GW = BN / 64, NU = BN / 32, NK = BN / 16;   // groups of 16 positions that a wave loads; score blocks, steps of the second product
@@ -680,7 +727,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         }
     }
     AttRow R = att_row(A, at, at.row0 + w * 32 + n, kvh);
-    att_limits(A, shared, att_seq(A, shared, at, M.starts, R), R);
+    att_limits<TREE>(A, shared, att_seq(A, shared, at, M.starts, R), R);
     // queries: operand B, lane (hh, n) holds dims 16 s + 8 hh .. + 8 of row n
     u4 q[KS];
     {
@@ -695,7 +742,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     // the wave's and the workgroup's positions
     const bool some = R.live && R.lo < R.hi;
     const int wlo = wave_min(some ? R.lo : INT32_MAX), whi = wave_max(some ? R.hi : 0);
-    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
+    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.full : INT32_MAX);
     if (l == 0) { M.range[0][w] = wlo; M.range[1][w] = whi; M.range[2][w] = inlo; M.range[3][w] = inhi; }
     __syncthreads();
     int lo = INT32_MAX, hi = 0, glo = 0, ghi = INT32_MAX;
@@ -754,24 +801,37 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     };
     auto math = [&](f16v *s, int p) {
         const float dist = BIAS ? (float)(R.pos - p - 4 * hh) : 0.0f;
+        const bool path = TREE && BIAS && p + BN > inhi;   // drafted tokens among the tile's positions
 #pragma unroll
-        for (int u = 0; u < NU; u++)
+        for (int u = 0; u < NU; u++) {
+            TreeFar far;
+            if (path) far = tree_far(A, R, p + 32 * u + 4 * hh);
 #pragma unroll
             for (int j = 0; j < 16; j++) {
+                const int at = 8 * (j >> 2) + (j & 3);
                 float x = s[u][j];
                 if (CAP) x = __builtin_amdgcn_rcpf(1.0f + exp2_(x * A.s1));   // tanh z = 1 - 2 / (1 + exp 2 z)
                 if (CAP && BIAS) x = fmaf(-2.0f * A.s2, x, A.s2);
-                if (BIAS) x = fmaf(-slope, fabsf(dist - (float)(32 * u + 8 * (j >> 2) + (j & 3))), x);
+                if (BIAS) x = fmaf(-slope, path ? tree_distance(R, far, at) : fabsf(dist - (float)(32 * u + at)), x);
                 s[u][j] = x;
             }
+        }
     };
     // a tile that is not seen whole: a score of -inf where a row does not look
     auto mask = [&](f16v *s, int p, unsigned bad) {
+        if (TREE) {
+#pragma unroll
+            for (int u = 0; u < NU; u++) {
+                const uint32_t v = (uint32_t)tree_sees(A, R, p + 32 * u + 4 * hh);
+#pragma unroll
+                for (int j = 0; j < 16; j++) s[u][j] = (v >> (8 * (j >> 2) + (j & 3))) & 1 ? s[u][j] : NONE;
+            }
+        }
         const unsigned at = (unsigned)(p + 4 * hh - R.lo), span = (unsigned)max(R.hi - R.lo, 0);
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) s[u][j] = at + (32 * u + 8 * (j >> 2) + (j & 3)) < span ? s[u][j] : NONE;
+            for (int j = 0; j < 16; j++) if (!TREE) s[u][j] = at + (32 * u + 8 * (j >> 2) + (j & 3)) < span ? s[u][j] : NONE;
         if (bad)
 #pragma unroll
             for (int u = 0; u < NU; u++)
@@ -865,7 +925,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     auto add_odd = [&](uint32_t buf, int p, unsigned bad) {
 #pragma unroll 1
         for (int r = 0; r < BN; r++) {
-            const bool see = p + r >= R.lo && p + r < R.hi && !((bad >> (r >> 4)) & 1);
+            const bool see = (TREE ? (bool)(tree_sees(A, R, p + r) & 1) : p + r >= R.lo && p + r < R.hi) && !((bad >> (r >> 4)) & 1);
             uint32_t row = r * RB + 8 * hh, x = (r & (CH / 2 - 1)) << 5;
             asm("" : "+v"(row));   // its addresses are not worth a register outside
 #pragma unroll
@@ -1004,7 +1064,7 @@ template <int D> struct AttFewMem {
     };
     float2 stat[4][16];
 };
-template <int T, int D, bool CAP, bool BIAS>
+template <int T, int D, bool CAP, bool BIAS, bool TREE>
 __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, const unsigned block, AttFewMem<D> &M) {
     constexpr int KS = D / 32, E = D / 16;   // products over the dims, values of a row per lane
     const mmoe_attn_args &a = A.a;
@@ -1076,7 +1136,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     if (early) { id = ids(p); next = ids(p + 128); }
     const AttSeq sq = att_seq(A, shared, at, M.starts, R);
     if (early && p < end) { load_k(p, id); load_v(p, id); }
-    att_limits(A, shared, sq, R);
+    att_limits<TREE>(A, shared, sq, R);
     u4 q[KS];
     {
         const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * g;
@@ -1088,7 +1148,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     const int seen = wave_min(some ? R.lo : INT32_MAX);   // the first position that any row sees
     int p0 = max(from, seen & ~31), p1 = min(end, wave_max(some ? R.hi : 0));
     if (p0 >= p1) p0 = p1 = 0;   // nothing seen (p0 may be close to the largest int: no wave's first run is counted from it)
-    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
+    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.full : INT32_MAX);
     f4 acc[E];
 #pragma unroll
     for (int e = 0; e < E; e++) acc[e] = f4{0, 0, 0, 0};
@@ -1121,17 +1181,21 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         }
         after_scores();
         const float dist = BIAS ? (float)(R.pos - p - 4 * g) : 0.0f;
-        const bool part = p < inlo || p + 32 > inhi || r.bad;
+        const bool part = p < inlo || p + 32 > inhi || r.bad, path = TREE && BIAS && p + 32 > inhi;   // (drafted tokens among the run's)
         float mt = -__builtin_inff();
+        TreeFar far;
+        if (path) far = tree_far(A, R, p + 4 * g);
+        uint32_t sees = 0;
+        if (TREE && part) sees = (uint32_t)tree_sees(A, R, p + 4 * g);
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 float x = s[u][j] * A.s1;
                 if (CAP) x = fmaf(-2.0f * A.s2, __builtin_amdgcn_rcpf(1.0f + exp2_(x)), A.s2);
-                if (BIAS) x = fmaf(-slope, fabsf(dist - (float)(16 * u + j)), x);
+                if (BIAS) x = fmaf(-slope, path ? tree_distance(R, far, 16 * u + j) : fabsf(dist - (float)(16 * u + j)), x);
                 int at = p + 16 * u + 4 * g + j;
-                if (part) x = at >= R.lo && at < R.hi && !((r.bad >> u) & 1) ? x : -__builtin_inff();
+                if (part) x = (TREE ? (bool)((sees >> (16 * u + j)) & 1) : at >= R.lo && at < R.hi) && !((r.bad >> u) & 1) ? x : -__builtin_inff();
                 s[u][j] = x;
                 mt = fmaxf(mt, x);
             }
@@ -1215,7 +1279,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
             __builtin_amdgcn_wave_barrier();   // a wave's LDS operations stay in order
 #pragma unroll 1
             for (int k = 0; k < 32; k++) {
-                const bool see = p + k >= R.lo && p + k < R.hi && !((r.bad >> (k >> 4)) & 1);
+                const bool see = (TREE ? (bool)(tree_sees(A, R, p + k) & 1) : p + k >= R.lo && p + k < R.hi) && !((r.bad >> (k >> 4)) & 1);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -1287,20 +1351,20 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
 }
 
 // One launch for everything, the long work first. With no row tiles of 128 in it a kernel of its own: fewer registers, more waves.
-template <int T, int D, bool CAP, bool BIAS>
+template <int T, int D, bool CAP, bool BIAS, bool TREE>
 __global__ void __launch_bounds__(256, 2) k_attn_few(AttArgs A) {
     __shared__ AttFewMem<D> M;
     const unsigned b = blockIdx.x;
     const bool shared = b < A.n_sh;
-    att_few<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh, M);
+    att_few<T, D, CAP, BIAS, TREE>(A, shared, shared ? b : b - A.n_sh, M);
 }
-template <int T, int D, bool CAP, bool BIAS>
+template <int T, int D, bool CAP, bool BIAS, bool TREE>
 __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
     __shared__ union { AttTileMem<D> tile; AttFewMem<D> few; } M;
     const unsigned b = blockIdx.x;
     const bool shared = b < A.n_sh;
-    if (shared ? !A.sh_few : b < A.n_sh + A.n_tile) att_tile<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh, M.tile);
-    else att_few<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh - A.n_tile, M.few);
+    if (shared ? !A.sh_few : b < A.n_sh + A.n_tile) att_tile<T, D, CAP, BIAS, TREE>(A, shared, shared ? b : b - A.n_sh, M.tile);
+    else att_few<T, D, CAP, BIAS, TREE>(A, shared, shared ? b : b - A.n_sh - A.n_tile, M.few);
 }
 
 // The partial results of a row: their maxima and sums give each a weight. D / 4 lanes read a part; with all, every such group of the
@@ -1310,7 +1374,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
 #define ATT_PARTS 1024     // most partial results of a row
 #define ATT_PER 16
 template <int T, int D>
-__global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_only) {
+static __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_only) {
     constexpr int LPR = D / 4;
     const mmoe_attn_args &a = A.a;
     __shared__ float red[2][16], wt[ATT_PARTS];

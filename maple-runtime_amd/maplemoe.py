@@ -26,10 +26,10 @@ COMBINE_OVERWRITE, COMBINE_BATCH, COMBINE_ADD, COMBINE_STEP = 0, 1, 4, 6
 R = dict(LOGITS=0, TOP=1, TW=2, PLAN=3, UTOK=4, UW=5, TP=6, SP=7, QX=8, QSX=9, QSUMX=10, ACT=11, QA=12, QSA=13,
          QSUMA=14, DOWN=15, GU_I32=16, DN_I32=17, X=18, HN=19)
 KERNELS = ["rmsnorm", "router", "topk", "group", "quant", "gateup", "quant_act", "down", "combine", "dense", "qkn",
-           "att_scores", "att_softmax", "att_pv", "kv_plan", "rope", "att_paged"]
+           "att_scores", "att_softmax", "att_pv", "kv_plan", "rope", "att_paged", "tree", "att_tree", "kv_pages"]
 F32, F16, BF16 = 0, 1, 2
 DTYPE = dict(f32=F32, f16=F16, bf16=BF16)
-KV_MAXSEQ = 4096
+KV_MAXSEQ, KV_MAXLAYERS, TREE_MAX = 4096, 128, 512
 
 
 def _struct(name, doc, *fields):
@@ -47,6 +47,15 @@ Rope = _struct("Rope", "mmoe_rope_args", (C.c_void_p, "q k v q_out k_out"),
 PagedAttn = _struct("PagedAttn", "mmoe_attn_args", (C.c_void_p, "q out lse"), (C.c_int64, "q_token q_head out_token out_head"),
                     (C.c_void_p, "qstart len table lo hi slopes ws"), (C.c_size_t, "ws_bytes"),
                     (C.c_int32, "nseq ntok heads width max_q max_len shared window"), (C.c_float, "scale cap"))
+TreePlan = _struct("TreePlan", "mmoe_tree_plan_args", (C.c_void_p, "qstart len parent pos bits"), (C.c_int32, "nseq ntok words"))
+TreeAccept = _struct("TreeAccept", "mmoe_tree_accept_args", (C.c_void_p, "qstart len parent token next kept count ctx last"), (C.c_int32, "nseq ntok"))
+KvCompact = _struct("KvCompact", "mmoe_kv_compact_args", (C.c_void_p, "table first count kept"), (C.c_int32, "nseq width nkept"))
+KvFork = _struct("KvFork", "mmoe_kv_fork_args",
+                 (C.c_void_p, "src dst at ctx table ctx_out table_out holders free_list nfree nfree_out copy_from copy_to copy_count"),
+                 (C.c_int32, "nfork nseq width nblocks block_size shared"))
+KvCopy = _struct("KvCopy", "mmoe_kv_copy_args", (C.c_void_p, "copy_from copy_to copy_count"), (C.c_int32, "ncopy"))
+KvFree = _struct("KvFree", "mmoe_kv_free_args", (C.c_void_p, "ctx keep table nfree len free_list nfree_out holders"),
+                 (C.c_int32, "nseq width nblocks block_size shared"))
 
 _lib = None
 _slib = None
@@ -112,6 +121,11 @@ def _declare(L):
         "mmoe_kv_plan": (i, [C.POINTER(KvPlan)]), "mmoe_rope_freqs": (i, [i, d, d, i, d, d, vp]),
         "mmoe_rope_kv": (i, [C.POINTER(Rope), C.POINTER(KvCache)]),
         "mmoe_attn_paged_ws": (sz, [C.POINTER(PagedAttn), C.POINTER(KvCache)]), "mmoe_attn_paged": (i, [C.POINTER(PagedAttn), C.POINTER(KvCache)]),
+        "mmoe_tree_plan": (i, [C.POINTER(TreePlan)]), "mmoe_tree_accept": (i, [C.POINTER(TreeAccept)]),
+        "mmoe_attn_tree_ws": (sz, [C.POINTER(PagedAttn), C.POINTER(KvCache), vp, i]),
+        "mmoe_attn_tree": (i, [C.POINTER(PagedAttn), C.POINTER(KvCache), vp, i]),
+        "mmoe_kv_compact": (i, [C.POINTER(KvCompact), C.POINTER(KvCache), i]), "mmoe_kv_fork": (i, [C.POINTER(KvFork)]),
+        "mmoe_kv_copy": (i, [C.POINTER(KvCopy), C.POINTER(KvCache), i]), "mmoe_kv_free": (i, [C.POINTER(KvFree)]),
         "mmoe_ckpt_bf16": (vp, [i, i]), "mmoe_ckpt_load": (i, [i, i]),
     }
     for name, (res, args) in sig.items():
