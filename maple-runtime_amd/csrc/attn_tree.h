@@ -1,0 +1,251 @@
+// attn_tree.h -- attention of drafted tokens over the blocks (mmoe_attn_tree, drafts.hip).
+//
+// The row tiles are mmoe_attn_paged's (att_tile, with masks from the tokens' bits). What differs is who gets which: a draft makes few row tiles per
+// sequence, each as long as the sequence, so that time goes by how evenly they are shared out. The row tiles' positions are cut into pieces of at most a
+// number of steps (of TREE_BN positions) which is so chosen that there are no more pieces than the card has room for at once (two workgroups
+// per compute unit): a few more would wait for a second round. Every workgroup finds its piece from the sequences' lengths themselves, so grid and
+// workspace follow the numbers of workgroups and row tiles, not the bounds of the lengths.
+#pragma once
+#include "paged.h"
+
+// A row tile for the join: its first piece, how many, its first token, its first row among its sequence's, the sequence's rows. The first entry holds
+// the number of row tiles in `slot`; behind it the shared positions' tiles, then the sequences' own.
+struct TreeTile { int slot, parts, t0, row0, rows; };
+
+struct Draft {
+    struct Seq { int t0, t1, len, rows, tiles, from, to, steps; };
+    // the shared positions' rows (every token) as a sequence of its own
+    __device__ static __forceinline__ Seq of_shared(const AttArgs &A) {
+        Seq q = {0, 0, 0, A.a.shared ? att_start(A.a, A.a.nseq) * A.group : 0, 0, 0, A.a.shared, (A.a.shared + TREE_BN - 1) / TREE_BN};
+        q.tiles = (q.rows + ATT_BM - 1) / ATT_BM;
+        return q;
+    }
+    __device__ static __forceinline__ Seq of(const AttArgs &A, int s) {
+        const mmoe_attn_args &a = A.a;
+        Seq q = {};
+        if (s >= a.nseq) return q;
+        q.t0 = att_start(a, s); q.t1 = a.qstart[s + 1]; q.len = a.len[s];
+        const int n = max(q.t1, q.t0) - q.t0;
+        q.rows = min(max(min(q.t1, a.ntok) - q.t0, 0), a.max_q) * A.group;   // (inside the arrays)
+        q.tiles = (q.rows + ATT_BM - 1) / ATT_BM;
+        q.from = a.shared;
+        if (a.window > 0) q.from = max(q.from, q.len - n - a.window);
+        q.from &= ~(TREE_BN - 1);
+        q.to = min(q.len - max(n - a.max_q, 0), a.max_len);
+        q.steps = max(q.to - q.from + TREE_BN - 1, 0) / TREE_BN;
+        return q;
+    }
+    // pieces of a row tile: its steps times the pieces per step, rounded up (up to 2^-10 above a whole number that one is taken)
+    __device__ static __forceinline__ int cut(const Seq &q, float per) { return max((int)ceilf(fmaf((float)q.steps, per, -0x1p-10f)), 1); }
+    struct Mem { int sum[2][4], at[4]; };
+    __device__ static __forceinline__ int wave_sum(int v) { return wave_reduce(v, [](int x, int y) { return x + y; }); }
+    struct Piece { int seq, base, tiles, all_tiles, k; Seq q; };
+    // Piece id of a key/value head: its sequence (-1: the shared positions), that one's first piece and row tile, how many row tiles there are in all, the
+    // pieces of a row tile; false: there is no such piece. The same for every thread of the workgroup (256).
+    __device__ static __forceinline__ bool find(const AttArgs &A, int id, Mem &M, Piece &o) {
+        const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, n = A.a.nseq;
+        const Seq sh = of_shared(A), q = of(A, n <= 64 ? l : tid);
+        // a sum over all sequences: every wave by itself, or all of them together
+        auto total = [&](auto &&f) {
+            int v = f(q);
+            if (n <= 64) return wave_sum(v);
+            for (int s = tid + 256; s < n; s += 256) v += f(of(A, s));
+            v = wave_sum(v);
+            __syncthreads();
+            if (l == 0) M.sum[0][w] = v;
+            __syncthreads();
+            return M.sum[0][0] + M.sum[0][1] + M.sum[0][2] + M.sum[0][3];
+        };
+        o.all_tiles = sh.tiles + total([](const Seq &x) { return x.tiles; });
+        float per = 0.0f;   // pieces per step
+        if (A.room) {
+            // (the host has seen to it that all steps are a 32-bit number)
+            const int steps = sh.tiles * sh.steps + total([](const Seq &x) { return x.tiles * x.steps; });
+            // where the row tiles alone come near to what there is room for, there are more rounds anyway: half as large pieces then, and no search
+            const bool few = 4 * o.all_tiles <= 3 * A.room;
+            const int goal = few ? A.room : 2 * A.room;
+            // rounding up makes about half a piece more of each row tile
+            per = fminf(((float)goal - (few ? 0.5f * (float)o.all_tiles : 0.0f)) / (float)max(steps, 1), 1.0f / (float)A.least);
+            for (int i = 0; few; i++) {
+                const int got = sh.tiles * cut(sh, per) + total([&](const Seq &x) { return x.tiles * cut(x, per); });
+                if (got <= goal) break;
+                per = i < 6 ? per * fminf((float)goal / (float)got, 0.97f) : 0.0f;   // (at last each row tile one piece)
+            }
+        }
+        o.seq = -1; o.base = 0; o.tiles = 0; o.k = cut(sh, per); o.q = sh;
+        const int common = sh.tiles * o.k;
+        if (id < common) return true;
+        if (n <= 64) {
+            const int mine = q.tiles * cut(q, per), end = common + (int)scan_wave(mine), tiles = sh.tiles + (int)scan_wave(q.tiles) - q.tiles;
+            const int s = __popcll(__ballot(id >= end));   // a prefix of the lanes
+            if (s >= n) return false;
+            auto lane = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
+            o.seq = s; o.base = lane(end - mine); o.tiles = lane(tiles);
+            o.q = {lane(q.t0), lane(q.t1), lane(q.len), lane(q.rows), lane(q.tiles), lane(q.from), lane(q.to), lane(q.steps)};
+            o.k = cut(o.q, per);
+            return true;
+        }
+        int before = common, tiles = sh.tiles;
+        if (tid == 0) M.at[0] = -1;
+        for (int s0 = 0; s0 < n; s0 += 256) {
+            const Seq x = of(A, s0 + tid);
+            const int mine = x.tiles * cut(x, per);
+            int end = (int)scan_wave(mine), t = (int)scan_wave(x.tiles);
+            __syncthreads();   // the sums before have been read
+            if (l == 63) { M.sum[0][w] = end; M.sum[1][w] = t; }
+            __syncthreads();
+            int pieces = 0, ts = 0;
+            for (int i = 0; i < 4; i++) {
+                if (i < w) { end += M.sum[0][i]; t += M.sum[1][i]; }
+                pieces += M.sum[0][i]; ts += M.sum[1][i];
+            }
+            end += before; t += tiles;
+            if (id < end && id >= end - mine) { M.at[0] = s0 + tid; M.at[1] = end - mine; M.at[2] = t - x.tiles; }
+            before += pieces; tiles += ts;
+            if (id < before) break;
+        }
+        __syncthreads();
+        o.seq = __builtin_amdgcn_readfirstlane(M.at[0]); o.base = __builtin_amdgcn_readfirstlane(M.at[1]); o.tiles = __builtin_amdgcn_readfirstlane(M.at[2]);
+        if (o.seq < 0) return false;
+        o.q = of(A, o.seq);
+        o.k = cut(o.q, per);
+        return true;
+    }
+};
+
+template <int T, int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
+    __shared__ AttTileMem<D, TREE_BN> M;
+    __shared__ Draft::Mem F;
+    const int id = (int)A.by_kv(blockIdx.x), kvh = blockIdx.x - id * A.kv.heads;
+    Draft::Piece o;
+    if (!Draft::find(A, id, F, o)) return;
+    const Draft::Seq &q = o.q;
+    const int k = __builtin_amdgcn_readfirstlane(o.k), steps = __builtin_amdgcn_readfirstlane(q.steps), tile = (id - o.base) / k, i = id - o.base - tile * k;
+    if (o.tiles + tile >= A.most_tiles) return;   // (not if qstart ascends)
+    if (A.room && kvh == 0 && i == 0 && threadIdx.x == 0) {
+        A.tile_at[1 + o.tiles + tile] = {id, k, q.t0, tile * ATT_BM, q.rows};
+        if (id == 0) A.tile_at[0].slot = min(o.all_tiles, A.most_tiles);
+    }
+    const int each = steps / k, more = steps - each * k;
+    AttWork work = {};
+    work.shared = o.seq < 0;
+    work.at = {max(o.seq, 0), tile * ATT_BM, q.rows, q.t0};
+    work.t1 = q.t1; work.len = q.len;
+    work.kvh = kvh;
+    work.p0 = q.from + (i * each + min(i, more)) * TREE_BN;
+    work.p1 = min(work.p0 + (each + (i < more)) * TREE_BN, q.to);
+    work.whole = k == 1 && !A.a.shared;
+    work.slot = (int64_t)id * A.kv.heads + kvh;
+    att_tile<T, D, CAP, BIAS, true>(tree_args(), work, M);
+}
+
+// The partial results of a row tile put together, 32 rows by a workgroup: each result holds its values over its own sum, its maximum (in units of log 2)
+// and sum, negative where results may not be finite. A lane has a row and 4 of each 8 dims, a wave a quarter of the dims (wide) or of the results
+// (deep: then a quarter of the dims is a workgroup's own, and the waves join through LDS).
+#define TJ_U 4   // results under way
+template <int T, int D, bool DEEP>
+__global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
+    constexpr int C = D / 32;   // groups of 8 dims of a lane
+    const mmoe_attn_args &a = A.a;
+    __shared__ f4 acc[DEEP ? 3 : 1][C][64];
+    __shared__ float2 stat[DEEP ? 3 : 1][32];
+    const int l = threadIdx.x & 63, n = l & 31, hh = l >> 5, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned id = blockIdx.x;
+    int quarter = wv;
+    if (DEEP) { quarter = id & 3; id >>= 2; }
+    const int w = id & 3;   // the tile's wave, its key/value head, its number
+    id >>= 2;
+    const int tile = (int)A.by_kv(id), kvh = id - tile * A.kv.heads;
+    const int first = a.shared ? (att_start(a, a.nseq) * A.group + ATT_BM - 1) / ATT_BM : 0;   // row tiles over the shared positions
+    const TreeTile t = A.tile_at[1 + min(first + tile, A.most_tiles - 1)];
+    if (first + tile >= A.tile_at[0].slot || (t.parts == 1 && !a.shared)) return;   // none, or written by the piece that was all of it
+    // nothing outside the arrays, whatever qstart holds
+    auto inside = [&](const TreeTile &t) { return t.slot >= 0 && t.parts > 0 && t.parts <= A.most_pieces - t.slot; };
+    if (!inside(t) || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
+    const int r = t.row0 + w * 32 + n;
+    if (t.row0 + w * 32 >= t.rows) return;
+    const bool live = r < t.rows;
+    const int row = min(r, t.rows - 1), j = (int)A.by_group(row), tok = t.t0 + j, head = kvh * A.group + row - j * A.group;
+    int common = 0, at_sh = 0, slot_sh = 0;
+    if (a.shared) {
+        const int rs = tok * A.group + row - j * A.group;
+        const TreeTile &s = A.tile_at[1 + rs / ATT_BM];
+        if (inside(s)) { common = s.parts; slot_sh = s.slot; at_sh = rs % ATT_BM; }
+    }
+    const int most = DEEP || a.shared ? wave_max(common) : 0, parts = most + t.parts;   // (rows may lie in two shared tiles)
+    float m = -__builtin_inff(), sum = 0.0f;
+    f4 o[C] = {};
+    bool wild = false;
+    auto lowered_to = [&](float mn) {   // what is there counts from the maximum mn on
+        const float al = m == -__builtin_inff() ? 0.0f : exp2_(m - mn);
+        m = mn; sum *= al;
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[c][i] = al != 0.0f ? o[c][i] * al : only_odd(o[c][i]);
+    };
+    auto add = [&](float2 v, const f4 *y) {
+        if (v.y == 0.0f) return;
+        const float e = exp2_(v.x - m);
+        sum = fmaf(fabsf(v.y), e, sum);
+        wild |= v.y < 0.0f;
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[c][i] = e != 0.0f ? fmaf(e, y[c][i], o[c][i]) : o[c][i] + (v.y < 0.0f ? only_odd(y[c][i]) : 0.0f);
+    };
+    constexpr int STEP = DEEP ? 4 : 1;
+    for (int p0 = DEEP ? wv : 0; p0 < parts; p0 += TJ_U * STEP) {
+        float2 v[TJ_U];
+        f4 y[TJ_U][C];
+#pragma unroll
+        for (int u = 0; u < TJ_U; u++) {
+            const int p = p0 + u * STEP;
+            const bool c = p < most;
+            v[u] = make_float2(0.0f, 0.0f);
+            if (p >= parts || (c && p >= common)) continue;
+            const int at = c ? at_sh : w * 32 + n;
+            const int64_t wave = ((int64_t)(c ? slot_sh + p : t.slot + p - most) * A.kv.heads + kvh) * A.slot_waves + (at >> 5);
+            v[u] = A.pm[wave * 32 + (at & 31)];
+            const f4 *q = (const f4 *)(A.po + wave * 32 * D) + 32 * hh + (at & 31);
+#pragma unroll
+            for (int i = 0; i < C; i++) y[u][i] = q[(quarter * C + i) * 64];
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < TJ_U; u++) if (v[u].y != 0.0f) mn = fmaxf(mn, v[u].x);
+        if (mn > m) lowered_to(mn);
+#pragma unroll
+        for (int u = 0; u < TJ_U; u++) add(v[u], y[u]);
+    }
+    if (DEEP) {
+        if (wv) {
+#pragma unroll
+            for (int c = 0; c < C; c++) acc[wv - 1][c][l] = o[c];
+            if (hh == 0) stat[wv - 1][n] = make_float2(m, wild ? -sum : sum);
+        }
+        __syncthreads();
+        if (wv) return;
+        float mn = m;
+        for (int i = 0; i < 3; i++) if (stat[i][n].y != 0.0f) mn = fmaxf(mn, stat[i][n].x);
+        if (mn > m) lowered_to(mn);
+        for (int i = 0; i < 3; i++) {
+            f4 y[C];
+#pragma unroll
+            for (int c = 0; c < C; c++) y[c] = acc[i][c][l];
+            add(stat[i][n], y);
+        }
+    }
+    if (!live) return;
+    const float inv = 1.0f / sum;
+    uint16_t *out = (uint16_t *)a.out + (int64_t)tok * a.out_token + head * a.out_head + quarter * (D / 4) + 4 * hh;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        uint2 v = make_uint2(pack2<T>(o[c][0] * inv, o[c][1] * inv), pack2<T>(o[c][2] * inv, o[c][3] * inv));
+        if (sum == 0.0f) v = make_uint2(0, 0);
+        *(uint2 *)(out + 8 * c) = v;
+    }
+    if (a.lse && quarter == 0 && hh == 0) a.lse[(int64_t)tok * a.heads + head] = sum == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * ATT_LN2;
+}
+

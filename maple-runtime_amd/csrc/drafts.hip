@@ -1,6 +1,7 @@
 // drafts.hip -- drafted tokens and shared blocks (include/maplemoe.h, Part 3): argument checks and launches.
 #include "paged_host.h"
 #include "drafts.h"
+#include "attn_tree.h"
 
 static int check_bits(const char *who, const mmoe_attn_args *p, const mmoe_kv_cache *kv, int words) {
     if (check_attn(who, p, kv)) return -1;
@@ -8,6 +9,57 @@ static int check_bits(const char *who, const mmoe_attn_args *p, const mmoe_kv_ca
     if (words < 1 || words > MMOE_TREE_MAX / 64) REFUSE("%s: %d words of bits outside 1..%d", who, words, MMOE_TREE_MAX / 64);
     if (p->max_q > 64 * words) REFUSE("%s: max_q %d for %d words of bits", who, p->max_q, words);
     return 0;
+}
+
+// How a call of mmoe_attn_tree is divided (drafts.h). Only the values in the arguments count (a captured call keeps its grid). The numbers of
+// workgroups are for the 256 compute units of the one device that the kernels are built and were measured for.
+struct TreePlan {
+    int room, least, pieces, slot_waves, tiles;
+    unsigned join;
+    bool deep, fits;
+    size_t results, bytes;
+};
+static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
+    TreePlan p = {};
+    const int group = a.heads / kv.heads;
+    const int64_t rows = (int64_t)a.ntok * group, most = (int64_t)std::min(a.max_q, a.ntok) * group;
+    const int64_t tiles = std::min((int64_t)a.nseq * ((most + ATT_BM - 1) / ATT_BM), rows / ATT_BM + a.nseq) + (a.shared ? (rows + ATT_BM - 1) / ATT_BM : 0);
+    // Row tiles of so few positions, and so many of them, that they stay whole: nothing to join
+    const int64_t most_steps = (a.window ? std::min<int64_t>(a.max_len, (int64_t)a.window + a.max_q + TREE_BN) : a.max_len) / TREE_BN + 1;
+    const bool whole = !a.shared && most_steps <= 12 && tiles * kv.heads >= 192;
+    p.room = whole ? 0 : std::max(1, (kv.head_dim == 64 ? 768 : 512) / kv.heads);   // two workgroups per compute unit, three with heads of 64
+    p.least = 2;
+    const int64_t pieces = whole ? tiles : std::max(tiles <= p.room * 3 / 4 ? (int64_t)p.room : 2 * (int64_t)p.room + tiles, tiles), join = tiles * kv.heads * 4;
+    p.deep = join < 128;   // 32 rows of a key/value head each
+    p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(pieces * kv.heads, join * (p.deep ? 4 : 1)) * 256 <= (int64_t)MAX_THREADS;
+    p.pieces = (int)std::min<int64_t>(pieces, INT32_MAX); p.tiles = (int)std::min<int64_t>(tiles, INT32_MAX); p.join = (unsigned)(p.deep ? join * 4 : join);
+    p.slot_waves = a.shared ? ATT_BM / 32 : (int)std::min<int64_t>(ATT_BM, most + 31) / 32;
+    p.results = whole ? 0 : (size_t)pieces * kv.heads * p.slot_waves;
+    p.bytes = p.results * 32 * (kv.head_dim * 4 + 8) + (whole ? 0 : (size_t)(tiles + 1) * sizeof(TreeTile)) + 256;
+    return p;
+}
+
+template <int T, int D, bool CAP, bool BIAS>
+static int tree_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const TreePlan &p, const uint64_t *bits, int words) {
+    AttArgs A{};
+    A.a = a; A.kv = kv;
+    A.sh = log2_block(kv.block_size); A.group = a.heads / kv.heads;
+    A.by_kv = divisor(kv.heads); A.by_group = divisor(A.group);
+    A.s1 = CAP ? 2.0f * a.scale / a.cap * ATT_LOG2E : a.scale * ATT_LOG2E;
+    A.s2 = a.cap * ATT_LOG2E;
+    A.bits = bits; A.words = words;
+    A.room = p.room; A.least = p.least; A.most_tiles = p.tiles; A.most_pieces = p.pieces; A.slot_waves = p.slot_waves;
+    A.po = (float *)a.ws;
+    A.pm = (float2 *)(A.po + p.results * 32 * D);
+    A.tile_at = (TreeTile *)(A.pm + p.results * 32);
+    if (run(MMOE_K_ATT_TREE, k_attn_tree<T, D, CAP, BIAS>, (unsigned)p.pieces * kv.heads, 256, A)) return -1;
+    if (!p.room) return 0;
+    return p.deep ? run(MMOE_K_ATT_TREE, k_tree_join<T, D, true>, p.join, 256, A) : run(MMOE_K_ATT_TREE, k_tree_join<T, D, false>, p.join, 256, A);
+}
+template <int T, int D>
+static int tree_pick(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const TreePlan &p, const uint64_t *b, int w) {
+    if (a.cap > 0) return a.slopes ? tree_run<T, D, true, true>(a, kv, p, b, w) : tree_run<T, D, true, false>(a, kv, p, b, w);
+    return a.slopes ? tree_run<T, D, false, true>(a, kv, p, b, w) : tree_run<T, D, false, false>(a, kv, p, b, w);
 }
 
 // The layers' caches of a call that works on all of them
@@ -67,13 +119,25 @@ int mmoe_tree_plan(const mmoe_tree_plan_args *p) {
 size_t mmoe_attn_tree_ws(const mmoe_attn_args *p, const mmoe_kv_cache *kv, const uint64_t *bits, int words) {
     (void)bits;
     if (check_bits("mmoe_attn_tree", p, kv, words)) return 0;
-    return att_plan(*p, *kv).bytes;
+    return tree_plan(*p, *kv).bytes;
 }
 
 int mmoe_attn_tree(const mmoe_attn_args *p, const mmoe_kv_cache *kv, const uint64_t *bits, int words) {
     if (check_bits("mmoe_attn_tree", p, kv, words)) return -1;
+    const mmoe_attn_args &a = *p;
+    if (!a.nseq || !a.ntok) return 0;
+    if (!a.q || !a.out || !a.qstart || !a.len || !a.table || !bits) REFUSE("mmoe_attn_tree: a pointer is missing");
+    if (apart(a.q, 16) || apart(a.out, 16)) REFUSE("mmoe_attn_tree: q and out must be aligned to 16 bytes");
     if (apart(bits, 8)) REFUSE("mmoe_attn_tree: bits must be aligned to 8 bytes");
-    return att_call<true>("mmoe_attn_tree", *p, kv, bits, words);
+    const TreePlan pl = tree_plan(a, *kv);
+    if (!pl.fits) REFUSE("mmoe_attn_tree: %d sequences of up to %d positions, %d tokens, %d heads: too many for a launch", a.nseq, a.max_len, a.ntok, a.heads);
+    if (!a.ws || a.ws_bytes < pl.bytes || apart(a.ws, 256)) REFUSE("mmoe_attn_tree: workspace of %zu bytes (%zu needed, aligned to 256)", a.ws ? a.ws_bytes : 0, pl.bytes);
+    if (mm_ready()) return -1;
+    if (!a.max_q) return 0;   // no token is served
+    OnDevice dev;
+    if (!dev.ok) return -1;
+    if (kv->dtype == MMOE_F16) return kv->head_dim == 64 ? tree_pick<MMOE_F16, 64>(a, *kv, pl, bits, words) : tree_pick<MMOE_F16, 128>(a, *kv, pl, bits, words);
+    return kv->head_dim == 64 ? tree_pick<MMOE_BF16, 64>(a, *kv, pl, bits, words) : tree_pick<MMOE_BF16, 128>(a, *kv, pl, bits, words);
 }
 
 int mmoe_tree_accept(const mmoe_tree_accept_args *p) {

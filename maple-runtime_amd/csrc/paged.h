@@ -438,6 +438,7 @@ __global__ void __launch_bounds__(RP_T) k_rope(mmoe_rope_args a, mmoe_kv_cache k
 // rows' visible runs [lo, hi) are all there is to masks: a tile that every live row sees whole needs none.
 #define ATT_BM 128         // rows of a tile
 #define ATT_BN(D) (8192 / (D))   // and its positions: 32 KB of keys and values for either head size
+#define TREE_BN 64               // positions of a tile of drafted tokens' rows
 #define ATT_LOG2E 1.44269504088896340736f
 #define ATT_LN2 0.69314718055994530942f
 
@@ -476,8 +477,12 @@ struct AttArgs {
     float *po;
     float2 *pm;
     int64_t at_tile, at_few;
-    const uint64_t *bits;   // drafted tokens (TREE): words per token, bit j: it sees its sequence's j-th new token
-    int words;
+    // Drafted tokens (TREE, attn_tree.h): words of bits per token, bit j: it sees its sequence's j-th new token; the pieces that the row tiles of a key/
+    // value head are to be cut into (0: none, each stays whole), the fewest steps of one, the most row tiles and pieces there can be, waves (of 32
+    // rows) of a piece's partial results in po and pm; the row tiles
+    const uint64_t *bits;
+    int words, room, least, most_tiles, most_pieces, slot_waves;
+    struct TreeTile *tile_at;
 };
 
 template <int T> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
@@ -573,18 +578,20 @@ __device__ __forceinline__ AttSeq att_seq(const AttArgs &A, bool shared, const A
     } else { t0 = a.qstart[s]; t1 = a.qstart[s + 1]; }
     return {s, t0, t1};
 }
-// Masks of drafted tokens. What a token sees of the new ones is in its bits, so that of a run of 64 positions it sees a word: ones below the
+// Masks of drafted tokens. What a token sees of the new ones is in its bits, so that of a run of 32 positions it sees a word: ones below the
 // cached positions' end, its bits from there on, cut to [lo, hi) (hi is the token's own position's end: bits past it do not count).
 __device__ __forceinline__ uint64_t ones_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
+__device__ __forceinline__ uint32_t ones32(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 __device__ __forceinline__ uint64_t tree_word(const AttArgs &A, const AttRow &o, int i) {
     if (A.words == 1) return i == 0 ? o.bits : 0;
     return (unsigned)i < (unsigned)A.words ? A.bits[(int64_t)o.tok * A.words + i] : 0;
 }
-// the bits from node `at` on (which may be negative)
-__device__ __forceinline__ uint64_t tree_bits(const AttArgs &A, const AttRow &o, int at) {
+// the bits of 32 nodes from `at` on (which may be negative)
+__device__ __forceinline__ uint32_t tree_bits(const AttArgs &A, const AttRow &o, int at) {
     const int i = at >> 6, sh = at & 63;
-    const uint64_t v = tree_word(A, o, i) >> sh;
-    return sh ? v | tree_word(A, o, i + 1) << (64 - sh) : v;
+    uint64_t v = tree_word(A, o, i) >> sh;
+    if (sh > 32) v |= tree_word(A, o, i + 1) << (64 - sh);
+    return (uint32_t)v;
 }
 // how many are set of nodes from .. the token's own, without it
 __device__ __forceinline__ int tree_count(const AttArgs &A, const AttRow &o, int from) {
@@ -594,24 +601,21 @@ __device__ __forceinline__ int tree_count(const AttArgs &A, const AttRow &o, int
         n += __popcll(A.bits[(int64_t)o.tok * A.words + i] & ones_below(o.own - 64 * i) & ~ones_below(from - 64 * i));
     return n;
 }
-__device__ __forceinline__ uint64_t tree_sees(const AttArgs &A, const AttRow &o, int p) {   // of positions p .. p + 63
-    return (ones_below(o.ctx - p) | tree_bits(A, o, p - o.ctx)) & ones_below(o.hi - p) & ~ones_below(o.lo - p);
+__device__ __forceinline__ uint32_t tree_sees(const AttArgs &A, const AttRow &o, int p) {   // of positions p .. p + 31
+    return (ones32(o.ctx - p) | tree_bits(A, o, p - o.ctx)) & ones32(o.hi - p) & ~ones32(o.lo - p);
 }
-// The distance to position p + x (x below 64): along the path to a drafted token, which is one and the bits between. Bits of the run's nodes before the
-// token's own, and what lies behind the run.
-struct TreeFar { uint64_t bits; int at, rest; };
+// Distances. The path that a token sees, cached positions and all, is a chain of ones whose last is the token itself: the distance to position p + x is the
+// number of ones behind it. ones: of the 32 positions from p on; rest: how many lie behind those.
+struct TreeFar { uint32_t ones; int rest; };
 __device__ __forceinline__ TreeFar tree_far(const AttArgs &A, const AttRow &o, int p) {
-    const int at = p - o.ctx;
-    return {tree_bits(A, o, at) & ones_below(o.own - at), at, tree_count(A, o, at + 64) + 1};
+    const int at = p - o.ctx, end = o.own - at;
+    return {((ones32(-at) | tree_bits(A, o, at)) & ones32(end)) | (end >= 0 && end < 32 ? 1u << end : 0u),
+            max(-at - 32, 0) + tree_count(A, o, at + 32) + (end >= 32 ? 1 : 0)};
 }
-__device__ __forceinline__ float tree_distance(const AttRow &o, const TreeFar &f, int x) {
-    const int j = f.at + x;
-    return (float)(j < 0 ? o.pos - o.ctx - j : j >= o.own ? 0 : __popcll(f.bits >> x >> 1) + f.rest);
-}
+__device__ __forceinline__ float tree_distance(const TreeFar &f, int x) { return (float)(__popc(f.ones >> x >> 1) + f.rest); }
 
-template <bool TREE> __device__ __forceinline__ void att_limits(const AttArgs &A, bool shared, const AttSeq &q, AttRow &o) {
+template <bool TREE> __device__ __forceinline__ void att_limits(const AttArgs &A, bool shared, const AttSeq &q, AttRow &o, int len) {
     const mmoe_attn_args &a = A.a;
-    int len = a.len[q.s];
     o.pos = len - (q.t1 - o.tok);
     if (o.tok - q.t0 >= a.max_q) o.live = false;
     o.lo = a.lo ? max(a.lo[o.tok], 0) : 0;
@@ -654,27 +658,47 @@ template <int T> __device__ __forceinline__ uint32_t only_finite(uint32_t v) {
 // 8192 cubed reaches 1.28; the clock falls to 1.5 GHz); with a cap 530 to 553 (three more instructions and two of the transcendental unit per
 // score), with a distance bias 510 to 533. Short runs: 2.5 us to the first tile (sequence, limits, block ids, tile: loads that depend on each
 // other), 1.7 us per tile of a wave alone on its SIMD.
-template <int D> struct AttTileMem {
-    __attribute__((aligned(1024))) uint8_t first[2 * ATT_BN(D) * D * 2];   // keys and values of a tile
+template <int D, int BN = ATT_BN(D)> struct AttTileMem {
+    __attribute__((aligned(1024))) uint8_t first[2 * BN * D * 2];   // keys and values of a tile
     union {
-        __attribute__((aligned(1024))) uint8_t second[2 * ATT_BN(D) * D * 2];
+        __attribute__((aligned(1024))) uint8_t second[2 * BN * D * 2];
         int starts[MMOE_KV_MAXSEQ + 1];
     };
     int range[4][4], flag[2][4];
 };
+// A kernel's arguments, its first parameter, read from where the launch put them whenever this is asked for
+__device__ __forceinline__ const AttArgs &tree_args() {
+    auto p = (const __attribute__((address_space(4))) AttArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const AttArgs *)p;
+}
+// Which work: with TREE a piece that the caller has found (drafts.h), else the launch's block
+struct AttWork {
+    bool shared;
+    unsigned block;
+    AttTileAt at;      // TREE from here on: the row tile and its sequence's new tokens' end and length, its positions, where its result goes (whole: to
+    int t1, len;       // out, else to partial results `slot`)
+    int kvh, p0, p1;
+    bool whole;
+    int64_t slot;
+};
 template <int T, int D, bool CAP, bool BIAS, bool TREE>
-__device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, const unsigned block, AttTileMem<D> &M) {
+__device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, AttTileMem<D, TREE ? TREE_BN : ATT_BN(D)> &M) {
     constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // a row's bytes and chunks; rows of a load, loads of 16 rows
-    constexpr int BN = ATT_BN(D), GW = BN / 64, NU = BN / 32, NK = BN / 16;   // groups of 16 positions that a wave loads; score blocks, steps of the second product
+    constexpr int BN = TREE ? TREE_BN : ATT_BN(D), GW = BN / 64, NU = BN / 32, NK = BN / 16;   // groups of 16 positions that a wave loads; score blocks, steps of the second product
     constexpr uint32_t TB = BN * RB;
     const mmoe_attn_args &a = A.a;
-    const int nsplit = shared ? A.split_sh : A.split;
+    const bool shared = work.shared;
+    const int nsplit = TREE ? 1 : shared ? A.split_sh : A.split;
     const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 31, hh = l >> 5;
-    const unsigned rest = A.by_kv(block), v = (shared ? A.by_split_sh : A.by_split)(rest);
-    const int kvh = block - rest * A.kv.heads, split = rest - v * nsplit;
-    AttTileAt at;
-    // a sequence's last tiles see most: first (the sequences in reverse order, whatever their lengths)
-    if (!att_find(A, shared, ATT_BM, (shared ? A.tiles_sh : A.tiles) - 1 - (int)v, at)) return;
+    AttTileAt at = work.at;
+    int kvh = work.kvh, split = 0;
+    if (!TREE) {
+        const unsigned rest = A.by_kv(work.block), v = (shared ? A.by_split_sh : A.by_split)(rest);
+        kvh = work.block - rest * A.kv.heads; split = rest - v * nsplit;
+        // a sequence's last tiles see most: first (the sequences in reverse order, whatever their lengths)
+        if (!att_find(A, shared, ATT_BM, (shared ? A.tiles_sh : A.tiles) - 1 - (int)v, at)) return;
+    }
 
     // What the lane loads of a tile: row RPI i + l / CH of the wave's 16, piece l % CH of LDS, less the instruction's own offset (rows are at
     // least head_dim values apart, so it stays positive).
@@ -713,27 +737,47 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
             load_lds<NI>(from, off, buf + r * RB);
         }
     };
+    auto fetch_tile = [&](uint32_t buf, int p, const auto &blk) {
+        fetch(buf, A.kv.k, ko, p, blk);
+        fetch(buf + TB, A.kv.v, vo, p, blk);
+    };
     const uint32_t lds = (uint32_t)(uintptr_t)(lb *)M.first;   // tile i: keys at lds + 2 TB (i % 2), values TB behind them
     unsigned bad = 0, next = 0;   // the tile's lost blocks, the next one's
     int p0, p1;
     decltype(block_of(0, bad)) blk;
-    if (shared) {   // which positions is known already: the first tile comes while the rows look for their sequences
+    AttRow R = att_row(A, at, at.row0 + w * 32 + n, kvh);
+    // queries: operand B, lane (hh, n) holds dims 16 s + 8 hh .. + 8 of row n
+    u4 q[KS];
+    auto queries = [&] {
+        const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * hh;
+#pragma unroll
+        for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 16 * s);
+    };
+    if (TREE) { p0 = work.p0; p1 = work.p1; }
+    if (TREE && !shared) {
+        // which sequence is known already, so its rows' limits and queries are on their way before the first tile is: a wait for them later would
+        // be one for the tile, too
+        if (p0 < p1) blk = block_of(p0, bad);
+        att_limits<TREE>(A, false, {at.s, at.t0, work.t1}, R, work.len);
+        queries();
+        if (p0 < p1) fetch_tile(lds, p0, blk);
+    } else if (TREE) {
+        if (p0 < p1) {
+            blk = block_of(p0, bad);
+            fetch_tile(lds, p0, blk);
+        }
+    } else if (shared) {   // which positions is known already: the first tile comes while the rows look for their sequences
         const int run = ((a.shared + BN - 1) / BN + nsplit - 1) / nsplit * BN;
         p0 = split * run; p1 = min(p0 + run, a.shared);
         if (p0 < p1) {
             blk = block_of(p0, bad);
-            fetch(lds, A.kv.k, ko, p0, blk);
-            fetch(lds + TB, A.kv.v, vo, p0, blk);
+            fetch_tile(lds, p0, blk);
         }
     }
-    AttRow R = att_row(A, at, at.row0 + w * 32 + n, kvh);
-    att_limits<TREE>(A, shared, att_seq(A, shared, at, M.starts, R), R);
-    // queries: operand B, lane (hh, n) holds dims 16 s + 8 hh .. + 8 of row n
-    u4 q[KS];
-    {
-        const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * hh;
-#pragma unroll
-        for (int s = 0; s < KS; s++) q[s] = *(const gu4 *)(qp + 16 * s);
+    if (!TREE || shared) {
+        const AttSeq of = att_seq(A, shared, at, M.starts, R);
+        att_limits<TREE>(A, shared, of, R, a.len[of.s]);
+        queries();
     }
     // A score is sc s1 + s0 in units of log 2, in which sc is the product's with the bias in its units, or with a cap 1 / (1 + exp 2 z):
     // what is left of them is in the exponentials' own multiplication.
@@ -754,7 +798,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     const int seen = __builtin_amdgcn_readfirstlane(lo);   // the first position that any row sees
     lo = seen & ~(BN - 1); hi = __builtin_amdgcn_readfirstlane(hi);
     glo = __builtin_amdgcn_readfirstlane(glo); ghi = __builtin_amdgcn_readfirstlane(ghi);
-    if (shared) {
+    if (TREE || shared) {
         p1 = lo < hi ? min(p1, hi) : p0;   // (the first tile is there, also where it lies before lo: nobody looks)
         if (p0 >= p1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // and is not left on its way into LDS that is another's
     } else {
@@ -766,8 +810,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         }
         if (p0 < p1) {
             blk = block_of(p0, bad);
-            fetch(lds, A.kv.k, ko, p0, blk);
-            fetch(lds + TB, A.kv.v, vo, p0, blk);
+            fetch_tile(lds, p0, blk);
         }
     }
     // where it reads them back: K row n (and n + 32), pieces 2 k + hh; V rows vr (and on by eights), dims 32 i + 16 (l / 16 % 2) + 4 (l % 4) ..
@@ -812,7 +855,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                 float x = s[u][j];
                 if (CAP) x = __builtin_amdgcn_rcpf(1.0f + exp2_(x * A.s1));   // tanh z = 1 - 2 / (1 + exp 2 z)
                 if (CAP && BIAS) x = fmaf(-2.0f * A.s2, x, A.s2);
-                if (BIAS) x = fmaf(-slope, path ? tree_distance(R, far, at) : fabsf(dist - (float)(32 * u + at)), x);
+                if (BIAS) x = fmaf(-slope, path ? tree_distance(far, at) : fabsf(dist - (float)(32 * u + at)), x);
                 s[u][j] = x;
             }
         }
@@ -822,7 +865,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         if (TREE) {
 #pragma unroll
             for (int u = 0; u < NU; u++) {
-                const uint32_t v = (uint32_t)tree_sees(A, R, p + 32 * u + 4 * hh);
+                const uint32_t v = tree_sees(A, R, p + 32 * u + 4 * hh);
 #pragma unroll
                 for (int j = 0; j < 16; j++) s[u][j] = (v >> (8 * (j >> 2) + (j & 3))) & 1 ? s[u][j] : NONE;
             }
@@ -911,7 +954,8 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         const int bits = (__any((o & 0x80008000u) != 0) ? 1 : 0) | (__any((see & 0x80008000u) != 0) ? 2 : 0);
         if (l == 0) M.flag[f][w] = bits;
     };
-    auto found = [&](int f) { return __builtin_amdgcn_readfirstlane(M.flag[f][0] | M.flag[f][1] | M.flag[f][2] | M.flag[f][3]); };
+    auto any_wave = [&](const int *f) { return __builtin_amdgcn_readfirstlane(f[0] | f[1] | f[2] | f[3]); };
+    auto found = [&](int f) { return any_wave(M.flag[f]); };
     auto zero_odd = [&](uint32_t buf) {
 #pragma unroll
         for (int x = 0; x < GW * NI; x++) {
@@ -961,8 +1005,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
             __syncthreads();   // the tile has arrived, and every wave is done with the other buffers
             if (p + BN < p1) {
                 blk = block_of(p + BN, next);
-                fetch(kother, A.kv.k, ko, p + BN, blk);
-                fetch(kother + TB, A.kv.v, vo, p + BN, blk);
+                fetch_tile(kother, p + BN, blk);
             }
             const int odd = part ? found(i) : 0;
             if (odd) {
@@ -998,11 +1041,10 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
         wild = __any(!(top < __builtin_inff()));
         if (l == 0) M.range[0][w] = lost;
         __syncthreads();
-        if (!__builtin_amdgcn_readfirstlane(M.range[0][0] | M.range[0][1] | M.range[0][2] | M.range[0][3])) break;
+        if (!any_wave(M.range[0])) break;
         idp = INT32_MIN / 2;
         blk = block_of(p0, bad);
-        fetch(lds, A.kv.k, ko, p0, blk);
-        fetch(lds + TB, A.kv.v, vo, p0, blk);
+        fetch_tile(lds, p0, blk);
     }
     if (odd0 < odd1) {
         wild = true;
@@ -1019,9 +1061,10 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
     }
     sum = add_halves(sum);
     if (!R.live) return;
+    const AttArgs &E = TREE ? tree_args() : A;   // (read again: there are not registers enough to keep what only the end needs)
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    if (nsplit == 1 && !A.parts_sh) {
-        uint16_t *o = (uint16_t *)a.out + (int64_t)R.tok * a.out_token + R.head * a.out_head + 4 * hh;
+    if (TREE ? work.whole : nsplit == 1 && !E.parts_sh) {
+        uint16_t *o = (uint16_t *)E.a.out + (int64_t)R.tok * E.a.out_token + R.head * E.a.out_head + 4 * hh;
 #pragma unroll
         for (int i = 0; i < DS; i++)
 #pragma unroll
@@ -1030,13 +1073,23 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const bool shared, co
                 if (sum == 0.0f) v = make_uint2(0, 0);
                 *(uint2 *)(o + 32 * i + 2 * j) = v;
             }
-        if (a.lse && hh == 0) a.lse[(int64_t)R.tok * a.heads + R.head] = sum == 0.0f ? -__builtin_inff() : (mb + __builtin_amdgcn_logf(sum)) * ATT_LN2;
+        if (E.a.lse && hh == 0) E.a.lse[(int64_t)R.tok * E.a.heads + R.head] = sum == 0.0f ? -__builtin_inff() : (mb + __builtin_amdgcn_logf(sum)) * ATT_LN2;
         return;
     }
-    const int64_t row = (shared ? 0 : A.at_tile) + ((int64_t)split * a.ntok + R.tok) * a.heads + R.head;
-    if (hh == 0) A.pm[row] = make_float2(mb, wild ? -sum : sum);
+    if (TREE) {   // as the registers hold it: [wave][16 dims][lane][4 of them]
+        const int64_t at = work.slot * E.slot_waves + w;
+        if (hh == 0) E.pm[at * 32 + n] = make_float2(mb, wild ? -sum : sum);
+        f4 *o = (f4 *)(E.po + at * 32 * D) + l;
+#pragma unroll
+        for (int i = 0; i < DS; i++)
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) o[(4 * i + j / 4) * 64] = f4{acc[i][j], acc[i][j + 1], acc[i][j + 2], acc[i][j + 3]};
+        return;
+    }
+    const int64_t row = (shared ? 0 : E.at_tile) + ((int64_t)split * E.a.ntok + R.tok) * E.a.heads + R.head;
+    if (hh == 0) E.pm[row] = make_float2(mb, wild ? -sum : sum);
     if (sum == 0.0f) return;
-    float *o = A.po + row * D + 4 * hh;
+    float *o = E.po + row * D + 4 * hh;
 #pragma unroll
     for (int i = 0; i < DS; i++)
 #pragma unroll
@@ -1064,7 +1117,7 @@ template <int D> struct AttFewMem {
     };
     float2 stat[4][16];
 };
-template <int T, int D, bool CAP, bool BIAS, bool TREE>
+template <int T, int D, bool CAP, bool BIAS>
 __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, const unsigned block, AttFewMem<D> &M) {
     constexpr int KS = D / 32, E = D / 16;   // products over the dims, values of a row per lane
     const mmoe_attn_args &a = A.a;
@@ -1136,7 +1189,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     if (early) { id = ids(p); next = ids(p + 128); }
     const AttSeq sq = att_seq(A, shared, at, M.starts, R);
     if (early && p < end) { load_k(p, id); load_v(p, id); }
-    att_limits<TREE>(A, shared, sq, R);
+    att_limits<false>(A, shared, sq, R, a.len[sq.s]);
     u4 q[KS];
     {
         const uint16_t *qp = (const uint16_t *)a.q + (int64_t)R.tok * a.q_token + R.head * a.q_head + 8 * g;
@@ -1148,7 +1201,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
     const int seen = wave_min(some ? R.lo : INT32_MAX);   // the first position that any row sees
     int p0 = max(from, seen & ~31), p1 = min(end, wave_max(some ? R.hi : 0));
     if (p0 >= p1) p0 = p1 = 0;   // nothing seen (p0 may be close to the largest int: no wave's first run is counted from it)
-    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.full : INT32_MAX);
+    const int inlo = wave_max(R.live ? R.lo : 0), inhi = wave_min(R.live ? R.hi : INT32_MAX);
     f4 acc[E];
 #pragma unroll
     for (int e = 0; e < E; e++) acc[e] = f4{0, 0, 0, 0};
@@ -1181,21 +1234,17 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
         }
         after_scores();
         const float dist = BIAS ? (float)(R.pos - p - 4 * g) : 0.0f;
-        const bool part = p < inlo || p + 32 > inhi || r.bad, path = TREE && BIAS && p + 32 > inhi;   // (drafted tokens among the run's)
+        const bool part = p < inlo || p + 32 > inhi || r.bad;
         float mt = -__builtin_inff();
-        TreeFar far;
-        if (path) far = tree_far(A, R, p + 4 * g);
-        uint32_t sees = 0;
-        if (TREE && part) sees = (uint32_t)tree_sees(A, R, p + 4 * g);
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 float x = s[u][j] * A.s1;
                 if (CAP) x = fmaf(-2.0f * A.s2, __builtin_amdgcn_rcpf(1.0f + exp2_(x)), A.s2);
-                if (BIAS) x = fmaf(-slope, path ? tree_distance(R, far, 16 * u + j) : fabsf(dist - (float)(16 * u + j)), x);
+                if (BIAS) x = fmaf(-slope, fabsf(dist - (float)(16 * u + j)), x);
                 int at = p + 16 * u + 4 * g + j;
-                if (part) x = (TREE ? (bool)((sees >> (16 * u + j)) & 1) : at >= R.lo && at < R.hi) && !((r.bad >> u) & 1) ? x : -__builtin_inff();
+                if (part) x = at >= R.lo && at < R.hi && !((r.bad >> u) & 1) ? x : -__builtin_inff();
                 s[u][j] = x;
                 mt = fmaxf(mt, x);
             }
@@ -1279,7 +1328,7 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
             __builtin_amdgcn_wave_barrier();   // a wave's LDS operations stay in order
 #pragma unroll 1
             for (int k = 0; k < 32; k++) {
-                const bool see = (TREE ? (bool)(tree_sees(A, R, p + k) & 1) : p + k >= R.lo && p + k < R.hi) && !((r.bad >> (k >> 4)) & 1);
+                const bool see = p + k >= R.lo && p + k < R.hi && !((r.bad >> (k >> 4)) & 1);
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -1351,20 +1400,20 @@ __device__ __forceinline__ void att_few(const AttArgs &A, const bool shared, con
 }
 
 // One launch for everything, the long work first. With no row tiles of 128 in it a kernel of its own: fewer registers, more waves.
-template <int T, int D, bool CAP, bool BIAS, bool TREE>
+template <int T, int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(256, 2) k_attn_few(AttArgs A) {
     __shared__ AttFewMem<D> M;
     const unsigned b = blockIdx.x;
     const bool shared = b < A.n_sh;
-    att_few<T, D, CAP, BIAS, TREE>(A, shared, shared ? b : b - A.n_sh, M);
+    att_few<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh, M);
 }
-template <int T, int D, bool CAP, bool BIAS, bool TREE>
+template <int T, int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
     __shared__ union { AttTileMem<D> tile; AttFewMem<D> few; } M;
     const unsigned b = blockIdx.x;
     const bool shared = b < A.n_sh;
-    if (shared ? !A.sh_few : b < A.n_sh + A.n_tile) att_tile<T, D, CAP, BIAS, TREE>(A, shared, shared ? b : b - A.n_sh, M.tile);
-    else att_few<T, D, CAP, BIAS, TREE>(A, shared, shared ? b : b - A.n_sh - A.n_tile, M.few);
+    if (shared ? !A.sh_few : b < A.n_sh + A.n_tile) att_tile<T, D, CAP, BIAS, false>(A, {shared, shared ? b : b - A.n_sh}, M.tile);
+    else att_few<T, D, CAP, BIAS>(A, shared, shared ? b : b - A.n_sh - A.n_tile, M.few);
 }
 
 // The partial results of a row: their maxima and sums give each a weight. D / 4 lanes read a part; with all, every such group of the
@@ -1374,7 +1423,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tile(AttArgs A) {
 #define ATT_PARTS 1024     // most partial results of a row
 #define ATT_PER 16
 template <int T, int D>
-static __global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_only) {
+__global__ void __launch_bounds__(1024) k_attn_join(AttArgs A, int all, int few_only) {
     constexpr int LPR = D / 4;
     const mmoe_attn_args &a = A.a;
     __shared__ float red[2][16], wt[ATT_PARTS];

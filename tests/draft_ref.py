@@ -180,7 +180,11 @@ class TreeBatch(Batch):
     def upload(self, d):
         a = super().upload(d)
         self.p_bits = d.put(self.bits)
-        assert d.lib.mmoe_attn_tree_ws(a, self.cache, self.p_bits, self.words) == a.ws_bytes
+        self.plain_ws = a.ws, a.ws_bytes
+        size = d.lib.mmoe_attn_tree_ws(a, self.cache, self.p_bits, self.words)
+        assert size, d.lib.mmoe_last_error()
+        a.ws, a.ws_bytes = d.room(size + 256), size
+        d.write(a.ws + size, self.ws_guard)
         return a
 
     def run(self, d, note=""):

@@ -35,7 +35,7 @@ def test_tree_plan_refusals(kw, word):
     (dict(hi=P), {}, P, 1, b"hi"), ({}, {}, P, 0, b"words"), ({}, {}, P, 9, b"words"), (dict(max_q=65), {}, P, 1, b"max_q"), (dict(max_q=513), {}, P, 8, b"max_q"),
     ({}, {}, None, 1, b"pointer"), ({}, {}, P + 4, 1, b"aligned"), ({}, dict(head_dim=96), P, 1, b"head_dim"), ({}, dict(dtype=M.F32), P, 1, b"type"),
     (dict(heads=18), {}, P, 1, b"heads"), (dict(shared=8), {}, P, 1, b"shared"), (dict(window=-1), {}, P, 1, b"window"), (dict(cap=2000.0), {}, P, 1, b"cap"),
-    (dict(scale=float("nan")), {}, P, 1, b"scale"), (dict(q=None), {}, P, 1, b"pointer"), (dict(q=P + 8), {}, P, 1, b"aligned"), (dict(ws_bytes=10), {}, P, 1, b"workspace"),
+    (dict(scale=float("nan")), {}, P, 1, b"scale"), (dict(nseq=4096, ntok=1 << 18, max_q=512, width=1 << 22, max_len=1 << 26, heads=16), dict(heads=1), P, 8, b"too many"), (dict(q=None), {}, P, 1, b"pointer"), (dict(q=P + 8), {}, P, 1, b"aligned"), (dict(ws_bytes=10), {}, P, 1, b"workspace"),
     (dict(ws=P + 16), {}, P, 1, b"workspace"), (dict(max_len=129), {}, P, 1, b"max_len"), (dict(q_head=4), {}, P, 1, b"strides")])
 def test_attn_tree_refusals(kw, ckw, bits, words, word):
     refused(M.lib().mmoe_attn_tree(attn(**kw), cache(**ckw), bits, words), word)
@@ -44,7 +44,9 @@ def test_attn_tree_refusals(kw, ckw, bits, words, word):
 
 def test_attn_tree_workspace():
     lib = M.lib()
-    assert lib.mmoe_attn_tree_ws(attn(), cache(), P, 1) == lib.mmoe_attn_paged_ws(attn(), cache()) > 0
+    assert lib.mmoe_attn_tree_ws(attn(), cache(), P, 1) > 0
+    # it follows the tokens and the sequences, not the bound of their lengths
+    assert lib.mmoe_attn_tree_ws(attn(max_len=128), cache(), P, 1) == lib.mmoe_attn_tree_ws(attn(max_len=0), cache(), P, 1)
     assert lib.mmoe_attn_tree_ws(attn(hi=P), cache(), P, 1) == 0 and lib.mmoe_attn_tree_ws(attn(), cache(), P, 0) == 0
     assert lib.mmoe_attn_tree(None, cache(), P, 1) == -1 and lib.mmoe_attn_tree(attn(), None, P, 1) == -1
     assert lib.mmoe_attn_tree(attn(ntok=0), cache(), P, 1) == 0 and lib.mmoe_attn_tree(attn(nseq=0), cache(), P, 1) == 0

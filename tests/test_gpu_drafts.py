@@ -149,16 +149,18 @@ def test_limits_of_documents_bounds_and_lost_blocks():
 
 
 def test_a_chain_is_plain_attention():
-    """a draft without branches sees what mmoe_attn_paged's causal tokens see: the same bits come out"""
+    """a draft without branches sees what mmoe_attn_paged's causal tokens see"""
     rng = np.random.default_rng(9)
     for sizes, ctx, kw in (([3, 4], [100, 900], dict(heads=4, kv=1)), ([30, 64, 7], [700, 64, 2000], dict(heads=8, kv=2, kind="bf16")), ([64, 20], [300, 260], dict(heads=4, kv=4, dim=64, shared=256, alibi=True))):
         b = TreeBatch(rng, drafts(rng, sizes, 1), lens=[c + n for c, n in zip(ctx, sizes)], **kw)
         with Dev() as d:
-            a = b.upload(d)
+            b.run(d, "as a tree")
+            d.write(b.p_out, b.out0); d.write(b.p_lse, b.lse0)
+            a = b.args
+            (a.ws, a.ws_bytes), tree_ws = b.plain_ws, (a.ws, a.ws_bytes)
             M.check(d.lib.mmoe_attn_paged(a, b.cache), "plain")
-            plain = d.get(b.p_out, b.out0), d.get(b.p_lse, b.lse0)
-            M.check(d.lib.mmoe_attn_tree(a, b.cache, b.p_bits, b.words), "tree")
-            assert np.array_equal(plain[0], d.get(b.p_out, b.out0)) and np.array_equal(plain[1], d.get(b.p_lse, b.lse0))
+            b.check(d, "plain")
+            a.ws, a.ws_bytes = tree_ws
 
 
 def test_drafts_of_many_sequences():
