@@ -13,31 +13,38 @@ __device__ __forceinline__ NewTokens new_tokens(const int32_t *qstart, int s, in
 // ------------------------------------------------------------------------------------------------------
 // What drafted tokens follow (mmoe_tree_plan)
 // ------------------------------------------------------------------------------------------------------
-// A workgroup per sequence, a thread per node. By steps that double: what a node's 2^i-th ancestor follows, it follows, so nine rounds through
-// LDS settle the deepest tree of 512, and as many as the depth's logarithm any other.
+// A workgroup per sequence, a wave per word of 64 nodes, a lane per node. Within a word by steps that double (what a node's 2^i-th ancestor
+// follows, it follows), through the lanes: six steps at most, which leave each node the ancestors of its own word and the node of an earlier word
+// that the last of them follows, if any. Then word by word: that node's bits are whole by then.
 template <int W>
 __global__ void __launch_bounds__(64 * W) k_tree_plan(mmoe_tree_plan_args a) {
     __shared__ uint64_t sees[W][64 * W];
-    __shared__ int up[64 * W];
-    const int s = blockIdx.x, i = threadIdx.x;
+    const int s = blockIdx.x, i = threadIdx.x, l = i & 63, wave = __builtin_amdgcn_readfirstlane(i >> 6);
     const NewTokens q = a.nseq ? new_tokens(a.qstart, s, a.ntok) : NewTokens{0, 0};
     const int n = min(q.n, 64 * a.words), ctx = a.nseq ? a.len[s] - q.n : 0;
-    int to = -1;
-    if (i < n) to = a.parent[q.t0 + i];
-    if (to >= i) to = -1;
-    uint64_t b[W];
+    int out = -1;   // the node of an earlier word
+    if (i < n) out = a.parent[q.t0 + i];
+    if (out >= i) out = -1;
+    int to = out - 64 * wave;   // in the word: its lane
+    uint64_t own = 1ull << l;
+    while (__any(to >= 0)) {
+        const int from = max(to, 0);
+        const uint64_t more = (uint64_t)(uint32_t)__shfl((int)(own >> 32), from, 64) << 32 | (uint32_t)__shfl((int)own, from, 64);
+        const int next = __shfl(to, from, 64), past = __shfl(out, from, 64);
+        if (to >= 0) { own |= more; to = next; out = past; }
+    }
+    uint64_t b[W] = {};
 #pragma unroll
-    for (int w = 0; w < W; w++) b[w] = w == i >> 6 ? 1ull << (i & 63) : 0;
-    while (__syncthreads_or(to >= 0)) {
+    for (int v = 0; v < W; v++) {
+        if (W > 1 && v) __syncthreads();
+        if (wave != v) continue;
+        if (out >= 0)
 #pragma unroll
-        for (int w = 0; w < W; w++) sees[w][i] = b[w];
-        up[i] = to;
-        __syncthreads();
-        if (to >= 0) {
+            for (int w = 0; w < v; w++) b[w] = w <= out >> 6 ? sees[w][out] : 0;
+        b[v] = own;
+        if (v + 1 < W)
 #pragma unroll
-            for (int w = 0; w < W; w++) b[w] |= sees[w][to];
-            to = up[to];
-        }
+            for (int w = 0; w <= v; w++) sees[w][i] = b[w];
     }
     int depth = -1;
 #pragma unroll
@@ -102,41 +109,58 @@ __device__ __forceinline__ int64_t page_at(const PageArgs &P, int block, int at,
 }
 
 // Kept positions moved together. Entry j goes from k[j] to k[0] + j <= k[j], so that writing it touches the source of no later one: a
-// workgroup goes through the list in steps of as many entries as its threads hold, all read before any is written.
-#define KC_T 256
+// workgroup goes through the list in steps of as many entries as its threads hold, all of a step read before any is written; positions and blocks of the
+// next step are looked up while this one's values are on their way. A workgroup has `lanes` pieces of every position (of one array), so the
+// arrays and the pieces are what runs side by side.
 #define KC_U 8
-__global__ void __launch_bounds__(KC_T) k_kv_compact(mmoe_kv_compact_args a, PageArgs P, int lanes, int units, Div by_lanes, Div by_units, Div by_arrays, int arrays) {
-    const unsigned rest = by_units(blockIdx.x), s = by_arrays(rest);
-    const int unit = blockIdx.x - rest * units, array = rest - s * arrays;
+template <int TH>
+__global__ void __launch_bounds__(TH) k_kv_compact(mmoe_kv_compact_args a, PageArgs P, int lanes, int units, Div by_lanes, Div by_units, Div by_arrays, int arrays) {
+    // the arrays first: a position's pieces then lie on one die wherever the number of arrays is a multiple of the dies'
+    const unsigned rest = by_arrays(blockIdx.x), s = by_units(rest);
+    const int array = blockIdx.x - rest * arrays, unit = rest - s * units;
     const int first = a.first[s], n = a.count[s];
     if (first < 0 || first >= a.nkept || n < 2) return;
-    const int count = min(n, a.nkept - first), per = (int)by_lanes(KC_T), e = (int)by_lanes(threadIdx.x);
-    const int piece = unit * lanes + threadIdx.x - e * lanes;
+    const int count = min(n, a.nkept - first), per = (int)by_lanes(TH), e = (int)by_lanes(threadIdx.x);
+    const int piece = unit * lanes + threadIdx.x - e * lanes, bs1 = P.kv.block_size - 1;
     const bool on = e < per && piece < P.all;
     const int32_t *k = a.kept + first, *table = a.table + (int64_t)s * a.width;
     const int to0 = k[0];
     uint8_t *base = (uint8_t *)P.base[array];
     auto block = [&](int64_t p) { return p < 0 || (p >> P.sh) >= a.width ? -1 : table[p >> P.sh]; };
-    for (int j0 = 1; j0 < count; j0 += per * KC_U) {
-        u4 x[KC_U];
-        int64_t to[KC_U];
+    struct Step { int from[KC_U], b0[KC_U], b1[KC_U]; };
+    auto positions = [&](Step &x, int j0) {
 #pragma unroll
         for (int u = 0; u < KC_U; u++) {
             const int j = j0 + u * per + e;
-            to[u] = -1;
-            if (!on || j >= count) continue;
-            const int from = k[j];
-            const int64_t t = (int64_t)to0 + j;
-            if (from <= t) continue;
-            const int b0 = block(from), b1 = block(t);
-            if ((unsigned)b0 >= (unsigned)P.kv.nblocks || (unsigned)b1 >= (unsigned)P.kv.nblocks) continue;
-            x[u] = *(const gu4 *)(base + page_at(P, b0, from & (P.kv.block_size - 1), piece));
-            to[u] = page_at(P, b1, (int)t & (P.kv.block_size - 1), piece);
+            x.from[u] = on && j < count ? k[j] : -1;
         }
+    };
+    auto blocks = [&](Step &x, int j0) {
+#pragma unroll
+        for (int u = 0; u < KC_U; u++) {
+            const int64_t t = (int64_t)to0 + j0 + u * per + e;
+            const bool moves = x.from[u] > t;
+            x.b0[u] = moves ? block(x.from[u]) : -1;
+            x.b1[u] = moves ? block(t) : -1;
+        }
+    };
+    Step now, then;
+    positions(now, 1);
+    blocks(now, 1);
+    for (int j0 = 1; j0 < count; j0 += per * KC_U) {
+        const int j1 = j0 + per * KC_U;
+        u4 x[KC_U];
+#pragma unroll
+        for (int u = 0; u < KC_U; u++) {
+            if ((unsigned)now.b0[u] >= (unsigned)P.kv.nblocks || (unsigned)now.b1[u] >= (unsigned)P.kv.nblocks) { now.b1[u] = -1; continue; }
+            x[u] = *(const gu4 *)(base + page_at(P, now.b0[u], now.from[u] & bs1, piece));
+        }
+        if (j1 < count) { positions(then, j1); blocks(then, j1); }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // every wave's values are there before any is written over
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < KC_U; u++) if (to[u] >= 0) *(gu4 *)(base + to[u]) = x[u];
+        for (int u = 0; u < KC_U; u++) if (now.b1[u] >= 0) *(gu4 *)(base + page_at(P, now.b1[u], (to0 + j0 + u * per + e) & bs1, piece)) = x[u];
+        now = then;
     }
 }
 
@@ -168,19 +192,18 @@ __global__ void __launch_bounds__(KY_T) k_kv_copy(mmoe_kv_copy_args a, PageArgs 
 // ------------------------------------------------------------------------------------------------------
 // One workgroup settles which forks are made and which blocks they take (a prefix sum over them); the rows, which are independent, follow in the
 // same launch or in one of their own.
-__device__ __forceinline__ void fork_row(const mmoe_kv_fork_args &a, int sh, int src, int dst, int n, int lane, int lanes) {
-    const int keep = a.shared >> sh, cols = n <= a.shared ? (n + a.block_size - 1) >> sh : n >> sh;
-    for (int c = lane; c < cols; c += lanes) {
-        const int b = a.table[(int64_t)src * a.width + c];
-        a.table_out[(int64_t)dst * a.width + c] = b;
-        if (c >= keep && (unsigned)b < (unsigned)a.nblocks) atomicAdd(&a.holders[b], 1);
-    }
+// columns of a copy's row that are its source's
+__device__ __forceinline__ int fork_cols(const mmoe_kv_fork_args &a, int sh, int n) { return n <= a.shared ? (n + a.block_size - 1) >> sh : n >> sh; }
+__device__ __forceinline__ void fork_put(const mmoe_kv_fork_args &a, int sh, int dst, int c, int b) {
+    a.table_out[(int64_t)dst * a.width + c] = b;
+    if (c >= a.shared >> sh && (unsigned)b < (unsigned)a.nblocks) atomicAdd(&a.holders[b], 1);
 }
+#define KO_ONE 4096   // rows' entries that the one workgroup copies itself
 template <int PER>
-__global__ void __launch_bounds__(1024) k_kv_fork(mmoe_kv_fork_args a, int sh, int rows) {
+__global__ void __launch_bounds__(1024) k_kv_fork(mmoe_kv_fork_args a, int sh, int rows, Div by_width) {
     __shared__ int src_[PER * 1024], dst_[PER * 1024], len_[PER * 1024];
     __shared__ uint2 red[16];
-    const int tid = threadIdx.x, i0 = tid * PER, nt = blockDim.x;
+    const int tid = threadIdx.x, i0 = tid * PER;
     const int nfree = min(max(a.nfree[0], 0), a.nblocks);
     int src[PER], dst[PER], n[PER], begun[PER];
     unsigned need[PER], sum = 0, zero = 0, total, z;
@@ -218,12 +241,23 @@ __global__ void __launch_bounds__(1024) k_kv_fork(mmoe_kv_fork_args a, int sh, i
     }
     if (!rows) return;
     __syncthreads();
-    for (int i = tid >> 6; i < a.nfork; i += nt >> 6)
-        if (src_[i] >= 0) fork_row(a, sh, src_[i], dst_[i], len_[i], tid & 63, 64);
+    int b[KO_ONE / 1024], c[KO_ONE / 1024], to[KO_ONE / 1024];
+#pragma unroll
+    for (int u = 0; u < KO_ONE / 1024; u++) {   // every load under way at once
+        const int item = u * 1024 + tid, i = (int)by_width(item);
+        c[u] = item - i * a.width; to[u] = -1;
+        if (i >= a.nfork || src_[i] < 0 || c[u] >= fork_cols(a, sh, len_[i])) continue;
+        b[u] = a.table[(int64_t)src_[i] * a.width + c[u]];
+        to[u] = dst_[i];
+    }
+#pragma unroll
+    for (int u = 0; u < KO_ONE / 1024; u++) if (to[u] >= 0) fork_put(a, sh, to[u], c[u], b[u]);
 }
 __global__ void __launch_bounds__(256) k_kv_fork_rows(mmoe_kv_fork_args a, int sh) {
     const int src = a.src[blockIdx.x], dst = a.dst[blockIdx.x];
-    if ((unsigned)src < (unsigned)a.nseq && (unsigned)dst < (unsigned)a.nseq) fork_row(a, sh, src, dst, a.ctx_out[dst], threadIdx.x, 256);
+    if ((unsigned)src >= (unsigned)a.nseq || (unsigned)dst >= (unsigned)a.nseq) return;
+    const int cols = fork_cols(a, sh, a.ctx_out[dst]);
+    for (int c = threadIdx.x; c < cols; c += 256) fork_put(a, sh, dst, c, a.table[(int64_t)src * a.width + c]);
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -272,30 +306,46 @@ __global__ void __launch_bounds__(1024) k_kv_free(mmoe_kv_free_args a, int sh) {
         const int s = count_le(first, a.nseq, j) - 1;
         return a.table[(int64_t)s * a.width + col[s] + j - first[s]];
     };
+    // KF_U places a thread, one behind the other; those of the first round stay in registers
+    int b[KF_U];
+    auto round = [&](int j0) {
+#pragma unroll
+        for (int u = 0; u < KF_U; u++) {
+            const int j = j0 + tid * KF_U + u;
+            b[u] = j < n ? id(j) : -1;
+            if ((unsigned)b[u] >= (unsigned)a.nblocks) b[u] = -1;
+        }
+    };
+    const bool once = n <= nt * KF_U;
+    round(0);
     if (a.holders) {
-        for (int j = tid; j < n; j += nt) {
-            const int b = id(j);
-            if ((unsigned)b < (unsigned)a.nblocks) atomicSub(&a.holders[b], 1);
+        for (int j0 = 0; j0 < n; j0 += nt * KF_U) {
+            if (j0) round(j0);
+#pragma unroll
+            for (int u = 0; u < KF_U; u++) if (b[u] >= 0) atomicSub(&a.holders[b[u]], 1);
         }
         __threadfence();
         __syncthreads();
-        for (int j = tid; j < n; j += nt) {
-            const int b = id(j);
-            if ((unsigned)b < (unsigned)a.nblocks && __hip_atomic_load(&a.holders[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) < 0) atomicMin(&a.holders[b], -2 - j);
+        for (int j0 = 0; j0 < n; j0 += nt * KF_U) {
+            if (!once) round(j0);
+            int h[KF_U];
+#pragma unroll
+            for (int u = 0; u < KF_U; u++) h[u] = b[u] >= 0 ? __hip_atomic_load(&a.holders[b[u]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+#pragma unroll
+            for (int u = 0; u < KF_U; u++) if (h[u] < 0) atomicMin(&a.holders[b[u]], -2 - (j0 + tid * KF_U + u));
         }
         __threadfence();
         __syncthreads();
     }
     int at = nfree;
     for (int j0 = 0; j0 < n; j0 += nt * KF_U) {
-        int b[KF_U];
         unsigned mine = 0, none = 0, all, z2;
+        if (!once) round(j0);
 #pragma unroll
         for (int u = 0; u < KF_U; u++) {
             const int j = j0 + tid * KF_U + u;
-            b[u] = j < n ? id(j) : -1;
-            if ((unsigned)b[u] >= (unsigned)a.nblocks) b[u] = -1;
-            else if (a.holders && __hip_atomic_load(&a.holders[b[u]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != -2 - j) b[u] = -1;
+            if (b[u] < 0) continue;
+            if (a.holders && __hip_atomic_load(&a.holders[b[u]], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != -2 - j) b[u] = -1;
             mine += b[u] >= 0;
         }
         scan2(mine, none, &all, &z2, red);

@@ -162,15 +162,29 @@ int mmoe_kv_compact(const mmoe_kv_compact_args *p, const mmoe_kv_cache *kv, int 
     if (!a.nseq || !a.nkept) return 0;
     if (!a.table || !a.first || !a.count || !a.kept) REFUSE("mmoe_kv_compact: a pointer is missing");
     const PageArgs P = page_args(kv, layers);
-    int lanes = std::min(64, P.all);
-    while (lanes > 8 && (int64_t)a.nseq * 2 * layers * ((P.all + lanes - 1) / lanes) < 768) lanes = (lanes + 1) / 2;
-    const int units = (P.all + lanes - 1) / lanes;
-    const int64_t wgs = (int64_t)a.nseq * 2 * layers * units;
-    if (wgs * KC_T > (int64_t)MAX_THREADS) REFUSE("mmoe_kv_compact: %d sequences, %d layers, %d heads: too many for a launch", a.nseq, layers, kv->heads);
+    // Short lists (a step's accepted tokens): a wave goes through one. Else workgroups of 256 with as many pieces of a position, at least 128 bytes, as
+    // leave 768 of them (4 sequences of 5000, 24 layers, 0.4 kept: 164 us, of 1024 threads 168); where there are not so many, of 1024 threads, from 160 on
+    // (one sequence of 20000: 171 us, of 256 threads 194, with pieces of 64 bytes 207)
+    const int64_t arrays = 2 * layers, lists = a.nseq * arrays;
+    auto units_of = [&](int lanes) { return (P.all + lanes - 1) / lanes; };
+    auto pieces_for = [&](int wgs) {
+        int lanes = std::min(64, P.all);
+        while (lanes > 8 && lists * units_of(lanes) < wgs) lanes = (lanes + 1) / 2;
+        return lanes;
+    };
+    int threads = 64, lanes = std::min(64, P.all);
+    if (a.nkept / a.nseq > 64) {
+        threads = 256; lanes = pieces_for(768);
+        if (lists * units_of(lanes) < 768) { threads = 1024; lanes = pieces_for(160); }
+    }
+    const int units = units_of(lanes);
+    const int64_t wgs = lists * units;
+    if (wgs * threads > (int64_t)MAX_THREADS) REFUSE("mmoe_kv_compact: %d sequences, %d layers, %d heads: too many for a launch", a.nseq, layers, kv->heads);
     if (mm_ready()) return -1;
     OnDevice dev;
     if (!dev.ok) return -1;
-    return run(MMOE_K_KV_PAGES, k_kv_compact, (unsigned)wgs, KC_T, a, P, lanes, units, divisor(lanes), divisor(units), divisor(2 * layers), 2 * layers);
+    auto go = [&](auto kernel) { return run(MMOE_K_KV_PAGES, kernel, (unsigned)wgs, threads, a, P, lanes, units, divisor(lanes), divisor(units), divisor((uint32_t)arrays), (int)arrays); };
+    return threads == 64 ? go(k_kv_compact<64>) : threads == 256 ? go(k_kv_compact<256>) : go(k_kv_compact<1024>);
 }
 
 int mmoe_kv_copy(const mmoe_kv_copy_args *p, const mmoe_kv_cache *kv, int layers) {
@@ -201,8 +215,8 @@ int mmoe_kv_fork(const mmoe_kv_fork_args *p) {
     OnDevice dev;
     if (!dev.ok) return -1;
     const int sh = log2_block(a.block_size);
-    const bool one = (int64_t)a.nfork * a.width <= 4096;
-    if (a.nfork <= 1024 ? run(MMOE_K_KV_PAGES, k_kv_fork<1>, 1, 1024, a, sh, one) : run(MMOE_K_KV_PAGES, k_kv_fork<4>, 1, 1024, a, sh, one)) return -1;
+    const bool one = (int64_t)a.nfork * a.width <= KO_ONE;
+    if (a.nfork <= 1024 ? run(MMOE_K_KV_PAGES, k_kv_fork<1>, 1, 1024, a, sh, one, divisor(a.width)) : run(MMOE_K_KV_PAGES, k_kv_fork<4>, 1, 1024, a, sh, one, divisor(a.width))) return -1;
     return one || !a.nseq ? 0 : run(MMOE_K_KV_PAGES, k_kv_fork_rows, a.nfork, 256, a, sh);
 }
 
@@ -215,7 +229,7 @@ int mmoe_kv_free(const mmoe_kv_free_args *p) {
     OnDevice dev;
     if (!dev.ok) return -1;
     const int sh = log2_block(a.block_size);
-    return a.nseq <= 1024 ? run(MMOE_K_KV_PAGES, k_kv_free<1>, 1, 1024, a, sh) : run(MMOE_K_KV_PAGES, k_kv_free<4>, 1, 1024, a, sh);
+    return a.nseq <= 1024 ? run(MMOE_K_KV_PAGES, k_kv_free<1>, 1, a.nseq <= 256 ? 256 : 1024, a, sh) : run(MMOE_K_KV_PAGES, k_kv_free<4>, 1, 1024, a, sh);
 }
 
 }  // extern "C"
