@@ -6,10 +6,11 @@
 // per compute unit): a few more would wait for a second round. Every workgroup finds its piece from the sequences' lengths themselves, so grid and
 // workspace follow the numbers of workgroups and row tiles, not the bounds of the lengths.
 #pragma once
+#include <type_traits>
 #include "paged.h"
 
-// A row tile for the join: its first piece, how many, its first token, its first row among its sequence's, the sequence's rows. The first entry holds
-// the number of row tiles in `slot`; behind it the shared positions' tiles, then the sequences' own.
+// A sequence's row tile for the join: its first piece, how many, its first token, its first row among its sequence's, the sequence's rows. The first entry
+// holds the number of them in `slot` and in `parts` the pieces of a row tile over the shared positions, which are the first pieces of all.
 struct TreeTile { int slot, parts, t0, row0, rows; };
 
 struct Draft {
@@ -39,9 +40,9 @@ struct Draft {
     __device__ static __forceinline__ int cut(const Seq &q, float per) { return max((int)ceilf(fmaf((float)q.steps, per, -0x1p-10f)), 1); }
     struct Mem { int sum[2][4], at[4]; };
     __device__ static __forceinline__ int wave_sum(int v) { return wave_reduce(v, [](int x, int y) { return x + y; }); }
-    struct Piece { int seq, base, tiles, all_tiles, k; Seq q; };
-    // Piece id of a key/value head: its sequence (-1: the shared positions), that one's first piece and row tile, how many row tiles there are in all, the
-    // pieces of a row tile; false: there is no such piece. The same for every thread of the workgroup (256).
+    struct Piece { int seq, base, tiles, own_tiles, shared_k, k; Seq q; };
+    // Piece id of a key/value head: its sequence (-1: the shared positions), that one's first piece and row tile, how many row tiles the sequences have in
+    // all, the pieces of a row tile over the shared positions and of this one; false: there is no such piece. The same for every thread of the workgroup (256).
     __device__ static __forceinline__ bool find(const AttArgs &A, int id, Mem &M, Piece &o) {
         const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, n = A.a.nseq;
         const Seq sh = of_shared(A), q = of(A, n <= 64 ? l : tid);
@@ -56,27 +57,28 @@ struct Draft {
             __syncthreads();
             return M.sum[0][0] + M.sum[0][1] + M.sum[0][2] + M.sum[0][3];
         };
-        o.all_tiles = sh.tiles + total([](const Seq &x) { return x.tiles; });
+        o.own_tiles = total([](const Seq &x) { return x.tiles; });
+        const int all_tiles = sh.tiles + o.own_tiles;
         float per = 0.0f;   // pieces per step
         if (A.room) {
             // (the host has seen to it that all steps are a 32-bit number)
             const int steps = sh.tiles * sh.steps + total([](const Seq &x) { return x.tiles * x.steps; });
             // where the row tiles alone come near to what there is room for, there are more rounds anyway: half as large pieces then, and no search
-            const bool few = 4 * o.all_tiles <= 3 * A.room;
+            const bool few = 4 * all_tiles <= 3 * A.room;
             const int goal = few ? A.room : 2 * A.room;
             // rounding up makes about half a piece more of each row tile
-            per = fminf(((float)goal - (few ? 0.5f * (float)o.all_tiles : 0.0f)) / (float)max(steps, 1), 1.0f / (float)A.least);
+            per = fminf(((float)goal - (few ? 0.5f * (float)all_tiles : 0.0f)) / (float)max(steps, 1), 1.0f / (float)A.least);
             for (int i = 0; few; i++) {
                 const int got = sh.tiles * cut(sh, per) + total([&](const Seq &x) { return x.tiles * cut(x, per); });
                 if (got <= goal) break;
                 per = i < 6 ? per * fminf((float)goal / (float)got, 0.97f) : 0.0f;   // (at last each row tile one piece)
             }
         }
-        o.seq = -1; o.base = 0; o.tiles = 0; o.k = cut(sh, per); o.q = sh;
+        o.seq = -1; o.base = 0; o.tiles = 0; o.k = o.shared_k = cut(sh, per); o.q = sh;
         const int common = sh.tiles * o.k;
         if (id < common) return true;
         if (n <= 64) {
-            const int mine = q.tiles * cut(q, per), end = common + (int)scan_wave(mine), tiles = sh.tiles + (int)scan_wave(q.tiles) - q.tiles;
+            const int mine = q.tiles * cut(q, per), end = common + (int)scan_wave(mine), tiles = (int)scan_wave(q.tiles) - q.tiles;
             const int s = __popcll(__ballot(id >= end));   // a prefix of the lanes
             if (s >= n) return false;
             auto lane = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
@@ -85,7 +87,7 @@ struct Draft {
             o.k = cut(o.q, per);
             return true;
         }
-        int before = common, tiles = sh.tiles;
+        int before = common, tiles = 0;
         if (tid == 0) M.at[0] = -1;
         for (int s0 = 0; s0 < n; s0 += 256) {
             const Seq x = of(A, s0 + tid);
@@ -122,10 +124,10 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
     if (!Draft::find(A, id, F, o)) return;
     const Draft::Seq &q = o.q;
     const int k = __builtin_amdgcn_readfirstlane(o.k), steps = __builtin_amdgcn_readfirstlane(q.steps), tile = (id - o.base) / k, i = id - o.base - tile * k;
-    if (o.tiles + tile >= A.most_tiles) return;   // (not if qstart ascends)
+    if (o.seq >= 0 && o.tiles + tile >= A.most_tiles) return;   // (not if qstart ascends)
     if (A.room && kvh == 0 && i == 0 && threadIdx.x == 0) {
-        A.tile_at[1 + o.tiles + tile] = {id, k, q.t0, tile * ATT_BM, q.rows};
-        if (id == 0) A.tile_at[0].slot = min(o.all_tiles, A.most_tiles);
+        if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {id, k, q.t0, tile * ATT_BM, q.rows};
+        if (id == 0) A.tile_at[0] = {min(o.own_tiles, A.most_tiles), o.shared_k, 0, 0, 0};
     }
     const int each = steps / k, more = steps - each * k;
     AttWork work = {};
@@ -143,10 +145,9 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
 // The partial results of a row tile put together, 32 rows by a workgroup: each result holds its values over its own sum, its maximum (in units of log 2)
 // and sum, negative where results may not be finite. A lane has a row and 4 of each 8 dims, a wave a quarter of the dims (wide) or of the results
 // (deep: then a quarter of the dims is a workgroup's own, and the waves join through LDS).
-#define TJ_U 4   // results under way
 template <int T, int D, bool DEEP>
 __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
-    constexpr int C = D / 32;   // groups of 8 dims of a lane
+    constexpr int C = D / 32, TJ_U = 4;   // groups of 8 dims of a lane; results under way
     const mmoe_attn_args &a = A.a;
     __shared__ f4 acc[DEEP ? 3 : 1][C][64];
     __shared__ float2 stat[DEEP ? 3 : 1][32];
@@ -157,67 +158,61 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
     const int w = id & 3;   // the tile's wave, its key/value head, its number
     id >>= 2;
     const int tile = (int)A.by_kv(id), kvh = id - tile * A.kv.heads;
-    const int first = a.shared ? (att_start(a, a.nseq) * A.group + ATT_BM - 1) / ATT_BM : 0;   // row tiles over the shared positions
-    const TreeTile t = A.tile_at[1 + min(first + tile, A.most_tiles - 1)];
-    if (first + tile >= A.tile_at[0].slot || (t.parts == 1 && !a.shared)) return;   // none, or written by the piece that was all of it
+    const TreeTile head_of = A.tile_at[0], t = A.tile_at[1 + tile];
+    if (tile >= head_of.slot || (t.parts == 1 && !a.shared)) return;   // none, or written by the piece that was all of it
     // nothing outside the arrays, whatever qstart holds
-    auto inside = [&](const TreeTile &t) { return t.slot >= 0 && t.parts > 0 && t.parts <= A.most_pieces - t.slot; };
-    if (!inside(t) || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
+    if (t.slot < 0 || t.parts < 1 || t.parts > A.most_pieces - t.slot || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
     const int r = t.row0 + w * 32 + n;
     if (t.row0 + w * 32 >= t.rows) return;
     const bool live = r < t.rows;
     const int row = min(r, t.rows - 1), j = (int)A.by_group(row), tok = t.t0 + j, head = kvh * A.group + row - j * A.group;
-    int common = 0, at_sh = 0, slot_sh = 0;
-    if (a.shared) {
-        const int rs = tok * A.group + row - j * A.group;
-        const TreeTile &s = A.tile_at[1 + rs / ATT_BM];
-        if (inside(s)) { common = s.parts; slot_sh = s.slot; at_sh = rs % ATT_BM; }
-    }
-    const int most = DEEP || a.shared ? wave_max(common) : 0, parts = most + t.parts;   // (rows may lie in two shared tiles)
+    // the shared positions' row tiles hold every token's rows
+    const int common = a.shared ? head_of.parts : 0, rs = tok * A.group + row - j * A.group, slot_sh = rs / ATT_BM * common, at_sh = rs % ATT_BM;
+    if (common < 0 || common > A.most_pieces || (int64_t)(rs / ATT_BM + 1) * common > A.most_pieces) return;
+    const int parts = common + t.parts;
+    struct Result { float2 v; f4 y[C]; };
+    auto load = [&](Result &x, int p) {
+        const bool c = p < common;
+        const int at = c ? at_sh : w * 32 + n;
+        const int64_t wave = ((int64_t)(c ? slot_sh + p : t.slot + p - common) * A.kv.heads + kvh) * A.slot_waves + (at >> 5);
+        x.v = A.pm[wave * 32 + (at & 31)];
+        const f4 *q = (const f4 *)(A.po + wave * 32 * D) + 32 * hh + (at & 31);
+#pragma unroll
+        for (int i = 0; i < C; i++) x.y[i] = q[(quarter * C + i) * 64];
+    };
     float m = -__builtin_inff(), sum = 0.0f;
     f4 o[C] = {};
     bool wild = false;
-    auto lowered_to = [&](float mn) {   // what is there counts from the maximum mn on
-        const float al = m == -__builtin_inff() ? 0.0f : exp2_(m - mn);
-        m = mn; sum *= al;
-#pragma unroll
-        for (int c = 0; c < C; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[c][i] = al != 0.0f ? o[c][i] * al : only_odd(o[c][i]);
-    };
-    auto add = [&](float2 v, const f4 *y) {
-        if (v.y == 0.0f) return;
-        const float e = exp2_(v.x - m);
-        sum = fmaf(fabsf(v.y), e, sum);
-        wild |= v.y < 0.0f;
-#pragma unroll
-        for (int c = 0; c < C; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[c][i] = e != 0.0f ? fmaf(e, y[c][i], o[c][i]) : o[c][i] + (v.y < 0.0f ? only_odd(y[c][i]) : 0.0f);
-    };
-    constexpr int STEP = DEEP ? 4 : 1;
-    for (int p0 = DEEP ? wv : 0; p0 < parts; p0 += TJ_U * STEP) {
-        float2 v[TJ_U];
-        f4 y[TJ_U][C];
-#pragma unroll
-        for (int u = 0; u < TJ_U; u++) {
-            const int p = p0 + u * STEP;
-            const bool c = p < most;
-            v[u] = make_float2(0.0f, 0.0f);
-            if (p >= parts || (c && p >= common)) continue;
-            const int at = c ? at_sh : w * 32 + n;
-            const int64_t wave = ((int64_t)(c ? slot_sh + p : t.slot + p - most) * A.kv.heads + kvh) * A.slot_waves + (at >> 5);
-            v[u] = A.pm[wave * 32 + (at & 31)];
-            const f4 *q = (const f4 *)(A.po + wave * 32 * D) + 32 * hh + (at & 31);
-#pragma unroll
-            for (int i = 0; i < C; i++) y[u][i] = q[(quarter * C + i) * 64];
-        }
+    // N results more: no branches, so that the code is short (a call's first instructions come from memory, too)
+    auto add = [&](const Result *x, auto n) {
         float mn = m;
 #pragma unroll
-        for (int u = 0; u < TJ_U; u++) if (v[u].y != 0.0f) mn = fmaxf(mn, v[u].x);
-        if (mn > m) lowered_to(mn);
+        for (int u = 0; u < n.value; u++) mn = fmaxf(mn, x[u].v.y != 0.0f ? x[u].v.x : -__builtin_inff());
+        const float by = mn == -__builtin_inff() ? 0.0f : mn, al = exp2_(m - by);
+        m = mn; sum *= al;
 #pragma unroll
-        for (int u = 0; u < TJ_U; u++) add(v[u], y[u]);
+        for (int c = 0; c < C; c++) o[c] *= al;
+#pragma unroll
+        for (int u = 0; u < n.value; u++) {
+            const float e = x[u].v.y != 0.0f ? exp2_(x[u].v.x - by) : 0.0f;
+            sum = fmaf(fabsf(x[u].v.y), e, sum);
+            wild |= x[u].v.y < 0.0f;
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[c][i] = fmaf(e, x[u].y[c][i], o[c][i]);
+        }
+    };
+    constexpr int STEP = DEEP ? 4 : 1;
+#pragma unroll 1
+    for (int p0 = DEEP ? wv : 0; p0 < parts; p0 += TJ_U * STEP) {
+        Result x[TJ_U];
+#pragma unroll
+        for (int u = 0; u < TJ_U; u++) {
+            x[u] = {};
+            if (p0 + u * STEP < parts) load(x[u], p0 + u * STEP);
+        }
+        add(x, std::integral_constant<int, TJ_U>{});
     }
     if (DEEP) {
         if (wv) {
@@ -227,14 +222,27 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
         }
         __syncthreads();
         if (wv) return;
-        float mn = m;
-        for (int i = 0; i < 3; i++) if (stat[i][n].y != 0.0f) mn = fmaxf(mn, stat[i][n].x);
-        if (mn > m) lowered_to(mn);
-        for (int i = 0; i < 3; i++) {
-            f4 y[C];
+        Result x[3];
 #pragma unroll
-            for (int c = 0; c < C; c++) y[c] = acc[i][c][l];
-            add(stat[i][n], y);
+        for (int i = 0; i < 3; i++) {
+            x[i].v = stat[i][n];
+#pragma unroll
+            for (int c = 0; c < C; c++) x[i].y[c] = acc[i][c][l];
+        }
+        add(x, std::integral_constant<int, 3>{});
+    }
+    if (__any(wild && live)) {   // once more: results that are not finite count whatever their weight
+#pragma unroll
+        for (int c = 0; c < C; c++) o[c] = f4{0, 0, 0, 0};
+#pragma unroll 1
+        for (int p = 0; p < parts; p++) {
+            Result x;
+            load(x, p);
+            const float e = x.v.y != 0.0f ? exp2_(x.v.x - m) : 0.0f;
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[c][i] = e != 0.0f ? fmaf(e, x.y[c][i], o[c][i]) : x.v.y != 0.0f ? o[c][i] + only_odd(x.y[c][i]) : o[c][i];
         }
     }
     if (!live) return;

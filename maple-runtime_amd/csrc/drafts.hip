@@ -23,19 +23,19 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     TreePlan p = {};
     const int group = a.heads / kv.heads;
     const int64_t rows = (int64_t)a.ntok * group, most = (int64_t)std::min(a.max_q, a.ntok) * group;
-    const int64_t tiles = std::min((int64_t)a.nseq * ((most + ATT_BM - 1) / ATT_BM), rows / ATT_BM + a.nseq) + (a.shared ? (rows + ATT_BM - 1) / ATT_BM : 0);
+    const int64_t own = std::min((int64_t)a.nseq * ((most + ATT_BM - 1) / ATT_BM), rows / ATT_BM + a.nseq), tiles = own + (a.shared ? (rows + ATT_BM - 1) / ATT_BM : 0);
     // Row tiles of so few positions, and so many of them, that they stay whole: nothing to join
     const int64_t most_steps = (a.window ? std::min<int64_t>(a.max_len, (int64_t)a.window + a.max_q + TREE_BN) : a.max_len) / TREE_BN + 1;
     const bool whole = !a.shared && most_steps <= 12 && tiles * kv.heads >= 192;
     p.room = whole ? 0 : std::max(1, (kv.head_dim == 64 ? 768 : 512) / kv.heads);   // two workgroups per compute unit, three with heads of 64
     p.least = 2;
-    const int64_t pieces = whole ? tiles : std::max(tiles <= p.room * 3 / 4 ? (int64_t)p.room : 2 * (int64_t)p.room + tiles, tiles), join = tiles * kv.heads * 4;
+    const int64_t pieces = whole ? tiles : std::max(tiles <= p.room * 3 / 4 ? (int64_t)p.room : 2 * (int64_t)p.room + tiles, tiles), join = own * kv.heads * 4;
     p.deep = join < 128;   // 32 rows of a key/value head each
     p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(pieces * kv.heads, join * (p.deep ? 4 : 1)) * 256 <= (int64_t)MAX_THREADS;
-    p.pieces = (int)std::min<int64_t>(pieces, INT32_MAX); p.tiles = (int)std::min<int64_t>(tiles, INT32_MAX); p.join = (unsigned)(p.deep ? join * 4 : join);
+    p.pieces = (int)std::min<int64_t>(pieces, INT32_MAX); p.tiles = (int)std::min<int64_t>(own, INT32_MAX); p.join = (unsigned)(p.deep ? join * 4 : join);
     p.slot_waves = a.shared ? ATT_BM / 32 : (int)std::min<int64_t>(ATT_BM, most + 31) / 32;
     p.results = whole ? 0 : (size_t)pieces * kv.heads * p.slot_waves;
-    p.bytes = p.results * 32 * (kv.head_dim * 4 + 8) + (whole ? 0 : (size_t)(tiles + 1) * sizeof(TreeTile)) + 256;
+    p.bytes = p.results * 32 * (kv.head_dim * 4 + 8) + (whole ? 0 : (size_t)(own + 1) * sizeof(TreeTile)) + 256;
     return p;
 }
 
