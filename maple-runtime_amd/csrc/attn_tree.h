@@ -36,8 +36,12 @@ struct Draft {
         q.steps = max(q.to - q.from + TREE_BN - 1, 0) / TREE_BN;
         return q;
     }
-    // pieces of a row tile: its steps times the pieces per step, rounded up (up to 2^-10 above a whole number that one is taken)
-    __device__ static __forceinline__ int cut(const Seq &q, float per) { return max((int)ceilf(fmaf((float)q.steps, per, -0x1p-10f)), 1); }
+    // Pieces of a row tile: its steps times the pieces per step, rounded up (up to 2^-10 above a whole number that one is taken). Of two steps at
+    // least, but for the shortest tiles: 12 results are joined in the time of 6 (26 tokens over 700 positions, 11 steps: 12.6 us, in 6 pieces 13.6; but 60 over
+    // 3000: 48 pieces 19.6, 24 pieces 17.0)
+    __device__ static __forceinline__ int cut(const Seq &q, float per) {
+        return max(min((int)ceilf(fmaf((float)q.steps, per, -0x1p-10f)), max((q.steps + 1) >> 1, 12)), 1);
+    }
     struct Mem { int sum[2][4], at[4]; };
     __device__ static __forceinline__ int wave_sum(int v) { return wave_reduce(v, [](int x, int y) { return x + y; }); }
     struct Piece { int seq, base, tiles, own_tiles, shared_k, k; Seq q; };
@@ -67,7 +71,7 @@ struct Draft {
             const bool few = 4 * all_tiles <= 3 * A.room;
             const int goal = few ? A.room : 2 * A.room;
             // rounding up makes about half a piece more of each row tile
-            per = fminf(((float)goal - (few ? 0.5f * (float)all_tiles : 0.0f)) / (float)max(steps, 1), 1.0f / (float)A.least);
+            per = fminf(((float)goal - (few ? 0.5f * (float)all_tiles : 0.0f)) / (float)max(steps, 1), 1.0f);
             for (int i = 0; few; i++) {
                 const int got = sh.tiles * cut(sh, per) + total([&](const Seq &x) { return x.tiles * cut(x, per); });
                 if (got <= goal) break;
@@ -143,18 +147,18 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
 }
 
 // The partial results of a row tile put together, 32 rows by a workgroup: each result holds its values over its own sum, its maximum (in units of log 2)
-// and sum, negative where results may not be finite. A lane has a row and 4 of each 8 dims, a wave a quarter of the dims (wide) or of the results
-// (deep: then a quarter of the dims is a workgroup's own, and the waves join through LDS).
+// and sum, negative where results may not be finite. A lane has a row and 4 of each 8 dims, a wave a quarter of the dims; deep (few row tiles, so
+// perhaps many results of each): a wave has a quarter of the results, a workgroup an eighth of the dims, and the waves join through LDS.
 template <int T, int D, bool DEEP>
 __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
-    constexpr int C = D / 32, TJ_U = 4;   // groups of 8 dims of a lane; results under way
+    constexpr int C = DEEP ? D / 64 : D / 32, TJ_U = DEEP ? 8 : 4;   // groups of 8 dims of a lane; results under way
     const mmoe_attn_args &a = A.a;
     __shared__ f4 acc[DEEP ? 3 : 1][C][64];
     __shared__ float2 stat[DEEP ? 3 : 1][32];
     const int l = threadIdx.x & 63, n = l & 31, hh = l >> 5, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     unsigned id = blockIdx.x;
-    int quarter = wv;
-    if (DEEP) { quarter = id & 3; id >>= 2; }
+    int share = wv;   // of the dims
+    if (DEEP) { share = id & 7; id >>= 3; }
     const int w = id & 3;   // the tile's wave, its key/value head, its number
     id >>= 2;
     const int tile = (int)A.by_kv(id), kvh = id - tile * A.kv.heads;
@@ -178,7 +182,7 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
         x.v = A.pm[wave * 32 + (at & 31)];
         const f4 *q = (const f4 *)(A.po + wave * 32 * D) + 32 * hh + (at & 31);
 #pragma unroll
-        for (int i = 0; i < C; i++) x.y[i] = q[(quarter * C + i) * 64];
+        for (int i = 0; i < C; i++) x.y[i] = q[(share * C + i) * 64];
     };
     float m = -__builtin_inff(), sum = 0.0f;
     f4 o[C] = {};
@@ -247,13 +251,13 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
     }
     if (!live) return;
     const float inv = 1.0f / sum;
-    uint16_t *out = (uint16_t *)a.out + (int64_t)tok * a.out_token + head * a.out_head + quarter * (D / 4) + 4 * hh;
+    uint16_t *out = (uint16_t *)a.out + (int64_t)tok * a.out_token + head * a.out_head + share * (8 * C) + 4 * hh;
 #pragma unroll
     for (int c = 0; c < C; c++) {
         uint2 v = make_uint2(pack2<T>(o[c][0] * inv, o[c][1] * inv), pack2<T>(o[c][2] * inv, o[c][3] * inv));
         if (sum == 0.0f) v = make_uint2(0, 0);
         *(uint2 *)(out + 8 * c) = v;
     }
-    if (a.lse && quarter == 0 && hh == 0) a.lse[(int64_t)tok * a.heads + head] = sum == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * ATT_LN2;
+    if (a.lse && share == 0 && hh == 0) a.lse[(int64_t)tok * a.heads + head] = sum == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(sum)) * ATT_LN2;
 }
 

@@ -14,7 +14,7 @@ static int check_bits(const char *who, const mmoe_attn_args *p, const mmoe_kv_ca
 // How a call of mmoe_attn_tree is divided (drafts.h). Only the values in the arguments count (a captured call keeps its grid). The numbers of
 // workgroups are for the 256 compute units of the one device that the kernels are built and were measured for.
 struct TreePlan {
-    int room, least, pieces, slot_waves, tiles;
+    int room, pieces, slot_waves, tiles;
     unsigned join;
     bool deep, fits;
     size_t results, bytes;
@@ -28,11 +28,10 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     const int64_t most_steps = (a.window ? std::min<int64_t>(a.max_len, (int64_t)a.window + a.max_q + TREE_BN) : a.max_len) / TREE_BN + 1;
     const bool whole = !a.shared && most_steps <= 12 && tiles * kv.heads >= 192;
     p.room = whole ? 0 : std::max(1, (kv.head_dim == 64 ? 768 : 512) / kv.heads);   // two workgroups per compute unit, three with heads of 64
-    p.least = 2;
     const int64_t pieces = whole ? tiles : std::max(tiles <= p.room * 3 / 4 ? (int64_t)p.room : 2 * (int64_t)p.room + tiles, tiles), join = own * kv.heads * 4;
     p.deep = join < 128;   // 32 rows of a key/value head each
-    p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(pieces * kv.heads, join * (p.deep ? 4 : 1)) * 256 <= (int64_t)MAX_THREADS;
-    p.pieces = (int)std::min<int64_t>(pieces, INT32_MAX); p.tiles = (int)std::min<int64_t>(own, INT32_MAX); p.join = (unsigned)(p.deep ? join * 4 : join);
+    p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(pieces * kv.heads, join * (p.deep ? 8 : 1)) * 256 <= (int64_t)MAX_THREADS;
+    p.pieces = (int)std::min<int64_t>(pieces, INT32_MAX); p.tiles = (int)std::min<int64_t>(own, INT32_MAX); p.join = (unsigned)(p.deep ? join * 8 : join);
     p.slot_waves = a.shared ? ATT_BM / 32 : (int)std::min<int64_t>(ATT_BM, most + 31) / 32;
     p.results = whole ? 0 : (size_t)pieces * kv.heads * p.slot_waves;
     p.bytes = p.results * 32 * (kv.head_dim * 4 + 8) + (whole ? 0 : (size_t)(own + 1) * sizeof(TreeTile)) + 256;
@@ -48,7 +47,7 @@ static int tree_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const Tree
     A.s1 = CAP ? 2.0f * a.scale / a.cap * ATT_LOG2E : a.scale * ATT_LOG2E;
     A.s2 = a.cap * ATT_LOG2E;
     A.bits = bits; A.words = words;
-    A.room = p.room; A.least = p.least; A.most_tiles = p.tiles; A.most_pieces = p.pieces; A.slot_waves = p.slot_waves;
+    A.room = p.room; A.most_tiles = p.tiles; A.most_pieces = p.pieces; A.slot_waves = p.slot_waves;
     A.po = (float *)a.ws;
     A.pm = (float2 *)(A.po + p.results * 32 * D);
     A.tile_at = (TreeTile *)(A.pm + p.results * 32);

@@ -478,10 +478,10 @@ struct AttArgs {
     float2 *pm;
     int64_t at_tile, at_few;
     // Drafted tokens (TREE, attn_tree.h): words of bits per token, bit j: it sees its sequence's j-th new token; the pieces that the row tiles of a key/
-    // value head are to be cut into (0: none, each stays whole), the fewest steps of one, the most row tiles and pieces there can be, waves (of 32
-    // rows) of a piece's partial results in po and pm; the row tiles
+    // value head are to be cut into (0: none, each stays whole), the most row tiles and pieces there can be, waves (of 32 rows) of a piece's partial
+    // results in po and pm; the row tiles
     const uint64_t *bits;
-    int words, room, least, most_tiles, most_pieces, slot_waves;
+    int words, room, most_tiles, most_pieces, slot_waves;
     struct TreeTile *tile_at;
 };
 
