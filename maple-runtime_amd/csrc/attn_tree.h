@@ -9,9 +9,10 @@
 #include <type_traits>
 #include "paged.h"
 
-// A sequence's row tile for the join: its first piece, how many, its first token, its first row among its sequence's, the sequence's rows. The first entry
-// holds the number of them in `slot` and in `parts` the pieces of a row tile over the shared positions, which are the first pieces of all.
-struct TreeTile { int slot, parts, t0, row0, rows; };
+// A sequence's row tile for the join: its first piece, how many, how far apart, its first token, its first row among its sequence's, the sequence's rows. The
+// first entry holds the number of them in `slot` and in `parts` and `apart` the pieces of a row tile over the shared positions, which are the
+// first pieces of all.
+struct TreeTile { int slot, parts, apart, t0, row0, rows; };
 
 struct Draft {
     struct Seq { int t0, t1, len, rows, tiles, from, to, steps; };
@@ -44,10 +45,11 @@ struct Draft {
     }
     struct Mem { int sum[2][4], at[4]; };
     __device__ static __forceinline__ int wave_sum(int v) { return wave_reduce(v, [](int x, int y) { return x + y; }); }
-    struct Piece { int seq, base, tiles, own_tiles, shared_k, k; Seq q; };
-    // Piece id of a key/value head: its sequence (-1: the shared positions), that one's first piece and row tile, how many row tiles the sequences have in
-    // all, the pieces of a row tile over the shared positions and of this one; false: there is no such piece. The same for every thread of the workgroup (256).
-    __device__ static __forceinline__ bool find(const AttArgs &A, int id, Mem &M, Piece &o) {
+    struct Piece { int id, kvh, seq, base, tiles, own_tiles, shared_k, shared_tiles, k; Seq q; };
+    // The workgroup's piece: its number and key/value head, its sequence (-1: the shared positions), that one's first piece and row tile, how many row
+    // tiles the sequences have in all, the pieces of a row tile over the shared positions, their row tiles, the pieces of this row tile; false: none. The
+    // same for every thread of the workgroup (256).
+    __device__ static __forceinline__ bool find(const AttArgs &A, Mem &M, Piece &o) {
         const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, n = A.a.nseq;
         const Seq sh = of_shared(A), q = of(A, n <= 64 ? l : tid);
         // a sum over all sequences: every wave by itself, or all of them together
@@ -64,6 +66,7 @@ struct Draft {
         o.own_tiles = total([](const Seq &x) { return x.tiles; });
         const int all_tiles = sh.tiles + o.own_tiles;
         float per = 0.0f;   // pieces per step
+        int pieces = all_tiles;
         if (A.room) {
             // (the host has seen to it that all steps are a 32-bit number)
             const int steps = sh.tiles * sh.steps + total([](const Seq &x) { return x.tiles * x.steps; });
@@ -72,13 +75,19 @@ struct Draft {
             const int goal = few ? A.room : 2 * A.room;
             // rounding up makes about half a piece more of each row tile
             per = fminf(((float)goal - (few ? 0.5f * (float)all_tiles : 0.0f)) / (float)max(steps, 1), 1.0f);
-            for (int i = 0; few; i++) {
-                const int got = sh.tiles * cut(sh, per) + total([&](const Seq &x) { return x.tiles * cut(x, per); });
-                if (got <= goal) break;
-                per = i < 6 ? per * fminf((float)goal / (float)got, 0.97f) : 0.0f;   // (at last each row tile one piece)
+            for (int i = 0;; i++) {
+                pieces = sh.tiles * cut(sh, per) + total([&](const Seq &x) { return x.tiles * cut(x, per); });
+                if (!few || pieces <= goal) break;
+                per = i < 6 ? per * fminf((float)goal / (float)pieces, 0.97f) : 0.0f;   // (at last each row tile one piece)
             }
         }
-        o.seq = -1; o.base = 0; o.tiles = 0; o.k = o.shared_k = cut(sh, per); o.q = sh;
+        // Workgroups go to the card's dies in turn: each die a run of consecutive pieces, in which the row tiles of the same positions lie side by
+        // side and read them from the die's own cache
+        const int all = pieces * A.kv.heads, each = (all + 7) >> 3, at = (int)(blockIdx.x & 7) * each + (int)(blockIdx.x >> 3);
+        if ((int)(blockIdx.x >> 3) >= each || at >= all) return false;
+        o.kvh = at / pieces;
+        const int id = o.id = at - o.kvh * pieces;
+        o.seq = -1; o.base = 0; o.tiles = 0; o.k = o.shared_k = cut(sh, per); o.shared_tiles = sh.tiles; o.q = sh;
         const int common = sh.tiles * o.k;
         if (id < common) return true;
         if (n <= 64) {
@@ -100,14 +109,14 @@ struct Draft {
             __syncthreads();   // the sums before have been read
             if (l == 63) { M.sum[0][w] = end; M.sum[1][w] = t; }
             __syncthreads();
-            int pieces = 0, ts = 0;
+            int ps = 0, ts = 0;
             for (int i = 0; i < 4; i++) {
                 if (i < w) { end += M.sum[0][i]; t += M.sum[1][i]; }
-                pieces += M.sum[0][i]; ts += M.sum[1][i];
+                ps += M.sum[0][i]; ts += M.sum[1][i];
             }
             end += before; t += tiles;
             if (id < end && id >= end - mine) { M.at[0] = s0 + tid; M.at[1] = end - mine; M.at[2] = t - x.tiles; }
-            before += pieces; tiles += ts;
+            before += ps; tiles += ts;
             if (id < before) break;
         }
         __syncthreads();
@@ -123,26 +132,25 @@ template <int T, int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
     __shared__ AttTileMem<D, TREE_BN> M;
     __shared__ Draft::Mem F;
-    const int id = (int)A.by_kv(blockIdx.x), kvh = blockIdx.x - id * A.kv.heads;
     Draft::Piece o;
-    if (!Draft::find(A, id, F, o)) return;
+    if (!Draft::find(A, F, o)) return;
     const Draft::Seq &q = o.q;
-    const int k = __builtin_amdgcn_readfirstlane(o.k), steps = __builtin_amdgcn_readfirstlane(q.steps), tile = (id - o.base) / k, i = id - o.base - tile * k;
+    const int k = __builtin_amdgcn_readfirstlane(o.k), steps = __builtin_amdgcn_readfirstlane(q.steps), i = (o.id - o.base) / q.tiles, tile = o.id - o.base - i * q.tiles;
     if (o.seq >= 0 && o.tiles + tile >= A.most_tiles) return;   // (not if qstart ascends)
-    if (A.room && kvh == 0 && i == 0 && threadIdx.x == 0) {
-        if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {id, k, q.t0, tile * ATT_BM, q.rows};
-        if (id == 0) A.tile_at[0] = {min(o.own_tiles, A.most_tiles), o.shared_k, 0, 0, 0};
+    if (A.room && o.kvh == 0 && i == 0 && threadIdx.x == 0) {
+        if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {o.id, k, q.tiles, q.t0, tile * ATT_BM, q.rows};
+        if (o.id == 0) A.tile_at[0] = {min(o.own_tiles, A.most_tiles), o.shared_k, o.shared_tiles, 0, 0, 0};
     }
     const int each = steps / k, more = steps - each * k;
     AttWork work = {};
     work.shared = o.seq < 0;
     work.at = {max(o.seq, 0), tile * ATT_BM, q.rows, q.t0};
     work.t1 = q.t1; work.len = q.len;
-    work.kvh = kvh;
+    work.kvh = o.kvh;
     work.p0 = q.from + (i * each + min(i, more)) * TREE_BN;
     work.p1 = min(work.p0 + (each + (i < more)) * TREE_BN, q.to);
     work.whole = k == 1 && !A.a.shared;
-    work.slot = (int64_t)id * A.kv.heads + kvh;
+    work.slot = (int64_t)o.id * A.kv.heads + o.kvh;
     att_tile<T, D, CAP, BIAS, true>(tree_args(), work, M);
 }
 
@@ -151,7 +159,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
 // perhaps many results of each): a wave has a quarter of the results, a workgroup an eighth of the dims, and the waves join through LDS.
 template <int T, int D, bool DEEP>
 __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
-    constexpr int C = DEEP ? D / 64 : D / 32, TJ_U = DEEP ? 8 : 4;   // groups of 8 dims of a lane; results under way
+    constexpr int C = DEEP ? D / 64 : D / 32, TJ_U = DEEP ? 8 : 512 / D;   // groups of 8 dims of a lane; results under way
     const mmoe_attn_args &a = A.a;
     __shared__ f4 acc[DEEP ? 3 : 1][C][64];
     __shared__ float2 stat[DEEP ? 3 : 1][32];
@@ -165,20 +173,20 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
     const TreeTile head_of = A.tile_at[0], t = A.tile_at[1 + tile];
     if (tile >= head_of.slot || (t.parts == 1 && !a.shared)) return;   // none, or written by the piece that was all of it
     // nothing outside the arrays, whatever qstart holds
-    if (t.slot < 0 || t.parts < 1 || t.parts > A.most_pieces - t.slot || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
+    if (t.slot < 0 || t.parts < 1 || t.apart < 0 || t.slot + (t.parts - 1) * (int64_t)t.apart >= A.most_pieces || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
     const int r = t.row0 + w * 32 + n;
     if (t.row0 + w * 32 >= t.rows) return;
     const bool live = r < t.rows;
     const int row = min(r, t.rows - 1), j = (int)A.by_group(row), tok = t.t0 + j, head = kvh * A.group + row - j * A.group;
     // the shared positions' row tiles hold every token's rows
-    const int common = a.shared ? head_of.parts : 0, rs = tok * A.group + row - j * A.group, slot_sh = rs / ATT_BM * common, at_sh = rs % ATT_BM;
-    if (common < 0 || common > A.most_pieces || (int64_t)(rs / ATT_BM + 1) * common > A.most_pieces) return;
+    const int common = a.shared ? head_of.parts : 0, rs = tok * A.group + row - j * A.group, slot_sh = rs / ATT_BM, at_sh = rs % ATT_BM;
+    if (a.shared && (common < 0 || head_of.apart < 0 || slot_sh + (common - 1) * (int64_t)head_of.apart >= A.most_pieces)) return;
     const int parts = common + t.parts;
     struct Result { float2 v; f4 y[C]; };
     auto load = [&](Result &x, int p) {
         const bool c = p < common;
         const int at = c ? at_sh : w * 32 + n;
-        const int64_t wave = ((int64_t)(c ? slot_sh + p : t.slot + p - common) * A.kv.heads + kvh) * A.slot_waves + (at >> 5);
+        const int64_t wave = ((int64_t)(c ? slot_sh + p * head_of.apart : t.slot + (p - common) * t.apart) * A.kv.heads + kvh) * A.slot_waves + (at >> 5);
         x.v = A.pm[wave * 32 + (at & 31)];
         const f4 *q = (const f4 *)(A.po + wave * 32 * D) + 32 * hh + (at & 31);
 #pragma unroll

@@ -30,7 +30,7 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     p.room = whole ? 0 : std::max(1, (kv.head_dim == 64 ? 768 : 512) / kv.heads);   // two workgroups per compute unit, three with heads of 64
     const int64_t pieces = whole ? tiles : std::max(tiles <= p.room * 3 / 4 ? (int64_t)p.room : 2 * (int64_t)p.room + tiles, tiles), join = own * kv.heads * 4;
     p.deep = join < 128;   // 32 rows of a key/value head each
-    p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(pieces * kv.heads, join * (p.deep ? 8 : 1)) * 256 <= (int64_t)MAX_THREADS;
+    p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(pieces * kv.heads + 7, join * (p.deep ? 8 : 1)) * 256 <= (int64_t)MAX_THREADS;
     p.pieces = (int)std::min<int64_t>(pieces, INT32_MAX); p.tiles = (int)std::min<int64_t>(own, INT32_MAX); p.join = (unsigned)(p.deep ? join * 8 : join);
     p.slot_waves = a.shared ? ATT_BM / 32 : (int)std::min<int64_t>(ATT_BM, most + 31) / 32;
     p.results = whole ? 0 : (size_t)pieces * kv.heads * p.slot_waves;
@@ -51,7 +51,7 @@ static int tree_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const Tree
     A.po = (float *)a.ws;
     A.pm = (float2 *)(A.po + p.results * 32 * D);
     A.tile_at = (TreeTile *)(A.pm + p.results * 32);
-    if (run(MMOE_K_ATT_TREE, k_attn_tree<T, D, CAP, BIAS>, (unsigned)p.pieces * kv.heads, 256, A)) return -1;
+    if (run(MMOE_K_ATT_TREE, k_attn_tree<T, D, CAP, BIAS>, ((unsigned)p.pieces * kv.heads + 7) & ~7u, 256, A)) return -1;
     if (!p.room) return 0;
     return p.deep ? run(MMOE_K_ATT_TREE, k_tree_join<T, D, true>, p.join, 256, A) : run(MMOE_K_ATT_TREE, k_tree_join<T, D, false>, p.join, 256, A);
 }
