@@ -81,6 +81,7 @@ struct Draft {
                 per = i < 6 ? per * fminf((float)goal / (float)pieces, 0.97f) : 0.0f;   // (at last each row tile one piece)
             }
         }
+        if (pieces == 0 && A.room && blockIdx.x == 0 && tid == 0) A.tile_at[0] = {};   // the workspace may hold an earlier call's
         // Workgroups go to the card's dies in turn: each die a run of consecutive pieces, in which the row tiles of the same positions lie side by
         // side and read them from the die's own cache
         const int all = pieces * A.kv.heads, each = (all + 7) >> 3, at = (int)(blockIdx.x & 7) * each + (int)(blockIdx.x >> 3);

@@ -173,6 +173,19 @@ def test_drafts_of_many_sequences():
         b.run(d, "70 sequences")
 
 
+@pytest.mark.parametrize("shared", [0, 64])
+def test_a_step_without_new_tokens(shared):
+    """a captured step whose sequences all rest: the rows stay as they were, whatever the workspace holds of the step before"""
+    rng = np.random.default_rng(5)
+    b = TreeBatch(rng, drafts(rng, [9, 40], 5), lens=[900, 1500], heads=8, kv=2, shared=shared)
+    with Dev() as d:
+        b.run(d, "with tokens")
+        d.write(b.p_out, b.out0); d.write(b.p_lse, b.lse0)
+        d.write(b.args.qstart, np.zeros(3, np.int32))
+        M.check(d.lib.mmoe_attn_tree(b.args, b.cache, b.p_bits, b.words), "attention")
+        assert np.array_equal(d.get(b.p_out, b.out0), b.out0) and np.array_equal(d.get(b.p_lse, b.lse0), b.lse0)
+
+
 def test_drafts_past_32_bits():
     """a cache whose blocks lie 2^25 values apart: the last one begins at byte 8.6e9"""
     rng = np.random.default_rng(8)
