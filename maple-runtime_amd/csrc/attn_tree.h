@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
     if (!Draft::find(A, F, o)) return;
     const Draft::Seq &q = o.q;
     const int k = __builtin_amdgcn_readfirstlane(o.k), steps = __builtin_amdgcn_readfirstlane(q.steps), i = (o.id - o.base) / q.tiles, tile = o.id - o.base - i * q.tiles;
-    if (o.seq >= 0 && o.tiles + tile >= A.most_tiles) return;   // (not if qstart ascends)
+    if (o.id >= A.most_pieces || (o.seq >= 0 && o.tiles + tile >= A.most_tiles)) return;   // (not if qstart ascends)
     if (A.room && o.kvh == 0 && i == 0 && threadIdx.x == 0) {
         if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {o.id, k, q.tiles, q.t0, tile * ATT_BM, q.rows};
         if (o.id == 0) A.tile_at[0] = {min(o.own_tiles, A.most_tiles), o.shared_k, o.shared_tiles, 0, 0, 0};
@@ -173,8 +173,8 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
     const int tile = (int)A.by_kv(id), kvh = id - tile * A.kv.heads;
     const TreeTile head_of = A.tile_at[0], t = A.tile_at[1 + tile];
     if (tile >= head_of.slot || (t.parts == 1 && !a.shared)) return;   // none, or written by the piece that was all of it
-    // nothing outside the arrays, whatever qstart holds
-    if (t.slot < 0 || t.parts < 1 || t.apart < 0 || t.slot + (t.parts - 1) * (int64_t)t.apart >= A.most_pieces || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
+    // nothing outside the arrays, whatever qstart holds (where it does not ascend, row tiles may be those of an earlier call)
+    if (w >= A.slot_waves || t.row0 >= t.rows || t.slot < 0 || t.parts < 1 || t.apart < 0 || t.slot + (t.parts - 1) * (int64_t)t.apart >= A.most_pieces || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
     const int r = t.row0 + w * 32 + n;
     if (t.row0 + w * 32 >= t.rows) return;
     const bool live = r < t.rows;

@@ -186,6 +186,26 @@ def test_a_step_without_new_tokens(shared):
         assert np.array_equal(d.get(b.p_out, b.out0), b.out0) and np.array_equal(d.get(b.p_lse, b.lse0), b.lse0)
 
 
+@pytest.mark.parametrize("heads,kv,shared,most", [(8, 2, 0, 40), (4, 4, 64, 40), (64, 1, 0, 40)])
+def test_starts_that_do_not_ascend(heads, kv, shared, most):
+    """sequences that claim one another's tokens, in more row tiles than the tokens make: nothing is written outside the rows and the workspace"""
+    rng = np.random.default_rng(heads)
+    n = 60
+    b = TreeBatch(rng, drafts(rng, [most] + [1] * (n - 1), 5), lens=[most + 200] + [200 + s for s in range(1, n)], heads=heads, kv=kv, shared=shared, pad=30)
+    with Dev() as d:
+        a = b.upload(d)
+        last = b.ntok - 30
+        for start in ([0, last] * (n // 2) + [last], [last] * n + [0], [0] + [last - 3 * s for s in range(n)], [0, 2 ** 31 - 1, -2 ** 31, last] * (n // 4) + [last]):
+            d.write(a.qstart, np.array(start[:n + 1], np.int32))
+            for fill in (0, 0x7f, 0xff):
+                d.write(a.ws, np.full(a.ws_bytes, fill, np.uint8))
+                M.check(d.lib.mmoe_attn_tree(a, b.cache, b.p_bits, b.words), "attention")
+                raw = d.get(b.p_out, b.out0)
+                body = raw[:, 8:8 + heads * 136].reshape(b.ntok, heads, 136)
+                assert (raw[:, :8] == 0x1234).all() and (raw[:, 8 + heads * 136:] == 0x1234).all() and (body[:, :, 128:] == 0x1234).all()
+                assert np.array_equal(d.get(a.ws + a.ws_bytes, b.ws_guard), b.ws_guard), "written behind the workspace"
+
+
 def test_drafts_past_32_bits():
     """a cache whose blocks lie 2^25 values apart: the last one begins at byte 8.6e9"""
     rng = np.random.default_rng(8)
