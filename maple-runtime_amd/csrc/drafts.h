@@ -3,11 +3,11 @@
 #pragma once
 #include "paged.h"
 
-// Where sequence s's new tokens begin and how many they are, inside the arrays whatever qstart holds
-struct NewTokens { int t0, n; };
-__device__ __forceinline__ NewTokens new_tokens(const int32_t *qstart, int s, int ntok) {
-    const int t0 = min(max(qstart[s], 0), ntok), t1 = min(max(qstart[s + 1], t0), ntok);
-    return {t0, t1 - t0};
+// Where sequence s's new tokens begin and how many of them lie inside the arrays, whatever qstart holds; what was cached before all of them
+struct NewTokens { int t0, n, ctx; };
+__device__ __forceinline__ NewTokens new_tokens(const int32_t *qstart, const int32_t *len, int s, int ntok) {
+    const int t0 = min(max(qstart[s], 0), ntok), t1 = max(qstart[s + 1], t0);
+    return {t0, min(t1, ntok) - t0, len[s] - (t1 - t0)};
 }
 
 // ------------------------------------------------------------------------------------------------------
@@ -20,8 +20,8 @@ template <int W>
 __global__ void __launch_bounds__(64 * W) k_tree_plan(mmoe_tree_plan_args a) {
     __shared__ uint64_t sees[W][64 * W];
     const int s = blockIdx.x, i = threadIdx.x, l = i & 63, wave = __builtin_amdgcn_readfirstlane(i >> 6);
-    const NewTokens q = a.nseq ? new_tokens(a.qstart, s, a.ntok) : NewTokens{0, 0};
-    const int n = min(q.n, 64 * a.words), ctx = a.nseq ? a.len[s] - q.n : 0;
+    const NewTokens q = a.nseq ? new_tokens(a.qstart, a.len, s, a.ntok) : NewTokens{0, 0, 0};
+    const int n = min(q.n, 64 * a.words);
     int out = -1;   // the node of an earlier word
     if (i < n) out = a.parent[q.t0 + i];
     if (out >= i) out = -1;
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(64 * W) k_tree_plan(mmoe_tree_plan_args a) {
 #pragma unroll
     for (int w = 0; w < W; w++) depth += __popcll(b[w]);
     if (i < n) {
-        a.pos[q.t0 + i] = ctx + depth;
+        a.pos[q.t0 + i] = q.ctx + depth;
 #pragma unroll
         for (int w = 0; w < W; w++) if (w < a.words) a.bits[(int64_t)(q.t0 + i) * a.words + w] = b[w];
     }
@@ -73,8 +73,8 @@ __global__ void __launch_bounds__(64 * W) k_tree_plan(mmoe_tree_plan_args a) {
 __global__ void __launch_bounds__(128) k_tree_accept(mmoe_tree_accept_args a) {
     __shared__ int child[MMOE_TREE_MAX];
     const int s = blockIdx.x;
-    const NewTokens q = new_tokens(a.qstart, s, a.ntok);
-    const int n = min(q.n, MMOE_TREE_MAX), ctx = a.len[s] - q.n;
+    const NewTokens q = new_tokens(a.qstart, a.len, s, a.ntok);
+    const int n = min(q.n, MMOE_TREE_MAX);
     for (int i = threadIdx.x; i < n; i += 128) child[i] = INT32_MAX;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += 128) {
@@ -85,12 +85,12 @@ __global__ void __launch_bounds__(128) k_tree_accept(mmoe_tree_accept_args a) {
     if (threadIdx.x) return;
     int count = 0, last = 0;
     for (int i = 0; i < n; i = child[i]) {   // (a child lies behind its parent: the walk ends)
-        a.kept[q.t0 + count++] = ctx + i;
+        a.kept[q.t0 + count++] = q.ctx + i;
         last = i;
     }
     a.count[s] = count;
     a.last[s] = n ? a.next[q.t0 + last] : -1;
-    a.ctx[s] = ctx + count;
+    a.ctx[s] = q.ctx + count;
 }
 
 // ------------------------------------------------------------------------------------------------------

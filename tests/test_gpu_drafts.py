@@ -307,6 +307,23 @@ def test_accept_where_parents_are_none():
         assert np.array_equal(w, g)
 
 
+def test_tokens_past_the_arrays():
+    """a last sequence of which only some tokens lie inside the arrays: their positions are those that mmoe_attn_tree takes them to have"""
+    rng = np.random.default_rng(7)
+    qstart, length, ntok = np.array([0, 20, 50]), np.array([70, 130]), 41
+    parent = np.array(tree(rng, 20, 3) + tree(rng, 30, 3), np.int64)
+    pos, bits = tree_plan(qstart, length, parent, 1, 50)
+    got = run_tree_plan(qstart, length, parent[:ntok], 1, ntok)
+    assert np.array_equal(got[0], pos[:ntok]) and np.array_equal(got[1], bits[:ntok]) and pos[20] == 100
+    token = np.arange(50)                       # only what lies inside is ever the model's choice
+    choice = np.concatenate([np.full(20, 99), np.where(np.arange(20, 50) + 1 < ntok, np.arange(21, 51), 99)])
+    parent[20:] = np.arange(-1, 29)
+    want, out = accept(qstart, length, parent, token, choice, np.full(50, -77)), run_accept(qstart, length, parent[:ntok], token[:ntok], choice[:ntok])
+    assert want[1].tolist() == [1, 21] and np.array_equal(out[0], want[0][:ntok])
+    for w, g in zip(want[1:], out[1:]):
+        assert np.array_equal(w, g)
+
+
 # ---------------------------------------------------------------------------------------------------- the operators together
 class Drafting:
     """A server that drafts: sequences whose next tokens are trees, accepted by a model that is a table of what follows what. Two layers' caches;
