@@ -412,7 +412,8 @@ int mmoe_tree_plan(const mmoe_tree_plan_args *a);
  *   cached positions p:  max(lo[t], pos - window) <= p < ctx;   new tokens j <= i (at position ctx + j) whose bit is set, whatever the window
  * where pos = ctx + the number of its bits below i, and slopes count |pos - p| to a cached position and, to token j < i, one and the bits
  * between j and i (on mmoe_tree_plan's bits: the steps along the path). bits[ntok][words] need not be a tree's: any bits do; those past i count
- * for nothing. hi must be NULL and max_q at most 64 words. mmoe_attn_tree_ws: as mmoe_attn_paged_ws. */
+ * for nothing. hi must be NULL and max_q at most 64 words. The workspace's size (0: arguments that are refused) follows from the tokens, sequences and
+ * heads, not from max_len; its content does not matter, calls that may run at the same time need one each. */
 size_t mmoe_attn_tree_ws(const mmoe_attn_args *a, const mmoe_kv_cache *kv, const uint64_t *bits, int words);
 int mmoe_attn_tree(const mmoe_attn_args *a, const mmoe_kv_cache *kv, const uint64_t *bits, int words);
 
@@ -472,7 +473,7 @@ int mmoe_kv_copy(const mmoe_kv_copy_args *a, const mmoe_kv_cache *kv, int layers
  * those. A block that others hold (holders NULL: none is) loses a holder; one that nobody holds any more goes to the end of the list, blocks in the order
  * in which their last holders lie in the tables. Ids that are no blocks of the cache are left out. A sequence whose kept positions would
  * end inside a block that others hold as the call begins, so that its next tokens would be written into it, keeps all (len[s] = ctx[s]: fork it at that length instead).
- * len may be ctx or keep, and nfree_out may be nfree. */
+ * len may be ctx or keep, and nfree_out may be nfree. nseq * width at most 2^30. */
 typedef struct {
     const int32_t *ctx, *keep, *table, *nfree;
     int32_t *len, *free_list, *nfree_out, *holders;

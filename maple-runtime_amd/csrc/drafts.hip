@@ -223,6 +223,7 @@ int mmoe_kv_free(const mmoe_kv_free_args *p) {
     if (!p) REFUSE("mmoe_kv_free: no arguments");
     const mmoe_kv_free_args &a = *p;
     if (check_tables("mmoe_kv_free", a.nseq, a.width, a.nblocks, a.block_size, a.shared)) return -1;
+    if ((int64_t)a.nseq * a.width > MAX_LEN) REFUSE("mmoe_kv_free: %d tables of %d blocks: more than 2^30 places", a.nseq, a.width);
     if (!a.nfree || !a.nfree_out || (a.nseq && (!a.ctx || !a.keep || !a.table || !a.len)) || (a.nblocks && !a.free_list)) REFUSE("mmoe_kv_free: a pointer is missing");
     if (mm_ready()) return -1;
     OnDevice dev;

@@ -106,7 +106,7 @@ def test_fork_refusals(kw, word):
     refused(M.lib().mmoe_kv_fork(M.KvFork(**dict(a, **kw))), word)
 
 
-@pytest.mark.parametrize("kw,word", TABLES + [(dict(keep=None), b"pointer"), (dict(len=None), b"pointer")])
+@pytest.mark.parametrize("kw,word", TABLES + [(dict(keep=None), b"pointer"), (dict(len=None), b"pointer"), (dict(nseq=4096, width=(1 << 18) + 1), b"places")])
 def test_free_refusals(kw, word):
     a = dict(ctx=P, keep=P, table=P, nfree=P, len=P, free_list=P, nfree_out=P, nseq=2, width=4, nblocks=10, block_size=16)
     refused(M.lib().mmoe_kv_free(M.KvFree(**dict(a, **kw))), word)
