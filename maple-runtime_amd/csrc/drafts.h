@@ -15,14 +15,17 @@ __device__ __forceinline__ NewTokens new_tokens(const int32_t *qstart, const int
 // ------------------------------------------------------------------------------------------------------
 // A workgroup per sequence, a wave per word of 64 nodes, a lane per node. Within a word by steps that double (what a node's 2^i-th ancestor
 // follows, it follows), through the lanes: six steps at most, which leave each node the ancestors of its own word and the node of an earlier word
-// that the last of them follows, if any. Then word by word: that node's bits are whole by then.
+// that the last of them follows, if any. From there every node goes from word to word by itself, through LDS. A wave's rows of bits lie one behind
+// the other and are written so.
 template <int W>
 __global__ void __launch_bounds__(64 * W) k_tree_plan(mmoe_tree_plan_args a) {
-    __shared__ uint64_t sees[W][64 * W];
+    __shared__ uint64_t words[W * 64];       // each node's bits of its own word
+    __shared__ int outs[W * 64];             // and the node of an earlier word
+    __shared__ uint64_t rows[W][W * 64];     // a wave's rows as they are written
     const int s = blockIdx.x, i = threadIdx.x, l = i & 63, wave = __builtin_amdgcn_readfirstlane(i >> 6);
     const NewTokens q = a.nseq ? new_tokens(a.qstart, a.len, s, a.ntok) : NewTokens{0, 0, 0};
     const int n = min(q.n, 64 * a.words);
-    int out = -1;   // the node of an earlier word
+    int out = -1;
     if (i < n) out = a.parent[q.t0 + i];
     if (out >= i) out = -1;
     int to = out - 64 * wave;   // in the word: its lane
@@ -34,25 +37,31 @@ __global__ void __launch_bounds__(64 * W) k_tree_plan(mmoe_tree_plan_args a) {
         if (to >= 0) { own |= more; to = next; out = past; }
     }
     uint64_t b[W] = {};
-#pragma unroll
-    for (int v = 0; v < W; v++) {
-        if (W > 1 && v) __syncthreads();
-        if (wave != v) continue;
-        if (out >= 0)
-#pragma unroll
-            for (int w = 0; w < v; w++) b[w] = w <= out >> 6 ? sees[w][out] : 0;
-        b[v] = own;
-        if (v + 1 < W)
-#pragma unroll
-            for (int w = 0; w <= v; w++) sees[w][i] = b[w];
+    if (W > 1) {
+        words[i] = own; outs[i] = out;
+        __syncthreads();
     }
-    int depth = -1;
+    int depth = __popcll(own) - 1;
 #pragma unroll
-    for (int w = 0; w < W; w++) depth += __popcll(b[w]);
-    if (i < n) {
-        a.pos[q.t0 + i] = q.ctx + depth;
+    for (int w = W - 1; w >= 0; w--) {
+        if (w == wave) b[w] = own;
+        if (w < wave && out >= 64 * w) {
+            b[w] = words[out]; out = outs[out];
+            depth += __popcll(b[w]);
+        }
+    }
+    if (i < n) a.pos[q.t0 + i] = q.ctx + depth;
+    // row by row, `words` words each; the places of a row turned by its number, so that the lanes' places lie in different banks
+    const int per = a.words, live = min(max(n - 64 * wave, 0), 64) * per;
 #pragma unroll
-        for (int w = 0; w < W; w++) if (w < a.words) a.bits[(int64_t)(q.t0 + i) * a.words + w] = b[w];
+    for (int w = 0; w < W; w++) rows[wave][l * W + ((w + l) & (W - 1))] = b[w];
+    __builtin_amdgcn_wave_barrier();
+    const unsigned by = (65536 + per - 1) / per;   // x / per for x < 512
+    uint64_t *bits = a.bits + (int64_t)(q.t0 + 64 * wave) * per;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        const int x = 64 * w + l, r = (int)(x * by >> 16), c = x - r * per;
+        if (x < live) bits[x] = rows[wave][r * W + ((c + r) & (W - 1))];
     }
     // nodes past the words, and tokens of no sequence
     for (int t = q.t0 + n + i; t < q.t0 + q.n; t += 64 * W) {
