@@ -823,6 +823,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
     for (int i = 0; i < DS; i++) va[i] = vr * RB + ((64 * i + 32 * ((l >> 4) & 1) + 8 * (l & 3)) ^ ((vr & (CH / 2 - 1)) << 5));
     f16v acc[DS], sc[NU];
     float m, mb, sum;   // mb: m - lift, - lift while m is -inf
+    float shift = 0.0f; // of the tile's scores (TREE with a bias: the row's distance to the tile, the same for every position of it)
     bool far;           // a maximum of the wave is past ATT_FAR
     constexpr bool FALLS = CAP && !BIAS;   // sc falls as the score grows
     constexpr float NONE = FALLS ? __builtin_inff() : -__builtin_inff();   // sc of a position that is not seen
@@ -845,6 +846,8 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
     auto math = [&](f16v *s, int p) {
         const float dist = BIAS ? (float)(R.pos - p - 4 * hh) : 0.0f;
         const bool path = TREE && BIAS && p + BN > inhi;   // drafted tokens among the tile's positions
+        // else every position lies before the row's own: the distance is the tile's less the place in it
+        if (TREE && BIAS) shift = path ? 0.0f : -slope * dist;
 #pragma unroll
         for (int u = 0; u < NU; u++) {
             TreeFar far;
@@ -855,7 +858,8 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
                 float x = s[u][j];
                 if (CAP) x = __builtin_amdgcn_rcpf(1.0f + exp2_(x * A.s1));   // tanh z = 1 - 2 / (1 + exp 2 z)
                 if (CAP && BIAS) x = fmaf(-2.0f * A.s2, x, A.s2);
-                if (BIAS) x = fmaf(-slope, path ? tree_distance(far, at) : fabsf(dist - (float)(32 * u + at)), x);
+                if (TREE && BIAS) x = path ? fmaf(-slope, tree_distance(far, at), x) : fmaf(slope, (float)(32 * u + at), x);
+                else if (BIAS) x = fmaf(-slope, fabsf(dist - (float)(32 * u + at)), x);
                 s[u][j] = x;
             }
         }
@@ -884,6 +888,17 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
     auto largest = [&](const f16v *s) {
         float top[4];   // no chain of 32
         auto higher = [](float x, float y) { return FALLS ? min_(x, y) : max_(x, y); };
+        if (TREE) {   // three to an instruction (a score that is NaN makes the maximum NaN: the row's result is that anyway)
+            auto of3 = [](float x, float y, float z) {
+                return FALLS ? __builtin_elementwise_minimum(__builtin_elementwise_minimum(x, y), z) : __builtin_elementwise_maximum(__builtin_elementwise_maximum(x, y), z);
+            };
+#pragma unroll
+            for (int i = 0; i < 4; i++) top[i] = of3(s[0][3 * i], s[0][3 * i + 1], s[0][3 * i + 2]);
+            top[0] = of3(top[0], s[0][12], s[0][13]); top[1] = of3(top[1], s[0][14], s[0][15]);
+#pragma unroll
+            for (int i = 2; i < 8 * NU - 6; i++) top[i & 3] = of3(top[i & 3], s[(2 * i + 12) / 16][(2 * i + 12) % 16], s[(2 * i + 13) / 16][(2 * i + 13) % 16]);
+            return max_halves(fmaf(of3(of3(top[0], top[1], top[2]), top[3], top[3]), s1, BIAS ? fmaf(shift, s1, s0) : s0));
+        }
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll
@@ -916,7 +931,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
         __builtin_amdgcn_sched_barrier(0);
         u4 pf[NK];
         float part = 0;
-        const float mul = far ? 1.0f : s1, off = far ? -mb : s0 - mb;
+        const float mul = far ? 1.0f : s1, off = far ? -mb : TREE && BIAS ? fmaf(shift, s1, s0 - mb) : s0 - mb;
 #pragma unroll
         for (int u = 0; u < NU; u++)
 #pragma unroll
@@ -1024,7 +1039,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
 #pragma unroll
                     for (int u = 0; u < NU; u++)
 #pragma unroll
-                        for (int j = 0; j < 16; j++) sc[u][j] = fmaf(sc[u][j], s1, s0);
+                        for (int j = 0; j < 16; j++) sc[u][j] = fmaf(sc[u][j], s1, TREE && BIAS ? fmaf(shift, s1, s0) : s0);
                 }
                 __builtin_amdgcn_s_setprio(1);
                 product(vbuf);
