@@ -15,8 +15,9 @@ __device__ __forceinline__ NewTokens new_tokens(const int32_t *qstart, const int
 // ------------------------------------------------------------------------------------------------------
 // A workgroup per sequence, a wave per word of 64 nodes, a lane per node. Within a word by steps that double (what a node's 2^i-th ancestor
 // follows, it follows), through the lanes: six steps at most, which leave each node the ancestors of its own word and the node of an earlier word
-// that the last of them follows, if any. From there every node goes from word to word by itself, through LDS. A wave's rows of bits lie one behind
-// the other and are written so.
+// that the last of them follows, if any. From there every node goes from word to word by itself, through LDS (word by word for all nodes at once, with a
+// barrier for each: 7.3 us instead of 4.9 below). A wave's rows of bits lie one behind the other and are written so. Bound by latency: the launch,
+// the tree's place, its parents, the steps. Measured: 64 trees of 10 to 40 nodes 4.1 us, 200 of 300 to 512 nodes 4.9 us (5.9 MB, 1.2 TB/s).
 template <int W>
 __global__ void __launch_bounds__(64 * W) k_tree_plan(mmoe_tree_plan_args a) {
     __shared__ uint64_t words[W * 64];       // each node's bits of its own word
@@ -77,8 +78,8 @@ __global__ void __launch_bounds__(64 * W) k_tree_plan(mmoe_tree_plan_args a) {
 // ------------------------------------------------------------------------------------------------------
 // Which drafted tokens stay (mmoe_tree_accept)
 // ------------------------------------------------------------------------------------------------------
-// A workgroup per sequence: every node that is what the model chose behind its parent offers itself to it, the lowest one wins; then the walk from node
-// 0 is a chain of reads from LDS.
+// A workgroup per sequence: every node that is what the model chose behind its parent offers itself to it, the lowest one wins (so the order of the
+// atomics does not matter); then the walk from node 0 is a chain of reads from LDS. Latency: 2.4 to 3.0 us for 5 and for 64 sequences.
 __global__ void __launch_bounds__(128) k_tree_accept(mmoe_tree_accept_args a) {
     __shared__ int child[MMOE_TREE_MAX];
     const int s = blockIdx.x;
@@ -120,7 +121,9 @@ __device__ __forceinline__ int64_t page_at(const PageArgs &P, int block, int at,
 // Kept positions moved together. Entry j goes from k[j] to k[0] + j <= k[j], so that writing it touches the source of no later one: a
 // workgroup goes through the list in steps of as many entries as its threads hold, all of a step read before any is written; positions and blocks of the
 // next step are looked up while this one's values are on their way. A workgroup has `lanes` pieces of every position (of one array), so the
-// arrays and the pieces are what runs side by side.
+// arrays and the pieces are what runs side by side. Bound by memory where lists are long: one sequence of 20000 positions cut to 8000 in 24 layers, 4
+// heads of 128, 786 MB: 171 us, 4.6 TB/s (a copy reaches 5.1); without the look-ups a step ahead 420; with the values a step ahead too, no faster. What
+// a draft leaves behind (64 sequences, a few tokens each, 12.6 MB): 5.7 us, five loads that depend on one another.
 #define KC_U 8
 template <int TH>
 __global__ void __launch_bounds__(TH) k_kv_compact(mmoe_kv_compact_args a, PageArgs P, int lanes, int units, Div by_lanes, Div by_units, Div by_arrays, int arrays) {
@@ -173,6 +176,8 @@ __global__ void __launch_bounds__(TH) k_kv_compact(mmoe_kv_compact_args a, PageA
     }
 }
 
+// A workgroup has KY_U KY_T pieces of 16 bytes of one block of one array, all on their way at once. Bound by memory: 48 begun blocks of a beam
+// search's step in 24 layers, 89 MB: 16 us, 5.5 TB/s with what the caches hold; 32 of 16 positions: 4.5 us, latency.
 #define KY_T 256
 #define KY_U 8
 __global__ void __launch_bounds__(KY_T) k_kv_copy(mmoe_kv_copy_args a, PageArgs P, int units, Div by_units, Div by_arrays, int arrays) {
@@ -200,7 +205,8 @@ __global__ void __launch_bounds__(KY_T) k_kv_copy(mmoe_kv_copy_args a, PageArgs 
 // Copies of sequences (mmoe_kv_fork)
 // ------------------------------------------------------------------------------------------------------
 // One workgroup settles which forks are made and which blocks they take (a prefix sum over them); the rows, which are independent, follow in the
-// same launch or in one of their own.
+// same launch or, where they have more than KO_ONE entries, in one of their own. Latency: the lengths, the list, the rows: 2.8 to 3.4 us for 64 beams and
+// 32 samples (rows by waves 5.3, workgroups of 256 10).
 // columns of a copy's row that are its source's
 __device__ __forceinline__ int fork_cols(const mmoe_kv_fork_args &a, int sh, int n) { return n <= a.shared ? (n + a.block_size - 1) >> sh : n >> sh; }
 __device__ __forceinline__ void fork_put(const mmoe_kv_fork_args &a, int sh, int dst, int c, int b) {
@@ -274,7 +280,9 @@ __global__ void __launch_bounds__(256) k_kv_fork_rows(mmoe_kv_fork_args a, int s
 // ------------------------------------------------------------------------------------------------------
 // What sequences give up, one behind the other, is a list of places in the tables; a block goes back with the last of them that drops it to
 // nobody. Three passes over that list with holders: every place drops a holder; of the places of a block that nobody holds now the last one marks
-// it; the marked ones are appended in order. Sums and marks, not the order of the atomics, decide, so the list comes out the same every time.
+// it; the marked ones are appended in order. Sums and marks, not the order of the atomics, decide, so the list comes out the same every time. One
+// workgroup, since the list is one; latency: 2.2 us for 5 sequences, 3.1 for 64 that give up a draft's blocks, 7.8 for 64 rows of a beam search that
+// give up all of theirs (800 places, three rounds of atomics).
 #define KF_U 4
 template <int PER>
 __global__ void __launch_bounds__(1024) k_kv_free(mmoe_kv_free_args a, int sh) {

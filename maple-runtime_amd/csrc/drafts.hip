@@ -11,7 +11,7 @@ static int check_bits(const char *who, const mmoe_attn_args *p, const mmoe_kv_ca
     return 0;
 }
 
-// How a call of mmoe_attn_tree is divided (drafts.h). Only the values in the arguments count (a captured call keeps its grid). The numbers of
+// How a call of mmoe_attn_tree is divided (attn_tree.h). Only the values in the arguments count (a captured call keeps its grid). The numbers of
 // workgroups are for the 256 compute units of the one device that the kernels are built and were measured for.
 struct TreePlan {
     int room, pieces, slot_waves, tiles;
@@ -24,12 +24,17 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     const int group = a.heads / kv.heads;
     const int64_t rows = (int64_t)a.ntok * group, most = (int64_t)std::min(a.max_q, a.ntok) * group;
     const int64_t own = std::min((int64_t)a.nseq * ((most + ATT_BM - 1) / ATT_BM), rows / ATT_BM + a.nseq), tiles = own + (a.shared ? (rows + ATT_BM - 1) / ATT_BM : 0);
-    // Row tiles of so few positions, and so many of them, that they stay whole: nothing to join
+    // Row tiles of so few positions, and so many of them, that they stay whole: nothing to join (32 drafts of 64 tokens in a window of 512, 256 row tiles:
+    // 25 us, cut 36; 24 drafts, 192: 23.6, cut 29.2; 48 drafts of 4 over 600, 192: 18.9, cut 22.3)
     const int64_t most_steps = (a.window ? std::min<int64_t>(a.max_len, (int64_t)a.window + a.max_q + TREE_BN) : a.max_len) / TREE_BN + 1;
     const bool whole = !a.shared && most_steps <= 12 && tiles * kv.heads >= 192;
-    p.room = whole ? 0 : std::max(1, (kv.head_dim == 64 ? 768 : 512) / kv.heads);   // two workgroups per compute unit, three with heads of 64
+    // What the card holds at once: two workgroups per compute unit, three with heads of 64 (64 drafts of 10 to 40 tokens over 50 to 3000 positions, heads of 128:
+    // 68 us, with 768 pieces 75; 17 drafts behind 2048 shared positions, heads of 64: 32 us, with 512 pieces 37)
+    p.room = whole ? 0 : std::max(1, (kv.head_dim == 64 ? 768 : 512) / kv.heads);
     const int64_t pieces = whole ? tiles : std::max(tiles <= p.room * 3 / 4 ? (int64_t)p.room : 2 * (int64_t)p.room + tiles, tiles), join = own * kv.heads * 4;
-    p.deep = join < 128;   // 32 rows of a key/value head each
+    // Few row tiles, so perhaps many results of each, and few workgroups of 32 rows and a key/value head: eight workgroups for one (26 tokens over 700
+    // positions, 16: 12.5 us instead of 14.6; over 30000 34 instead of 66; 3 drafts of 60 over 3000, 96: 24.7 instead of 26; 16 of 20 over 2000, 256: 28.6 instead of 27.5)
+    p.deep = join < 128;
     p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(pieces * kv.heads + 7, join * (p.deep ? 8 : 1)) * 256 <= (int64_t)MAX_THREADS;
     p.pieces = (int)std::min<int64_t>(pieces, INT32_MAX); p.tiles = (int)std::min<int64_t>(own, INT32_MAX); p.join = (unsigned)(p.deep ? join * 8 : join);
     p.slot_waves = a.shared ? ATT_BM / 32 : (int)std::min<int64_t>(ATT_BM, most + 31) / 32;
@@ -161,8 +166,9 @@ int mmoe_kv_compact(const mmoe_kv_compact_args *p, const mmoe_kv_cache *kv, int 
     if (!a.nseq || !a.nkept) return 0;
     if (!a.table || !a.first || !a.count || !a.kept) REFUSE("mmoe_kv_compact: a pointer is missing");
     const PageArgs P = page_args(kv, layers);
-    // Short lists (a step's accepted tokens): a wave goes through one. Else workgroups of 256 with as many pieces of a position, at least 128 bytes, as
-    // leave 768 of them (4 sequences of 5000, 24 layers, 0.4 kept: 164 us, of 1024 threads 168); where there are not so many, of 1024 threads, from 160 on
+    // Short lists (a step's accepted tokens, a few of those that there is room for): a wave goes through one (64 sequences that drafted 64 tokens: 15.3 us,
+    // by workgroups of 256 17.4; were 60 of them kept, 31 and 20). Else workgroups of 256 with as many pieces of a position, at least 128 bytes, as
+    // leave 768 of them (4 sequences of 5000, 24 layers, 0.4 kept: 167 us, of 1024 threads 171); where there are not so many, of 1024 threads, from 160 on
     // (one sequence of 20000: 171 us, of 256 threads 194, with pieces of 64 bytes 207)
     const int64_t arrays = 2 * layers, lists = a.nseq * arrays;
     auto units_of = [&](int lanes) { return (P.all + lanes - 1) / lanes; };
