@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(1024) k_kv_plan(mmoe_kv_plan_args a, int sh, i
 
 // The tokens of a large step, in a launch of their own over the whole card: 60000 in 2.7 us (their starts into LDS, then a search and two
 // dependent loads; 0.5 MB written)
-static __global__ void __launch_bounds__(256) k_kv_tokens(mmoe_kv_plan_args a, int sh) {
+inline __global__ void __launch_bounds__(256) k_kv_tokens(mmoe_kv_plan_args a, int sh) {
     __shared__ int start[MMOE_KV_MAXSEQ + 1];
     for (int i = threadIdx.x; i <= a.nseq; i += 256) start[i] = a.qstart[i];
     __syncthreads();
