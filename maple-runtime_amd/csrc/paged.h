@@ -247,24 +247,6 @@ __global__ void __launch_bounds__(1024) k_kv_plan(mmoe_kv_plan_args a, int sh, i
     }
 }
 
-// The tokens of a large step, in a launch of their own over the whole card: 60000 in 2.7 us (their starts into LDS, then a search and two
-// dependent loads; 0.5 MB written)
-inline __global__ void __launch_bounds__(256) k_kv_tokens(mmoe_kv_plan_args a, int sh) {
-    __shared__ int start[MMOE_KV_MAXSEQ + 1];
-    for (int i = threadIdx.x; i <= a.nseq; i += 256) start[i] = a.qstart[i];
-    __syncthreads();
-    const int t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= a.ntok) return;
-    int pos = 0, slot = -1;
-    if (t < start[a.nseq]) {
-        const int s = count_le(start, a.nseq, t) - 1;
-        pos = a.len[s] - (start[s + 1] - t);
-        const int blk = a.table[(int64_t)s * a.width + (pos >> sh)];
-        if ((unsigned)blk < (unsigned)a.nblocks) slot = (blk << sh) + (pos & (a.block_size - 1));
-    }
-    a.pos[t] = pos; a.slot[t] = slot;
-}
-
 // ------------------------------------------------------------------------------------------------------
 // Rotary positions and the cache write (mmoe_rope_kv)
 // ------------------------------------------------------------------------------------------------------
