@@ -43,19 +43,17 @@ struct Draft {
     __device__ static __forceinline__ int cut(const Seq &q, float per) {
         return max(min((int)ceilf(fmaf((float)q.steps, per, -0x1p-10f)), max((q.steps + 1) >> 1, 12)), 1);
     }
-    struct Mem { int sum[2][4], at[4]; };
+    struct Mem { int sum[3][4], at[4]; };
     __device__ static __forceinline__ int wave_sum(int v) { return wave_reduce(v, [](int x, int y) { return x + y; }); }
-    struct Piece { int id, kvh, seq, base, tiles, own_tiles, shared_k, shared_tiles, k; Seq q; };
-    // The workgroup's piece: its number and key/value head, its sequence (-1: the shared positions), that one's first piece and row tile, how many row
-    // tiles the sequences have in all, the pieces of a row tile over the shared positions, their row tiles, the pieces of this row tile; false: none. The
-    // same for every thread of the workgroup (256).
-    __device__ static __forceinline__ bool find(const AttArgs &A, Mem &M, Piece &o) {
+    // Pieces per step; how many pieces there are, row tiles of the sequences and over the shared positions, pieces of one of the latter (which come first)
+    struct Cut { float per; int pieces, own_tiles, shared_tiles, shared_k; };
+    // The same for every thread of the workgroup (256). MANY: more than 64 sequences, else every wave does it by itself
+    template <bool MANY> __device__ static __forceinline__ Cut plan(const AttArgs &A, Mem &M) {
         const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, n = A.a.nseq;
-        const Seq sh = of_shared(A), q = of(A, n <= 64 ? l : tid);
-        // a sum over all sequences: every wave by itself, or all of them together
+        const Seq sh = of_shared(A), q = of(A, MANY ? tid : l);
         auto total = [&](auto &&f) {
             int v = f(q);
-            if (n <= 64) return wave_sum(v);
+            if (!MANY) return wave_sum(v);
             for (int s = tid + 256; s < n; s += 256) v += f(of(A, s));
             v = wave_sum(v);
             __syncthreads();
@@ -63,9 +61,11 @@ struct Draft {
             __syncthreads();
             return M.sum[0][0] + M.sum[0][1] + M.sum[0][2] + M.sum[0][3];
         };
-        o.own_tiles = total([](const Seq &x) { return x.tiles; });
-        const int all_tiles = sh.tiles + o.own_tiles;
-        float per = 0.0f;   // pieces per step
+        Cut c;
+        c.own_tiles = total([](const Seq &x) { return x.tiles; });
+        c.shared_tiles = sh.tiles;
+        const int all_tiles = sh.tiles + c.own_tiles;
+        float per = 0.0f;
         int pieces = all_tiles;
         if (A.room) {
             // (the host has seen to it that all steps are a 32-bit number)
@@ -82,49 +82,53 @@ struct Draft {
             }
         }
         if (pieces == 0 && A.room && blockIdx.x == 0 && tid == 0) A.tile_at[0] = {};   // the workspace may hold an earlier call's
-        // Workgroups go to the card's dies in turn: each die a run of consecutive pieces, in which the row tiles of the same positions lie side by
-        // side and read them from the die's own cache
-        const int all = pieces * A.kv.heads, each = (all + 7) >> 3, at = (int)(blockIdx.x & 7) * each + (int)(blockIdx.x >> 3);
-        if ((int)(blockIdx.x >> 3) >= each || at >= all) return false;
-        o.kvh = at / pieces;
-        const int id = o.id = at - o.kvh * pieces;
-        o.seq = -1; o.base = 0; o.tiles = 0; o.k = o.shared_k = cut(sh, per); o.shared_tiles = sh.tiles; o.q = sh;
-        const int common = sh.tiles * o.k;
-        if (id < common) return true;
-        if (n <= 64) {
-            const int mine = q.tiles * cut(q, per), end = common + (int)scan_wave(mine), tiles = (int)scan_wave(q.tiles) - q.tiles;
+        c.per = per; c.pieces = pieces; c.shared_k = cut(sh, per);
+        return c;
+    }
+    // A piece: its sequence (-1: the shared positions), that one's first piece, first result and row tile, the pieces of its row tile
+    struct Piece { int seq, base, result, tiles, k; Seq q; };
+    template <bool MANY> __device__ static __forceinline__ bool piece(const AttArgs &A, Mem &M, const Cut &c, int id, Piece &o) {
+        const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, n = A.a.nseq, common = c.shared_tiles * c.shared_k;
+        if (id < common) {
+            o = {-1, 0, 0, 0, c.shared_k, of_shared(A)};
+            return true;
+        }
+        if (!MANY) {   // (a result for every piece)
+            const Seq q = of(A, l);
+            const int mine = q.tiles * cut(q, c.per), end = common + (int)scan_wave(mine), tiles = (int)scan_wave(q.tiles) - q.tiles;
             const int s = __popcll(__ballot(id >= end));   // a prefix of the lanes
             if (s >= n) return false;
             auto lane = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
-            o.seq = s; o.base = lane(end - mine); o.tiles = lane(tiles);
+            o.seq = s; o.base = o.result = lane(end - mine); o.tiles = lane(tiles);
             o.q = {lane(q.t0), lane(q.t1), lane(q.len), lane(q.rows), lane(q.tiles), lane(q.from), lane(q.to), lane(q.steps)};
-            o.k = cut(o.q, per);
+            o.k = cut(o.q, c.per);
             return true;
         }
-        int before = common, tiles = 0;
+        int before = common, tiles = 0, results = common;
         if (tid == 0) M.at[0] = -1;
         for (int s0 = 0; s0 < n; s0 += 256) {
             const Seq x = of(A, s0 + tid);
-            const int mine = x.tiles * cut(x, per);
-            int end = (int)scan_wave(mine), t = (int)scan_wave(x.tiles);
+            const int k = cut(x, c.per), mine = x.tiles * k, kept = k > 1 || A.a.shared ? mine : 0;
+            int end = (int)scan_wave(mine), t = (int)scan_wave(x.tiles), r = (int)scan_wave(kept);
             __syncthreads();   // the sums before have been read
-            if (l == 63) { M.sum[0][w] = end; M.sum[1][w] = t; }
+            if (l == 63) { M.sum[0][w] = end; M.sum[1][w] = t; M.sum[2][w] = r; }
             __syncthreads();
-            int ps = 0, ts = 0;
+            int ps = 0, ts = 0, rs = 0;
             for (int i = 0; i < 4; i++) {
-                if (i < w) { end += M.sum[0][i]; t += M.sum[1][i]; }
-                ps += M.sum[0][i]; ts += M.sum[1][i];
+                if (i < w) { end += M.sum[0][i]; t += M.sum[1][i]; r += M.sum[2][i]; }
+                ps += M.sum[0][i]; ts += M.sum[1][i]; rs += M.sum[2][i];
             }
-            end += before; t += tiles;
-            if (id < end && id >= end - mine) { M.at[0] = s0 + tid; M.at[1] = end - mine; M.at[2] = t - x.tiles; }
-            before += ps; tiles += ts;
+            end += before; t += tiles; r += results;
+            if (id < end && id >= end - mine) { M.at[0] = s0 + tid; M.at[1] = end - mine; M.at[2] = t - x.tiles; M.at[3] = r - kept; }
+            before += ps; tiles += ts; results += rs;
             if (id < before) break;
         }
         __syncthreads();
         o.seq = __builtin_amdgcn_readfirstlane(M.at[0]); o.base = __builtin_amdgcn_readfirstlane(M.at[1]); o.tiles = __builtin_amdgcn_readfirstlane(M.at[2]);
+        o.result = __builtin_amdgcn_readfirstlane(M.at[3]);
         if (o.seq < 0) return false;
         o.q = of(A, o.seq);
-        o.k = cut(o.q, per);
+        o.k = cut(o.q, c.per);
         return true;
     }
 };
@@ -138,30 +142,45 @@ struct Draft {
 // to 30000, capped: 173 us, 0.71 PFLOP/s, the matrix products beside three exponentials' work; 32 drafts of 64 in a window of 512: 24.6 us, whole row
 // tiles, one wave per SIMD: 10 steps of 3450 cycles behind 14000 of dependent loads; 17 drafts behind 2048 shared positions, heads of 64 with slopes:
 // 32.2 us, the exponentials and the sums beside them (seven and a half operations a score); one draft of 26 over 700: 12.5 us, latency.
-template <int T, int D, bool CAP, bool BIAS>
+// MANY: of more than 64 sequences most may be without tokens, so that there is a bound on the pieces far above their number: a workgroup takes more than
+// one, one after the other, where there are more than the launch has workgroups.
+template <int T, int D, bool CAP, bool BIAS, bool MANY>
 __global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
     __shared__ AttTileMem<D, TREE_BN> M;
     __shared__ Draft::Mem F;
-    Draft::Piece o;
-    if (!Draft::find(A, F, o)) return;
-    const Draft::Seq &q = o.q;
-    const int k = __builtin_amdgcn_readfirstlane(o.k), steps = __builtin_amdgcn_readfirstlane(q.steps), i = (o.id - o.base) / q.tiles, tile = o.id - o.base - i * q.tiles;
-    if (o.id >= A.most_pieces || (o.seq >= 0 && o.tiles + tile >= A.most_tiles)) return;   // (not if qstart ascends)
-    if (A.room && o.kvh == 0 && i == 0 && threadIdx.x == 0) {
-        if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {o.id, k, q.tiles, q.t0, tile * ATT_BM, q.rows};
-        if (o.id == 0) A.tile_at[0] = {min(o.own_tiles, A.most_tiles), o.shared_k, o.shared_tiles, 0, 0, 0};
+    const Draft::Cut c = Draft::plan<MANY>(A, F);
+    // Workgroups go to the card's dies in turn: each die a run of consecutive pieces, in which the row tiles of the same positions lie side by
+    // side and read them from the die's own cache
+    const int all = c.pieces * A.kv.heads, each = (all + 7) >> 3;
+    for (int y = blockIdx.x >> 3; y < each; y += gridDim.x >> 3) {
+        const int at = (int)(blockIdx.x & 7) * each + y, kvh = at / c.pieces, id = at - kvh * c.pieces;
+        Draft::Piece o;
+        if (at >= all || !Draft::piece<MANY>(A, F, c, id, o)) return;
+        const Draft::Seq &q = o.q;
+        const int k = __builtin_amdgcn_readfirstlane(o.k), steps = __builtin_amdgcn_readfirstlane(q.steps), i = (id - o.base) / q.tiles, tile = id - o.base - i * q.tiles;
+        const bool whole = k == 1 && !A.a.shared;
+        const int result = o.result + (id - o.base);
+        // (both fit if qstart ascends)
+        if ((whole || result < A.most_results) && (o.seq < 0 || o.tiles + tile < A.most_tiles)) {
+            if (A.room && kvh == 0 && i == 0 && threadIdx.x == 0) {
+                if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {result, k, q.tiles, q.t0, tile * ATT_BM, q.rows};
+                if (id == 0) A.tile_at[0] = {min(c.own_tiles, A.most_tiles), c.shared_k, c.shared_tiles, 0, 0, 0};
+            }
+            const int len = steps / k, more = steps - len * k;   // the first of them a step longer
+            AttWork work = {};
+            work.shared = o.seq < 0;
+            work.at = {max(o.seq, 0), tile * ATT_BM, q.rows, q.t0};
+            work.t1 = q.t1; work.len = q.len;
+            work.kvh = kvh;
+            work.p0 = q.from + (i * len + min(i, more)) * TREE_BN;
+            work.p1 = min(work.p0 + (len + (i < more)) * TREE_BN, q.to);
+            work.whole = whole;
+            work.slot = (int64_t)result * A.kv.heads + kvh;
+            att_tile<T, D, CAP, BIAS, true>(tree_args(), work, M);
+        }
+        if (!MANY) return;
+        __syncthreads();   // every wave is done with LDS
     }
-    const int each = steps / k, more = steps - each * k;
-    AttWork work = {};
-    work.shared = o.seq < 0;
-    work.at = {max(o.seq, 0), tile * ATT_BM, q.rows, q.t0};
-    work.t1 = q.t1; work.len = q.len;
-    work.kvh = o.kvh;
-    work.p0 = q.from + (i * each + min(i, more)) * TREE_BN;
-    work.p1 = min(work.p0 + (each + (i < more)) * TREE_BN, q.to);
-    work.whole = k == 1 && !A.a.shared;
-    work.slot = (int64_t)o.id * A.kv.heads + o.kvh;
-    att_tile<T, D, CAP, BIAS, true>(tree_args(), work, M);
 }
 
 // The partial results of a row tile put together, 32 rows by a workgroup: each result holds its values over its own sum, its maximum (in units of log 2)
@@ -186,14 +205,14 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
     const TreeTile head_of = A.tile_at[0], t = A.tile_at[1 + tile];
     if (tile >= head_of.slot || (t.parts == 1 && !a.shared)) return;   // none, or written by the piece that was all of it
     // nothing outside the arrays, whatever qstart holds (where it does not ascend, row tiles may be those of an earlier call)
-    if (w >= A.slot_waves || t.row0 >= t.rows || t.slot < 0 || t.parts < 1 || t.apart < 0 || t.slot + (t.parts - 1) * (int64_t)t.apart >= A.most_pieces || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
+    if (w >= A.slot_waves || t.row0 >= t.rows || t.slot < 0 || t.parts < 1 || t.apart < 0 || t.slot + (t.parts - 1) * (int64_t)t.apart >= A.most_results || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
     const int r = t.row0 + w * 32 + n;
     if (t.row0 + w * 32 >= t.rows) return;
     const bool live = r < t.rows;
     const int row = min(r, t.rows - 1), j = (int)A.by_group(row), tok = t.t0 + j, head = kvh * A.group + row - j * A.group;
     // the shared positions' row tiles hold every token's rows
     const int common = a.shared ? head_of.parts : 0, rs = tok * A.group + row - j * A.group, slot_sh = rs / ATT_BM, at_sh = rs % ATT_BM;
-    if (a.shared && (common < 0 || head_of.apart < 0 || slot_sh + (common - 1) * (int64_t)head_of.apart >= A.most_pieces)) return;
+    if (a.shared && (common < 0 || head_of.apart < 0 || slot_sh + (common - 1) * (int64_t)head_of.apart >= A.most_results)) return;
     const int parts = common + t.parts;
     struct Result { float2 v; f4 y[C]; };
     auto load = [&](Result &x, int p) {

@@ -14,9 +14,9 @@ static int check_bits(const char *who, const mmoe_attn_args *p, const mmoe_kv_ca
 // How a call of mmoe_attn_tree is divided (attn_tree.h). Only the values in the arguments count (a captured call keeps its grid). The numbers of
 // workgroups are for the 256 compute units of the one device that the kernels are built and were measured for.
 struct TreePlan {
-    int room, pieces, slot_waves, tiles;
-    unsigned join;
-    bool deep, fits;
+    int room, most_results, slot_waves, tiles;
+    unsigned wgs, join;
+    bool many, deep, fits;
     size_t results, bytes;
 };
 static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
@@ -30,15 +30,24 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     const bool whole = !a.shared && most_steps <= 12 && tiles * kv.heads >= 192;
     // What the card holds at once: two workgroups per compute unit, three with heads of 64 (64 drafts of 10 to 40 tokens over 50 to 3000 positions, heads of 128:
     // 68 us, with 768 pieces 75; 17 drafts behind 2048 shared positions, heads of 64: 32 us, with 512 pieces 37)
-    p.room = whole ? 0 : std::max(1, (kv.head_dim == 64 ? 768 : 512) / kv.heads);
+    const int once = kv.head_dim == 64 ? 768 : 512;
+    p.room = whole ? 0 : std::max(1, once / kv.heads);
     const int64_t pieces = whole ? tiles : std::max(tiles <= p.room * 3 / 4 ? (int64_t)p.room : 2 * (int64_t)p.room + tiles, tiles), join = own * kv.heads * 4;
     // Few row tiles, so perhaps many results of each, and few workgroups of 32 rows and a key/value head: eight workgroups for one (26 tokens over 700
     // positions, 16: 12.5 us instead of 14.6; over 30000 34 instead of 66; 3 drafts of 60 over 3000, 96: 24.7 instead of 26; 16 of 20 over 2000, 256: 28.6 instead of 27.5)
     p.deep = join < 128;
-    p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(pieces * kv.heads + 7, join * (p.deep ? 8 : 1)) * 256 <= (int64_t)MAX_THREADS;
-    p.pieces = (int)std::min<int64_t>(pieces, INT32_MAX); p.tiles = (int)std::min<int64_t>(own, INT32_MAX); p.join = (unsigned)(p.deep ? join * 8 : join);
+    p.many = a.nseq > 64;
+    // Of up to 64 sequences a workgroup for each piece that there may be. Of more a workgroup for each that the card holds at once: 64 drafts of 20 tokens in
+    // a batch of 1024 (4096) sequences, the others without, 54 (79) us instead of 76 (374); 256 drafts of 4 over 1500, all there, 155 instead of 149
+    const int64_t wgs = std::min((pieces * kv.heads + 7) & ~(int64_t)7, p.many ? (int64_t)once : INT64_MAX);
+    p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(wgs, join * (p.deep ? 8 : 1)) * 256 <= (int64_t)MAX_THREADS;
+    p.wgs = (unsigned)wgs; p.tiles = (int)std::min<int64_t>(own, INT32_MAX); p.join = (unsigned)(p.deep ? join * 8 : join);
+    // Results: one for each piece, but of many sequences' only those of row tiles that are cut (each of at least two pieces, which a cut into 2 room
+    // parts makes less than 4 room of)
+    const int64_t results = whole ? 0 : p.many && !a.shared ? std::min(pieces, (int64_t)4 * p.room) : pieces;
+    p.most_results = (int)std::min<int64_t>(results, INT32_MAX);
     p.slot_waves = a.shared ? ATT_BM / 32 : (int)std::min<int64_t>(ATT_BM, most + 31) / 32;
-    p.results = whole ? 0 : (size_t)pieces * kv.heads * p.slot_waves;
+    p.results = (size_t)results * kv.heads * p.slot_waves;
     p.bytes = p.results * 32 * (kv.head_dim * 4 + 8) + (whole ? 0 : (size_t)(own + 1) * sizeof(TreeTile)) + 256;
     return p;
 }
@@ -52,11 +61,11 @@ static int tree_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const Tree
     A.s1 = CAP ? 2.0f * a.scale / a.cap * ATT_LOG2E : a.scale * ATT_LOG2E;
     A.s2 = a.cap * ATT_LOG2E;
     A.bits = bits; A.words = words;
-    A.room = p.room; A.most_tiles = p.tiles; A.most_pieces = p.pieces; A.slot_waves = p.slot_waves;
+    A.room = p.room; A.most_tiles = p.tiles; A.most_results = p.most_results; A.slot_waves = p.slot_waves;
     A.po = (float *)a.ws;
     A.pm = (float2 *)(A.po + p.results * 32 * D);
     A.tile_at = (TreeTile *)(A.pm + p.results * 32);
-    if (run(MMOE_K_ATT_TREE, k_attn_tree<T, D, CAP, BIAS>, ((unsigned)p.pieces * kv.heads + 7) & ~7u, 256, A)) return -1;
+    if (p.many ? run(MMOE_K_ATT_TREE, k_attn_tree<T, D, CAP, BIAS, true>, p.wgs, 256, A) : run(MMOE_K_ATT_TREE, k_attn_tree<T, D, CAP, BIAS, false>, p.wgs, 256, A)) return -1;
     if (!p.room) return 0;
     return p.deep ? run(MMOE_K_ATT_TREE, k_tree_join<T, D, true>, p.join, 256, A) : run(MMOE_K_ATT_TREE, k_tree_join<T, D, false>, p.join, 256, A);
 }

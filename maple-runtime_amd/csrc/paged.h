@@ -463,7 +463,7 @@ struct AttArgs {
     // value head are to be cut into (0: none, each stays whole), the most row tiles and pieces there can be, waves (of 32 rows) of a piece's partial
     // results in po and pm; the row tiles
     const uint64_t *bits;
-    int words, room, most_tiles, most_pieces, slot_waves;
+    int words, room, most_tiles, most_results, slot_waves;
     struct TreeTile *tile_at;
 };
 
@@ -672,7 +672,9 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
     const mmoe_attn_args &a = A.a;
     const bool shared = work.shared;
     const int nsplit = TREE ? 1 : shared ? A.split_sh : A.split;
-    const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = l & 31, hh = l >> 5;
+    int tid = threadIdx.x;
+    if (TREE) asm volatile("" : "+v"(tid));   // what follows from it is not worth registers from one piece to the next
+    const int l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = l & 31, hh = l >> 5;
     AttTileAt at = work.at;
     int kvh = work.kvh, split = 0;
     if (!TREE) {

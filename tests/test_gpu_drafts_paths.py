@@ -28,6 +28,10 @@ MANY = {  # nodes of sequence s, cached positions of sequence s, sequences, opti
     "whole, 64 sequences": (lambda s: 2 + s % 3, lambda s: 5 * s, 64, dict(heads=8, kv=4, dim=64, kind="bf16", alibi=True)),
     "pieces joined by rows": (lambda s: 3 + s, lambda s: 3000 + 100 * s, 8, dict(heads=8, kv=4)),
     "pieces joined by rows, heads of 64": (lambda s: 3 + s, lambda s: 3000 - 300 * s, 9, dict(heads=8, kv=4, dim=64, kind="bf16")),
+    "900 sequences, most without tokens": (lambda s: 7 if s % 30 == 11 else 0, lambda s: 40 * s if s % 30 == 11 else 9, 900, dict(heads=8, kv=2, pad=500, max_q=64)),
+    "900 sequences, most without tokens, shared": (lambda s: 2 if s % 100 == 50 else 0, lambda s: 128 + s, 900, dict(heads=4, kv=2, shared=128, dim=64, max_q=20)),
+    "more pieces than workgroups": (lambda s: 1 + s % 2, lambda s: 10 + s % 60, 700, dict(heads=4, kv=4, dim=64, kind="bf16")),
+    "more pieces than workgroups, cut": (lambda s: 1, lambda s: 700 + s, 160, dict(heads=6, kv=6, dim=64, alibi=True)),
     "one long, the others none": (lambda s: 2 if s == 40 else 0, lambda s: 8000 if s == 40 else 50, 64, dict(heads=4, kv=2)),
 }
 
