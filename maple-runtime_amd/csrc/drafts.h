@@ -28,8 +28,8 @@ __global__ void __launch_bounds__(64 * W) k_tree_plan(mmoe_tree_plan_args a) {
     const int n = min(q.n, 64 * a.words);
     int out = -1;
     if (i < n) out = a.parent[q.t0 + i];
-    if (out >= i) out = -1;
-    int to = out - 64 * wave;   // in the word: its lane
+    if (out < 0 || out >= i) out = -1;   // (before the subtraction, which would make a lane of a number near the smallest: a node may then follow itself)
+    int to = out - 64 * wave;            // in the word: its lane, below the node's own, so that the steps end
     uint64_t own = 1ull << l;
     while (__any(to >= 0)) {
         const int from = max(to, 0);
