@@ -93,13 +93,21 @@ struct Draft {
             o = {-1, 0, 0, 0, c.shared_k, of_shared(A)};
             return true;
         }
-        if (!MANY) {   // (a result for every piece)
+        // results are kept for row tiles that are cut, and for all with shared positions
+        auto kept_of = [&](const Seq &x, int k) { return k > 1 || A.a.shared ? x.tiles * k : 0; };
+        if (!MANY) {
             const Seq q = of(A, l);
-            const int mine = q.tiles * cut(q, c.per), end = common + (int)scan_wave(mine), tiles = (int)scan_wave(q.tiles) - q.tiles;
+            const int k = cut(q, c.per), mine = q.tiles * k;
+            const int end = common + (int)scan_wave(mine), tiles = (int)scan_wave(q.tiles) - q.tiles;
+            int result = 0;
+            if (A.room) {   // (else every row tile is whole)
+                const int kept = kept_of(q, k);
+                result = common + (int)scan_wave(kept) - kept;
+            }
             const int s = __popcll(__ballot(id >= end));   // a prefix of the lanes
             if (s >= n) return false;
             auto lane = [&](int v) { return __builtin_amdgcn_readlane(v, s); };
-            o.seq = s; o.base = o.result = lane(end - mine); o.tiles = lane(tiles);
+            o.seq = s; o.base = lane(end - mine); o.result = lane(result); o.tiles = lane(tiles);
             o.q = {lane(q.t0), lane(q.t1), lane(q.len), lane(q.rows), lane(q.tiles), lane(q.from), lane(q.to), lane(q.steps)};
             o.k = cut(o.q, c.per);
             return true;
@@ -108,7 +116,7 @@ struct Draft {
         if (tid == 0) M.at[0] = -1;
         for (int s0 = 0; s0 < n; s0 += 256) {
             const Seq x = of(A, s0 + tid);
-            const int k = cut(x, c.per), mine = x.tiles * k, kept = k > 1 || A.a.shared ? mine : 0;
+            const int k = cut(x, c.per), mine = x.tiles * k, kept = kept_of(x, k);
             int end = (int)scan_wave(mine), t = (int)scan_wave(x.tiles), r = (int)scan_wave(kept);
             __syncthreads();   // the sums before have been read
             if (l == 63) { M.sum[0][w] = end; M.sum[1][w] = t; M.sum[2][w] = r; }

@@ -31,8 +31,9 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     // What the card holds at once: two workgroups per compute unit, three with heads of 64 (64 drafts of 10 to 40 tokens over 50 to 3000 positions, heads of 128:
     // 68 us, with 768 pieces 75; 17 drafts behind 2048 shared positions, heads of 64: 32 us, with 512 pieces 37)
     const int once = kv.head_dim == 64 ? 768 : 512;
-    p.room = whole ? 0 : std::max(1, once / kv.heads);
-    const int64_t pieces = whole ? tiles : std::max(tiles <= p.room * 3 / 4 ? (int64_t)p.room : 2 * (int64_t)p.room + tiles, tiles), join = own * kv.heads * 4;
+    const int room = std::max(1, once / kv.heads);
+    p.room = whole ? 0 : room;
+    const int64_t most_pieces = std::max(tiles <= room * 3 / 4 ? (int64_t)room : 2 * (int64_t)room + tiles, tiles), pieces = whole ? tiles : most_pieces, join = own * kv.heads * 4;
     // Few row tiles, so perhaps many results of each, and few workgroups of 32 rows and a key/value head: eight workgroups for one (26 tokens over 700
     // positions, 16: 12.5 us instead of 14.6; over 30000 34 instead of 66; 3 drafts of 60 over 3000, 96: 24.7 instead of 26; 16 of 20 over 2000, 256: 28.6 instead of 27.5)
     p.deep = join < 128;
@@ -42,13 +43,14 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     const int64_t wgs = std::min((pieces * kv.heads + 7) & ~(int64_t)7, p.many ? (int64_t)once : INT64_MAX);
     p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(wgs, join * (p.deep ? 8 : 1)) * 256 <= (int64_t)MAX_THREADS;
     p.wgs = (unsigned)wgs; p.tiles = (int)std::min<int64_t>(own, INT32_MAX); p.join = (unsigned)(p.deep ? join * 8 : join);
-    // Results: one for each piece, but of many sequences' only those of row tiles that are cut (each of at least two pieces, which a cut into 2 room
-    // parts makes less than 4 room of)
-    const int64_t results = whole ? 0 : p.many && !a.shared ? std::min(pieces, (int64_t)4 * p.room) : pieces;
+    // Results: one for each piece, but without shared positions only for those of row tiles that are cut (each of at least two pieces, which a cut into
+    // 2 room parts makes less than 4 room of). There is room for them also where the row tiles stay whole, so that a workspace serves every bound of
+    // the lengths and every window, and more of it never does with less.
+    const int64_t results = a.shared ? most_pieces : std::min(most_pieces, (int64_t)4 * room);
     p.most_results = (int)std::min<int64_t>(results, INT32_MAX);
     p.slot_waves = a.shared ? ATT_BM / 32 : (int)std::min<int64_t>(ATT_BM, most + 31) / 32;
     p.results = (size_t)results * kv.heads * p.slot_waves;
-    p.bytes = p.results * 32 * (kv.head_dim * 4 + 8) + (whole ? 0 : (size_t)(own + 1) * sizeof(TreeTile)) + 256;
+    p.bytes = p.results * 32 * (kv.head_dim * 4 + 8) + (size_t)(own + 1) * sizeof(TreeTile) + 256;
     return p;
 }
 
