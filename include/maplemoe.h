@@ -412,7 +412,7 @@ int mmoe_tree_plan(const mmoe_tree_plan_args *a);
  *   cached positions p:  max(lo[t], pos - window) <= p < ctx;   new tokens j <= i (at position ctx + j) whose bit is set, whatever the window
  * where pos = ctx + the number of its bits below i, and slopes count |pos - p| to a cached position and, to token j < i, one and the bits
  * between j and i (on mmoe_tree_plan's bits: the steps along the path). bits[ntok][words] need not be a tree's: any bits do; those past i count
- * for nothing. hi must be NULL and max_q at most 64 words. The workspace's size (0: arguments that are refused) follows from ntok, max_q and nseq (more for
+ * for nothing. hi must be NULL and max_q at most 64 words. The workspace's size (0: arguments that are refused; it does not look at bits) follows from ntok, max_q and nseq (more for
  * more), the heads and whether shared is 0 (more if not), not from max_len or window: one for the largest serves every step and every layer of the same
  * heads. Its content does not matter, calls that may run at the same time need one each. */
 size_t mmoe_attn_tree_ws(const mmoe_attn_args *a, const mmoe_kv_cache *kv, const uint64_t *bits, int words);

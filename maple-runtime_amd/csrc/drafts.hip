@@ -54,6 +54,11 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     return p;
 }
 
+static int check_launch(const mmoe_attn_args &a, const TreePlan &p) {
+    if (!p.fits) REFUSE("mmoe_attn_tree: %d sequences of up to %d positions, %d tokens, %d heads: too many for a launch", a.nseq, a.max_len, a.ntok, a.heads);
+    return 0;
+}
+
 template <int T, int D, bool CAP, bool BIAS>
 static int tree_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const TreePlan &p, const uint64_t *bits, int words) {
     AttArgs A{};
@@ -132,9 +137,10 @@ int mmoe_tree_plan(const mmoe_tree_plan_args *p) {
 }
 
 size_t mmoe_attn_tree_ws(const mmoe_attn_args *p, const mmoe_kv_cache *kv, const uint64_t *bits, int words) {
-    (void)bits;
+    (void)bits;   // (what it points to does not count, nor whether it does)
     if (check_bits("mmoe_attn_tree", p, kv, words)) return 0;
-    return tree_plan(*p, *kv).bytes;
+    const TreePlan pl = tree_plan(*p, *kv);
+    return check_launch(*p, pl) ? 0 : pl.bytes;
 }
 
 int mmoe_attn_tree(const mmoe_attn_args *p, const mmoe_kv_cache *kv, const uint64_t *bits, int words) {
@@ -145,7 +151,7 @@ int mmoe_attn_tree(const mmoe_attn_args *p, const mmoe_kv_cache *kv, const uint6
     if (apart(a.q, 16) || apart(a.out, 16)) REFUSE("mmoe_attn_tree: q and out must be aligned to 16 bytes");
     if (apart(bits, 8)) REFUSE("mmoe_attn_tree: bits must be aligned to 8 bytes");
     const TreePlan pl = tree_plan(a, *kv);
-    if (!pl.fits) REFUSE("mmoe_attn_tree: %d sequences of up to %d positions, %d tokens, %d heads: too many for a launch", a.nseq, a.max_len, a.ntok, a.heads);
+    if (check_launch(a, pl)) return -1;
     if (!a.ws || a.ws_bytes < pl.bytes || apart(a.ws, 256)) REFUSE("mmoe_attn_tree: workspace of %zu bytes (%zu needed, aligned to 256)", a.ws ? a.ws_bytes : 0, pl.bytes);
     if (mm_ready()) return -1;
     if (!a.max_q) return 0;   // no token is served

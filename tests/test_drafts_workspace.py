@@ -36,3 +36,12 @@ def test_it_grows_with_tokens_and_sequences(ckw, heads, shared):
                 x = at(n, t, q)
                 assert x and x == at(n, t, q) and at(n, t, q, 0) <= x == at(n, t, q, 4 * shared)
                 assert all(at(m, t, q) <= x for m in seqs if m < n) and all(at(n, u, q) <= x for u in toks if u < t) and all(at(n, t, r) <= x for r in most if r < q), (n, t, q)
+
+
+@pytest.mark.parametrize("kw,ckw", [(dict(nseq=4096, ntok=1 << 18, max_q=512, width=1 << 22, max_len=1 << 26, heads=16), dict(heads=1)),
+                                    (dict(nseq=64, ntok=1 << 20, max_q=512, width=1 << 26, max_len=1 << 30, heads=1024), dict(heads=1))])
+def test_no_size_for_what_is_too_much_for_a_launch(kw, ckw):
+    refused(M.lib().mmoe_attn_tree(attn(**kw), cache(**ckw), P, 8), b"too many")
+    M.lib().mmoe_attn_tree(None, cache(), P, 1)      # another message
+    assert M.lib().mmoe_attn_tree_ws(attn(**kw), cache(**ckw), P, 8) == 0 and b"too many" in M.lib().mmoe_last_error()
+    assert M.lib().mmoe_attn_tree_ws(attn(**dict(kw, max_len=1000)), cache(**ckw), P, 8) > 0
