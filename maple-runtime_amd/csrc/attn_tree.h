@@ -9,13 +9,18 @@
 #include <type_traits>
 #include "paged.h"
 
-// A sequence's row tile for the join: its first piece, how many, how far apart, its first token, its first row among its sequence's, the sequence's rows. The
-// first entry holds the number of them in `slot` and in `parts` and `apart` the pieces of a row tile over the shared positions, which are the
-// first pieces of all.
+// Partial results are kept in waves of 32 rows. Those over the shared positions come first, then sequence by sequence, of each what it has over its first
+// positions (the waves of all its rows, key/value head by key/value head), then over the next ones, ... Where one begins is counted per key/value head.
+// A sequence's row tile for the join: where its sequence's results begin, how many there are over its positions, the waves of each, its first token, its
+// first row among its sequence's, the sequence's rows. The first entry holds the number of them in `slot`, and of the shared positions' results `parts`
+// and `apart`.
 struct TreeTile { int slot, parts, apart, t0, row0, rows; };
 
 struct Draft {
-    struct Seq { int t0, t1, len, rows, tiles, from, to, steps; };
+    struct Seq {
+        int t0, t1, len, rows, tiles, from, to, steps;
+        __device__ __forceinline__ int waves() const { return (rows + 31) >> 5; }
+    };
     // the shared positions' rows (every token) as a sequence of its own
     __device__ static __forceinline__ Seq of_shared(const AttArgs &A) {
         Seq q = {0, 0, 0, A.a.shared ? att_start(A.a, A.a.nseq) * A.group : 0, 0, 0, A.a.shared, (A.a.shared + TREE_BN - 1) / TREE_BN};
@@ -45,8 +50,9 @@ struct Draft {
     }
     struct Mem { int sum[3][4], at[4]; };
     __device__ static __forceinline__ int wave_sum(int v) { return wave_reduce(v, [](int x, int y) { return x + y; }); }
-    // Pieces per step; how many pieces there are, row tiles of the sequences and over the shared positions, pieces of one of the latter (which come first)
-    struct Cut { float per; int pieces, own_tiles, shared_tiles, shared_k; };
+    // Pieces per step; how many pieces there are, row tiles of the sequences and over the shared positions, waves of the latter, pieces of one of them (which
+    // come first)
+    struct Cut { float per; int pieces, own_tiles, shared_tiles, shared_waves, shared_k; };
     // The same for every thread of the workgroup (256). MANY: more than 64 sequences, else every wave does it by itself
     template <bool MANY> __device__ static __forceinline__ Cut plan(const AttArgs &A, Mem &M) {
         const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, n = A.a.nseq;
@@ -63,7 +69,7 @@ struct Draft {
         };
         Cut c;
         c.own_tiles = total([](const Seq &x) { return x.tiles; });
-        c.shared_tiles = sh.tiles;
+        c.shared_tiles = sh.tiles; c.shared_waves = sh.waves();
         const int all_tiles = sh.tiles + c.own_tiles;
         float per = 0.0f;
         int pieces = all_tiles;
@@ -88,13 +94,13 @@ struct Draft {
     // A piece: its sequence (-1: the shared positions), that one's first piece, first result and row tile, the pieces of its row tile
     struct Piece { int seq, base, result, tiles, k; Seq q; };
     template <bool MANY> __device__ static __forceinline__ bool piece(const AttArgs &A, Mem &M, const Cut &c, int id, Piece &o) {
-        const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, n = A.a.nseq, common = c.shared_tiles * c.shared_k;
+        const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, n = A.a.nseq, common = c.shared_tiles * c.shared_k, common_waves = c.shared_waves * c.shared_k;
         if (id < common) {
             o = {-1, 0, 0, 0, c.shared_k, of_shared(A)};
             return true;
         }
         // results are kept for row tiles that are cut, and for all with shared positions
-        auto kept_of = [&](const Seq &x, int k) { return k > 1 || A.a.shared ? x.tiles * k : 0; };
+        auto kept_of = [&](const Seq &x, int k) { return k > 1 || A.a.shared ? x.waves() * k : 0; };
         if (!MANY) {
             const Seq q = of(A, l);
             const int k = cut(q, c.per), mine = q.tiles * k;
@@ -102,7 +108,7 @@ struct Draft {
             int result = 0;
             if (A.room) {   // (else every row tile is whole)
                 const int kept = kept_of(q, k);
-                result = common + (int)scan_wave(kept) - kept;
+                result = common_waves + (int)scan_wave(kept) - kept;
             }
             const int s = __popcll(__ballot(id >= end));   // a prefix of the lanes
             if (s >= n) return false;
@@ -112,7 +118,7 @@ struct Draft {
             o.k = cut(o.q, c.per);
             return true;
         }
-        int before = common, tiles = 0, results = common;
+        int before = common, tiles = 0, results = common_waves;
         if (tid == 0) M.at[0] = -1;
         for (int s0 = 0; s0 < n; s0 += 256) {
             const Seq x = of(A, s0 + tid);
@@ -167,12 +173,12 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
         const Draft::Seq &q = o.q;
         const int k = __builtin_amdgcn_readfirstlane(o.k), steps = __builtin_amdgcn_readfirstlane(q.steps), i = (id - o.base) / q.tiles, tile = id - o.base - i * q.tiles;
         const bool whole = k == 1 && !A.a.shared;
-        const int result = o.result + (id - o.base);
+        const int waves = q.waves(), result = o.result + i * waves;
         // (both fit if qstart ascends)
-        if ((whole || result < A.most_results) && (o.seq < 0 || o.tiles + tile < A.most_tiles)) {
+        if ((whole || result + waves <= A.most_waves) && (o.seq < 0 || o.tiles + tile < A.most_tiles)) {
             if (A.room && kvh == 0 && i == 0 && threadIdx.x == 0) {
-                if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {result, k, q.tiles, q.t0, tile * ATT_BM, q.rows};
-                if (id == 0) A.tile_at[0] = {min(c.own_tiles, A.most_tiles), c.shared_k, c.shared_tiles, 0, 0, 0};
+                if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {result, k, waves, q.t0, tile * ATT_BM, q.rows};
+                if (id == 0) A.tile_at[0] = {min(c.own_tiles, A.most_tiles), c.shared_k, c.shared_waves, 0, 0, 0};
             }
             const int len = steps / k, more = steps - len * k;   // the first of them a step longer
             AttWork work = {};
@@ -183,7 +189,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
             work.p0 = q.from + (i * len + min(i, more)) * TREE_BN;
             work.p1 = min(work.p0 + (len + (i < more)) * TREE_BN, q.to);
             work.whole = whole;
-            work.slot = (int64_t)result * A.kv.heads + kvh;
+            work.slot = (int64_t)result * A.kv.heads + kvh * waves + tile * (ATT_BM / 32);
             att_tile<T, D, CAP, BIAS, true>(tree_args(), work, M);
         }
         if (!MANY) return;
@@ -213,22 +219,23 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
     const TreeTile head_of = A.tile_at[0], t = A.tile_at[1 + tile];
     if (tile >= head_of.slot || (t.parts == 1 && !a.shared)) return;   // none, or written by the piece that was all of it
     // nothing outside the arrays, whatever qstart holds (where it does not ascend, row tiles may be those of an earlier call)
-    if (w >= A.slot_waves || t.row0 >= t.rows || t.slot < 0 || t.parts < 1 || t.apart < 0 || t.slot + (t.parts - 1) * (int64_t)t.apart >= A.most_results || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
+    if (t.row0 >= t.rows || t.slot < 0 || t.parts < 1 || t.apart < 0 || t.slot + t.parts * (int64_t)t.apart > A.most_waves || (t.row0 >> 5) + w >= t.apart || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
     const int r = t.row0 + w * 32 + n;
     if (t.row0 + w * 32 >= t.rows) return;
     const bool live = r < t.rows;
     const int row = min(r, t.rows - 1), j = (int)A.by_group(row), tok = t.t0 + j, head = kvh * A.group + row - j * A.group;
-    // the shared positions' row tiles hold every token's rows
-    const int common = a.shared ? head_of.parts : 0, rs = tok * A.group + row - j * A.group, slot_sh = rs / ATT_BM, at_sh = rs % ATT_BM;
-    if (a.shared && (common < 0 || head_of.apart < 0 || slot_sh + (common - 1) * (int64_t)head_of.apart >= A.most_results)) return;
+    // the results over the shared positions hold every token's rows
+    const int common = a.shared ? head_of.parts : 0, rs = tok * A.group + row - j * A.group;
+    if (a.shared && (common < 0 || head_of.apart < 0 || rs >> 5 >= head_of.apart || common * (int64_t)head_of.apart > A.most_waves)) return;
     const int parts = common + t.parts;
     struct Result { float2 v; f4 y[C]; };
     auto load = [&](Result &x, int p) {
         const bool c = p < common;
-        const int at = c ? at_sh : w * 32 + n;
-        const int64_t wave = ((int64_t)(c ? slot_sh + p * head_of.apart : t.slot + (p - common) * t.apart) * A.kv.heads + kvh) * A.slot_waves + (at >> 5);
-        x.v = A.pm[wave * 32 + (at & 31)];
-        const f4 *q = (const f4 *)(A.po + wave * 32 * D) + 32 * hh + (at & 31);
+        const int at = c ? rs & 31 : n;
+        const int apart = c ? head_of.apart : t.apart;
+        const int64_t wave = (int64_t)(c ? p * apart : t.slot + (p - common) * apart) * A.kv.heads + kvh * apart + (c ? rs >> 5 : (t.row0 >> 5) + w);
+        x.v = A.pm[wave * 32 + at];
+        const f4 *q = (const f4 *)(A.po + wave * 32 * D) + 32 * hh + at;
 #pragma unroll
         for (int i = 0; i < C; i++) x.y[i] = q[(share * C + i) * 64];
     };

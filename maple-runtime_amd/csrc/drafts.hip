@@ -14,7 +14,7 @@ static int check_bits(const char *who, const mmoe_attn_args *p, const mmoe_kv_ca
 // How a call of mmoe_attn_tree is divided (attn_tree.h). Only the values in the arguments count (a captured call keeps its grid). The numbers of
 // workgroups are for the 256 compute units of the one device that the kernels are built and were measured for.
 struct TreePlan {
-    int room, most_results, slot_waves, tiles;
+    int room, most_waves, tiles;
     unsigned wgs, join;
     bool many, deep, fits;
     size_t results, bytes;
@@ -23,7 +23,9 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     TreePlan p = {};
     const int group = a.heads / kv.heads;
     const int64_t rows = (int64_t)a.ntok * group, most = (int64_t)std::min(a.max_q, a.ntok) * group;
-    const int64_t own = std::min((int64_t)a.nseq * ((most + ATT_BM - 1) / ATT_BM), rows / ATT_BM + a.nseq), tiles = own + (a.shared ? (rows + ATT_BM - 1) / ATT_BM : 0);
+    // sequences with tokens; row tiles of their own (and waves of 32 rows), all row tiles
+    const int64_t busy = std::min(a.nseq, a.ntok), own = std::min(busy * ((most + ATT_BM - 1) / ATT_BM), rows / ATT_BM + busy), own_waves = std::min(busy * ((most + 31) / 32), rows / 32 + busy);
+    const int64_t sh_tiles = a.shared ? (rows + ATT_BM - 1) / ATT_BM : 0, tiles = own + sh_tiles;
     // Row tiles of so few positions, and so many of them, that they stay whole: nothing to join (32 drafts of 64 tokens in a window of 512, 256 row tiles:
     // 25 us, cut 36; 24 drafts, 192: 23.6, cut 29.2; 48 drafts of 4 over 600, 192: 18.9, cut 22.3)
     const int64_t most_steps = (a.window ? std::min<int64_t>(a.max_len, (int64_t)a.window + a.max_q + TREE_BN) : a.max_len) / TREE_BN + 1;
@@ -39,17 +41,22 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     p.deep = join < 128;
     p.many = a.nseq > 64;
     // Of up to 64 sequences a workgroup for each piece that there may be. Of more a workgroup for each that the card holds at once: 64 drafts of 20 tokens in
-    // a batch of 1024 (4096) sequences, the others without, 54 (79) us instead of 76 (374); 256 drafts of 4 over 1500, all there, 155 instead of 149
+    // a batch of 1024 (4096) sequences, the others without, 54 (73) us instead of 76 (374); 256 drafts of 4 over 1500, all there, 154 instead of 149
     const int64_t wgs = std::min((pieces * kv.heads + 7) & ~(int64_t)7, p.many ? (int64_t)once : INT64_MAX);
     p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(wgs, join * (p.deep ? 8 : 1)) * 256 <= (int64_t)MAX_THREADS;
     p.wgs = (unsigned)wgs; p.tiles = (int)std::min<int64_t>(own, INT32_MAX); p.join = (unsigned)(p.deep ? join * 8 : join);
-    // Results: one for each piece, but without shared positions only for those of row tiles that are cut (each of at least two pieces, which a cut into
-    // 2 room parts makes less than 4 room of). There is room for them also where the row tiles stay whole, so that a workspace serves every bound of
-    // the lengths and every window, and more of it never does with less.
-    const int64_t results = a.shared ? most_pieces : std::min(most_pieces, (int64_t)4 * room);
-    p.most_results = (int)std::min<int64_t>(results, INT32_MAX);
-    p.slot_waves = a.shared ? ATT_BM / 32 : (int)std::min<int64_t>(ATT_BM, most + 31) / 32;
-    p.results = (size_t)results * kv.heads * p.slot_waves;
+    // Results, in waves of 32 rows: of up to `room` pieces where the row tiles are few; else one of every row, and as many more as a cut into 2 room parts
+    // makes (rounded up, each row tile is one more than its share of them). Without shared positions only those of row tiles that are cut, each
+    // of at least two pieces, which makes less than 4 room. There is room for them also where the row tiles stay whole, so that a workspace serves every
+    // bound of the lengths and every window, and more of it never does with less.
+    const int64_t piece_waves = a.shared ? ATT_BM / 32 : std::min<int64_t>(ATT_BM, most + 31) / 32;
+    int64_t waves = piece_waves * room;
+    if (tiles > room * 3 / 4) {
+        waves = piece_waves * 2 * room + own_waves + sh_tiles * (ATT_BM / 32);
+        if (!a.shared) waves = std::min(waves, piece_waves * 4 * room);
+    }
+    p.most_waves = (int)std::min<int64_t>(waves, INT32_MAX);
+    p.results = (size_t)waves * kv.heads;
     p.bytes = p.results * 32 * (kv.head_dim * 4 + 8) + (size_t)(own + 1) * sizeof(TreeTile) + 256;
     return p;
 }
@@ -68,7 +75,7 @@ static int tree_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const Tree
     A.s1 = CAP ? 2.0f * a.scale / a.cap * ATT_LOG2E : a.scale * ATT_LOG2E;
     A.s2 = a.cap * ATT_LOG2E;
     A.bits = bits; A.words = words;
-    A.room = p.room; A.most_tiles = p.tiles; A.most_results = p.most_results; A.slot_waves = p.slot_waves;
+    A.room = p.room; A.most_tiles = p.tiles; A.most_waves = p.most_waves;
     A.po = (float *)a.ws;
     A.pm = (float2 *)(A.po + p.results * 32 * D);
     A.tile_at = (TreeTile *)(A.pm + p.results * 32);

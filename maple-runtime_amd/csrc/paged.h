@@ -460,10 +460,10 @@ struct AttArgs {
     float2 *pm;
     int64_t at_tile, at_few;
     // Drafted tokens (TREE, attn_tree.h): words of bits per token, bit j: it sees its sequence's j-th new token; the pieces that the row tiles of a key/
-    // value head are to be cut into (0: none, each stays whole), the most row tiles and pieces there can be, waves (of 32 rows) of a piece's partial
-    // results in po and pm; the row tiles
+    // value head are to be cut into (0: none, each stays whole), the most row tiles there can be and the most waves (of 32 rows) of their partial results in
+    // po and pm; the row tiles
     const uint64_t *bits;
-    int words, room, most_tiles, most_results, slot_waves;
+    int words, room, most_tiles, most_waves;
     struct TreeTile *tile_at;
 };
 
@@ -1076,7 +1076,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
         return;
     }
     if (TREE) {   // as the registers hold it: [wave][16 dims][lane][4 of them]
-        const int64_t at = work.slot * E.slot_waves + w;
+        const int64_t at = work.slot + w;
         if (hh == 0) E.pm[at * 32 + n] = make_float2(mb, wild ? -sum : sum);
         f4 *o = (f4 *)(E.po + at * 32 * D) + l;
 #pragma unroll

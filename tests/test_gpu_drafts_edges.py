@@ -2,8 +2,9 @@
 import numpy as np
 import pytest
 
-from draft_ref import tree, tree_plan
-from test_gpu_drafts import run_tree_plan
+from draft_ref import TreeBatch, tree, tree_plan
+from paged_ref import Dev
+from test_gpu_drafts import drafts, run_tree_plan
 
 pytestmark = pytest.mark.gpu
 LEAST = -2 ** 31
@@ -24,3 +25,26 @@ def test_parents_near_the_smallest_number(sizes, words, none):
     length = np.array(sizes) + rng.integers(0, 1 << 29, len(sizes))
     got, want = run_tree_plan(qstart, length, parent, words, len(parent)), tree_plan(qstart, length, parent, words, len(parent))
     assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+KEPT = {  # nodes of sequence s, cached positions of sequence s, sequences, options
+    "cut and shared, few of 400 with tokens": (lambda s: 20 if s % 40 == 7 else 0, lambda s: 3000 - 5 * s if s % 40 == 7 else 70, 400, dict(heads=8, kv=2, shared=64, pad=40)),
+    "row tiles, cut and shared": (lambda s: 30 - 3 * s, lambda s: 130 + 400 * s, 6, dict(heads=16, kv=1, shared=128, kind="bf16")),
+    "row tiles, cut and shared, 66 sequences": (lambda s: 27 if s in (3, 64) else s % 2, lambda s: 2500 if s == 64 else 70, 66, dict(heads=24, kv=2, dim=64, shared=64)),
+    "one row short of a wave, one over": (lambda s: (7, 8, 9, 31, 32, 33)[s % 6], lambda s: 300 * (s % 7), 12, dict(heads=4, kv=1)),
+    "one row short of a wave, one over, shared": (lambda s: (31, 32, 33, 1, 64, 63)[s], lambda s: 256 + 300 * s, 6, dict(heads=2, kv=2, dim=64, shared=256, kind="bf16")),
+    "uncut row tiles, shared": (lambda s: 1 + s % 5, lambda s: 64 + s % 50, 300, dict(heads=12, kv=4, shared=64)),
+    "fewer tokens than sequences": (lambda s: int(s == 2000), lambda s: 900 if s == 2000 else 3, 4096, dict(heads=4, kv=1, kind="bf16")),
+}
+
+
+@pytest.mark.parametrize("name", list(KEPT))
+def test_results_kept(name):
+    """partial results lie wave by wave: row tiles of several waves beside ones of a part of one, with shared positions before them; nothing behind the workspace"""
+    nodes, ctx, n, kw = KEPT[name]
+    print(f"\n  {name}", flush=True)
+    rng = np.random.default_rng(len(name))
+    sizes = [nodes(s) for s in range(n)]
+    b = TreeBatch(rng, drafts(rng, sizes, 4), lens=[ctx(s) + x for s, x in enumerate(sizes)], **kw)
+    with Dev() as d:
+        b.run(d, name)
