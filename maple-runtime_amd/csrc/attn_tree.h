@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
         for (int u = 0; u < n.value; u++) {
             const float e = x[u].v.y != 0.0f ? exp2_(x[u].v.x - by) : 0.0f;
             sum = fmaf(fabsf(x[u].v.y), e, sum);
-            wild |= x[u].v.y < 0.0f;
+            wild |= __float_as_int(x[u].v.y) < 0;   // (a sum of 0 has a sign, too)
 #pragma unroll
             for (int c = 0; c < C; c++)
 #pragma unroll
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
         }
         add(x, std::integral_constant<int, 3>{});
     }
-    if (__any(wild && live)) {   // once more: results that are not finite count whatever their weight
+    if (__any(wild && live)) {   // once more: results that are not finite count whatever their weight, and where every score was -inf
 #pragma unroll
         for (int c = 0; c < C; c++) o[c] = f4{0, 0, 0, 0};
 #pragma unroll 1
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
 #pragma unroll
             for (int c = 0; c < C; c++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[c][i] = e != 0.0f ? fmaf(e, x.y[c][i], o[c][i]) : x.v.y != 0.0f ? o[c][i] + only_odd(x.y[c][i]) : o[c][i];
+                for (int i = 0; i < 4; i++) o[c][i] = e != 0.0f ? fmaf(e, x.y[c][i], o[c][i]) : o[c][i] + only_odd(x.y[c][i]);
         }
     }
     if (!live) return;

@@ -2,8 +2,9 @@
 import numpy as np
 import pytest
 
+import maplemoe as M
 from draft_ref import TreeBatch, tree, tree_plan
-from paged_ref import Dev
+from paged_ref import Dev, decode, encode
 from test_gpu_drafts import drafts, run_tree_plan
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +49,50 @@ def test_results_kept(name):
     b = TreeBatch(rng, drafts(rng, sizes, 4), lens=[ctx(s) + x for s, x in enumerate(sizes)], **kw)
     with Dev() as d:
         b.run(d, name)
+
+
+HIDDEN = {  # nodes, lengths, positions whose score is -inf, the one of them that holds infinities, options
+    "whole": ([2] * 200, [300] * 200, (0, 250), 70, dict(heads=1, kv=1)),
+    "one draft, a piece and more": ([20], [6000], (0, 3000), 1500, dict(heads=4, kv=1)),
+    "one draft, the middle": ([20], [6000], (2000, 5000), 3333, dict(heads=8, kv=2)),
+    "joined by rows": ([30] * 10, [2500] * 10, (300, 2400), 1700, dict(heads=16, kv=4)),
+    "the shared positions": ([5, 30], [2600, 3000], (0, 2048), 999, dict(heads=4, kv=1, shared=2048)),
+    "many sequences": ([3] * 70, [3000] * 70, (0, 2900), 1, dict(heads=4, kv=2)),
+}
+
+
+@pytest.mark.parametrize("kind,dim", [("f16", 64), ("bf16", 128)])
+@pytest.mark.parametrize("name", list(HIDDEN))
+def test_infinite_values_where_every_score_is_minus_infinity(name, kind, dim):
+    """a part of the positions as long as a piece or longer has scores of -inf, and an infinite value among them reaches every token that sees it, however
+    the call is divided; the other dims are what they are without it, but for the order of their sums: within the bound of either"""
+    nodes, lens, (p0, p1), at, kw = HIDDEN[name]
+    print(f"\n  {name} {kind}", flush=True)
+    rng = np.random.default_rng(len(name) + dim)
+    b = TreeBatch(rng, drafts(rng, nodes, 3), lens=lens, kind=kind, dim=dim, **kw)
+    b.scale = 1.0
+    k, q = 0.3 * decode(b.k, kind), decode(b.q, kind)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    for s in range(len(lens)):
+        p = np.arange(p0, p1)
+        k[b.table[s, p // b.bs], p % b.bs] = 0.0
+        k[b.table[s, p // b.bs], p % b.bs, :, 0] = -np.inf
+    b.k, b.q = encode(k, kind), encode(q, kind)
+    with Dev() as d:
+        b.run(d, "finite values")
+        want, _, off, _ = b.expect()
+        v = decode(b.v, kind)
+        for s in range(len(lens)):
+            v[b.table[s, at // b.bs], at % b.bs, :, 5] = np.inf
+            v[b.table[s, at // b.bs], at % b.bs, :, 6] = -np.inf
+            v[b.table[s, at // b.bs], at % b.bs, :, 7] = np.nan
+        b.v = encode(v, kind)
+        a = b.upload(d)
+        M.check(d.lib.mmoe_attn_tree(a, b.cache, b.p_bits, b.words), "attention")
+        out = d.get(b.p_out, b.out0)
+    n, h = b.ntok, b.heads
+    got = decode(out[:, 8:8 + h * (dim + 8)].reshape(n, h, dim + 8)[..., :dim].copy(), kind)
+    assert (got[..., 5] == np.inf).all() and (got[..., 6] == -np.inf).all() and np.isnan(got[..., 7]).all()
+    rest = [i for i in range(dim) if i not in (5, 6, 7)]
+    bad = np.abs(got - want)[..., rest] > off[..., rest]
+    assert not bad.any(), np.argwhere(bad)[:5]
