@@ -410,12 +410,16 @@ typedef struct {
 int mmoe_tree_plan(const mmoe_tree_plan_args *a);
 
 /* Attention of drafted tokens: mmoe_attn_paged but for what is visible. With ctx = len[s] less the sequence's new tokens, token i of them sees
- *   cached positions p:  max(lo[t], pos - window) <= p < ctx;   new tokens j <= i (at position ctx + j) whose bit is set, whatever the window
+ *   cached positions p:  max(lo[t], pos - window) <= p < ctx;   new tokens j <= i (at position ctx + j) whose bit is set
  * where pos = ctx + the number of its bits below i, and slopes count |pos - p| to a cached position and, to token j < i, one and the bits
- * between j and i (on mmoe_tree_plan's bits: the steps along the path). bits[ntok][words] need not be a tree's: any bits do; those past i count
- * for nothing. hi must be NULL and max_q at most 64 words. The workspace's size (0: arguments that are refused; it does not look at bits) follows from ntok, max_q and nseq (more for
- * more), the heads and whether shared is 0 (more if not), not from max_len or window: one for the largest serves every step and every layer of the same
- * heads. Its content does not matter, calls that may run at the same time need one each. */
+ * between j and i (on mmoe_tree_plan's bits: the steps along the path). The window does not hide new tokens: where no path is longer than it, that is
+ * what a model with a window sees. Where one may be, add MMOE_TREE_WINDOW to words: of its path a token then sees itself and the `window` tokens
+ * before, cached or new, so that a draft without branches sees what mmoe_attn_paged's tokens see.
+ * bits[ntok][words] need not be a tree's: any bits do; those past i count for nothing. hi must be NULL and max_q at most 64 words.
+ * The workspace's size (0: arguments that are refused; it does not look at bits) follows from ntok, max_q and nseq (more for more), the heads and whether
+ * shared is 0 (more if not), not from max_len or window: one for the largest serves every step and every layer of the same heads. Its content does not
+ * matter, calls that may run at the same time need one each. */
+#define MMOE_TREE_WINDOW 256
 size_t mmoe_attn_tree_ws(const mmoe_attn_args *a, const mmoe_kv_cache *kv, const uint64_t *bits, int words);
 int mmoe_attn_tree(const mmoe_attn_args *a, const mmoe_kv_cache *kv, const uint64_t *bits, int words);
 

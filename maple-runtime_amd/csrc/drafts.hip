@@ -3,6 +3,7 @@
 #include "drafts.h"
 #include "attn_tree.h"
 
+// words: without MMOE_TREE_WINDOW
 static int check_bits(const char *who, const mmoe_attn_args *p, const mmoe_kv_cache *kv, int words) {
     if (check_attn(who, p, kv)) return -1;
     if (p->hi) REFUSE("%s: hi is set (new tokens are seen by their bits)", who);
@@ -67,14 +68,14 @@ static int check_launch(const mmoe_attn_args &a, const TreePlan &p) {
 }
 
 template <int T, int D, bool CAP, bool BIAS>
-static int tree_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const TreePlan &p, const uint64_t *bits, int words) {
+static int tree_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const TreePlan &p, const uint64_t *bits, int words, int path) {
     AttArgs A{};
     A.a = a; A.kv = kv;
     A.sh = log2_block(kv.block_size); A.group = a.heads / kv.heads;
     A.by_kv = divisor(kv.heads); A.by_group = divisor(A.group);
     A.s1 = CAP ? 2.0f * a.scale / a.cap * ATT_LOG2E : a.scale * ATT_LOG2E;
     A.s2 = a.cap * ATT_LOG2E;
-    A.bits = bits; A.words = words;
+    A.bits = bits; A.words = words; A.path = path;
     A.room = p.room; A.most_tiles = p.tiles; A.most_waves = p.most_waves;
     A.po = (float *)a.ws;
     A.pm = (float2 *)(A.po + p.results * 32 * D);
@@ -84,9 +85,9 @@ static int tree_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const Tree
     return p.deep ? run(MMOE_K_ATT_TREE, k_tree_join<T, D, true>, p.join, 256, A) : run(MMOE_K_ATT_TREE, k_tree_join<T, D, false>, p.join, 256, A);
 }
 template <int T, int D>
-static int tree_pick(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const TreePlan &p, const uint64_t *b, int w) {
-    if (a.cap > 0) return a.slopes ? tree_run<T, D, true, true>(a, kv, p, b, w) : tree_run<T, D, true, false>(a, kv, p, b, w);
-    return a.slopes ? tree_run<T, D, false, true>(a, kv, p, b, w) : tree_run<T, D, false, false>(a, kv, p, b, w);
+static int tree_pick(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const TreePlan &p, const uint64_t *b, int w, int path) {
+    if (a.cap > 0) return a.slopes ? tree_run<T, D, true, true>(a, kv, p, b, w, path) : tree_run<T, D, true, false>(a, kv, p, b, w, path);
+    return a.slopes ? tree_run<T, D, false, true>(a, kv, p, b, w, path) : tree_run<T, D, false, false>(a, kv, p, b, w, path);
 }
 
 // The layers' caches of a call that works on all of them
@@ -145,12 +146,14 @@ int mmoe_tree_plan(const mmoe_tree_plan_args *p) {
 
 size_t mmoe_attn_tree_ws(const mmoe_attn_args *p, const mmoe_kv_cache *kv, const uint64_t *bits, int words) {
     (void)bits;   // (what it points to does not count, nor whether it does)
-    if (check_bits("mmoe_attn_tree", p, kv, words)) return 0;
+    if (check_bits("mmoe_attn_tree", p, kv, words & ~MMOE_TREE_WINDOW)) return 0;
     const TreePlan pl = tree_plan(*p, *kv);
     return check_launch(*p, pl) ? 0 : pl.bytes;
 }
 
 int mmoe_attn_tree(const mmoe_attn_args *p, const mmoe_kv_cache *kv, const uint64_t *bits, int words) {
+    const bool along = words & MMOE_TREE_WINDOW;
+    words &= ~MMOE_TREE_WINDOW;
     if (check_bits("mmoe_attn_tree", p, kv, words)) return -1;
     const mmoe_attn_args &a = *p;
     if (!a.nseq || !a.ntok) return 0;
@@ -164,8 +167,9 @@ int mmoe_attn_tree(const mmoe_attn_args *p, const mmoe_kv_cache *kv, const uint6
     if (!a.max_q) return 0;   // no token is served
     OnDevice dev;
     if (!dev.ok) return -1;
-    if (kv->dtype == MMOE_F16) return kv->head_dim == 64 ? tree_pick<MMOE_F16, 64>(a, *kv, pl, bits, words) : tree_pick<MMOE_F16, 128>(a, *kv, pl, bits, words);
-    return kv->head_dim == 64 ? tree_pick<MMOE_BF16, 64>(a, *kv, pl, bits, words) : tree_pick<MMOE_BF16, 128>(a, *kv, pl, bits, words);
+    const int path = along && a.window ? a.window : INT32_MAX;
+    if (kv->dtype == MMOE_F16) return kv->head_dim == 64 ? tree_pick<MMOE_F16, 64>(a, *kv, pl, bits, words, path) : tree_pick<MMOE_F16, 128>(a, *kv, pl, bits, words, path);
+    return kv->head_dim == 64 ? tree_pick<MMOE_BF16, 64>(a, *kv, pl, bits, words, path) : tree_pick<MMOE_BF16, 128>(a, *kv, pl, bits, words, path);
 }
 
 int mmoe_tree_accept(const mmoe_tree_accept_args *p) {

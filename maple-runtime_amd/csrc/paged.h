@@ -464,6 +464,7 @@ struct AttArgs {
     // po and pm; the row tiles
     const uint64_t *bits;
     int words, room, most_tiles, most_waves;
+    int path;   // the drafted tokens of its path that a token sees beside itself
     struct TreeTile *tile_at;
 };
 
@@ -583,6 +584,24 @@ __device__ __forceinline__ int tree_count(const AttArgs &A, const AttRow &o, int
         n += __popcll(A.bits[(int64_t)o.tok * A.words + i] & ones_below(o.own - 64 * i) & ~ones_below(from - 64 * i));
     return n;
 }
+// the place of set bit k (counted from 0) of those below the token's own, of which there are more
+__device__ __forceinline__ int tree_place(const AttArgs &A, const AttRow &o, int k) {
+    int i = 0;
+    uint64_t v = 0;
+    for (;; i++) {
+        v = tree_word(A, o, i);
+        const int n = __popcll(v);
+        if (k < n || i >= A.words - 1) break;
+        k -= n;
+    }
+    int at = 0;
+#pragma unroll
+    for (int half = 32; half; half >>= 1) {
+        const int n = __popcll(v >> at & ones_below(half));
+        if (k >= n) { k -= n; at += half; }
+    }
+    return 64 * i + at;
+}
 __device__ __forceinline__ uint32_t tree_sees(const AttArgs &A, const AttRow &o, int p) {   // of positions p .. p + 31
     return (ones32(o.ctx - p) | tree_bits(A, o, p - o.ctx)) & ones32(o.hi - p) & ~ones32(o.lo - p);
 }
@@ -608,7 +627,10 @@ template <bool TREE> __device__ __forceinline__ void att_limits(const AttArgs &A
         o.pos = o.ctx + tree_count(A, o, 0);
     }
     if (a.window > 0) o.lo = max(o.lo, o.pos - a.window);
-    if (TREE) o.lo = max(min(o.lo, o.ctx), 0);   // new tokens are seen by their bits alone
+    if (TREE) {   // new tokens are seen by their bits alone, unless the window cuts their path
+        const int hidden = o.pos - o.ctx - A.path;
+        o.lo = hidden > 0 ? o.ctx + tree_place(A, o, hidden) : max(min(o.lo, o.ctx), 0);
+    }
     o.hi = max(min(min(o.hi, len), a.max_len), 0);
     if (shared) o.hi = min(o.hi, a.shared); else o.lo = max(o.lo, a.shared);
     o.full = TREE ? min(o.hi, o.ctx) : o.hi;

@@ -29,7 +29,7 @@ KERNELS = ["rmsnorm", "router", "topk", "group", "quant", "gateup", "quant_act",
            "att_scores", "att_softmax", "att_pv", "kv_plan", "rope", "att_paged", "tree", "att_tree", "kv_pages"]
 F32, F16, BF16 = 0, 1, 2
 DTYPE = dict(f32=F32, f16=F16, bf16=BF16)
-KV_MAXSEQ, KV_MAXLAYERS, TREE_MAX = 4096, 128, 512
+KV_MAXSEQ, KV_MAXLAYERS, TREE_MAX, TREE_WINDOW = 4096, 128, 512, 256
 
 
 def _struct(name, doc, *fields):

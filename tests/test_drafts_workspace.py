@@ -5,8 +5,8 @@ import maplemoe as M
 from test_drafts_args import P, attn, cache, refused
 
 
-def size(ckw={}, **kw):
-    return M.lib().mmoe_attn_tree_ws(attn(**kw), cache(**ckw), P, kw.pop("words", 1))
+def size(ckw={}, words=1, **kw):
+    return M.lib().mmoe_attn_tree_ws(attn(**kw), cache(**ckw), P, words)
 
 
 @pytest.mark.parametrize("kw,ckw", [(dict(nseq=64, ntok=256, max_q=4), {}), (dict(nseq=48, ntok=192, max_q=4), {}), (dict(nseq=200, ntok=800, max_q=4), {}), (dict(nseq=32, ntok=2048, max_q=64), {}),
@@ -55,3 +55,11 @@ def test_sequences_at_rest_take_no_room(shared):
     waves = 256 * 4 + 160 + 160 + 1280 if shared else 256 * 3 + 160 + 1280
     assert at <= waves * 32 * 4 * 520 + 4096 * 64 and at < (176e6 if shared else 104e6)
     assert at <= size(nseq=1280, ntok=1280, max_q=20, width=512, max_len=8192, shared=shared)
+
+
+def test_words_with_the_window_along_the_path():
+    W = M.TREE_WINDOW
+    assert size(window=9, words=1 | W) == size(window=9) and size(words=8 | W) > 0
+    for words in (W, 9 | W, 2 * W | 1, -1, 1 - W):
+        refused(M.lib().mmoe_attn_tree(attn(), cache(), P, words), b"words")
+    refused(M.lib().mmoe_attn_tree(attn(max_q=65), cache(), P, 1 | W), b"max_q")

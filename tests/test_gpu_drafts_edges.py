@@ -4,7 +4,7 @@ import pytest
 
 import maplemoe as M
 from draft_ref import TreeBatch, tree, tree_plan
-from paged_ref import Dev, decode, encode
+from paged_ref import HALF, Dev, attend, decode, encode
 from test_gpu_drafts import drafts, run_tree_plan
 
 pytestmark = pytest.mark.gpu
@@ -96,3 +96,95 @@ def test_infinite_values_where_every_score_is_minus_infinity(name, kind, dim):
     rest = [i for i in range(dim) if i not in (5, 6, 7)]
     bad = np.abs(got - want)[..., rest] > off[..., rest]
     assert not bad.any(), np.argwhere(bad)[:5]
+
+
+# ---------------------------------------------------------------------------------------------------- windows that count along the path
+class AlongThePath(TreeBatch):
+    """with MMOE_TREE_WINDOW: a token sees itself and the `window` tokens of its path before it, cached or drafted"""
+
+    def expect(self):
+        out = np.zeros((self.ntok, self.heads, self.dim))
+        lse, off, loff = np.zeros((self.ntok, self.heads)), np.zeros(out.shape), np.zeros((self.ntok, self.heads))
+        q = decode(self.q, self.kind)
+        for s, rows in enumerate(self.rows):
+            k, v = self.cached(s)
+            ctx = self.lens[s] - len(rows)
+            b = self.table[s][np.arange(self.lens[s]) // self.bs]
+            there = (b >= 0) & (b < self.nblocks) & (np.arange(self.lens[s]) < self.max_len)
+            for i, row in enumerate(rows):
+                t = self.qstart[s] + i
+                way = np.array(list(range(ctx)) + [ctx + j for j in range(i) if row[j]] + [ctx + i])
+                pos = len(way) - 1
+                see = there[way] & (np.arange(len(way)) >= pos - self.window)
+                see[:ctx] &= np.arange(ctx) >= (0 if self.lo is None else int(self.lo[t]))
+                see[-1] &= bool(row[i])
+                with np.errstate(all="ignore"):
+                    o, l, e, f = attend(q[t:t + 1], k[way], v[way], np.array([pos]), see[None], self.scale, self.cap, self.slopes, HALF[self.kind])
+                out[t], lse[t], off[t], loff[t] = o[0], l[0], e[0], f[0]
+        return out, lse, off, loff
+
+    def run(self, d, note=""):
+        a = self.upload(d)
+        words = self.words | M.TREE_WINDOW
+        assert d.lib.mmoe_attn_tree_ws(a, self.cache, self.p_bits, words) == a.ws_bytes
+        M.check(d.lib.mmoe_attn_tree(a, self.cache, self.p_bits, words), "mmoe_attn_tree")
+        return self.check(d, note)
+
+
+ALONG = [  # nodes, cached positions, back, options
+    ([64, 30, 5], [100, 200, 900], 1, dict(heads=2, kv=1, window=7, kind="bf16")),
+    ([64, 30, 5], [100, 200, 900], 2, dict(heads=4, kv=2, window=1)),
+    ([64, 64], [100, 200], 1, dict(heads=2, kv=1, window=32)),
+    ([61, 20], [70, 190], 2, dict(heads=12, kv=12, dim=64, alibi=True, cap=15.0, window=10)),
+    ([130, 140], [600, 128], 1, dict(heads=2, kv=1, window=90, alibi=True, words=3, kind="bf16")),
+    ([512, 300], [100, 7], 1, dict(heads=1, kv=1, dim=64, words=8, window=64)),
+    ([512], [0], 2, dict(heads=2, kv=1, words=8, window=130, kind="bf16")),
+    ([61, 64, 5], [130, 64 + 70, 200], 1, dict(heads=4, kv=4, dim=64, alibi=True, shared=64, window=40, kind="bf16")),
+    ([20, 33], [300, 40], 3, dict(heads=8, kv=2, window=400, lo=lambda pos: pos - 30)),
+    ([40, 50], [300, 100], 1, dict(heads=4, kv=2, window=2 ** 31 - 1)),
+    ([30] * 70, [100] * 70, 1, dict(heads=4, kv=1, window=9)),
+    ([33, 9], [64, 128], 1, dict(heads=4, kv=1, window=33, cap=20.0)),
+]
+
+
+@pytest.mark.parametrize("i", range(len(ALONG)))
+def test_windows_along_the_path(i):
+    sizes, ctx, back, kw = ALONG[i]
+    print(f"\n  {sizes[:4]} over {ctx[:4]}, {kw}", flush=True)
+    rng = np.random.default_rng(300 + i)
+    b = AlongThePath(rng, drafts(rng, sizes, back), lens=[c + n for c, n in zip(ctx, sizes)], **kw)
+    with Dev() as d:
+        b.run(d, f"case {i}")
+
+
+@pytest.mark.parametrize("n,ctx,heads,kv,dim,window", [(40, 100, 4, 2, 128, 3), (70, 31, 4, 4, 64, 12), (64, 0, 2, 1, 64, 1)])
+def test_windows_along_any_bits(n, ctx, heads, kv, dim, window):
+    """bits that are no tree's: the last `window` set ones before the token's own, which may be left out itself"""
+    rng = np.random.default_rng(n)
+    rows = rng.random((n, n)) < 0.5
+    rows[1], rows[n - 1] = False, True
+    b = AlongThePath(rng, [rows, rng.random((n, n)) < 0.8], lens=[ctx + n, ctx + n + 300], heads=heads, kv=kv, dim=dim, window=window, kind="bf16")
+    with Dev() as d:
+        b.run(d, f"{n} tokens")
+
+
+@pytest.mark.parametrize("sizes,ctx,kw", [([64, 20], [300, 100], dict(heads=4, kv=2, window=7)), ([40], [10], dict(heads=2, kv=1, dim=64, window=39, kind="bf16")),
+                                          ([64, 9, 33], [0, 50, 400], dict(heads=4, kv=4, dim=64, window=20, alibi=True))])
+def test_a_chain_in_a_window_is_plain_attention(sizes, ctx, kw):
+    """a draft without branches sees what mmoe_attn_paged's tokens see; so it does without MMOE_TREE_WINDOW where the window is no shorter than it"""
+    rng = np.random.default_rng(len(sizes))
+    for more in (0, 64):
+        kw = dict(kw, window=kw["window"] + more)
+        b = AlongThePath(rng, drafts(rng, sizes, 1), lens=[c + n for c, n in zip(ctx, sizes)], **kw)
+        with Dev() as d:
+            b.run(d, "as a tree")
+            a = b.args
+            if more:
+                d.write(b.p_out, b.out0); d.write(b.p_lse, b.lse0)
+                M.check(d.lib.mmoe_attn_tree(a, b.cache, b.p_bits, b.words), "a window longer than the paths")
+                b.check(d, "without the flag")
+            d.write(b.p_out, b.out0); d.write(b.p_lse, b.lse0)
+            (a.ws, a.ws_bytes), tree_ws = b.plain_ws, (a.ws, a.ws_bytes)
+            M.check(d.lib.mmoe_attn_paged(a, b.cache), "plain")
+            a.ws, a.ws_bytes = tree_ws
+            b.check(d, "plain")
