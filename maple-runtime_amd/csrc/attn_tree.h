@@ -76,9 +76,12 @@ struct Draft {
         if (A.room) {
             // (the host has seen to it that all steps are a 32-bit number)
             const int steps = sh.tiles * sh.steps + total([](const Seq &x) { return x.tiles * x.steps; });
-            // where the row tiles alone come near to what there is room for, there are more rounds anyway: half as large pieces then, and no search
-            const bool few = 4 * all_tiles <= 3 * A.room;
-            const int goal = few ? A.room : 2 * A.room;
+            // Up to as many row tiles as there is room for a search for pieces that fit at once. More of them take more rounds anyway: as long as a share of
+            // the room makes them, which cuts the longest only, and no search. 20 tokens over 1500, 16 and 4 heads of 128 (128 pieces fit): 72 sequences 62
+            // us and 120 85, without the search, in pieces half as large, 82 and 116; 200 sequences 145 us, in pieces half as large 177 (but 200 of 10 over 3000
+            // with heads of 64: 165, 160)
+            const bool few = all_tiles <= A.room;
+            const int goal = A.room;
             // rounding up makes about half a piece more of each row tile
             per = fminf(((float)goal - (few ? 0.5f * (float)all_tiles : 0.0f)) / (float)max(steps, 1), 1.0f);
             for (int i = 0;; i++) {

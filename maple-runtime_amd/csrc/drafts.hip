@@ -32,11 +32,11 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     const int64_t most_steps = (a.window ? std::min<int64_t>(a.max_len, (int64_t)a.window + a.max_q + TREE_BN) : a.max_len) / TREE_BN + 1;
     const bool whole = !a.shared && most_steps <= 12 && tiles * kv.heads >= 192;
     // What the card holds at once: two workgroups per compute unit, three with heads of 64 (64 drafts of 10 to 40 tokens over 50 to 3000 positions, heads of 128:
-    // 68 us, with 768 pieces 75; 17 drafts behind 2048 shared positions, heads of 64: 32 us, with 512 pieces 37)
+    // 68 us, with 768 pieces 75; 17 drafts behind 2048 shared positions, heads of 64: 32 us, with 512 pieces 37, but 16 of 20 over 3000 23.4, with 512 21.9)
     const int once = kv.head_dim == 64 ? 768 : 512;
     const int room = std::max(1, once / kv.heads);
     p.room = whole ? 0 : room;
-    const int64_t most_pieces = std::max(tiles <= room * 3 / 4 ? (int64_t)room : 2 * (int64_t)room + tiles, tiles), pieces = whole ? tiles : most_pieces, join = own * kv.heads * 4;
+    const int64_t most_pieces = std::max(tiles <= room ? (int64_t)room : room + tiles, tiles), pieces = whole ? tiles : most_pieces, join = own * kv.heads * 4;
     // Few row tiles, so perhaps many results of each, and few workgroups of 32 rows and a key/value head: eight workgroups for one (26 tokens over 700
     // positions, 16: 12.5 us instead of 14.6; over 30000 34 instead of 66; 3 drafts of 60 over 3000, 96: 24.7 instead of 26; 16 of 20 over 2000, 256: 28.6 instead of 27.5)
     p.deep = join < 128;
@@ -46,15 +46,15 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
     const int64_t wgs = std::min((pieces * kv.heads + 7) & ~(int64_t)7, p.many ? (int64_t)once : INT64_MAX);
     p.fits = tiles * ((int64_t)a.max_len / TREE_BN + 2) <= INT32_MAX && std::max(wgs, join * (p.deep ? 8 : 1)) * 256 <= (int64_t)MAX_THREADS;
     p.wgs = (unsigned)wgs; p.tiles = (int)std::min<int64_t>(own, INT32_MAX); p.join = (unsigned)(p.deep ? join * 8 : join);
-    // Results, in waves of 32 rows: of up to `room` pieces where the row tiles are few; else one of every row, and as many more as a cut into 2 room parts
-    // makes (rounded up, each row tile is one more than its share of them). Without shared positions only those of row tiles that are cut, each
-    // of at least two pieces, which makes less than 4 room. There is room for them also where the row tiles stay whole, so that a workspace serves every
+    // Results, in waves of 32 rows: of up to `room` pieces where the row tiles are no more; else one of every row, and as many more as a cut into `room`
+    // parts makes (rounded up, each row tile is one more than its share of them). Without shared positions only those of row tiles that are cut, each
+    // of at least two pieces, which makes less than 2 room. There is room for them also where the row tiles stay whole, so that a workspace serves every
     // bound of the lengths and every window, and more of it never does with less.
     const int64_t piece_waves = a.shared ? ATT_BM / 32 : std::min<int64_t>(ATT_BM, most + 31) / 32;
     int64_t waves = piece_waves * room;
-    if (tiles > room * 3 / 4) {
-        waves = piece_waves * 2 * room + own_waves + sh_tiles * (ATT_BM / 32);
-        if (!a.shared) waves = std::min(waves, piece_waves * 4 * room);
+    if (tiles > room) {
+        waves = piece_waves * room + own_waves + sh_tiles * (ATT_BM / 32);
+        if (!a.shared) waves = std::min(waves, piece_waves * 2 * room);
     }
     p.most_waves = (int)std::min<int64_t>(waves, INT32_MAX);
     p.results = (size_t)waves * kv.heads;

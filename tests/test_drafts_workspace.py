@@ -50,10 +50,10 @@ def test_no_size_for_what_is_too_much_for_a_launch(kw, ckw):
 @pytest.mark.parametrize("shared", [0, 2048])
 def test_sequences_at_rest_take_no_room(shared):
     """64 drafts of 20 tokens in a batch of 4096: what is kept follows the tokens. Of each of 4 key/value heads 5120 rows over the shared positions and of
-    their own (1280 sequences of one token at the worst), and 256 pieces of 128 rows that a cut adds, 520 bytes a row and head"""
+    their own (1280 sequences of one token at the worst), and 128 pieces of 128 rows that a cut adds, 520 bytes a row and head"""
     at = size(nseq=4096, ntok=1280, max_q=20, width=512, max_len=8192, shared=shared)
-    waves = 256 * 4 + 160 + 160 + 1280 if shared else 256 * 3 + 160 + 1280
-    assert at <= waves * 32 * 4 * 520 + 4096 * 64 and at < (176e6 if shared else 104e6)
+    waves = 128 * 4 + 160 + 160 + 1280 if shared else 128 * 3 + 160 + 1280
+    assert at <= waves * 32 * 4 * 520 + 4096 * 64 and at < (142e6 if shared else 52e6)
     assert at <= size(nseq=1280, ntok=1280, max_q=20, width=512, max_len=8192, shared=shared)
 
 
