@@ -22,12 +22,12 @@ struct Draft {
         __device__ __forceinline__ int waves() const { return (rows + 31) >> 5; }
     };
     // the shared positions' rows (every token) as a sequence of its own
-    __device__ static __forceinline__ Seq of_shared(const AttArgs &A) {
+    __device__ static __forceinline__ Seq of_shared(const TreeArgs &A) {
         Seq q = {0, 0, 0, A.a.shared ? att_start(A.a, A.a.nseq) * A.group : 0, 0, 0, A.a.shared, (A.a.shared + TREE_BN - 1) / TREE_BN};
         q.tiles = (q.rows + ATT_BM - 1) / ATT_BM;
         return q;
     }
-    __device__ static __forceinline__ Seq of(const AttArgs &A, int s) {
+    __device__ static __forceinline__ Seq of(const TreeArgs &A, int s) {
         const mmoe_attn_args &a = A.a;
         Seq q = {};
         if (s >= a.nseq) return q;
@@ -54,7 +54,7 @@ struct Draft {
     // come first)
     struct Cut { float per; int pieces, own_tiles, shared_tiles, shared_waves, shared_k; };
     // The same for every thread of the workgroup (256). MANY: more than 64 sequences, else every wave does it by itself
-    template <bool MANY> __device__ static __forceinline__ Cut plan(const AttArgs &A, Mem &M) {
+    template <bool MANY> __device__ static __forceinline__ Cut plan(const TreeArgs &A, Mem &M) {
         const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, n = A.a.nseq;
         const Seq sh = of_shared(A), q = of(A, MANY ? tid : l);
         auto total = [&](auto &&f) {
@@ -96,7 +96,7 @@ struct Draft {
     }
     // A piece: its sequence (-1: the shared positions), that one's first piece, first result and row tile, the pieces of its row tile
     struct Piece { int seq, base, result, tiles, k; Seq q; };
-    template <bool MANY> __device__ static __forceinline__ bool piece(const AttArgs &A, Mem &M, const Cut &c, int id, Piece &o) {
+    template <bool MANY> __device__ static __forceinline__ bool piece(const TreeArgs &A, Mem &M, const Cut &c, int id, Piece &o) {
         const int tid = threadIdx.x, l = tid & 63, w = tid >> 6, n = A.a.nseq, common = c.shared_tiles * c.shared_k, common_waves = c.shared_waves * c.shared_k;
         if (id < common) {
             o = {-1, 0, 0, 0, c.shared_k, of_shared(A)};
@@ -162,7 +162,7 @@ struct Draft {
 // MANY: of more than 64 sequences most may be without tokens, so that there is a bound on the pieces far above their number: a workgroup takes more than
 // one, one after the other, where there are more than the launch has workgroups.
 template <int T, int D, bool CAP, bool BIAS, bool MANY>
-__global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
+__global__ void __launch_bounds__(256, 2) k_attn_tree(TreeArgs A) {
     __shared__ AttTileMem<D, TREE_BN> M;
     __shared__ Draft::Mem F;
     const Draft::Cut c = Draft::plan<MANY>(A, F);
@@ -207,7 +207,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(AttArgs A) {
 // instructions come from memory as well, and branches between the loads cost as much as the loads. Measured: 3.9 us for one draft's 12 results, 8 us
 // for 64 drafts (17 MB).
 template <int T, int D, bool DEEP>
-__global__ void __launch_bounds__(256) k_tree_join(AttArgs A) {
+__global__ void __launch_bounds__(256) k_tree_join(TreeArgs A) {
     constexpr int C = DEEP ? D / 64 : D / 32, TJ_U = DEEP ? 8 : 512 / D;   // groups of 8 dims of a lane; results under way
     const mmoe_attn_args &a = A.a;
     __shared__ f4 acc[DEEP ? 3 : 1][C][64];

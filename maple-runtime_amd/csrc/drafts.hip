@@ -69,7 +69,7 @@ static int check_launch(const mmoe_attn_args &a, const TreePlan &p) {
 
 template <int T, int D, bool CAP, bool BIAS>
 static int tree_run(const mmoe_attn_args &a, const mmoe_kv_cache &kv, const TreePlan &p, const uint64_t *bits, int words, int path) {
-    AttArgs A{};
+    TreeArgs A{};
     A.a = a; A.kv = kv;
     A.sh = log2_block(kv.block_size); A.group = a.heads / kv.heads;
     A.by_kv = divisor(kv.heads); A.by_group = divisor(A.group);

@@ -459,14 +459,20 @@ struct AttArgs {
     float *po;
     float2 *pm;
     int64_t at_tile, at_few;
-    // Drafted tokens (TREE, attn_tree.h): words of bits per token, bit j: it sees its sequence's j-th new token; the pieces that the row tiles of a key/
-    // value head are to be cut into (0: none, each stays whole), the most row tiles there can be and the most waves (of 32 rows) of their partial results in
-    // po and pm; the row tiles
+};
+// and of drafted tokens (TREE, attn_tree.h), by themselves since a launch waits for its arguments (mmoe_attn_paged for 7 tokens behind shared positions 13.1
+// us, with these behind its own 13.7)
+struct TreeArgs : AttArgs {
+    // words of bits per token, bit j: it sees its sequence's j-th new token; the drafted tokens of its path that a token sees beside itself
     const uint64_t *bits;
-    int words, room, most_tiles, most_waves;
-    int path;   // the drafted tokens of its path that a token sees beside itself
+    int words, path;
+    // the pieces that the row tiles of a key/value head are to be cut into (0: none, each stays whole), the most row tiles there can be and the most waves (of
+    // 32 rows) of their partial results in po and pm; the row tiles
+    int room, most_tiles, most_waves;
     struct TreeTile *tile_at;
 };
+template <bool TREE> struct ArgsOf { typedef AttArgs type; };
+template <> struct ArgsOf<true> { typedef TreeArgs type; };
 
 template <int T> __device__ __forceinline__ f16v mfma32(u4 a, u4 b, f16v c) {
     if (T == MMOE_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
@@ -565,19 +571,19 @@ __device__ __forceinline__ AttSeq att_seq(const AttArgs &A, bool shared, const A
 // cached positions' end, its bits from there on, cut to [lo, hi) (hi is the token's own position's end: bits past it do not count).
 __device__ __forceinline__ uint64_t ones_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
 __device__ __forceinline__ uint32_t ones32(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
-__device__ __forceinline__ uint64_t tree_word(const AttArgs &A, const AttRow &o, int i) {
+__device__ __forceinline__ uint64_t tree_word(const TreeArgs &A, const AttRow &o, int i) {
     if (A.words == 1) return i == 0 ? o.bits : 0;
     return (unsigned)i < (unsigned)A.words ? A.bits[(int64_t)o.tok * A.words + i] : 0;
 }
 // the bits of 32 nodes from `at` on (which may be negative)
-__device__ __forceinline__ uint32_t tree_bits(const AttArgs &A, const AttRow &o, int at) {
+__device__ __forceinline__ uint32_t tree_bits(const TreeArgs &A, const AttRow &o, int at) {
     const int i = at >> 6, sh = at & 63;
     uint64_t v = tree_word(A, o, i) >> sh;
     if (sh > 32) v |= tree_word(A, o, i + 1) << (64 - sh);
     return (uint32_t)v;
 }
 // how many are set of nodes from .. the token's own, without it
-__device__ __forceinline__ int tree_count(const AttArgs &A, const AttRow &o, int from) {
+__device__ __forceinline__ int tree_count(const TreeArgs &A, const AttRow &o, int from) {
     if (A.words == 1) return __popcll(o.bits & ones_below(o.own) & ~ones_below(from));
     int n = 0;
     for (int i = max(from, 0) >> 6; i < min(A.words, (o.own + 63) >> 6); i++)
@@ -585,7 +591,7 @@ __device__ __forceinline__ int tree_count(const AttArgs &A, const AttRow &o, int
     return n;
 }
 // the place of set bit k (counted from 0) of those below the token's own, of which there are more
-__device__ __forceinline__ int tree_place(const AttArgs &A, const AttRow &o, int k) {
+__device__ __forceinline__ int tree_place(const TreeArgs &A, const AttRow &o, int k) {
     int i = 0;
     uint64_t v = 0;
     for (;; i++) {
@@ -602,32 +608,32 @@ __device__ __forceinline__ int tree_place(const AttArgs &A, const AttRow &o, int
     }
     return 64 * i + at;
 }
-__device__ __forceinline__ uint32_t tree_sees(const AttArgs &A, const AttRow &o, int p) {   // of positions p .. p + 31
+__device__ __forceinline__ uint32_t tree_sees(const TreeArgs &A, const AttRow &o, int p) {   // of positions p .. p + 31
     return (ones32(o.ctx - p) | tree_bits(A, o, p - o.ctx)) & ones32(o.hi - p) & ~ones32(o.lo - p);
 }
 // Distances. The path that a token sees, cached positions and all, is a chain of ones whose last is the token itself: the distance to position p + x is the
 // number of ones behind it. ones: of the 32 positions from p on; rest: how many lie behind those.
 struct TreeFar { uint32_t ones; int rest; };
-__device__ __forceinline__ TreeFar tree_far(const AttArgs &A, const AttRow &o, int p) {
+__device__ __forceinline__ TreeFar tree_far(const TreeArgs &A, const AttRow &o, int p) {
     const int at = p - o.ctx, end = o.own - at;
     return {((ones32(-at) | tree_bits(A, o, at)) & ones32(end)) | (end >= 0 && end < 32 ? 1u << end : 0u),
             max(-at - 32, 0) + tree_count(A, o, at + 32) + (end >= 32 ? 1 : 0)};
 }
 __device__ __forceinline__ float tree_distance(const TreeFar &f, int x) { return (float)(__popc(f.ones >> x >> 1) + f.rest); }
 
-template <bool TREE> __device__ __forceinline__ void att_limits(const AttArgs &A, bool shared, const AttSeq &q, AttRow &o, int len) {
+template <bool TREE> __device__ __forceinline__ void att_limits(const typename ArgsOf<TREE>::type &A, bool shared, const AttSeq &q, AttRow &o, int len) {
     const mmoe_attn_args &a = A.a;
     o.pos = len - (q.t1 - o.tok);
     if (o.tok - q.t0 >= a.max_q) o.live = false;
     o.lo = a.lo ? max(a.lo[o.tok], 0) : 0;
     o.hi = !TREE && a.hi ? a.hi[o.tok] : o.pos + 1;
-    if (TREE) {
+    if constexpr (TREE) {
         o.ctx = len - (q.t1 - q.t0); o.own = o.tok - q.t0;
         if (A.words == 1) o.bits = A.bits[o.tok];
         o.pos = o.ctx + tree_count(A, o, 0);
     }
     if (a.window > 0) o.lo = max(o.lo, o.pos - a.window);
-    if (TREE) {   // new tokens are seen by their bits alone, unless the window cuts their path
+    if constexpr (TREE) {   // new tokens are seen by their bits alone, unless the window cuts their path
         const int hidden = o.pos - o.ctx - A.path;
         o.lo = hidden > 0 ? o.ctx + tree_place(A, o, hidden) : max(min(o.lo, o.ctx), 0);
     }
@@ -671,10 +677,10 @@ template <int D, int BN = ATT_BN(D)> struct AttTileMem {
     int range[4][4], flag[2][4];
 };
 // A kernel's arguments, its first parameter, read from where the launch put them whenever this is asked for
-__device__ __forceinline__ const AttArgs &tree_args() {
-    auto p = (const __attribute__((address_space(4))) AttArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+__device__ __forceinline__ const TreeArgs &tree_args() {
+    auto p = (const __attribute__((address_space(4))) TreeArgs *)__builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(p));
-    return *(const AttArgs *)p;
+    return *(const TreeArgs *)p;
 }
 // Which work: with TREE a piece that the caller has found (drafts.h), else the launch's block
 struct AttWork {
@@ -687,7 +693,7 @@ struct AttWork {
     int64_t slot;
 };
 template <int T, int D, bool CAP, bool BIAS, bool TREE>
-__device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, AttTileMem<D, TREE ? TREE_BN : ATT_BN(D)> &M) {
+__device__ __forceinline__ void att_tile(const typename ArgsOf<TREE>::type &A, const AttWork &work, AttTileMem<D, TREE ? TREE_BN : ATT_BN(D)> &M) {
     constexpr int RB = D * 2, CH = D / 8, RPI = 64 / CH, NI = 16 / RPI, KS = D / 16, DS = D / 32;   // a row's bytes and chunks; rows of a load, loads of 16 rows
     constexpr int BN = TREE ? TREE_BN : ATT_BN(D), GW = BN / 64, NU = BN / 32, NK = BN / 16;   // groups of 16 positions that a wave loads; score blocks, steps of the second product
     constexpr uint32_t TB = BN * RB;
@@ -856,8 +862,8 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
         if (TREE && BIAS) shift = path ? 0.0f : -slope * dist;
 #pragma unroll
         for (int u = 0; u < NU; u++) {
-            TreeFar far;
-            if (path) far = tree_far(A, R, p + 32 * u + 4 * hh);
+            TreeFar far = {};
+            if constexpr (TREE) if (path) far = tree_far(A, R, p + 32 * u + 4 * hh);
 #pragma unroll
             for (int j = 0; j < 16; j++) {
                 const int at = 8 * (j >> 2) + (j & 3);
@@ -872,7 +878,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
     };
     // a tile that is not seen whole: a score of -inf where a row does not look
     auto mask = [&](f16v *s, int p, unsigned bad) {
-        if (TREE) {
+        if constexpr (TREE) {
 #pragma unroll
             for (int u = 0; u < NU; u++) {
                 const uint32_t v = tree_sees(A, R, p + 32 * u + 4 * hh);
@@ -990,7 +996,9 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
     auto add_odd = [&](uint32_t buf, int p, unsigned bad) {
 #pragma unroll 1
         for (int r = 0; r < BN; r++) {
-            const bool see = (TREE ? (bool)(tree_sees(A, R, p + r) & 1) : p + r >= R.lo && p + r < R.hi) && !((bad >> (r >> 4)) & 1);
+            bool see = p + r >= R.lo && p + r < R.hi;
+            if constexpr (TREE) see = tree_sees(A, R, p + r) & 1;
+            see = see && !((bad >> (r >> 4)) & 1);
             uint32_t row = r * RB + 8 * hh, x = (r & (CH / 2 - 1)) << 5;
             asm("" : "+v"(row));   // its addresses are not worth a register outside
 #pragma unroll
@@ -1082,7 +1090,7 @@ __device__ __forceinline__ void att_tile(const AttArgs &A, const AttWork &work, 
     }
     sum = add_halves(sum);
     if (!R.live) return;
-    const AttArgs &E = TREE ? tree_args() : A;   // (read again: there are not registers enough to keep what only the end needs)
+    const auto &E = [&]() -> const auto & { if constexpr (TREE) return tree_args(); else return A; }();   // (read again: there are not registers enough to keep what only the end needs)
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     if (TREE ? work.whole : nsplit == 1 && !E.parts_sh) {
         uint16_t *o = (uint16_t *)E.a.out + (int64_t)R.tok * E.a.out_token + R.head * E.a.out_head + 4 * hh;
