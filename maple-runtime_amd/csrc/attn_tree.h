@@ -11,10 +11,10 @@
 
 // Partial results are kept in waves of 32 rows. Those over the shared positions come first, then sequence by sequence, of each what it has over its first
 // positions (the waves of all its rows, key/value head by key/value head), then over the next ones, ... Where one begins is counted per key/value head.
-// A sequence's row tile for the join: where its sequence's results begin, how many there are over its positions, the waves of each, its first token, its
-// first row among its sequence's, the sequence's rows. The first entry holds the number of them in `slot`, and of the shared positions' results `parts`
-// and `apart`.
-struct TreeTile { int slot, parts, apart, t0, row0, rows; };
+// A sequence's row tile for the join: the first wave of its first result (of key/value head 0), how many results there are over its positions and how far
+// apart, and how far key/value heads are; its first token, its first row among its sequence's, the sequence's rows. The first entry holds the number of
+// them in `first`, and of the shared positions' results `parts`, `apart` and `waves`.
+struct __attribute__((aligned(32))) TreeTile { int first, parts, apart, waves, t0, row0, rows; };
 
 struct Draft {
     struct Seq {
@@ -176,12 +176,12 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(TreeArgs A) {
         const Draft::Seq &q = o.q;
         const int k = __builtin_amdgcn_readfirstlane(o.k), steps = __builtin_amdgcn_readfirstlane(q.steps), i = (id - o.base) / q.tiles, tile = id - o.base - i * q.tiles;
         const bool whole = k == 1 && !A.a.shared;
-        const int waves = q.waves(), result = o.result + i * waves;
+        const int waves = q.waves(), first = tile * (ATT_BM / 32), result = o.result + i * waves;
         // (both fit if qstart ascends)
         if ((whole || result + waves <= A.most_waves) && (o.seq < 0 || o.tiles + tile < A.most_tiles)) {
             if (A.room && kvh == 0 && i == 0 && threadIdx.x == 0) {
-                if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {result, k, waves, q.t0, tile * ATT_BM, q.rows};
-                if (id == 0) A.tile_at[0] = {min(c.own_tiles, A.most_tiles), c.shared_k, c.shared_waves, 0, 0, 0};
+                if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {result * A.kv.heads + first, k, waves * A.kv.heads, waves, q.t0, tile * ATT_BM, q.rows};
+                if (id == 0) A.tile_at[0] = {min(c.own_tiles, A.most_tiles), c.shared_k, c.shared_waves * A.kv.heads, c.shared_waves};
             }
             const int len = steps / k, more = steps - len * k;   // the first of them a step longer
             AttWork work = {};
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(TreeArgs A) {
             work.p0 = q.from + (i * len + min(i, more)) * TREE_BN;
             work.p1 = min(work.p0 + (len + (i < more)) * TREE_BN, q.to);
             work.whole = whole;
-            work.slot = (int64_t)result * A.kv.heads + kvh * waves + tile * (ATT_BM / 32);
+            work.slot = (int64_t)result * A.kv.heads + kvh * waves + first;
             att_tile<T, D, CAP, BIAS, true>(tree_args(), work, M);
         }
         if (!MANY) return;
@@ -220,25 +220,28 @@ __global__ void __launch_bounds__(256) k_tree_join(TreeArgs A) {
     id >>= 2;
     const int tile = (int)A.by_kv(id), kvh = id - tile * A.kv.heads;
     const TreeTile head_of = A.tile_at[0], t = A.tile_at[1 + tile];
-    if (tile >= head_of.slot || (t.parts == 1 && !a.shared)) return;   // none, or written by the piece that was all of it
-    // nothing outside the arrays, whatever qstart holds (where it does not ascend, row tiles may be those of an earlier call)
-    if (t.row0 >= t.rows || t.slot < 0 || t.parts < 1 || t.apart < 0 || t.slot + t.parts * (int64_t)t.apart > A.most_waves || (t.row0 >> 5) + w >= t.apart || t.t0 < 0 || t.row0 < 0 || t.rows > (int64_t)(a.ntok - t.t0) * A.group) return;
+    const int64_t first = t.first + kvh * (int64_t)t.waves + w, most = (int64_t)A.most_waves * A.kv.heads;
     const int r = t.row0 + w * 32 + n;
-    if (t.row0 + w * 32 >= t.rows) return;
     const bool live = r < t.rows;
     const int row = min(r, t.rows - 1), j = (int)A.by_group(row), tok = t.t0 + j, head = kvh * A.group + row - j * A.group;
     // the results over the shared positions hold every token's rows
     const int common = a.shared ? head_of.parts : 0, rs = tok * A.group + row - j * A.group;
-    if (a.shared && (common < 0 || head_of.apart < 0 || rs >> 5 >= head_of.apart || common * (int64_t)head_of.apart > A.most_waves)) return;
+    const int64_t first_sh = kvh * (int64_t)head_of.waves + (rs >> 5);
+    // None, or written by the piece that was all of it; nothing outside the arrays, whatever qstart holds (where it does not ascend, row tiles may be those of
+    // an earlier call). One condition: the kernel's arguments are then asked for at once, not branch by branch.
+    const bool some = (tile < head_of.first) & ((t.parts > 1) | (a.shared > 0)) & (t.parts > 0) & ((t.first | t.waves | t.apart | t.t0 | t.row0) >= 0) & (t.row0 + w * 32 < t.rows) &
+                      (first + (t.parts - 1) * (int64_t)t.apart < most) & (t.rows <= (int64_t)(a.ntok - t.t0) * A.group);
+    const bool some_sh = (a.shared == 0) | (((common | head_of.apart | head_of.waves) >= 0) & (first_sh + (common - 1) * (int64_t)head_of.apart < most));
+    if (!some || !some_sh) return;
     const int parts = common + t.parts;
+    const float2 *pm = A.pm + first * 32 + n, *pm_sh = A.pm + first_sh * 32 + (rs & 31);
+    const f4 *po = (const f4 *)A.po + first * (8 * D) + 32 * hh + n, *po_sh = (const f4 *)A.po + first_sh * (8 * D) + 32 * hh + (rs & 31);
     struct Result { float2 v; f4 y[C]; };
     auto load = [&](Result &x, int p) {
         const bool c = p < common;
-        const int at = c ? rs & 31 : n;
-        const int apart = c ? head_of.apart : t.apart;
-        const int64_t wave = (int64_t)(c ? p * apart : t.slot + (p - common) * apart) * A.kv.heads + kvh * apart + (c ? rs >> 5 : (t.row0 >> 5) + w);
-        x.v = A.pm[wave * 32 + at];
-        const f4 *q = (const f4 *)(A.po + wave * 32 * D) + 32 * hh + at;
+        const int64_t at = (c ? p * (int64_t)head_of.apart : (p - common) * (int64_t)t.apart) * 32;
+        x.v = (c ? pm_sh : pm)[at];
+        const f4 *q = (c ? po_sh : po) + at * (D / 4);
 #pragma unroll
         for (int i = 0; i < C; i++) x.y[i] = q[(share * C + i) * 64];
     };

@@ -56,7 +56,7 @@ static TreePlan tree_plan(const mmoe_attn_args &a, const mmoe_kv_cache &kv) {
         waves = piece_waves * room + own_waves + sh_tiles * (ATT_BM / 32);
         if (!a.shared) waves = std::min(waves, piece_waves * 2 * room);
     }
-    p.most_waves = (int)std::min<int64_t>(waves, INT32_MAX);
+    p.most_waves = (int)waves;   // (with heads 2^27 at most: a call has no more than 2^30 rows)
     p.results = (size_t)waves * kv.heads;
     p.bytes = p.results * 32 * (kv.head_dim * 4 + 8) + (size_t)(own + 1) * sizeof(TreeTile) + 256;
     return p;

@@ -633,10 +633,7 @@ template <bool TREE> __device__ __forceinline__ void att_limits(const typename A
         o.pos = o.ctx + tree_count(A, o, 0);
     }
     if (a.window > 0) o.lo = max(o.lo, o.pos - a.window);
-    if constexpr (TREE) {   // new tokens are seen by their bits alone, unless the window cuts their path
-        const int hidden = o.pos - o.ctx - A.path;
-        o.lo = hidden > 0 ? o.ctx + tree_place(A, o, hidden) : max(min(o.lo, o.ctx), 0);
-    }
+    if (TREE) o.lo = max(min(o.lo, o.ctx), 0);   // new tokens are seen by their bits alone
     o.hi = max(min(min(o.hi, len), a.max_len), 0);
     if (shared) o.hi = min(o.hi, a.shared); else o.lo = max(o.lo, a.shared);
     o.full = TREE ? min(o.hi, o.ctx) : o.hi;
@@ -790,6 +787,10 @@ __device__ __forceinline__ void att_tile(const typename ArgsOf<TREE>::type &A, c
         const AttSeq of = att_seq(A, shared, at, M.starts, R);
         att_limits<TREE>(A, shared, of, R, a.len[of.s]);
         queries();
+    }
+    if constexpr (TREE) {   // unless the window cuts their path
+        const int hidden = R.pos - R.ctx - A.path;
+        if (hidden > 0) R.lo = max(R.ctx + tree_place(A, R, hidden), shared ? 0 : a.shared);
     }
     // A score is sc s1 + s0 in units of log 2, in which sc is the product's with the bias in its units, or with a cap 1 / (1 + exp 2 z):
     // what is left of them is in the exponentials' own multiplication.
