@@ -188,3 +188,19 @@ def test_a_chain_in_a_window_is_plain_attention(sizes, ctx, kw):
             M.check(d.lib.mmoe_attn_paged(a, b.cache), "plain")
             a.ws, a.ws_bytes = tree_ws
             b.check(d, "plain")
+
+
+# ---------------------------------------------------------------------------------------------------- limits behind shared positions
+@pytest.mark.parametrize("kw", [dict(lo=lambda pos: 90 + (pos % 7) * 30), dict(lo=lambda pos: pos - 20), dict(lo=lambda pos: np.full(len(pos), 1 << 29)), dict(max_q=30), dict(max_q=2),
+                                dict(max_len=128), dict(max_len=250), dict(max_len=510), dict(lost=[(0, 3), (0, 20), (1, 12), (2, 33)]), dict(cut=50, pad=7), dict(with_lse=False),
+                                dict(window=40), dict(window=250, alibi=True), dict(shared=64, lost=[(0, 0), (0, 3)], cap=20.0)], ids=lambda kw: "-".join(kw))
+def test_limits_behind_shared_positions(kw):
+    """masks that hide all of the shared positions, or a part; sequences of which some tokens are not served; positions and blocks that are not there"""
+    rng = np.random.default_rng(11)
+    sizes, ctx = [40, 3, 64], [300, 200, 500]
+    b = TreeBatch(rng, drafts(rng, sizes, 6), lens=[c + n for c, n in zip(ctx, sizes)], heads=4, kv=2, kind="bf16", **dict(dict(shared=128), **kw))
+    if "lost" in kw:      # the shared positions' blocks are row 0's
+        for s in (1, 2):
+            b.table[s, :b.shared // b.bs] = b.table[0, :b.shared // b.bs]
+    with Dev() as d:
+        b.run(d, str(list(kw)))
