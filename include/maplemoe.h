@@ -455,8 +455,8 @@ int mmoe_kv_compact(const mmoe_kv_compact_args *a, const mmoe_kv_cache *kv, int 
  * table: full blocks are shared (holders[block]++, but for those of the `shared` prefix, which nobody gives back), for a begun one a new
  * block is taken from the end of the list, and copy_from[i], copy_to[i], copy_count[i] say what mmoe_kv_copy has to copy (-1, -1, 0: nothing).
  * ctx_out[dst[i]] = n. holders[nblocks]: how many sequences hold a block beside the first; 0 at the start, and blocks that mmoe_kv_plan takes have 0.
- * From the first fork for which no block is left on, none is made: ctx_out[dst[i]] = 0, the row as it was. Rows that are not 0 .. nseq - 1 are
- * left out. nfree_out[0] = free blocks left. dst: no row twice. table_out may be table and ctx_out ctx, if no dst is a src then (a beam
+ * From the first fork for which no block is left on, none is made: ctx_out[dst[i]] = 0, the row as it was. A fork whose dst is not in 0 .. nseq - 1 is
+ * left out (as padding has to be); one whose src is not makes a copy of nothing: ctx_out[dst[i]] = 0, the row as it was. nfree_out[0] = free blocks left. dst: no row twice. table_out may be table and ctx_out ctx, if no dst is a src then (a beam
  * search, whose rows follow one another, needs a second table). Where sequences share blocks, mmoe_kv_free gives them back, not mmoe_kv_plan's done. */
 typedef struct {
     const int32_t *src, *dst, *at, *ctx, *table;

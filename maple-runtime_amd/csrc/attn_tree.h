@@ -156,9 +156,9 @@ struct Draft {
 // byte of the cache has to be read once (the row tiles of a sequence read it at the same time, from their die's cache), the pieces begin together and
 // the last ends long after the median one. Measured with the join: 64 drafts of 10 to 40 tokens over 50 to 3000 positions, 16 and 4 heads of 128, 215 MB:
 // 68 us, 3.2 TB/s (41 would be a copy's rate; pieces have 17 steps in the middle and 24 at most; begin 6 us, join 8); 4 drafts of 100 to 200 over 20000
-// to 30000, capped: 173 us, 0.71 PFLOP/s, the matrix products beside three exponentials' work; 32 drafts of 64 in a window of 512: 24.6 us, whole row
+// to 30000, capped: 168 to 184 us on several cards, 0.66 to 0.72 PFLOP/s, the matrix products beside three exponentials' work; 32 drafts of 64 in a window of 512: 24.6 us, whole row
 // tiles, one wave per SIMD: 10 steps of 3450 cycles behind 14000 of dependent loads; 17 drafts behind 2048 shared positions, heads of 64 with slopes:
-// 32.2 us, the exponentials and the sums beside them (seven and a half operations a score); one draft of 26 over 700: 12.5 us, latency.
+// 32.4 us, the exponentials and the sums beside them (seven and a half operations a score); one draft of 26 over 700: 12.5 us, latency.
 // MANY: of more than 64 sequences most may be without tokens, so that there is a bound on the pieces far above their number: a workgroup takes more than
 // one, one after the other, where there are more than the launch has workgroups.
 template <int T, int D, bool CAP, bool BIAS, bool MANY>
@@ -200,8 +200,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(TreeArgs A) {
     }
 }
 
-// The partial results of a row tile put together, 32 rows by a workgroup: each result holds its values over its own sum, its maximum (in units of log 2)
-// and sum, negative where results may not be finite. A lane has a row and 4 of each 8 dims, a wave a quarter of the dims; deep (few row tiles, so
+// The partial results of a row tile put together, 32 rows by a workgroup: each result holds its weighted values, not yet divided, the maximum that its
+// weights are counted from (in units of log 2) and their sum, with the sign set where results may not be finite. A lane has a row and 4 of each 8 dims, a wave a quarter of the dims; deep (few row tiles, so
 // perhaps many results of each): a wave has a quarter of the results, a workgroup an eighth of the dims, and the waves join through LDS. The
 // results come from memory (the pieces ran on other dies), so loads of eight results at once are what counts, and short code: a call's first
 // instructions come from memory as well, and branches between the loads cost as much as the loads. Measured: 3.9 us for one draft's 12 results, 8 us

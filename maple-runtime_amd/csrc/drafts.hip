@@ -197,7 +197,8 @@ int mmoe_kv_compact(const mmoe_kv_compact_args *p, const mmoe_kv_cache *kv, int 
     // Short lists (a step's accepted tokens, a few of those that there is room for): a wave goes through one (64 sequences that drafted 64 tokens: 15.3 us,
     // by workgroups of 256 17.4; were 60 of them kept, 31 and 20). Else workgroups of 256 with as many pieces of a position, at least 128 bytes, as
     // leave 768 of them (4 sequences of 5000, 24 layers, 0.4 kept: 167 us, of 1024 threads 171); where there are not so many, of 1024 threads, from 160 on
-    // (one sequence of 20000: 171 us, of 256 threads 194, with pieces of 64 bytes 207)
+    // (one sequence of 20000: 171 us, of 256 threads 194, with pieces of 64 bytes 207). A list goes through one workgroup per array and pieces, so that few
+    // layers leave most of the card idle: of 20000 positions 6 layers 66 us (of 256 threads 115; 38 would be a copy's), one 37 (97; 6.4)
     const int64_t arrays = 2 * layers, lists = a.nseq * arrays;
     auto units_of = [&](int lanes) { return (P.all + lanes - 1) / lanes; };
     auto pieces_for = [&](int wgs) {

@@ -453,8 +453,8 @@ struct AttArgs {
     int split_sh, split, chunk, chunks;   // runs of the shared positions, runs per row tile of the own ones; positions per chunk, most chunks
     int parts_sh;        // partial results of the shared positions: split_sh, or 0
     float s1, s2;        // cap 0: score = s1 q.k in units of log 2; else s2 tanh z, with exp(2 z) = exp2(s1 q.k)
-    // partial results, [head_dim] values over their own sum each, and their maxima (in units of log 2) and sums (negative where results may not
-    // be finite): of the shared positions
+    // partial results, [head_dim] weighted values each, not yet divided, and the maxima that the weights are counted from (in units of log 2) and their
+    // sums (negative where results may not be finite): of the shared positions
     // [split_sh][ntok][heads], from at_tile on of row tiles over the own ones [split][ntok][heads], from at_few on of chunks [chunks][nseq][16 kv heads]
     float *po;
     float2 *pm;
@@ -679,7 +679,7 @@ __device__ __forceinline__ const TreeArgs &tree_args() {
     asm volatile("" : "+s"(p));
     return *(const TreeArgs *)p;
 }
-// Which work: with TREE a piece that the caller has found (drafts.h), else the launch's block
+// Which work: with TREE a piece that the caller has found (attn_tree.h), else the launch's block
 struct AttWork {
     bool shared;
     unsigned block;
