@@ -156,9 +156,10 @@ struct Draft {
 // byte of the cache has to be read once (the row tiles of a sequence read it at the same time, from their die's cache), the pieces begin together and
 // the last ends long after the median one. Measured with the join: 64 drafts of 10 to 40 tokens over 50 to 3000 positions, 16 and 4 heads of 128, 215 MB:
 // 68 us, 3.2 TB/s (41 would be a copy's rate; pieces have 17 steps in the middle and 24 at most; begin 6 us, join 8); 4 drafts of 100 to 200 over 20000
-// to 30000, capped: 168 to 184 us on several cards, 0.66 to 0.72 PFLOP/s, the matrix products beside three exponentials' work; 32 drafts of 64 in a window of 512: 24.6 us, whole row
-// tiles, one wave per SIMD: 10 steps of 3450 cycles behind 14000 of dependent loads; 17 drafts behind 2048 shared positions, heads of 64 with slopes:
-// 32.4 us, the exponentials and the sums beside them (seven and a half operations a score); one draft of 26 over 700: 12.5 us, latency.
+// to 30000, capped: 168 to 184 us on several cards, 0.66 to 0.72 PFLOP/s, the matrix products beside three exponentials' work; 32 drafts of 64 in a window
+// of 512: 24.6 us, whole row tiles, one wave per SIMD: 10 steps of 3450 cycles behind 14000 of dependent loads; 17 drafts behind 2048 shared positions,
+// heads of 64 with slopes: 32.4 us, the exponentials and the sums beside them (seven and a half operations a score); one draft of 26 over 700: 12.7 us,
+// latency.
 // MANY: of more than 64 sequences most may be without tokens, so that there is a bound on the pieces far above their number: a workgroup takes more than
 // one, one after the other, where there are more than the launch has workgroups.
 template <int T, int D, bool CAP, bool BIAS, bool MANY>
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(TreeArgs A) {
     const Draft::Cut c = Draft::plan<MANY>(A, F);
     // Workgroups go to the card's dies in turn: each die a run of consecutive pieces, in which the row tiles of the same positions lie side by
     // side and read them from the die's own cache
-    const int all = c.pieces * A.kv.heads, each = (all + 7) >> 3;
+    const int all = max(c.pieces, 0) * A.kv.heads, each = (all + 7) >> 3;
     for (int y = blockIdx.x >> 3; y < each; y += gridDim.x >> 3) {
         const int at = (int)(blockIdx.x & 7) * each + y, kvh = at / c.pieces, id = at - kvh * c.pieces;
         Draft::Piece o;
@@ -177,8 +178,8 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(TreeArgs A) {
         const int k = __builtin_amdgcn_readfirstlane(o.k), steps = __builtin_amdgcn_readfirstlane(q.steps), i = (id - o.base) / q.tiles, tile = id - o.base - i * q.tiles;
         const bool whole = k == 1 && !A.a.shared;
         const int waves = q.waves(), first = tile * (ATT_BM / 32), result = o.result + i * waves;
-        // (both fit if qstart ascends)
-        if ((whole || result + waves <= A.most_waves) && (o.seq < 0 || o.tiles + tile < A.most_tiles)) {
+        // (both fit if qstart ascends; if it does not, sums of what sequences claim may even have wrapped around)
+        if ((whole || (result >= 0 && result + (int64_t)waves <= A.most_waves)) && (o.seq < 0 || (unsigned)(o.tiles + tile) < (unsigned)A.most_tiles)) {
             if (A.room && kvh == 0 && i == 0 && threadIdx.x == 0) {
                 if (o.seq >= 0) A.tile_at[1 + o.tiles + tile] = {result * A.kv.heads + first, k, waves * A.kv.heads, waves, q.t0, tile * ATT_BM, q.rows};
                 if (id == 0) A.tile_at[0] = {min(c.own_tiles, A.most_tiles), c.shared_k, c.shared_waves * A.kv.heads, c.shared_waves};
@@ -201,11 +202,11 @@ __global__ void __launch_bounds__(256, 2) k_attn_tree(TreeArgs A) {
 }
 
 // The partial results of a row tile put together, 32 rows by a workgroup: each result holds its weighted values, not yet divided, the maximum that its
-// weights are counted from (in units of log 2) and their sum, with the sign set where results may not be finite. A lane has a row and 4 of each 8 dims, a wave a quarter of the dims; deep (few row tiles, so
-// perhaps many results of each): a wave has a quarter of the results, a workgroup an eighth of the dims, and the waves join through LDS. The
-// results come from memory (the pieces ran on other dies), so loads of eight results at once are what counts, and short code: a call's first
-// instructions come from memory as well, and branches between the loads cost as much as the loads. Measured: 3.9 us for one draft's 12 results, 8 us
-// for 64 drafts (17 MB).
+// weights are counted from (in units of log 2) and their sum, with the sign set where results may not be finite. A lane has a row and 4 of each 8 dims,
+// a wave a quarter of the dims; deep (few row tiles, so perhaps many results of each): a wave has a quarter of the results, a workgroup an eighth of
+// the dims, and the waves join through LDS. The results come from memory (the pieces ran on other dies), so loads of eight results at once are what
+// counts, and short code: a call's first instructions come from memory as well, and branches between the loads cost as much as the loads. Measured: 2.9
+// to 4.1 us for one draft's 12 results, 8.5 us for 64 drafts (17 MB).
 template <int T, int D, bool DEEP>
 __global__ void __launch_bounds__(256) k_tree_join(TreeArgs A) {
     constexpr int C = DEEP ? D / 64 : D / 32, TJ_U = DEEP ? 8 : 512 / D;   // groups of 8 dims of a lane; results under way
