@@ -31,15 +31,17 @@ struct Draft {
         const mmoe_attn_args &a = A.a;
         Seq q = {};
         if (s >= a.nseq) return q;
-        q.t0 = att_start(a, s); q.t1 = a.qstart[s + 1]; q.len = a.len[s];
-        const int n = max(q.t1, q.t0) - q.t0;
-        q.rows = min(max(min(q.t1, a.ntok) - q.t0, 0), a.max_q) * A.group;   // (inside the arrays)
+        // Whatever qstart and len hold, the rows lie inside the arrays and the positions inside the table: no difference here can wrap around (0 <= t0 <=
+        // ntok, t1 >= t0, len >= 0)
+        q.t0 = att_start(a, s); q.t1 = max(a.qstart[s + 1], q.t0); q.len = max(a.len[s], 0);
+        const int n = q.t1 - q.t0, ctx = q.len - n;
+        q.rows = min(min(q.t1, a.ntok) - q.t0, a.max_q) * A.group;
         q.tiles = (q.rows + ATT_BM - 1) / ATT_BM;
         q.from = a.shared;
-        if (a.window > 0) q.from = max(q.from, q.len - n - a.window);
+        if (a.window > 0 && ctx > a.window) q.from = max(q.from, ctx - a.window);
         q.from &= ~(TREE_BN - 1);
         q.to = min(q.len - max(n - a.max_q, 0), a.max_len);
-        q.steps = max(q.to - q.from + TREE_BN - 1, 0) / TREE_BN;
+        q.steps = q.to > q.from ? (q.to - q.from + TREE_BN - 1) / TREE_BN : 0;
         return q;
     }
     // Pieces of a row tile: its steps times the pieces per step, rounded up (up to 2^-10 above a whole number that one is taken). Of two steps at

@@ -204,3 +204,32 @@ def test_limits_behind_shared_positions(kw):
             b.table[s, :b.shared // b.bs] = b.table[0, :b.shared // b.bs]
     with Dev() as d:
         b.run(d, str(list(kw)))
+
+
+# ---------------------------------------------------------------------------------------------------- starts and lengths of any value
+@pytest.mark.parametrize("heads,kv,shared,window,dim,n", [(64, 1, 0, 0, 128, 60), (8, 2, 0, 100, 128, 60), (4, 4, 64, 0, 64, 60), (4, 2, 0, 2 ** 31 - 1, 64, 72),
+                                                          (4, 1, 128, 2 ** 31 - 1, 128, 72)])
+def test_starts_and_lengths_of_any_value(heads, kv, shared, window, dim, n):
+    """differences of starts that pass 32 bits: no row past the tokens that the call is told of is written, nor anything behind the workspace. The arrays have
+    room for 130 tokens more"""
+    rng = np.random.default_rng(heads + window % 7)
+    most, more = 40, 130
+    b = TreeBatch(rng, drafts(rng, [most] + [1] * (n - 1), 5), lens=[most + 200] + [200 + s for s in range(1, n)], heads=heads, kv=kv, dim=dim, shared=shared, window=window, pad=30 + more,
+                  cut=most + n - 1 + 30)
+    big = 2 ** 31 - 1
+    with Dev() as d:
+        a = b.upload(d)
+        last, lens = most + n - 1, np.array(b.lens, np.int32)
+        starts = [[0, big, LEAST, last] * (n // 4) + [last], [big, LEAST] * (n // 2) + [big], [LEAST] * n + [big], [b.cut, LEAST + 7] * (n // 2) + [0], [-1, b.cut - 1, LEAST, b.cut + 9] * (n // 4) + [5],
+                  [0] * n + [big]]
+        for start in starts:
+            for length in (lens, np.full(n, big), np.full(n, LEAST), np.where(np.arange(n) % 2, lens, -lens)):
+                d.write(a.qstart, np.array(start[:n + 1], np.int32)); d.write(a.len, np.array(length, np.int32))
+                for fill in (0, 0x7f, 0xff):
+                    d.write(a.ws, np.full(a.ws_bytes, fill, np.uint8))
+                    M.check(d.lib.mmoe_attn_tree(a, b.cache, b.p_bits, b.words), "attention")
+                    raw, lse = d.get(b.p_out, b.out0), d.get(b.p_lse, b.lse0)
+                    assert (raw[b.cut:] == 0x1234).all() and (lse[b.cut:] == 77.0).all(), (start[:4], length[:2])
+                    body = raw[:, 8:8 + heads * (dim + 8)].reshape(b.ntok, heads, dim + 8)
+                    assert (raw[:, :8] == 0x1234).all() and (raw[:, 8 + heads * (dim + 8):] == 0x1234).all() and (body[:, :, dim:] == 0x1234).all()
+                    assert np.array_equal(d.get(a.ws + a.ws_bytes, b.ws_guard), b.ws_guard), "written behind the workspace"
